@@ -1,4 +1,4 @@
-"""ctypes binding of libhbfsim_b200.so (include/hbfsim/api.h + batch_v1.h).
+"""ctypes binding of libhbfsim_b200.so (include/hbfsim/api.h, batch_v1.h, kv_v1.h).
 
 The struct definitions below mirror the C headers field for field.  Loading
 fails loudly when the library is missing: there is no CPU fallback.
@@ -11,6 +11,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libhbfsim_b200.so"
 
 u8, u32, u64, dbl = ctypes.c_uint8, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_double
+i64 = ctypes.c_int64
 vp, cp, i32 = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int
 
 HBFSIM_OK = 0
@@ -145,6 +146,45 @@ class LinkResultV1(ctypes.Structure):
                 ("r_credits", u32), ("status", i32), ("reserved", u32)]
 
 
+# include/hbfsim/kv_v1.h
+KV_BF16, KV_F16 = 0, 1
+
+
+class KvCacheV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("kv_heads", u32), ("head_dim", u32),
+                ("block_tokens", u32), ("reserved", u32), ("pages", u64), ("data", vp),
+                ("scale", vp), ("bounds", vp)]
+
+
+class KvAppendBatchV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("type", u32), ("seqs", u32),
+                ("width", u32), ("reserved", u32), ("tokens", u64), ("k", vp), ("v", vp),
+                ("k_stride_token", i64), ("k_stride_head", i64), ("v_stride_token", i64),
+                ("v_stride_head", i64), ("table", vp), ("table_stride", i64), ("start", vp),
+                ("offsets", vp)]
+
+
+class KvQueryV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("type", u32), ("seqs", u32),
+                ("tokens", u32), ("q_heads", u32), ("width", u32), ("reserved", u32), ("q", vp),
+                ("q_stride_seq", i64), ("q_stride_token", i64), ("q_stride_head", i64),
+                ("table", vp), ("table_stride", i64), ("lengths", vp)]
+
+
+class KvAttentionArgsV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("softmax_scale", ctypes.c_float),
+                ("top", u32), ("blocks", vp), ("counts", vp), ("out", vp), ("lse", vp),
+                ("weights", vp), ("workspace", vp), ("workspace_bytes", u64)]
+
+
+class KvEvictBatchV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("seqs", u32), ("kv_heads", u32),
+                ("width", u32), ("block_tokens", u32), ("keep", u32), ("sink", u32),
+                ("recent", u32), ("decay", u32), ("score", vp), ("weights", vp), ("table", vp),
+                ("table_stride", i64), ("lengths", vp), ("score_out", vp), ("table_out", vp),
+                ("lengths_out", vp), ("freed", vp), ("freed_counts", vp)]
+
+
 # Every exported function with its signature (restype, argtypes).
 SIGNATURES = {
     "hbfsim_abi_version": (u32, []),
@@ -196,6 +236,12 @@ SIGNATURES = {
     "hbfsim_get_retention_v1": (i32, [vp, vp, vp, vp, vp, u64, ctypes.POINTER(u64)]),
     "hbfsim_prefetch_sweep_v1": (i32, [vp, u64, vp, u32, vp, vp]),
     "hbfsim_link_batch_v1": (i32, [vp, u32, vp, vp, vp, vp, vp, vp]),  # arrays by address
+    "hbfsim_kv_append_v1": (i32, [vp, vp, vp]),
+    "hbfsim_kv_select_workspace_v1": (u64, [vp, vp]),
+    "hbfsim_kv_select_v1": (i32, [vp, vp, u32, u32, u32, vp, vp, vp, u64, vp]),
+    "hbfsim_kv_attention_workspace_v1": (u64, [vp, vp, vp]),
+    "hbfsim_kv_attention_v1": (i32, [vp, vp, vp, vp]),
+    "hbfsim_kv_evict_v1": (i32, [vp, vp]),
 }
 
 

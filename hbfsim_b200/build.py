@@ -17,7 +17,8 @@ LIB = PKG / "libhbfsim_b200.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["timing.cu", "empirical.cu", "context.cu", "thermal.cu", "capacity.cu",
-           "retention.cu", "prefetch.cu", "link.cu", "profile.cpp"]
+           "retention.cu", "prefetch.cu", "link.cu", "kv_append.cu", "kv_select.cu",
+           "kv_attention.cu", "kv_evict.cu", "profile.cpp"]
 
 
 def sources() -> list[Path]:

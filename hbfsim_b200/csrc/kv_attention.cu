@@ -1,0 +1,600 @@
+// kv_attention.cu -- attention of the newest tokens over the 8-bit paged
+// cache (kv_v1.h), over all blocks of a sequence or over listed ones.
+//
+// The query rows that share a key/value head (group heads times tokens) are
+// taken 8 or 16 at a time as the narrow side of the tensor-core products, so
+// that the tokens are the wide one:
+//
+//   S^T [16 tokens x 8 rows]  = K [16 x D] Q^T [D x 8]
+//   O^T [D x 8 rows]         += V^T [D x 16 tokens] P^T [16 x 8]
+//
+// K and V are read in their natural order straight into the fragments of
+// mma.m16n8k16: the order of the channels inside a dot product and of the
+// tokens inside a sum is free, so each lane takes 16 contiguous bytes.  e4m3
+// widens to f16 without loss; a block's scales are powers of two and are
+// applied in fp32 to the scores and to the probabilities (relative to the
+// largest value scale met so far), so no product is rounded by them.  Queries
+// are scaled per row by a power of two into f16's range, exact as well.
+// Scores, the running maximum, sums and the output accumulate in fp32.  The
+// probabilities are rounded to f16 (2^-11 relative, no more than the output
+// type's own rounding) for the second product only; the sums and the block
+// weights use them unrounded.
+//
+// A CTA's 4 warps stride over the 16-token tiles of their share of one
+// segment (sequence, head, row tile; for lists also the token), join through
+// shared memory and leave one partial result; combine_kernel joins the
+// shares, and weight_kernel turns the tiles' logarithmic sums into block
+// weights.
+#include "kv.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+namespace hbfb {
+namespace {
+
+constexpr u32 kWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr u32 kWeightBlocks = 256;  // blocks per CTA of weight_kernel
+
+struct AttentionArgs {
+    KvView c;
+    KvQuery q;
+    float scale2;          // softmax scale times log2(e)
+    u32 top;               // lists; 0: every block
+    const int* blocks;
+    const int* counts;
+    void* out;
+    float* lse;
+    float* weights;
+    // segments: ((seq * lists + t) * heads + h) * row_tiles + rt, lists = tokens or 1
+    u32 lists, row_tiles, rows;   // rows of one (sequence, list, head)
+    u32 splits, tiles;            // shares per segment; 16-token tiles per segment at most
+    float* part_o;                // [segments][splits][8 NT][D]
+    float2* part_ml;              // [segments][splits][8 NT]: maximum, sum
+    float* tile_lse;              // [segments][tiles][8 NT], or NULL
+    float* row_lse;               // [segments][8 NT]
+};
+
+__device__ __forceinline__ u32 e4m3x2_to_f16x2(u32 two)
+{
+    u32 r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<u16>(two)));
+    return r;
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0,
+                                         u32 b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ u32 transpose8x8(u32 x)
+{
+    u32 r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+__device__ __forceinline__ u32 pack_f16(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const u32*>(&h);
+}
+
+__device__ __forceinline__ float load_elem(const void* p, i64 i, u32 type)
+{
+    return type == HBFSIM_KV_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
+                                  : __half2float(static_cast<const __half*>(p)[i]);
+}
+
+struct Segment {
+    u32 seq, t, h, rt, index;
+    int length;      // tokens of the sequence
+    u32 tiles;       // 16-token tiles of this segment
+};
+
+__device__ __forceinline__ Segment segment_of(const AttentionArgs& a, u32 index)
+{
+    Segment s;
+    s.index = index;
+    s.rt = index % a.row_tiles;
+    u32 r = index / a.row_tiles;
+    s.h = r % a.c.heads;
+    r /= a.c.heads;
+    s.t = r % a.lists;
+    s.seq = r / a.lists;
+    s.length = kv_length(a.q.lengths, s.seq, a.q.width, a.c.block);
+    if (a.blocks) {
+        const int n = a.counts[(static_cast<u64>(s.seq) * a.lists + s.t) * a.c.heads + s.h];
+        s.tiles = static_cast<u32>(min(max(n, 0), static_cast<int>(a.top))) * (a.c.block / 16);
+    } else {
+        s.tiles = (static_cast<u32>(s.length) + 15) / 16;
+    }
+    return s;
+}
+
+// Position of the query token behind a row of the segment (-1: sees nothing).
+__device__ __forceinline__ int row_position(const AttentionArgs& a, const Segment& s, u32 row)
+{
+    const u32 t = a.blocks ? s.t : row / a.q.group;
+    return max(s.length - static_cast<int>(a.q.tokens) + static_cast<int>(t), -1);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionArgs a)
+{
+    constexpr int R = 8 * NT;
+    constexpr int KC = D / 64;      // 16-byte pieces of a key row per lane
+    constexpr int VW = D / 32;      // 4-byte words of a value row per lane
+    __shared__ float join_o[kWarps][R][D];
+    __shared__ float2 join_ml[kWarps][R];
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
+    const Segment seg = segment_of(a, blockIdx.x / a.splits);
+    const u32 split = blockIdx.x % a.splits;
+    // this CTA's share of the tiles
+    const u32 per = (seg.tiles + a.splits - 1) / a.splits;
+    const u32 first = min(split * per, seg.tiles), end = min(first + per, seg.tiles);
+    const u32 rows = min(static_cast<u32>(R), a.rows - seg.rt * R);
+    const u32 block = a.c.block, per_block = block / 16;
+
+    // queries: row n = 8 nt + g, scaled by a power of two so that the largest is in [2^14, 2^15)
+    u32 qf[NT][D / 16][2];
+    float factor[NT][2];   // of the columns 2c, 2c+1: scale2 over the row's power of two
+    int sees[NT][2];       // last position seen
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const u32 n = nt * 8 + g;
+        float x[KC][16];
+        float most = 0.0f;
+        if (n < rows) {
+            const u32 row = seg.rt * R + n;
+            const u32 t = a.blocks ? seg.t : row / a.q.group;
+            const u32 qh = seg.h * a.q.group + row % a.q.group;
+            const i64 at = static_cast<i64>(seg.seq) * a.q.stride_seq +
+                           static_cast<i64>(t) * a.q.stride_token +
+                           static_cast<i64>(qh) * a.q.stride_head;
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[k][i] = load_elem(a.q.q, at + k * 64 + c * 16 + i, a.q.type);
+                    if (fabsf(x[k][i]) <= 3.402823466e38f) most = fmaxf(most, fabsf(x[k][i]));
+                }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[k][i] = 0.0f;
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        int e = 15;
+        if (most > 0.0f) frexpf(most, &e);
+        e = max(15 - e, -126);
+        e = min(e, 126);
+        const float up = kv_power(e);
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                qf[nt][k * 4 + w][0] = pack_f16(x[k][4 * w] * up, x[k][4 * w + 1] * up);
+                qf[nt][k * 4 + w][1] = pack_f16(x[k][4 * w + 2] * up, x[k][4 * w + 3] * up);
+            }
+        const float f = a.scale2 * kv_power(-e);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            factor[nt][i] = __shfl_sync(0xffffffffu, f, (2 * c + i) * 4);
+            const u32 m = nt * 8 + 2 * c + i;
+            sees[nt][i] = row_position(a, seg, seg.rt * R + min(m, rows - 1));
+        }
+    }
+    const int sees_least = row_position(a, seg, seg.rt * R);
+    const int sees_most = row_position(a, seg, seg.rt * R + rows - 1);
+
+    float o[NT][D / 16][4];
+    float m[NT][2], l[NT][2];
+    float value_scale = 0.0f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.0f;
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.0f;
+    }
+    const int* table = a.q.table + static_cast<i64>(seg.seq) * a.q.table_stride;
+    const int* list = a.blocks ? a.blocks + ((static_cast<u64>(seg.seq) * a.lists + seg.t) *
+                                                 a.c.heads + seg.h) * a.top
+                               : nullptr;
+    const u32 have = (static_cast<u32>(seg.length) + block - 1) / block;
+    for (u32 tile = first + warp; tile < end; tile += kWarps) {
+        u32 j = tile / per_block;
+        if (list) j = static_cast<u32>(list[j]);
+        const int page = j < have ? kv_page(table, j, a.c.pages) : -1;
+        const int p0 = static_cast<int>(j * block + (tile % per_block) * 16);
+        float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + tile) * R
+                                     : nullptr;
+        if (page < 0 || p0 > sees_most) {
+            if (tile_out && lane < R) tile_out[lane] = -INFINITY;
+            continue;
+        }
+        const u64 at = (static_cast<u64>(page) * a.c.heads + seg.h) * 2;
+        const u8* kp = a.c.data + (at * block + (tile % per_block) * 16) * D;
+        const u8* vp = kp + static_cast<u64>(block) * D;
+        uint4 k0[KC], k1[KC];
+        u32 v[4][VW];
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            k0[k] = *reinterpret_cast<const uint4*>(kp + g * D + k * 64 + c * 16);
+            k1[k] = *reinterpret_cast<const uint4*>(kp + (g + 8) * D + k * 64 + c * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u32 token = 2 * c + (i & 1) + (i >> 1) * 8;
+#pragma unroll
+            for (int w = 0; w < VW; ++w)
+                v[i][w] = *reinterpret_cast<const u32*>(vp + token * D + g * (D / 8) + w * 4);
+        }
+        const float key_scale = a.c.scale[at], new_scale = a.c.scale[at + 1];
+
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[nt][k] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            const u32 w0[4] = {k0[k].x, k0[k].y, k0[k].z, k0[k].w};
+            const u32 w1[4] = {k1[k].x, k1[k].y, k1[k].z, k1[k].w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const u32 a0 = e4m3x2_to_f16x2(w0[w]), a2 = e4m3x2_to_f16x2(w0[w] >> 16);
+                const u32 a1 = e4m3x2_to_f16x2(w1[w]), a3 = e4m3x2_to_f16x2(w1[w] >> 16);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma16816(s[nt], a0, a1, a2, a3, qf[nt][k * 4 + w][0], qf[nt][k * 4 + w][1]);
+            }
+        }
+        const bool edge = p0 + 15 > sees_least;
+        u32 keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // value tokens that some row sees
+        if (edge) {
+            const int n = sees_most - p0 - static_cast<int>(2 * c);  // token 2c + i is seen if i <= n
+            keep_lo = (n >= 0 ? 0x0000ffffu : 0u) | (n >= 1 ? 0xffff0000u : 0u);
+            keep_hi = (n >= 8 ? 0x0000ffffu : 0u) | (n >= 9 ? 0xffff0000u : 0u);
+        }
+        // largest value scale so far; a change rescales what is summed
+        float carry = 1.0f;
+        if (new_scale > value_scale) {
+            carry = value_scale / new_scale;
+            value_scale = new_scale;
+        }
+        const float relative = new_scale / value_scale;
+        u32 b[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
+            float sum[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x0 = s[nt][i] * (factor[nt][i] * key_scale);
+                float x1 = s[nt][2 + i] * (factor[nt][i] * key_scale);
+                if (edge) {
+                    if (p0 + static_cast<int>(g) > sees[nt][i]) x0 = -INFINITY;
+                    if (p0 + static_cast<int>(g) + 8 > sees[nt][i]) x1 = -INFINITY;
+                }
+                float most = fmaxf(x0, x1);
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1)
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+                const float now = fmaxf(m[nt][i], most);
+                const float base = now == -INFINITY ? 0.0f : now;
+                const float shrink = exp2f(m[nt][i] - base);
+                m[nt][i] = now;
+                p[i] = exp2f(x0 - base);
+                p[2 + i] = exp2f(x1 - base);
+                sum[i] = p[i] + p[2 + i];
+                l[nt][i] = l[nt][i] * shrink + sum[i];
+                const float f = shrink * carry;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    o[nt][k][i] *= f;
+                    o[nt][k][2 + i] *= f;
+                }
+            }
+            b[nt][0] = transpose8x8(pack_f16(p[0] * relative, p[1] * relative));
+            b[nt][1] = transpose8x8(pack_f16(p[2] * relative, p[3] * relative));
+            if (tile_out) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1)
+                        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], off);
+                    if (g == 0)
+                        tile_out[nt * 8 + 2 * c + i] =
+                            sum[i] == 0.0f ? -INFINITY : log2f(sum[i]) + m[nt][i];
+                }
+            }
+        }
+        const bool staggered = edge && sees_least < sees_most;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+            const u32 lo01 = __byte_perm(v[0][w], v[1][w], 0x5140), lo23 = __byte_perm(v[0][w], v[1][w], 0x7362);
+            const u32 hi01 = __byte_perm(v[2][w], v[3][w], 0x5140), hi23 = __byte_perm(v[2][w], v[3][w], 0x7362);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const u32 lo = half ? lo23 : lo01, hi = half ? hi23 : hi01;
+                const u32 a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
+                const u32 a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+                const int k = w * 2 + half;
+                if (!staggered) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma16816(o[nt][k], a0 & keep_lo, a1 & keep_lo, a2 & keep_hi, a3 & keep_hi,
+                                 b[nt][0], b[nt][1]);
+                } else {
+                    // rows end at different tokens: a value past a row's end (it may be NaN)
+                    // must not meet the row at all, so each end is taken by itself
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float old[4], made[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) old[i] = made[i] = o[nt][k][i];
+                        for (int last = sees_least; last <= sees_most; ++last) {
+                            const int n = last - p0 - static_cast<int>(2 * c);
+                            const u32 lo_mask = (n >= 0 ? 0x0000ffffu : 0u) | (n >= 1 ? 0xffff0000u : 0u);
+                            const u32 hi_mask = (n >= 8 ? 0x0000ffffu : 0u) | (n >= 9 ? 0xffff0000u : 0u);
+                            float one[4] = {old[0], old[1], old[2], old[3]};
+                            mma16816(one, a0 & lo_mask, a1 & lo_mask, a2 & hi_mask, a3 & hi_mask,
+                                     b[nt][0], b[nt][1]);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                if (sees[nt][i] == last) {
+                                    made[i] = one[i];
+                                    made[2 + i] = one[2 + i];
+                                }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[nt][k][i] = made[i];
+                    }
+                }
+            }
+        }
+    }
+    // join the warps: every warp's sums at its own maximum, values times its scale
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float sum = l[nt][i];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            const u32 row = nt * 8 + 2 * c + i;
+            if (g == 0) join_ml[warp][row] = make_float2(m[nt][i], sum);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                join_o[warp][row][g * (D / 8) + 2 * k] = o[nt][k][i] * value_scale;
+                join_o[warp][row][g * (D / 8) + 2 * k + 1] = o[nt][k][2 + i] * value_scale;
+            }
+        }
+    __syncthreads();
+    const u64 part = static_cast<u64>(seg.index) * a.splits + split;
+    for (u32 x = threadIdx.x; x < R * D; x += blockDim.x) {
+        const u32 row = x / D, d = x % D;
+        float top = -INFINITY;
+#pragma unroll
+        for (u32 w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w][row].x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, value = 0.0f;
+#pragma unroll
+        for (u32 w = 0; w < kWarps; ++w) {
+            const float f = exp2f(join_ml[w][row].x - base);
+            sum += join_ml[w][row].y * f;
+            value += join_o[w][row][d] * f;
+        }
+        a.part_o[part * R * D + x] = value;
+        if (d == 0) a.part_ml[part * R + row] = make_float2(top, sum);
+    }
+}
+
+// One CTA per segment: the shares of every row joined, normalised, rounded.
+__global__ void __launch_bounds__(128) combine_kernel(const AttentionArgs a, u32 R)
+{
+    const u32 D = a.c.dim;
+    const Segment seg = segment_of(a, blockIdx.x);
+    const u32 rows = min(R, a.rows - seg.rt * R);
+    const float2* ml = a.part_ml + static_cast<u64>(seg.index) * a.splits * R;
+    const float* part = a.part_o + static_cast<u64>(seg.index) * a.splits * R * D;
+    for (u32 x = threadIdx.x; x < rows * D; x += blockDim.x) {
+        const u32 r = x / D, d = x % D, row = seg.rt * R + r;
+        float top = -INFINITY;
+        for (u32 s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s * R + r].x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, value = 0.0f;
+        for (u32 s = 0; s < a.splits; ++s) {
+            const float f = exp2f(ml[s * R + r].x - base);
+            sum += ml[s * R + r].y * f;
+            value += part[static_cast<u64>(s) * R * D + x] * f;
+        }
+        const float y = sum == 0.0f ? 0.0f : value / sum;
+        const u32 t = a.blocks ? seg.t : row / a.q.group;
+        const u32 qh = seg.h * a.q.group + row % a.q.group;
+        const u64 to = (static_cast<u64>(seg.seq) * a.q.tokens + t) * a.q.q_heads + qh;
+        if (a.q.type == HBFSIM_KV_BF16)
+            static_cast<__nv_bfloat16*>(a.out)[to * D + d] = __float2bfloat16_rn(y);
+        else
+            static_cast<__half*>(a.out)[to * D + d] = __float2half_rn(y);
+        if (d == 0) {
+            const float lse2 = sum == 0.0f ? -INFINITY : log2f(sum) + top;
+            if (a.lse) a.lse[to] = lse2 * kLn2;
+            a.row_lse[static_cast<u64>(seg.index) * R + r] = lse2;
+        }
+    }
+}
+
+// Softmax weight of each block: one CTA per (sequence, head, kWeightBlocks blocks).
+// The sums over rows, tiles and lists run in a fixed order.
+__global__ void __launch_bounds__(kWeightBlocks) weight_kernel(const AttentionArgs a, u32 R)
+{
+    __shared__ float sum[kWeightBlocks];
+    const u32 chunk = blockIdx.x, h = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads;
+    const u32 from = chunk * kWeightBlocks, per_block = a.c.block / 16;
+    const u32 i = threadIdx.x;
+    sum[i] = 0.0f;
+    __syncthreads();
+    for (u32 t = 0; t < a.lists; ++t) {
+        for (u32 rt = 0; rt < a.row_tiles; ++rt) {
+            const u32 index = ((seq * a.lists + t) * a.c.heads + h) * a.row_tiles + rt;
+            const Segment seg = segment_of(a, index);
+            const u32 rows = min(R, a.rows - rt * R);
+            const u32 listed = seg.tiles / per_block + (seg.tiles % per_block ? 1 : 0);
+            const int* list = a.blocks ? a.blocks + ((static_cast<u64>(seq) * a.lists + t) *
+                                                         a.c.heads + h) * a.top
+                                       : nullptr;
+            // a list names a block once, so no two threads add to one sum
+            for (u32 base = list ? 0 : from; base < (list ? listed : min(listed, from + kWeightBlocks));
+                 base += kWeightBlocks) {
+                const u32 k = base + i;
+                float w = 0.0f;
+                u32 j = 0xffffffffu;
+                if (k < listed) {
+                    j = list ? static_cast<u32>(list[k]) : k;
+                    if (j >= from && j < from + kWeightBlocks) {
+                        for (u32 tile = k * per_block; tile < min((k + 1) * per_block, seg.tiles); ++tile) {
+                            const float* x = a.tile_lse + (static_cast<u64>(index) * a.tiles + tile) * R;
+                            const float* y = a.row_lse + static_cast<u64>(index) * R;
+                            for (u32 r = 0; r < rows; ++r)
+                                if (x[r] != -INFINITY) w += exp2f(x[r] - y[r]);
+                        }
+                    } else {
+                        j = 0xffffffffu;
+                    }
+                }
+                if (j != 0xffffffffu) sum[j - from] += w;
+                __syncthreads();
+            }
+        }
+    }
+    const u32 j = from + i;
+    if (j < a.q.width) a.weights[(static_cast<u64>(seq) * a.c.heads + h) * a.q.width + j] = sum[i];
+}
+
+struct Plan {
+    u32 nt, lists, rows, row_tiles, splits, tiles;
+    u64 segments, part_o, part_ml, tile_lse, row_lse, bytes;
+};
+
+// Splits: enough CTAs to fill the GPU four deep, at least 8 tiles to a share.
+Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weights)
+{
+    Plan p{};
+    p.lists = lists ? q.tokens : 1;
+    p.rows = lists ? q.group : q.group * q.tokens;
+    p.nt = p.rows > 8 && v.dim < 256 ? 2 : 1;
+    const u32 R = 8 * p.nt;
+    p.row_tiles = (p.rows + R - 1) / R;
+    p.tiles = (lists ? top : q.width) * (v.block / 16);
+    p.segments = static_cast<u64>(q.seqs) * p.lists * v.heads * p.row_tiles;
+    const u64 want = (592 + p.segments - 1) / std::max<u64>(1, p.segments);
+    p.splits = static_cast<u32>(std::max<u64>(1, std::min<u64>(want, (p.tiles + 7) / 8)));
+    u64 at = 0;
+    auto take = [&](u64 bytes) {
+        const u64 here = at;
+        at += kv_round_up(bytes, 256);
+        return here;
+    };
+    p.part_o = take(p.segments * p.splits * R * v.dim * 4);
+    p.part_ml = take(p.segments * p.splits * R * 8);
+    p.row_lse = take(p.segments * R * 4);
+    p.tile_lse = take(weights ? p.segments * p.tiles * R * 4 : 0);
+    p.bytes = at;
+    return p;
+}
+
+int check_args(const hbfsim_kv_attention_args_v1* g)
+{
+    if (!g || g->struct_size != sizeof(*g) || g->version != HBFSIM_KV_V1_VERSION)
+        return HBFSIM_INVALID_ARGUMENT;
+    if ((g->blocks == nullptr) != (g->counts == nullptr)) return HBFSIM_INVALID_ARGUMENT;
+    if (g->blocks && (g->top == 0 || g->top > kKvMaxWidth)) return HBFSIM_INVALID_ARGUMENT;
+    if (!(g->softmax_scale == g->softmax_scale) || g->softmax_scale > 3.0e38f ||
+        g->softmax_scale < -3.0e38f)
+        return HBFSIM_INVALID_ARGUMENT;
+    return HBFSIM_OK;
+}
+
+template <int D, int NT>
+int launch(const AttentionArgs& a, u64 segments, cudaStream_t s)
+{
+    attention_kernel<D, NT><<<static_cast<u32>(segments * a.splits), kWarps * 32, 0, s>>>(a);
+    combine_kernel<<<static_cast<u32>(segments), 128, 0, s>>>(a, 8 * NT);
+    if (a.weights) {
+        const dim3 grid((a.q.width + kWeightBlocks - 1) / kWeightBlocks, a.q.seqs * a.c.heads);
+        weight_kernel<<<grid, kWeightBlocks, 0, s>>>(a, 8 * NT);
+    }
+    return cudaGetLastError() == cudaSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+}
+
+}  // namespace
+}  // namespace hbfb
+
+using namespace hbfb;
+
+extern "C" uint64_t hbfsim_kv_attention_workspace_v1(const hbfsim_kv_cache_v1* cache,
+                                                     const hbfsim_kv_query_v1* query,
+                                                     const hbfsim_kv_attention_args_v1* args)
+{
+    KvView v{};
+    KvQuery q{};
+    if (kv_check_cache(cache, v) || kv_check_query(query, v, q) || check_args(args)) return 0;
+    if (q.seqs == 0 || q.tokens == 0) return 0;
+    return plan_of(v, q, args->blocks != nullptr, args->top, args->weights != nullptr).bytes;
+}
+
+extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
+                                      const hbfsim_kv_query_v1* query,
+                                      const hbfsim_kv_attention_args_v1* args, void* stream)
+{
+    AttentionArgs a{};
+    if (const int rc = kv_check_cache(cache, a.c)) return rc;
+    if (const int rc = kv_check_query(query, a.c, a.q)) return rc;
+    if (const int rc = check_args(args)) return rc;
+    if (a.q.seqs == 0 || a.q.tokens == 0) return HBFSIM_OK;
+    const Plan p = plan_of(a.c, a.q, args->blocks != nullptr, args->top, args->weights != nullptr);
+    if (p.segments * p.splits > 0x7fffffffull || a.q.seqs * static_cast<u64>(a.c.heads) > 65535)
+        return HBFSIM_UNSUPPORTED;
+    if (!args->out || !args->workspace || args->workspace_bytes < p.bytes ||
+        !kv_aligned(args->workspace, 16) || !kv_aligned(args->out, 2) ||
+        !kv_aligned(args->lse, 4) || !kv_aligned(args->weights, 4) ||
+        !kv_aligned(args->blocks, 4) || !kv_aligned(args->counts, 4))
+        return HBFSIM_INVALID_ARGUMENT;
+    a.scale2 = args->softmax_scale * kLog2e;
+    a.top = args->top;
+    a.blocks = args->blocks;
+    a.counts = args->counts;
+    a.out = args->out;
+    a.lse = args->lse;
+    a.weights = a.q.width ? args->weights : nullptr;
+    a.lists = p.lists;
+    a.row_tiles = p.row_tiles;
+    a.rows = p.rows;
+    a.splits = p.splits;
+    a.tiles = p.tiles;
+    u8* w = static_cast<u8*>(args->workspace);
+    a.part_o = reinterpret_cast<float*>(w + p.part_o);
+    a.part_ml = reinterpret_cast<float2*>(w + p.part_ml);
+    a.row_lse = reinterpret_cast<float*>(w + p.row_lse);
+    a.tile_lse = a.weights ? reinterpret_cast<float*>(w + p.tile_lse) : nullptr;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a.c.dim == 64)
+        return p.nt == 2 ? launch<64, 2>(a, p.segments, s) : launch<64, 1>(a, p.segments, s);
+    if (a.c.dim == 128)
+        return p.nt == 2 ? launch<128, 2>(a, p.segments, s) : launch<128, 1>(a, p.segments, s);
+    return launch<256, 1>(a, p.segments, s);
+}
