@@ -20,11 +20,14 @@
 // type's own rounding) for the second product only; the sums and the block
 // weights use them unrounded.
 //
-// A CTA's 4 warps stride over the 16-token tiles of their share of one
-// segment (sequence, head, row tile; for lists also the token), join through
-// shared memory and leave one partial result; combine_kernel joins the
-// shares, and weight_kernel turns the tiles' logarithmic sums into block
-// weights.
+// Work: the 16-token tiles of all segments (sequence, head, row tile; for
+// lists also the token) form one line that is cut into equal shares, one per
+// resident CTA, so that ragged lengths leave no SM idle.  A CTA's 4 warps
+// stride over the tiles of its share of a segment, each with a ring of
+// asynchronous copies of its own (no block barrier inside the loop), join
+// through shared memory and leave one partial result per segment met;
+// finish_kernel joins the partials of a segment and turns the tiles'
+// logarithmic sums into block weights.
 #include "kv.h"
 
 #include <cuda_bf16.h>
@@ -36,8 +39,9 @@ namespace hbfb {
 namespace {
 
 constexpr u32 kWarps = 4;
+constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr u32 kWeightBlocks = 256;  // blocks per CTA of weight_kernel
+constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
 struct AttentionArgs {
     KvView c;
@@ -49,13 +53,15 @@ struct AttentionArgs {
     void* out;
     float* lse;
     float* weights;
-    // segments: ((seq * lists + t) * heads + h) * row_tiles + rt, lists = tokens or 1
+    // segments: ((seq * lists + t) * heads + h) * row_tiles + rt, lists = tokens or 1;
+    // `units` runs of `per_unit` neighbouring segments have equally many tiles
     u32 lists, row_tiles, rows;   // rows of one (sequence, list, head)
-    u32 splits, tiles;            // shares per segment; 16-token tiles per segment at most
-    float* part_o;                // [segments][splits][8 NT][D]
-    float2* part_ml;              // [segments][splits][8 NT]: maximum, sum
+    u32 units, per_unit;
+    u32 workers;                  // CTAs of attention_kernel
+    u32 tiles;                    // 16-token tiles per segment at most
+    float* part_o;                // [workers + segments][8 NT][D], at worker + segment
+    float2* part_ml;              // [workers + segments][8 NT]: maximum, sum
     float* tile_lse;              // [segments][tiles][8 NT], or NULL
-    float* row_lse;               // [segments][8 NT]
 };
 
 __device__ __forceinline__ u32 e4m3x2_to_f16x2(u32 two)
@@ -93,11 +99,51 @@ __device__ __forceinline__ float load_elem(const void* p, i64 i, u32 type)
                                   : __half2float(static_cast<const __half*>(p)[i]);
 }
 
+__device__ __forceinline__ float exp2_fast(float x)  // 2^-22 relative, 0 for -inf
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ void copy16(u32 to, const void* from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+__device__ __forceinline__ void copy8(u32 to, const void* from)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+}
+
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void copy_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Place of byte o of a tile side in shared memory: the 16-byte pieces of a
+// 128-byte line are exchanged by the line's number, so that the lanes that
+// read one channel range of 4 tokens, or 8 tokens of one range, meet
+// different banks.
+__device__ __forceinline__ u32 swizzle(u32 o) { return o ^ ((o >> 3) & 0x70u); }
+
 struct Segment {
     u32 seq, t, h, rt, index;
     int length;      // tokens of the sequence
     u32 tiles;       // 16-token tiles of this segment
 };
+
+// 16-token tiles of each segment of a unit (a sequence, or one list).
+__device__ __forceinline__ u32 unit_tiles(const AttentionArgs& a, u32 unit)
+{
+    if (a.blocks)
+        return static_cast<u32>(min(max(a.counts[unit], 0), static_cast<int>(a.top))) *
+               (a.c.block / 16);
+    return (static_cast<u32>(kv_length(a.q.lengths, unit, a.q.width, a.c.block)) + 15) / 16;
+}
 
 __device__ __forceinline__ Segment segment_of(const AttentionArgs& a, u32 index)
 {
@@ -110,13 +156,66 @@ __device__ __forceinline__ Segment segment_of(const AttentionArgs& a, u32 index)
     s.t = r % a.lists;
     s.seq = r / a.lists;
     s.length = kv_length(a.q.lengths, s.seq, a.q.width, a.c.block);
-    if (a.blocks) {
-        const int n = a.counts[(static_cast<u64>(s.seq) * a.lists + s.t) * a.c.heads + s.h];
-        s.tiles = static_cast<u32>(min(max(n, 0), static_cast<int>(a.top))) * (a.c.block / 16);
-    } else {
-        s.tiles = (static_cast<u32>(s.length) + 15) / 16;
-    }
+    s.tiles = unit_tiles(a, index / a.per_unit);
     return s;
+}
+
+// The line of all tiles: its length, and where `unit` begins on it.
+__device__ void line_of(const AttentionArgs& a, u32 unit, u64* shared2, u64& total, u64& before)
+{
+    u64 all = 0, first = 0;
+    for (u32 u = threadIdx.x; u < a.units; u += blockDim.x) {
+        const u64 n = static_cast<u64>(unit_tiles(a, u)) * a.per_unit;
+        all += n;
+        if (u < unit) first += n;
+    }
+    if (threadIdx.x < 2) shared2[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        first += __shfl_xor_sync(0xffffffffu, first, o);
+    }
+    if ((threadIdx.x & 31u) == 0) {
+        atomicAdd(reinterpret_cast<unsigned long long*>(&shared2[0]), all);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&shared2[1]), first);
+    }
+    __syncthreads();
+    total = shared2[0];
+    before = shared2[1];
+}
+
+// Tiles per share.
+__device__ __forceinline__ u64 share_of(const AttentionArgs& a, u64 total)
+{
+    const u64 even = (total + a.workers - 1) / a.workers;
+    return even > kShare ? even : kShare;
+}
+
+// The unit that holds place `at` of the line (at < total), and where it begins.
+__device__ void find_unit(const AttentionArgs& a, u64 at, u64* shared2, u32& unit, u64& begin)
+{
+    u64 done = 0;
+    for (u32 base = 0; base < a.units; base += 32) {  // every warp by itself
+        const u32 lane = threadIdx.x & 31u, u = base + lane;
+        const u64 n = u < a.units ? static_cast<u64>(unit_tiles(a, u)) * a.per_unit : 0;
+        u64 upto = n;
+#pragma unroll
+        for (u32 o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const u32 holds = __ballot_sync(0xffffffffu, at < done + upto);
+        if (holds) {
+            const int k = __ffs(holds) - 1;
+            unit = base + k;
+            begin = done + __shfl_sync(0xffffffffu, upto - n, k);
+            return;
+        }
+        done += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    unit = a.units;
+    begin = done;
 }
 
 // Position of the query token behind a row of the segment (-1: sees nothing).
@@ -126,22 +225,84 @@ __device__ __forceinline__ int row_position(const AttentionArgs& a, const Segmen
     return max(s.length - static_cast<int>(a.q.tokens) + static_cast<int>(t), -1);
 }
 
+// CTAs per SM and the depth of a warp's ring: about 192 KB of rings per SM.
+constexpr u32 per_sm(u32 dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
+template <int D>
+constexpr u32 kStages = D == 256 ? 3 : 4;
+template <int D>
+constexpr u32 kRing = kWarps * kStages<D> * 32 * D;  // bytes
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionArgs a)
+constexpr u32 kSmem = (kRing<D> > kWarps * 8 * NT * D * 4 ? kRing<D> : kWarps * 8 * NT * D * 4) +
+                      kWarps * kStages<D> * 16 + kWarps * 8 * NT * 8 + 16;
+
+// One segment's tiles [first, end) by one CTA; the partial result goes to `part`.
+template <int D, int NT>
+__device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segment& seg, u32 first,
+                                            u32 end, u64 part, u8* smem)
 {
     constexpr int R = 8 * NT;
     constexpr int KC = D / 64;      // 16-byte pieces of a key row per lane
     constexpr int VW = D / 32;      // 4-byte words of a value row per lane
-    __shared__ float join_o[kWarps][R][D];
-    __shared__ float2 join_ml[kWarps][R];
+    constexpr u32 NS = kStages<D>;
+    constexpr u32 kSide = 16 * D;   // bytes of a tile's keys, and of its values
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
-    const Segment seg = segment_of(a, blockIdx.x / a.splits);
-    const u32 split = blockIdx.x % a.splits;
-    // this CTA's share of the tiles
-    const u32 per = (seg.tiles + a.splits - 1) / a.splits;
-    const u32 first = min(split * per, seg.tiles), end = min(first + per, seg.tiles);
+    u8* ring = smem + warp * NS * 2 * kSide;
+    float* join_o = reinterpret_cast<float*>(smem);  // [kWarps][R][D], after the loop
+    constexpr u32 kUpper = kSmem<D, NT> - 16 - kWarps * R * 8 - kWarps * NS * 16;
+    int4* note = reinterpret_cast<int4*>(smem + kUpper) + warp * NS;  // position, -, scales
+    float2* join_ml = reinterpret_cast<float2*>(smem + kUpper + kWarps * NS * 16);  // [kWarps][R]
+    const u32 ring_at = static_cast<u32>(__cvta_generic_to_shared(ring));
+    const u32 note_at = static_cast<u32>(__cvta_generic_to_shared(note));
     const u32 rows = min(static_cast<u32>(R), a.rows - seg.rt * R);
     const u32 block = a.c.block, per_block = block / 16;
+
+    const int sees_least = row_position(a, seg, seg.rt * R);
+    const int sees_most = row_position(a, seg, seg.rt * R + rows - 1);
+    const int* table = a.q.table + static_cast<i64>(seg.seq) * a.q.table_stride;
+    const int* list = a.blocks ? a.blocks + ((static_cast<u64>(seg.seq) * a.lists + seg.t) *
+                                                 a.c.heads + seg.h) * a.top
+                               : nullptr;
+    const u32 have = (static_cast<u32>(seg.length) + block - 1) / block;
+    const u32 turns = first + warp < end ? (end - first - warp + kWarps - 1) / kWarps : 0;
+
+    // Copies of the warp's i-th tile into stage i % NS.  The blocks and pages of 32 turns are
+    // looked up at once, one per lane.
+    int my_page = -1;
+    u32 my_block = 0;
+    auto issue = [&](u32 i) {
+        if (i < turns) {
+            if (i % 32 == 0) {
+                my_page = -1;
+                if (i + lane < turns) {
+                    my_block = (first + warp + (i + lane) * kWarps) / per_block;
+                    if (list) my_block = static_cast<u32>(list[my_block]);
+                    if (my_block < have) my_page = kv_page(table, my_block, a.c.pages);
+                }
+            }
+            const int page = __shfl_sync(0xffffffffu, my_page, i % 32);
+            const u32 j = __shfl_sync(0xffffffffu, my_block, i % 32);
+            const u32 sub = (first + warp + i * kWarps) % per_block, stage = i % NS;
+            const int p0 = static_cast<int>(j * block + sub * 16);
+            const bool there = page >= 0 && p0 <= sees_most;
+            if (lane == 0) note[stage].x = there ? p0 : -1;
+            if (there) {
+                const u64 at = (static_cast<u64>(page) * a.c.heads + seg.h) * 2;
+                const u8* from = a.c.data + (at * block + sub * 16) * D;
+                const u32 to = ring_at + stage * 2 * kSide;
+#pragma unroll
+                for (u32 k = 0; k < kSide; k += 512)
+                    copy16(to + swizzle(k + lane * 16), from + k + lane * 16);
+                from += static_cast<u64>(block) * D;
+#pragma unroll
+                for (u32 k = 0; k < kSide; k += 512)
+                    copy16(to + kSide + swizzle(k + lane * 16), from + k + lane * 16);
+                if (lane == 0) copy8(note_at + stage * 16 + 8, a.c.scale + at);
+            }
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (u32 i = 0; i + 1 < NS; ++i) issue(i);
 
     // queries: row n = 8 nt + g, scaled by a power of two so that the largest is in [2^14, 2^15)
     u32 qf[NT][D / 16][2];
@@ -163,7 +324,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionA
             for (int k = 0; k < KC; ++k)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    x[k][i] = load_elem(a.q.q, at + k * 64 + c * 16 + i, a.q.type);
+                    x[k][i] = load_elem(a.q.q, at + (c * KC + k) * 16 + i, a.q.type);
                     if (fabsf(x[k][i]) <= 3.402823466e38f) most = fmaxf(most, fabsf(x[k][i]));
                 }
         } else {
@@ -194,8 +355,6 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionA
             sees[nt][i] = row_position(a, seg, seg.rt * R + min(m, rows - 1));
         }
     }
-    const int sees_least = row_position(a, seg, seg.rt * R);
-    const int sees_most = row_position(a, seg, seg.rt * R + rows - 1);
 
     float o[NT][D / 16][4];
     float m[NT][2], l[NT][2];
@@ -209,40 +368,46 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionA
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.0f;
     }
-    const int* table = a.q.table + static_cast<i64>(seg.seq) * a.q.table_stride;
-    const int* list = a.blocks ? a.blocks + ((static_cast<u64>(seg.seq) * a.lists + seg.t) *
-                                                 a.c.heads + seg.h) * a.top
-                               : nullptr;
-    const u32 have = (static_cast<u32>(seg.length) + block - 1) / block;
-    for (u32 tile = first + warp; tile < end; tile += kWarps) {
-        u32 j = tile / per_block;
-        if (list) j = static_cast<u32>(list[j]);
-        const int page = j < have ? kv_page(table, j, a.c.pages) : -1;
-        const int p0 = static_cast<int>(j * block + (tile % per_block) * 16);
+    for (u32 i = 0; i < turns; ++i) {
+        copy_wait<NS - 2>();
+        __syncwarp();  // the stage is there, and every lane is done with the one before it
+        issue(i + NS - 1);
+        const u32 tile = first + warp + i * kWarps, stage = i % NS;
         float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + tile) * R
                                      : nullptr;
-        if (page < 0 || p0 > sees_most) {
+        const int4 noted = note[stage];
+        const int p0 = noted.x;
+        if (p0 < 0) {
             if (tile_out && lane < R) tile_out[lane] = -INFINITY;
             continue;
         }
-        const u64 at = (static_cast<u64>(page) * a.c.heads + seg.h) * 2;
-        const u8* kp = a.c.data + (at * block + (tile % per_block) * 16) * D;
-        const u8* vp = kp + static_cast<u64>(block) * D;
+        const u8* kp = ring + stage * 2 * kSide;
+        const float key_scale = __int_as_float(noted.z), new_scale = __int_as_float(noted.w);
         uint4 k0[KC], k1[KC];
         u32 v[4][VW];
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
-            k0[k] = *reinterpret_cast<const uint4*>(kp + g * D + k * 64 + c * 16);
-            k1[k] = *reinterpret_cast<const uint4*>(kp + (g + 8) * D + k * 64 + c * 16);
+            k0[k] = *reinterpret_cast<const uint4*>(kp + swizzle(g * D + (c * KC + k) * 16));
+            k1[k] = *reinterpret_cast<const uint4*>(kp + swizzle((g + 8) * D + (c * KC + k) * 16));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const u32 token = 2 * c + (i & 1) + (i >> 1) * 8;
+        for (int x = 0; x < 4; ++x) {
+            const u32 o = (2 * c + (x & 1) + (x >> 1) * 8) * D + g * (D / 8);
+            if constexpr (VW == 2) {
+                const uint2 y = *reinterpret_cast<const uint2*>(kp + kSide + swizzle(o));
+                v[x][0] = y.x;
+                v[x][1] = y.y;
+            } else {
 #pragma unroll
-            for (int w = 0; w < VW; ++w)
-                v[i][w] = *reinterpret_cast<const u32*>(vp + token * D + g * (D / 8) + w * 4);
+                for (int w = 0; w < VW; w += 4) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(kp + kSide + swizzle(o + w * 4));
+                    v[x][w] = y.x;
+                    v[x][w + 1] = y.y;
+                    v[x][w + 2] = y.z;
+                    v[x][w + 3] = y.w;
+                }
+            }
         }
-        const float key_scale = a.c.scale[at], new_scale = a.c.scale[at + 1];
 
         float s[NT][4];
 #pragma unroll
@@ -279,8 +444,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionA
         u32 b[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float p[4];
-            float sum[2];
+            float p[4], sum[2], f[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 float x0 = s[nt][i] * (factor[nt][i] * key_scale);
@@ -295,17 +459,21 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionA
                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
                 const float now = fmaxf(m[nt][i], most);
                 const float base = now == -INFINITY ? 0.0f : now;
-                const float shrink = exp2f(m[nt][i] - base);
+                const float shrink = exp2_fast(m[nt][i] - base);
                 m[nt][i] = now;
-                p[i] = exp2f(x0 - base);
-                p[2 + i] = exp2f(x1 - base);
+                p[i] = exp2_fast(x0 - base);
+                p[2 + i] = exp2_fast(x1 - base);
                 sum[i] = p[i] + p[2 + i];
                 l[nt][i] = l[nt][i] * shrink + sum[i];
-                const float f = shrink * carry;
+                f[i] = shrink * carry;
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                    o[nt][k][i] *= f;
-                    o[nt][k][2 + i] *= f;
+                    o[nt][k][0] *= f[0];
+                    o[nt][k][2] *= f[0];
+                    o[nt][k][1] *= f[1];
+                    o[nt][k][3] *= f[1];
                 }
             }
             b[nt][0] = transpose8x8(pack_f16(p[0] * relative, p[1] * relative));
@@ -367,6 +535,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionA
             }
         }
     }
+    copy_wait<0>();
+    __syncthreads();  // every ring is at rest: its memory takes the joined values
     // join the warps: every warp's sums at its own maximum, values times its scale
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -376,121 +546,177 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionA
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             const u32 row = nt * 8 + 2 * c + i;
-            if (g == 0) join_ml[warp][row] = make_float2(m[nt][i], sum);
+            if (g == 0) join_ml[warp * R + row] = make_float2(m[nt][i], sum);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-                join_o[warp][row][g * (D / 8) + 2 * k] = o[nt][k][i] * value_scale;
-                join_o[warp][row][g * (D / 8) + 2 * k + 1] = o[nt][k][2 + i] * value_scale;
+                float* to = join_o + (warp * R + row) * D + g * (D / 8) + 2 * k;
+                to[0] = o[nt][k][i] * value_scale;
+                to[1] = o[nt][k][2 + i] * value_scale;
             }
         }
     __syncthreads();
-    const u64 part = static_cast<u64>(seg.index) * a.splits + split;
     for (u32 x = threadIdx.x; x < R * D; x += blockDim.x) {
-        const u32 row = x / D, d = x % D;
+        const u32 row = x / D;
         float top = -INFINITY;
 #pragma unroll
-        for (u32 w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w][row].x);
+        for (u32 w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * R + row].x);
         const float base = top == -INFINITY ? 0.0f : top;
         float sum = 0.0f, value = 0.0f;
 #pragma unroll
         for (u32 w = 0; w < kWarps; ++w) {
-            const float f = exp2f(join_ml[w][row].x - base);
-            sum += join_ml[w][row].y * f;
-            value += join_o[w][row][d] * f;
+            const float f = exp2_fast(join_ml[w * R + row].x - base);
+            sum += join_ml[w * R + row].y * f;
+            value += join_o[w * R * D + x] * f;
         }
         a.part_o[part * R * D + x] = value;
-        if (d == 0) a.part_ml[part * R + row] = make_float2(top, sum);
+        if (x % D == 0) a.part_ml[part * R + row] = make_float2(top, sum);
+    }
+    __syncthreads();  // before the next segment's copies
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, per_sm(D)) attention_kernel(const AttentionArgs a)
+{
+    extern __shared__ __align__(128) u8 smem[];
+    u64* shared2 = reinterpret_cast<u64*>(smem + kSmem<D, NT> - 16);
+    u64 total, before;
+    line_of(a, 0, shared2, total, before);
+    const u64 share = share_of(a, total);
+    u64 at = blockIdx.x * share;
+    const u64 stop = min(at + share, total);
+    if (at >= stop) return;
+    u32 unit;
+    u64 begin;
+    find_unit(a, at, shared2, unit, begin);
+    u32 tiles = unit_tiles(a, unit);
+    while (at < stop) {
+        while (tiles == 0 || at >= begin + static_cast<u64>(tiles) * a.per_unit) {
+            begin += static_cast<u64>(tiles) * a.per_unit;
+            tiles = unit_tiles(a, ++unit);
+        }
+        const u32 inside = static_cast<u32>((at - begin) / tiles);
+        const u64 here = begin + static_cast<u64>(inside) * tiles;
+        const Segment seg = segment_of(a, unit * a.per_unit + inside);
+        const u32 first = static_cast<u32>(at - here);
+        const u32 end = static_cast<u32>(min(stop - here, static_cast<u64>(tiles)));
+        run_segment<D, NT>(a, seg, first, end, static_cast<u64>(blockIdx.x) + seg.index, smem);
+        at = here + end;
     }
 }
 
-// One CTA per segment: the shares of every row joined, normalised, rounded.
-__global__ void __launch_bounds__(128) combine_kernel(const AttentionArgs a, u32 R)
+// One CTA per (sequence, head, kFinishThreads blocks): joins the partial
+// results of its part of the rows, and sums the weights of its blocks.  All
+// sums run in a fixed order.
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R)
 {
-    const u32 D = a.c.dim;
-    const Segment seg = segment_of(a, blockIdx.x);
-    const u32 rows = min(R, a.rows - seg.rt * R);
-    const float2* ml = a.part_ml + static_cast<u64>(seg.index) * a.splits * R;
-    const float* part = a.part_o + static_cast<u64>(seg.index) * a.splits * R * D;
-    for (u32 x = threadIdx.x; x < rows * D; x += blockDim.x) {
-        const u32 r = x / D, d = x % D, row = seg.rt * R + r;
-        float top = -INFINITY;
-        for (u32 s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s * R + r].x);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, value = 0.0f;
-        for (u32 s = 0; s < a.splits; ++s) {
-            const float f = exp2f(ml[s * R + r].x - base);
-            sum += ml[s * R + r].y * f;
-            value += part[static_cast<u64>(s) * R * D + x] * f;
-        }
-        const float y = sum == 0.0f ? 0.0f : value / sum;
-        const u32 t = a.blocks ? seg.t : row / a.q.group;
-        const u32 qh = seg.h * a.q.group + row % a.q.group;
-        const u64 to = (static_cast<u64>(seg.seq) * a.q.tokens + t) * a.q.q_heads + qh;
-        if (a.q.type == HBFSIM_KV_BF16)
-            static_cast<__nv_bfloat16*>(a.out)[to * D + d] = __float2bfloat16_rn(y);
-        else
-            static_cast<__half*>(a.out)[to * D + d] = __float2half_rn(y);
-        if (d == 0) {
-            const float lse2 = sum == 0.0f ? -INFINITY : log2f(sum) + top;
-            if (a.lse) a.lse[to] = lse2 * kLn2;
-            a.row_lse[static_cast<u64>(seg.index) * R + r] = lse2;
-        }
-    }
-}
-
-// Softmax weight of each block: one CTA per (sequence, head, kWeightBlocks blocks).
-// The sums over rows, tiles and lists run in a fixed order.
-__global__ void __launch_bounds__(kWeightBlocks) weight_kernel(const AttentionArgs a, u32 R)
-{
-    __shared__ float sum[kWeightBlocks];
-    const u32 chunk = blockIdx.x, h = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads;
-    const u32 from = chunk * kWeightBlocks, per_block = a.c.block / 16;
+    __shared__ u64 shared2[2];
+    __shared__ float2 row_ml[16];     // maximum and sum of the rows at hand
+    __shared__ float sum[kFinishThreads];
+    const u32 chunk = blockIdx.x, chunks = gridDim.x;
+    const u32 h = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads;
+    const u32 from = chunk * kFinishThreads, per_block = a.c.block / 16, D = a.c.dim;
+    const u32 first_segment = (seq * a.lists * a.c.heads + h) * a.row_tiles;
+    const u32 first_unit = first_segment / a.per_unit;
+    u64 total, begin;
+    line_of(a, first_unit, shared2, total, begin);
+    const u64 share = share_of(a, total);
     const u32 i = threadIdx.x;
     sum[i] = 0.0f;
-    __syncthreads();
+    u32 unit = first_unit;
     for (u32 t = 0; t < a.lists; ++t) {
         for (u32 rt = 0; rt < a.row_tiles; ++rt) {
             const u32 index = ((seq * a.lists + t) * a.c.heads + h) * a.row_tiles + rt;
+            while (unit < index / a.per_unit) {
+                begin += static_cast<u64>(unit_tiles(a, unit)) * a.per_unit;
+                ++unit;
+            }
             const Segment seg = segment_of(a, index);
             const u32 rows = min(R, a.rows - rt * R);
-            const u32 listed = seg.tiles / per_block + (seg.tiles % per_block ? 1 : 0);
+            const u64 here = begin + static_cast<u64>(index % a.per_unit) * seg.tiles;
+            // partials of this segment: workers w0 .. w0 + parts - 1
+            const u64 w0 = seg.tiles ? here / share : 0;
+            const u32 parts = seg.tiles ? static_cast<u32>((here + seg.tiles - 1) / share - w0) + 1 : 0;
+            const float2* ml = a.part_ml + (w0 + index) * R;
+            __syncthreads();
+            if (i < rows) {
+                float top = -INFINITY, all = 0.0f;
+                for (u32 s = 0; s < parts; ++s) top = fmaxf(top, ml[s * R + i].x);
+                const float base = top == -INFINITY ? 0.0f : top;
+                for (u32 s = 0; s < parts; ++s) all += ml[s * R + i].y * exp2_fast(ml[s * R + i].x - base);
+                row_ml[i] = make_float2(base, all);
+            }
+            __syncthreads();
+            const float* part = a.part_o + (w0 + index) * R * D;
+            // the chunks of CTAs share the segment's rows
+            for (u32 x = chunk * kFinishThreads + i; x < rows * D; x += chunks * kFinishThreads) {
+                const u32 r = x / D, d = x % D, row = rt * R + r;
+                float value = 0.0f;
+                for (u32 s = 0; s < parts; ++s)
+                    value += part[static_cast<u64>(s) * R * D + x] * exp2_fast(ml[s * R + r].x - row_ml[r].x);
+                const float all = row_ml[r].y;
+                const float y = all == 0.0f ? 0.0f : value / all;
+                const u32 tt = a.blocks ? t : row / a.q.group;
+                const u32 qh = h * a.q.group + row % a.q.group;
+                const u64 to = (static_cast<u64>(seq) * a.q.tokens + tt) * a.q.q_heads + qh;
+                if (a.q.type == HBFSIM_KV_BF16)
+                    static_cast<__nv_bfloat16*>(a.out)[to * D + d] = __float2bfloat16_rn(y);
+                else
+                    static_cast<__half*>(a.out)[to * D + d] = __float2half_rn(y);
+                if (d == 0 && a.lse)
+                    a.lse[to] = all == 0.0f ? -INFINITY : (log2f(all) + row_ml[r].x) * kLn2;
+            }
+            if (!a.tile_lse) continue;
+            if (i < rows) row_ml[i].x += log2f(row_ml[i].y);  // only its own row's thread reads .y
+            __syncthreads();
+            const u32 listed = (seg.tiles + per_block - 1) / per_block;
             const int* list = a.blocks ? a.blocks + ((static_cast<u64>(seq) * a.lists + t) *
                                                          a.c.heads + h) * a.top
                                        : nullptr;
             // a list names a block once, so no two threads add to one sum
-            for (u32 base = list ? 0 : from; base < (list ? listed : min(listed, from + kWeightBlocks));
-                 base += kWeightBlocks) {
+            const u32 stop = list ? listed : min(listed, from + kFinishThreads);
+            for (u32 base = list ? 0 : from; base < stop; base += kFinishThreads) {
                 const u32 k = base + i;
-                float w = 0.0f;
-                u32 j = 0xffffffffu;
                 if (k < listed) {
-                    j = list ? static_cast<u32>(list[k]) : k;
-                    if (j >= from && j < from + kWeightBlocks) {
+                    const u32 j = list ? static_cast<u32>(list[k]) : k;
+                    if (j >= from && j - from < kFinishThreads) {
+                        float w = 0.0f;
                         for (u32 tile = k * per_block; tile < min((k + 1) * per_block, seg.tiles); ++tile) {
                             const float* x = a.tile_lse + (static_cast<u64>(index) * a.tiles + tile) * R;
-                            const float* y = a.row_lse + static_cast<u64>(index) * R;
                             for (u32 r = 0; r < rows; ++r)
-                                if (x[r] != -INFINITY) w += exp2f(x[r] - y[r]);
+                                if (x[r] != -INFINITY) w += exp2_fast(x[r] - row_ml[r].x);
                         }
-                    } else {
-                        j = 0xffffffffu;
+                        sum[j - from] += w;
                     }
                 }
-                if (j != 0xffffffffu) sum[j - from] += w;
                 __syncthreads();
             }
         }
     }
     const u32 j = from + i;
-    if (j < a.q.width) a.weights[(static_cast<u64>(seq) * a.c.heads + h) * a.q.width + j] = sum[i];
+    if (a.tile_lse && j < a.q.width)
+        a.weights[(static_cast<u64>(seq) * a.c.heads + h) * a.q.width + j] = sum[i];
 }
 
 struct Plan {
-    u32 nt, lists, rows, row_tiles, splits, tiles;
-    u64 segments, part_o, part_ml, tile_lse, row_lse, bytes;
+    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles;
+    u64 segments, part_o, part_ml, tile_lse, bytes;
 };
 
-// Splits: enough CTAs to fill the GPU four deep, at least 8 tiles to a share.
+int sm_count()
+{
+    static int counts[64];  // by device; the value does not change
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 148;
+    if (device >= 64) device = 63;
+    if (counts[device] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0)
+            n = 148;
+        counts[device] = n;
+    }
+    return counts[device];
+}
+
 Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weights)
 {
     Plan p{};
@@ -500,18 +726,21 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     const u32 R = 8 * p.nt;
     p.row_tiles = (p.rows + R - 1) / R;
     p.tiles = (lists ? top : q.width) * (v.block / 16);
-    p.segments = static_cast<u64>(q.seqs) * p.lists * v.heads * p.row_tiles;
-    const u64 want = (592 + p.segments - 1) / std::max<u64>(1, p.segments);
-    p.splits = static_cast<u32>(std::max<u64>(1, std::min<u64>(want, (p.tiles + 7) / 8)));
+    p.units = lists ? q.seqs * q.tokens * v.heads : q.seqs;
+    p.per_unit = lists ? p.row_tiles : v.heads * p.row_tiles;
+    p.segments = static_cast<u64>(p.units) * p.per_unit;
+    // as many CTAs as are resident at once, fewer for little work
+    const u64 most = (p.segments * p.tiles + kShare - 1) / kShare;
+    p.workers = static_cast<u32>(
+        std::max<u64>(1, std::min<u64>(most, static_cast<u64>(per_sm(v.dim)) * sm_count())));
     u64 at = 0;
     auto take = [&](u64 bytes) {
         const u64 here = at;
         at += kv_round_up(bytes, 256);
         return here;
     };
-    p.part_o = take(p.segments * p.splits * R * v.dim * 4);
-    p.part_ml = take(p.segments * p.splits * R * 8);
-    p.row_lse = take(p.segments * R * 4);
+    p.part_o = take((p.segments + p.workers) * R * v.dim * 4);
+    p.part_ml = take((p.segments + p.workers) * R * 8);
     p.tile_lse = take(weights ? p.segments * p.tiles * R * 4 : 0);
     p.bytes = at;
     return p;
@@ -530,14 +759,15 @@ int check_args(const hbfsim_kv_attention_args_v1* g)
 }
 
 template <int D, int NT>
-int launch(const AttentionArgs& a, u64 segments, cudaStream_t s)
+int launch(const AttentionArgs& a, cudaStream_t s)
 {
-    attention_kernel<D, NT><<<static_cast<u32>(segments * a.splits), kWarps * 32, 0, s>>>(a);
-    combine_kernel<<<static_cast<u32>(segments), 128, 0, s>>>(a, 8 * NT);
-    if (a.weights) {
-        const dim3 grid((a.q.width + kWeightBlocks - 1) / kWeightBlocks, a.q.seqs * a.c.heads);
-        weight_kernel<<<grid, kWeightBlocks, 0, s>>>(a, 8 * NT);
-    }
+    if (cudaFuncSetAttribute(attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kSmem<D, NT>) != cudaSuccess)
+        return HBFSIM_CUDA_ERROR;
+    attention_kernel<D, NT><<<a.workers, kWarps * 32, kSmem<D, NT>, s>>>(a);
+    const dim3 grid(std::max(1u, (a.q.width + kFinishThreads - 1) / kFinishThreads),
+                    a.q.seqs * a.c.heads);
+    finish_kernel<<<grid, kFinishThreads, 0, s>>>(a, 8 * NT);
     return cudaGetLastError() == cudaSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
@@ -567,7 +797,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     if (const int rc = check_args(args)) return rc;
     if (a.q.seqs == 0 || a.q.tokens == 0) return HBFSIM_OK;
     const Plan p = plan_of(a.c, a.q, args->blocks != nullptr, args->top, args->weights != nullptr);
-    if (p.segments * p.splits > 0x7fffffffull || a.q.seqs * static_cast<u64>(a.c.heads) > 65535)
+    if (p.segments > 0x7fffffffull || a.q.seqs * static_cast<u64>(a.c.heads) > 65535)
         return HBFSIM_UNSUPPORTED;
     if (!args->out || !args->workspace || args->workspace_bytes < p.bytes ||
         !kv_aligned(args->workspace, 16) || !kv_aligned(args->out, 2) ||
@@ -584,17 +814,16 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     a.lists = p.lists;
     a.row_tiles = p.row_tiles;
     a.rows = p.rows;
-    a.splits = p.splits;
+    a.units = p.units;
+    a.per_unit = p.per_unit;
+    a.workers = p.workers;
     a.tiles = p.tiles;
     u8* w = static_cast<u8*>(args->workspace);
     a.part_o = reinterpret_cast<float*>(w + p.part_o);
     a.part_ml = reinterpret_cast<float2*>(w + p.part_ml);
-    a.row_lse = reinterpret_cast<float*>(w + p.row_lse);
     a.tile_lse = a.weights ? reinterpret_cast<float*>(w + p.tile_lse) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a.c.dim == 64)
-        return p.nt == 2 ? launch<64, 2>(a, p.segments, s) : launch<64, 1>(a, p.segments, s);
-    if (a.c.dim == 128)
-        return p.nt == 2 ? launch<128, 2>(a, p.segments, s) : launch<128, 1>(a, p.segments, s);
-    return launch<256, 1>(a, p.segments, s);
+    if (a.c.dim == 64) return p.nt == 2 ? launch<64, 2>(a, s) : launch<64, 1>(a, s);
+    if (a.c.dim == 128) return p.nt == 2 ? launch<128, 2>(a, s) : launch<128, 1>(a, s);
+    return launch<256, 1>(a, s);
 }
