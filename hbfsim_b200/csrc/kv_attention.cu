@@ -34,6 +34,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace hbfb {
 namespace {
@@ -104,6 +105,19 @@ __device__ __forceinline__ float exp2_fast(float x)  // 2^-22 relative, 0 for -i
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+
+__device__ __forceinline__ float log2_fast(float x)  // 2^-22 absolute or relative, -inf for 0
+{
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 1 / x for a power of two x, 2^-126 <= x <= 2^126: exact.
+__device__ __forceinline__ float inverse_power(float x)
+{
+    return __int_as_float((254 << 23) - __float_as_int(x));
 }
 
 __device__ __forceinline__ void copy16(u32 to, const void* from)
@@ -226,9 +240,9 @@ __device__ __forceinline__ int row_position(const AttentionArgs& a, const Segmen
 }
 
 // CTAs per SM and the depth of a warp's ring: about 192 KB of rings per SM.
-constexpr u32 per_sm(u32 dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
+constexpr u32 per_sm(u32 dim, u32 nt) { return dim == 256 ? 2 : dim * nt == 256 ? 3 : 4; }
 template <int D>
-constexpr u32 kStages = D == 256 ? 3 : 4;
+constexpr u32 kStages = D == 64 ? 4 : 3;
 template <int D>
 constexpr u32 kRing = kWarps * kStages<D> * 32 * D;  // bytes
 template <int D, int NT>
@@ -254,7 +268,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     const u32 ring_at = static_cast<u32>(__cvta_generic_to_shared(ring));
     const u32 note_at = static_cast<u32>(__cvta_generic_to_shared(note));
     const u32 rows = min(static_cast<u32>(R), a.rows - seg.rt * R);
-    const u32 block = a.c.block, per_block = block / 16;
+    const u32 block = a.c.block, sub_bits = 27 - __clz(block);  // tiles of a block: 1 << sub_bits
 
     const int sees_least = row_position(a, seg, seg.rt * R);
     const int sees_most = row_position(a, seg, seg.rt * R + rows - 1);
@@ -265,44 +279,50 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     const u32 have = (static_cast<u32>(seg.length) + block - 1) / block;
     const u32 turns = first + warp < end ? (end - first - warp + kWarps - 1) / kWarps : 0;
 
-    // Copies of the warp's i-th tile into stage i % NS.  The blocks and pages of 32 turns are
+    // Copies of the warp's i-th tile into a stage (i % NS).  The blocks and pages of 32 turns are
     // looked up at once, one per lane.
     int my_page = -1;
     u32 my_block = 0;
-    auto issue = [&](u32 i) {
+    auto issue = [&](u32 i, u32 stage) {
         if (i < turns) {
             if (i % 32 == 0) {
                 my_page = -1;
                 if (i + lane < turns) {
-                    my_block = (first + warp + (i + lane) * kWarps) / per_block;
+                    my_block = (first + warp + (i + lane) * kWarps) >> sub_bits;
                     if (list) my_block = static_cast<u32>(list[my_block]);
                     if (my_block < have) my_page = kv_page(table, my_block, a.c.pages);
                 }
             }
             const int page = __shfl_sync(0xffffffffu, my_page, i % 32);
             const u32 j = __shfl_sync(0xffffffffu, my_block, i % 32);
-            const u32 sub = (first + warp + i * kWarps) % per_block, stage = i % NS;
+            const u32 sub = (first + warp + i * kWarps) & ((1u << sub_bits) - 1u);
             const int p0 = static_cast<int>(j * block + sub * 16);
             const bool there = page >= 0 && p0 <= sees_most;
             if (lane == 0) note[stage].x = there ? p0 : -1;
             if (there) {
                 const u64 at = (static_cast<u64>(page) * a.c.heads + seg.h) * 2;
-                const u8* from = a.c.data + (at * block + sub * 16) * D;
+                const u8* from = a.c.data + (at * block + sub * 16) * D + lane * 16;
+                const u8* from_v = from + block * D;
+                // swizzle(k + lane * 16) for k a multiple of 512: the line number's third bit is k's
                 const u32 to = ring_at + stage * 2 * kSide;
+                const u32 even = to + swizzle(lane * 16), odd = to + swizzle(512 + lane * 16);
 #pragma unroll
-                for (u32 k = 0; k < kSide; k += 512)
-                    copy16(to + swizzle(k + lane * 16), from + k + lane * 16);
-                from += static_cast<u64>(block) * D;
+                for (u32 k = 0; k < kSide; k += 1024) {
+                    copy16(even + k, from + k);
+                    copy16(odd + k, from + k + 512);
+                }
 #pragma unroll
-                for (u32 k = 0; k < kSide; k += 512)
-                    copy16(to + kSide + swizzle(k + lane * 16), from + k + lane * 16);
+                for (u32 k = 0; k < kSide; k += 1024) {
+                    copy16(even + kSide + k, from_v + k);
+                    copy16(odd + kSide + k, from_v + k + 512);
+                }
                 if (lane == 0) copy8(note_at + stage * 16 + 8, a.c.scale + at);
             }
         }
         copy_commit();
     };
 #pragma unroll
-    for (u32 i = 0; i + 1 < NS; ++i) issue(i);
+    for (u32 i = 0; i + 1 < NS; ++i) issue(i, i);
 
     // queries: row n = 8 nt + g, scaled by a power of two so that the largest is in [2^14, 2^15)
     u32 qf[NT][D / 16][2];
@@ -358,7 +378,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 
     float o[NT][D / 16][4];
     float m[NT][2], l[NT][2];
-    float value_scale = 0.0f;
+    float value_scale = 0.0f, value_inverse = 0.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -368,39 +388,56 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.0f;
     }
-    for (u32 i = 0; i < turns; ++i) {
-        copy_wait<NS - 2>();
-        __syncwarp();  // the stage is there, and every lane is done with the one before it
-        issue(i + NS - 1);
-        const u32 tile = first + warp + i * kWarps, stage = i % NS;
-        float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + tile) * R
-                                     : nullptr;
-        const int4 noted = note[stage];
-        const int p0 = noted.x;
-        if (p0 < 0) {
-            if (tile_out && lane < R) tile_out[lane] = -INFINITY;
-            continue;
-        }
-        const u8* kp = ring + stage * 2 * kSide;
-        const float key_scale = __int_as_float(noted.z), new_scale = __int_as_float(noted.w);
-        uint4 k0[KC], k1[KC];
-        u32 v[4][VW];
+    // where the lane's pieces lie in a tile side, and the same 8 tokens further: at D = 64 that
+    // is 4 lines on, which turns the exchange by 4
+    auto further = [](u32 at) { return D == 64 ? (at ^ 0x40u) + 512u : at + 8u * D; };
+    u32 key_at[KC], value_at[2][VW >= 4 ? VW / 4 : 1];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) key_at[k] = swizzle(g * D + (c * KC + k) * 16);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int w = 0; w < (VW >= 4 ? VW / 4 : 1); ++w)
+            value_at[x][w] = kSide + swizzle((2 * c + x) * D + g * (D / 8) + w * 16);
+
+    // One tile.  `edge`: some row does not see all of its tokens.
+    auto consume = [&](auto is_edge, const u8* tile, int p0, float key_scale, float new_scale,
+                       float* tile_out) {
+        constexpr bool kEdge = decltype(is_edge)::value;
+        float s[NT][4], s2[NT][4];  // two sums, so that products need not wait for each other
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[nt][k] = s2[nt][k] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
-            k0[k] = *reinterpret_cast<const uint4*>(kp + swizzle(g * D + (c * KC + k) * 16));
-            k1[k] = *reinterpret_cast<const uint4*>(kp + swizzle((g + 8) * D + (c * KC + k) * 16));
+            const uint4 k0 = *reinterpret_cast<const uint4*>(tile + key_at[k]);
+            const uint4 k1 = *reinterpret_cast<const uint4*>(tile + further(key_at[k]));
+            const u32 w0[4] = {k0.x, k0.y, k0.z, k0.w};
+            const u32 w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const u32 a0 = e4m3x2_to_f16x2(w0[w]), a2 = e4m3x2_to_f16x2(w0[w] >> 16);
+                const u32 a1 = e4m3x2_to_f16x2(w1[w]), a3 = e4m3x2_to_f16x2(w1[w] >> 16);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma16816(w & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][k * 4 + w][0],
+                             qf[nt][k * 4 + w][1]);
+            }
         }
+        u32 v[4][VW];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            const u32 o = (2 * c + (x & 1) + (x >> 1) * 8) * D + g * (D / 8);
             if constexpr (VW == 2) {
-                const uint2 y = *reinterpret_cast<const uint2*>(kp + kSide + swizzle(o));
+                const uint2 y = *reinterpret_cast<const uint2*>(
+                    tile + (x >> 1 ? further(value_at[x & 1][0]) : value_at[x & 1][0]));
                 v[x][0] = y.x;
                 v[x][1] = y.y;
             } else {
 #pragma unroll
                 for (int w = 0; w < VW; w += 4) {
-                    const uint4 y = *reinterpret_cast<const uint4*>(kp + kSide + swizzle(o + w * 4));
+                    const u32 at = value_at[x & 1][w / 4];
+                    const uint4 y = *reinterpret_cast<const uint4*>(tile + (x >> 1 ? further(at) : at));
                     v[x][w] = y.x;
                     v[x][w + 1] = y.y;
                     v[x][w + 2] = y.z;
@@ -408,48 +445,24 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 }
             }
         }
-
-        float s[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[nt][k] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KC; ++k) {
-            const u32 w0[4] = {k0[k].x, k0[k].y, k0[k].z, k0[k].w};
-            const u32 w1[4] = {k1[k].x, k1[k].y, k1[k].z, k1[k].w};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const u32 a0 = e4m3x2_to_f16x2(w0[w]), a2 = e4m3x2_to_f16x2(w0[w] >> 16);
-                const u32 a1 = e4m3x2_to_f16x2(w1[w]), a3 = e4m3x2_to_f16x2(w1[w] >> 16);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    mma16816(s[nt], a0, a1, a2, a3, qf[nt][k * 4 + w][0], qf[nt][k * 4 + w][1]);
-            }
-        }
-        const bool edge = p0 + 15 > sees_least;
-        u32 keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // value tokens that some row sees
-        if (edge) {
-            const int n = sees_most - p0 - static_cast<int>(2 * c);  // token 2c + i is seen if i <= n
-            keep_lo = (n >= 0 ? 0x0000ffffu : 0u) | (n >= 1 ? 0xffff0000u : 0u);
-            keep_hi = (n >= 8 ? 0x0000ffffu : 0u) | (n >= 9 ? 0xffff0000u : 0u);
-        }
         // largest value scale so far; a change rescales what is summed
         float carry = 1.0f;
         if (new_scale > value_scale) {
-            carry = value_scale / new_scale;
+            carry = value_scale * inverse_power(new_scale);
             value_scale = new_scale;
+            value_inverse = inverse_power(new_scale);
         }
-        const float relative = new_scale / value_scale;
+        const float relative = new_scale * value_inverse;
         u32 b[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float p[4], sum[2], f[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float x0 = s[nt][i] * (factor[nt][i] * key_scale);
-                float x1 = s[nt][2 + i] * (factor[nt][i] * key_scale);
-                if (edge) {
+                const float scaled = factor[nt][i] * key_scale;
+                float x0 = (s[nt][i] + s2[nt][i]) * scaled;
+                float x1 = (s[nt][2 + i] + s2[nt][2 + i]) * scaled;
+                if constexpr (kEdge) {
                     if (p0 + static_cast<int>(g) > sees[nt][i]) x0 = -INFINITY;
                     if (p0 + static_cast<int>(g) + 8 > sees[nt][i]) x1 = -INFINITY;
                 }
@@ -484,55 +497,88 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1)
                         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], off);
-                    if (g == 0)
-                        tile_out[nt * 8 + 2 * c + i] =
-                            sum[i] == 0.0f ? -INFINITY : log2f(sum[i]) + m[nt][i];
+                    sum[i] = sum[i] == 0.0f ? -INFINITY : log2_fast(sum[i]) + m[nt][i];
                 }
+                if (g == 0)
+                    *reinterpret_cast<float2*>(tile_out + nt * 8 + 2 * c) = make_float2(sum[0], sum[1]);
             }
         }
-        const bool staggered = edge && sees_least < sees_most;
+        u32 keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // value tokens that some row sees
+        bool staggered = false;
+        if constexpr (kEdge) {
+            const int n = sees_most - p0 - static_cast<int>(2 * c);  // token 2c + i is seen if i <= n
+            keep_lo = (n >= 0 ? 0x0000ffffu : 0u) | (n >= 1 ? 0xffff0000u : 0u);
+            keep_hi = (n >= 8 ? 0x0000ffffu : 0u) | (n >= 9 ? 0xffff0000u : 0u);
+            staggered = sees_least < sees_most;
+        }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
-            const u32 lo01 = __byte_perm(v[0][w], v[1][w], 0x5140), lo23 = __byte_perm(v[0][w], v[1][w], 0x7362);
-            const u32 hi01 = __byte_perm(v[2][w], v[3][w], 0x5140), hi23 = __byte_perm(v[2][w], v[3][w], 0x7362);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const u32 lo = half ? lo23 : lo01, hi = half ? hi23 : hi01;
-                const u32 a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
-                const u32 a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+                const u32 pick = half ? 0x7362 : 0x5140;
+                const u32 lo = __byte_perm(v[0][w], v[1][w], pick), hi = __byte_perm(v[2][w], v[3][w], pick);
+                u32 a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
+                u32 a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
                 const int k = w * 2 + half;
-                if (!staggered) {
+                if constexpr (kEdge) {
+                    if (staggered) {
+                        // rows end at different tokens: a value past a row's end (it may be NaN)
+                        // must not meet the row at all, so each end is taken by itself
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma16816(o[nt][k], a0 & keep_lo, a1 & keep_lo, a2 & keep_hi, a3 & keep_hi,
-                                 b[nt][0], b[nt][1]);
-                } else {
-                    // rows end at different tokens: a value past a row's end (it may be NaN)
-                    // must not meet the row at all, so each end is taken by itself
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float old[4], made[4];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float old[4], made[4];
+                            for (int i = 0; i < 4; ++i) old[i] = made[i] = o[nt][k][i];
+                            for (int last = sees_least; last <= sees_most; ++last) {
+                                const int n = last - p0 - static_cast<int>(2 * c);
+                                const u32 lo_mask = (n >= 0 ? 0x0000ffffu : 0u) | (n >= 1 ? 0xffff0000u : 0u);
+                                const u32 hi_mask = (n >= 8 ? 0x0000ffffu : 0u) | (n >= 9 ? 0xffff0000u : 0u);
+                                float one[4] = {old[0], old[1], old[2], old[3]};
+                                mma16816(one, a0 & lo_mask, a1 & lo_mask, a2 & hi_mask, a3 & hi_mask,
+                                         b[nt][0], b[nt][1]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) old[i] = made[i] = o[nt][k][i];
-                        for (int last = sees_least; last <= sees_most; ++last) {
-                            const int n = last - p0 - static_cast<int>(2 * c);
-                            const u32 lo_mask = (n >= 0 ? 0x0000ffffu : 0u) | (n >= 1 ? 0xffff0000u : 0u);
-                            const u32 hi_mask = (n >= 8 ? 0x0000ffffu : 0u) | (n >= 9 ? 0xffff0000u : 0u);
-                            float one[4] = {old[0], old[1], old[2], old[3]};
-                            mma16816(one, a0 & lo_mask, a1 & lo_mask, a2 & hi_mask, a3 & hi_mask,
-                                     b[nt][0], b[nt][1]);
+                                for (int i = 0; i < 2; ++i)
+                                    if (sees[nt][i] == last) {
+                                        made[i] = one[i];
+                                        made[2 + i] = one[2 + i];
+                                    }
+                            }
 #pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                if (sees[nt][i] == last) {
-                                    made[i] = one[i];
-                                    made[2 + i] = one[2 + i];
-                                }
+                            for (int i = 0; i < 4; ++i) o[nt][k][i] = made[i];
                         }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[nt][k][i] = made[i];
+                        continue;
                     }
+                    a0 &= keep_lo;
+                    a1 &= keep_lo;
+                    a2 &= keep_hi;
+                    a3 &= keep_hi;
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma16816(o[nt][k], a0, a1, a2, a3, b[nt][0], b[nt][1]);
             }
+        }
+    };
+
+    u32 stage = 0;
+    for (u32 i = 0; i < turns; ++i) {
+        copy_wait<NS - 2>();
+        __syncwarp();  // the stage is there, and every lane is done with the one before it
+        issue(i + NS - 1, stage == 0 ? NS - 1 : stage - 1);
+        const int4 noted = note[stage];
+        float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + first +
+                                                     warp + i * kWarps) * R
+                                     : nullptr;
+        const u8* tile = ring + stage * 2 * kSide;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        if (noted.x < 0) {
+            if (tile_out && lane < R) tile_out[lane] = -INFINITY;
+        } else if (noted.x + 15 > sees_least) {
+            consume(std::true_type{}, tile, noted.x, __int_as_float(noted.z), __int_as_float(noted.w),
+                    tile_out);
+        } else {
+            consume(std::false_type{}, tile, noted.x, __int_as_float(noted.z), __int_as_float(noted.w),
+                    tile_out);
         }
     }
     copy_wait<0>();
@@ -575,7 +621,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, per_sm(D)) attention_kernel(const AttentionArgs a)
+__global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(const AttentionArgs a)
 {
     extern __shared__ __align__(128) u8 smem[];
     u64* shared2 = reinterpret_cast<u64*>(smem + kSmem<D, NT> - 16);
@@ -611,6 +657,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
 {
     __shared__ u64 shared2[2];
     __shared__ float2 row_ml[16];     // maximum and sum of the rows at hand
+    __shared__ float row_lse[16];     // their logarithm
     __shared__ float sum[kFinishThreads];
     const u32 chunk = blockIdx.x, chunks = gridDim.x;
     const u32 h = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads;
@@ -644,6 +691,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                 const float base = top == -INFINITY ? 0.0f : top;
                 for (u32 s = 0; s < parts; ++s) all += ml[s * R + i].y * exp2_fast(ml[s * R + i].x - base);
                 row_ml[i] = make_float2(base, all);
+                row_lse[i] = all == 0.0f ? -INFINITY : log2f(all) + base;
             }
             __syncthreads();
             const float* part = a.part_o + (w0 + index) * R * D;
@@ -663,11 +711,9 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                 else
                     static_cast<__half*>(a.out)[to * D + d] = __float2half_rn(y);
                 if (d == 0 && a.lse)
-                    a.lse[to] = all == 0.0f ? -INFINITY : (log2f(all) + row_ml[r].x) * kLn2;
+                    a.lse[to] = row_lse[r] * kLn2;
             }
             if (!a.tile_lse) continue;
-            if (i < rows) row_ml[i].x += log2f(row_ml[i].y);  // only its own row's thread reads .y
-            __syncthreads();
             const u32 listed = (seg.tiles + per_block - 1) / per_block;
             const int* list = a.blocks ? a.blocks + ((static_cast<u64>(seq) * a.lists + t) *
                                                          a.c.heads + h) * a.top
@@ -683,7 +729,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                         for (u32 tile = k * per_block; tile < min((k + 1) * per_block, seg.tiles); ++tile) {
                             const float* x = a.tile_lse + (static_cast<u64>(index) * a.tiles + tile) * R;
                             for (u32 r = 0; r < rows; ++r)
-                                if (x[r] != -INFINITY) w += exp2_fast(x[r] - row_ml[r].x);
+                                if (x[r] != -INFINITY) w += exp2_fast(x[r] - row_lse[r]);
                         }
                         sum[j - from] += w;
                     }
@@ -732,7 +778,7 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     // as many CTAs as are resident at once, fewer for little work
     const u64 most = (p.segments * p.tiles + kShare - 1) / kShare;
     p.workers = static_cast<u32>(
-        std::max<u64>(1, std::min<u64>(most, static_cast<u64>(per_sm(v.dim)) * sm_count())));
+        std::max<u64>(1, std::min<u64>(most, static_cast<u64>(per_sm(v.dim, p.nt)) * sm_count())));
     u64 at = 0;
     auto take = [&](u64 bytes) {
         const u64 here = at;
