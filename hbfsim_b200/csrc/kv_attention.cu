@@ -41,6 +41,9 @@ namespace {
 
 constexpr u32 kWarps = 4;
 constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
+// How far (in log2) a score may exceed the reference before the reference moves: a tile then
+// costs a vote instead of a maximum over the lanes.  2^kAbove keeps f16 probabilities finite.
+constexpr float kAbove = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
@@ -62,6 +65,7 @@ struct AttentionArgs {
     u32 tiles;                    // 16-token tiles per segment at most
     float* part_o;                // [workers + segments][8 NT][D], at worker + segment
     float2* part_ml;              // [workers + segments][8 NT]: maximum, sum
+    uint2* span;                  // [segments]: first and last worker (segments with tiles)
     float* tile_lse;              // [segments][tiles][8 NT], or NULL
 };
 
@@ -174,29 +178,19 @@ __device__ __forceinline__ Segment segment_of(const AttentionArgs& a, u32 index)
     return s;
 }
 
-// The line of all tiles: its length, and where `unit` begins on it.
-__device__ void line_of(const AttentionArgs& a, u32 unit, u64* shared2, u64& total, u64& before)
+// Length of the line of all tiles.
+__device__ u64 line_of(const AttentionArgs& a, u64* shared)
 {
-    u64 all = 0, first = 0;
-    for (u32 u = threadIdx.x; u < a.units; u += blockDim.x) {
-        const u64 n = static_cast<u64>(unit_tiles(a, u)) * a.per_unit;
-        all += n;
-        if (u < unit) first += n;
-    }
-    if (threadIdx.x < 2) shared2[threadIdx.x] = 0;
+    u64 all = 0;
+    for (u32 u = threadIdx.x; u < a.units; u += blockDim.x)
+        all += static_cast<u64>(unit_tiles(a, u)) * a.per_unit;
+    if (threadIdx.x == 0) *shared = 0;
     __syncthreads();
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        all += __shfl_xor_sync(0xffffffffu, all, o);
-        first += __shfl_xor_sync(0xffffffffu, first, o);
-    }
-    if ((threadIdx.x & 31u) == 0) {
-        atomicAdd(reinterpret_cast<unsigned long long*>(&shared2[0]), all);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&shared2[1]), first);
-    }
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if ((threadIdx.x & 31u) == 0) atomicAdd(reinterpret_cast<unsigned long long*>(shared), all);
     __syncthreads();
-    total = shared2[0];
-    before = shared2[1];
+    return *shared;
 }
 
 // Tiles per share.
@@ -207,7 +201,7 @@ __device__ __forceinline__ u64 share_of(const AttentionArgs& a, u64 total)
 }
 
 // The unit that holds place `at` of the line (at < total), and where it begins.
-__device__ void find_unit(const AttentionArgs& a, u64 at, u64* shared2, u32& unit, u64& begin)
+__device__ void find_unit(const AttentionArgs& a, u64 at, u32& unit, u64& begin)
 {
     u64 done = 0;
     for (u32 base = 0; base < a.units; base += 32) {  // every warp by itself
@@ -279,6 +273,9 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     const u32 have = (static_cast<u32>(seg.length) + block - 1) / block;
     const u32 turns = first + warp < end ? (end - first - warp + kWarps - 1) / kWarps : 0;
 
+    const u32 page_bytes = a.c.heads * 2 * block * D, page_scales = a.c.heads * 2;
+    const u8* head_data = a.c.data + seg.h * 2 * block * D + lane * 16;
+    const float* head_scale = a.c.scale + seg.h * 2;
     // Copies of the warp's i-th tile into a stage (i % NS).  The blocks and pages of 32 turns are
     // looked up at once, one per lane.
     int my_page = -1;
@@ -300,8 +297,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             const bool there = page >= 0 && p0 <= sees_most;
             if (lane == 0) note[stage].x = there ? p0 : -1;
             if (there) {
-                const u64 at = (static_cast<u64>(page) * a.c.heads + seg.h) * 2;
-                const u8* from = a.c.data + (at * block + sub * 16) * D + lane * 16;
+                const u8* from = head_data + static_cast<u64>(page) * page_bytes + sub * (16 * D);
                 const u8* from_v = from + block * D;
                 // swizzle(k + lane * 16) for k a multiple of 512: the line number's third bit is k's
                 const u32 to = ring_at + stage * 2 * kSide;
@@ -316,7 +312,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                     copy16(even + kSide + k, from_v + k);
                     copy16(odd + kSide + k, from_v + k + 512);
                 }
-                if (lane == 0) copy8(note_at + stage * 16 + 8, a.c.scale + at);
+                if (lane == 0) copy8(note_at + stage * 16 + 8, head_scale + static_cast<u64>(page) * page_scales);
             }
         }
         copy_commit();
@@ -446,61 +442,73 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             }
         }
         // largest value scale so far; a change rescales what is summed
-        float carry = 1.0f;
         if (new_scale > value_scale) {
-            carry = value_scale * inverse_power(new_scale);
-            value_scale = new_scale;
             value_inverse = inverse_power(new_scale);
+            const float carry = value_scale * value_inverse;
+            value_scale = new_scale;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[nt][k][i] *= carry;
         }
         const float relative = new_scale * value_inverse;
         u32 b[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float p[4], sum[2], f[2];
+            float p[4], sum[2];
+            bool above = false;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float scaled = factor[nt][i] * key_scale;
-                float x0 = (s[nt][i] + s2[nt][i]) * scaled;
-                float x1 = (s[nt][2 + i] + s2[nt][2 + i]) * scaled;
+                p[i] = (s[nt][i] + s2[nt][i]) * scaled;
+                p[2 + i] = (s[nt][2 + i] + s2[nt][2 + i]) * scaled;
                 if constexpr (kEdge) {
-                    if (p0 + static_cast<int>(g) > sees[nt][i]) x0 = -INFINITY;
-                    if (p0 + static_cast<int>(g) + 8 > sees[nt][i]) x1 = -INFINITY;
+                    if (p0 + static_cast<int>(g) > sees[nt][i]) p[i] = -INFINITY;
+                    if (p0 + static_cast<int>(g) + 8 > sees[nt][i]) p[2 + i] = -INFINITY;
                 }
-                float most = fmaxf(x0, x1);
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1)
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-                const float now = fmaxf(m[nt][i], most);
-                const float base = now == -INFINITY ? 0.0f : now;
-                const float shrink = exp2_fast(m[nt][i] - base);
-                m[nt][i] = now;
-                p[i] = exp2_fast(x0 - base);
-                p[2 + i] = exp2_fast(x1 - base);
-                sum[i] = p[i] + p[2 + i];
-                l[nt][i] = l[nt][i] * shrink + sum[i];
-                f[i] = shrink * carry;
+                above |= fmaxf(p[i], p[2 + i]) > m[nt][i] + kAbove;
             }
-            if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
+            // the reference of the exponentials follows the maximum only when a score is far
+            // above it; until then probabilities reach 2^kAbove
+            if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    o[nt][k][0] *= f[0];
-                    o[nt][k][2] *= f[0];
-                    o[nt][k][1] *= f[1];
-                    o[nt][k][3] *= f[1];
+                for (int i = 0; i < 2; ++i) {
+                    float most = fmaxf(p[i], p[2 + i]);
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1)
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+                    const float now = fmaxf(m[nt][i], most);
+                    const float shrink = now == -INFINITY ? 1.0f : exp2_fast(m[nt][i] - now);
+                    m[nt][i] = now;
+                    l[nt][i] *= shrink;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        o[nt][k][i] *= shrink;
+                        o[nt][k][2 + i] *= shrink;
+                    }
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float base = m[nt][i] == -INFINITY ? 0.0f : m[nt][i];
+                p[i] = exp2_fast(p[i] - base);
+                p[2 + i] = exp2_fast(p[2 + i] - base);
+                sum[i] = p[i] + p[2 + i];
+                l[nt][i] += sum[i];
             }
             b[nt][0] = transpose8x8(pack_f16(p[0] * relative, p[1] * relative));
             b[nt][1] = transpose8x8(pack_f16(p[2] * relative, p[3] * relative));
             if (tile_out) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1)
-                        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], off);
-                    sum[i] = sum[i] == 0.0f ? -INFINITY : log2_fast(sum[i]) + m[nt][i];
-                }
-                if (g == 0)
-                    *reinterpret_cast<float2*>(tile_out + nt * 8 + 2 * c) = make_float2(sum[0], sum[1]);
+                // the two columns' sums over the lanes of all g, the even g keeping the first
+                const float mine = g & 1 ? sum[1] : sum[0], other = g & 1 ? sum[0] : sum[1];
+                float all = mine + __shfl_xor_sync(0xffffffffu, other, 4);
+                all += __shfl_xor_sync(0xffffffffu, all, 8);
+                all += __shfl_xor_sync(0xffffffffu, all, 16);
+                if (g < 2)
+                    tile_out[nt * 8 + 2 * c + g] =
+                        all == 0.0f ? -INFINITY : log2_fast(all) + (g ? m[nt][1] : m[nt][0]);
             }
         }
         u32 keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // value tokens that some row sees
@@ -561,14 +569,13 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     };
 
     u32 stage = 0;
+    float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + first + warp) * R
+                                 : nullptr;
     for (u32 i = 0; i < turns; ++i) {
         copy_wait<NS - 2>();
         __syncwarp();  // the stage is there, and every lane is done with the one before it
         issue(i + NS - 1, stage == 0 ? NS - 1 : stage - 1);
         const int4 noted = note[stage];
-        float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + first +
-                                                     warp + i * kWarps) * R
-                                     : nullptr;
         const u8* tile = ring + stage * 2 * kSide;
         stage = stage + 1 == NS ? 0 : stage + 1;
         if (noted.x < 0) {
@@ -580,6 +587,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             consume(std::false_type{}, tile, noted.x, __int_as_float(noted.z), __int_as_float(noted.w),
                     tile_out);
         }
+        if (tile_out) tile_out += kWarps * R;
     }
     copy_wait<0>();
     __syncthreads();  // every ring is at rest: its memory takes the joined values
@@ -624,16 +632,14 @@ template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(const AttentionArgs a)
 {
     extern __shared__ __align__(128) u8 smem[];
-    u64* shared2 = reinterpret_cast<u64*>(smem + kSmem<D, NT> - 16);
-    u64 total, before;
-    line_of(a, 0, shared2, total, before);
+    const u64 total = line_of(a, reinterpret_cast<u64*>(smem + kSmem<D, NT> - 16));
     const u64 share = share_of(a, total);
     u64 at = blockIdx.x * share;
     const u64 stop = min(at + share, total);
     if (at >= stop) return;
     u32 unit;
     u64 begin;
-    find_unit(a, at, shared2, unit, begin);
+    find_unit(a, at, unit, begin);
     u32 tiles = unit_tiles(a, unit);
     while (at < stop) {
         while (tiles == 0 || at >= begin + static_cast<u64>(tiles) * a.per_unit) {
@@ -645,107 +651,149 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
         const Segment seg = segment_of(a, unit * a.per_unit + inside);
         const u32 first = static_cast<u32>(at - here);
         const u32 end = static_cast<u32>(min(stop - here, static_cast<u64>(tiles)));
+        if (threadIdx.x == 0) {
+            if (first == 0) a.span[seg.index].x = blockIdx.x;
+            if (end == tiles) a.span[seg.index].y = blockIdx.x;
+        }
         run_segment<D, NT>(a, seg, first, end, static_cast<u64>(blockIdx.x) + seg.index, smem);
         at = here + end;
     }
 }
 
-// One CTA per (sequence, head, kFinishThreads blocks): joins the partial
-// results of its part of the rows, and sums the weights of its blocks.  All
-// sums run in a fixed order.
-__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R)
+// CTAs (x, sequence * heads + head).  The segments of a (sequence, head) are
+// joined by the CTAs x = 0, 1, .. in turn, or, with more CTAs than segments,
+// each by `slices` of them; with weights every CTA also sums those of its
+// share of the blocks.  All sums run in a fixed order.
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R, u32 slices)
 {
-    __shared__ u64 shared2[2];
-    __shared__ float2 row_ml[16];     // maximum and sum of the rows at hand
-    __shared__ float row_lse[16];     // their logarithm
-    __shared__ float sum[kFinishThreads];
-    const u32 chunk = blockIdx.x, chunks = gridDim.x;
+    __shared__ float row_top[16], row_sum[16], row_lse[16];  // of the segment at hand
+    __shared__ float4 join[kFinishThreads];
+    const u32 i = threadIdx.x, lane = i & 31u, warp = i >> 5;
     const u32 h = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads;
-    const u32 from = chunk * kFinishThreads, per_block = a.c.block / 16, D = a.c.dim;
-    const u32 first_segment = (seq * a.lists * a.c.heads + h) * a.row_tiles;
-    const u32 first_unit = first_segment / a.per_unit;
-    u64 total, begin;
-    line_of(a, first_unit, shared2, total, begin);
-    const u64 share = share_of(a, total);
-    const u32 i = threadIdx.x;
-    sum[i] = 0.0f;
-    u32 unit = first_unit;
-    for (u32 t = 0; t < a.lists; ++t) {
-        for (u32 rt = 0; rt < a.row_tiles; ++rt) {
-            const u32 index = ((seq * a.lists + t) * a.c.heads + h) * a.row_tiles + rt;
-            while (unit < index / a.per_unit) {
-                begin += static_cast<u64>(unit_tiles(a, unit)) * a.per_unit;
-                ++unit;
+    const u32 sub_bits = 27 - __clz(a.c.block), D = a.c.dim;
+    const u32 each = (a.q.width + gridDim.x - 1) / gridDim.x;
+    const u32 from = min(blockIdx.x * each, a.q.width), to_block = min(from + each, a.q.width);
+    float* weights = a.tile_lse ? a.weights + (static_cast<u64>(seq) * a.c.heads + h) * a.q.width
+                                : nullptr;
+    for (u32 n = 0; n < a.lists * a.row_tiles; ++n) {
+        u32 slice = n % gridDim.x == blockIdx.x ? 0 : slices;
+        if (slices > 1) slice = blockIdx.x - n * slices;  // wraps for CTAs of other segments
+        const bool joins = slice < slices;
+        if (!joins && !weights) continue;
+        const u32 t = n / a.row_tiles, rt = n % a.row_tiles;
+        const u32 index = ((seq * a.lists + t) * a.c.heads + h) * a.row_tiles + rt;
+        const u32 rows = min(R, a.rows - rt * R);
+        const u32 tiles = unit_tiles(a, index / a.per_unit);
+        const uint2 span = tiles ? a.span[index] : make_uint2(1, 0);  // its first and last worker
+        const u32 parts = span.y + 1 - span.x;
+        const u64 first = static_cast<u64>(span.x) + index;
+        const float2* ml = a.part_ml + first * R;
+        __syncthreads();
+        for (u32 r = warp; r < rows; r += kFinishThreads / 32) {
+            float top = -INFINITY, all = 0.0f;
+            for (u32 s = lane; s < parts; s += 32) top = fmaxf(top, ml[s * R + r].x);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (u32 s = lane; s < parts; s += 32) all += ml[s * R + r].y * exp2_fast(ml[s * R + r].x - base);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            if (lane == 0) {
+                row_top[r] = base;
+                row_sum[r] = all;
+                row_lse[r] = all == 0.0f ? -INFINITY : log2f(all) + base;
             }
-            const Segment seg = segment_of(a, index);
-            const u32 rows = min(R, a.rows - rt * R);
-            const u64 here = begin + static_cast<u64>(index % a.per_unit) * seg.tiles;
-            // partials of this segment: workers w0 .. w0 + parts - 1
-            const u64 w0 = seg.tiles ? here / share : 0;
-            const u32 parts = seg.tiles ? static_cast<u32>((here + seg.tiles - 1) / share - w0) + 1 : 0;
-            const float2* ml = a.part_ml + (w0 + index) * R;
-            __syncthreads();
-            if (i < rows) {
-                float top = -INFINITY, all = 0.0f;
-                for (u32 s = 0; s < parts; ++s) top = fmaxf(top, ml[s * R + i].x);
-                const float base = top == -INFINITY ? 0.0f : top;
-                for (u32 s = 0; s < parts; ++s) all += ml[s * R + i].y * exp2_fast(ml[s * R + i].x - base);
-                row_ml[i] = make_float2(base, all);
-                row_lse[i] = all == 0.0f ? -INFINITY : log2f(all) + base;
-            }
-            __syncthreads();
-            const float* part = a.part_o + (w0 + index) * R * D;
-            // the chunks of CTAs share the segment's rows
-            for (u32 x = chunk * kFinishThreads + i; x < rows * D; x += chunks * kFinishThreads) {
-                const u32 r = x / D, d = x % D, row = rt * R + r;
-                float value = 0.0f;
-                for (u32 s = 0; s < parts; ++s)
-                    value += part[static_cast<u64>(s) * R * D + x] * exp2_fast(ml[s * R + r].x - row_ml[r].x);
-                const float all = row_ml[r].y;
-                const float y = all == 0.0f ? 0.0f : value / all;
+        }
+        __syncthreads();
+        if (joins) {
+            // four channels per thread; groups of threads take the partials in turn
+            const u32 all_pieces = rows * D / 4;
+            const u32 piece0 = all_pieces * slice / slices;
+            const u32 pieces = all_pieces * (slice + 1) / slices - piece0;
+            const u32 groups = max(1u, kFinishThreads / pieces);
+            const float4* part = reinterpret_cast<const float4*>(a.part_o + first * R * D);
+            const u32 group = i / pieces;
+            for (u32 at = pieces < kFinishThreads ? i % pieces : i; at < pieces; at += kFinishThreads) {
+                const u32 x = piece0 + at, r = x * 4 / D;
+                const float base = row_top[r];
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (group < groups || groups == 1) {
+#pragma unroll 8
+                    for (u32 s = groups == 1 ? 0 : group; s < parts; s += groups) {
+                        const float4 y = part[static_cast<u64>(s) * (R * D / 4) + x];
+                        const float f = exp2_fast(ml[s * R + r].x - base);
+                        v.x += y.x * f;
+                        v.y += y.y * f;
+                        v.z += y.z * f;
+                        v.w += y.w * f;
+                    }
+                }
+                if (groups > 1) {
+                    join[i] = v;
+                    __syncthreads();  // pieces < kFinishThreads: every thread is here once
+                    if (group) break;
+                    for (u32 k = 1; k < groups; ++k) {
+                        const float4 y = join[k * pieces + at];
+                        v.x += y.x;
+                        v.y += y.y;
+                        v.z += y.z;
+                        v.w += y.w;
+                    }
+                }
+                const float inverse = row_sum[r] == 0.0f ? 0.0f : 1.0f / row_sum[r];
+                const u32 row = rt * R + r, d = x * 4 % D;
                 const u32 tt = a.blocks ? t : row / a.q.group;
                 const u32 qh = h * a.q.group + row % a.q.group;
                 const u64 to = (static_cast<u64>(seq) * a.q.tokens + tt) * a.q.q_heads + qh;
-                if (a.q.type == HBFSIM_KV_BF16)
-                    static_cast<__nv_bfloat16*>(a.out)[to * D + d] = __float2bfloat16_rn(y);
-                else
-                    static_cast<__half*>(a.out)[to * D + d] = __float2half_rn(y);
-                if (d == 0 && a.lse)
-                    a.lse[to] = row_lse[r] * kLn2;
-            }
-            if (!a.tile_lse) continue;
-            const u32 listed = (seg.tiles + per_block - 1) / per_block;
-            const int* list = a.blocks ? a.blocks + ((static_cast<u64>(seq) * a.lists + t) *
-                                                         a.c.heads + h) * a.top
-                                       : nullptr;
-            // a list names a block once, so no two threads add to one sum
-            const u32 stop = list ? listed : min(listed, from + kFinishThreads);
-            for (u32 base = list ? 0 : from; base < stop; base += kFinishThreads) {
-                const u32 k = base + i;
-                if (k < listed) {
-                    const u32 j = list ? static_cast<u32>(list[k]) : k;
-                    if (j >= from && j - from < kFinishThreads) {
-                        float w = 0.0f;
-                        for (u32 tile = k * per_block; tile < min((k + 1) * per_block, seg.tiles); ++tile) {
-                            const float* x = a.tile_lse + (static_cast<u64>(index) * a.tiles + tile) * R;
-                            for (u32 r = 0; r < rows; ++r)
-                                if (x[r] != -INFINITY) w += exp2_fast(x[r] - row_lse[r]);
-                        }
-                        sum[j - from] += w;
-                    }
+                const float y[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
+#pragma unroll
+                for (u32 k = 0; k < 4; ++k) {
+                    if (a.q.type == HBFSIM_KV_BF16)
+                        static_cast<__nv_bfloat16*>(a.out)[to * D + d + k] = __float2bfloat16_rn(y[k]);
+                    else
+                        static_cast<__half*>(a.out)[to * D + d + k] = __float2half_rn(y[k]);
                 }
-                __syncthreads();
+                if (d == 0 && a.lse) a.lse[to] = row_lse[r] * kLn2;
+            }
+        }
+        if (!weights) continue;
+        const u32 listed = (tiles + (1u << sub_bits) - 1) >> sub_bits;
+        const float* lse = a.tile_lse + static_cast<u64>(index) * a.tiles * R;
+        auto weight_of = [&](u32 k) {
+            float w = 0.0f;
+            for (u32 tile = k << sub_bits; tile < min((k + 1) << sub_bits, tiles); ++tile) {
+                const float4* x = reinterpret_cast<const float4*>(lse + static_cast<u64>(tile) * R);
+                for (u32 r = 0; r < rows; r += 4) {
+                    const float4 y = x[r / 4];
+                    const float z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (u32 q = 0; q < 4; ++q)
+                        if (r + q < rows && z[q] != -INFINITY) w += exp2_fast(z[q] - row_lse[r + q]);
+                }
+            }
+            return w;
+        };
+        if (!a.blocks) {
+            for (u32 j = from + i; j < to_block; j += kFinishThreads) {
+                const float w = j < listed ? weight_of(j) : 0.0f;
+                weights[j] = n ? weights[j] + w : w;  // the same thread's own
+            }
+        } else {
+            const int* list = a.blocks + ((static_cast<u64>(seq) * a.lists + t) * a.c.heads + h) * a.top;
+            if (rt == 0 && t == 0)
+                for (u32 j = from + i; j < to_block; j += kFinishThreads) weights[j] = 0.0f;
+            __syncthreads();
+            for (u32 k = i; k < listed; k += kFinishThreads) {
+                const u32 j = static_cast<u32>(list[k]);
+                if (j >= from && j < to_block) weights[j] += weight_of(k);  // a list names it once
             }
         }
     }
-    const u32 j = from + i;
-    if (a.tile_lse && j < a.q.width)
-        a.weights[(static_cast<u64>(seq) * a.c.heads + h) * a.q.width + j] = sum[i];
 }
 
 struct Plan {
     u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles;
-    u64 segments, part_o, part_ml, tile_lse, bytes;
+    u64 segments, part_o, part_ml, span, tile_lse, bytes;
 };
 
 int sm_count()
@@ -787,6 +835,7 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     };
     p.part_o = take((p.segments + p.workers) * R * v.dim * 4);
     p.part_ml = take((p.segments + p.workers) * R * 8);
+    p.span = take(p.segments * 8);
     p.tile_lse = take(weights ? p.segments * p.tiles * R * 4 : 0);
     p.bytes = at;
     return p;
@@ -811,9 +860,14 @@ int launch(const AttentionArgs& a, cudaStream_t s)
                              kSmem<D, NT>) != cudaSuccess)
         return HBFSIM_CUDA_ERROR;
     attention_kernel<D, NT><<<a.workers, kWarps * 32, kSmem<D, NT>, s>>>(a);
-    const dim3 grid(std::max(1u, (a.q.width + kFinishThreads - 1) / kFinishThreads),
-                    a.q.seqs * a.c.heads);
-    finish_kernel<<<grid, kFinishThreads, 0, s>>>(a, 8 * NT);
+    // one CTA per segment; for the weights of long sequences more, up to what is resident at once
+    const u32 pairs = a.q.seqs * a.c.heads, segments = a.lists * a.row_tiles;
+    u32 across = segments;
+    if (a.weights)
+        across = std::max(across, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
+                                           4u * sm_count() / pairs));
+    const u32 slices = std::min(std::max(1u, across / segments), 8u);
+    finish_kernel<<<dim3(across, pairs), kFinishThreads, 0, s>>>(a, 8 * NT, slices);
     return cudaGetLastError() == cudaSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
@@ -867,6 +921,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     u8* w = static_cast<u8*>(args->workspace);
     a.part_o = reinterpret_cast<float*>(w + p.part_o);
     a.part_ml = reinterpret_cast<float2*>(w + p.part_ml);
+    a.span = reinterpret_cast<uint2*>(w + p.span);
     a.tile_lse = a.weights ? reinterpret_cast<float*>(w + p.tile_lse) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a.c.dim == 64) return p.nt == 2 ? launch<64, 2>(a, s) : launch<64, 1>(a, s);
