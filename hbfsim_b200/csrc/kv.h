@@ -9,6 +9,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 namespace hbfb {
 
 constexpr u32 kKvMaxTokens = 16;      // query tokens per sequence and call
@@ -83,6 +85,46 @@ inline int kv_check_query(const hbfsim_kv_query_v1* q, const KvView& v, KvQuery&
                   q->q_heads / v.heads, q->width, q->type};
     return HBFSIM_OK;
 }
+
+#if defined(__CUDACC__)
+// Dynamic shared memory beyond 48 KB has to be allowed once per kernel and
+// device; `seen` (one per kernel) remembers the devices.
+template <typename Kernel>
+inline bool kv_allow_smem(Kernel* kernel, u32 bytes, std::atomic<u64>& seen)
+{
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return false;
+    const u64 bit = device < 64 ? u64{1} << device : 0;
+    if (seen.load(std::memory_order_acquire) & bit) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(bytes)) != cudaSuccess)
+        return false;
+    seen.fetch_or(bit, std::memory_order_release);
+    return true;
+}
+
+// Launches a kernel that may be set up while the kernel before it on the
+// stream still runs (programmatic dependent launch): it has to begin with
+// kv_wait_before, which returns once that kernel's writes are visible.
+template <typename... Params, typename... Args>
+inline bool kv_launch_behind(void (*kernel)(Params...), dim3 grid, u32 threads, cudaStream_t stream,
+                             Args... args)
+{
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess;
+}
+
+__device__ __forceinline__ void kv_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void kv_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
 
 inline u64 kv_round_up(u64 n, u64 to) { return (n + to - 1) / to * to; }
 

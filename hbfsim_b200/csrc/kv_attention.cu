@@ -632,6 +632,7 @@ template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(const AttentionArgs a)
 {
     extern __shared__ __align__(128) u8 smem[];
+    kv_let_next();
     const u64 total = line_of(a, reinterpret_cast<u64*>(smem + kSmem<D, NT> - 16));
     const u64 share = share_of(a, total);
     u64 at = blockIdx.x * share;
@@ -669,6 +670,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
     __shared__ float row_top[16], row_sum[16], row_lse[16];  // of the segment at hand
     __shared__ float4 join[kFinishThreads];
     const u32 i = threadIdx.x, lane = i & 31u, warp = i >> 5;
+    kv_wait_before();
     const u32 h = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads;
     const u32 sub_bits = 27 - __clz(a.c.block), D = a.c.dim;
     const u32 each = (a.q.width + gridDim.x - 1) / gridDim.x;
@@ -856,9 +858,8 @@ int check_args(const hbfsim_kv_attention_args_v1* g)
 template <int D, int NT>
 int launch(const AttentionArgs& a, cudaStream_t s)
 {
-    if (cudaFuncSetAttribute(attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kSmem<D, NT>) != cudaSuccess)
-        return HBFSIM_CUDA_ERROR;
+    static std::atomic<u64> seen{0};
+    if (!kv_allow_smem(attention_kernel<D, NT>, kSmem<D, NT>, seen)) return HBFSIM_CUDA_ERROR;
     attention_kernel<D, NT><<<a.workers, kWarps * 32, kSmem<D, NT>, s>>>(a);
     // one CTA per segment; for the weights of long sequences more, up to what is resident at once
     const u32 pairs = a.q.seqs * a.c.heads, segments = a.lists * a.row_tiles;
@@ -867,8 +868,9 @@ int launch(const AttentionArgs& a, cudaStream_t s)
         across = std::max(across, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
                                            4u * sm_count() / pairs));
     const u32 slices = std::min(std::max(1u, across / segments), 8u);
-    finish_kernel<<<dim3(across, pairs), kFinishThreads, 0, s>>>(a, 8 * NT, slices);
-    return cudaGetLastError() == cudaSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, a,
+                                     static_cast<u32>(8 * NT), slices);
+    return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
 }  // namespace

@@ -21,6 +21,7 @@ namespace {
 
 constexpr u32 kScoreThreads = 256, kScoreBlocks = 64;  // blocks per CTA
 constexpr u32 kListThreads = 256;
+constexpr u32 kMostQueryBytes = 200 * 1024;  // of shared memory, for the whole-number queries
 constexpr u32 kAbsent = 0u;           // key of a block that cannot be listed
 constexpr u32 kAlways = 0xffffffffu;  // key of a block that is always listed
 
@@ -62,6 +63,7 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectArgs a
 {
     constexpr u32 L = D / 16;   // lanes per (block, head): 16 channels each
     extern __shared__ __align__(16) short whole[];  // [tokens][heads][2][D]: up, down
+    kv_let_next();
     const u32 seq = blockIdx.y, heads = a.c.heads, tokens = a.q.tokens, group = a.q.group;
     const int length = kv_length(a.q.lengths, seq, a.q.width, a.c.block);
     const u32 have = blocks_of_token(length, tokens, tokens - 1, a.c.block);
@@ -151,6 +153,7 @@ __global__ void __launch_bounds__(kListThreads) list_kernel(const SelectArgs a)
     __shared__ u32 histogram[256];
     __shared__ u32 shared2[2];
     __shared__ u32 warp_sums[33];
+    kv_wait_before();
     const u64 at = blockIdx.x;  // (sequence, token, head)
     const u32 heads = a.c.heads, tokens = a.q.tokens;
     const u32 t = static_cast<u32>(at / heads % tokens), seq = static_cast<u32>(at / heads / tokens);
@@ -209,15 +212,13 @@ template <int D>
 int launch(const SelectArgs& a, cudaStream_t s)
 {
     const u32 smem = a.q.tokens * a.c.heads * 2 * D * static_cast<u32>(sizeof(short));
-    if (cudaFuncSetAttribute(score_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess) {
-        cudaGetLastError();
-        return HBFSIM_UNSUPPORTED;
-    }
+    static std::atomic<u64> seen{0};
+    if (!kv_allow_smem(score_kernel<D>, kMostQueryBytes, seen)) return HBFSIM_CUDA_ERROR;
     const dim3 grid((a.q.width + kScoreBlocks - 1) / kScoreBlocks, a.q.seqs);
     if (a.q.width) score_kernel<D><<<grid, kScoreThreads, smem, s>>>(a);
-    list_kernel<<<a.q.seqs * a.q.tokens * a.c.heads, kListThreads, 0, s>>>(a);
-    return cudaGetLastError() == cudaSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    const bool ok = kv_launch_behind(list_kernel, dim3(a.q.seqs * a.q.tokens * a.c.heads),
+                                     kListThreads, s, a);
+    return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
 }  // namespace
@@ -248,7 +249,7 @@ extern "C" int hbfsim_kv_select_v1(const hbfsim_kv_cache_v1* cache,
     const u64 lists = static_cast<u64>(a.q.seqs) * a.q.tokens * a.c.heads;
     if (lists == 0) return HBFSIM_OK;
     // shared memory of the whole-number queries
-    if (static_cast<u64>(a.q.tokens) * a.c.heads * a.c.dim * 4 > 200u * 1024)
+    if (static_cast<u64>(a.q.tokens) * a.c.heads * a.c.dim * 4 > kMostQueryBytes)
         return HBFSIM_UNSUPPORTED;
     if (a.q.seqs > 65535 || !blocks || !counts) return HBFSIM_INVALID_ARGUMENT;
     if (workspace_bytes < workspace_bytes_of(a.c, a.q) || (a.q.width && !workspace) ||

@@ -16,16 +16,23 @@ to that stream.
 """
 from __future__ import annotations
 
-import ctypes
-import math
+import struct
 from typing import NamedTuple
 
 from . import _lib
 from ._lib import check
-from .api import _stream_handle
+from .api import CUDA_STREAM_LEGACY
 
 __all__ = ["KvCache", "KvAttention", "KvSelection", "KvEviction", "kv_append", "kv_attention",
            "kv_select", "kv_evict", "kv_block_reads"]
+
+# The C structures of kv_v1.h as packed bytes (no padding: 8-byte fields lie at multiples of 8);
+# _lib has the same structures field by field.
+_CACHE = struct.Struct("<6I4Q")
+_APPEND = struct.Struct("<6I3Q4qQq2Q")
+_QUERY = struct.Struct("<8IQ3qQqQ")
+_ATTENTION = struct.Struct("<2IfI7Q")
+_EVICT = struct.Struct("<10I3Qq6Q")
 
 
 class KvAttention(NamedTuple):
@@ -59,28 +66,31 @@ class KvCache:
     head_dim]).  The layout and the meaning are in kv_v1.h."""
 
     __slots__ = ("data", "scale", "bounds", "pages", "kv_heads", "block_tokens", "head_dim",
-                 "device", "_struct", "_ref")
+                 "index", "_packed")
 
     def __init__(self, data, scale, bounds):
         import torch
-        _need(data.dim() == 5 and data.shape[2] == 2 and data.dtype == torch.float8_e4m3fn,
+        shape = data.shape
+        _need(len(shape) == 5 and shape[2] == 2 and data.dtype == torch.float8_e4m3fn,
               "data: float8_e4m3fn [pages, kv_heads, 2, block_tokens, head_dim]")
-        self.pages, self.kv_heads, _, self.block_tokens, self.head_dim = data.shape
-        head = (self.pages, self.kv_heads, 2)
-        _need(scale.dtype == torch.float32 and tuple(scale.shape) == head,
+        pages, heads, _, block, dim = shape
+        _need(scale.dtype == torch.float32 and scale.shape == (pages, heads, 2),
               "scale: float32 [pages, kv_heads, 2]")
-        _need(bounds.dtype == torch.int8 and tuple(bounds.shape) == head + (self.head_dim,),
+        _need(bounds.dtype == torch.int8 and bounds.shape == (pages, heads, 2, dim),
               "bounds: int8 [pages, kv_heads, 2, head_dim]")
         _need(data.is_contiguous() and scale.is_contiguous() and bounds.is_contiguous(),
               "data, scale and bounds have to be contiguous")
-        self.device = data.device
-        _need(data.is_cuda and scale.device == data.device and bounds.device == data.device,
+        self.index = index = data.get_device()  # of the CUDA device
+        _need(index >= 0 and scale.get_device() == index and bounds.get_device() == index,
               "data, scale and bounds have to be on one CUDA device")
         self.data, self.scale, self.bounds = data, scale, bounds
-        self._struct = _lib.KvCacheV1(ctypes.sizeof(_lib.KvCacheV1), 1, self.kv_heads,
-                                      self.head_dim, self.block_tokens, 0, self.pages,
-                                      data.data_ptr(), scale.data_ptr(), bounds.data_ptr())
-        self._ref = ctypes.addressof(self._struct)
+        self.pages, self.kv_heads, self.block_tokens, self.head_dim = pages, heads, block, dim
+        self._packed = _CACHE.pack(_CACHE.size, 1, heads, dim, block, 0, pages, data.data_ptr(),
+                                   scale.data_ptr(), bounds.data_ptr())
+
+    @property
+    def device(self):
+        return self.data.device
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int = 128, block_tokens: int = 16,
@@ -107,42 +117,47 @@ def _type(t) -> int:
     return _lib.KV_F16
 
 
-def _check_table(cache_device, table, per_seq, names):
+def _check_table(index, table, per_seq, name):
+    """Shape of the block table; `per_seq` is the int32 tensor that goes with its rows."""
     import torch
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.device == cache_device
-          and (table.shape[1] <= 1 or table.stride(1) == 1),
+    shape = table.shape
+    _need(len(shape) == 2 and table.dtype == torch.int32 and table.get_device() == index
+          and (table.stride(1) == 1 or shape[1] <= 1),
           "table: int32 [seqs, width] on the cache's device, rows contiguous")
-    for x, name in zip(per_seq, names):
-        _need(x.dim() == 1 and x.dtype == torch.int32 and x.shape[0] == table.shape[0]
-              and x.device == cache_device and (x.shape[0] <= 1 or x.stride(0) == 1),
-              f"{name}: int32 [seqs] on the cache's device, contiguous")
+    _need(per_seq.dtype == torch.int32 and per_seq.shape == shape[:1]
+          and per_seq.get_device() == index and (per_seq.stride(0) == 1 or shape[0] <= 1),
+          f"{name}: int32 [seqs] on the cache's device, contiguous")
+    return shape
 
 
 class _On:
-    """Makes the device and the stream current for the allocations of a call."""
+    """Makes a device and a stream current for the allocations of a call."""
 
-    __slots__ = ("device", "stream", "guard", "context")
-
-    def __init__(self, device, stream):
-        self.device, self.stream = device, stream
+    def __init__(self, index, stream):
+        import torch
+        _need(stream is None or stream.device.index == index, "the stream is of another device")
+        self.inside = [torch.cuda.device(index)]
+        if stream is not None:
+            self.inside.append(torch.cuda.stream(stream))
 
     def __enter__(self):
-        import torch
-        self.guard = self.context = None
-        if self.device.index is not None and self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        if self.stream is not None:
-            _need(self.stream.device == self.device, "the stream is of another device")
-            self.context = torch.cuda.stream(self.stream)
-            self.context.__enter__()
-        return _stream_handle(self.stream)
+        for x in self.inside:
+            x.__enter__()
 
     def __exit__(self, *exc):
-        if self.context is not None:
-            self.context.__exit__(*exc)
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        for x in reversed(self.inside):
+            x.__exit__(*exc)
+
+
+def _here(index, stream) -> bool:
+    """Whether the call's device is current and its stream is the current one."""
+    import torch
+    return stream is None and torch._C._cuda_getDevice() == index
+
+
+def _handle(index) -> int:
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index) or CUDA_STREAM_LEGACY
 
 
 def kv_append(cache: KvCache, k, v, table, start, offsets=None, stream=None) -> None:
@@ -153,44 +168,54 @@ def kv_append(cache: KvCache, k, v, table, start, offsets=None, stream=None) -> 
     [offsets[s], offsets[s + 1]); any strides with a contiguous last axis.
     start: int32 [seqs], tokens a sequence held before.  Writes data, scale
     and bounds of the touched blocks in place."""
+    if not _here(cache.index, stream):
+        with _On(cache.index, stream):
+            return kv_append(cache, k, v, table, start, offsets)
     import torch
-    _check_table(cache.device, table, (start,), ("start",))
-    seqs, width = table.shape
-    _need(k.shape == v.shape and k.dtype == v.dtype and k.device == v.device == cache.device
-          and k.dim() == (4 if offsets is None else 3)
-          and k.shape[-2:] == (cache.kv_heads, cache.head_dim),
+    seqs, width = _check_table(cache.index, table, start, "start")
+    shape = k.shape
+    _need(shape == v.shape and k.dtype == v.dtype and k.get_device() == cache.index
+          and v.get_device() == cache.index and len(shape) == (4 if offsets is None else 3)
+          and shape[-2] == cache.kv_heads and shape[-1] == cache.head_dim,
           "k and v: one shape and type, [seqs, n, kv_heads, head_dim] or with offsets "
           "[tokens, kv_heads, head_dim], on the cache's device")
     if offsets is None:
-        _need(k.shape[0] == seqs, "k: as many sequences as the table")
+        _need(shape[0] == seqs, "k: as many sequences as the table")
         k, v = k.flatten(0, 1), v.flatten(0, 1)  # a copy where one stride cannot serve both axes
+        at = 0
     else:
-        _need(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.shape[0] == seqs + 1
-              and offsets.device == cache.device and offsets.is_contiguous(),
+        _need(offsets.dtype == torch.int32 and offsets.shape == (seqs + 1,)
+              and offsets.get_device() == cache.index and offsets.is_contiguous(),
               "offsets: int32 [seqs + 1] on the cache's device, contiguous")
+        at = offsets.data_ptr()
     tokens = k.shape[0]
     if tokens == 0:
         return
-    _need(k.stride(-1) == 1 and v.stride(-1) == 1, "the last axis of k and v has to be contiguous")
-    batch = _lib.KvAppendBatchV1(ctypes.sizeof(_lib.KvAppendBatchV1), 1, _type(k), seqs, width, 0,
-                                 tokens, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
-                                 v.stride(0), v.stride(1), table.data_ptr(), table.stride(0),
-                                 start.data_ptr(), 0 if offsets is None else offsets.data_ptr())
-    with _On(cache.device, stream) as handle:
-        check(_lib.load().hbfsim_kv_append_v1(cache._ref, ctypes.addressof(batch), handle),
-              "hbfsim_kv_append_v1")
+    k_token, k_head, k_dim = k.stride()
+    v_token, v_head, v_dim = v.stride()
+    _need(k_dim == 1 and v_dim == 1, "the last axis of k and v has to be contiguous")
+    batch = _APPEND.pack(_APPEND.size, 1, _type(k), seqs, width, 0, tokens, k.data_ptr(),
+                         v.data_ptr(), k_token, k_head, v_token, v_head, table.data_ptr(),
+                         table.stride(0), start.data_ptr(), at)
+    check(_lib.load().hbfsim_kv_append_v1(cache._packed, batch, _handle(cache.index)),
+          "hbfsim_kv_append_v1")
 
 
-def _query(cache: KvCache, q, table, lengths):
-    _check_table(cache.device, table, (lengths,), ("lengths",))
-    _need(q.dim() == 4 and q.shape[0] == table.shape[0] and q.shape[3] == cache.head_dim
-          and q.device == cache.device, "q: [seqs, tokens, q_heads, head_dim] on the cache's device")
-    _need(q.shape[2] > 0 and q.shape[2] % cache.kv_heads == 0,
-          "q_heads has to be a multiple of kv_heads")
-    _need(q.stride(3) == 1, "the last axis of q has to be contiguous")
-    return _lib.KvQueryV1(ctypes.sizeof(_lib.KvQueryV1), 1, _type(q), q.shape[0], q.shape[1],
-                          q.shape[2], table.shape[1], 0, q.data_ptr(), q.stride(0), q.stride(1),
-                          q.stride(2), table.data_ptr(), table.stride(0), lengths.data_ptr())
+def _query(cache: KvCache, q, table, lengths) -> tuple:
+    """The packed query and its sizes: (bytes, seqs, tokens, q_heads, width)."""
+    table_seqs, width = _check_table(cache.index, table, lengths, "lengths")
+    _need(q.dim() == 4 and q.get_device() == cache.index,
+          "q: [seqs, tokens, q_heads, head_dim] on the cache's device")
+    seqs, tokens, q_heads, dim = q.shape
+    _need(seqs == table_seqs and dim == cache.head_dim,
+          "q: [seqs, tokens, q_heads, head_dim] with the table's seqs and the cache's head_dim")
+    _need(q_heads > 0 and q_heads % cache.kv_heads == 0, "q_heads has to be a multiple of kv_heads")
+    by_seq, by_token, by_head, by_dim = q.stride()
+    _need(by_dim == 1, "the last axis of q has to be contiguous")
+    packed = _QUERY.pack(_QUERY.size, 1, _type(q), seqs, tokens, q_heads, width, 0, q.data_ptr(),
+                         by_seq, by_token, by_head, table.data_ptr(), table.stride(0),
+                         lengths.data_ptr())
+    return packed, seqs, tokens, q_heads, width
 
 
 def kv_select(cache: KvCache, q, table, lengths, top: int, sink: int = 1, recent: int = 1,
@@ -202,19 +227,20 @@ def kv_select(cache: KvCache, q, table, lengths, top: int, sink: int = 1, recent
     q: [seqs, tokens, q_heads, head_dim], the newest tokens, which `lengths`
     counts.  Returns blocks (int32 [seqs, tokens, kv_heads, top], ascending,
     -1 behind the count) and counts (int32 [seqs, tokens, kv_heads])."""
+    if not _here(cache.index, stream):
+        with _On(cache.index, stream):
+            return kv_select(cache, q, table, lengths, top, sink, recent)
     import torch
-    query = _query(cache, q, table, lengths)
-    lib = _lib.load()
-    with _On(cache.device, stream) as handle:
-        shape = (q.shape[0], q.shape[1], cache.kv_heads)
-        blocks = torch.empty(shape + (max(0, top),), dtype=torch.int32, device=cache.device)
-        counts = torch.empty(shape, dtype=torch.int32, device=cache.device)
-        ref = ctypes.addressof(query)
-        size = lib.hbfsim_kv_select_workspace_v1(cache._ref, ref)
-        space = torch.empty(size, dtype=torch.uint8, device=cache.device)
-        check(lib.hbfsim_kv_select_v1(cache._ref, ref, max(0, top), max(0, sink), max(0, recent),
-                                      blocks.data_ptr(), counts.data_ptr(), space.data_ptr(),
-                                      size, handle), "hbfsim_kv_select_v1")
+    _need(top >= 0 and sink >= 0 and recent >= 0, "top, sink and recent are counts")
+    query, seqs, tokens, _, _ = _query(cache, q, table, lengths)
+    lib, device = _lib.load(), q.device
+    blocks = torch.empty((seqs, tokens, cache.kv_heads, top), dtype=torch.int32, device=device)
+    counts = torch.empty((seqs, tokens, cache.kv_heads), dtype=torch.int32, device=device)
+    size = lib.hbfsim_kv_select_workspace_v1(cache._packed, query)
+    space = torch.empty(size, dtype=torch.uint8, device=device)
+    check(lib.hbfsim_kv_select_v1(cache._packed, query, top, sink, recent, blocks.data_ptr(),
+                                  counts.data_ptr(), space.data_ptr(), size, _handle(cache.index)),
+          "hbfsim_kv_select_v1")
     return KvSelection(blocks, counts)
 
 
@@ -229,43 +255,43 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
     natural logarithm of the sum of exponentials) and, if asked for, weights
     (float32 [seqs, kv_heads, width]: softmax weight of every block, summed
     over the group's heads and the tokens; else None)."""
+    if not _here(cache.index, stream):
+        with _On(cache.index, stream):
+            return kv_attention(cache, q, table, lengths, scale, blocks, counts, weights)
     import torch
-    query = _query(cache, q, table, lengths)
-    top = 0
+    query, seqs, tokens, q_heads, width = _query(cache, q, table, lengths)
+    top = blocks_at = counts_at = 0
     if blocks is not None:
-        shape = (q.shape[0], q.shape[1], cache.kv_heads)
+        shape = (seqs, tokens, cache.kv_heads)
         _need(counts is not None and blocks.dtype == torch.int32 and counts.dtype == torch.int32
-              and blocks.dim() == 4 and tuple(blocks.shape[:3]) == shape
-              and tuple(counts.shape) == shape and blocks.is_contiguous()
-              and counts.is_contiguous() and blocks.device == counts.device == cache.device,
+              and blocks.dim() == 4 and blocks.shape[:3] == shape and counts.shape == shape
+              and blocks.is_contiguous() and counts.is_contiguous()
+              and blocks.get_device() == cache.index and counts.get_device() == cache.index,
               "blocks and counts: int32 [seqs, tokens, kv_heads(, top)] on the cache's device, "
               "contiguous")
         top = blocks.shape[3]
         _need(top > 0, "a list has to have room for one block")
+        blocks_at, counts_at = blocks.data_ptr() or 16, counts.data_ptr() or 16  # 0: no lists
     else:
         _need(counts is None, "counts without blocks")
-    lib = _lib.load()
-    with _On(cache.device, stream) as handle:
-        out = torch.empty(q.shape, dtype=q.dtype, device=cache.device)
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=cache.device)
-        mass = None
-        if weights:
-            mass = torch.empty((q.shape[0], cache.kv_heads, table.shape[1]), dtype=torch.float32,
-                               device=cache.device)
-            if q.shape[1] == 0:
-                mass.zero_()
-        args = _lib.KvAttentionArgsV1(
-            ctypes.sizeof(_lib.KvAttentionArgsV1), 1,
-            1.0 / math.sqrt(cache.head_dim) if scale is None else scale, top,
-            None if blocks is None else blocks.data_ptr() or 16,
-            None if blocks is None else counts.data_ptr() or 16, out.data_ptr(), lse.data_ptr(),
-            mass.data_ptr() if weights else None, None, 0)
-        ref, query_ref = ctypes.addressof(args), ctypes.addressof(query)
-        args.workspace_bytes = lib.hbfsim_kv_attention_workspace_v1(cache._ref, query_ref, ref)
-        space = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=cache.device)
-        args.workspace = space.data_ptr()
-        check(lib.hbfsim_kv_attention_v1(cache._ref, query_ref, ref, handle),
-              "hbfsim_kv_attention_v1")
+    lib, device = _lib.load(), q.device
+    out = torch.empty((seqs, tokens, q_heads, cache.head_dim), dtype=q.dtype, device=device)
+    lse = torch.empty((seqs, tokens, q_heads), dtype=torch.float32, device=device)
+    mass, mass_at = None, 0
+    if weights:
+        # with no query token nothing is launched and every weight is 0
+        make = torch.empty if tokens else torch.zeros
+        mass = make((seqs, cache.kv_heads, width), dtype=torch.float32, device=device)
+        mass_at = mass.data_ptr()
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    head = (_ATTENTION.size, 1, scale, top, blocks_at, counts_at, out.data_ptr(), lse.data_ptr(),
+            mass_at)
+    size = lib.hbfsim_kv_attention_workspace_v1(cache._packed, query, _ATTENTION.pack(*head, 0, 0))
+    space = torch.empty(size, dtype=torch.uint8, device=device)
+    check(lib.hbfsim_kv_attention_v1(cache._packed, query,
+                                     _ATTENTION.pack(*head, space.data_ptr(), size),
+                                     _handle(cache.index)), "hbfsim_kv_attention_v1")
     return KvAttention(out, lse, mass)
 
 
@@ -278,32 +304,34 @@ def kv_evict(score, weights, table, lengths, keep: int, block_tokens: int = 16, 
     first `sink` nor the last `recent`.  Returns the new score, table and
     lengths, the pages freed (in block order, -1 behind) and their counts;
     the inputs stay as they are."""
+    index = table.get_device()
+    _need(index >= 0, "the tensors have to be on a CUDA device")
+    if not _here(index, stream):
+        with _On(index, stream):
+            return kv_evict(score, weights, table, lengths, keep, block_tokens, sink, recent, decay)
     import torch
-    _check_table(table.device, table, (lengths,), ("lengths",))
-    seqs, width = table.shape
-    _need(table.is_cuda, "the tensors have to be on a CUDA device")
-    _need(score.dtype == torch.int64 and tuple(score.shape) == (seqs, width)
-          and score.is_contiguous() and score.device == table.device,
-          "score: int64 [seqs, width], contiguous")
+    shape = seqs, width = _check_table(index, table, lengths, "lengths")
+    _need(score.dtype == torch.int64 and score.shape == shape and score.is_contiguous()
+          and score.get_device() == index, "score: int64 [seqs, width], contiguous")
     _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[0] == seqs
           and weights.shape[2] == width and weights.is_contiguous()
-          and weights.device == table.device,
+          and weights.get_device() == index,
           "weights: float32 [seqs, kv_heads, width], contiguous")
-    lib = _lib.load()
-    with _On(table.device, stream) as handle:
-        got = KvEviction(torch.empty_like(score),
-                         torch.empty((seqs, width), dtype=torch.int32, device=table.device),
-                         torch.empty(seqs, dtype=torch.int32, device=table.device),
-                         torch.empty((seqs, width), dtype=torch.int32, device=table.device),
-                         torch.empty(seqs, dtype=torch.int32, device=table.device))
-        batch = _lib.KvEvictBatchV1(
-            ctypes.sizeof(_lib.KvEvictBatchV1), 1, seqs, weights.shape[1], width, block_tokens,
-            max(0, keep), max(0, sink), max(0, recent), max(0, decay), score.data_ptr(),
-            weights.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(),
-            got.score.data_ptr(), got.table.data_ptr(), got.lengths.data_ptr(),
-            got.freed.data_ptr(), got.freed_counts.data_ptr())
-        check(lib.hbfsim_kv_evict_v1(ctypes.addressof(batch), handle), "hbfsim_kv_evict_v1")
-    return got
+    _need(min(keep, block_tokens, sink, recent, decay) >= 0,
+          "keep, block_tokens, sink, recent and decay are counts")
+    device = table.device
+    new_score = torch.empty_like(score)
+    new_table = torch.empty(shape, dtype=torch.int32, device=device)
+    new_lengths = torch.empty(seqs, dtype=torch.int32, device=device)
+    freed = torch.empty(shape, dtype=torch.int32, device=device)
+    freed_counts = torch.empty(seqs, dtype=torch.int32, device=device)
+    batch = _EVICT.pack(_EVICT.size, 1, seqs, weights.shape[1], width, block_tokens, keep, sink,
+                        recent, decay, score.data_ptr(), weights.data_ptr(), table.data_ptr(),
+                        table.stride(0), lengths.data_ptr(), new_score.data_ptr(),
+                        new_table.data_ptr(), new_lengths.data_ptr(), freed.data_ptr(),
+                        freed_counts.data_ptr())
+    check(_lib.load().hbfsim_kv_evict_v1(batch, _handle(index)), "hbfsim_kv_evict_v1")
+    return KvEviction(new_score, new_table, new_lengths, freed, freed_counts)
 
 
 def kv_block_reads(cache: KvCache, table, blocks, counts, base: int):
