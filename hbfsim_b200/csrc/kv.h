@@ -7,6 +7,8 @@
 #include "../../include/hbfsim/kv_v1.h"
 #include "common.h"
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -33,6 +35,7 @@ struct KvQuery {
     i64 table_stride;
     const int* lengths;
     u32 seqs, tokens, q_heads, group, width, type;
+    bool wide;  // every head begins on a 16-byte boundary
 };
 
 inline bool kv_aligned(const void* p, std::uintptr_t a)
@@ -82,7 +85,9 @@ inline int kv_check_query(const hbfsim_kv_query_v1* q, const KvView& v, KvQuery&
     }
     out = KvQuery{q->q, q->q_stride_seq, q->q_stride_token, q->q_stride_head, q->table,
                   q->table_stride, q->lengths, q->seqs, q->tokens, q->q_heads,
-                  q->q_heads / v.heads, q->width, q->type};
+                  q->q_heads / v.heads, q->width, q->type,
+                  kv_aligned(q->q, 16) && q->q_stride_seq % 8 == 0 &&
+                      q->q_stride_token % 8 == 0 && q->q_stride_head % 8 == 0};
     return HBFSIM_OK;
 }
 
@@ -108,7 +113,7 @@ inline bool kv_allow_smem(Kernel* kernel, u32 bytes, std::atomic<u64>& seen)
 // kv_wait_before, which returns once that kernel's writes are visible.
 template <typename... Params, typename... Args>
 inline bool kv_launch_behind(void (*kernel)(Params...), dim3 grid, u32 threads, cudaStream_t stream,
-                             Args... args)
+                             u32 smem, Args... args)
 {
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -117,6 +122,7 @@ inline bool kv_launch_behind(void (*kernel)(Params...), dim3 grid, u32 threads, 
     config.gridDim = grid;
     config.blockDim = dim3(threads);
     config.stream = stream;
+    config.dynamicSmemBytes = smem;
     config.attrs = &attribute;
     config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess;
@@ -125,6 +131,20 @@ inline bool kv_launch_behind(void (*kernel)(Params...), dim3 grid, u32 threads, 
 __device__ __forceinline__ void kv_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void kv_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 #endif
+
+inline int kv_sm_count()
+{
+    static std::atomic<int> counts[64];  // by device; the value does not change
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device > 63) return 148;
+    int n = counts[device].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0)
+            n = 148;
+        counts[device].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
 
 inline u64 kv_round_up(u64 n, u64 to) { return (n + to - 1) / to * to; }
 
@@ -141,6 +161,47 @@ __device__ __forceinline__ int kv_page(const int* table, u32 j, u32 pages)
 {
     const int p = table[j];
     return static_cast<u32>(p) < pages ? p : -1;
+}
+
+// N neighbouring elements of a bf16 or f16 array from `at` on; `wide`: base
+// and `at` allow loads of up to 16 bytes.
+template <int N>
+__device__ __forceinline__ void kv_load(const void* p, i64 at, u32 type, bool wide, float (&x)[N])
+{
+    const unsigned short* from = static_cast<const unsigned short*>(p) + at;
+    u32 w[N / 2];  // pairs of elements
+    if (wide) {
+        if constexpr (N == 2) {
+            w[0] = *reinterpret_cast<const u32*>(from);
+        } else if constexpr (N == 4) {
+            const uint2 y = *reinterpret_cast<const uint2*>(from);
+            w[0] = y.x;
+            w[1] = y.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 8) {
+                const uint4 y = *reinterpret_cast<const uint4*>(from + i);
+                w[i / 2] = y.x;
+                w[i / 2 + 1] = y.y;
+                w[i / 2 + 2] = y.z;
+                w[i / 2 + 3] = y.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) w[i / 2] = from[i] | static_cast<u32>(from[i + 1]) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        if (type == HBFSIM_KV_BF16) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = y.x;
+            x[2 * i + 1] = y.y;
+        }
+    }
 }
 
 // 2^e in 32 bits, -127 < e < 128.
@@ -173,60 +234,180 @@ __device__ __forceinline__ u32 kv_block_scan(u32 x, u32* warp_sums)
     return x + (warp ? warp_sums[warp - 1] : 0);
 }
 
-// The `rank`-th smallest (from 1) of the keys key(0..n-1) that are not
-// skipped, by 8-bit digits from the top: `histogram` (256 words) counts the
-// digit among the keys that share the prefix found so far.  All threads call
-// it; `below` gets how many keys are smaller than the result.
+// Shared memory of the block-wide selection below.
+constexpr u32 kKvBins = 2048, kKvWords = 1024;
+struct KvSelectShared {
+    u32 histogram[kKvBins];   // also the prefix sums of `words`
+    u32 words[kKvWords];
+    u32 warp_sums[33];
+    u32 found[3];
+    u64 lo, hi;
+};
+constexpr u32 kKvAll = 0xffffffffu;
+
+// Threshold of the `rank` smallest (rank >= 1) among the keys of 0..n-1 that
+// `key_at(i, k)` admits: those below `limit` and `equals` of those at it
+// (kKvAll: all of them).  Each pass spreads the keys of the range at hand
+// over bins and goes on with the bin that holds the rank.  The bins of the
+// first pass grow with the distance from the least key (32 to an octave), so
+// that sizes of many orders do not crowd a few counters; the 2048 of later
+// passes are equal.  Two passes are the rule; 64-bit keys take 7 at most.
+// All threads call it.
+// `least` and `greatest` are this thread's of the keys (~0 and 0 without one).
 template <typename Key, typename KeyAt>
-__device__ Key kv_select_rank(u32 n, u32 rank, KeyAt key_at, u32* histogram, u32* shared2,
-                              u32& below)
+__device__ void kv_rank_limit(u32 n, u32 rank, Key least, Key greatest, KeyAt key_at,
+                              KvSelectShared& sm, Key& limit, u32& equals)
 {
-    constexpr int kBits = sizeof(Key) * 8;
-    Key prefix = 0;
-    u32 left = rank;
-    below = 0;
-    for (int shift = kBits - 8; shift >= 0; shift -= 8) {
-        for (u32 i = threadIdx.x; i < 256; i += blockDim.x) histogram[i] = 0;
+    const u32 lane = threadIdx.x & 31u;
+    if (threadIdx.x == 0) {
+        sm.lo = ~u64{0};
+        sm.hi = 0;
+    }
+    __syncthreads();
+    u64 lo = least, hi = greatest;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (lane == 0) {
+        atomicMin(reinterpret_cast<unsigned long long*>(&sm.lo), lo);
+        atomicMax(reinterpret_cast<unsigned long long*>(&sm.hi), hi);
+    }
+    __syncthreads();
+    lo = sm.lo;
+    hi = sm.hi;
+    bool octaves = true;
+    for (;;) {
+        if (lo >= hi) {  // one value is left
+            limit = static_cast<Key>(lo);
+            equals = rank;
+            return;
+        }
+        const int bits = 64 - __clzll(static_cast<long long>(hi - lo));
+        const int shift = max(0, bits - 11);
+        auto bin_of = [&](u64 d) -> u32 {
+            if (!octaves) return static_cast<u32>(d >> shift);
+            if (d < 32) return static_cast<u32>(d);
+            const int top = 63 - __clzll(static_cast<long long>(d));  // 5 bits below the top one
+            return static_cast<u32>((top - 4) * 32) + (static_cast<u32>(d >> (top - 5)) & 31u);
+        };
+        for (u32 i = threadIdx.x; i < kKvBins; i += blockDim.x) sm.histogram[i] = 0;
         __syncthreads();
+        u32 at_lo = 0;  // keys at `lo` (blocks of no weight, say) would crowd one counter
         for (u32 i = threadIdx.x; i < n; i += blockDim.x) {
             Key k;
-            if (!key_at(i, k)) continue;
-            if (shift + 8 < kBits && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-            atomicAdd(&histogram[static_cast<u32>(k >> shift) & 255u], 1u);
+            if (!key_at(i, k) || k < lo || k > hi) continue;
+            if (k == lo) ++at_lo;
+            else atomicAdd(&sm.histogram[bin_of(k - lo)], 1u);
+        }
+        at_lo = __reduce_add_sync(0xffffffffu, at_lo);
+        if (lane == 0 && at_lo) atomicAdd(&sm.histogram[0], at_lo);
+        __syncthreads();
+        const u32 each = kKvBins / blockDim.x, from = threadIdx.x * each;  // 2 to 8 bins a thread
+        u32 sum = 0;
+        for (u32 t = 0; t < each; ++t) sum += sm.histogram[from + t];
+        u32 upto = kv_block_scan(sum, sm.warp_sums);
+        u32 before = upto - sum;
+        if (before < rank && rank <= upto) {
+            u32 t = from;
+            while (before + sm.histogram[t] < rank) before += sm.histogram[t++];
+            sm.found[0] = t;
+            sm.found[1] = before;
+            sm.found[2] = sm.histogram[t];
         }
         __syncthreads();
-        if (threadIdx.x < 32) {  // one warp walks the 256 counts, 8 per lane
-            u32 c[8], sum = 0;
-#pragma unroll
-            for (u32 t = 0; t < 8; ++t) {
-                c[t] = histogram[threadIdx.x * 8 + t];
-                sum += c[t];
-            }
-            u32 upto = sum;
-#pragma unroll
-            for (u32 o = 1; o < 32; o <<= 1) {
-                const u32 y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (threadIdx.x >= o) upto += y;
-            }
-            u32 before = upto - sum;
-            if (before < left && left <= upto) {
-#pragma unroll
-                for (u32 t = 0; t < 8; ++t) {
-                    if (before < left && left <= before + c[t]) {
-                        shared2[0] = threadIdx.x * 8 + t;
-                        shared2[1] = before;
-                    }
-                    before += c[t];
-                }
-            }
+        const u32 bin = sm.found[0], count = sm.found[2];
+        rank -= sm.found[1];
+        if (octaves && bin >= 32) {
+            const int width = static_cast<int>(bin / 32) - 1;  // log2 of the bin's width
+            lo += static_cast<u64>(32 + bin % 32) << width;
+            hi = min(hi, lo + ((u64{1} << width) - 1));
+        } else {
+            const int width = octaves ? 0 : shift;
+            lo += static_cast<u64>(bin) << width;
+            hi = min(hi, lo + ((u64{1} << width) - 1));
         }
-        __syncthreads();
-        prefix |= static_cast<Key>(shared2[0]) << shift;
-        left -= shared2[1];
-        below += shared2[1];
-        __syncthreads();
+        octaves = false;
+        if (rank == count) {  // the whole bin
+            limit = static_cast<Key>(hi);
+            equals = kKvAll;
+            return;
+        }
+        __syncthreads();  // `found` and the bins are read
     }
-    return prefix;
+}
+
+// Walks 0..n-1 in order: state(i) is 0 (not chosen), 1 (chosen) or 2 (one of
+// the equals, of which the first `equals` are chosen).  For every i,
+// value = load(i), then store(i, value, chosen, how many chosen came before),
+// with a block barrier between them if kBarrier (stores may reach what a load
+// of the same round reads).  Counts come from ballots, one word per 32
+// elements, and one block-wide scan per 32768 elements.
+template <bool kBarrier, typename State, typename Load, typename Store>
+__device__ void kv_walk(u32 n, u32 equals, KvSelectShared& sm, State state, Load load, Store store)
+{
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const u32 under = (1u << lane) - 1u;
+    u32* prefix = sm.histogram;
+    u32 chosen_before = 0, equal_before = 0;
+    // exclusive prefix sums of the words' bit counts; returns their sum
+    auto scan_words = [&](u32 many) {
+        u32 carry = 0;
+        for (u32 base = 0; base < many; base += blockDim.x) {
+            const u32 w = base + threadIdx.x;
+            const u32 bits = w < many ? __popc(sm.words[w]) : 0;
+            const u32 upto = kv_block_scan(bits, sm.warp_sums);
+            if (w < many) prefix[w] = carry + upto - bits;
+            carry += sm.warp_sums[32];
+        }
+        __syncthreads();
+        return carry;
+    };
+    for (u32 first = 0; first < n; first += kKvWords * 32) {
+        const u32 many = min(n - first, kKvWords * 32), words = (many + 31) / 32;
+        const u32 rounds = (words + warps - 1) / warps;
+        __syncthreads();
+        if (equals != kKvAll) {
+            for (u32 r = 0; r < rounds; ++r) {
+                const u32 w = r * warps + warp, i = w * 32 + lane;
+                const u32 m = __ballot_sync(0xffffffffu, i < many && state(first + i) == 2);
+                if (lane == 0 && w < words) sm.words[w] = m;
+            }
+            __syncthreads();
+            const u32 all = scan_words(words);
+            // from here on the words hold what is chosen; a warp reads and writes its own words
+            for (u32 r = 0; r < rounds; ++r) {
+                const u32 w = r * warps + warp, i = w * 32 + lane;
+                const u32 eq = w < words ? sm.words[w] : 0;
+                const bool one = i < many && state(first + i) == 1;
+                const bool rank_ok = w < words && equal_before + prefix[w] + __popc(eq & under) < equals;
+                const u32 m = __ballot_sync(0xffffffffu, one || ((eq >> lane & 1u) && rank_ok));
+                __syncwarp();
+                if (lane == 0 && w < words) sm.words[w] = m;
+            }
+            equal_before += all;
+        } else {
+            for (u32 r = 0; r < rounds; ++r) {
+                const u32 w = r * warps + warp, i = w * 32 + lane;
+                const u32 m = __ballot_sync(0xffffffffu, i < many && state(first + i) != 0);
+                if (lane == 0 && w < words) sm.words[w] = m;
+            }
+        }
+        __syncthreads();
+        const u32 all = scan_words(words);
+        for (u32 r = 0; r < rounds; ++r) {
+            const u32 w = r * warps + warp, i = w * 32 + lane;
+            const bool in = i < many;
+            auto value = load(first + (in ? i : 0));
+            if constexpr (kBarrier) __syncthreads();
+            if (in) {
+                const u32 m = sm.words[w];
+                store(first + i, value, (m >> lane & 1u) != 0, chosen_before + prefix[w] + __popc(m & under));
+            }
+        }
+        chosen_before += all;
+    }
 }
 
 #endif  // __CUDACC__

@@ -30,9 +30,6 @@
 // logarithmic sums into block weights.
 #include "kv.h"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -96,12 +93,6 @@ __device__ __forceinline__ u32 pack_f16(float lo, float hi)
 {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const u32*>(&h);
-}
-
-__device__ __forceinline__ float load_elem(const void* p, i64 i, u32 type)
-{
-    return type == HBFSIM_KV_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
-                                  : __half2float(static_cast<const __half*>(p)[i]);
 }
 
 __device__ __forceinline__ float exp2_fast(float x)  // 2^-22 relative, 0 for -inf
@@ -337,12 +328,12 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                            static_cast<i64>(t) * a.q.stride_token +
                            static_cast<i64>(qh) * a.q.stride_head;
 #pragma unroll
-            for (int k = 0; k < KC; ++k)
+            for (int k = 0; k < KC; ++k) {
+                kv_load<16>(a.q.q, at + (c * KC + k) * 16, a.q.type, a.q.wide, x[k]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[k][i] = load_elem(a.q.q, at + (c * KC + k) * 16 + i, a.q.type);
+                for (int i = 0; i < 16; ++i)
                     if (fabsf(x[k][i]) <= 3.402823466e38f) most = fmaxf(most, fabsf(x[k][i]));
-                }
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < KC; ++k)
@@ -798,21 +789,6 @@ struct Plan {
     u64 segments, part_o, part_ml, span, tile_lse, bytes;
 };
 
-int sm_count()
-{
-    static int counts[64];  // by device; the value does not change
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess) return 148;
-    if (device >= 64) device = 63;
-    if (counts[device] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0)
-            n = 148;
-        counts[device] = n;
-    }
-    return counts[device];
-}
-
 Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weights)
 {
     Plan p{};
@@ -828,7 +804,7 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     // as many CTAs as are resident at once, fewer for little work
     const u64 most = (p.segments * p.tiles + kShare - 1) / kShare;
     p.workers = static_cast<u32>(
-        std::max<u64>(1, std::min<u64>(most, static_cast<u64>(per_sm(v.dim, p.nt)) * sm_count())));
+        std::max<u64>(1, std::min<u64>(most, static_cast<u64>(per_sm(v.dim, p.nt)) * kv_sm_count())));
     u64 at = 0;
     auto take = [&](u64 bytes) {
         const u64 here = at;
@@ -866,9 +842,9 @@ int launch(const AttentionArgs& a, cudaStream_t s)
     u32 across = segments;
     if (a.weights)
         across = std::max(across, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
-                                           4u * sm_count() / pairs));
+                                           4u * kv_sm_count() / pairs));
     const u32 slices = std::min(std::max(1u, across / segments), 8u);
-    const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, a,
+    const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, 0, a,
                                      static_cast<u32>(8 * NT), slices);
     return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }

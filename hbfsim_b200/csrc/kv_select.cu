@@ -2,25 +2,31 @@
 //
 // A group's score of a block is linear in the block's bounds once the
 // queries are split by sign: sum_d up_d * hi_d + down_d * lo_d with
-// up = sum_g max(qi, 0), down = sum_g min(qi, 0).  So a block costs two dot
-// products of 16-bit by 8-bit whole numbers (dp2a) per group instead of one
-// pass per query head, and 2 * head_dim bytes, 1/16 of its keys and values
-// at 16 tokens a block.
+// up = sum_g max(qi, 0), down = sum_g min(qi, 0).  So a block costs one dot
+// product of 2 * head_dim channels per group instead of one per query head,
+// and 2 * head_dim bytes, 1/16 of its keys and values at 16 tokens a block.
+// The sums go through the tensor cores as 8-bit whole numbers: up and down
+// (at most 64 * 127) are split into 128 * high + low, two columns of the
+// narrow side; 16 blocks of a head are the wide side, read straight into the
+// fragments, 16 bytes per lane.  (Two-way dot instructions took 4 times the
+// instructions and were bound by them.)
 //
 // score_kernel streams the bounds and writes a 32-bit ordered key per
-// (token, head, block); list_kernel, one CTA per (sequence, token, head),
-// finds the key of the last block to list by radix selection and writes the
-// list in block order.
+// (token, head, block): the blocks of all sequences form one line that is cut
+// into equal shares, one per resident CTA.  list_kernel, one CTA per
+// (sequence, token, head), finds the key of the last block to list by a
+// selection on the keys (in shared memory up to kHeldKeys blocks) and writes
+// the list in block order.
 #include "kv.h"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include <algorithm>
 
 namespace hbfb {
 namespace {
 
-constexpr u32 kScoreThreads = 256, kScoreBlocks = 64;  // blocks per CTA
-constexpr u32 kListThreads = 256;
+constexpr u32 kScoreThreads = 256, kScorePerSm = 3;
+constexpr u32 kScoreShare = 32;      // blocks of a CTA at least
+constexpr u32 kHeldKeys = 32 * 1024; // 128 KB of keys
 constexpr u32 kMostQueryBytes = 200 * 1024;  // of shared memory, for the whole-number queries
 constexpr u32 kAbsent = 0u;           // key of a block that cannot be listed
 constexpr u32 kAlways = 0xffffffffu;  // key of a block that is always listed
@@ -34,14 +40,16 @@ struct SelectArgs {
     int* counts;
 };
 
-__device__ __forceinline__ float query_at(const KvQuery& q, u32 seq, u32 token, u32 head, u32 d)
+// E neighbouring channels of a query, those that are not finite as 0.
+template <int E>
+__device__ __forceinline__ void query_at(const KvQuery& q, u32 seq, u32 token, u32 head, u32 d,
+                                         float (&x)[E])
 {
     const i64 at = static_cast<i64>(seq) * q.stride_seq + static_cast<i64>(token) * q.stride_token +
                    static_cast<i64>(head) * q.stride_head + d;
-    const float x = q.type == HBFSIM_KV_BF16
-                        ? __bfloat162float(static_cast<const __nv_bfloat16*>(q.q)[at])
-                        : __half2float(static_cast<const __half*>(q.q)[at]);
-    return fabsf(x) <= 3.402823466e38f ? x : 0.0f;  // not finite: 0
+    kv_load<E>(q.q, at, q.type, q.wide, x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = fabsf(x[e]) <= 3.402823466e38f ? x[e] : 0.0f;
 }
 
 // Blocks that a query token may look at: those up to its own position.
@@ -58,147 +66,244 @@ __device__ __forceinline__ u32 order_key(float x)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectArgs a)
+__device__ __forceinline__ u32 blocks_of_sequence(const SelectArgs& a, u32 seq)
 {
-    constexpr u32 L = D / 16;   // lanes per (block, head): 16 channels each
-    extern __shared__ __align__(16) short whole[];  // [tokens][heads][2][D]: up, down
+    return blocks_of_token(kv_length(a.q.lengths, seq, a.q.width, a.c.block), a.q.tokens,
+                           a.q.tokens - 1, a.c.block);
+}
+
+// Bytes between the columns (token, high or low) of a head's whole-number
+// queries in shared memory: down then up, and padding that puts neighbouring
+// columns on different banks.
+HD constexpr u32 column_bytes(u32 dim) { return 2 * dim + 64; }
+
+__device__ __forceinline__ void mma16832(int (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int D>
+__global__ void __launch_bounds__(kScoreThreads, kScorePerSm) score_kernel(const SelectArgs a)
+{
+    constexpr u32 kChunks = D / 32;  // 16-byte pieces of a block's bounds per lane
+    constexpr u32 kColumn = column_bytes(D);
+    extern __shared__ __align__(16) std::int8_t whole[];  // [heads][2 tokens][kColumn]
+    __shared__ u64 line;
     kv_let_next();
-    const u32 seq = blockIdx.y, heads = a.c.heads, tokens = a.q.tokens, group = a.q.group;
-    const int length = kv_length(a.q.lengths, seq, a.q.width, a.c.block);
-    const u32 have = blocks_of_token(length, tokens, tokens - 1, a.c.block);
-    const u32 first = blockIdx.x * kScoreBlocks;
-    if (first >= have) return;
-    const u32 many = min(kScoreBlocks, have - first);
-    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    for (u32 th = warp; th < tokens * heads; th += warps) {
-        const u32 t = th / heads, h = th % heads;
-        float most = 0.0f;
-        for (u32 i = lane; i < group * D; i += 32)
-            most = fmaxf(most, fabsf(query_at(a.q, seq, t, h * group + i / D, i % D)));
+    const u32 heads = a.c.heads, tokens = a.q.tokens, group = a.q.group;
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = kScoreThreads / 32;
+    // the line of all sequences' blocks, and this CTA's share of it
+    u64 all = 0;
+    for (u32 s = threadIdx.x; s < a.q.seqs; s += kScoreThreads) all += blocks_of_sequence(a, s);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        int x = 0;
-        frexpf(most, &x);
-        const float up_scale = kv_power(7 - max(x, -100));
-        for (u32 d = lane; d < D; d += 32) {
-            int up = 0, down = 0;
-            for (u32 g = 0; g < group; ++g) {
-                const float r = rintf(query_at(a.q, seq, t, h * group + g, d) * up_scale);
-                const int qi = static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
-                up += max(qi, 0);
-                down += min(qi, 0);
-            }
-            whole[(th * 2) * D + d] = static_cast<short>(up);
-            whole[(th * 2 + 1) * D + d] = static_cast<short>(down);
-        }
-    }
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (threadIdx.x == 0) line = 0;
     __syncthreads();
-    const int* table = a.q.table + static_cast<i64>(seq) * a.q.table_stride;
-    const u32 part = threadIdx.x % L;
-    const u32 items = many * heads;
-    // every lane of a warp takes the same number of turns (the sums below shuffle)
-    for (u32 base = warp * (32 / L); base < items; base += warps * (32 / L)) {
-        const u32 item = base + lane / L;
-        const bool in = item < items;
-        const u32 j = first + (in ? item / heads : 0), h = in ? item % heads : 0;
-        const int page = in ? kv_page(table, j, a.c.pages) : -1;
-        uint4 lo{}, hi{};
-        float scale = 0.0f;
-        if (page >= 0) {
-            const u64 at = static_cast<u64>(page) * heads + h;
-            const uint4* b = reinterpret_cast<const uint4*>(a.c.bounds + at * 2 * D);
-            lo = b[part];
-            hi = b[L + part];
-            scale = a.c.scale[at * 2];
-        }
-        for (u32 t = 0; t < tokens; ++t) {
-            const int4* w = reinterpret_cast<const int4*>(whole + ((t * heads + h) * 2) * D + part * 16);
-            const int4 u0 = w[0], u1 = w[1], n0 = w[D / 8], n1 = w[D / 8 + 1];
-            int sum = 0;
-            sum = __dp2a_lo(u0.x, static_cast<int>(hi.x), sum);
-            sum = __dp2a_hi(u0.y, static_cast<int>(hi.x), sum);
-            sum = __dp2a_lo(u0.z, static_cast<int>(hi.y), sum);
-            sum = __dp2a_hi(u0.w, static_cast<int>(hi.y), sum);
-            sum = __dp2a_lo(u1.x, static_cast<int>(hi.z), sum);
-            sum = __dp2a_hi(u1.y, static_cast<int>(hi.z), sum);
-            sum = __dp2a_lo(u1.z, static_cast<int>(hi.w), sum);
-            sum = __dp2a_hi(u1.w, static_cast<int>(hi.w), sum);
-            sum = __dp2a_lo(n0.x, static_cast<int>(lo.x), sum);
-            sum = __dp2a_hi(n0.y, static_cast<int>(lo.x), sum);
-            sum = __dp2a_lo(n0.z, static_cast<int>(lo.y), sum);
-            sum = __dp2a_hi(n0.w, static_cast<int>(lo.y), sum);
-            sum = __dp2a_lo(n1.x, static_cast<int>(lo.z), sum);
-            sum = __dp2a_hi(n1.y, static_cast<int>(lo.z), sum);
-            sum = __dp2a_lo(n1.z, static_cast<int>(lo.w), sum);
-            sum = __dp2a_hi(n1.w, static_cast<int>(lo.w), sum);
+    if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&line), all);
+    __syncthreads();
+    const u64 share = max(static_cast<u64>(kScoreShare), (line + gridDim.x - 1) / gridDim.x);
+    u64 at = blockIdx.x * share;
+    const u64 stop = min(at + share, line);
+    if (at >= stop) return;
+    u32 seq = 0, have = 0;
+    u64 begin = 0;
+    for (u32 base = 0; base < a.q.seqs; base += 32) {  // the sequence that holds `at`
+        const u32 n = base + lane < a.q.seqs ? blocks_of_sequence(a, base + lane) : 0;
+        u32 upto = n;
 #pragma unroll
-            for (u32 o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (in && part == 0) {
-                const u32 mine = blocks_of_token(length, tokens, t, a.c.block);
-                u32 key = kAbsent;
-                if (page >= 0 && j < mine) {
-                    key = j < a.sink || j + a.recent >= mine
-                              ? kAlways
-                              : order_key(__fmul_rn(__int2float_rn(sum), scale));
+        for (u32 o = 1; o < 32; o <<= 1) {
+            const u32 y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const u32 holds = __ballot_sync(0xffffffffu, at < begin + upto);
+        if (holds) {
+            const int k = __ffs(holds) - 1;
+            seq = base + k;
+            have = __shfl_sync(0xffffffffu, n, k);
+            begin += __shfl_sync(0xffffffffu, upto - n, k);
+            break;
+        }
+        begin += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    for (; at < stop; begin += have, have = ++seq < a.q.seqs ? blocks_of_sequence(a, seq) : 0) {
+        const u32 first = static_cast<u32>(at - begin);
+        const u32 end = static_cast<u32>(min(stop - begin, static_cast<u64>(have)));
+        if (first >= end) continue;
+        at = begin + end;
+        const int length = kv_length(a.q.lengths, seq, a.q.width, a.c.block);
+        __syncthreads();  // the queries of the sequence before are used
+        for (u32 th = warp; th < tokens * heads; th += warps) {
+            const u32 t = th / heads, h = th % heads;
+            constexpr int E = D / 32;  // channels of a lane
+            float most = 0.0f;
+#pragma unroll 4
+            for (u32 i = 0; i < group; ++i) {
+                float x[E];
+                query_at<E>(a.q, seq, t, h * group + i, lane * E, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) most = fmaxf(most, fabsf(x[e]));
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            int x = 0;
+            frexpf(most, &x);
+            const float up_scale = kv_power(7 - max(x, -100));
+            int up[E], down[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) up[e] = down[e] = 0;
+#pragma unroll 4
+            for (u32 i = 0; i < group; ++i) {
+                float x[E];
+                query_at<E>(a.q, seq, t, h * group + i, lane * E, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float r = rintf(x[e] * up_scale);
+                    const int qi = static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
+                    up[e] += max(qi, 0);
+                    down[e] += min(qi, 0);
                 }
-                a.keys[((static_cast<u64>(seq) * tokens + t) * heads + h) * a.q.width + j] = key;
+            }
+            // column 2 t: the high parts, 2 t + 1: the low ones; first down, then up
+            std::int8_t* to = whole + (h * 2 * tokens + 2 * t) * kColumn + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                to[e] = static_cast<std::int8_t>(-(-down[e] >> 7));
+                to[kColumn + e] = static_cast<std::int8_t>(-(-down[e] & 127));
+                to[D + e] = static_cast<std::int8_t>(up[e] >> 7);
+                to[D + kColumn + e] = static_cast<std::int8_t>(up[e] & 127);
+            }
+        }
+        __syncthreads();
+        const int* table = a.q.table + static_cast<i64>(seq) * a.q.table_stride;
+        const u32 g = lane >> 2, c = lane & 3u;
+        const u32 tasks = (end - first + 15) / 16 * heads;  // 16 blocks of one head
+        auto page_of = [&](u32 task, u32 more) {
+            const u32 j = first + task / heads * 16 + g + more;
+            return task < tasks && j < end ? kv_page(table, j, a.c.pages) : -1;
+        };
+        int next0 = page_of(warp, 0), next1 = page_of(warp, 8);
+        for (u32 task = warp; task < tasks; task += warps) {
+            const u32 h = task % heads, j0 = first + task / heads * 16 + g, j1 = j0 + 8;
+            const int page0 = next0, page1 = next1;
+            uint4 x0[kChunks], x1[kChunks];
+            float scale0 = 0.0f, scale1 = 0.0f;
+#pragma unroll
+            for (u32 k = 0; k < kChunks; ++k) x0[k] = x1[k] = make_uint4(0, 0, 0, 0);
+            if (page0 >= 0) {
+                const u64 x = static_cast<u64>(page0) * heads + h;
+                const uint4* b = reinterpret_cast<const uint4*>(a.c.bounds + x * 2 * D) + c;
+#pragma unroll
+                for (u32 k = 0; k < kChunks; ++k) x0[k] = b[k * 4];
+                scale0 = a.c.scale[x * 2];
+            }
+            if (page1 >= 0) {
+                const u64 x = static_cast<u64>(page1) * heads + h;
+                const uint4* b = reinterpret_cast<const uint4*>(a.c.bounds + x * 2 * D) + c;
+#pragma unroll
+                for (u32 k = 0; k < kChunks; ++k) x1[k] = b[k * 4];
+                scale1 = a.c.scale[x * 2];
+            }
+            next0 = page_of(task + warps, 0);
+            next1 = page_of(task + warps, 8);
+            // four tokens at a time: column g is the high or low part of token t0 + g / 2
+            for (u32 t0 = 0; t0 < tokens; t0 += 4) {
+                int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
+                const bool used = t0 + g / 2 < tokens;
+                const std::int8_t* column = whole + (h * 2 * tokens + 2 * t0 + g) * kColumn + c * 16;
+#pragma unroll
+                for (u32 k = 0; k < kChunks; ++k) {
+                    uint4 y = make_uint4(0, 0, 0, 0);
+                    if (used) y = *reinterpret_cast<const uint4*>(column + k * 64);
+                    mma16832(s0, x0[k].x, x1[k].x, x0[k].y, x1[k].y, y.x, y.y);
+                    mma16832(s1, x0[k].z, x1[k].z, x0[k].w, x1[k].w, y.z, y.w);
+                }
+                const u32 t = t0 + c;  // this lane's columns 2c and 2c + 1
+                if (t < tokens) {
+                    const u32 mine = blocks_of_token(length, tokens, t, a.c.block);
+                    u32* keys = a.keys + ((static_cast<u64>(seq) * tokens + t) * heads + h) * a.q.width;
+                    auto put = [&](u32 j, int page, int sum, float scale) {
+                        u32 key = kAbsent;
+                        if (page >= 0 && j < mine)
+                            key = j < a.sink || j + a.recent >= mine
+                                      ? kAlways
+                                      : order_key(__fmul_rn(__int2float_rn(sum), scale));
+                        if (j < end) keys[j] = key;
+                    };
+                    put(j0, page0, (s0[0] + s1[0]) * 128 + s0[1] + s1[1], scale0);
+                    put(j1, page1, (s0[2] + s1[2]) * 128 + s0[3] + s1[3], scale1);
+                }
             }
         }
     }
 }
 
-__global__ void __launch_bounds__(kListThreads) list_kernel(const SelectArgs a)
+__global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a)
 {
-    __shared__ u32 histogram[256];
-    __shared__ u32 shared2[2];
-    __shared__ u32 warp_sums[33];
+    extern __shared__ __align__(16) u32 held[];
+    __shared__ KvSelectShared sm;
+    __shared__ u32 counted[2];  // blocks that are there, and those always listed
     kv_wait_before();
     const u64 at = blockIdx.x;  // (sequence, token, head)
     const u32 heads = a.c.heads, tokens = a.q.tokens;
     const u32 t = static_cast<u32>(at / heads % tokens), seq = static_cast<u32>(at / heads / tokens);
     const int length = kv_length(a.q.lengths, seq, a.q.width, a.c.block);
     const u32 have = blocks_of_token(length, tokens, t, a.c.block);
-    const u32* keys = a.keys + at * a.q.width;
+    const u32* row = a.keys + at * a.q.width;
+    const bool hold = a.q.width <= kHeldKeys;
+    const u32* keys = hold ? held : row;
     int* list = a.blocks + at * a.top;
-    // blocks that are there
-    u32 mine = 0;
-    for (u32 j = threadIdx.x; j < have; j += blockDim.x) mine += keys[j] != kAbsent;
-    kv_block_scan(mine, warp_sums);
-    const u32 present = warp_sums[32];
-    const u32 take = min(a.top, present);
-    // the greatest keys are the smallest of their complements
-    u32 limit = 0xffffffffu, equals = 0;
+    if (threadIdx.x < 2) counted[threadIdx.x] = 0;
     __syncthreads();
-    if (take < present && take) {
-        u32 below;
-        limit = kv_select_rank<u32>(
-            have, take,
+    u32 there = 0, always = 0, least = ~0u, greatest = 0;
+#pragma unroll 8
+    for (u32 j = threadIdx.x; j < have; j += blockDim.x) {
+        const u32 k = row[j];
+        if (hold) held[j] = k;
+        there += k != kAbsent;
+        always += k == kAlways;
+        if (k != kAbsent && k != kAlways) {
+            least = min(least, ~k);
+            greatest = max(greatest, ~k);
+        }
+    }
+    there = __reduce_add_sync(0xffffffffu, there);
+    always = __reduce_add_sync(0xffffffffu, always);
+    if ((threadIdx.x & 31u) == 0) {
+        atomicAdd(&counted[0], there);
+        atomicAdd(&counted[1], always);
+    }
+    __syncthreads();
+    there = counted[0];
+    always = counted[1];
+    const u32 take = min(a.top, there);
+    // the greatest keys are the smallest of their complements; those always listed need no rank
+    u32 limit = 0xffffffffu, equals = kKvAll;
+    if (take < there && take > always)
+        kv_rank_limit<u32>(
+            have, take - always, least, greatest,
             [&](u32 j, u32& k) {
                 k = keys[j];
-                if (k == kAbsent) return false;
+                if (k == kAbsent || k == kAlways) return false;
                 k = ~k;
                 return true;
             },
-            histogram, shared2, below);
-        equals = take - below;
-    }
-    u32 listed_before = 0, equal_before = 0;
-    for (u32 base = 0; base < have; base += blockDim.x) {
-        const u32 j = base + threadIdx.x;
-        const u32 key = j < have ? keys[j] : kAbsent;
-        const bool in = key != kAbsent;
-        bool listed = in;
-        if (take < present) {
-            const u32 equal = in && ~key == limit ? 1u : 0u;
-            const u32 upto = equal_before + kv_block_scan(equal, warp_sums);
-            equal_before += warp_sums[32];
-            listed = in && (~key < limit || (equal && upto <= equals));
-        }
-        const u32 upto = listed_before + kv_block_scan(listed ? 1u : 0u, warp_sums);
-        listed_before += warp_sums[32];
-        if (listed && upto <= a.top) list[upto - 1] = static_cast<int>(j);
-    }
+            sm, limit, equals);
+    else if (take < there)
+        limit = 0, equals = 0;  // none but those always listed
+    kv_walk<false>(
+        have, equals, sm,
+        [&](u32 j) -> u32 {
+            const u32 k = keys[j];
+            if (k == kAbsent) return 0;
+            return k == kAlways || ~k < limit ? 1 : ~k == limit ? 2 : 0;
+        },
+        [](u32) { return 0; },
+        [&](u32 j, int, bool listed, u32 before) {
+            if (listed && before < a.top) list[before] = static_cast<int>(j);
+        });
     for (u32 i = take + threadIdx.x; i < a.top; i += blockDim.x) list[i] = -1;
     if (threadIdx.x == 0) a.counts[at] = static_cast<int>(take);
 }
@@ -211,13 +316,18 @@ u64 workspace_bytes_of(const KvView& v, const KvQuery& q)
 template <int D>
 int launch(const SelectArgs& a, cudaStream_t s)
 {
-    const u32 smem = a.q.tokens * a.c.heads * 2 * D * static_cast<u32>(sizeof(short));
+    const u32 smem = a.q.tokens * a.c.heads * 2 * column_bytes(D);
     static std::atomic<u64> seen{0};
     if (!kv_allow_smem(score_kernel<D>, kMostQueryBytes, seen)) return HBFSIM_CUDA_ERROR;
-    const dim3 grid((a.q.width + kScoreBlocks - 1) / kScoreBlocks, a.q.seqs);
-    if (a.q.width) score_kernel<D><<<grid, kScoreThreads, smem, s>>>(a);
-    const bool ok = kv_launch_behind(list_kernel, dim3(a.q.seqs * a.q.tokens * a.c.heads),
-                                     kListThreads, s, a);
+    const u64 most = (static_cast<u64>(a.q.seqs) * a.q.width + kScoreShare - 1) / kScoreShare;
+    const u32 grid = static_cast<u32>(std::min<u64>(most, static_cast<u64>(kScorePerSm) * kv_sm_count()));
+    if (grid) score_kernel<D><<<grid, kScoreThreads, smem, s>>>(a);
+    // a long row is one CTA's: more threads for it
+    static std::atomic<u64> seen_list{0};
+    if (!kv_allow_smem(list_kernel, kHeldKeys * 4, seen_list)) return HBFSIM_CUDA_ERROR;
+    const u32 threads = a.q.width <= 512 ? 128 : a.q.width <= 4096 ? 256 : 1024;
+    const bool ok = kv_launch_behind(list_kernel, dim3(a.q.seqs * a.q.tokens * a.c.heads), threads, s,
+                                     a.q.width <= kHeldKeys ? a.q.width * 4 : 0, a);
     return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
@@ -249,9 +359,9 @@ extern "C" int hbfsim_kv_select_v1(const hbfsim_kv_cache_v1* cache,
     const u64 lists = static_cast<u64>(a.q.seqs) * a.q.tokens * a.c.heads;
     if (lists == 0) return HBFSIM_OK;
     // shared memory of the whole-number queries
-    if (static_cast<u64>(a.q.tokens) * a.c.heads * a.c.dim * 4 > kMostQueryBytes)
+    if (static_cast<u64>(a.q.tokens) * a.c.heads * 2 * column_bytes(a.c.dim) > kMostQueryBytes)
         return HBFSIM_UNSUPPORTED;
-    if (a.q.seqs > 65535 || !blocks || !counts) return HBFSIM_INVALID_ARGUMENT;
+    if (!blocks || !counts) return HBFSIM_INVALID_ARGUMENT;
     if (workspace_bytes < workspace_bytes_of(a.c, a.q) || (a.q.width && !workspace) ||
         !kv_aligned(workspace, 16) || !kv_aligned(blocks, 4) || !kv_aligned(counts, 4))
         return HBFSIM_INVALID_ARGUMENT;
