@@ -20,6 +20,7 @@ constexpr u32 kKvMaxGroup = 64;       // query heads per key/value head
 constexpr u32 kKvMaxWidth = 1u << 24; // blocks per sequence
 constexpr u32 kKvMaxSeqs = 1u << 16;
 constexpr u32 kKvMaxHeads = 1u << 10;
+constexpr u32 kKvTeam = 8;            // CTAs that select from one row at most
 
 struct KvView {
     u8* data;
@@ -91,6 +92,20 @@ inline int kv_check_query(const hbfsim_kv_query_v1* q, const KvView& v, KvQuery&
     return HBFSIM_OK;
 }
 
+inline int kv_sm_count()
+{
+    static std::atomic<int> counts[64];  // by device; the value does not change
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device > 63) return 148;
+    int n = counts[device].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0)
+            n = 148;
+        counts[device].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 #if defined(__CUDACC__)
 // Dynamic shared memory beyond 48 KB has to be allowed once per kernel and
 // device; `seen` (one per kernel) remembers the devices.
@@ -108,43 +123,51 @@ inline bool kv_allow_smem(Kernel* kernel, u32 bytes, std::atomic<u64>& seen)
     return true;
 }
 
+// CTAs to a row of `width` keys: a power of two up to kKvTeam, as long as
+// every CTA gets an SM of its own and at least 1024 keys.
+inline u32 kv_team_size(u64 rows, u32 width)
+{
+    u32 size = 1;
+    while (size < kKvTeam && rows * size * 2 <= static_cast<u64>(kv_sm_count()) &&
+           width / (size * 2) >= 1024)
+        size *= 2;
+    return size;
+}
+
+// Threads for a slice of a row: two keys each or more, a power of two (the
+// bins are shared out evenly).
+inline u32 kv_team_threads(u32 slice)
+{
+    return slice <= 256 ? 128 : slice <= 512 ? 256 : slice <= 1024 ? 512 : 1024;
+}
+
 // Launches a kernel that may be set up while the kernel before it on the
 // stream still runs (programmatic dependent launch): it has to begin with
 // kv_wait_before, which returns once that kernel's writes are visible.
 template <typename... Params, typename... Args>
 inline bool kv_launch_behind(void (*kernel)(Params...), dim3 grid, u32 threads, cudaStream_t stream,
-                             u32 smem, Args... args)
+                             u32 smem, u32 cluster, Args... args)
 {
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = grid;
     config.blockDim = dim3(threads);
     config.stream = stream;
     config.dynamicSmemBytes = smem;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess;
 }
 
 __device__ __forceinline__ void kv_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void kv_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 #endif
-
-inline int kv_sm_count()
-{
-    static std::atomic<int> counts[64];  // by device; the value does not change
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || device > 63) return 148;
-    int n = counts[device].load(std::memory_order_relaxed);
-    if (n == 0) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0)
-            n = 148;
-        counts[device].store(n, std::memory_order_relaxed);
-    }
-    return n;
-}
 
 inline u64 kv_round_up(u64 n, u64 to) { return (n + to - 1) / to * to; }
 
@@ -234,29 +257,66 @@ __device__ __forceinline__ u32 kv_block_scan(u32 x, u32* warp_sums)
     return x + (warp ? warp_sums[warp - 1] : 0);
 }
 
-// Shared memory of the block-wide selection below.
+// Selection over a row of keys by a team: one CTA, or a cluster of up to 8,
+// each with a slice of the row, that count together through distributed
+// shared memory (a row of 16,000 keys is bound by one SM's instructions).
 constexpr u32 kKvBins = 2048, kKvWords = 1024;
 struct KvSelectShared {
-    u32 histogram[kKvBins];   // also the prefix sums of `words`
+    u32 histogram[kKvBins];   // this CTA's counts; also the prefix sums of `words`
+    u32 total[kKvBins];       // the team's
     u32 words[kKvWords];
     u32 warp_sums[33];
     u32 found[3];
+    u32 counts[2];
     u64 lo, hi;
 };
 constexpr u32 kKvAll = 0xffffffffu;
 
-// Threshold of the `rank` smallest (rank >= 1) among the keys of 0..n-1 that
-// `key_at(i, k)` admits: those below `limit` and `equals` of those at it
-// (kKvAll: all of them).  Each pass spreads the keys of the range at hand
-// over bins and goes on with the bin that holds the rank.  The bins of the
-// first pass grow with the distance from the least key (32 to an octave), so
-// that sizes of many orders do not crowd a few counters; the 2048 of later
-// passes are equal.  Two passes are the rule; 64-bit keys take 7 at most.
-// All threads call it.
-// `least` and `greatest` are this thread's of the keys (~0 and 0 without one).
+struct KvTeam {
+    u32 rank, size;
+};
+
+__device__ __forceinline__ void kv_team_sync(const KvTeam& team)
+{
+    if (team.size == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
+
+// A word of the shared memory of another CTA of the team.
+template <typename T>
+__device__ __forceinline__ T kv_peek(const T* mine, u32 rank)
+{
+    u32 at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;"
+        : "=r"(at)
+        : "r"(static_cast<u32>(__cvta_generic_to_shared(mine))), "r"(rank));
+    T x;
+    if constexpr (sizeof(T) == 8)
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(at) : "memory");
+    else
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+    return x;
+}
+
+__device__ __forceinline__ int kv_top_bit(u32 x) { return 31 - __clz(static_cast<int>(x)); }
+__device__ __forceinline__ int kv_top_bit(u64 x) { return 63 - __clzll(static_cast<long long>(x)); }
+
+// Threshold of the `rank` smallest (rank >= 1) among the keys of the team
+// that `key_at(i, k)` admits, i = 0..n-1 in each CTA: those below `limit` and
+// `equals` of those at it (kKvAll: all of them).  Each pass spreads the keys
+// of the range at hand over bins and goes on with the bin that holds the
+// rank.  The bins of the first pass grow with the distance from the least
+// key (32 to an octave), so that sizes of many orders do not crowd a few
+// counters; the 2048 of later passes are equal.  Two passes are the rule;
+// 64-bit keys take 7 at most.  `least` and `greatest` are this thread's of
+// the keys (~0 and 0 without one).  All threads of the team call it.
 template <typename Key, typename KeyAt>
-__device__ void kv_rank_limit(u32 n, u32 rank, Key least, Key greatest, KeyAt key_at,
-                              KvSelectShared& sm, Key& limit, u32& equals)
+__device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Key greatest,
+                              KeyAt key_at, KvSelectShared& sm, Key& limit, u32& equals)
 {
     const u32 lane = threadIdx.x & 31u;
     if (threadIdx.x == 0) {
@@ -264,32 +324,36 @@ __device__ void kv_rank_limit(u32 n, u32 rank, Key least, Key greatest, KeyAt ke
         sm.hi = 0;
     }
     __syncthreads();
-    u64 lo = least, hi = greatest;
+    Key lo = least, hi = greatest;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     if (lane == 0) {
-        atomicMin(reinterpret_cast<unsigned long long*>(&sm.lo), lo);
-        atomicMax(reinterpret_cast<unsigned long long*>(&sm.hi), hi);
+        atomicMin(reinterpret_cast<unsigned long long*>(&sm.lo), static_cast<u64>(lo));
+        atomicMax(reinterpret_cast<unsigned long long*>(&sm.hi), static_cast<u64>(hi));
     }
-    __syncthreads();
-    lo = sm.lo;
-    hi = sm.hi;
+    kv_team_sync(team);
+    lo = static_cast<Key>(sm.lo);
+    hi = static_cast<Key>(sm.hi);
+    for (u32 r = 0; r < team.size; ++r)
+        if (r != team.rank) {
+            lo = min(lo, static_cast<Key>(kv_peek(&sm.lo, r)));
+            hi = max(hi, static_cast<Key>(kv_peek(&sm.hi, r)));
+        }
     bool octaves = true;
     for (;;) {
         if (lo >= hi) {  // one value is left
-            limit = static_cast<Key>(lo);
+            limit = lo;
             equals = rank;
             return;
         }
-        const int bits = 64 - __clzll(static_cast<long long>(hi - lo));
-        const int shift = max(0, bits - 11);
-        auto bin_of = [&](u64 d) -> u32 {
+        const int shift = max(0, kv_top_bit(static_cast<Key>(hi - lo)) + 1 - 11);
+        auto bin_of = [&](Key d) -> u32 {
             if (!octaves) return static_cast<u32>(d >> shift);
             if (d < 32) return static_cast<u32>(d);
-            const int top = 63 - __clzll(static_cast<long long>(d));  // 5 bits below the top one
+            const int top = kv_top_bit(d);  // 5 bits below the top one
             return static_cast<u32>((top - 4) * 32) + (static_cast<u32>(d >> (top - 5)) & 31u);
         };
         for (u32 i = threadIdx.x; i < kKvBins; i += blockDim.x) sm.histogram[i] = 0;
@@ -303,56 +367,67 @@ __device__ void kv_rank_limit(u32 n, u32 rank, Key least, Key greatest, KeyAt ke
         }
         at_lo = __reduce_add_sync(0xffffffffu, at_lo);
         if (lane == 0 && at_lo) atomicAdd(&sm.histogram[0], at_lo);
-        __syncthreads();
-        const u32 each = kKvBins / blockDim.x, from = threadIdx.x * each;  // 2 to 8 bins a thread
+        kv_team_sync(team);
+        u32* total = sm.histogram;
+        if (team.size > 1) {
+            total = sm.total;
+            for (u32 i = threadIdx.x; i < kKvBins; i += blockDim.x) {
+                u32 sum = 0;
+                for (u32 r = 0; r < team.size; ++r) sum += kv_peek(&sm.histogram[i], r);
+                total[i] = sum;
+            }
+            __syncthreads();
+        }
+        const u32 each = kKvBins / blockDim.x, from = threadIdx.x * each;  // 2 to 16 bins a thread
         u32 sum = 0;
-        for (u32 t = 0; t < each; ++t) sum += sm.histogram[from + t];
-        u32 upto = kv_block_scan(sum, sm.warp_sums);
+        for (u32 t = 0; t < each; ++t) sum += total[from + t];
+        const u32 upto = kv_block_scan(sum, sm.warp_sums);
         u32 before = upto - sum;
         if (before < rank && rank <= upto) {
             u32 t = from;
-            while (before + sm.histogram[t] < rank) before += sm.histogram[t++];
+            while (before + total[t] < rank) before += total[t++];
             sm.found[0] = t;
             sm.found[1] = before;
-            sm.found[2] = sm.histogram[t];
+            sm.found[2] = total[t];
         }
-        __syncthreads();
+        kv_team_sync(team);  // `found` is there, and nobody reads this CTA's counts any more
         const u32 bin = sm.found[0], count = sm.found[2];
         rank -= sm.found[1];
+        int width = octaves ? 0 : shift;  // log2 of the bin's width
         if (octaves && bin >= 32) {
-            const int width = static_cast<int>(bin / 32) - 1;  // log2 of the bin's width
-            lo += static_cast<u64>(32 + bin % 32) << width;
-            hi = min(hi, lo + ((u64{1} << width) - 1));
+            width = static_cast<int>(bin / 32) - 1;
+            lo += static_cast<Key>(32 + bin % 32) << width;
         } else {
-            const int width = octaves ? 0 : shift;
-            lo += static_cast<u64>(bin) << width;
-            hi = min(hi, lo + ((u64{1} << width) - 1));
+            lo += static_cast<Key>(bin) << width;
         }
+        hi = min(hi, static_cast<Key>(lo + ((Key{1} << width) - 1)));
         octaves = false;
         if (rank == count) {  // the whole bin
-            limit = static_cast<Key>(hi);
+            limit = hi;
             equals = kKvAll;
             return;
         }
-        __syncthreads();  // `found` and the bins are read
     }
 }
 
-// Walks 0..n-1 in order: state(i) is 0 (not chosen), 1 (chosen) or 2 (one of
-// the equals, of which the first `equals` are chosen).  For every i,
-// value = load(i), then store(i, value, chosen, how many chosen came before),
-// with a block barrier between them if kBarrier (stores may reach what a load
-// of the same round reads).  Counts come from ballots, one word per 32
-// elements, and one block-wide scan per 32768 elements.
+// Walks the team's elements in order (0..n-1 in each CTA, CTAs by rank; with
+// more than one CTA n is at most 32768): state(i) is 0 (not chosen), 1
+// (chosen) or 2 (one of the equals, of which the first `equals` are chosen).
+// For every i, value = load(i), then store(i, value, chosen, how many chosen
+// came before), with a block barrier between them if kBarrier (stores may
+// reach what a load of the same round reads).  Counts come from ballots, one
+// word per 32 elements, and one block-wide scan per 32768 elements.
 template <bool kBarrier, typename State, typename Load, typename Store>
-__device__ void kv_walk(u32 n, u32 equals, KvSelectShared& sm, State state, Load load, Store store)
+__device__ void kv_walk(const KvTeam& team, u32 n, u32 equals, KvSelectShared& sm, State state,
+                        Load load, Store store)
 {
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const u32 under = (1u << lane) - 1u;
     u32* prefix = sm.histogram;
-    u32 chosen_before = 0, equal_before = 0;
-    // exclusive prefix sums of the words' bit counts; returns their sum
-    auto scan_words = [&](u32 many) {
+    u32 before[2] = {0, 0};  // chosen, equals in front of the elements at hand
+    // Exclusive prefix sums of the words' bit counts; returns their sum.  A team's CTAs add
+    // what the ones in front counted to before[which].
+    auto scan_words = [&](u32 many, int which) {
         u32 carry = 0;
         for (u32 base = 0; base < many; base += blockDim.x) {
             const u32 w = base + threadIdx.x;
@@ -361,10 +436,16 @@ __device__ void kv_walk(u32 n, u32 equals, KvSelectShared& sm, State state, Load
             if (w < many) prefix[w] = carry + upto - bits;
             carry += sm.warp_sums[32];
         }
+        if (team.size > 1) {
+            if (threadIdx.x == 0) sm.counts[which] = carry;
+            kv_team_sync(team);
+            for (u32 r = 0; r < team.rank; ++r) before[which] += kv_peek(&sm.counts[which], r);
+        }
         __syncthreads();
         return carry;
     };
-    for (u32 first = 0; first < n; first += kKvWords * 32) {
+    u32 first = 0;
+    do {
         const u32 many = min(n - first, kKvWords * 32), words = (many + 31) / 32;
         const u32 rounds = (words + warps - 1) / warps;
         __syncthreads();
@@ -375,18 +456,17 @@ __device__ void kv_walk(u32 n, u32 equals, KvSelectShared& sm, State state, Load
                 if (lane == 0 && w < words) sm.words[w] = m;
             }
             __syncthreads();
-            const u32 all = scan_words(words);
+            const u32 all = scan_words(words, 1);
             // from here on the words hold what is chosen; a warp reads and writes its own words
             for (u32 r = 0; r < rounds; ++r) {
                 const u32 w = r * warps + warp, i = w * 32 + lane;
                 const u32 eq = w < words ? sm.words[w] : 0;
                 const bool one = i < many && state(first + i) == 1;
-                const bool rank_ok = w < words && equal_before + prefix[w] + __popc(eq & under) < equals;
+                const bool rank_ok = w < words && before[1] + prefix[w] + __popc(eq & under) < equals;
                 const u32 m = __ballot_sync(0xffffffffu, one || ((eq >> lane & 1u) && rank_ok));
-                __syncwarp();
                 if (lane == 0 && w < words) sm.words[w] = m;
             }
-            equal_before += all;
+            before[1] += all;
         } else {
             for (u32 r = 0; r < rounds; ++r) {
                 const u32 w = r * warps + warp, i = w * 32 + lane;
@@ -395,7 +475,7 @@ __device__ void kv_walk(u32 n, u32 equals, KvSelectShared& sm, State state, Load
             }
         }
         __syncthreads();
-        const u32 all = scan_words(words);
+        const u32 all = scan_words(words, 0);
         for (u32 r = 0; r < rounds; ++r) {
             const u32 w = r * warps + warp, i = w * 32 + lane;
             const bool in = i < many;
@@ -403,11 +483,12 @@ __device__ void kv_walk(u32 n, u32 equals, KvSelectShared& sm, State state, Load
             if constexpr (kBarrier) __syncthreads();
             if (in) {
                 const u32 m = sm.words[w];
-                store(first + i, value, (m >> lane & 1u) != 0, chosen_before + prefix[w] + __popc(m & under));
+                store(first + i, value, (m >> lane & 1u) != 0, before[0] + prefix[w] + __popc(m & under));
             }
         }
-        chosen_before += all;
-    }
+        before[0] += all;
+        first += kKvWords * 32;
+    } while (first < n);
 }
 
 #endif  // __CUDACC__

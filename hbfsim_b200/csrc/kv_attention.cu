@@ -844,7 +844,7 @@ int launch(const AttentionArgs& a, cudaStream_t s)
         across = std::max(across, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
                                            4u * kv_sm_count() / pairs));
     const u32 slices = std::min(std::max(1u, across / segments), 8u);
-    const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, 0, a,
+    const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, 0, 1, a,
                                      static_cast<u32>(8 * NT), slices);
     return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }

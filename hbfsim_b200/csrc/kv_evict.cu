@@ -1,19 +1,18 @@
 // kv_evict.cu -- blocks of least accumulated attention weight leave a block
 // table (kv_v1.h).
 //
-// One CTA per sequence.  The weights become whole numbers (2^30 to a query)
-// before anything is added, so scores and decisions do not depend on the
-// order of the sums.  Pass 1 adds the step's weights to every block's score
-// (kept in shared memory up to kHeldBlocks blocks, else in the output; few
-// long sequences have it done by a kernel of its own over all SMs); the
-// score of the last block to leave is found by a selection on the scores;
-// the walk in block order then closes up the survivors.
+// One team (a CTA, or a cluster with few long sequences) per sequence.  The
+// weights become whole numbers (2^30 to a query) before anything is added, so
+// scores and decisions do not depend on the order of the sums.  Pass 1 adds
+// the step's weights to every block's score (kept in shared memory up to
+// kHeldBlocks blocks a CTA, else in the output); the score of the last block
+// to leave is found by a selection on the scores; the walk in block order
+// then closes up the survivors.
 #include "kv.h"
 
 namespace hbfb {
 namespace {
 
-constexpr u32 kEvictThreads = 1024, kAddThreads = 128;
 constexpr u32 kHeldBlocks = 24 * 1024;  // 192 KB of scores
 
 struct EvictArgs {
@@ -47,42 +46,36 @@ __device__ __forceinline__ i64 new_score(const EvictArgs& a, u64 row, u32 j)
     return s;
 }
 
-__global__ void __launch_bounds__(kAddThreads) add_kernel(const EvictArgs a)
+// `slice`: blocks of a row that one CTA of the team has.
+__global__ void __launch_bounds__(1024) evict_kernel(const EvictArgs a, u32 team_size, u32 slice)
 {
-    kv_let_next();
-    const u32 seq = blockIdx.y, j = blockIdx.x * kAddThreads + threadIdx.x;
-    const u32 blocks = (static_cast<u32>(kv_length(a.lengths, seq, a.width, a.block)) + a.block - 1) / a.block;
-    const u64 row = static_cast<u64>(seq) * a.width;
-    if (j < blocks) a.score_out[row + j] = new_score(a, row, j);
-}
-
-// `added`: add_kernel has put the new scores into score_out.
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a, bool added)
-{
-    kv_wait_before();
     extern __shared__ __align__(16) i64 held[];
     __shared__ KvSelectShared sm;
-    const u32 seq = blockIdx.x;
+    kv_wait_before();
+    const KvTeam team{blockIdx.x % team_size, team_size};
+    const u32 seq = blockIdx.x / team_size;
     const int length = kv_length(a.lengths, seq, a.width, a.block);
     const u32 blocks = (static_cast<u32>(length) + a.block - 1) / a.block;
     const u32 leave = blocks > a.keep ? blocks - a.keep : 0;
     const u64 row = static_cast<u64>(seq) * a.width;
+    const u32 first = team.rank * slice, end = min(first + slice, a.width);  // this CTA's
     const int* table = a.table + static_cast<i64>(seq) * a.table_stride;
     i64* score_out = a.score_out + row;
-    i64* score = a.width <= kHeldBlocks && leave ? held : score_out;
+    const bool hold = slice <= kHeldBlocks && leave;
+    i64* score = hold ? held : score_out + first;  // of block `first` on
     int* table_out = a.table_out + row;
     int* freed = a.freed + row;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && team.rank == 0) {
         a.lengths_out[seq] = length - static_cast<int>(leave * a.block);
         a.freed_counts[seq] = static_cast<int>(leave);
     }
     const u32 from = a.sink, to = blocks - min(a.recent, blocks);  // those that may leave
     u64 least = ~u64{0}, greatest = 0;
     // pass 1: every block's new score
-    for (u32 j = threadIdx.x; j < a.width; j += blockDim.x) {
+    for (u32 j = first + threadIdx.x; j < end; j += blockDim.x) {
         if (j < blocks) {
-            const i64 s = added ? score_out[j] : new_score(a, row, j);
-            score[j] = s;
+            const i64 s = new_score(a, row, j);
+            score[j - first] = s;
             if (leave == 0) table_out[j] = table[j];
             if (j >= from && j < to) {
                 least = min(least, score_key(s));
@@ -90,7 +83,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a,
             }
         }
         if (j >= blocks - leave) {  // behind the survivors
-            if (j >= blocks || score != score_out) score_out[j] = 0;
+            if (j >= blocks || hold) score_out[j] = 0;
             table_out[j] = -1;
         }
         if (j >= leave) freed[j] = -1;
@@ -100,37 +93,37 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a,
     // the score of the last block to leave, and how many of its equals do
     u64 limit;
     u32 equals;
+    const u32 mine = min(max(blocks, first), end) - first;  // blocks of this CTA in use
     kv_rank_limit<u64>(
-        to, leave, least, greatest,
-        [&](u32 j, u64& k) {
-            k = score_key(score[j]);
-            return j >= from;
+        team, mine, leave, least, greatest,
+        [&](u32 i, u64& k) {
+            k = score_key(score[i]);
+            return first + i >= from && first + i < to;
         },
         sm, limit, equals);
     struct Entry {
         i64 score;
         int page;
     };
-    auto state = [&](u32 j) -> u32 {
-        if (j < from || j >= to) return 0;
-        const u64 k = score_key(score[j]);
+    auto state = [&](u32 i) -> u32 {
+        if (first + i < from || first + i >= to) return 0;
+        const u64 k = score_key(score[i]);
         return k < limit ? 1 : k == limit ? 2 : 0;
     };
-    auto load = [&](u32 j) { return Entry{score[j], table[j]}; };
-    auto store = [&](u32 j, const Entry& e, bool gone, u32 gone_before) {
+    auto load = [&](u32 i) { return i < mine ? Entry{score[i], table[first + i]} : Entry{0, 0}; };
+    auto store = [&](u32 i, const Entry& e, bool gone, u32 gone_before) {
         if (gone) {
             freed[gone_before] = e.page;
         } else {  // survivors only move towards the front
-            score_out[j - gone_before] = e.score;
-            table_out[j - gone_before] = e.page;
+            score_out[first + i - gone_before] = e.score;
+            table_out[first + i - gone_before] = e.page;
         }
     };
-    if (score != score_out) kv_walk<false>(blocks, equals, sm, state, load, store);
-    else kv_walk<true>(blocks, equals, sm, state, load, store);
-    if (score == score_out) {  // what lies behind the survivors was needed until now
-        __syncthreads();
+    if (hold) kv_walk<false>(team, mine, equals, sm, state, load, store);
+    else kv_walk<true>(team, mine, equals, sm, state, load, store);
+    kv_team_sync(team);  // nobody leaves while another may read its counts
+    if (!hold)  // what lies behind the survivors was needed until now
         for (u32 j = blocks - leave + threadIdx.x; j < blocks; j += blockDim.x) score_out[j] = 0;
-    }
 }
 
 }  // namespace
@@ -165,12 +158,14 @@ extern "C" int hbfsim_kv_evict_v1(const hbfsim_kv_evict_batch_v1* b, void* strea
                 b->recent,     b->decay};
     static std::atomic<u64> seen{0};
     if (!kv_allow_smem(evict_kernel, kHeldBlocks * 8, seen)) return HBFSIM_CUDA_ERROR;
-    const u32 smem = b->width <= kHeldBlocks ? b->width * 8 : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // Fewer sequences than half the SMs and more than two rounds of a CTA each: all SMs add.
-    const bool apart = b->seqs * 2 < static_cast<u32>(kv_sm_count()) && b->width > 2 * kEvictThreads;
-    if (apart)
-        add_kernel<<<dim3((b->width + kAddThreads - 1) / kAddThreads, b->seqs), kAddThreads, 0, s>>>(a);
-    const bool ok = kv_launch_behind(evict_kernel, dim3(b->seqs), kEvictThreads, s, smem, a, apart);
-    return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    u32 team = kv_team_size(b->seqs, b->width);
+    u32 slice = (b->width + team - 1) / team;
+    if (slice > kHeldBlocks) {  // a row that no team can hold is walked in place by one CTA
+        team = 1;
+        slice = b->width;
+    }
+    const bool ok = kv_launch_behind(evict_kernel, dim3(b->seqs * team), kv_team_threads(slice), s,
+                                     slice <= kHeldBlocks ? slice * 8 : 0, team, a, team, slice);
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }

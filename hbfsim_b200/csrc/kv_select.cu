@@ -13,10 +13,10 @@
 //
 // score_kernel streams the bounds and writes a 32-bit ordered key per
 // (token, head, block): the blocks of all sequences form one line that is cut
-// into equal shares, one per resident CTA.  list_kernel, one CTA per
-// (sequence, token, head), finds the key of the last block to list by a
-// selection on the keys (in shared memory up to kHeldKeys blocks) and writes
-// the list in block order.
+// into equal shares, one per resident CTA.  list_kernel, one team (a CTA, or
+// a cluster for few long rows) per (sequence, token, head), finds the key of
+// the last block to list by a selection on the keys (in shared memory up to
+// kHeldKeys blocks a CTA) and writes the list in block order.
 #include "kv.h"
 
 #include <algorithm>
@@ -240,28 +240,31 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm) score_kernel(const
     }
 }
 
-__global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a)
+// `slice`: blocks of a row that one CTA of the team has.
+__global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team_size, u32 slice)
 {
     extern __shared__ __align__(16) u32 held[];
     __shared__ KvSelectShared sm;
     __shared__ u32 counted[2];  // blocks that are there, and those always listed
     kv_wait_before();
-    const u64 at = blockIdx.x;  // (sequence, token, head)
+    const KvTeam team{blockIdx.x % team_size, team_size};
+    const u64 at = blockIdx.x / team_size;  // (sequence, token, head)
     const u32 heads = a.c.heads, tokens = a.q.tokens;
     const u32 t = static_cast<u32>(at / heads % tokens), seq = static_cast<u32>(at / heads / tokens);
     const int length = kv_length(a.q.lengths, seq, a.q.width, a.c.block);
     const u32 have = blocks_of_token(length, tokens, t, a.c.block);
-    const u32* row = a.keys + at * a.q.width;
-    const bool hold = a.q.width <= kHeldKeys;
+    const u32 first = team.rank * slice, mine = min(max(have, first), first + slice) - first;
+    const u32* row = a.keys + at * a.q.width + first;
+    const bool hold = slice <= kHeldKeys;
     const u32* keys = hold ? held : row;
     int* list = a.blocks + at * a.top;
     if (threadIdx.x < 2) counted[threadIdx.x] = 0;
     __syncthreads();
     u32 there = 0, always = 0, least = ~0u, greatest = 0;
 #pragma unroll 8
-    for (u32 j = threadIdx.x; j < have; j += blockDim.x) {
-        const u32 k = row[j];
-        if (hold) held[j] = k;
+    for (u32 i = threadIdx.x; i < mine; i += blockDim.x) {
+        const u32 k = row[i];
+        if (hold) held[i] = k;
         there += k != kAbsent;
         always += k == kAlways;
         if (k != kAbsent && k != kAlways) {
@@ -275,17 +278,22 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a)
         atomicAdd(&counted[0], there);
         atomicAdd(&counted[1], always);
     }
-    __syncthreads();
+    kv_team_sync(team);
     there = counted[0];
     always = counted[1];
+    for (u32 r = 0; r < team.size; ++r)
+        if (r != team.rank) {
+            there += kv_peek(&counted[0], r);
+            always += kv_peek(&counted[1], r);
+        }
     const u32 take = min(a.top, there);
     // the greatest keys are the smallest of their complements; those always listed need no rank
     u32 limit = 0xffffffffu, equals = kKvAll;
     if (take < there && take > always)
         kv_rank_limit<u32>(
-            have, take - always, least, greatest,
-            [&](u32 j, u32& k) {
-                k = keys[j];
+            team, mine, take - always, least, greatest,
+            [&](u32 i, u32& k) {
+                k = keys[i];
                 if (k == kAbsent || k == kAlways) return false;
                 k = ~k;
                 return true;
@@ -294,18 +302,21 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a)
     else if (take < there)
         limit = 0, equals = 0;  // none but those always listed
     kv_walk<false>(
-        have, equals, sm,
-        [&](u32 j) -> u32 {
-            const u32 k = keys[j];
+        team, mine, equals, sm,
+        [&](u32 i) -> u32 {
+            const u32 k = keys[i];
             if (k == kAbsent) return 0;
             return k == kAlways || ~k < limit ? 1 : ~k == limit ? 2 : 0;
         },
         [](u32) { return 0; },
-        [&](u32 j, int, bool listed, u32 before) {
-            if (listed && before < a.top) list[before] = static_cast<int>(j);
+        [&](u32 i, int, bool listed, u32 before) {
+            if (listed && before < a.top) list[before] = static_cast<int>(first + i);
         });
-    for (u32 i = take + threadIdx.x; i < a.top; i += blockDim.x) list[i] = -1;
-    if (threadIdx.x == 0) a.counts[at] = static_cast<int>(take);
+    if (team.rank == 0) {
+        for (u32 i = take + threadIdx.x; i < a.top; i += blockDim.x) list[i] = -1;
+        if (threadIdx.x == 0) a.counts[at] = static_cast<int>(take);
+    }
+    kv_team_sync(team);  // nobody leaves while another may read its counts
 }
 
 u64 workspace_bytes_of(const KvView& v, const KvQuery& q)
@@ -322,12 +333,19 @@ int launch(const SelectArgs& a, cudaStream_t s)
     const u64 most = (static_cast<u64>(a.q.seqs) * a.q.width + kScoreShare - 1) / kScoreShare;
     const u32 grid = static_cast<u32>(std::min<u64>(most, static_cast<u64>(kScorePerSm) * kv_sm_count()));
     if (grid) score_kernel<D><<<grid, kScoreThreads, smem, s>>>(a);
-    // a long row is one CTA's: more threads for it
     static std::atomic<u64> seen_list{0};
     if (!kv_allow_smem(list_kernel, kHeldKeys * 4, seen_list)) return HBFSIM_CUDA_ERROR;
-    const u32 threads = a.q.width <= 512 ? 128 : a.q.width <= 4096 ? 256 : 1024;
-    const bool ok = kv_launch_behind(list_kernel, dim3(a.q.seqs * a.q.tokens * a.c.heads), threads, s,
-                                     a.q.width <= kHeldKeys ? a.q.width * 4 : 0, a);
+    const u32 rows = a.q.seqs * a.q.tokens * a.c.heads;
+    u32 team = kv_team_size(rows, a.q.width), slice = (a.q.width + team - 1) / team;
+    if (slice > kHeldKeys) {  // a row that no team can hold is one CTA's
+        team = 1;
+        slice = a.q.width;
+    }
+    // many rows: small CTAs, several to an SM
+    u32 threads = kv_team_threads(slice);
+    if (rows > 2 * static_cast<u32>(kv_sm_count())) threads = std::min(threads, 256u);
+    const bool ok = kv_launch_behind(list_kernel, dim3(rows * team), threads, s,
+                                     slice <= kHeldKeys ? slice * 4 : 0, team, a, team, slice);
     return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 

@@ -583,3 +583,44 @@ def test_decode_steps_and_their_reads(tmp_path):
         score, table, lengths = rest.score, rest.table.cpu().numpy(), rest.lengths.cpu().numpy()
         assert (-(-lengths // block) <= keep).all()
     ctx.close()
+
+
+@pytest.mark.parametrize("seqs,blocks,keep,kind", [(1, 3000, 2000, "equal"), (1, 20000, 100, "octaves"),
+                                                   (2, 9000, 8999, "zeros"), (1, 5000, 40, "equal"),
+                                                   (1, 250000, 1000, "octaves")])
+def test_evict_long_rows(seqs, blocks, keep, kind):
+    """Rows that several thread blocks share, and one that none can hold: all scores equal,
+    scores of many orders, mostly zeros."""
+    torch = torch_()
+    from hbfsim_b200 import kv_evict
+    rng = np.random.default_rng(blocks)
+    table = rng.permutation(seqs * blocks).reshape(seqs, blocks).astype(np.int32)
+    lengths = [blocks * 16 - 5 * b for b in range(seqs)]
+    weights = np.zeros((seqs, 2, blocks), np.float32)
+    if kind == "equal":
+        score = np.full((seqs, blocks), 77, np.int64)
+    elif kind == "zeros":
+        score = np.where(rng.random((seqs, blocks)) < 0.001, 5, 0)
+    else:
+        score = (2.0 ** rng.uniform(0, 50, (seqs, blocks))).astype(np.int64)
+        weights = (2.0 ** rng.uniform(-30, 5, weights.shape)).astype(np.float32)
+    got = kv_evict(torch.from_numpy(score).cuda(), torch.from_numpy(weights).cuda(), int32(table),
+                   int32(lengths), keep)
+    want = ko.evict(score, weights, table, lengths, keep, 16, 1, 1, 0)
+    for a, b, name in zip(got, want, got._fields):
+        assert np.array_equal(a.cpu().numpy(), b), name
+
+
+@pytest.mark.parametrize("blocks,top,heads", [(6000, 37, 2), (40000, 5000, 1), (300000, 64, 1)])
+def test_select_long_rows(blocks, top, heads):
+    """Rows that several thread blocks share, and one that none can hold; few distinct pages, so
+    that ties decide at the end of the list."""
+    torch = torch_()
+    from hbfsim_b200 import kv_select
+    rng = np.random.default_rng(blocks)
+    dim, block = 64, 16
+    cache = random_cache(rng, 300, heads, block, dim)
+    table = rng.integers(0, 300, (1, blocks)).astype(np.int32)
+    q = torch.from_numpy(rng.standard_normal((1, 1, heads, dim))).to(torch.bfloat16).cuda()
+    got = kv_select(to_gpu(cache), q, int32(table), int32([blocks * block - 3]), top)
+    assert_lists(got, ko.select(cache, q.double().cpu().numpy(), table, [blocks * block - 3], top, 1, 1))
