@@ -262,13 +262,13 @@ __device__ __forceinline__ u32 kv_block_scan(u32 x, u32* warp_sums)
 // shared memory (a row of 16,000 keys is bound by one SM's instructions).
 constexpr u32 kKvBins = 2048, kKvWords = 1024;
 struct KvSelectShared {
-    u32 histogram[kKvBins];   // this CTA's counts; also the prefix sums of `words`
-    u32 total[kKvBins];       // the team's
+    u32 histogram[kKvBins];   // counts of the bins; also the prefix sums of `words`
+    u32 group[kKvBins / 32];  // sums of 32 counts
     u32 words[kKvWords];
     u32 warp_sums[33];
     u32 found[3];
-    u32 counts[2];
-    u64 lo, hi;
+    u32 counts[2], in_front;
+    u64 range[32][2], team_range[2];  // least and greatest key of the warps, of the CTA
 };
 constexpr u32 kKvAll = 0xffffffffu;
 
@@ -302,6 +302,14 @@ __device__ __forceinline__ T kv_peek(const T* mine, u32 rank)
     return x;
 }
 
+// Sum of a word over the CTAs [0, ranks) of the team: one lane per CTA, all
+// lanes of the warp get it.
+__device__ __forceinline__ u32 kv_team_sum(const u32* mine, u32 ranks)
+{
+    const u32 lane = threadIdx.x & 31u;
+    return __reduce_add_sync(0xffffffffu, lane < ranks ? kv_peek(mine, lane) : 0);
+}
+
 __device__ __forceinline__ int kv_top_bit(u32 x) { return 31 - __clz(static_cast<int>(x)); }
 __device__ __forceinline__ int kv_top_bit(u64 x) { return 63 - __clzll(static_cast<long long>(x)); }
 
@@ -319,29 +327,48 @@ __device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Ke
                               KeyAt key_at, KvSelectShared& sm, Key& limit, u32& equals)
 {
     const u32 lane = threadIdx.x & 31u;
-    if (threadIdx.x == 0) {
-        sm.lo = ~u64{0};
-        sm.hi = 0;
+    Key lo = least, hi = greatest;
+    auto reduce = [&]() {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+    };
+    reduce();
+    if (lane == 0) {
+        sm.range[threadIdx.x >> 5][0] = lo;
+        sm.range[threadIdx.x >> 5][1] = hi;
     }
     __syncthreads();
-    Key lo = least, hi = greatest;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = ~Key{0};
+    hi = 0;
+    if (lane < blockDim.x >> 5) {
+        lo = static_cast<Key>(sm.range[lane][0]);
+        hi = static_cast<Key>(sm.range[lane][1]);
     }
-    if (lane == 0) {
-        atomicMin(reinterpret_cast<unsigned long long*>(&sm.lo), static_cast<u64>(lo));
-        atomicMax(reinterpret_cast<unsigned long long*>(&sm.hi), static_cast<u64>(hi));
-    }
-    kv_team_sync(team);
-    lo = static_cast<Key>(sm.lo);
-    hi = static_cast<Key>(sm.hi);
-    for (u32 r = 0; r < team.size; ++r)
-        if (r != team.rank) {
-            lo = min(lo, static_cast<Key>(kv_peek(&sm.lo, r)));
-            hi = max(hi, static_cast<Key>(kv_peek(&sm.hi, r)));
+    reduce();
+    if (team.size > 1) {
+        if (threadIdx.x == 0) {
+            sm.team_range[0] = lo;
+            sm.team_range[1] = hi;
         }
+        kv_team_sync(team);
+        if (threadIdx.x < 32) {  // one warp asks the others' CTAs
+            if (lane < team.size) {
+                lo = static_cast<Key>(kv_peek(&sm.team_range[0], lane));
+                hi = static_cast<Key>(kv_peek(&sm.team_range[1], lane));
+            }
+            reduce();
+            if (lane == 0) {
+                sm.range[0][0] = lo;
+                sm.range[0][1] = hi;
+            }
+        }
+        __syncthreads();
+        lo = static_cast<Key>(sm.range[0][0]);
+        hi = static_cast<Key>(sm.range[0][1]);
+    }
     bool octaves = true;
     for (;;) {
         if (lo >= hi) {  // one value is left
@@ -367,28 +394,61 @@ __device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Ke
         }
         at_lo = __reduce_add_sync(0xffffffffu, at_lo);
         if (lane == 0 && at_lo) atomicAdd(&sm.histogram[0], at_lo);
-        kv_team_sync(team);
-        u32* total = sm.histogram;
-        if (team.size > 1) {
-            total = sm.total;
-            for (u32 i = threadIdx.x; i < kKvBins; i += blockDim.x) {
-                u32 sum = 0;
-                for (u32 r = 0; r < team.size; ++r) sum += kv_peek(&sm.histogram[i], r);
-                total[i] = sum;
+        __syncthreads();
+        if (team.size == 1) {
+            const u32 each = kKvBins / blockDim.x, from = threadIdx.x * each;  // 2 to 16 bins a thread
+            u32 sum = 0;
+            for (u32 t = 0; t < each; ++t) sum += sm.histogram[from + t];
+            const u32 upto = kv_block_scan(sum, sm.warp_sums);
+            u32 before = upto - sum;
+            if (before < rank && rank <= upto) {
+                u32 t = from;
+                while (before + sm.histogram[t] < rank) before += sm.histogram[t++];
+                sm.found[0] = t;
+                sm.found[1] = before;
+                sm.found[2] = sm.histogram[t];
             }
-            __syncthreads();
-        }
-        const u32 each = kKvBins / blockDim.x, from = threadIdx.x * each;  // 2 to 16 bins a thread
-        u32 sum = 0;
-        for (u32 t = 0; t < each; ++t) sum += total[from + t];
-        const u32 upto = kv_block_scan(sum, sm.warp_sums);
-        u32 before = upto - sum;
-        if (before < rank && rank <= upto) {
-            u32 t = from;
-            while (before + total[t] < rank) before += total[t++];
-            sm.found[0] = t;
-            sm.found[1] = before;
-            sm.found[2] = total[t];
+        } else {
+            // Words of other CTAs are dear: first the sums of 32 bins each, then the 32 bins of
+            // the group that holds the rank, by one warp.
+            const u32 warps = blockDim.x >> 5;
+            for (u32 w = threadIdx.x >> 5; w < kKvBins / 32; w += warps) {
+                const u32 sum = __reduce_add_sync(0xffffffffu, sm.histogram[w * 32 + lane]);
+                if (lane == 0) sm.group[w] = sum;
+            }
+            kv_team_sync(team);
+            if (threadIdx.x < 32) {
+                u32 before = 0, at = 0;
+                // place of the rank among 32 counts, one per lane, each the team's sum
+                auto narrow = [&](const u32* mine) -> bool {
+                    u32 part[kKvTeam], sum = 0;  // all reads under way before the first sum
+#pragma unroll
+                    for (u32 r = 0; r < kKvTeam; ++r) part[r] = r < team.size ? kv_peek(mine + lane, r) : 0;
+#pragma unroll
+                    for (u32 r = 0; r < kKvTeam; ++r) sum += part[r];
+                    u32 upto = sum;
+#pragma unroll
+                    for (u32 o = 1; o < 32; o <<= 1) {
+                        const u32 y = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += y;
+                    }
+                    const u32 here = __ballot_sync(0xffffffffu, before + upto >= rank);
+                    at = here ? __ffs(here) - 1 : 31;
+                    const u32 in_front = __shfl_sync(0xffffffffu, upto - sum, at);
+                    const u32 count = __shfl_sync(0xffffffffu, sum, at);
+                    before += here ? in_front : __shfl_sync(0xffffffffu, upto, 31);
+                    if (lane == 0) sm.found[2] = count;
+                    return here != 0;
+                };
+                u32 group = 0;
+                while (!narrow(sm.group + group) && group + 64 <= kKvBins / 32) group += 32;
+                group += at;
+                narrow(sm.histogram + group * 32);
+                if (lane == 0) {
+                    sm.found[0] = group * 32 + at;
+                    sm.found[1] = before;
+                }
+            }
         }
         kv_team_sync(team);  // `found` is there, and nobody reads this CTA's counts any more
         const u32 bin = sm.found[0], count = sm.found[2];
@@ -439,7 +499,12 @@ __device__ void kv_walk(const KvTeam& team, u32 n, u32 equals, KvSelectShared& s
         if (team.size > 1) {
             if (threadIdx.x == 0) sm.counts[which] = carry;
             kv_team_sync(team);
-            for (u32 r = 0; r < team.rank; ++r) before[which] += kv_peek(&sm.counts[which], r);
+            if (threadIdx.x < 32) {
+                const u32 sum = kv_team_sum(&sm.counts[which], team.rank);
+                if (lane == 0) sm.in_front = sum;
+            }
+            __syncthreads();
+            before[which] += sm.in_front;
         }
         __syncthreads();
         return carry;

@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
 {
     extern __shared__ __align__(16) u32 held[];
     __shared__ KvSelectShared sm;
-    __shared__ u32 counted[2];  // blocks that are there, and those always listed
+    __shared__ u32 counted[4];  // blocks that are there, those always listed; the team's
     kv_wait_before();
     const KvTeam team{blockIdx.x % team_size, team_size};
     const u64 at = blockIdx.x / team_size;  // (sequence, token, head)
@@ -279,13 +279,18 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
         atomicAdd(&counted[1], always);
     }
     kv_team_sync(team);
-    there = counted[0];
-    always = counted[1];
-    for (u32 r = 0; r < team.size; ++r)
-        if (r != team.rank) {
-            there += kv_peek(&counted[0], r);
-            always += kv_peek(&counted[1], r);
+    if (team.size > 1) {
+        if (threadIdx.x < 32) {
+            const u32 all = kv_team_sum(&counted[0], team.size), all_always = kv_team_sum(&counted[1], team.size);
+            if (threadIdx.x == 0) {
+                counted[2] = all;
+                counted[3] = all_always;
+            }
         }
+        __syncthreads();
+    }
+    there = counted[team.size > 1 ? 2 : 0];
+    always = counted[team.size > 1 ? 3 : 1];
     const u32 take = min(a.top, there);
     // the greatest keys are the smallest of their complements; those always listed need no rank
     u32 limit = 0xffffffffu, equals = kKvAll;
