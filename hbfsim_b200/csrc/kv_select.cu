@@ -56,7 +56,7 @@ __device__ __forceinline__ void query_at(const KvQuery& q, u32 seq, u32 token, u
 __device__ __forceinline__ u32 blocks_of_token(int length, u32 tokens, u32 t, u32 block)
 {
     const int last = length - static_cast<int>(tokens) + static_cast<int>(t);
-    return last < 0 ? 0u : static_cast<u32>(last) / block + 1u;
+    return last < 0 ? 0u : (static_cast<u32>(last) >> (31 - __clz(block))) + 1u;  // 16, 32 or 64
 }
 
 // Finite floats in their order, above kAbsent and below kAlways.
@@ -179,40 +179,48 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm) score_kernel(const
         __syncthreads();
         const int* table = a.q.table + static_cast<i64>(seq) * a.q.table_stride;
         const u32 g = lane >> 2, c = lane & 3u;
-        const u32 tasks = (end - first + 15) / 16 * heads;  // 16 blocks of one head
-        auto page_of = [&](u32 task, u32 more) {
-            const u32 j = first + task / heads * 16 + g + more;
-            return task < tasks && j < end ? kv_page(table, j, a.c.pages) : -1;
+        // Tasks: 16 blocks of one head, heads first, by the warps in turn.
+        const u32 rows = (end - first + 15) / 16, skip_rows = warps / heads, skip_heads = warps % heads;
+        auto page_of = [&](u32 row, u32 more) {
+            const u32 j = first + row * 16 + g + more;
+            return row < rows && j < end ? kv_page(table, j, a.c.pages) : -1;
         };
-        int next0 = page_of(warp, 0), next1 = page_of(warp, 8);
-        for (u32 task = warp; task < tasks; task += warps) {
-            const u32 h = task % heads, j0 = first + task / heads * 16 + g, j1 = j0 + 8;
+        u32 row = warp / heads, h = warp % heads;
+        int next0 = page_of(row, 0), next1 = page_of(row, 8);
+        while (row < rows) {
+            const u32 j0 = first + row * 16 + g, j1 = j0 + 8, head = h;
             const int page0 = next0, page1 = next1;
+            row += skip_rows;
+            h += skip_heads;
+            if (h >= heads) {
+                h -= heads;
+                ++row;
+            }
             uint4 x0[kChunks], x1[kChunks];
             float scale0 = 0.0f, scale1 = 0.0f;
 #pragma unroll
             for (u32 k = 0; k < kChunks; ++k) x0[k] = x1[k] = make_uint4(0, 0, 0, 0);
             if (page0 >= 0) {
-                const u64 x = static_cast<u64>(page0) * heads + h;
+                const u64 x = static_cast<u64>(page0) * heads + head;
                 const uint4* b = reinterpret_cast<const uint4*>(a.c.bounds + x * 2 * D) + c;
 #pragma unroll
                 for (u32 k = 0; k < kChunks; ++k) x0[k] = b[k * 4];
                 scale0 = a.c.scale[x * 2];
             }
             if (page1 >= 0) {
-                const u64 x = static_cast<u64>(page1) * heads + h;
+                const u64 x = static_cast<u64>(page1) * heads + head;
                 const uint4* b = reinterpret_cast<const uint4*>(a.c.bounds + x * 2 * D) + c;
 #pragma unroll
                 for (u32 k = 0; k < kChunks; ++k) x1[k] = b[k * 4];
                 scale1 = a.c.scale[x * 2];
             }
-            next0 = page_of(task + warps, 0);
-            next1 = page_of(task + warps, 8);
+            next0 = page_of(row, 0);
+            next1 = page_of(row, 8);
             // four tokens at a time: column g is the high or low part of token t0 + g / 2
             for (u32 t0 = 0; t0 < tokens; t0 += 4) {
                 int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
                 const bool used = t0 + g / 2 < tokens;
-                const std::int8_t* column = whole + (h * 2 * tokens + 2 * t0 + g) * kColumn + c * 16;
+                const std::int8_t* column = whole + (head * 2 * tokens + 2 * t0 + g) * kColumn + c * 16;
 #pragma unroll
                 for (u32 k = 0; k < kChunks; ++k) {
                     uint4 y = make_uint4(0, 0, 0, 0);
@@ -223,7 +231,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm) score_kernel(const
                 const u32 t = t0 + c;  // this lane's columns 2c and 2c + 1
                 if (t < tokens) {
                     const u32 mine = blocks_of_token(length, tokens, t, a.c.block);
-                    u32* keys = a.keys + ((static_cast<u64>(seq) * tokens + t) * heads + h) * a.q.width;
+                    u32* keys = a.keys + ((static_cast<u64>(seq) * tokens + t) * heads + head) * a.q.width;
                     auto put = [&](u32 j, int page, int sum, float scale) {
                         u32 key = kAbsent;
                         if (page >= 0 && j < mine)
