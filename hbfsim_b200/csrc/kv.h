@@ -227,6 +227,28 @@ __device__ __forceinline__ void kv_load(const void* p, i64 at, u32 type, bool wi
     }
 }
 
+// Asynchronous copies from global to shared memory.
+__device__ __forceinline__ u32 kv_shared(const void* p) { return static_cast<u32>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void kv_copy16(u32 to, const void* from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void kv_copy16(void* to, const void* from) { kv_copy16(kv_shared(to), from); }
+__device__ __forceinline__ void kv_copy8(u32 to, const void* from)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void kv_copy4(void* to, const void* from)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(kv_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void kv_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void kv_copy_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // 2^e in 32 bits, -127 < e < 128.
 __device__ __forceinline__ float kv_power(int e) { return __int_as_float((e + 127) << 23); }
 

@@ -115,24 +115,6 @@ __device__ __forceinline__ float inverse_power(float x)
     return __int_as_float((254 << 23) - __float_as_int(x));
 }
 
-__device__ __forceinline__ void copy16(u32 to, const void* from)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-
-__device__ __forceinline__ void copy8(u32 to, const void* from)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
-}
-
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
-template <int N>
-__device__ __forceinline__ void copy_wait()
-{
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Place of byte o of a tile side in shared memory: the 16-byte pieces of a
 // 128-byte line are exchanged by the line's number, so that the lanes that
 // read one channel range of 4 tokens, or 8 tokens of one range, meet
@@ -295,18 +277,18 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 const u32 even = to + swizzle(lane * 16), odd = to + swizzle(512 + lane * 16);
 #pragma unroll
                 for (u32 k = 0; k < kSide; k += 1024) {
-                    copy16(even + k, from + k);
-                    copy16(odd + k, from + k + 512);
+                    kv_copy16(even + k, from + k);
+                    kv_copy16(odd + k, from + k + 512);
                 }
 #pragma unroll
                 for (u32 k = 0; k < kSide; k += 1024) {
-                    copy16(even + kSide + k, from_v + k);
-                    copy16(odd + kSide + k, from_v + k + 512);
+                    kv_copy16(even + kSide + k, from_v + k);
+                    kv_copy16(odd + kSide + k, from_v + k + 512);
                 }
-                if (lane == 0) copy8(note_at + stage * 16 + 8, head_scale + static_cast<u64>(page) * page_scales);
+                if (lane == 0) kv_copy8(note_at + stage * 16 + 8, head_scale + static_cast<u64>(page) * page_scales);
             }
         }
-        copy_commit();
+        kv_copy_commit();
     };
 #pragma unroll
     for (u32 i = 0; i + 1 < NS; ++i) issue(i, i);
@@ -563,7 +545,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + first + warp) * R
                                  : nullptr;
     for (u32 i = 0; i < turns; ++i) {
-        copy_wait<NS - 2>();
+        kv_copy_wait<NS - 2>();
         __syncwarp();  // the stage is there, and every lane is done with the one before it
         issue(i + NS - 1, stage == 0 ? NS - 1 : stage - 1);
         const int4 noted = note[stage];
@@ -580,7 +562,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         }
         if (tile_out) tile_out += kWarps * R;
     }
-    copy_wait<0>();
+    kv_copy_wait<0>();
     __syncthreads();  // every ring is at rest: its memory takes the joined values
     // join the warps: every warp's sums at its own maximum, values times its scale
 #pragma unroll

@@ -7,16 +7,17 @@
 // and 2 * head_dim bytes, 1/16 of its keys and values at 16 tokens a block.
 // The sums go through the tensor cores as 8-bit whole numbers: up and down
 // (at most 64 * 127) are split into 128 * high + low, two columns of the
-// narrow side; 16 blocks of a head are the wide side, read straight into the
-// fragments, 16 bytes per lane.  (Two-way dot instructions took 4 times the
-// instructions and were bound by them.)
+// narrow side; 16 blocks of a head are the wide side.  (Two-way dot
+// instructions took 4 times the instructions and were bound by them.)
 //
-// score_kernel streams the bounds and writes a 32-bit ordered key per
-// (token, head, block): the blocks of all sequences form one line that is cut
-// into equal shares, one per resident CTA.  list_kernel, one team (a CTA, or
-// a cluster for few long rows) per (sequence, token, head), finds the key of
-// the last block to list by a selection on the keys (in shared memory up to
-// kHeldKeys blocks a CTA) and writes the list in block order.
+// query_kernel makes the whole numbers once; score_kernel streams the bounds
+// through a ring of asynchronous copies per warp and writes a 32-bit ordered
+// key per (token, head, block): the blocks of all sequences form one line
+// that is cut into equal shares, one per resident CTA.  list_kernel, one team
+// (a CTA, or a cluster for few long rows) per (sequence, token, head), finds
+// the key of the last block to list by a selection on the keys (in shared
+// memory up to kHeldKeys blocks a CTA) and writes the list in block order.
+// Each kernel is set up while the one before it runs.
 #include "kv.h"
 
 #include <algorithm>
@@ -24,10 +25,10 @@
 namespace hbfb {
 namespace {
 
-constexpr u32 kScoreThreads = 256, kScorePerSm = 3;
+constexpr u32 kQueryWarps = 4;
+constexpr u32 kScoreWarps = 8;
 constexpr u32 kScoreShare = 32;      // blocks of a CTA at least
 constexpr u32 kHeldKeys = 32 * 1024; // 128 KB of keys
-constexpr u32 kMostQueryBytes = 200 * 1024;  // of shared memory, for the whole-number queries
 constexpr u32 kAbsent = 0u;           // key of a block that cannot be listed
 constexpr u32 kAlways = 0xffffffffu;  // key of a block that is always listed
 
@@ -35,7 +36,8 @@ struct SelectArgs {
     KvView c;
     KvQuery q;
     u32 top, sink, recent;
-    u32* keys;  // [seqs][tokens][heads][width]
+    std::int8_t* whole;  // [seqs][heads][2 tokens][2 D]: high and low parts, down then up
+    u32* keys;           // [seqs][tokens][heads][width]
     int* blocks;
     int* counts;
 };
@@ -72,11 +74,6 @@ __device__ __forceinline__ u32 blocks_of_sequence(const SelectArgs& a, u32 seq)
                            a.q.tokens - 1, a.c.block);
 }
 
-// Bytes between the columns (token, high or low) of a head's whole-number
-// queries in shared memory: down then up, and padding that puts neighbouring
-// columns on different banks.
-HD constexpr u32 column_bytes(u32 dim) { return 2 * dim + 64; }
-
 __device__ __forceinline__ void mma16832(int (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 b1)
 {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -85,19 +82,81 @@ __device__ __forceinline__ void mma16832(int (&d)[4], u32 a0, u32 a1, u32 a2, u3
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// One warp per (sequence, token, head): the group's queries as whole numbers.
 template <int D>
-__global__ void __launch_bounds__(kScoreThreads, kScorePerSm) score_kernel(const SelectArgs a)
+__global__ void __launch_bounds__(kQueryWarps * 32) query_kernel(const SelectArgs a)
 {
-    constexpr u32 kChunks = D / 32;  // 16-byte pieces of a block's bounds per lane
-    constexpr u32 kColumn = column_bytes(D);
-    extern __shared__ __align__(16) std::int8_t whole[];  // [heads][2 tokens][kColumn]
+    constexpr int E = D / 32;  // channels of a lane
+    kv_let_next();
+    const u32 heads = a.c.heads, tokens = a.q.tokens, group = a.q.group, lane = threadIdx.x & 31u;
+    const u32 at = blockIdx.x * kQueryWarps + (threadIdx.x >> 5);
+    if (at >= a.q.seqs * tokens * heads) return;
+    const u32 h = at % heads, t = at / heads % tokens, seq = at / heads / tokens;
+    float most = 0.0f;
+#pragma unroll 4
+    for (u32 i = 0; i < group; ++i) {
+        float x[E];
+        query_at<E>(a.q, seq, t, h * group + i, lane * E, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) most = fmaxf(most, fabsf(x[e]));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    int x = 0;
+    frexpf(most, &x);
+    const float up_scale = kv_power(7 - max(x, -100));
+    int up[E], down[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) up[e] = down[e] = 0;
+#pragma unroll 4
+    for (u32 i = 0; i < group; ++i) {
+        float x[E];
+        query_at<E>(a.q, seq, t, h * group + i, lane * E, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float r = rintf(x[e] * up_scale);
+            const int qi = static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
+            up[e] += max(qi, 0);
+            down[e] += min(qi, 0);
+        }
+    }
+    // column 2 t: the high parts, 2 t + 1: the low ones
+    std::int8_t* to = a.whole + ((static_cast<u64>(seq) * heads + h) * 2 * tokens + 2 * t) * 2 * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        to[e] = static_cast<std::int8_t>(-(-down[e] >> 7));
+        to[2 * D + e] = static_cast<std::int8_t>(-(-down[e] & 127));
+        to[D + e] = static_cast<std::int8_t>(up[e] >> 7);
+        to[3 * D + e] = static_cast<std::int8_t>(up[e] & 127);
+    }
+}
+
+// A stage of a warp's ring: the bounds of 16 blocks (a block's 64-byte pieces
+// are exchanged in pairs by its number's last bit, against bank conflicts),
+// their scales and whether they are there.
+template <int D>
+constexpr u32 kScoreStage = 16 * 2 * D + 128;
+template <int D>
+constexpr u32 kScoreStages = D == 256 ? 2 : 3;
+template <int D>
+constexpr u32 kScoreSmem = kScoreWarps * kScoreStages<D> * kScoreStage<D>;
+// CTAs per SM by shared memory: about 200 KB of rings.
+HD constexpr u32 score_per_sm(u32 dim) { return dim == 64 ? 3 : dim == 128 ? 2 : 1; }
+
+template <int D>
+__global__ void __launch_bounds__(kScoreWarps * 32, score_per_sm(D)) score_kernel(const SelectArgs a)
+{
+    constexpr u32 kChunks = D / 32;  // 64-byte pieces of a block's bounds
+    constexpr u32 NS = kScoreStages<D>;
+    extern __shared__ __align__(128) u8 smem[];
     __shared__ u64 line;
     kv_let_next();
-    const u32 heads = a.c.heads, tokens = a.q.tokens, group = a.q.group;
-    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = kScoreThreads / 32;
+    const u32 heads = a.c.heads, tokens = a.q.tokens;
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
+    u8* ring = smem + warp * NS * kScoreStage<D>;
     // the line of all sequences' blocks, and this CTA's share of it
     u64 all = 0;
-    for (u32 s = threadIdx.x; s < a.q.seqs; s += kScoreThreads) all += blocks_of_sequence(a, s);
+    for (u32 s = threadIdx.x; s < a.q.seqs; s += kScoreWarps * 32) all += blocks_of_sequence(a, s);
 #pragma unroll
     for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     if (threadIdx.x == 0) line = 0;
@@ -107,10 +166,9 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm) score_kernel(const
     const u64 share = max(static_cast<u64>(kScoreShare), (line + gridDim.x - 1) / gridDim.x);
     u64 at = blockIdx.x * share;
     const u64 stop = min(at + share, line);
-    if (at >= stop) return;
     u32 seq = 0, have = 0;
     u64 begin = 0;
-    for (u32 base = 0; base < a.q.seqs; base += 32) {  // the sequence that holds `at`
+    for (u32 base = 0; at < stop && base < a.q.seqs; base += 32) {  // the sequence that holds `at`
         const u32 n = base + lane < a.q.seqs ? blocks_of_sequence(a, base + lane) : 0;
         u32 upto = n;
 #pragma unroll
@@ -128,124 +186,110 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm) score_kernel(const
         }
         begin += __shfl_sync(0xffffffffu, upto, 31);
     }
+    bool queries = false;  // whether query_kernel's results may be read
     for (; at < stop; begin += have, have = ++seq < a.q.seqs ? blocks_of_sequence(a, seq) : 0) {
         const u32 first = static_cast<u32>(at - begin);
         const u32 end = static_cast<u32>(min(stop - begin, static_cast<u64>(have)));
         if (first >= end) continue;
         at = begin + end;
         const int length = kv_length(a.q.lengths, seq, a.q.width, a.c.block);
-        __syncthreads();  // the queries of the sequence before are used
-        for (u32 th = warp; th < tokens * heads; th += warps) {
-            const u32 t = th / heads, h = th % heads;
-            constexpr int E = D / 32;  // channels of a lane
-            float most = 0.0f;
-#pragma unroll 4
-            for (u32 i = 0; i < group; ++i) {
-                float x[E];
-                query_at<E>(a.q, seq, t, h * group + i, lane * E, x);
-#pragma unroll
-                for (int e = 0; e < E; ++e) most = fmaxf(most, fabsf(x[e]));
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            int x = 0;
-            frexpf(most, &x);
-            const float up_scale = kv_power(7 - max(x, -100));
-            int up[E], down[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) up[e] = down[e] = 0;
-#pragma unroll 4
-            for (u32 i = 0; i < group; ++i) {
-                float x[E];
-                query_at<E>(a.q, seq, t, h * group + i, lane * E, x);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float r = rintf(x[e] * up_scale);
-                    const int qi = static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
-                    up[e] += max(qi, 0);
-                    down[e] += min(qi, 0);
-                }
-            }
-            // column 2 t: the high parts, 2 t + 1: the low ones; first down, then up
-            std::int8_t* to = whole + (h * 2 * tokens + 2 * t) * kColumn + lane * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                to[e] = static_cast<std::int8_t>(-(-down[e] >> 7));
-                to[kColumn + e] = static_cast<std::int8_t>(-(-down[e] & 127));
-                to[D + e] = static_cast<std::int8_t>(up[e] >> 7);
-                to[D + kColumn + e] = static_cast<std::int8_t>(up[e] & 127);
-            }
-        }
-        __syncthreads();
         const int* table = a.q.table + static_cast<i64>(seq) * a.q.table_stride;
-        const u32 g = lane >> 2, c = lane & 3u;
         // Tasks: 16 blocks of one head, heads first, by the warps in turn.
-        const u32 rows = (end - first + 15) / 16, skip_rows = warps / heads, skip_heads = warps % heads;
-        auto page_of = [&](u32 row, u32 more) {
-            const u32 j = first + row * 16 + g + more;
-            return row < rows && j < end ? kv_page(table, j, a.c.pages) : -1;
-        };
-        u32 row = warp / heads, h = warp % heads;
-        int next0 = page_of(row, 0), next1 = page_of(row, 8);
-        while (row < rows) {
-            const u32 j0 = first + row * 16 + g, j1 = j0 + 8, head = h;
-            const int page0 = next0, page1 = next1;
+        const u32 rows = (end - first + 15) / 16;
+        const u32 skip_rows = kScoreWarps / heads, skip_heads = kScoreWarps % heads;
+        auto advance = [&](u32& row, u32& h) {
             row += skip_rows;
             h += skip_heads;
             if (h >= heads) {
                 h -= heads;
                 ++row;
             }
-            uint4 x0[kChunks], x1[kChunks];
-            float scale0 = 0.0f, scale1 = 0.0f;
+        };
+        auto page_of = [&](u32 row) {  // of the task's block lane % 16
+            const u32 j = first + row * 16 + (lane & 15u);
+            return row < rows && j < end ? kv_page(table, j, a.c.pages) : -1;
+        };
+        u32 issue_row = warp / heads, issue_h = warp % heads;
+        int issue_page = page_of(issue_row);
+        auto issue = [&](u32 stage) {
+            const int page = issue_page;
+            const u32 row = issue_row, h = issue_h;
+            advance(issue_row, issue_h);
+            issue_page = page_of(issue_row);
+            if (row < rows) {
+                u8* to = ring + stage * kScoreStage<D>;
+                // 2 D bytes of a block: D / 8 lanes, 16 bytes each
+                constexpr u32 kLanes = D / 8 < 32 ? D / 8 : 32, kAtOnce = 32 / kLanes;
 #pragma unroll
-            for (u32 k = 0; k < kChunks; ++k) x0[k] = x1[k] = make_uint4(0, 0, 0, 0);
-            if (page0 >= 0) {
-                const u64 x = static_cast<u64>(page0) * heads + head;
-                const uint4* b = reinterpret_cast<const uint4*>(a.c.bounds + x * 2 * D) + c;
-#pragma unroll
-                for (u32 k = 0; k < kChunks; ++k) x0[k] = b[k * 4];
-                scale0 = a.c.scale[x * 2];
+                for (u32 r = 0; r < 16; r += kAtOnce) {
+                    const u32 block = r + lane / kLanes;
+                    const int from = __shfl_sync(0xffffffffu, page, block);
+                    if (from >= 0) {
+                        const std::int8_t* source =
+                            a.c.bounds + (static_cast<u64>(from) * heads + h) * 2 * D;
+                        const u32 piece = lane % kLanes;
+                        kv_copy16(to + block * 2 * D + ((piece >> 2) ^ (block & 1u)) * 64 + (piece & 3u) * 16,
+                                  source + piece * 16);
+                    }
+                }
+                if (lane < 16) {
+                    u32* notes = reinterpret_cast<u32*>(to + 16 * 2 * D);
+                    notes[16 + lane] = page >= 0;
+                    if (page >= 0) kv_copy4(notes + lane, a.c.scale + (static_cast<u64>(page) * heads + h) * 2);
+                }
             }
-            if (page1 >= 0) {
-                const u64 x = static_cast<u64>(page1) * heads + head;
-                const uint4* b = reinterpret_cast<const uint4*>(a.c.bounds + x * 2 * D) + c;
+            kv_copy_commit();
+        };
 #pragma unroll
-                for (u32 k = 0; k < kChunks; ++k) x1[k] = b[k * 4];
-                scale1 = a.c.scale[x * 2];
-            }
-            next0 = page_of(row, 0);
-            next1 = page_of(row, 8);
+        for (u32 i = 0; i + 1 < NS; ++i) issue(i);
+        if (!queries) kv_wait_before();
+        queries = true;
+        u32 stage = 0;
+        for (u32 row = warp / heads, h = warp % heads; row < rows; advance(row, h)) {
+            kv_copy_wait<NS - 2>();
+            __syncwarp();  // the stage is there, and every lane is done with the one before it
+            issue(stage == 0 ? NS - 1 : stage - 1);
+            const u8* tile = ring + stage * kScoreStage<D>;
+            stage = stage + 1 == NS ? 0 : stage + 1;
+            const u32* notes = reinterpret_cast<const u32*>(tile + 16 * 2 * D);
+            const u32 j0 = first + row * 16 + g;
             // four tokens at a time: column g is the high or low part of token t0 + g / 2
             for (u32 t0 = 0; t0 < tokens; t0 += 4) {
                 int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
                 const bool used = t0 + g / 2 < tokens;
-                const std::int8_t* column = whole + (head * 2 * tokens + 2 * t0 + g) * kColumn + c * 16;
+                const std::int8_t* column =
+                    a.whole + ((static_cast<u64>(seq) * heads + h) * 2 * tokens + 2 * t0 + g) * 2 * D + c * 16;
 #pragma unroll
                 for (u32 k = 0; k < kChunks; ++k) {
                     uint4 y = make_uint4(0, 0, 0, 0);
                     if (used) y = *reinterpret_cast<const uint4*>(column + k * 64);
-                    mma16832(s0, x0[k].x, x1[k].x, x0[k].y, x1[k].y, y.x, y.y);
-                    mma16832(s1, x0[k].z, x1[k].z, x0[k].w, x1[k].w, y.z, y.w);
+                    const u8* piece = tile + g * 2 * D + (k ^ (g & 1u)) * 64 + c * 16;
+                    const uint4 x0 = *reinterpret_cast<const uint4*>(piece);
+                    const uint4 x1 = *reinterpret_cast<const uint4*>(piece + 8 * 2 * D);
+                    mma16832(s0, x0.x, x1.x, x0.y, x1.y, y.x, y.y);
+                    mma16832(s1, x0.z, x1.z, x0.w, x1.w, y.z, y.w);
                 }
                 const u32 t = t0 + c;  // this lane's columns 2c and 2c + 1
                 if (t < tokens) {
                     const u32 mine = blocks_of_token(length, tokens, t, a.c.block);
-                    u32* keys = a.keys + ((static_cast<u64>(seq) * tokens + t) * heads + head) * a.q.width;
-                    auto put = [&](u32 j, int page, int sum, float scale) {
+                    u32* keys = a.keys + ((static_cast<u64>(seq) * tokens + t) * heads + h) * a.q.width;
+                    auto put = [&](u32 j, u32 note, int sum) {
                         u32 key = kAbsent;
-                        if (page >= 0 && j < mine)
+                        if (notes[16 + note] && j < mine)
                             key = j < a.sink || j + a.recent >= mine
                                       ? kAlways
-                                      : order_key(__fmul_rn(__int2float_rn(sum), scale));
+                                      : order_key(__fmul_rn(__int2float_rn(sum), __uint_as_float(notes[note])));
                         if (j < end) keys[j] = key;
                     };
-                    put(j0, page0, (s0[0] + s1[0]) * 128 + s0[1] + s1[1], scale0);
-                    put(j1, page1, (s0[2] + s1[2]) * 128 + s0[3] + s1[3], scale1);
+                    put(j0, g, (s0[0] + s1[0]) * 128 + s0[1] + s1[1]);
+                    put(j0 + 8, g + 8, (s0[2] + s1[2]) * 128 + s0[3] + s1[3]);
                 }
             }
         }
+        kv_copy_wait<0>();
+        __syncwarp();  // before the next sequence's copies
     }
+    if (!queries) kv_wait_before();  // list_kernel waits for this kernel alone
 }
 
 // `slice`: blocks of a row that one CTA of the team has.
@@ -332,23 +376,32 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
     kv_team_sync(team);  // nobody leaves while another may read its counts
 }
 
+u64 whole_bytes(const KvView& v, const KvQuery& q)
+{
+    return kv_round_up(static_cast<u64>(q.seqs) * v.heads * 2 * q.tokens * 2 * v.dim, 256);
+}
+
 u64 workspace_bytes_of(const KvView& v, const KvQuery& q)
 {
-    return kv_round_up(static_cast<u64>(q.seqs) * q.tokens * v.heads * q.width * 4, 256);
+    return whole_bytes(v, q) +
+           kv_round_up(static_cast<u64>(q.seqs) * q.tokens * v.heads * q.width * 4, 256);
 }
 
 template <int D>
 int launch(const SelectArgs& a, cudaStream_t s)
 {
-    const u32 smem = a.q.tokens * a.c.heads * 2 * column_bytes(D);
     static std::atomic<u64> seen{0};
-    if (!kv_allow_smem(score_kernel<D>, kMostQueryBytes, seen)) return HBFSIM_CUDA_ERROR;
-    const u64 most = (static_cast<u64>(a.q.seqs) * a.q.width + kScoreShare - 1) / kScoreShare;
-    const u32 grid = static_cast<u32>(std::min<u64>(most, static_cast<u64>(kScorePerSm) * kv_sm_count()));
-    if (grid) score_kernel<D><<<grid, kScoreThreads, smem, s>>>(a);
+    if (!kv_allow_smem(score_kernel<D>, kScoreSmem<D>, seen)) return HBFSIM_CUDA_ERROR;
+    const u32 rows = a.q.seqs * a.q.tokens * a.c.heads;
+    bool ok = true;
+    if (a.q.width) {
+        query_kernel<D><<<(rows + kQueryWarps - 1) / kQueryWarps, kQueryWarps * 32, 0, s>>>(a);
+        const u64 most = (static_cast<u64>(a.q.seqs) * a.q.width + kScoreShare - 1) / kScoreShare;
+        const u32 grid = static_cast<u32>(std::min<u64>(most, static_cast<u64>(score_per_sm(D)) * kv_sm_count()));
+        ok = kv_launch_behind(score_kernel<D>, dim3(grid), kScoreWarps * 32, s, kScoreSmem<D>, 1, a);
+    }
     static std::atomic<u64> seen_list{0};
     if (!kv_allow_smem(list_kernel, kHeldKeys * 4, seen_list)) return HBFSIM_CUDA_ERROR;
-    const u32 rows = a.q.seqs * a.q.tokens * a.c.heads;
     u32 team = kv_team_size(rows, a.q.width), slice = (a.q.width + team - 1) / team;
     if (slice > kHeldKeys) {  // a row that no team can hold is one CTA's
         team = 1;
@@ -357,8 +410,8 @@ int launch(const SelectArgs& a, cudaStream_t s)
     // many rows: small CTAs, several to an SM
     u32 threads = kv_team_threads(slice);
     if (rows > 2 * static_cast<u32>(kv_sm_count())) threads = std::min(threads, 256u);
-    const bool ok = kv_launch_behind(list_kernel, dim3(rows * team), threads, s,
-                                     slice <= kHeldKeys ? slice * 4 : 0, team, a, team, slice);
+    ok = kv_launch_behind(list_kernel, dim3(rows * team), threads, s,
+                          slice <= kHeldKeys ? slice * 4 : 0, team, a, team, slice) && ok;
     return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
@@ -389,9 +442,6 @@ extern "C" int hbfsim_kv_select_v1(const hbfsim_kv_cache_v1* cache,
         return HBFSIM_INVALID_ARGUMENT;
     const u64 lists = static_cast<u64>(a.q.seqs) * a.q.tokens * a.c.heads;
     if (lists == 0) return HBFSIM_OK;
-    // shared memory of the whole-number queries
-    if (static_cast<u64>(a.q.tokens) * a.c.heads * 2 * column_bytes(a.c.dim) > kMostQueryBytes)
-        return HBFSIM_UNSUPPORTED;
     if (!blocks || !counts) return HBFSIM_INVALID_ARGUMENT;
     if (workspace_bytes < workspace_bytes_of(a.c, a.q) || (a.q.width && !workspace) ||
         !kv_aligned(workspace, 16) || !kv_aligned(blocks, 4) || !kv_aligned(counts, 4))
@@ -399,7 +449,8 @@ extern "C" int hbfsim_kv_select_v1(const hbfsim_kv_cache_v1* cache,
     a.top = top;
     a.sink = sink;
     a.recent = recent;
-    a.keys = static_cast<u32*>(workspace);
+    a.whole = static_cast<std::int8_t*>(workspace);
+    a.keys = reinterpret_cast<u32*>(static_cast<u8*>(workspace) + whole_bytes(a.c, a.q));
     a.blocks = blocks;
     a.counts = counts;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
