@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, score_per_sm(D)) score_kerne
     const u32 heads = a.c.heads, tokens = a.q.tokens;
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
     u8* ring = smem + warp * NS * kScoreStage<D>;
+    const u32 page_bytes = heads * 2 * D, page_scales = heads * 2;
     // the line of all sequences' blocks, and this CTA's share of it
     u64 all = 0;
     for (u32 s = threadIdx.x; s < a.q.seqs; s += kScoreWarps * 32) all += blocks_of_sequence(a, s);
@@ -211,6 +212,9 @@ __global__ void __launch_bounds__(kScoreWarps * 32, score_per_sm(D)) score_kerne
         };
         u32 issue_row = warp / heads, issue_h = warp % heads;
         int issue_page = page_of(issue_row);
+        // 2 D bytes of a block: D / 8 lanes, 16 bytes each
+        constexpr u32 kLanes = D / 8, kAtOnce = 32 / kLanes;
+        const u32 block_at = lane / kLanes, piece = lane % kLanes;
         auto issue = [&](u32 stage) {
             const int page = issue_page;
             const u32 row = issue_row, h = issue_h;
@@ -218,24 +222,21 @@ __global__ void __launch_bounds__(kScoreWarps * 32, score_per_sm(D)) score_kerne
             issue_page = page_of(issue_row);
             if (row < rows) {
                 u8* to = ring + stage * kScoreStage<D>;
-                // 2 D bytes of a block: D / 8 lanes, 16 bytes each
-                constexpr u32 kLanes = D / 8 < 32 ? D / 8 : 32, kAtOnce = 32 / kLanes;
+                // a block that is not there is noted; its copy takes some page's bounds
+                const u32 real = static_cast<u32>(max(page, 0));
+                const u64 source = reinterpret_cast<u64>(a.c.bounds) + h * 2 * D + static_cast<u64>(real) * page_bytes;
+                const u32 even = kv_shared(to) + block_at * 2 * D + ((piece >> 2) ^ (block_at & 1u)) * 64 + (piece & 3u) * 16;
 #pragma unroll
                 for (u32 r = 0; r < 16; r += kAtOnce) {
-                    const u32 block = r + lane / kLanes;
-                    const int from = __shfl_sync(0xffffffffu, page, block);
-                    if (from >= 0) {
-                        const std::int8_t* source =
-                            a.c.bounds + (static_cast<u64>(from) * heads + h) * 2 * D;
-                        const u32 piece = lane % kLanes;
-                        kv_copy16(to + block * 2 * D + ((piece >> 2) ^ (block & 1u)) * 64 + (piece & 3u) * 16,
-                                  source + piece * 16);
-                    }
+                    const u64 from = __shfl_sync(0xffffffffu, source, r + block_at) + piece * 16;
+                    // one block at once: the pieces of odd blocks are exchanged
+                    const u32 odd = kAtOnce == 1 && (r & 1u) ? 64u : 0u;
+                    kv_copy16((even ^ odd) + r * 2 * D, reinterpret_cast<const void*>(from));
                 }
                 if (lane < 16) {
                     u32* notes = reinterpret_cast<u32*>(to + 16 * 2 * D);
                     notes[16 + lane] = page >= 0;
-                    if (page >= 0) kv_copy4(notes + lane, a.c.scale + (static_cast<u64>(page) * heads + h) * 2);
+                    kv_copy4(notes + lane, a.c.scale + h * 2 + static_cast<u64>(real) * page_scales);
                 }
             }
             kv_copy_commit();
@@ -244,7 +245,20 @@ __global__ void __launch_bounds__(kScoreWarps * 32, score_per_sm(D)) score_kerne
         for (u32 i = 0; i + 1 < NS; ++i) issue(i);
         if (!queries) kv_wait_before();
         queries = true;
-        u32 stage = 0;
+        // Column g of a group of four tokens is the high or low part of token t0 + g / 2.  The
+        // first group's stays in registers for as long as the warp's head does.
+        const std::int8_t* columns = a.whole + static_cast<u64>(seq) * heads * 2 * tokens * 2 * D;
+        auto column_of = [&](u32 h, u32 t0, uint4 (&y)[kChunks]) {
+            const bool used = t0 + g / 2 < tokens;
+            const std::int8_t* column = columns + (static_cast<u64>(h) * 2 * tokens + 2 * t0 + g) * 2 * D + c * 16;
+#pragma unroll
+            for (u32 k = 0; k < kChunks; ++k) {
+                y[k] = make_uint4(0, 0, 0, 0);
+                if (used) y[k] = *reinterpret_cast<const uint4*>(column + k * 64);
+            }
+        };
+        uint4 y[kChunks];
+        u32 y_head = heads, stage = 0;
         for (u32 row = warp / heads, h = warp % heads; row < rows; advance(row, h)) {
             kv_copy_wait<NS - 2>();
             __syncwarp();  // the stage is there, and every lane is done with the one before it
@@ -253,36 +267,38 @@ __global__ void __launch_bounds__(kScoreWarps * 32, score_per_sm(D)) score_kerne
             stage = stage + 1 == NS ? 0 : stage + 1;
             const u32* notes = reinterpret_cast<const u32*>(tile + 16 * 2 * D);
             const u32 j0 = first + row * 16 + g;
-            // four tokens at a time: column g is the high or low part of token t0 + g / 2
+            const bool there0 = notes[16 + g] != 0, there1 = notes[24 + g] != 0;
+            const float scale0 = __uint_as_float(notes[g]), scale1 = __uint_as_float(notes[8 + g]);
+            const u8* even = tile + g * 2 * D + (g & 1u) * 64 + c * 16;  // pieces 0, 2, ..
+            const u8* odd = tile + g * 2 * D + (~g & 1u) * 64 + c * 16;  // pieces 1, 3, ..
+            u32* keys = a.keys + (static_cast<u64>(seq) * tokens * heads + h) * a.q.width + j0;
             for (u32 t0 = 0; t0 < tokens; t0 += 4) {
+                if (t0 || y_head != h) {
+                    column_of(h, t0, y);
+                    y_head = tokens <= 4 ? h : heads;
+                }
                 int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
-                const bool used = t0 + g / 2 < tokens;
-                const std::int8_t* column =
-                    a.whole + ((static_cast<u64>(seq) * heads + h) * 2 * tokens + 2 * t0 + g) * 2 * D + c * 16;
 #pragma unroll
                 for (u32 k = 0; k < kChunks; ++k) {
-                    uint4 y = make_uint4(0, 0, 0, 0);
-                    if (used) y = *reinterpret_cast<const uint4*>(column + k * 64);
-                    const u8* piece = tile + g * 2 * D + (k ^ (g & 1u)) * 64 + c * 16;
-                    const uint4 x0 = *reinterpret_cast<const uint4*>(piece);
-                    const uint4 x1 = *reinterpret_cast<const uint4*>(piece + 8 * 2 * D);
-                    mma16832(s0, x0.x, x1.x, x0.y, x1.y, y.x, y.y);
-                    mma16832(s1, x0.z, x1.z, x0.w, x1.w, y.z, y.w);
+                    const u8* at_piece = (k & 1u ? odd : even) + (k & ~1u) * 64;
+                    const uint4 x0 = *reinterpret_cast<const uint4*>(at_piece);
+                    const uint4 x1 = *reinterpret_cast<const uint4*>(at_piece + 8 * 2 * D);
+                    mma16832(s0, x0.x, x1.x, x0.y, x1.y, y[k].x, y[k].y);
+                    mma16832(s1, x0.z, x1.z, x0.w, x1.w, y[k].z, y[k].w);
                 }
                 const u32 t = t0 + c;  // this lane's columns 2c and 2c + 1
                 if (t < tokens) {
                     const u32 mine = blocks_of_token(length, tokens, t, a.c.block);
-                    u32* keys = a.keys + ((static_cast<u64>(seq) * tokens + t) * heads + h) * a.q.width;
-                    auto put = [&](u32 j, u32 note, int sum) {
-                        u32 key = kAbsent;
-                        if (notes[16 + note] && j < mine)
-                            key = j < a.sink || j + a.recent >= mine
-                                      ? kAlways
-                                      : order_key(__fmul_rn(__int2float_rn(sum), __uint_as_float(notes[note])));
-                        if (j < end) keys[j] = key;
+                    u32* to = keys + static_cast<u64>(t) * heads * a.q.width;
+                    auto put = [&](u32 more, bool there, float scale, int sum) {
+                        const u32 j = j0 + more;
+                        u32 key = order_key(__fmul_rn(__int2float_rn(sum), scale));
+                        if (j < a.sink || j + a.recent >= mine) key = kAlways;
+                        if (!there || j >= mine) key = kAbsent;
+                        if (j < end) to[more] = key;
                     };
-                    put(j0, g, (s0[0] + s1[0]) * 128 + s0[1] + s1[1]);
-                    put(j0 + 8, g + 8, (s0[2] + s1[2]) * 128 + s0[3] + s1[3]);
+                    put(0, there0, scale0, (s0[0] + s1[0]) * 128 + s0[1] + s1[1]);
+                    put(8, there1, scale1, (s0[2] + s1[2]) * 128 + s0[3] + s1[3]);
                 }
             }
         }
