@@ -124,12 +124,12 @@ inline bool kv_allow_smem(Kernel* kernel, u32 bytes, std::atomic<u64>& seen)
 }
 
 // CTAs to a row of `width` keys: a power of two up to kKvTeam, as long as
-// every CTA gets an SM of its own and at least 1024 keys.
+// every CTA gets an SM of its own and at least 2048 keys.
 inline u32 kv_team_size(u64 rows, u32 width)
 {
     u32 size = 1;
     while (size < kKvTeam && rows * size * 2 <= static_cast<u64>(kv_sm_count()) &&
-           width / (size * 2) >= 1024)
+           width / (size * 2) >= 2048)
         size *= 2;
     return size;
 }
@@ -288,9 +288,13 @@ struct KvSelectShared {
     u32 group[kKvBins / 32];  // sums of 32 counts
     u32 words[kKvWords];
     u32 warp_sums[33];
-    u32 found[3];
+    u32 found[3];             // bin, keys below it, keys in it
     u32 counts[2], in_front;
     u64 range[32][2], team_range[2];  // least and greatest key of the warps, of the CTA
+    u32 tally[32][2], team_tally[2];  // the caller's two counts, likewise
+    u64 few[32];              // the last candidates
+    u32 few_count, few_equals;
+    u64 few_limit;
 };
 constexpr u32 kKvAll = 0xffffffffu;
 
@@ -335,84 +339,114 @@ __device__ __forceinline__ u32 kv_team_sum(const u32* mine, u32 ranks)
 __device__ __forceinline__ int kv_top_bit(u32 x) { return 31 - __clz(static_cast<int>(x)); }
 __device__ __forceinline__ int kv_top_bit(u64 x) { return 63 - __clzll(static_cast<long long>(x)); }
 
-// Threshold of the `rank` smallest (rank >= 1) among the keys of the team
-// that `key_at(i, k)` admits, i = 0..n-1 in each CTA: those below `limit` and
-// `equals` of those at it (kKvAll: all of them).  Each pass spreads the keys
-// of the range at hand over bins and goes on with the bin that holds the
-// rank.  The bins of the first pass grow with the distance from the least
-// key (32 to an octave), so that sizes of many orders do not crowd a few
-// counters; the 2048 of later passes are equal.  Two passes are the rule;
-// 64-bit keys take 7 at most.  `least` and `greatest` are this thread's of
-// the keys (~0 and 0 without one).  All threads of the team call it.
-template <typename Key, typename KeyAt>
-__device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Key greatest,
-                              KeyAt key_at, KvSelectShared& sm, Key& limit, u32& equals)
+// What the team's threads found when they went over the keys: the least and
+// greatest key (~0 and 0 without one) and two counts.  Clears the bins too.
+template <typename Key>
+__device__ void kv_gather(const KvTeam& team, KvSelectShared& sm, Key& least, Key& greatest, u32& tally0,
+                          u32& tally1)
 {
-    const u32 lane = threadIdx.x & 31u;
-    Key lo = least, hi = greatest;
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     auto reduce = [&]() {
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
-            lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+            greatest = max(greatest, __shfl_xor_sync(0xffffffffu, greatest, o));
         }
+        tally0 = __reduce_add_sync(0xffffffffu, tally0);
+        tally1 = __reduce_add_sync(0xffffffffu, tally1);
     };
     reduce();
     if (lane == 0) {
-        sm.range[threadIdx.x >> 5][0] = lo;
-        sm.range[threadIdx.x >> 5][1] = hi;
+        sm.range[warp][0] = least;
+        sm.range[warp][1] = greatest;
+        sm.tally[warp][0] = tally0;
+        sm.tally[warp][1] = tally1;
+    }
+    for (u32 i = threadIdx.x; i < kKvBins; i += blockDim.x) sm.histogram[i] = 0;
+    __syncthreads();
+    const bool in = lane < blockDim.x >> 5;  // every warp for itself
+    least = in ? static_cast<Key>(sm.range[lane][0]) : static_cast<Key>(~Key{0});
+    greatest = in ? static_cast<Key>(sm.range[lane][1]) : Key{0};
+    tally0 = in ? sm.tally[lane][0] : 0;
+    tally1 = in ? sm.tally[lane][1] : 0;
+    reduce();
+    if (team.size == 1) return;
+    if (threadIdx.x == 0) {
+        sm.team_range[0] = least;
+        sm.team_range[1] = greatest;
+        sm.team_tally[0] = tally0;
+        sm.team_tally[1] = tally1;
+    }
+    kv_team_sync(team);
+    if (warp == 0) {  // one warp asks the other CTAs
+        const bool ask = lane < team.size;
+        least = ask ? static_cast<Key>(kv_peek(&sm.team_range[0], lane)) : static_cast<Key>(~Key{0});
+        greatest = ask ? static_cast<Key>(kv_peek(&sm.team_range[1], lane)) : Key{0};
+        tally0 = ask ? kv_peek(&sm.team_tally[0], lane) : 0;
+        tally1 = ask ? kv_peek(&sm.team_tally[1], lane) : 0;
+        reduce();
+        if (lane == 0) {
+            sm.range[0][0] = least;
+            sm.range[0][1] = greatest;
+            sm.tally[0][0] = tally0;
+            sm.tally[0][1] = tally1;
+        }
     }
     __syncthreads();
-    lo = ~Key{0};
-    hi = 0;
-    if (lane < blockDim.x >> 5) {
-        lo = static_cast<Key>(sm.range[lane][0]);
-        hi = static_cast<Key>(sm.range[lane][1]);
-    }
-    reduce();
-    if (team.size > 1) {
-        if (threadIdx.x == 0) {
-            sm.team_range[0] = lo;
-            sm.team_range[1] = hi;
-        }
-        kv_team_sync(team);
-        if (threadIdx.x < 32) {  // one warp asks the others' CTAs
-            if (lane < team.size) {
-                lo = static_cast<Key>(kv_peek(&sm.team_range[0], lane));
-                hi = static_cast<Key>(kv_peek(&sm.team_range[1], lane));
-            }
-            reduce();
-            if (lane == 0) {
-                sm.range[0][0] = lo;
-                sm.range[0][1] = hi;
-            }
-        }
-        __syncthreads();
-        lo = static_cast<Key>(sm.range[0][0]);
-        hi = static_cast<Key>(sm.range[0][1]);
-    }
-    bool octaves = true;
-    for (;;) {
+    least = static_cast<Key>(sm.range[0][0]);
+    greatest = static_cast<Key>(sm.range[0][1]);
+    tally0 = sm.tally[0][0];
+    tally1 = sm.tally[0][1];
+}
+
+// Threshold of the `rank` smallest (rank >= 1) among the keys of the team
+// that `key_at(i, k)` admits, i = 0..n-1 in each CTA, all in [lo, hi] (from
+// kv_gather, which also cleared the bins): those below `limit` and `equals`
+// of those at it (kKvAll: all of them).  Each pass spreads the keys of the
+// range at hand over bins and goes on with the bin that holds the rank, until
+// a warp can order what is in it.  The bins of the first pass grow with the
+// distance from the least key (32 to an octave), so that sizes of many orders
+// do not crowd a few counters; the 2048 of later passes are equal.  One pass
+// is the rule for a few thousand keys; 64-bit keys take 7 at most.  All
+// threads of the team call it.
+template <typename Key, typename KeyAt>
+__device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key lo, Key hi, KeyAt key_at,
+                              KvSelectShared& sm, Key& limit, u32& equals)
+{
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (bool octaves = true;; octaves = false) {
         if (lo >= hi) {  // one value is left
             limit = lo;
             equals = rank;
             return;
         }
         const int shift = max(0, kv_top_bit(static_cast<Key>(hi - lo)) + 1 - 11);
-        auto bin_of = [&](Key d) -> u32 {
-            if (!octaves) return static_cast<u32>(d >> shift);
+        auto octave_bin = [](Key d) -> u32 {
             if (d < 32) return static_cast<u32>(d);
             const int top = kv_top_bit(d);  // 5 bits below the top one
-            return static_cast<u32>((top - 4) * 32) + (static_cast<u32>(d >> (top - 5)) & 31u);
+            return static_cast<u32>((top - 5) * 32) + static_cast<u32>(d >> (top - 5));
         };
-        for (u32 i = threadIdx.x; i < kKvBins; i += blockDim.x) sm.histogram[i] = 0;
-        __syncthreads();
+        if (!octaves) {
+            for (u32 i = threadIdx.x; i < kKvBins; i += blockDim.x) sm.histogram[i] = 0;
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) sm.few_count = 0;
         u32 at_lo = 0;  // keys at `lo` (blocks of no weight, say) would crowd one counter
-        for (u32 i = threadIdx.x; i < n; i += blockDim.x) {
-            Key k;
-            if (!key_at(i, k) || k < lo || k > hi) continue;
-            if (k == lo) ++at_lo;
-            else atomicAdd(&sm.histogram[bin_of(k - lo)], 1u);
+        if (octaves) {
+#pragma unroll 4
+            for (u32 i = threadIdx.x; i < n; i += blockDim.x) {
+                Key k;
+                if (!key_at(i, k)) continue;
+                if (k == lo) ++at_lo;
+                else atomicAdd(&sm.histogram[octave_bin(static_cast<Key>(k - lo))], 1u);
+            }
+        } else {
+            for (u32 i = threadIdx.x; i < n; i += blockDim.x) {
+                Key k;
+                if (!key_at(i, k) || k < lo || k > hi) continue;
+                if (k == lo) ++at_lo;
+                else atomicAdd(&sm.histogram[static_cast<u32>((k - lo) >> shift)], 1u);
+            }
         }
         at_lo = __reduce_add_sync(0xffffffffu, at_lo);
         if (lane == 0 && at_lo) atomicAdd(&sm.histogram[0], at_lo);
@@ -421,7 +455,15 @@ __device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Ke
             const u32 each = kKvBins / blockDim.x, from = threadIdx.x * each;  // 2 to 16 bins a thread
             u32 sum = 0;
             for (u32 t = 0; t < each; ++t) sum += sm.histogram[from + t];
-            const u32 upto = kv_block_scan(sum, sm.warp_sums);
+            u32 upto = sum;
+#pragma unroll
+            for (u32 o = 1; o < 32; o <<= 1) {
+                const u32 y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            if (lane == 31) sm.warp_sums[warp] = upto;
+            __syncthreads();
+            upto += __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_sums[lane] : 0);
             u32 before = upto - sum;
             if (before < rank && rank <= upto) {
                 u32 t = from;
@@ -433,13 +475,12 @@ __device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Ke
         } else {
             // Words of other CTAs are dear: first the sums of 32 bins each, then the 32 bins of
             // the group that holds the rank, by one warp.
-            const u32 warps = blockDim.x >> 5;
-            for (u32 w = threadIdx.x >> 5; w < kKvBins / 32; w += warps) {
+            for (u32 w = warp; w < kKvBins / 32; w += warps) {
                 const u32 sum = __reduce_add_sync(0xffffffffu, sm.histogram[w * 32 + lane]);
                 if (lane == 0) sm.group[w] = sum;
             }
             kv_team_sync(team);
-            if (threadIdx.x < 32) {
+            if (warp == 0) {
                 u32 before = 0, at = 0;
                 // place of the rank among 32 counts, one per lane, each the team's sum
                 auto narrow = [&](const u32* mine) -> bool {
@@ -483,12 +524,51 @@ __device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Ke
             lo += static_cast<Key>(bin) << width;
         }
         hi = min(hi, static_cast<Key>(lo + ((Key{1} << width) - 1)));
-        octaves = false;
         if (rank == count) {  // the whole bin
             limit = hi;
             equals = kKvAll;
             return;
         }
+        if (count > 32) continue;
+        // The bin's keys, one per lane, each ordered by how many are below it.
+        for (u32 i = threadIdx.x; i < n; i += blockDim.x) {
+            Key k;
+            if (key_at(i, k) && k >= lo && k <= hi) sm.few[atomicAdd(&sm.few_count, 1u) & 31u] = k;
+        }
+        kv_team_sync(team);
+        if (team.size == 1 || warp == 0) {  // every warp for itself, or one that asks the others
+            Key k = static_cast<Key>(sm.few[lane]);
+            if (team.size > 1) {
+                u32 upto = 0;
+                for (u32 r = 0; r < team.size; ++r) {
+                    const u32 its = kv_peek(&sm.few_count, r);
+                    if (lane >= upto && lane < upto + its) k = static_cast<Key>(kv_peek(&sm.few[lane - upto], r));
+                    upto += its;
+                }
+            }
+            u32 below = 0, same = 0;
+            for (u32 x = 0; x < count; ++x) {
+                const Key other = __shfl_sync(0xffffffffu, k, x);
+                below += other < k;
+                same += other == k;
+            }
+            const bool it = lane < count && below < rank && rank <= below + same;
+            const u32 who = __ballot_sync(0xffffffffu, it);
+            const int one = who ? __ffs(who) - 1 : 0;
+            limit = __shfl_sync(0xffffffffu, k, one);
+            equals = rank - __shfl_sync(0xffffffffu, below, one);
+            if (equals == __shfl_sync(0xffffffffu, same, one)) equals = kKvAll;
+            if (lane == 0 && team.size > 1) {
+                sm.few_limit = limit;
+                sm.few_equals = equals;
+            }
+        }
+        if (team.size > 1) {
+            __syncthreads();
+            limit = static_cast<Key>(sm.few_limit);
+            equals = sm.few_equals;
+        }
+        return;
     }
 }
 
@@ -499,7 +579,7 @@ __device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key least, Ke
 // came before), with a block barrier between them if kBarrier (stores may
 // reach what a load of the same round reads).  Counts come from ballots, one
 // word per 32 elements, and one block-wide scan per 32768 elements.
-template <bool kBarrier, typename State, typename Load, typename Store>
+template <bool kBarrier, bool kChosen, typename State, typename Load, typename Store>
 __device__ void kv_walk(const KvTeam& team, u32 n, u32 equals, KvSelectShared& sm, State state,
                         Load load, Store store)
 {
@@ -511,24 +591,39 @@ __device__ void kv_walk(const KvTeam& team, u32 n, u32 equals, KvSelectShared& s
     // what the ones in front counted to before[which].
     auto scan_words = [&](u32 many, int which) {
         u32 carry = 0;
-        for (u32 base = 0; base < many; base += blockDim.x) {
-            const u32 w = base + threadIdx.x;
-            const u32 bits = w < many ? __popc(sm.words[w]) : 0;
-            const u32 upto = kv_block_scan(bits, sm.warp_sums);
-            if (w < many) prefix[w] = carry + upto - bits;
-            carry += sm.warp_sums[32];
+        if (many <= 128) {  // every warp for itself: they write the same
+            for (u32 base = 0; base < many; base += 32) {
+                const u32 w = base + lane, bits = w < many ? __popc(sm.words[w]) : 0;
+                u32 upto = bits;
+#pragma unroll
+                for (u32 o = 1; o < 32; o <<= 1) {
+                    const u32 y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                if (w < many) prefix[w] = carry + upto - bits;
+                carry += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            __syncwarp();
+        } else {
+            for (u32 base = 0; base < many; base += blockDim.x) {
+                const u32 w = base + threadIdx.x;
+                const u32 bits = w < many ? __popc(sm.words[w]) : 0;
+                const u32 upto = kv_block_scan(bits, sm.warp_sums);
+                if (w < many) prefix[w] = carry + upto - bits;
+                carry += sm.warp_sums[32];
+            }
+            __syncthreads();
         }
         if (team.size > 1) {
             if (threadIdx.x == 0) sm.counts[which] = carry;
             kv_team_sync(team);
-            if (threadIdx.x < 32) {
+            if (warp == 0) {
                 const u32 sum = kv_team_sum(&sm.counts[which], team.rank);
                 if (lane == 0) sm.in_front = sum;
             }
             __syncthreads();
             before[which] += sm.in_front;
         }
-        __syncthreads();
         return carry;
     };
     u32 first = 0;
@@ -544,7 +639,8 @@ __device__ void kv_walk(const KvTeam& team, u32 n, u32 equals, KvSelectShared& s
             }
             __syncthreads();
             const u32 all = scan_words(words, 1);
-            // from here on the words hold what is chosen; a warp reads and writes its own words
+            __syncthreads();  // every warp has read the words
+            // from here on they hold what is chosen; a warp reads and writes its own words
             for (u32 r = 0; r < rounds; ++r) {
                 const u32 w = r * warps + warp, i = w * 32 + lane;
                 const u32 eq = w < words ? sm.words[w] : 0;
@@ -562,15 +658,21 @@ __device__ void kv_walk(const KvTeam& team, u32 n, u32 equals, KvSelectShared& s
             }
         }
         __syncthreads();
+        // (the prefix sums in use above are read: a barrier lies behind)
         const u32 all = scan_words(words, 0);
         for (u32 r = 0; r < rounds; ++r) {
             const u32 w = r * warps + warp, i = w * 32 + lane;
             const bool in = i < many;
+            if constexpr (kChosen && !kBarrier) {
+                if (w >= words || sm.words[w] == 0) continue;  // a warp at once
+            }
             auto value = load(first + (in ? i : 0));
             if constexpr (kBarrier) __syncthreads();
             if (in) {
                 const u32 m = sm.words[w];
-                store(first + i, value, (m >> lane & 1u) != 0, before[0] + prefix[w] + __popc(m & under));
+                const bool chosen = (m >> lane & 1u) != 0;
+                if (!kChosen || chosen)
+                    store(first + i, value, chosen, before[0] + prefix[w] + __popc(m & under));
             }
         }
         before[0] += all;

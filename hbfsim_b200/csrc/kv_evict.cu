@@ -89,7 +89,8 @@ __global__ void __launch_bounds__(1024) evict_kernel(const EvictArgs a, u32 team
         if (j >= leave) freed[j] = -1;
     }
     if (leave == 0) return;
-    __syncthreads();
+    u32 none0 = 0, none1 = 0;
+    kv_gather(team, sm, least, greatest, none0, none1);
     // the score of the last block to leave, and how many of its equals do
     u64 limit;
     u32 equals;
@@ -119,8 +120,8 @@ __global__ void __launch_bounds__(1024) evict_kernel(const EvictArgs a, u32 team
             table_out[first + i - gone_before] = e.page;
         }
     };
-    if (hold) kv_walk<false>(team, mine, equals, sm, state, load, store);
-    else kv_walk<true>(team, mine, equals, sm, state, load, store);
+    if (hold) kv_walk<false, false>(team, mine, equals, sm, state, load, store);
+    else kv_walk<true, false>(team, mine, equals, sm, state, load, store);
     kv_team_sync(team);  // nobody leaves while another may read its counts
     if (!hold)  // what lies behind the survivors was needed until now
         for (u32 j = blocks - leave + threadIdx.x; j < blocks; j += blockDim.x) score_out[j] = 0;

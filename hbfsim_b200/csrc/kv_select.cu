@@ -313,7 +313,6 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
 {
     extern __shared__ __align__(16) u32 held[];
     __shared__ KvSelectShared sm;
-    __shared__ u32 counted[4];  // blocks that are there, those always listed; the team's
     kv_wait_before();
     const KvTeam team{blockIdx.x % team_size, team_size};
     const u64 at = blockIdx.x / team_size;  // (sequence, token, head)
@@ -326,9 +325,8 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
     const bool hold = slice <= kHeldKeys;
     const u32* keys = hold ? held : row;
     int* list = a.blocks + at * a.top;
-    if (threadIdx.x < 2) counted[threadIdx.x] = 0;
-    __syncthreads();
-    u32 there = 0, always = 0, least = ~0u, greatest = 0;
+    u32 there = 0, always = 0;  // blocks that are there, and those always listed
+    u32 least = ~0u, greatest = 0;
 #pragma unroll 8
     for (u32 i = threadIdx.x; i < mine; i += blockDim.x) {
         const u32 k = row[i];
@@ -340,25 +338,7 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
             greatest = max(greatest, ~k);
         }
     }
-    there = __reduce_add_sync(0xffffffffu, there);
-    always = __reduce_add_sync(0xffffffffu, always);
-    if ((threadIdx.x & 31u) == 0) {
-        atomicAdd(&counted[0], there);
-        atomicAdd(&counted[1], always);
-    }
-    kv_team_sync(team);
-    if (team.size > 1) {
-        if (threadIdx.x < 32) {
-            const u32 all = kv_team_sum(&counted[0], team.size), all_always = kv_team_sum(&counted[1], team.size);
-            if (threadIdx.x == 0) {
-                counted[2] = all;
-                counted[3] = all_always;
-            }
-        }
-        __syncthreads();
-    }
-    there = counted[team.size > 1 ? 2 : 0];
-    always = counted[team.size > 1 ? 3 : 1];
+    kv_gather(team, sm, least, greatest, there, always);
     const u32 take = min(a.top, there);
     // the greatest keys are the smallest of their complements; those always listed need no rank
     u32 limit = 0xffffffffu, equals = kKvAll;
@@ -374,7 +354,7 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
             sm, limit, equals);
     else if (take < there)
         limit = 0, equals = 0;  // none but those always listed
-    kv_walk<false>(
+    kv_walk<false, true>(
         team, mine, equals, sm,
         [&](u32 i) -> u32 {
             const u32 k = keys[i];
@@ -382,8 +362,8 @@ __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team
             return k == kAlways || ~k < limit ? 1 : ~k == limit ? 2 : 0;
         },
         [](u32) { return 0; },
-        [&](u32 i, int, bool listed, u32 before) {
-            if (listed && before < a.top) list[before] = static_cast<int>(first + i);
+        [&](u32 i, int, bool, u32 before) {
+            if (before < a.top) list[before] = static_cast<int>(first + i);
         });
     if (team.rank == 0) {
         for (u32 i = take + threadIdx.x; i < a.top; i += blockDim.x) list[i] = -1;
