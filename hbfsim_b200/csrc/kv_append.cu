@@ -232,6 +232,21 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, u32 head, u32 
     }
 }
 
+// The last sequence that starts at or before a token, by a warp: 32 places at a time.
+__device__ __forceinline__ u32 sequence_of(const AppendArgs& a, i64 token)
+{
+    const u32 lane = threadIdx.x & 31u;
+    u32 lo = 0, hi = a.seqs;  // it is in [lo, hi)
+    while (hi - lo > 1) {
+        const u32 step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const u32 before = __ballot_sync(0xffffffffu, at < hi && (lane == 0 || a.offsets[at] <= token));
+        const u32 last = 31 - __clz(before);  // offsets ascend: the lanes before it say yes as well
+        hi = min(hi, lo + (last + 1) * step);
+        lo += last * step;
+    }
+    return lo;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendArgs a)
 {
@@ -242,13 +257,18 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendA
     const i64 token = static_cast<i64>(blockIdx.x) * a.chunk + lane;
     bool leads = lane < a.chunk && token < a.tokens;
     int page = -1;
-    u32 slot = 0, count = 0;
+    u32 slot = 0, count = 0, seq_first = 0, seq_last = 0;
+    if (a.offsets) {  // sequences of the chunk's first and last token
+        const i64 base = static_cast<i64>(blockIdx.x) * a.chunk;
+        seq_first = sequence_of(a, base);
+        seq_last = a.chunk > 1 ? sequence_of(a, min(base + a.chunk, static_cast<i64>(a.tokens)) - 1) : seq_first;
+    }
     if (leads) {
         u32 seq;
         i64 first, end;
         if (a.offsets) {
-            u32 lo = 0, hi = a.seqs;  // offsets[lo] <= token < offsets[hi]
-            leads = token >= a.offsets[0] && token < a.offsets[hi];
+            u32 lo = seq_first, hi = seq_last + 1;  // offsets[lo] <= token < offsets[hi]
+            leads = token >= a.offsets[0] && token < a.offsets[a.seqs];
             while (hi - lo > 1) {
                 const u32 mid = (lo + hi) >> 1;
                 if (token >= a.offsets[mid]) lo = mid;
