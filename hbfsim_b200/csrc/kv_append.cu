@@ -3,16 +3,16 @@
 // One warp per (touched block, head, side).  A CTA's warps look at a chunk of
 // up to 32 tokens, one per lane, and do the blocks whose first new token is
 // among them, each warp for its head and side; few tokens get chunks of one,
-// so that every block has a warp of its own at once.  A lane holds its
-// channels of 16 tokens in registers between the two passes: the largest
-// magnitude, which gives the scale, then the stored values (blocks of more
-// tokens are read again).  Everything is a power of two away from the input,
+// so that every block has a warp of its own at once.  For a block of new
+// tokens alone a lane holds its channels of 16 tokens in registers between
+// the two passes: the largest magnitude, which gives the scale, then the
+// stored values (blocks of more tokens are read again).  Everything is a power of two away from the input,
 // so the only rounding is the one to e4m3.
 #include "kv.h"
 
 #include <cuda_fp8.h>
 
-#include <algorithm>
+#include <type_traits>
 
 namespace hbfb {
 namespace {
@@ -25,7 +25,7 @@ struct AppendArgs {
     KvView c;
     const void* x[2];
     i64 stride_token[2], stride_head[2];
-    bool wide[2];  // every head begins on a 16-byte boundary
+    bool wide;  // every head of k and v begins on a 16-byte boundary
     const int* table;
     i64 table_stride;
     const int* start;
@@ -38,10 +38,14 @@ template <typename T>
 struct Pair;
 template <>
 struct Pair<__nv_bfloat16> {
-    static __device__ __forceinline__ u32 largest(u32 a, u32 b)  // of magnitudes; NaN loses
+    // the lesser and the greater of each, NaN if either is
+    static __device__ __forceinline__ void span(u32& lo, u32& hi, u32 x)
     {
-        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-        return *reinterpret_cast<const u32*>(&m);
+        const __nv_bfloat162 y = *reinterpret_cast<__nv_bfloat162*>(&x);
+        const __nv_bfloat162 l = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&lo), y);
+        const __nv_bfloat162 h = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&hi), y);
+        lo = *reinterpret_cast<const u32*>(&l);
+        hi = *reinterpret_cast<const u32*>(&h);
     }
     static __device__ __forceinline__ float2 floats(u32 x)
     {
@@ -50,10 +54,13 @@ struct Pair<__nv_bfloat16> {
 };
 template <>
 struct Pair<__half> {
-    static __device__ __forceinline__ u32 largest(u32 a, u32 b)
+    static __device__ __forceinline__ void span(u32& lo, u32& hi, u32 x)
     {
-        const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-        return *reinterpret_cast<const u32*>(&m);
+        const __half2 y = *reinterpret_cast<__half2*>(&x);
+        const __half2 l = __hmin2_nan(*reinterpret_cast<__half2*>(&lo), y);
+        const __half2 h = __hmax2_nan(*reinterpret_cast<__half2*>(&hi), y);
+        lo = *reinterpret_cast<const u32*>(&l);
+        hi = *reinterpret_cast<const u32*>(&h);
     }
     static __device__ __forceinline__ float2 floats(u32 x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
 };
@@ -80,42 +87,129 @@ __device__ __forceinline__ u32 store_e4m3(float2 x)
     return __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
 }
 
-// A lane's channels of the new tokens among 16 rows of a block; 0 in the other rows.
-template <int W>
-__device__ __forceinline__ void load_rows(const u16* x, i64 stride, u32 row0, u32 slot, u32 count, bool wide,
-                                          u32 (&raw)[16][W])
+// A lane's channels of one token.
+template <int W, bool kWide>
+__device__ __forceinline__ void load_row(const u16* from, u32 (&raw)[W])
 {
+    if constexpr (!kWide) {
 #pragma unroll
-    for (u32 r = 0; r < 16; ++r) {
-#pragma unroll
-        for (int w = 0; w < W; ++w) raw[r][w] = 0;
-        const u32 t = row0 + r - slot;  // wraps for earlier rows
-        if (t < count) {
-            const u16* from = x + t * stride;
-            if (wide) {
-                if constexpr (W == 1) {
-                    raw[r][0] = *reinterpret_cast<const u32*>(from);
-                } else if constexpr (W == 2) {
-                    const uint2 y = *reinterpret_cast<const uint2*>(from);
-                    raw[r][0] = y.x;
-                    raw[r][1] = y.y;
-                } else {
-                    const uint4 y = *reinterpret_cast<const uint4*>(from);
-                    raw[r][0] = y.x;
-                    raw[r][1] = y.y;
-                    raw[r][2] = y.z;
-                    raw[r][3] = y.w;
-                }
-            } else {
-#pragma unroll
-                for (int w = 0; w < W; ++w) raw[r][w] = from[2 * w] | static_cast<u32>(from[2 * w + 1]) << 16;
-            }
-        }
+        for (int w = 0; w < W; ++w) raw[w] = from[2 * w] | static_cast<u32>(from[2 * w + 1]) << 16;
+    } else if constexpr (W == 1) {
+        raw[0] = *reinterpret_cast<const u32*>(from);
+    } else if constexpr (W == 2) {
+        const uint2 y = *reinterpret_cast<const uint2*>(from);
+        raw[0] = y.x;
+        raw[1] = y.y;
+    } else {
+        const uint4 y = *reinterpret_cast<const uint4*>(from);
+        raw[0] = y.x;
+        raw[1] = y.y;
+        raw[2] = y.z;
+        raw[3] = y.w;
     }
 }
 
-// One block, head and side by one warp.
-template <typename T, int D>
+// Bounds of a lane's channels from the least and greatest stored values (pairs).
+template <int D>
+__device__ __forceinline__ void put_bounds(const AppendArgs& a, int page, u32 head, const u32 (&lo)[D / 64],
+                                           const u32 (&hi)[D / 64])
+{
+    constexpr int W = D / 64;
+    std::int8_t* bound = a.c.bounds + (static_cast<u64>(page) * a.c.heads + head) * 2 * D + (threadIdx.x & 31u) * 2 * W;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const float2 l = __half22float2(stored_f16(lo[w])), h = __half22float2(stored_f16(hi[w]));
+        *reinterpret_cast<char2*>(bound + 2 * w) =
+            make_char2(static_cast<signed char>(floorf(l.x * 0.25f)), static_cast<signed char>(floorf(l.y * 0.25f)));
+        *reinterpret_cast<char2*>(bound + D + 2 * w) =
+            make_char2(static_cast<signed char>(ceilf(h.x * 0.25f)), static_cast<signed char>(ceilf(h.y * 0.25f)));
+    }
+}
+
+// A row's stored values.
+template <int W>
+__device__ __forceinline__ void put_row(u8* to, const u32 (&b)[W])
+{
+    if constexpr (W == 1) *reinterpret_cast<u16*>(to) = static_cast<u16>(b[0]);
+    else if constexpr (W == 2) *reinterpret_cast<u32*>(to) = b[0] | b[1] << 16;
+    else *reinterpret_cast<uint2*>(to) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+}
+
+// A block whose tokens are all new, head and side by one warp; false, with
+// nothing written, where an element is not finite.  Rounding keeps the order,
+// so the least and greatest of the input give both the scale and the bounds.
+template <typename T, int D, bool kWide>
+__device__ __forceinline__ bool append_full(const AppendArgs& a, u32 head, u32 side, u32 token, int page)
+{
+    constexpr int W = D / 64;  // pairs of channels of a lane
+    const u32 lane = threadIdx.x & 31u, block = a.c.block;
+    const i64 stride = a.stride_token[side];
+    const u16* x = static_cast<const u16*>(a.x[side]) + static_cast<i64>(token) * stride +
+                   static_cast<i64>(head) * a.stride_head[side] + lane * 2 * W;
+    const u64 at = (static_cast<u64>(page) * a.c.heads + head) * 2 + side;
+    u32 raw[16][W], lo[W], hi[W];
+    auto load_rows = [&](u32 row0) {
+#pragma unroll
+        for (u32 r = 0; r < 16; ++r) load_row<W, kWide>(x + (row0 + r) * stride, raw[r]);
+    };
+    load_rows(0);
+#pragma unroll
+    for (int w = 0; w < W; ++w) lo[w] = hi[w] = raw[0][w];
+    for (u32 row0 = 0;;) {
+#pragma unroll
+        for (u32 r = 0; r < 16; ++r)
+#pragma unroll
+            for (int w = 0; w < W; ++w) Pair<T>::span(lo[w], hi[w], raw[r][w]);
+        row0 += 16;
+        if (row0 == block) break;
+        load_rows(row0);
+    }
+    float most = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const float2 l = Pair<T>::floats(lo[w]), h = Pair<T>::floats(hi[w]);
+        const float m = fmaxf(fmaxf(fabsf(l.x), fabsf(l.y)), fmaxf(fabsf(h.x), fabsf(h.y)));
+        finite &= m <= 3.402823466e38f && l.x == l.x && l.y == l.y;
+        most = fmaxf(most, m);
+    }
+    if (!__all_sync(0xffffffffu, finite)) return false;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const float now = kv_power(scale_exponent(most)), inverse = 1.0f / now;
+    if (lane == 0) a.c.scale[at] = now;
+    auto stored = [&](u32 pair) {
+        float2 y = Pair<T>::floats(pair);
+        y.x *= inverse;
+        y.y *= inverse;
+        return store_e4m3(y);
+    };
+    u8* out = a.c.data + at * block * D + lane * 2 * W;
+    for (u32 row0 = 0;;) {
+        if (block > 16) load_rows(row0);
+#pragma unroll
+        for (u32 r = 0; r < 16; ++r) {
+            u32 b[W];
+#pragma unroll
+            for (int w = 0; w < W; ++w) b[w] = stored(raw[r][w]);
+            put_row<W>(out + (row0 + r) * D, b);
+        }
+        row0 += 16;
+        if (row0 == block) break;
+    }
+    if (side == 0) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            lo[w] = stored(lo[w]);
+            hi[w] = stored(hi[w]);
+        }
+        put_bounds<D>(a, page, head, lo, hi);
+    }
+    return true;
+}
+
+// Any block, head and side by one warp: `slot` tokens held before, `count` new ones.
+template <typename T, int D, bool kWide>
 __device__ __forceinline__ void append_block(const AppendArgs& a, u32 head, u32 side, u32 token, int page, u32 slot,
                                              u32 count)
 {
@@ -126,29 +220,37 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, u32 head, u32 
                    static_cast<i64>(head) * a.stride_head[side] + lane * 2 * W;
     const u64 at = (static_cast<u64>(page) * a.c.heads + head) * 2 + side;
     u8* out = a.c.data + at * block * D + lane * 2 * W;
-    const float was = slot ? a.c.scale[at] : 0.0f;
-    u32 raw[16][W];
-    float most = 0.0f;
-    for (u32 row0 = 0; row0 < block; row0 += 16) {
-        if (row0 >= slot + count || row0 + 16 <= slot) continue;
-        load_rows<W>(x, stride, row0, slot, count, a.wide[side], raw);
-        u32 m = 0;
+    // what 16 rows hold, all reads under way at once
+    constexpr int H = W == 4 ? 2 : 1;  // words of a lane's stored values in a row
+    u32 held[16][H];
+    auto load_held = [&](u32 row0) {
 #pragma unroll
-        for (u32 r = 0; r < 16; ++r)
+        for (u32 r = 0; r < 16; ++r) {
 #pragma unroll
-            for (int w = 0; w < W; ++w) m = Pair<T>::largest(m, raw[r][w] & 0x7fff7fffu);
-        float2 y = Pair<T>::floats(m);
-        if (!(fmaxf(y.x, y.y) <= 3.402823466e38f)) {  // infinities: what is finite counts
-            y = make_float2(0.0f, 0.0f);
+            for (int w = 0; w < H; ++w) held[r][w] = 0;
+            if (row0 + r < slot) {
+                const u8* from = out + (row0 + r) * D;
+                if constexpr (W == 1) {
+                    held[r][0] = *reinterpret_cast<const u16*>(from);
+                } else {
 #pragma unroll
-            for (u32 r = 0; r < 16; ++r)
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const float2 z = Pair<T>::floats(raw[r][w]);
-                    y.x = fmaxf(y.x, fmaxf(finite_or_0(z.x), finite_or_0(z.y)));
+                    for (int w = 0; w < H; ++w) held[r][w] = reinterpret_cast<const u32*>(from)[w];
                 }
+            }
         }
-        most = fmaxf(most, fmaxf(y.x, y.y));
+    };
+    if (side == 0) load_held(0);  // the keys' bounds need them in any case
+    const float was = slot ? a.c.scale[at] : 0.0f;
+    float most = 0.0f;
+#pragma unroll 2
+    for (u32 t = 0; t < count; ++t) {
+        u32 raw[W];
+        load_row<W, kWide>(x + t * stride, raw);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 y = Pair<T>::floats(raw[w]);
+            most = fmaxf(most, fmaxf(finite_or_0(y.x), finite_or_0(y.y)));
+        }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -163,72 +265,64 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, u32 head, u32 
         least[w] = __float2half2_rn(448.0f);
         greatest[w] = __float2half2_rn(-448.0f);
     }
-    for (u32 row0 = 0; row0 < block; row0 += 16) {
-        if (block > 16 && row0 < slot + count && row0 + 16 > slot)
-            load_rows<W>(x, stride, row0, slot, count, a.wide[side], raw);
+    auto bound = [&](const u32 (&b)[W]) {
 #pragma unroll
-        for (u32 r = 0; r < 16; ++r) {
-            const u32 row = row0 + r;
-            u32 b[W];  // pairs of stored values
-            bool write = true;
-            if (row < slot) {
-                write = shrink != 1.0f;
-                if (!write && side) continue;
+        for (int w = 0; w < W; ++w) {
+            __half2 y = stored_f16(b[w]);
+            // NaN counts as 0
+            const u32 z = *reinterpret_cast<u32*>(&y) & __heq2_mask(y, y);
+            y = *reinterpret_cast<const __half2*>(&z);
+            least[w] = __hmin2(least[w], y);
+            greatest[w] = __hmax2(greatest[w], y);
+        }
+    };
+    if (side == 0 || shrink != 1.0f) {  // values need nothing else
+        for (u32 row0 = 0; row0 < slot; row0 += 16) {
+            if (row0 || side) load_held(row0);
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    b[w] = *reinterpret_cast<const u16*>(out + row * D + 2 * w);
-                    if (write) {
+            for (u32 r = 0; r < 16; ++r) {
+                if (row0 + r >= slot) break;
+                u32 b[W];
+#pragma unroll
+                for (int w = 0; w < W; ++w) b[w] = held[r][w / 2] >> (w & 1) * 16 & 0xffffu;
+                if (shrink != 1.0f) {
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
                         float2 y = __half22float2(stored_f16(b[w]));
                         y.x *= shrink;
                         y.y *= shrink;
                         b[w] = store_e4m3(y);
                     }
+                    put_row<W>(out + (row0 + r) * D, b);
                 }
-            } else if (row < slot + count) {
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    float2 y = Pair<T>::floats(raw[r][w]);
-                    y.x *= inverse;
-                    y.y *= inverse;
-                    b[w] = store_e4m3(y);
-                }
-            } else {
-#pragma unroll
-                for (int w = 0; w < W; ++w) b[w] = 0;
-            }
-            if (write) {
-                u8* to = out + row * D;
-                if constexpr (W == 1) {
-                    *reinterpret_cast<u16*>(to) = static_cast<u16>(b[0]);
-                } else if constexpr (W == 2) {
-                    *reinterpret_cast<u32*>(to) = b[0] | b[1] << 16;
-                } else {
-                    *reinterpret_cast<uint2*>(to) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-                }
-            }
-            if (side == 0 && row < slot + count) {
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    __half2 y = stored_f16(b[w]);
-                    // NaN counts as 0
-                    const u32 z = *reinterpret_cast<u32*>(&y) & __heq2_mask(y, y);
-                    y = *reinterpret_cast<const __half2*>(&z);
-                    least[w] = __hmin2(least[w], y);
-                    greatest[w] = __hmax2(greatest[w], y);
-                }
+                if (side == 0) bound(b);
             }
         }
     }
-    if (side == 0) {
-        std::int8_t* bound = a.c.bounds + (static_cast<u64>(page) * a.c.heads + head) * 2 * D + lane * 2 * W;
+#pragma unroll 2
+    for (u32 t = 0; t < count; ++t) {
+        u32 raw[W], b[W];
+        load_row<W, kWide>(x + t * stride, raw);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float2 lo = __half22float2(least[w]), hi = __half22float2(greatest[w]);
-            *reinterpret_cast<char2*>(bound + 2 * w) =
-                make_char2(static_cast<signed char>(floorf(lo.x * 0.25f)), static_cast<signed char>(floorf(lo.y * 0.25f)));
-            *reinterpret_cast<char2*>(bound + D + 2 * w) =
-                make_char2(static_cast<signed char>(ceilf(hi.x * 0.25f)), static_cast<signed char>(ceilf(hi.y * 0.25f)));
+            float2 y = Pair<T>::floats(raw[w]);
+            y.x *= inverse;
+            y.y *= inverse;
+            b[w] = store_e4m3(y);
         }
+        put_row<W>(out + (slot + t) * D, b);
+        if (side == 0) bound(b);
+    }
+    const u32 none[W] = {};
+    for (u32 row = slot + count; row < block; ++row) put_row<W>(out + row * D, none);
+    if (side == 0) {
+        u32 lo[W], hi[W];  // the values are stored ones: rounding them again changes nothing
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            lo[w] = store_e4m3(__half22float2(least[w]));
+            hi[w] = store_e4m3(__half22float2(greatest[w]));
+        }
+        put_bounds<D>(a, page, head, lo, hi);
     }
 }
 
@@ -247,8 +341,8 @@ __device__ __forceinline__ u32 sequence_of(const AppendArgs& a, i64 token)
     return lo;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendArgs a)
+template <typename T, int D, bool kWide>
+__global__ void __launch_bounds__(kAppendWarps * 32, D == 256 ? 3 : 6) append_kernel(const AppendArgs a)
 {
     const u32 lane = threadIdx.x & 31u;
     const u32 pair = blockIdx.y * kAppendWarps + (threadIdx.x >> 5), head = pair >> 1, side = pair & 1u;
@@ -296,9 +390,11 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendA
     }
     for (u32 left = __ballot_sync(0xffffffffu, leads); left; left &= left - 1) {
         const int who = __ffs(left) - 1;
-        append_block<T, D>(a, head, side, static_cast<u32>(blockIdx.x * a.chunk + who),
-                           __shfl_sync(0xffffffffu, page, who), __shfl_sync(0xffffffffu, slot, who),
-                           __shfl_sync(0xffffffffu, count, who));
+        const u32 its_token = blockIdx.x * a.chunk + static_cast<u32>(who);
+        const int its_page = __shfl_sync(0xffffffffu, page, who);
+        const u32 its_slot = __shfl_sync(0xffffffffu, slot, who), its_count = __shfl_sync(0xffffffffu, count, who);
+        if (its_count < a.c.block || !append_full<T, D, kWide>(a, head, side, its_token, its_page))
+            append_block<T, D, kWide>(a, head, side, its_token, its_page, its_slot, its_count);
     }
 }
 
@@ -306,9 +402,14 @@ template <typename T>
 int launch(const AppendArgs& a, cudaStream_t s)
 {
     const dim3 grid((a.tokens + a.chunk - 1) / a.chunk, (a.c.heads * 2 + kAppendWarps - 1) / kAppendWarps);
-    if (a.c.dim == 64) append_kernel<T, 64><<<grid, kAppendWarps * 32, 0, s>>>(a);
-    else if (a.c.dim == 128) append_kernel<T, 128><<<grid, kAppendWarps * 32, 0, s>>>(a);
-    else append_kernel<T, 256><<<grid, kAppendWarps * 32, 0, s>>>(a);
+    auto run = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        if (a.wide) append_kernel<T, D, true><<<grid, kAppendWarps * 32, 0, s>>>(a);
+        else append_kernel<T, D, false><<<grid, kAppendWarps * 32, 0, s>>>(a);
+    };
+    if (a.c.dim == 64) run(std::integral_constant<int, 64>{});
+    else if (a.c.dim == 128) run(std::integral_constant<int, 128>{});
+    else run(std::integral_constant<int, 256>{});
     return cudaGetLastError() == cudaSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
@@ -350,8 +451,7 @@ extern "C" int hbfsim_kv_append_v1(const hbfsim_kv_cache_v1* cache,
     a.width = b->width;
     a.tokens = static_cast<u32>(b->tokens);
     auto wide = [](const void* p, i64 token, i64 head) { return kv_aligned(p, 16) && token % 8 == 0 && head % 8 == 0; };
-    a.wide[0] = wide(b->k, b->k_stride_token, b->k_stride_head);
-    a.wide[1] = wide(b->v, b->v_stride_token, b->v_stride_head);
+    a.wide = wide(b->k, b->k_stride_token, b->k_stride_head) && wide(b->v, b->v_stride_token, b->v_stride_head);
     // one token to a chunk while all chunks' warps are resident at once (16 to an SM), more beyond
     a.chunk = 1;
     while (a.chunk < 32 && static_cast<u64>(a.tokens) * v.heads * 2 > static_cast<u64>(a.chunk) * 16 * kv_sm_count())
