@@ -2,11 +2,11 @@
 // cache (kv_v1.h), over all blocks of a sequence or over listed ones.
 //
 // The query rows that share a key/value head (group heads times tokens) are
-// taken 8 or 16 at a time as the narrow side of the tensor-core products, so
+// taken 8 to 32 at a time as the narrow side of the tensor-core products, so
 // that the tokens are the wide one:
 //
-//   S^T [16 tokens x 8 rows]  = K [16 x D] Q^T [D x 8]
-//   O^T [D x 8 rows]         += V^T [D x 16 tokens] P^T [16 x 8]
+//   S^T [16 tokens x rows]  = K [16 x D] Q^T [D x rows]
+//   O^T [D x rows]         += V^T [D x 16 tokens] P^T [16 x rows]
 //
 // K and V are read in their natural order straight into the fragments of
 // mma.m16n8k16: the order of the channels inside a dot product and of the
@@ -206,15 +206,32 @@ __device__ __forceinline__ int row_position(const AttentionArgs& a, const Segmen
     return max(s.length - static_cast<int>(a.q.tokens) + static_cast<int>(t), -1);
 }
 
-// CTAs per SM and the depth of a warp's ring: about 192 KB of rings per SM.
-constexpr u32 per_sm(u32 dim, u32 nt) { return dim == 256 ? 2 : dim * nt == 256 ? 3 : 4; }
+// Row tiles of 8 rows a CTA takes at most: the output accumulators of 32 rows
+// of 128 channels are 128 registers of a lane.
+constexpr u32 most_nt(u32 dim) { return dim == 256 ? 2 : 4; }
+// CTAs per SM and the depth of a warp's ring, by registers and about 192 KB of rings.
+constexpr u32 per_sm(u32 dim, u32 nt)
+{
+    return dim == 256 ? 2 : dim == 128 ? (nt == 1 ? 4 : nt == 2 ? 3 : 2) : (nt <= 2 ? 4 : 3);
+}
 template <int D>
 constexpr u32 kStages = D == 64 ? 4 : 3;
 template <int D>
 constexpr u32 kRing = kWarps * kStages<D> * 32 * D;  // bytes
+// One row tile's queries stay in registers; more are read from shared memory for each tile.
 template <int D, int NT>
-constexpr u32 kSmem = (kRing<D> > kWarps * 8 * NT * D * 4 ? kRing<D> : kWarps * 8 * NT * D * 4) +
-                      kWarps * kStages<D> * 16 + kWarps * 8 * NT * 8 + 16;
+constexpr bool kSharedQueries = NT > 1 || D == 256;
+// Shared memory: rings (later the joined values), notes, sums, queries, row factors and ends, a word.
+template <int D, int NT>
+struct Layout {
+    static constexpr u32 notes = kRing<D> > kWarps * 8 * NT * D * 4 ? kRing<D> : kWarps * 8 * NT * D * 4;
+    static constexpr u32 join_ml = notes + kWarps * kStages<D> * 16;
+    static constexpr u32 queries = join_ml + kWarps * 8 * NT * 8;
+    static constexpr u32 factors = queries + (kSharedQueries<D, NT> ? NT * D * 16 : 0);
+    static constexpr u32 ends = factors + 8 * NT * 4;
+    static constexpr u32 line = ends + 8 * NT * 4;
+    static constexpr u32 bytes = line + 16;
+};
 
 // One segment's tiles [first, end) by one CTA; the partial result goes to `part`.
 template <int D, int NT>
@@ -229,9 +246,13 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
     u8* ring = smem + warp * NS * 2 * kSide;
     float* join_o = reinterpret_cast<float*>(smem);  // [kWarps][R][D], after the loop
-    constexpr u32 kUpper = kSmem<D, NT> - 16 - kWarps * R * 8 - kWarps * NS * 16;
-    int4* note = reinterpret_cast<int4*>(smem + kUpper) + warp * NS;  // position, -, scales
-    float2* join_ml = reinterpret_cast<float2*>(smem + kUpper + kWarps * NS * 16);  // [kWarps][R]
+    using L = Layout<D, NT>;
+    constexpr bool kShared = kSharedQueries<D, NT>;
+    int4* note = reinterpret_cast<int4*>(smem + L::notes) + warp * NS;  // position, -, scales
+    float2* join_ml = reinterpret_cast<float2*>(smem + L::join_ml);     // [kWarps][R]
+    uint4* queries = reinterpret_cast<uint4*>(smem + L::queries);       // [NT][D / 32][32 lanes]
+    float* factors = reinterpret_cast<float*>(smem + L::factors);       // [R]
+    int* ends = reinterpret_cast<int*>(smem + L::ends);                 // [R]: last position a row sees
     const u32 ring_at = static_cast<u32>(__cvta_generic_to_shared(ring));
     const u32 note_at = static_cast<u32>(__cvta_generic_to_shared(note));
     const u32 rows = min(static_cast<u32>(R), a.rows - seg.rt * R);
@@ -293,12 +314,11 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 #pragma unroll
     for (u32 i = 0; i + 1 < NS; ++i) issue(i, i);
 
-    // queries: row n = 8 nt + g, scaled by a power of two so that the largest is in [2^14, 2^15)
-    u32 qf[NT][D / 16][2];
-    float factor[NT][2];   // of the columns 2c, 2c+1: scale2 over the row's power of two
-    int sees[NT][2];       // last position seen
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    // Queries: row n = 8 nt + g, scaled by a power of two so that the largest is in
+    // [2^14, 2^15); its factor is scale2 over that power.
+    u32 qf[kShared ? 1 : D / 16][2];
+    float factor0 = 0.0f, factor1 = 0.0f;  // of the columns 2c, 2c + 1
+    for (u32 nt = kShared ? warp : 0; nt < NT; nt += kShared ? kWarps : 1) {
         const u32 n = nt * 8 + g;
         float x[KC][16];
         float most = 0.0f;
@@ -329,21 +349,33 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         e = max(15 - e, -126);
         e = min(e, 126);
         const float up = kv_power(e);
-#pragma unroll
-        for (int k = 0; k < KC; ++k)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                qf[nt][k * 4 + w][0] = pack_f16(x[k][4 * w] * up, x[k][4 * w + 1] * up);
-                qf[nt][k * 4 + w][1] = pack_f16(x[k][4 * w + 2] * up, x[k][4 * w + 3] * up);
-            }
         const float f = a.scale2 * kv_power(-e);
+        if constexpr (kShared) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            factor[nt][i] = __shfl_sync(0xffffffffu, f, (2 * c + i) * 4);
-            const u32 m = nt * 8 + 2 * c + i;
-            sees[nt][i] = row_position(a, seg, seg.rt * R + min(m, rows - 1));
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int w = 0; w < 4; w += 2)
+                    queries[(nt * (D / 32) + k * 2 + w / 2) * 32 + lane] =
+                        make_uint4(pack_f16(x[k][4 * w] * up, x[k][4 * w + 1] * up),
+                                   pack_f16(x[k][4 * w + 2] * up, x[k][4 * w + 3] * up),
+                                   pack_f16(x[k][4 * w + 4] * up, x[k][4 * w + 5] * up),
+                                   pack_f16(x[k][4 * w + 6] * up, x[k][4 * w + 7] * up));
+            if (c == 0) factors[n] = f;
+        } else {
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    qf[k * 4 + w][0] = pack_f16(x[k][4 * w] * up, x[k][4 * w + 1] * up);
+                    qf[k * 4 + w][1] = pack_f16(x[k][4 * w + 2] * up, x[k][4 * w + 3] * up);
+                }
+            factor0 = __shfl_sync(0xffffffffu, f, 8 * c);
+            factor1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);
         }
     }
+    if (threadIdx.x < R)
+        ends[threadIdx.x] = row_position(a, seg, seg.rt * R + min(static_cast<u32>(threadIdx.x), rows - 1));
+    __syncthreads();
 
     float o[NT][D / 16][4];
     float m[NT][2], l[NT][2];
@@ -369,15 +401,31 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         for (int w = 0; w < (VW >= 4 ? VW / 4 : 1); ++w)
             value_at[x][w] = kSide + swizzle((2 * c + x) * D + g * (D / 8) + w * 16);
 
+    // Mask of the f16 halves that are numbers, and the first token (0..15) of a row of the value
+    // fragment, over the 4 lanes that hold it, that is none (a large number without one).
+    auto numbers = [](u32 x) {
+        const __half2 y = *reinterpret_cast<const __half2*>(&x);
+        return __heq2_mask(y, y);
+    };
+    auto first_nan = [&](u32 lo, u32 hi) {
+        int t = !(lo & 0xffffu) ? 0 : !(lo >> 16) ? 1 : !(hi & 0xffffu) ? 8 : !(hi >> 16) ? 9 : 1 << 20;
+        t += static_cast<int>(2 * c);
+        t = min(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        return min(t, __shfl_xor_sync(0xffffffffu, t, 2));
+    };
     // One tile.  `edge`: some row does not see all of its tokens.
     auto consume = [&](auto is_edge, const u8* tile, int p0, float key_scale, float new_scale,
                        float* tile_out) {
         constexpr bool kEdge = decltype(is_edge)::value;
-        float s[NT][4], s2[NT][4];  // two sums, so that products need not wait for each other
+        // with one row tile two sums, so that products need not wait for each other
+        constexpr int kSums = NT == 1 ? 2 : 1;
+        float s[NT][kSums][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[nt][k] = s2[nt][k] = 0.0f;
+            for (int x = 0; x < kSums; ++x)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[nt][x][k] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
             const uint4 k0 = *reinterpret_cast<const uint4*>(tile + key_at[k]);
@@ -385,15 +433,30 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             const u32 w0[4] = {k0.x, k0.y, k0.z, k0.w};
             const u32 w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const u32 a0 = e4m3x2_to_f16x2(w0[w]), a2 = e4m3x2_to_f16x2(w0[w] >> 16);
-                const u32 a1 = e4m3x2_to_f16x2(w1[w]), a3 = e4m3x2_to_f16x2(w1[w] >> 16);
+            for (int w = 0; w < 4; w += 2) {
+                u32 x[2][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    mma16816(w & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][k * 4 + w][0],
-                             qf[nt][k * 4 + w][1]);
+                for (int i = 0; i < 2; ++i) {
+                    x[i][0] = e4m3x2_to_f16x2(w0[w + i]);
+                    x[i][1] = e4m3x2_to_f16x2(w1[w + i]);
+                    x[i][2] = e4m3x2_to_f16x2(w0[w + i] >> 16);
+                    x[i][3] = e4m3x2_to_f16x2(w1[w + i] >> 16);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    uint4 q;
+                    if constexpr (kShared) q = queries[(nt * (D / 32) + k * 2 + w / 2) * 32 + lane];
+                    else q = make_uint4(qf[k * 4 + w][0], qf[k * 4 + w][1], qf[k * 4 + w + 1][0], qf[k * 4 + w + 1][1]);
+                    mma16816(s[nt][0], x[0][0], x[0][1], x[0][2], x[0][3], q.x, q.y);
+                    mma16816(s[nt][kSums - 1], x[1][0], x[1][1], x[1][2], x[1][3], q.z, q.w);
+                }
             }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if constexpr (kSums == 2) s[nt][0][k] += s[nt][1][k];
         u32 v[4][VW];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -432,14 +495,17 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         for (int nt = 0; nt < NT; ++nt) {
             float p[4], sum[2];
             bool above = false;
+            float2 factor = make_float2(factor0, factor1);
+            if constexpr (kShared) factor = *reinterpret_cast<const float2*>(factors + nt * 8 + 2 * c);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float scaled = factor[nt][i] * key_scale;
-                p[i] = (s[nt][i] + s2[nt][i]) * scaled;
-                p[2 + i] = (s[nt][2 + i] + s2[nt][2 + i]) * scaled;
+                const float scaled = (i ? factor.y : factor.x) * key_scale;
+                p[i] = s[nt][0][i] * scaled;
+                p[2 + i] = s[nt][0][2 + i] * scaled;
                 if constexpr (kEdge) {
-                    if (p0 + static_cast<int>(g) > sees[nt][i]) p[i] = -INFINITY;
-                    if (p0 + static_cast<int>(g) + 8 > sees[nt][i]) p[2 + i] = -INFINITY;
+                    const int end = ends[nt * 8 + 2 * c + i];
+                    if (p0 + static_cast<int>(g) > end) p[i] = -INFINITY;
+                    if (p0 + static_cast<int>(g) + 8 > end) p[2 + i] = -INFINITY;
                 }
                 above |= fmaxf(p[i], p[2 + i]) > m[nt][i] + kAbove;
             }
@@ -502,37 +568,30 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 u32 a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
                 const int k = w * 2 + half;
                 if constexpr (kEdge) {
-                    if (staggered) {
-                        // rows end at different tokens: a value past a row's end (it may be NaN)
-                        // must not meet the row at all, so each end is taken by itself
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            float old[4], made[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) old[i] = made[i] = o[nt][k][i];
-                            for (int last = sees_least; last <= sees_most; ++last) {
-                                const int n = last - p0 - static_cast<int>(2 * c);
-                                const u32 lo_mask = (n >= 0 ? 0x0000ffffu : 0u) | (n >= 1 ? 0xffff0000u : 0u);
-                                const u32 hi_mask = (n >= 8 ? 0x0000ffffu : 0u) | (n >= 9 ? 0xffff0000u : 0u);
-                                float one[4] = {old[0], old[1], old[2], old[3]};
-                                mma16816(one, a0 & lo_mask, a1 & lo_mask, a2 & hi_mask, a3 & hi_mask,
-                                         b[nt][0], b[nt][1]);
-#pragma unroll
-                                for (int i = 0; i < 2; ++i)
-                                    if (sees[nt][i] == last) {
-                                        made[i] = one[i];
-                                        made[2 + i] = one[2 + i];
-                                    }
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[nt][k][i] = made[i];
-                        }
-                        continue;
-                    }
                     a0 &= keep_lo;
                     a1 &= keep_lo;
                     a2 &= keep_hi;
                     a3 &= keep_hi;
+                    if (staggered) {
+                        // Rows end at different tokens: a NaN past a row's end must not meet the
+                        // row, so NaN goes in as 0 and then to the rows that see it.
+                        const u32 n0 = numbers(a0), n1 = numbers(a1), n2 = numbers(a2), n3 = numbers(a3);
+                        if (__any_sync(0xffffffffu, (n0 & n1 & n2 & n3) != 0xffffffffu)) {
+                            a0 &= n0;
+                            a1 &= n1;
+                            a2 &= n2;
+                            a3 &= n3;
+                            const int t0 = p0 + first_nan(n0, n2), t1 = p0 + first_nan(n1, n3);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const int end = ends[nt * 8 + 2 * c + i];
+                                    if (end >= t0) o[nt][k][i] = __int_as_float(0x7fffffff);
+                                    if (end >= t1) o[nt][k][2 + i] = __int_as_float(0x7fffffff);
+                                }
+                        }
+                    }
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -606,7 +665,7 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
 {
     extern __shared__ __align__(128) u8 smem[];
     kv_let_next();
-    const u64 total = line_of(a, reinterpret_cast<u64*>(smem + kSmem<D, NT> - 16));
+    const u64 total = line_of(a, reinterpret_cast<u64*>(smem + Layout<D, NT>::line));
     const u64 share = share_of(a, total);
     u64 at = blockIdx.x * share;
     const u64 stop = min(at + share, total);
@@ -640,7 +699,7 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
 // share of the blocks.  All sums run in a fixed order.
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R, u32 slices)
 {
-    __shared__ float row_top[16], row_sum[16], row_lse[16];  // of the segment at hand
+    __shared__ float row_top[32], row_sum[32], row_lse[32];  // of the segment at hand
     __shared__ float4 join[kFinishThreads];
     const u32 i = threadIdx.x, lane = i & 31u, warp = i >> 5;
     kv_wait_before();
@@ -776,7 +835,9 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     Plan p{};
     p.lists = lists ? q.tokens : 1;
     p.rows = lists ? q.group : q.group * q.tokens;
-    p.nt = p.rows > 8 && v.dim < 256 ? 2 : 1;
+    // as few passes over the tiles as registers allow, of equal width
+    const u32 eights = (p.rows + 7) / 8, passes = (eights + most_nt(v.dim) - 1) / most_nt(v.dim);
+    p.nt = (eights + passes - 1) / passes;
     const u32 R = 8 * p.nt;
     p.row_tiles = (p.rows + R - 1) / R;
     p.tiles = (lists ? top : q.width) * (v.block / 16);
@@ -817,8 +878,8 @@ template <int D, int NT>
 int launch(const AttentionArgs& a, cudaStream_t s)
 {
     static std::atomic<u64> seen{0};
-    if (!kv_allow_smem(attention_kernel<D, NT>, kSmem<D, NT>, seen)) return HBFSIM_CUDA_ERROR;
-    attention_kernel<D, NT><<<a.workers, kWarps * 32, kSmem<D, NT>, s>>>(a);
+    if (!kv_allow_smem(attention_kernel<D, NT>, Layout<D, NT>::bytes, seen)) return HBFSIM_CUDA_ERROR;
+    attention_kernel<D, NT><<<a.workers, kWarps * 32, Layout<D, NT>::bytes, s>>>(a);
     // one CTA per segment; for the weights of long sequences more, up to what is resident at once
     const u32 pairs = a.q.seqs * a.c.heads, segments = a.lists * a.row_tiles;
     u32 across = segments;
@@ -884,7 +945,16 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     a.span = reinterpret_cast<uint2*>(w + p.span);
     a.tile_lse = a.weights ? reinterpret_cast<float*>(w + p.tile_lse) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a.c.dim == 64) return p.nt == 2 ? launch<64, 2>(a, s) : launch<64, 1>(a, s);
-    if (a.c.dim == 128) return p.nt == 2 ? launch<128, 2>(a, s) : launch<128, 1>(a, s);
-    return launch<256, 1>(a, s);
+    switch (a.c.dim * 8 + p.nt) {
+    case 64 * 8 + 1: return launch<64, 1>(a, s);
+    case 64 * 8 + 2: return launch<64, 2>(a, s);
+    case 64 * 8 + 3: return launch<64, 3>(a, s);
+    case 64 * 8 + 4: return launch<64, 4>(a, s);
+    case 128 * 8 + 1: return launch<128, 1>(a, s);
+    case 128 * 8 + 2: return launch<128, 2>(a, s);
+    case 128 * 8 + 3: return launch<128, 3>(a, s);
+    case 128 * 8 + 4: return launch<128, 4>(a, s);
+    case 256 * 8 + 1: return launch<256, 1>(a, s);
+    default: return launch<256, 2>(a, s);
+    }
 }
