@@ -41,6 +41,7 @@ constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
 // How far (in log2) a score may exceed the reference before the reference moves: a tile then
 // costs a vote instead of a maximum over the lanes.  2^kAbove keeps f16 probabilities finite.
 constexpr float kAbove = 8.0f;
+constexpr float kNoScore = -3.0e38f;  // reference of a row without a score
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
@@ -66,11 +67,12 @@ struct AttentionArgs {
     float* tile_lse;              // [segments][tiles][8 NT], or NULL
 };
 
-__device__ __forceinline__ u32 e4m3x2_to_f16x2(u32 two)
+// Four stored values as f16 pairs: exact.
+__device__ __forceinline__ void e4m3x4_to_f16(u32 four, u32& lo, u32& hi)
 {
-    u32 r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<u16>(two)));
-    return r;
+    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
 }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0,
@@ -93,6 +95,12 @@ __device__ __forceinline__ u32 pack_f16(float lo, float hi)
 {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const u32*>(&h);
+}
+
+__device__ __forceinline__ u32 times(u32 pair, __half2 by)
+{
+    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), by);
+    return *reinterpret_cast<const u32*>(&y);
 }
 
 __device__ __forceinline__ float exp2_fast(float x)  // 2^-22 relative, 0 for -inf
@@ -386,7 +394,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.0f;
-        m[nt][0] = m[nt][1] = -INFINITY;
+        m[nt][0] = m[nt][1] = kNoScore;
         l[nt][0] = l[nt][1] = 0.0f;
     }
     // where the lane's pieces lie in a tile side, and the same 8 tokens further: at D = 64 that
@@ -437,10 +445,8 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 u32 x[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    x[i][0] = e4m3x2_to_f16x2(w0[w + i]);
-                    x[i][1] = e4m3x2_to_f16x2(w1[w + i]);
-                    x[i][2] = e4m3x2_to_f16x2(w0[w + i] >> 16);
-                    x[i][3] = e4m3x2_to_f16x2(w1[w + i] >> 16);
+                    e4m3x4_to_f16(w0[w + i], x[i][0], x[i][2]);
+                    e4m3x4_to_f16(w1[w + i], x[i][1], x[i][3]);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -489,37 +495,41 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[nt][k][i] *= carry;
         }
-        const float relative = new_scale * value_inverse;
+        const __half2 relative = __float2half2_rn(new_scale * value_inverse);
         u32 b[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float p[4], sum[2];
-            bool above = false;
             float2 factor = make_float2(factor0, factor1);
             if constexpr (kShared) factor = *reinterpret_cast<const float2*>(factors + nt * 8 + 2 * c);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float scaled = (i ? factor.y : factor.x) * key_scale;
-                p[i] = s[nt][0][i] * scaled;
-                p[2 + i] = s[nt][0][2 + i] * scaled;
-                if constexpr (kEdge) {
-                    const int end = ends[nt * 8 + 2 * c + i];
-                    if (p0 + static_cast<int>(g) > end) p[i] = -INFINITY;
-                    if (p0 + static_cast<int>(g) + 8 > end) p[2 + i] = -INFINITY;
-                }
-                above |= fmaxf(p[i], p[2 + i]) > m[nt][i] + kAbove;
-            }
-            // the reference of the exponentials follows the maximum only when a score is far
-            // above it; until then probabilities reach 2^kAbove
-            if (__any_sync(0xffffffffu, above)) {
+            const float scaled[2] = {factor.x * key_scale, factor.y * key_scale};
+            // scores against the reference of their row
+            auto against = [&]() {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float most = fmaxf(p[i], p[2 + i]);
+                    p[i] = fmaf(s[nt][0][i], scaled[i], -m[nt][i]);
+                    p[2 + i] = fmaf(s[nt][0][2 + i], scaled[i], -m[nt][i]);
+                    if constexpr (kEdge) {
+                        const int end = ends[nt * 8 + 2 * c + i];
+                        if (p0 + static_cast<int>(g) > end) p[i] = -INFINITY;
+                        if (p0 + static_cast<int>(g) + 8 > end) p[2 + i] = -INFINITY;
+                    }
+                }
+            };
+            against();
+            // the reference of the exponentials follows the maximum only when a score is far
+            // above it; until then probabilities reach 2^kAbove
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])) > kAbove)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float most = -INFINITY;
+                    if (p[i] > -INFINITY) most = s[nt][0][i] * scaled[i];
+                    if (p[2 + i] > -INFINITY) most = fmaxf(most, s[nt][0][2 + i] * scaled[i]);
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1)
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
                     const float now = fmaxf(m[nt][i], most);
-                    const float shrink = now == -INFINITY ? 1.0f : exp2_fast(m[nt][i] - now);
+                    const float shrink = exp2_fast(m[nt][i] - now);
                     m[nt][i] = now;
                     l[nt][i] *= shrink;
 #pragma unroll
@@ -528,17 +538,17 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                         o[nt][k][2 + i] *= shrink;
                     }
                 }
+                against();
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float base = m[nt][i] == -INFINITY ? 0.0f : m[nt][i];
-                p[i] = exp2_fast(p[i] - base);
-                p[2 + i] = exp2_fast(p[2 + i] - base);
+                p[i] = exp2_fast(p[i]);
+                p[2 + i] = exp2_fast(p[2 + i]);
                 sum[i] = p[i] + p[2 + i];
                 l[nt][i] += sum[i];
             }
-            b[nt][0] = transpose8x8(pack_f16(p[0] * relative, p[1] * relative));
-            b[nt][1] = transpose8x8(pack_f16(p[2] * relative, p[3] * relative));
+            b[nt][0] = transpose8x8(times(pack_f16(p[0], p[1]), relative));
+            b[nt][1] = transpose8x8(times(pack_f16(p[2], p[3]), relative));
             if (tile_out) {
                 // the two columns' sums over the lanes of all g, the even g keeping the first
                 const float mine = g & 1 ? sum[1] : sum[0], other = g & 1 ? sum[0] : sum[1];
@@ -564,8 +574,9 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             for (int half = 0; half < 2; ++half) {
                 const u32 pick = half ? 0x7362 : 0x5140;
                 const u32 lo = __byte_perm(v[0][w], v[1][w], pick), hi = __byte_perm(v[2][w], v[3][w], pick);
-                u32 a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
-                u32 a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+                u32 a0, a1, a2, a3;
+                e4m3x4_to_f16(lo, a0, a1);
+                e4m3x4_to_f16(hi, a2, a3);
                 const int k = w * 2 + half;
                 if constexpr (kEdge) {
                     a0 &= keep_lo;
@@ -632,7 +643,8 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             const u32 row = nt * 8 + 2 * c + i;
-            if (g == 0) join_ml[warp * R + row] = make_float2(m[nt][i], sum);
+            if (g == 0)
+                join_ml[warp * R + row] = make_float2(m[nt][i] == kNoScore ? -INFINITY : m[nt][i], sum);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
                 float* to = join_o + (warp * R + row) * D + g * (D / 8) + 2 * k;
