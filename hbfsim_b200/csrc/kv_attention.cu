@@ -159,52 +159,56 @@ __device__ __forceinline__ Segment segment_of(const AttentionArgs& a, u32 index)
     return s;
 }
 
-// Length of the line of all tiles.
-__device__ u64 line_of(const AttentionArgs& a, u64* shared)
-{
-    u64 all = 0;
-    for (u32 u = threadIdx.x; u < a.units; u += blockDim.x)
-        all += static_cast<u64>(unit_tiles(a, u)) * a.per_unit;
-    if (threadIdx.x == 0) *shared = 0;
-    __syncthreads();
-#pragma unroll
-    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    if ((threadIdx.x & 31u) == 0) atomicAdd(reinterpret_cast<unsigned long long*>(shared), all);
-    __syncthreads();
-    return *shared;
-}
-
-// Tiles per share.
+// Tiles per share of a line of `total` tiles.
 __device__ __forceinline__ u64 share_of(const AttentionArgs& a, u64 total)
 {
     const u64 even = (total + a.workers - 1) / a.workers;
     return even > kShare ? even : kShare;
 }
 
-// The unit that holds place `at` of the line (at < total), and where it begins.
-__device__ void find_unit(const AttentionArgs& a, u64 at, u32& unit, u64& begin)
+// Where this CTA's share of the line of all tiles begins and ends, the unit
+// that holds its beginning and where that unit begins.  Each thread has a run
+// of units; a scan over the block gives their places.
+struct Place {
+    u64 at, stop, begin;
+    u32 unit;
+};
+
+__device__ __forceinline__ Place place_of(const AttentionArgs& a, u64* sums, Place* found)
 {
-    u64 done = 0;
-    for (u32 base = 0; base < a.units; base += 32) {  // every warp by itself
-        const u32 lane = threadIdx.x & 31u, u = base + lane;
-        const u64 n = u < a.units ? static_cast<u64>(unit_tiles(a, u)) * a.per_unit : 0;
-        u64 upto = n;
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const u32 each = (a.units + kWarps * 32 - 1) / (kWarps * 32);
+    const u32 from = min(threadIdx.x * each, a.units), to = min(from + each, a.units);
+    u64 mine = 0;
+#pragma unroll 4
+    for (u32 u = from; u < to; ++u) mine += static_cast<u64>(unit_tiles(a, u)) * a.per_unit;
+    u64 upto = mine;
 #pragma unroll
-        for (u32 o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-        }
-        const u32 holds = __ballot_sync(0xffffffffu, at < done + upto);
-        if (holds) {
-            const int k = __ffs(holds) - 1;
-            unit = base + k;
-            begin = done + __shfl_sync(0xffffffffu, upto - n, k);
-            return;
-        }
-        done += __shfl_sync(0xffffffffu, upto, 31);
+    for (u32 o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
     }
-    unit = a.units;
-    begin = done;
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    u64 total = 0;
+#pragma unroll
+    for (u32 w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += sums[w];
+        total += sums[w];
+    }
+    const u64 share = share_of(a, total), at = blockIdx.x * share;
+    if (threadIdx.x == 0 && at >= total) found->at = found->stop = 0;
+    if (at < total && at >= upto - mine && at < upto) {
+        Place p{at, min(at + share, total), upto - mine, from};
+        for (;; ++p.unit) {
+            const u64 n = static_cast<u64>(unit_tiles(a, p.unit)) * a.per_unit;
+            if (at < p.begin + n) break;
+            p.begin += n;
+        }
+        *found = p;
+    }
+    __syncthreads();
+    return *found;
 }
 
 // Position of the query token behind a row of the segment (-1: sees nothing).
@@ -232,13 +236,14 @@ constexpr bool kSharedQueries = NT > 1 || D == 256;
 // Shared memory: rings (later the joined values), notes, sums, queries, row factors and ends, a word.
 template <int D, int NT>
 struct Layout {
-    static constexpr u32 notes = kRing<D> > kWarps * 8 * NT * D * 4 ? kRing<D> : kWarps * 8 * NT * D * 4;
+    static constexpr u32 join = kWarps * 8 * NT * (D + 8) * 4;
+    static constexpr u32 notes = kRing<D> > join ? kRing<D> : join;
     static constexpr u32 join_ml = notes + kWarps * kStages<D> * 16;
     static constexpr u32 queries = join_ml + kWarps * 8 * NT * 8;
     static constexpr u32 factors = queries + (kSharedQueries<D, NT> ? NT * D * 16 : 0);
     static constexpr u32 ends = factors + 8 * NT * 4;
     static constexpr u32 line = ends + 8 * NT * 4;
-    static constexpr u32 bytes = line + 16;
+    static constexpr u32 bytes = line + 8 * kWarps + sizeof(u64) * 4;
 };
 
 // One segment's tiles [first, end) by one CTA; the partial result goes to `part`.
@@ -253,7 +258,9 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     constexpr u32 kSide = 16 * D;   // bytes of a tile's keys, and of its values
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
     u8* ring = smem + warp * NS * 2 * kSide;
-    float* join_o = reinterpret_cast<float*>(smem);  // [kWarps][R][D], after the loop
+    // after the loop [kWarps][R][D + 8], channel g D/8 + 2k + e of a row at 16 k + 2 g + e: then the
+    // lanes that write together meet different banks
+    float* join_o = reinterpret_cast<float*>(smem);
     using L = Layout<D, NT>;
     constexpr bool kShared = kSharedQueries<D, NT>;
     int4* note = reinterpret_cast<int4*>(smem + L::notes) + warp * NS;  // position, -, scales
@@ -646,15 +653,14 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             if (g == 0)
                 join_ml[warp * R + row] = make_float2(m[nt][i] == kNoScore ? -INFINITY : m[nt][i], sum);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                float* to = join_o + (warp * R + row) * D + g * (D / 8) + 2 * k;
-                to[0] = o[nt][k][i] * value_scale;
-                to[1] = o[nt][k][2 + i] * value_scale;
-            }
+            for (int k = 0; k < D / 16; ++k)
+                *reinterpret_cast<float2*>(join_o + (warp * R + row) * (D + 8) + k * 16 + g * 2) =
+                    make_float2(o[nt][k][i] * value_scale, o[nt][k][2 + i] * value_scale);
         }
     __syncthreads();
     for (u32 x = threadIdx.x; x < R * D; x += blockDim.x) {
-        const u32 row = x / D;
+        const u32 row = x / D, d = x % D;
+        const u32 place = row * (D + 8) + d % (D / 8) / 2 * 16 + d / (D / 8) * 2 + d % 2;
         float top = -INFINITY;
 #pragma unroll
         for (u32 w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * R + row].x);
@@ -664,7 +670,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         for (u32 w = 0; w < kWarps; ++w) {
             const float f = exp2_fast(join_ml[w * R + row].x - base);
             sum += join_ml[w * R + row].y * f;
-            value += join_o[w * R * D + x] * f;
+            value += join_o[w * R * (D + 8) + place] * f;
         }
         a.part_o[part * R * D + x] = value;
         if (x % D == 0) a.part_ml[part * R + row] = make_float2(top, sum);
@@ -676,15 +682,13 @@ template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(const AttentionArgs a)
 {
     extern __shared__ __align__(128) u8 smem[];
+    using L = Layout<D, NT>;
     kv_let_next();
-    const u64 total = line_of(a, reinterpret_cast<u64*>(smem + Layout<D, NT>::line));
-    const u64 share = share_of(a, total);
-    u64 at = blockIdx.x * share;
-    const u64 stop = min(at + share, total);
+    const Place place = place_of(a, reinterpret_cast<u64*>(smem + L::line), reinterpret_cast<Place*>(smem + L::line + 8 * kWarps));
+    u64 at = place.at, begin = place.begin;
+    const u64 stop = place.stop;
     if (at >= stop) return;
-    u32 unit;
-    u64 begin;
-    find_unit(a, at, unit, begin);
+    u32 unit = place.unit;
     u32 tiles = unit_tiles(a, unit);
     while (at < stop) {
         while (tiles == 0 || at >= begin + static_cast<u64>(tiles) * a.per_unit) {
