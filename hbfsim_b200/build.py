@@ -7,8 +7,11 @@ so it can be bound from ctypes, cgo, JNI or a C/C++ host alike.
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -33,22 +36,34 @@ def stale() -> bool:
     return any(p.stat().st_mtime > built for p in deps)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not stale():
-        return LIB
-    cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared",
-           "-Xcompiler", "-fPIC", "-cudart", "static",
-           "-Xptxas", "-warn-spills",
-           "-o", str(LIB), *map(str, sources())]
-    # exported C ABI: visibility comes from the version script below
-    script = CSRC / "exports.map"
-    cmd += ["-Xlinker", f"--version-script={script}"]
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("nvcc build of libhbfsim_b200.so failed")
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    if not force and not stale():
+        return LIB
+    flags = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
+    # exported C ABI: visibility comes from the version script below
+    script = CSRC / "exports.map"
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [Path(tmp) / (src.stem + ".o") for src in sources()]
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:  # file by file
+            list(pool.map(lambda x: _run([*flags, "-Xptxas", "-warn-spills", "-c", str(x[0]), "-o",
+                                          str(x[1])], verbose), zip(sources(), objects)))
+        made = Path(tmp) / LIB.name
+        _run([*flags, "-shared", "-cudart", "static", "-o", str(made), *map(str, objects),
+              "-Xlinker", f"--version-script={script}"], verbose)
+        # in place at once: a process that has the old file loaded keeps it
+        staged = LIB.with_suffix(".so.new")
+        shutil.copyfile(made, staged)
+        staged.chmod(0o755)
+        os.replace(staged, LIB)
     return LIB
 
 
