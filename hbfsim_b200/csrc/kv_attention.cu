@@ -43,6 +43,7 @@ constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
 constexpr float kAbove = 8.0f;
 constexpr float kNoScore = -3.0e38f;  // reference of a row without a score
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr u32 kWholeTiles = 32;     // segments of so many tiles at most need no finishing kernel
 constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
 struct AttentionArgs {
@@ -221,6 +222,20 @@ __device__ __forceinline__ int row_position(const AttentionArgs& a, const Segmen
 // Row tiles of 8 rows a CTA takes at most: the output accumulators of 32 rows
 // of 128 channels are 128 registers of a lane.
 constexpr u32 most_nt(u32 dim) { return dim == 256 ? 2 : 4; }
+// Row of out and lse behind a row of the segment.
+__device__ __forceinline__ u64 out_row(const AttentionArgs& a, const Segment& s, u32 row)
+{
+    const u32 t = a.blocks ? s.t : row / a.q.group;
+    return (static_cast<u64>(s.seq) * a.q.tokens + t) * a.q.q_heads + s.h * a.q.group + row % a.q.group;
+}
+
+__device__ __forceinline__ void put_out(const AttentionArgs& a, const Segment& s, u32 row, u32 d, float y)
+{
+    const u64 at = out_row(a, s, row) * a.c.dim + d;
+    if (a.q.type == HBFSIM_KV_BF16) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+    else static_cast<__half*>(a.out)[at] = __float2half_rn(y);
+}
+
 // CTAs per SM and the depth of a warp's ring, by registers and about 192 KB of rings.
 constexpr u32 per_sm(u32 dim, u32 nt)
 {
@@ -242,12 +257,13 @@ struct Layout {
     static constexpr u32 queries = join_ml + kWarps * 8 * NT * 8;
     static constexpr u32 factors = queries + (kSharedQueries<D, NT> ? NT * D * 16 : 0);
     static constexpr u32 ends = factors + 8 * NT * 4;
-    static constexpr u32 line = ends + 8 * NT * 4;
+    static constexpr u32 whole_lse = ends + 8 * NT * 4;  // [kWholeTiles][8 NT]
+    static constexpr u32 line = whole_lse + kWholeTiles * 8 * NT * 4;
     static constexpr u32 bytes = line + 8 * kWarps + sizeof(u64) * 4;
 };
 
 // One segment's tiles [first, end) by one CTA; the partial result goes to `part`.
-template <int D, int NT>
+template <int D, int NT, bool kWhole>
 __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segment& seg, u32 first,
                                             u32 end, u64 part, u8* smem)
 {
@@ -619,8 +635,10 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     };
 
     u32 stage = 0;
-    float* tile_out = a.tile_lse ? a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + first + warp) * R
-                                 : nullptr;
+    float* whole_lse = reinterpret_cast<float*>(smem + L::whole_lse);
+    float* tile_out = nullptr;
+    if (a.weights)
+        tile_out = (kWhole ? whole_lse : a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + first) * R) + warp * R;
     for (u32 i = 0; i < turns; ++i) {
         kv_copy_wait<NS - 2>();
         __syncwarp();  // the stage is there, and every lane is done with the one before it
@@ -672,17 +690,47 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             sum += join_ml[w * R + row].y * f;
             value += join_o[w * R * (D + 8) + place] * f;
         }
-        a.part_o[part * R * D + x] = value;
-        if (x % D == 0) a.part_ml[part * R + row] = make_float2(top, sum);
+        if constexpr (!kWhole) {
+            a.part_o[part * R * D + x] = value;
+            if (d == 0) a.part_ml[part * R + row] = make_float2(top, sum);
+        } else if (row < rows) {
+            put_out(a, seg, seg.rt * R + row, d, sum == 0.0f ? 0.0f : value / sum);
+            if (d == 0) {
+                const float lse2 = sum == 0.0f ? -INFINITY : log2f(sum) + base;
+                factors[row] = lse2;  // the queries' factors are not needed any more
+                if (a.lse) a.lse[out_row(a, seg, seg.rt * R + row)] = lse2 * kLn2;
+            }
+        }
     }
     __syncthreads();  // before the next segment's copies
+    if (kWhole && a.weights) {  // one row tile and one list: the weights are this CTA's
+        float* weights = a.weights + (static_cast<u64>(seg.seq) * a.c.heads + seg.h) * a.q.width;
+        const u32 listed = (end + (1u << sub_bits) - 1) >> sub_bits;
+        if (list || listed < a.q.width) {
+            for (u32 j = threadIdx.x; j < a.q.width; j += blockDim.x) weights[j] = 0.0f;
+            __syncthreads();
+        }
+        for (u32 k = threadIdx.x; k < listed; k += blockDim.x) {
+            float w = 0.0f;
+            for (u32 t = k << sub_bits; t < min((k + 1) << sub_bits, end); ++t)
+                for (u32 r = 0; r < rows; ++r)
+                    if (whole_lse[t * R + r] != -INFINITY) w += exp2_fast(whole_lse[t * R + r] - factors[r]);
+            const u32 j = list ? static_cast<u32>(list[k]) : k;
+            if (j < a.q.width) weights[j] = w;
+        }
+    }
 }
 
-template <int D, int NT>
+template <int D, int NT, bool kWhole>
 __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(const AttentionArgs a)
 {
     extern __shared__ __align__(128) u8 smem[];
     using L = Layout<D, NT>;
+    if constexpr (kWhole) {  // one CTA per segment, which it finishes
+        const Segment seg = segment_of(a, blockIdx.x);
+        run_segment<D, NT, true>(a, seg, 0, seg.tiles, 0, smem);
+        return;
+    }
     kv_let_next();
     const Place place = place_of(a, reinterpret_cast<u64*>(smem + L::line), reinterpret_cast<Place*>(smem + L::line + 8 * kWarps));
     u64 at = place.at, begin = place.begin;
@@ -704,7 +752,7 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
             if (first == 0) a.span[seg.index].x = blockIdx.x;
             if (end == tiles) a.span[seg.index].y = blockIdx.x;
         }
-        run_segment<D, NT>(a, seg, first, end, static_cast<u64>(blockIdx.x) + seg.index, smem);
+        run_segment<D, NT, false>(a, seg, first, end, static_cast<u64>(blockIdx.x) + seg.index, smem);
         at = here + end;
     }
 }
@@ -842,7 +890,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
 }
 
 struct Plan {
-    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles;
+    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole;
     u64 segments, part_o, part_ml, span, tile_lse, bytes;
 };
 
@@ -864,6 +912,14 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     const u64 most = (p.segments * p.tiles + kShare - 1) / kShare;
     p.workers = static_cast<u32>(
         std::max<u64>(1, std::min<u64>(most, static_cast<u64>(per_sm(v.dim, p.nt)) * kv_sm_count())));
+    // Short segments (by the table's width or the lists' length) are finished where they are
+    // summed: one launch, where the even split takes two.
+    p.whole = p.tiles <= kWholeTiles && (!weights || p.lists * p.row_tiles == 1);
+    if (p.whole) {
+        p.workers = static_cast<u32>(p.segments);
+        p.bytes = 256;
+        return p;
+    }
     u64 at = 0;
     auto take = [&](u64 bytes) {
         const u64 here = at;
@@ -890,12 +946,20 @@ int check_args(const hbfsim_kv_attention_args_v1* g)
     return HBFSIM_OK;
 }
 
-template <int D, int NT>
-int launch(const AttentionArgs& a, cudaStream_t s)
+template <int D, int NT, bool kWhole>
+bool launch_attention(const AttentionArgs& a, cudaStream_t s)
 {
     static std::atomic<u64> seen{0};
-    if (!kv_allow_smem(attention_kernel<D, NT>, Layout<D, NT>::bytes, seen)) return HBFSIM_CUDA_ERROR;
-    attention_kernel<D, NT><<<a.workers, kWarps * 32, Layout<D, NT>::bytes, s>>>(a);
+    if (!kv_allow_smem(attention_kernel<D, NT, kWhole>, Layout<D, NT>::bytes, seen)) return false;
+    attention_kernel<D, NT, kWhole><<<a.workers, kWarps * 32, Layout<D, NT>::bytes, s>>>(a);
+    return cudaGetLastError() == cudaSuccess;
+}
+
+template <int D, int NT>
+int launch(const AttentionArgs& a, bool whole, cudaStream_t s)
+{
+    if (whole) return launch_attention<D, NT, true>(a, s) ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    if (!launch_attention<D, NT, false>(a, s)) return HBFSIM_CUDA_ERROR;
     // one CTA per segment; for the weights of long sequences more, up to what is resident at once
     const u32 pairs = a.q.seqs * a.c.heads, segments = a.lists * a.row_tiles;
     u32 across = segments;
@@ -905,7 +969,7 @@ int launch(const AttentionArgs& a, cudaStream_t s)
     const u32 slices = std::min(std::max(1u, across / segments), 8u);
     const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, 0, 1, a,
                                      static_cast<u32>(8 * NT), slices);
-    return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
 }  // namespace
@@ -959,18 +1023,18 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     a.part_o = reinterpret_cast<float*>(w + p.part_o);
     a.part_ml = reinterpret_cast<float2*>(w + p.part_ml);
     a.span = reinterpret_cast<uint2*>(w + p.span);
-    a.tile_lse = a.weights ? reinterpret_cast<float*>(w + p.tile_lse) : nullptr;
+    a.tile_lse = a.weights && !p.whole ? reinterpret_cast<float*>(w + p.tile_lse) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (a.c.dim * 8 + p.nt) {
-    case 64 * 8 + 1: return launch<64, 1>(a, s);
-    case 64 * 8 + 2: return launch<64, 2>(a, s);
-    case 64 * 8 + 3: return launch<64, 3>(a, s);
-    case 64 * 8 + 4: return launch<64, 4>(a, s);
-    case 128 * 8 + 1: return launch<128, 1>(a, s);
-    case 128 * 8 + 2: return launch<128, 2>(a, s);
-    case 128 * 8 + 3: return launch<128, 3>(a, s);
-    case 128 * 8 + 4: return launch<128, 4>(a, s);
-    case 256 * 8 + 1: return launch<256, 1>(a, s);
-    default: return launch<256, 2>(a, s);
+    case 64 * 8 + 1: return launch<64, 1>(a, p.whole, s);
+    case 64 * 8 + 2: return launch<64, 2>(a, p.whole, s);
+    case 64 * 8 + 3: return launch<64, 3>(a, p.whole, s);
+    case 64 * 8 + 4: return launch<64, 4>(a, p.whole, s);
+    case 128 * 8 + 1: return launch<128, 1>(a, p.whole, s);
+    case 128 * 8 + 2: return launch<128, 2>(a, p.whole, s);
+    case 128 * 8 + 3: return launch<128, 3>(a, p.whole, s);
+    case 128 * 8 + 4: return launch<128, 4>(a, p.whole, s);
+    case 256 * 8 + 1: return launch<256, 1>(a, p.whole, s);
+    default: return launch<256, 2>(a, p.whole, s);
     }
 }

@@ -230,14 +230,13 @@ def kv_select(cache: KvCache, q, table, lengths, top: int, sink: int = 1, recent
     if not _here(cache.index, stream):
         with _On(cache.index, stream):
             return kv_select(cache, q, table, lengths, top, sink, recent)
-    import torch
     _need(top >= 0 and sink >= 0 and recent >= 0, "top, sink and recent are counts")
     query, seqs, tokens, _, _ = _query(cache, q, table, lengths)
-    lib, device = _lib.load(), q.device
-    blocks = torch.empty((seqs, tokens, cache.kv_heads, top), dtype=torch.int32, device=device)
-    counts = torch.empty((seqs, tokens, cache.kv_heads), dtype=torch.int32, device=device)
+    lib = _lib.load()
+    blocks = table.new_empty((seqs, tokens, cache.kv_heads, top))
+    counts = table.new_empty((seqs, tokens, cache.kv_heads))
     size = lib.hbfsim_kv_select_workspace_v1(cache._packed, query)
-    space = torch.empty(size, dtype=torch.uint8, device=device)
+    space = cache.bounds.new_empty(size)
     check(lib.hbfsim_kv_select_v1(cache._packed, query, top, sink, recent, blocks.data_ptr(),
                                   counts.data_ptr(), space.data_ptr(), size, _handle(cache.index)),
           "hbfsim_kv_select_v1")
@@ -274,21 +273,21 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
         blocks_at, counts_at = blocks.data_ptr() or 16, counts.data_ptr() or 16  # 0: no lists
     else:
         _need(counts is None, "counts without blocks")
-    lib, device = _lib.load(), q.device
-    out = torch.empty((seqs, tokens, q_heads, cache.head_dim), dtype=q.dtype, device=device)
-    lse = torch.empty((seqs, tokens, q_heads), dtype=torch.float32, device=device)
+    lib = _lib.load()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = cache.scale.new_empty((seqs, tokens, q_heads))
     mass, mass_at = None, 0
     if weights:
         # with no query token nothing is launched and every weight is 0
-        make = torch.empty if tokens else torch.zeros
-        mass = make((seqs, cache.kv_heads, width), dtype=torch.float32, device=device)
+        make = cache.scale.new_empty if tokens else cache.scale.new_zeros
+        mass = make((seqs, cache.kv_heads, width))
         mass_at = mass.data_ptr()
     if scale is None:
         scale = cache.head_dim ** -0.5
     head = (_ATTENTION.size, 1, scale, top, blocks_at, counts_at, out.data_ptr(), lse.data_ptr(),
             mass_at)
     size = lib.hbfsim_kv_attention_workspace_v1(cache._packed, query, _ATTENTION.pack(*head, 0, 0))
-    space = torch.empty(size, dtype=torch.uint8, device=device)
+    space = cache.bounds.new_empty(size)
     check(lib.hbfsim_kv_attention_v1(cache._packed, query,
                                      _ATTENTION.pack(*head, space.data_ptr(), size),
                                      _handle(cache.index)), "hbfsim_kv_attention_v1")
@@ -319,12 +318,9 @@ def kv_evict(score, weights, table, lengths, keep: int, block_tokens: int = 16, 
           "weights: float32 [seqs, kv_heads, width], contiguous")
     _need(min(keep, block_tokens, sink, recent, decay) >= 0,
           "keep, block_tokens, sink, recent and decay are counts")
-    device = table.device
     new_score = torch.empty_like(score)
-    new_table = torch.empty(shape, dtype=torch.int32, device=device)
-    new_lengths = torch.empty(seqs, dtype=torch.int32, device=device)
-    freed = torch.empty(shape, dtype=torch.int32, device=device)
-    freed_counts = torch.empty(seqs, dtype=torch.int32, device=device)
+    new_table, freed = table.new_empty((2, seqs, width)).unbind(0)
+    new_lengths, freed_counts = table.new_empty((2, seqs)).unbind(0)
     batch = _EVICT.pack(_EVICT.size, 1, seqs, weights.shape[1], width, block_tokens, keep, sink,
                         recent, decay, score.data_ptr(), weights.data_ptr(), table.data_ptr(),
                         table.stride(0), lengths.data_ptr(), new_score.data_ptr(),

@@ -244,16 +244,22 @@ ATTENDS = [  # dim, block, heads, group, tokens, type, lengths
     (64, 16, 2, 64, 1, "f16", [50, 16]),
     (128, 32, 1, 12, 16, "f16", [10, 16, 40]),
     (64, 16, 1, 1, 1, "bf16", [5000]),
+    (64, 16, 2, 8, 3, "f16", [700, 23]),
+    (128, 16, 1, 8, 4, "bf16", [333]),
+    (256, 32, 1, 4, 6, "f16", [450, 6]),
 ]
 
 
+@pytest.mark.parametrize("extra", [3, 40])
 @pytest.mark.parametrize("dim,block,heads,group,tokens,kind,lengths", ATTENDS)
-def test_attention(dim, block, heads, group, tokens, kind, lengths):
+def test_attention(dim, block, heads, group, tokens, kind, lengths, extra):
+    """extra: blocks that the table has room for beyond the longest sequence (short rows are
+    finished by one kernel, wider ones are shared out and joined)."""
     torch = torch_()
     rng = np.random.default_rng(dim + block + heads + group + tokens)
     pages = int(sum(-(-n // block) for n in lengths)) + 2
     cache = random_cache(rng, pages, heads, block, dim)
-    table = make_table(rng, lengths, block, pages, extra=3)
+    table = make_table(rng, lengths, block, pages, extra=extra)
     # what no token uses is NaN
     for b, n in enumerate(lengths):
         if n % block:
@@ -325,15 +331,17 @@ def test_attention_extreme_sizes(q_size, key_exp, value_exp):
     attend_and_check(cache, q, table, [300], scale=-scale)
 
 
-def test_attention_nan_stays_in_the_rows_that_see_it():
+@pytest.mark.parametrize("dim,group,tokens,extra", [(64, 2, 6, 0), (128, 8, 4, 40), (256, 3, 5, 0),
+                                                    (128, 4, 2, 0)])
+def test_attention_nan_stays_in_the_rows_that_see_it(dim, group, tokens, extra):
     """A key and a value that are NaN at the last positions: earlier query tokens must not
     meet them, later ones do."""
     torch = torch_()
     from hbfsim_b200 import kv_attention
     rng = np.random.default_rng(14)
-    dim, block, heads, group, tokens, n = 64, 16, 1, 2, 6, 40
+    block, heads, n = 16, 1, 40
     cache = random_cache(rng, 3, heads, block, dim)
-    table = make_table(rng, [n], block, 3)
+    table = make_table(rng, [n], block, 3, extra=extra)
     q = torch.from_numpy(rng.standard_normal((1, tokens, group, dim))).to(torch.float16).cuda()
     clean = attend_and_check(cache, q, table, [n], weights=False)
     for side in (0, 1):
