@@ -26,8 +26,8 @@
 // stride over the tiles of its share of a segment, each with a ring of
 // asynchronous copies of its own (no block barrier inside the loop), join
 // through shared memory and leave one partial result per segment met;
-// finish_kernel joins the partials of a segment and turns the tiles'
-// logarithmic sums into block weights.
+// finish_kernel joins the partials of a segment and turns the tiles' sums
+// into block weights.
 #include "kv.h"
 
 #include <algorithm>
@@ -65,7 +65,7 @@ struct AttentionArgs {
     float* part_o;                // [workers + segments][8 NT][D], at worker + segment
     float2* part_ml;              // [workers + segments][8 NT]: maximum, sum
     uint2* span;                  // [segments]: first and last worker (segments with tiles)
-    float* tile_lse;              // [segments][tiles][8 NT], or NULL
+    float2* tile_sums;            // [segments][tiles][8 NT] or NULL: sum of exponentials, reference
 };
 
 // Four stored values as f16 pairs: exact.
@@ -108,13 +108,6 @@ __device__ __forceinline__ float exp2_fast(float x)  // 2^-22 relative, 0 for -i
 {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-__device__ __forceinline__ float log2_fast(float x)  // 2^-22 absolute or relative, -inf for 0
-{
-    float r;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -257,8 +250,8 @@ struct Layout {
     static constexpr u32 queries = join_ml + kWarps * 8 * NT * 8;
     static constexpr u32 factors = queries + (kSharedQueries<D, NT> ? NT * D * 16 : 0);
     static constexpr u32 ends = factors + 8 * NT * 4;
-    static constexpr u32 whole_lse = ends + 8 * NT * 4;  // [kWholeTiles][8 NT]
-    static constexpr u32 line = whole_lse + kWholeTiles * 8 * NT * 4;
+    static constexpr u32 whole_sums = ends + 8 * NT * 4;  // [kWholeTiles][8 NT]
+    static constexpr u32 line = whole_sums + kWholeTiles * 8 * NT * 8;
     static constexpr u32 bytes = line + 8 * kWarps + sizeof(u64) * 4;
 };
 
@@ -446,7 +439,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     };
     // One tile.  `edge`: some row does not see all of its tokens.
     auto consume = [&](auto is_edge, const u8* tile, int p0, float key_scale, float new_scale,
-                       float* tile_out) {
+                       float2* tile_out) {
         constexpr bool kEdge = decltype(is_edge)::value;
         // with one row tile two sums, so that products need not wait for each other
         constexpr int kSums = NT == 1 ? 2 : 1;
@@ -578,9 +571,8 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 float all = mine + __shfl_xor_sync(0xffffffffu, other, 4);
                 all += __shfl_xor_sync(0xffffffffu, all, 8);
                 all += __shfl_xor_sync(0xffffffffu, all, 16);
-                if (g < 2)
-                    tile_out[nt * 8 + 2 * c + g] =
-                        all == 0.0f ? -INFINITY : log2_fast(all) + (g ? m[nt][1] : m[nt][0]);
+                const u32 row = nt * 8 + 2 * c + g;
+                if (g < 2 && row < rows) tile_out[row] = make_float2(all, g ? m[nt][1] : m[nt][0]);
             }
         }
         u32 keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // value tokens that some row sees
@@ -635,10 +627,10 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     };
 
     u32 stage = 0;
-    float* whole_lse = reinterpret_cast<float*>(smem + L::whole_lse);
-    float* tile_out = nullptr;
+    float2* whole_sums = reinterpret_cast<float2*>(smem + L::whole_sums);
+    float2* tile_out = nullptr;
     if (a.weights)
-        tile_out = (kWhole ? whole_lse : a.tile_lse + (static_cast<u64>(seg.index) * a.tiles + first) * R) + warp * R;
+        tile_out = (kWhole ? whole_sums : a.tile_sums + (static_cast<u64>(seg.index) * a.tiles + first) * R) + warp * R;
     for (u32 i = 0; i < turns; ++i) {
         kv_copy_wait<NS - 2>();
         __syncwarp();  // the stage is there, and every lane is done with the one before it
@@ -647,7 +639,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         const u8* tile = ring + stage * 2 * kSide;
         stage = stage + 1 == NS ? 0 : stage + 1;
         if (noted.x < 0) {
-            if (tile_out && lane < R) tile_out[lane] = -INFINITY;
+            if (tile_out && lane < rows) tile_out[lane] = make_float2(0.0f, kNoScore);
         } else if (noted.x + 15 > sees_least) {
             consume(std::true_type{}, tile, noted.x, __int_as_float(noted.z), __int_as_float(noted.w),
                     tile_out);
@@ -676,6 +668,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                     make_float2(o[nt][k][i] * value_scale, o[nt][k][2 + i] * value_scale);
         }
     __syncthreads();
+    float* inverses = reinterpret_cast<float*>(ends);
     for (u32 x = threadIdx.x; x < R * D; x += blockDim.x) {
         const u32 row = x / D, d = x % D;
         const u32 place = row * (D + 8) + d % (D / 8) / 2 * 16 + d / (D / 8) * 2 + d % 2;
@@ -696,9 +689,9 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         } else if (row < rows) {
             put_out(a, seg, seg.rt * R + row, d, sum == 0.0f ? 0.0f : value / sum);
             if (d == 0) {
-                const float lse2 = sum == 0.0f ? -INFINITY : log2f(sum) + base;
-                factors[row] = lse2;  // the queries' factors are not needed any more
-                if (a.lse) a.lse[out_row(a, seg, seg.rt * R + row)] = lse2 * kLn2;
+                factors[row] = base;  // the queries' factors and ends are not needed any more
+                inverses[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (a.lse) a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
             }
         }
     }
@@ -714,7 +707,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             float w = 0.0f;
             for (u32 t = k << sub_bits; t < min((k + 1) << sub_bits, end); ++t)
                 for (u32 r = 0; r < rows; ++r)
-                    if (whole_lse[t * R + r] != -INFINITY) w += exp2_fast(whole_lse[t * R + r] - factors[r]);
+                    w += whole_sums[t * R + r].x * (exp2_fast(whole_sums[t * R + r].y - factors[r]) * inverses[r]);
             const u32 j = list ? static_cast<u32>(list[k]) : k;
             if (j < a.q.width) weights[j] = w;
         }
@@ -763,7 +756,7 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
 // share of the blocks.  All sums run in a fixed order.
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R, u32 slices)
 {
-    __shared__ float row_top[32], row_sum[32], row_lse[32];  // of the segment at hand
+    __shared__ float row_top[32], row_sum[32], row_inverse[32];  // of the segment at hand
     __shared__ float4 join[kFinishThreads];
     const u32 i = threadIdx.x, lane = i & 31u, warp = i >> 5;
     kv_wait_before();
@@ -771,7 +764,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
     const u32 sub_bits = 27 - __clz(a.c.block), D = a.c.dim;
     const u32 each = (a.q.width + gridDim.x - 1) / gridDim.x;
     const u32 from = min(blockIdx.x * each, a.q.width), to_block = min(from + each, a.q.width);
-    float* weights = a.tile_lse ? a.weights + (static_cast<u64>(seq) * a.c.heads + h) * a.q.width
+    float* weights = a.tile_sums ? a.weights + (static_cast<u64>(seq) * a.c.heads + h) * a.q.width
                                 : nullptr;
     for (u32 n = 0; n < a.lists * a.row_tiles; ++n) {
         u32 slice = n % gridDim.x == blockIdx.x ? 0 : slices;
@@ -799,7 +792,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
             if (lane == 0) {
                 row_top[r] = base;
                 row_sum[r] = all;
-                row_lse[r] = all == 0.0f ? -INFINITY : log2f(all) + base;
+                row_inverse[r] = all == 0.0f ? 0.0f : 1.0f / all;
             }
         }
         __syncthreads();
@@ -838,7 +831,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                         v.w += y.w;
                     }
                 }
-                const float inverse = row_sum[r] == 0.0f ? 0.0f : 1.0f / row_sum[r];
+                const float inverse = row_inverse[r];
                 const u32 row = rt * R + r, d = x * 4 % D;
                 const u32 tt = a.blocks ? t : row / a.q.group;
                 const u32 qh = h * a.q.group + row % a.q.group;
@@ -851,22 +844,21 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                     else
                         static_cast<__half*>(a.out)[to * D + d + k] = __float2half_rn(y[k]);
                 }
-                if (d == 0 && a.lse) a.lse[to] = row_lse[r] * kLn2;
+                if (d == 0 && a.lse)
+                    a.lse[to] = row_sum[r] == 0.0f ? -INFINITY : (log2f(row_sum[r]) + base) * kLn2;
             }
         }
         if (!weights) continue;
         const u32 listed = (tiles + (1u << sub_bits) - 1) >> sub_bits;
-        const float* lse = a.tile_lse + static_cast<u64>(index) * a.tiles * R;
+        const float2* sums = a.tile_sums + static_cast<u64>(index) * a.tiles * R;
         auto weight_of = [&](u32 k) {
             float w = 0.0f;
             for (u32 tile = k << sub_bits; tile < min((k + 1) << sub_bits, tiles); ++tile) {
-                const float4* x = reinterpret_cast<const float4*>(lse + static_cast<u64>(tile) * R);
-                for (u32 r = 0; r < rows; r += 4) {
-                    const float4 y = x[r / 4];
-                    const float z[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (u32 q = 0; q < 4; ++q)
-                        if (r + q < rows && z[q] != -INFINITY) w += exp2_fast(z[q] - row_lse[r + q]);
+                const float4* x = reinterpret_cast<const float4*>(sums + static_cast<u64>(tile) * R);
+                for (u32 r = 0; r < rows; r += 2) {
+                    const float4 y = x[r / 2];  // two rows' sums and references
+                    w += y.x * (exp2_fast(y.y - row_top[r]) * row_inverse[r]);
+                    if (r + 1 < rows) w += y.z * (exp2_fast(y.w - row_top[r + 1]) * row_inverse[r + 1]);
                 }
             }
             return w;
@@ -891,7 +883,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
 
 struct Plan {
     u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole;
-    u64 segments, part_o, part_ml, span, tile_lse, bytes;
+    u64 segments, part_o, part_ml, span, tile_sums, bytes;
 };
 
 Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weights)
@@ -929,7 +921,7 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     p.part_o = take((p.segments + p.workers) * R * v.dim * 4);
     p.part_ml = take((p.segments + p.workers) * R * 8);
     p.span = take(p.segments * 8);
-    p.tile_lse = take(weights ? p.segments * p.tiles * R * 4 : 0);
+    p.tile_sums = take(weights ? p.segments * p.tiles * R * 8 : 0);
     p.bytes = at;
     return p;
 }
@@ -1023,7 +1015,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     a.part_o = reinterpret_cast<float*>(w + p.part_o);
     a.part_ml = reinterpret_cast<float2*>(w + p.part_ml);
     a.span = reinterpret_cast<uint2*>(w + p.span);
-    a.tile_lse = a.weights && !p.whole ? reinterpret_cast<float*>(w + p.tile_lse) : nullptr;
+    a.tile_sums = a.weights && !p.whole ? reinterpret_cast<float2*>(w + p.tile_sums) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (a.c.dim * 8 + p.nt) {
     case 64 * 8 + 1: return launch<64, 1>(a, p.whole, s);
