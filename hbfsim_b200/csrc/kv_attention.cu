@@ -2,7 +2,7 @@
 // cache (kv_v1.h), over all blocks of a sequence or over listed ones.
 //
 // The query rows that share a key/value head (group heads times tokens) are
-// taken 8 to 32 at a time as the narrow side of the tensor-core products, so
+// taken 8 to 24 at a time as the narrow side of the tensor-core products, so
 // that the tokens are the wide one:
 //
 //   S^T [16 tokens x rows]  = K [16 x D] Q^T [D x rows]
@@ -212,9 +212,12 @@ __device__ __forceinline__ int row_position(const AttentionArgs& a, const Segmen
     return max(s.length - static_cast<int>(a.q.tokens) + static_cast<int>(t), -1);
 }
 
-// Row tiles of 8 rows a CTA takes at most: the output accumulators of 32 rows
-// of 128 channels are 128 registers of a lane.
-constexpr u32 most_nt(u32 dim) { return dim == 256 ? 2 : 4; }
+// Row tiles of 8 rows that a pass takes.  Wide passes widen the cache's values
+// less often but leave fewer warps on an SM: 24 rows of 128 channels in one
+// pass took 45 us where two passes of 16 took 49, 40 rows in three passes of
+// 16 took 63 where two of 24 took 69 (8 sequences of 700 to 9001 tokens, 8
+// heads).  At 256 channels the accumulators leave room for 16 rows.
+constexpr u32 pass_width(u32 eights, u32 dim) { return eights <= 2 || (eights == 3 && dim < 256) ? eights : 2; }
 // Row of out and lse behind a row of the segment.
 __device__ __forceinline__ u64 out_row(const AttentionArgs& a, const Segment& s, u32 row)
 {
@@ -232,7 +235,7 @@ __device__ __forceinline__ void put_out(const AttentionArgs& a, const Segment& s
 // CTAs per SM and the depth of a warp's ring, by registers and about 192 KB of rings.
 constexpr u32 per_sm(u32 dim, u32 nt)
 {
-    return dim == 256 ? 2 : dim == 128 ? (nt == 1 ? 4 : nt == 2 ? 3 : 2) : (nt <= 2 ? 4 : 3);
+    return dim == 256 ? 2 : dim == 128 ? 5 - nt : (nt <= 2 ? 4 : 3);
 }
 template <int D>
 constexpr u32 kStages = D == 64 ? 4 : 3;
@@ -756,7 +759,7 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
 // share of the blocks.  All sums run in a fixed order.
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R, u32 slices)
 {
-    __shared__ float row_top[32], row_sum[32], row_inverse[32];  // of the segment at hand
+    __shared__ float row_top[24], row_sum[24], row_inverse[24];  // of the segment at hand
     __shared__ float4 join[kFinishThreads];
     const u32 i = threadIdx.x, lane = i & 31u, warp = i >> 5;
     kv_wait_before();
@@ -891,9 +894,7 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     Plan p{};
     p.lists = lists ? q.tokens : 1;
     p.rows = lists ? q.group : q.group * q.tokens;
-    // as few passes over the tiles as registers allow, of equal width
-    const u32 eights = (p.rows + 7) / 8, passes = (eights + most_nt(v.dim) - 1) / most_nt(v.dim);
-    p.nt = (eights + passes - 1) / passes;
+    p.nt = pass_width((p.rows + 7) / 8, v.dim);
     const u32 R = 8 * p.nt;
     p.row_tiles = (p.rows + R - 1) / R;
     p.tiles = (lists ? top : q.width) * (v.block / 16);
@@ -952,12 +953,13 @@ int launch(const AttentionArgs& a, bool whole, cudaStream_t s)
 {
     if (whole) return launch_attention<D, NT, true>(a, s) ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
     if (!launch_attention<D, NT, false>(a, s)) return HBFSIM_CUDA_ERROR;
-    // one CTA per segment; for the weights of long sequences more, up to what is resident at once
+    // one CTA per segment or more, up to what is resident at once; for the weights no more than
+    // have blocks to sum
     const u32 pairs = a.q.seqs * a.c.heads, segments = a.lists * a.row_tiles;
-    u32 across = segments;
+    u32 across = std::max(segments, std::min(segments * 8, 4u * kv_sm_count() / pairs));
     if (a.weights)
-        across = std::max(across, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
-                                           4u * kv_sm_count() / pairs));
+        across = std::max(segments, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
+                                             4u * kv_sm_count() / pairs));
     const u32 slices = std::min(std::max(1u, across / segments), 8u);
     const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, 0, 1, a,
                                      static_cast<u32>(8 * NT), slices);
@@ -1021,11 +1023,9 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     case 64 * 8 + 1: return launch<64, 1>(a, p.whole, s);
     case 64 * 8 + 2: return launch<64, 2>(a, p.whole, s);
     case 64 * 8 + 3: return launch<64, 3>(a, p.whole, s);
-    case 64 * 8 + 4: return launch<64, 4>(a, p.whole, s);
     case 128 * 8 + 1: return launch<128, 1>(a, p.whole, s);
     case 128 * 8 + 2: return launch<128, 2>(a, p.whole, s);
     case 128 * 8 + 3: return launch<128, 3>(a, p.whole, s);
-    case 128 * 8 + 4: return launch<128, 4>(a, p.whole, s);
     case 256 * 8 + 1: return launch<256, 1>(a, p.whole, s);
     default: return launch<256, 2>(a, p.whole, s);
     }
