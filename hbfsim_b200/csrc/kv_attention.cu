@@ -235,10 +235,10 @@ __device__ __forceinline__ void put_out(const AttentionArgs& a, const Segment& s
 // CTAs per SM and the depth of a warp's ring, by registers and about 192 KB of rings.
 constexpr u32 per_sm(u32 dim, u32 nt)
 {
-    return dim == 256 ? 2 : dim == 128 ? 5 - nt : (nt <= 2 ? 4 : 3);
+    return dim == 256 ? 2 : dim == 128 ? (nt == 3 ? 2 : 3) : (nt <= 2 ? 4 : 3);
 }
 template <int D>
-constexpr u32 kStages = D == 64 ? 4 : 3;
+constexpr u32 kStages = D == 256 ? 3 : 4;
 template <int D>
 constexpr u32 kRing = kWarps * kStages<D> * 32 * D;  // bytes
 // One row tile's queries stay in registers; more are read from shared memory for each tile.
