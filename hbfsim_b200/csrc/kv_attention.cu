@@ -753,8 +753,8 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
     }
 }
 
-// CTAs (x, sequence * heads + head).  The segments of a (sequence, head) are
-// joined by the CTAs x = 0, 1, .. in turn, or, with more CTAs than segments,
+// CTAs (sequence * heads + head, y).  The segments of a (sequence, head) are
+// joined by the CTAs y = 0, 1, .. in turn, or, with more CTAs than segments,
 // each by `slices` of them; with weights every CTA also sums those of its
 // share of the blocks.  All sums run in a fixed order.
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R, u32 slices)
@@ -763,15 +763,15 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
     __shared__ float4 join[kFinishThreads];
     const u32 i = threadIdx.x, lane = i & 31u, warp = i >> 5;
     kv_wait_before();
-    const u32 h = blockIdx.y % a.c.heads, seq = blockIdx.y / a.c.heads;
+    const u32 h = blockIdx.x % a.c.heads, seq = blockIdx.x / a.c.heads;
     const u32 sub_bits = 27 - __clz(a.c.block), D = a.c.dim;
-    const u32 each = (a.q.width + gridDim.x - 1) / gridDim.x;
-    const u32 from = min(blockIdx.x * each, a.q.width), to_block = min(from + each, a.q.width);
+    const u32 each = (a.q.width + gridDim.y - 1) / gridDim.y;
+    const u32 from = min(blockIdx.y * each, a.q.width), to_block = min(from + each, a.q.width);
     float* weights = a.tile_sums ? a.weights + (static_cast<u64>(seq) * a.c.heads + h) * a.q.width
                                 : nullptr;
     for (u32 n = 0; n < a.lists * a.row_tiles; ++n) {
-        u32 slice = n % gridDim.x == blockIdx.x ? 0 : slices;
-        if (slices > 1) slice = blockIdx.x - n * slices;  // wraps for CTAs of other segments
+        u32 slice = n % gridDim.y == blockIdx.y ? 0 : slices;
+        if (slices > 1) slice = blockIdx.y - n * slices;  // wraps for CTAs of other segments
         const bool joins = slice < slices;
         if (!joins && !weights) continue;
         const u32 t = n / a.row_tiles, rt = n % a.row_tiles;
@@ -961,7 +961,7 @@ int launch(const AttentionArgs& a, bool whole, cudaStream_t s)
         across = std::max(segments, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
                                              4u * kv_sm_count() / pairs));
     const u32 slices = std::min(std::max(1u, across / segments), 8u);
-    const bool ok = kv_launch_behind(finish_kernel, dim3(across, pairs), kFinishThreads, s, 0, 1, a,
+    const bool ok = kv_launch_behind(finish_kernel, dim3(pairs, across), kFinishThreads, s, 0, 1, a,
                                      static_cast<u32>(8 * NT), slices);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
@@ -992,8 +992,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     if (const int rc = check_args(args)) return rc;
     if (a.q.seqs == 0 || a.q.tokens == 0) return HBFSIM_OK;
     const Plan p = plan_of(a.c, a.q, args->blocks != nullptr, args->top, args->weights != nullptr);
-    if (p.segments > 0x7fffffffull || a.q.seqs * static_cast<u64>(a.c.heads) > 65535)
-        return HBFSIM_UNSUPPORTED;
+    if (p.segments > 0x7fffffffull) return HBFSIM_UNSUPPORTED;
     if (!args->out || !args->workspace || args->workspace_bytes < p.bytes ||
         !kv_aligned(args->workspace, 16) || !kv_aligned(args->out, 2) ||
         !kv_aligned(args->lse, 4) || !kv_aligned(args->weights, 4) ||

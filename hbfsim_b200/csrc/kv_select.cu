@@ -442,11 +442,12 @@ extern "C" int hbfsim_kv_select_v1(const hbfsim_kv_cache_v1* cache,
     if (workspace_bytes < workspace_bytes_of(a.c, a.q) || (a.q.width && !workspace) ||
         !kv_aligned(workspace, 16) || !kv_aligned(blocks, 4) || !kv_aligned(counts, 4))
         return HBFSIM_INVALID_ARGUMENT;
+    a.whole = static_cast<std::int8_t*>(workspace);
+    a.keys = reinterpret_cast<u32*>(static_cast<u8*>(workspace) + whole_bytes(a.c, a.q));
+    if (a.c.pages == 0) a.q.width = 0;  // no block is there
     a.top = top;
     a.sink = sink;
     a.recent = recent;
-    a.whole = static_cast<std::int8_t*>(workspace);
-    a.keys = reinterpret_cast<u32*>(static_cast<u8*>(workspace) + whole_bytes(a.c, a.q));
     a.blocks = blocks;
     a.counts = counts;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -421,6 +421,64 @@ def test_pool_past_32_bit_offsets():
         assert torch.equal(a, b)
 
 
+def test_nothing_there():
+    """A pool without pages, a table without columns, no sequences, no query tokens: outputs are
+    what they are for a query that sees nothing."""
+    torch = torch_()
+    from hbfsim_b200 import KvCache, kv_append, kv_attention, kv_evict, kv_select
+    q = torch.ones((2, 1, 4, 64), dtype=torch.float16, device="cuda")
+    k = torch.ones((2, 1, 2, 64), dtype=torch.float16, device="cuda")
+    for pages, width in ((0, 3), (4, 0), (0, 0), (0, 3000)):
+        gpu = KvCache.empty(pages, 2, 64)
+        table = torch.zeros((2, width), dtype=torch.int32, device="cuda")
+        lengths = int32([20, 40])
+        kv_append(gpu, k, k, table, lengths)
+        got = kv_attention(gpu, q, table, lengths, weights=True)
+        assert not got.out.any() and torch.isneginf(got.lse).all() and not got.weights.any()
+        pick = kv_select(gpu, q, table, lengths, top=3)
+        assert (pick.blocks == -1).all() and not pick.counts.any()
+        got = kv_attention(gpu, q, table, lengths, blocks=pick.blocks, counts=pick.counts, weights=True)
+        assert not got.out.any() and torch.isneginf(got.lse).all() and not got.weights.any()
+    gpu = KvCache.empty(4, 2, 64)
+    none = torch.zeros((0, 3), dtype=torch.int32, device="cuda")
+    assert kv_attention(gpu, q[:0], none, int32([]), weights=True).weights.shape == (0, 2, 3)
+    assert kv_select(gpu, q[:0], none, int32([]), top=2).blocks.shape == (0, 1, 2, 2)
+    kv_append(gpu, k[:0], k[:0], none, int32([]))
+    table = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    got = kv_attention(gpu, q[:, :0], table, int32([3, 3]), weights=True)
+    assert got.out.shape == (2, 0, 4, 64) and not got.weights.any()
+    rest = kv_evict(torch.zeros((2, 0), dtype=torch.int64, device="cuda"),
+                    torch.zeros((2, 1, 0), device="cuda"), table[:, :0], int32([5, 0]), keep=2)
+    assert rest.lengths.tolist() == [0, 0] and rest.freed_counts.tolist() == [0, 0]
+
+
+def test_many_sequences():
+    """More (sequence, head) pairs than a grid's second axis holds."""
+    torch = torch_()
+    from hbfsim_b200 import kv_attention, kv_evict, kv_select
+    rng = np.random.default_rng(17)
+    seqs, heads, dim, block = 40000, 2, 64, 16
+    small = random_cache(rng, 8, heads, block, dim)
+    table = rng.integers(0, 8, (seqs, 2)).astype(np.int32)
+    lengths = rng.integers(0, 33, seqs)
+    q = torch.from_numpy(rng.standard_normal((64, 1, 2 * heads, dim))).to(torch.bfloat16).cuda()
+    q = q.repeat(seqs // 64, 1, 1, 1)
+    gpu = to_gpu(small)
+    wide = np.concatenate([table, np.full((seqs, 40), -1, np.int32)], 1)  # not finished in one kernel
+    probe = rng.integers(0, seqs, 50)
+    want = ko.attention(small, q[probe].double().cpu().numpy(), table[probe], lengths[probe], dim ** -0.5)
+    for t in (table, wide):
+        got = kv_attention(gpu, q, int32(t), int32(lengths), weights=True)
+        assert np.abs(got.out[probe].double().cpu().numpy() - want[0]).max() <= \
+            (2.0 ** -8 * np.abs(want[0]) + 2.0 ** -10 * want[3] + 2.0 ** -20).max()
+        assert np.abs(got.weights[probe][..., :2].double().cpu().numpy() - want[2]).max() <= 2.0 ** -17
+        pick = kv_select(gpu, q, int32(t), int32(lengths), top=2)
+        assert np.array_equal(pick.counts.cpu().numpy()[:, 0, 0], -(-lengths // block))
+    rest = kv_evict(torch.zeros((seqs, 2), dtype=torch.int64, device="cuda"),
+                    torch.rand((seqs, heads, 2), device="cuda"), int32(table), int32(lengths), keep=2)
+    assert not rest.freed_counts.any()
+
+
 # ---------------------------------------------------------------------------
 # block lists
 
