@@ -690,3 +690,22 @@ def test_select_long_rows(blocks, top, heads):
     q = torch.from_numpy(rng.standard_normal((1, 1, heads, dim))).to(torch.bfloat16).cuda()
     got = kv_select(to_gpu(cache), q, int32(table), int32([blocks * block - 3]), top)
     assert_lists(got, ko.select(cache, q.double().cpu().numpy(), table, [blocks * block - 3], top, 1, 1))
+
+
+def test_example(capsys):
+    """The example: fewer reads and less simulated time for the lists than for every block, and
+    what is evicted is what goes beyond `keep`."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "kv_decode.py"
+    spec = importlib.util.spec_from_file_location("kv_decode", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    got = module.main(["--seqs", "3", "--context", "500", "--steps", "20", "--top", "6", "--keep", "20"])
+    assert "listed_reads" in capsys.readouterr().out
+    assert got["listed_reads"] == 3 * 20 * 8 * 6
+    # 32 blocks after the first token; 20 stay, then one leaves for each that begins
+    begun = [-(-(500 + 20) // 16) - 32] * 3
+    assert got["evicted_blocks"] == sum(12 + n for n in begun)
+    assert got["every_reads"] > 3 * got["listed_reads"]
+    assert got["every_us_per_step"] > got["listed_us_per_step"] > 0
