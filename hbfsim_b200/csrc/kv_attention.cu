@@ -62,7 +62,8 @@ struct AttentionArgs {
     u32 units, per_unit;
     u32 workers;                  // CTAs of attention_kernel
     u32 tiles;                    // 16-token tiles per segment at most
-    float* part_o;                // [workers + segments][8 NT][D], at worker + segment
+    float* part_o;                // [workers + segments][8 NT][D], at worker + segment, channels
+                                  // in the joined order
     float2* part_ml;              // [workers + segments][8 NT]: maximum, sum
     uint2* span;                  // [segments]: first and last worker (segments with tiles)
     float2* tile_sums;            // [segments][tiles][8 NT] or NULL: sum of exponentials, reference
@@ -218,6 +219,11 @@ __device__ __forceinline__ int row_position(const AttentionArgs& a, const Segmen
 // 16 took 63 where two of 24 took 69 (8 sequences of 700 to 9001 tokens, 8
 // heads).  At 256 channels the accumulators leave room for 16 rows.
 constexpr u32 pass_width(u32 eights, u32 dim) { return eights <= 2 || (eights == 3 && dim < 256) ? eights : 2; }
+// Joined values lie as the lanes hold them: channel g D/8 + 2k + e of a row at
+// 16 k + 2 g + e, so that lanes that write or read together meet different
+// banks.  The channel at a place:
+__device__ __forceinline__ u32 channel_of(u32 dim, u32 at) { return at % 16 / 2 * (dim / 8) + at / 16 * 2 + at % 2; }
+
 // Row of out and lse behind a row of the segment.
 __device__ __forceinline__ u64 out_row(const AttentionArgs& a, const Segment& s, u32 row)
 {
@@ -270,8 +276,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     constexpr u32 kSide = 16 * D;   // bytes of a tile's keys, and of its values
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
     u8* ring = smem + warp * NS * 2 * kSide;
-    // after the loop [kWarps][R][D + 8], channel g D/8 + 2k + e of a row at 16 k + 2 g + e: then the
-    // lanes that write together meet different banks
+    // after the loop [kWarps][R][D + 8], channels in the joined order
     float* join_o = reinterpret_cast<float*>(smem);
     using L = Layout<D, NT>;
     constexpr bool kShared = kSharedQueries<D, NT>;
@@ -673,8 +678,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     __syncthreads();
     float* inverses = reinterpret_cast<float*>(ends);
     for (u32 x = threadIdx.x; x < R * D; x += blockDim.x) {
-        const u32 row = x / D, d = x % D;
-        const u32 place = row * (D + 8) + d % (D / 8) / 2 * 16 + d / (D / 8) * 2 + d % 2;
+        const u32 row = x / D, at = x % D;  // `at`: in the joined order
         float top = -INFINITY;
 #pragma unroll
         for (u32 w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * R + row].x);
@@ -684,14 +688,14 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         for (u32 w = 0; w < kWarps; ++w) {
             const float f = exp2_fast(join_ml[w * R + row].x - base);
             sum += join_ml[w * R + row].y * f;
-            value += join_o[w * R * (D + 8) + place] * f;
+            value += join_o[(w * R + row) * (D + 8) + at] * f;
         }
         if constexpr (!kWhole) {
             a.part_o[part * R * D + x] = value;
-            if (d == 0) a.part_ml[part * R + row] = make_float2(top, sum);
+            if (at == 0) a.part_ml[part * R + row] = make_float2(top, sum);
         } else if (row < rows) {
-            put_out(a, seg, seg.rt * R + row, d, sum == 0.0f ? 0.0f : value / sum);
-            if (d == 0) {
+            put_out(a, seg, seg.rt * R + row, channel_of(D, at), sum == 0.0f ? 0.0f : value / sum);
+            if (at == 0) {
                 factors[row] = base;  // the queries' factors and ends are not needed any more
                 inverses[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
                 if (a.lse) a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
@@ -751,6 +755,14 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
         run_segment<D, NT, false>(a, seg, first, end, static_cast<u64>(blockIdx.x) + seg.index, smem);
         at = here + end;
     }
+}
+
+__device__ __forceinline__ void put_pair(const AttentionArgs& a, u64 at, float x, float y)
+{
+    if (a.q.type == HBFSIM_KV_BF16)
+        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + at) = __floats2bfloat162_rn(x, y);
+    else
+        *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + at) = __floats2half2_rn(x, y);
 }
 
 // CTAs (sequence * heads + head, y).  The segments of a (sequence, head) are
@@ -835,19 +847,14 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                     }
                 }
                 const float inverse = row_inverse[r];
-                const u32 row = rt * R + r, d = x * 4 % D;
+                // two pairs of neighbouring channels, D / 8 apart
+                const u32 row = rt * R + r, at_row = x * 4 % D, d = channel_of(D, at_row);
                 const u32 tt = a.blocks ? t : row / a.q.group;
                 const u32 qh = h * a.q.group + row % a.q.group;
                 const u64 to = (static_cast<u64>(seq) * a.q.tokens + tt) * a.q.q_heads + qh;
-                const float y[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
-#pragma unroll
-                for (u32 k = 0; k < 4; ++k) {
-                    if (a.q.type == HBFSIM_KV_BF16)
-                        static_cast<__nv_bfloat16*>(a.out)[to * D + d + k] = __float2bfloat16_rn(y[k]);
-                    else
-                        static_cast<__half*>(a.out)[to * D + d + k] = __float2half_rn(y[k]);
-                }
-                if (d == 0 && a.lse)
+                put_pair(a, to * D + d, v.x * inverse, v.y * inverse);
+                put_pair(a, to * D + d + D / 8, v.z * inverse, v.w * inverse);
+                if (at_row == 0 && a.lse)
                     a.lse[to] = row_sum[r] == 0.0f ? -INFINITY : (log2f(row_sum[r]) + base) * kLn2;
             }
         }
@@ -994,7 +1001,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     const Plan p = plan_of(a.c, a.q, args->blocks != nullptr, args->top, args->weights != nullptr);
     if (p.segments > 0x7fffffffull) return HBFSIM_UNSUPPORTED;
     if (!args->out || !args->workspace || args->workspace_bytes < p.bytes ||
-        !kv_aligned(args->workspace, 16) || !kv_aligned(args->out, 2) ||
+        !kv_aligned(args->workspace, 16) || !kv_aligned(args->out, 4) ||
         !kv_aligned(args->lse, 4) || !kv_aligned(args->weights, 4) ||
         !kv_aligned(args->blocks, 4) || !kv_aligned(args->counts, 4))
         return HBFSIM_INVALID_ARGUMENT;

@@ -142,8 +142,8 @@ int hbfsim_kv_select_v1(const hbfsim_kv_cache_v1* cache,
  * listed ones (int32 [seqs][tokens][kv_heads][top], the first counts[...] of
  * each list, in any order and without repetition; an index that the sequence
  * does not have is passed over).
- * out: type, [seqs][tokens][q_heads][head_dim]; a token that sees nothing
- * gets 0.  lse (NULL to skip): fp32 [seqs][tokens][q_heads], natural
+ * out: type, [seqs][tokens][q_heads][head_dim], 4-byte aligned; a token that
+ * sees nothing gets 0.  lse (NULL to skip): fp32 [seqs][tokens][q_heads], natural
  * logarithm of the sum of exponentials, -inf for such a token.  weights
  * (NULL to skip): fp32 [seqs][kv_heads][width], softmax weight of each
  * block summed over the group's heads and the tokens, every entry written. */
