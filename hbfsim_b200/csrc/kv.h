@@ -141,27 +141,31 @@ inline u32 kv_team_threads(u32 slice)
     return slice <= 256 ? 128 : slice <= 512 ? 256 : slice <= 1024 ? 512 : 1024;
 }
 
-// Launches a kernel that may be set up while the kernel before it on the
-// stream still runs (programmatic dependent launch): it has to begin with
-// kv_wait_before, which returns once that kernel's writes are visible.
+// Launches a kernel in clusters of `cluster` CTAs.  `behind`: it may be set
+// up while the kernel before it on the stream still runs (programmatic
+// dependent launch); it then has to begin with kv_wait_before, which returns
+// once that kernel's writes are visible.
 template <typename... Params, typename... Args>
-inline bool kv_launch_behind(void (*kernel)(Params...), dim3 grid, u32 threads, cudaStream_t stream,
-                             u32 smem, u32 cluster, Args... args)
+inline bool kv_launch(void (*kernel)(Params...), dim3 grid, u32 threads, cudaStream_t stream, u32 smem,
+                      u32 cluster, bool behind, Args... args)
 {
     cudaLaunchAttribute attributes[2]{};
-    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[0].val.programmaticStreamSerializationAllowed = 1;
-    attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = cluster;
-    attributes[1].val.clusterDim.y = 1;
-    attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = grid;
     config.blockDim = dim3(threads);
-    config.stream = stream;
     config.dynamicSmemBytes = smem;
+    config.stream = stream;
     config.attrs = attributes;
-    config.numAttrs = cluster > 1 ? 2 : 1;
+    if (behind) {
+        attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attributes[config.numAttrs].val.clusterDim.x = cluster;
+        attributes[config.numAttrs].val.clusterDim.y = 1;
+        attributes[config.numAttrs++].val.clusterDim.z = 1;
+    }
     return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess;
 }
 

@@ -917,8 +917,7 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     p.whole = p.tiles <= kWholeTiles && (!weights || p.lists * p.row_tiles == 1);
     if (p.whole) {
         p.workers = static_cast<u32>(p.segments);
-        p.bytes = 256;
-        return p;
+        return p;  // no workspace
     }
     u64 at = 0;
     auto take = [&](u64 bytes) {
@@ -968,8 +967,8 @@ int launch(const AttentionArgs& a, bool whole, cudaStream_t s)
         across = std::max(segments, std::min((a.q.width + kFinishThreads - 1) / kFinishThreads,
                                              4u * kv_sm_count() / pairs));
     const u32 slices = std::min(std::max(1u, across / segments), 8u);
-    const bool ok = kv_launch_behind(finish_kernel, dim3(pairs, across), kFinishThreads, s, 0, 1, a,
-                                     static_cast<u32>(8 * NT), slices);
+    const bool ok = kv_launch(finish_kernel, dim3(pairs, across), kFinishThreads, s, 0, 1, true, a,
+                              static_cast<u32>(8 * NT), slices);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
@@ -1000,7 +999,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     if (a.q.seqs == 0 || a.q.tokens == 0) return HBFSIM_OK;
     const Plan p = plan_of(a.c, a.q, args->blocks != nullptr, args->top, args->weights != nullptr);
     if (p.segments > 0x7fffffffull) return HBFSIM_UNSUPPORTED;
-    if (!args->out || !args->workspace || args->workspace_bytes < p.bytes ||
+    if (!args->out || (p.bytes && !args->workspace) || args->workspace_bytes < p.bytes ||
         !kv_aligned(args->workspace, 16) || !kv_aligned(args->out, 4) ||
         !kv_aligned(args->lse, 4) || !kv_aligned(args->weights, 4) ||
         !kv_aligned(args->blocks, 4) || !kv_aligned(args->counts, 4))

@@ -51,7 +51,6 @@ __global__ void __launch_bounds__(1024) evict_kernel(const EvictArgs a, u32 team
 {
     extern __shared__ __align__(16) i64 held[];
     __shared__ KvSelectShared sm;
-    kv_wait_before();
     const KvTeam team{blockIdx.x % team_size, team_size};
     const u32 seq = blockIdx.x / team_size;
     const int length = kv_length(a.lengths, seq, a.width, a.block);
@@ -166,7 +165,7 @@ extern "C" int hbfsim_kv_evict_v1(const hbfsim_kv_evict_batch_v1* b, void* strea
         team = 1;
         slice = b->width;
     }
-    const bool ok = kv_launch_behind(evict_kernel, dim3(b->seqs * team), kv_team_threads(slice), s,
-                                     slice <= kHeldBlocks ? slice * 8 : 0, team, a, team, slice);
+    const bool ok = kv_launch(evict_kernel, dim3(b->seqs * team), kv_team_threads(slice), s,
+                              slice <= kHeldBlocks ? slice * 8 : 0, team, false, a, team, slice);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }

@@ -394,7 +394,7 @@ int launch(const SelectArgs& a, cudaStream_t s)
         query_kernel<D><<<(rows + kQueryWarps - 1) / kQueryWarps, kQueryWarps * 32, 0, s>>>(a);
         const u64 most = (static_cast<u64>(a.q.seqs) * a.q.width + kScoreShare - 1) / kScoreShare;
         const u32 grid = static_cast<u32>(std::min<u64>(most, static_cast<u64>(score_per_sm(D)) * kv_sm_count()));
-        ok = kv_launch_behind(score_kernel<D>, dim3(grid), kScoreWarps * 32, s, kScoreSmem<D>, 1, a);
+        ok = kv_launch(score_kernel<D>, dim3(grid), kScoreWarps * 32, s, kScoreSmem<D>, 1, true, a);
     }
     static std::atomic<u64> seen_list{0};
     if (!kv_allow_smem(list_kernel, kHeldKeys * 4, seen_list)) return HBFSIM_CUDA_ERROR;
@@ -406,8 +406,8 @@ int launch(const SelectArgs& a, cudaStream_t s)
     // many rows: small CTAs, several to an SM
     u32 threads = kv_team_threads(slice);
     if (rows > 2 * static_cast<u32>(kv_sm_count())) threads = std::min(threads, 256u);
-    ok = kv_launch_behind(list_kernel, dim3(rows * team), threads, s,
-                          slice <= kHeldKeys ? slice * 4 : 0, team, a, team, slice) && ok;
+    ok = kv_launch(list_kernel, dim3(rows * team), threads, s, slice <= kHeldKeys ? slice * 4 : 0, team, true, a,
+                   team, slice) && ok;
     return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 

@@ -287,9 +287,8 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
     head = (_ATTENTION.size, 1, scale, top, blocks_at, counts_at, out.data_ptr(), lse.data_ptr(),
             mass_at)
     size = lib.hbfsim_kv_attention_workspace_v1(cache._packed, query, _ATTENTION.pack(*head, 0, 0))
-    space = cache.bounds.new_empty(size)
-    check(lib.hbfsim_kv_attention_v1(cache._packed, query,
-                                     _ATTENTION.pack(*head, space.data_ptr(), size),
+    space = cache.bounds.new_empty(size).data_ptr() if size else 0
+    check(lib.hbfsim_kv_attention_v1(cache._packed, query, _ATTENTION.pack(*head, space, size),
                                      _handle(cache.index)), "hbfsim_kv_attention_v1")
     return KvAttention(out, lse, mass)
 
@@ -318,9 +317,10 @@ def kv_evict(score, weights, table, lengths, keep: int, block_tokens: int = 16, 
           "weights: float32 [seqs, kv_heads, width], contiguous")
     _need(min(keep, block_tokens, sink, recent, decay) >= 0,
           "keep, block_tokens, sink, recent and decay are counts")
-    new_score = torch.empty_like(score)
-    new_table, freed = table.new_empty((2, seqs, width)).unbind(0)
-    new_lengths, freed_counts = table.new_empty((2, seqs)).unbind(0)
+    plain, like = torch.contiguous_format, torch.empty_like
+    new_score = like(score)
+    new_table, freed = like(table, memory_format=plain), like(table, memory_format=plain)
+    new_lengths, freed_counts = like(lengths, memory_format=plain), like(lengths, memory_format=plain)
     batch = _EVICT.pack(_EVICT.size, 1, seqs, weights.shape[1], width, block_tokens, keep, sink,
                         recent, decay, score.data_ptr(), weights.data_ptr(), table.data_ptr(),
                         table.stride(0), lengths.data_ptr(), new_score.data_ptr(),

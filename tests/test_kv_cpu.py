@@ -113,8 +113,30 @@ def test_select_refusals(lib, top, sink, recent, size, blocks):
     dict(blocks=4096, counts=4096, top=0), dict(out=None), dict(out=4097), dict(lse=4098),
     dict(weights=4098), dict(workspace=None), dict(workspace=4104), dict(workspace_bytes=16)])
 def test_attention_refusals(lib, over):
-    assert lib.hbfsim_kv_attention_v1(ref(cache()), ref(query()), ref(attention(**over)),
+    wide = query(width=40, table_stride=40)  # a call that needs a workspace
+    assert lib.hbfsim_kv_attention_v1(ref(cache()), ref(wide), ref(attention(**over)),
                                       None) == INVALID
+
+
+def test_attention_workspace_sizes(lib):
+    """Short rows need none; wide ones grow with the sequences and with the weights."""
+    size = lambda q, **over: lib.hbfsim_kv_attention_workspace_v1(ref(cache()), ref(q), ref(attention(**over)))
+    assert size(query()) == 0
+    wide = [size(query(width=200, seqs=s), weights=w) for s in (2, 4) for w in (None, 4096)]
+    assert 0 < wide[0] < wide[1] and wide[0] < wide[2] < wide[3]
+    assert all(w % 256 == 0 for w in wide)
+
+
+def test_packed_structures():
+    """The structures that Python packs are those of the header, byte for byte."""
+    from hbfsim_b200 import kv
+    for packed, struct in ((kv._CACHE, _lib.KvCacheV1), (kv._APPEND, _lib.KvAppendBatchV1),
+                           (kv._QUERY, _lib.KvQueryV1), (kv._ATTENTION, _lib.KvAttentionArgsV1),
+                           (kv._EVICT, _lib.KvEvictBatchV1)):
+        assert packed.size == ctypes.sizeof(struct)
+        values = [0.5 if kind is ctypes.c_float else 7 * i + 1
+                  for i, (_, kind) in enumerate(struct._fields_)]
+        assert packed.pack(*values) == bytes(struct(*values))
 
 
 @pytest.mark.parametrize("over,rc", [
