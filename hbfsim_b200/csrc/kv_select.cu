@@ -13,11 +13,12 @@
 // query_kernel makes the whole numbers once; score_kernel streams the bounds
 // through a ring of asynchronous copies per warp and writes a 32-bit ordered
 // key per (token, head, block): the blocks of all sequences form one line
-// that is cut into equal shares, one per resident CTA.  list_kernel, one team
-// (a CTA, or a cluster for few long rows) per (sequence, token, head), finds
-// the key of the last block to list by a selection on the keys (in shared
-// memory up to kHeldKeys blocks a CTA) and writes the list in block order.
-// Each kernel is set up while the one before it runs.
+// that is cut into equal shares, one per resident CTA.  Then the key of the
+// last block to list is found for every (sequence, token, head), and the list
+// is written in block order: by short_list_kernel, a CTA per row with the keys
+// in registers, up to kShortRow blocks; else by list_kernel, a team (a CTA, or
+// a cluster for few long rows) per row with the keys in shared memory up to
+// kHeldKeys a CTA.  Each kernel is set up while the one before it runs.
 #include "kv.h"
 
 #include <algorithm>
@@ -29,6 +30,11 @@ constexpr u32 kQueryWarps = 4;
 constexpr u32 kScoreWarps = 8;
 constexpr u32 kScoreShare = 32;      // blocks of a CTA at least
 constexpr u32 kHeldKeys = 32 * 1024; // 128 KB of keys
+// Blocks of a row that registers hold.  Against list_kernel's bins: 8 us instead of 14 for 512
+// rows of up to 2048 blocks, the call 303 us instead of 386 for 384 rows of 16000 and 20.6 us
+// instead of 21.3 for 8.  At 32768 (32 keys a thread, which spill) 8 rows of 16385 took 29.4 us
+// instead of 20.6.
+constexpr u32 kShortRow = 16384;
 constexpr u32 kAbsent = 0u;           // key of a block that cannot be listed
 constexpr u32 kAlways = 0xffffffffu;  // key of a block that is always listed
 
@@ -308,7 +314,112 @@ __global__ void __launch_bounds__(kScoreWarps * 32, score_per_sm(D)) score_kerne
     if (!queries) kv_wait_before();  // list_kernel waits for this kernel alone
 }
 
-// `slice`: blocks of a row that one CTA of the team has.
+// Rows of at most 32 K W blocks: a CTA of W warps per (sequence, token, head), which hold the row in
+// registers, finds the key of the last block to list bit by bit; a bit costs a count and one
+// barrier.
+template <u32 W, int K>
+__global__ void __launch_bounds__(W * 32) short_list_kernel(const SelectArgs a)
+{
+    __shared__ uint4 found[W];
+    __shared__ u32 counts[2][W];  // of the warps, in turns
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, under = (1u << lane) - 1u;
+    kv_wait_before();
+    const u64 at = blockIdx.x;
+    const u32 heads = a.c.heads, tokens = a.q.tokens;
+    const u32 t = static_cast<u32>(at / heads % tokens), seq = static_cast<u32>(at / heads / tokens);
+    const int length = kv_length(a.q.lengths, seq, a.q.width, a.c.block);
+    const u32 have = blocks_of_token(length, tokens, t, a.c.block);
+    // a warp's blocks: a run of whole 32s
+    const u32 each = (have + W * 32 - 1) / (W * 32) * 32, from = warp * each, to = min(from + each, have);
+    const u32* row = a.keys + at * a.q.width;
+    u32 k[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const u32 j = from + i * 32 + lane;
+        k[i] = j < to ? row[j] : kAbsent;
+    }
+    u32 there = 0, always = 0, least = ~0u, greatest = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        there += k[i] != kAbsent;
+        always += k[i] == kAlways;
+        if (k[i] != kAbsent && k[i] != kAlways) {
+            least = min(least, k[i]);
+            greatest = max(greatest, k[i]);
+        }
+    }
+    there = __reduce_add_sync(0xffffffffu, there);
+    always = __reduce_add_sync(0xffffffffu, always);
+    least = __reduce_min_sync(0xffffffffu, least);
+    greatest = __reduce_max_sync(0xffffffffu, greatest);
+    if (lane == 0) found[warp] = make_uint4(there, always, least, greatest);
+    __syncthreads();
+    const uint4 its = lane < W ? found[lane] : make_uint4(0, 0, ~0u, 0);
+    there = __reduce_add_sync(0xffffffffu, its.x);
+    always = __reduce_add_sync(0xffffffffu, its.y);
+    least = __reduce_min_sync(0xffffffffu, its.z);
+    greatest = __reduce_max_sync(0xffffffffu, its.w);
+    u32 turn = 0;
+    // the sum of the counts that the first `warps` warps bring
+    auto share = [&](u32 mine, u32 warps) {
+        turn ^= 1u;  // the slots of the turn before may still be read
+        if (lane == 0) counts[turn][warp] = mine;
+        __syncthreads();
+        return __reduce_add_sync(0xffffffffu, lane < warps ? counts[turn][lane] : 0);
+    };
+    const u32 take = min(a.top, there);
+    // Listed: the keys above `limit` and the first `equals` at it.
+    u32 limit = kAlways, equals = take;
+    if (take == there) {
+        limit = kAbsent + 1, equals = kKvAll;
+    } else if (take > always) {
+        auto reach = [&](u32 x) {  // keys that are x at least
+            u32 n[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < K; ++i) n[i % 4] += k[i] >= x;
+            return share(__reduce_add_sync(0xffffffffu, n[0] + n[1] + n[2] + n[3]), W);
+        };
+        const u32 differ = least ^ greatest;
+        u32 bit = differ ? 0x80000000u >> __clz(static_cast<int>(differ)) : 0;
+        limit = greatest & ~(bit ? 2 * bit - 1 : 0);  // the bits that all keys share
+        u32 count = 0;
+        for (; bit && count != take; bit >>= 1) {
+            const u32 n = reach(limit | bit);
+            if (n >= take) limit |= bit, count = n;
+        }
+        equals = count == take ? kKvAll : take - reach(limit + 1);
+    }
+    u32 same = 0;  // keys at the limit in front, and listed ones
+    if (equals != kKvAll) {
+        u32 n = 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) n += k[i] == limit;
+        same = share(__reduce_add_sync(0xffffffffu, n), warp);
+    }
+    u32 listed[K], before = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        bool chosen = k[i] >= limit;
+        if (equals != kKvAll) {
+            const u32 equal = __ballot_sync(0xffffffffu, k[i] == limit);
+            chosen = k[i] > limit || (k[i] == limit && same + __popc(equal & under) < equals);
+            same += __popc(equal);
+        }
+        listed[i] = __ballot_sync(0xffffffffu, chosen);
+        before += __popc(listed[i]);
+    }
+    before = share(before, warp);
+    int* list = a.blocks + at * a.top;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        if (listed[i] >> lane & 1u) list[before + __popc(listed[i] & under)] = static_cast<int>(from + i * 32 + lane);
+        before += __popc(listed[i]);
+    }
+    for (u32 i = take + threadIdx.x; i < a.top; i += W * 32) list[i] = -1;
+    if (threadIdx.x == 0) a.counts[at] = static_cast<int>(take);
+}
+
+// Any row.  `slice`: blocks of a row that one CTA of the team has.
 __global__ void __launch_bounds__(1024) list_kernel(const SelectArgs a, u32 team_size, u32 slice)
 {
     extern __shared__ __align__(16) u32 held[];
@@ -395,6 +506,18 @@ int launch(const SelectArgs& a, cudaStream_t s)
         const u64 most = (static_cast<u64>(a.q.seqs) * a.q.width + kScoreShare - 1) / kScoreShare;
         const u32 grid = static_cast<u32>(std::min<u64>(most, static_cast<u64>(score_per_sm(D)) * kv_sm_count()));
         ok = kv_launch(score_kernel<D>, dim3(grid), kScoreWarps * 32, s, kScoreSmem<D>, 1, true, a);
+    }
+    if (a.q.width <= kShortRow) {
+        // Keys per lane against warps per barrier: 16 x 4 took 41.0 us for 512 rows of up to 2048
+        // (the whole call), 8 x 8 42.2 us; 8 x 16 20.2 us for 32 rows of 4000, 16 x 8 22.1 us.
+        auto* kernel = short_list_kernel<4, 4>;
+        u32 warps = 4;
+        if (a.q.width > 512) kernel = short_list_kernel<4, 16>;
+        if (a.q.width > 2048) kernel = short_list_kernel<16, 8>, warps = 16;
+        if (a.q.width > 4096) kernel = short_list_kernel<32, 8>, warps = 32;
+        if (a.q.width > 8192) kernel = short_list_kernel<32, 16>, warps = 32;
+        ok = kv_launch(kernel, dim3(rows), warps * 32, s, 0, 1, true, a) && ok;
+        return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
     }
     static std::atomic<u64> seen_list{0};
     if (!kv_allow_smem(list_kernel, kHeldKeys * 4, seen_list)) return HBFSIM_CUDA_ERROR;

@@ -692,6 +692,25 @@ def test_select_long_rows(blocks, top, heads):
     assert_lists(got, ko.select(cache, q.double().cpu().numpy(), table, [blocks * block - 3], top, 1, 1))
 
 
+@pytest.mark.parametrize("blocks, top, recent", [
+    (511, 40, 1), (512, 512, 3), (513, 512, 1), (2048, 1, 1), (2049, 2000, 900), (4096, 77, 70), (4097, 4000, 1),
+    (8192, 256, 1), (8193, 8192, 5000), (16384, 300, 300), (16385, 16385, 2)])
+def test_select_widths(blocks, top, recent):
+    """Tables at the widths where the selection changes its form; rows from empty to full, with few
+    distinct pages (ties), and lists from always listed blocks alone to every block."""
+    torch = torch_()
+    from hbfsim_b200 import kv_select
+    rng = np.random.default_rng(blocks + top)
+    heads, dim, block, tokens = 2, 64, 16, 2
+    cache = random_cache(rng, 40, heads, block, dim)
+    lengths = [blocks * block, 0, 1, blocks * block // 2 + 5, min(blocks * block, (top + 1) * block)]
+    table = rng.integers(0, 40, (len(lengths), blocks)).astype(np.int32)
+    table[rng.random(table.shape) < 0.02] = -1
+    q = torch.from_numpy(rng.standard_normal((len(lengths), tokens, 3 * heads, dim))).to(torch.bfloat16).cuda()
+    got = kv_select(to_gpu(cache), q, int32(table), int32(lengths), top, 0, recent)
+    assert_lists(got, ko.select(cache, q.double().cpu().numpy(), table, lengths, top, 0, recent))
+
+
 def test_example(capsys):
     """The example: fewer reads and less simulated time for the lists than for every block, and
     what is evicted is what goes beyond `keep`."""
