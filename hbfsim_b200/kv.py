@@ -287,8 +287,9 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
     head = (_ATTENTION.size, 1, scale, top, blocks_at, counts_at, out.data_ptr(), lse.data_ptr(),
             mass_at)
     size = lib.hbfsim_kv_attention_workspace_v1(cache._packed, query, _ATTENTION.pack(*head, 0, 0))
-    space = cache.bounds.new_empty(size).data_ptr() if size else 0
-    check(lib.hbfsim_kv_attention_v1(cache._packed, query, _ATTENTION.pack(*head, space, size),
+    space = cache.bounds.new_empty(size) if size else None  # held until the launch
+    space_at = space.data_ptr() if size else 0
+    check(lib.hbfsim_kv_attention_v1(cache._packed, query, _ATTENTION.pack(*head, space_at, size),
                                      _handle(cache.index)), "hbfsim_kv_attention_v1")
     return KvAttention(out, lse, mass)
 
