@@ -1,13 +1,19 @@
 // kv_append.cu -- new tokens into the 8-bit paged cache (kv_v1.h).
 //
 // One warp per (touched block, head, side).  A CTA's warps look at a chunk of
-// up to 32 tokens, one per lane, and do the blocks whose first new token is
+// up to 16 tokens, one per lane, and do the blocks whose first new token is
 // among them, each warp for its head and side; few tokens get chunks of one,
 // so that every block has a warp of its own at once.  For a block of new
 // tokens alone a lane holds its channels of 16 tokens in registers between
 // the two passes: the largest magnitude, which gives the scale, then the
-// stored values (blocks of more tokens are read again).  Everything is a power of two away from the input,
-// so the only rounding is the one to e4m3.
+// stored values (blocks of more tokens are read again).  Everything is a
+// power of two away from the input, so the only rounding is the one to e4m3.
+//
+// Prompts of 31,668 tokens in all (8 heads of 128 channels) take 42 us: 199 MB
+// of input and blocks at 4.7 TB/s, 73 % of a copy's rate, with half of the
+// issue slots taken (9 instructions a value) at 24 warps an SM.  A step's 64
+// tokens take 4.2 us and one token 3.2 us, a launch and one chain of reads
+// (start, table, the block's scale, its values).
 #include "kv.h"
 
 #include <cuda_fp8.h>
@@ -452,9 +458,11 @@ extern "C" int hbfsim_kv_append_v1(const hbfsim_kv_cache_v1* cache,
     a.tokens = static_cast<u32>(b->tokens);
     auto wide = [](const void* p, i64 token, i64 head) { return kv_aligned(p, 16) && token % 8 == 0 && head % 8 == 0; };
     a.wide = wide(b->k, b->k_stride_token, b->k_stride_head) && wide(b->v, b->v_stride_token, b->v_stride_head);
-    // one token to a chunk while all chunks' warps are resident at once (16 to an SM), more beyond
+    // One token to a chunk while all chunks' warps are resident at once (16 to an SM), up to 16
+    // beyond (8 heads of 128 channels: 64 tokens took 4.2 us with 1 and 26 us with 16, 31,668
+    // tokens 145 us with 1 and 42 us with 16).
     a.chunk = 1;
-    while (a.chunk < 32 && static_cast<u64>(a.tokens) * v.heads * 2 > static_cast<u64>(a.chunk) * 16 * kv_sm_count())
+    while (a.chunk < 16 && static_cast<u64>(a.tokens) * v.heads * 2 > static_cast<u64>(a.chunk) * 16 * kv_sm_count())
         a.chunk *= 2;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return b->type == HBFSIM_KV_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
