@@ -43,7 +43,9 @@ constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
 constexpr float kAbove = 8.0f;
 constexpr float kNoScore = -3.0e38f;  // reference of a row without a score
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr u32 kWholeTiles = 32;     // segments of so many tiles at most need no finishing kernel
+// Tiles of a segment that one CTA may take whole, at most.  With two row tiles or more the work per
+// tile is larger: 400 segments of 125 tiles and 16 rows took 78 us whole and 58 us split.
+constexpr u32 whole_tiles(u32 nt) { return nt == 1 ? 128 : 32; }
 constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
 struct AttentionArgs {
@@ -259,9 +261,10 @@ struct Layout {
     static constexpr u32 queries = join_ml + kWarps * 8 * NT * 8;
     static constexpr u32 factors = queries + (kSharedQueries<D, NT> ? NT * D * 16 : 0);
     static constexpr u32 ends = factors + 8 * NT * 4;
-    static constexpr u32 whole_sums = ends + 8 * NT * 4;  // [kWholeTiles][8 NT]
-    static constexpr u32 line = whole_sums + kWholeTiles * 8 * NT * 8;
+    static constexpr u32 line = ends + 8 * NT * 4;  // of the split; for whole segments:
+    static constexpr u32 whole_sums = line;         // [tiles][8 NT], if there are weights
     static constexpr u32 bytes = line + 8 * kWarps + sizeof(u64) * 4;
+    static constexpr u32 most = whole_sums + whole_tiles(NT) * 8 * NT * 8;
 };
 
 // One segment's tiles [first, end) by one CTA; the partial result goes to `part`.
@@ -910,11 +913,19 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     p.segments = static_cast<u64>(p.units) * p.per_unit;
     // as many CTAs as are resident at once, fewer for little work
     const u64 most = (p.segments * p.tiles + kShare - 1) / kShare;
-    p.workers = static_cast<u32>(
-        std::max<u64>(1, std::min<u64>(most, static_cast<u64>(per_sm(v.dim, p.nt)) * kv_sm_count())));
+    const u64 resident = static_cast<u64>(per_sm(v.dim, p.nt)) * kv_sm_count();
+    p.workers = static_cast<u32>(std::max<u64>(1, std::min<u64>(most, resident)));
     // Short segments (by the table's width or the lists' length) are finished where they are
-    // summed: one launch, where the even split takes two.
-    p.whole = p.tiles <= kWholeTiles && (!weights || p.lists * p.row_tiles == 1);
+    // summed: one launch, where the even split takes two and joins.  The longer they are, the more
+    // of them there have to be.  With 128 channels 64 segments of 20 tiles take 9.7 us whole and
+    // 15.5 us split, 64 of 63 tiles 15.1 and 16.7 us (16 of them 14.9 and 15.1 us), 64 of 94 tiles
+    // 19.6 and 18.4 us, 128 of 94 tiles 19.8 and 21.0 us, 400 of 128 tiles 36.6 and 41.2 us.  More
+    // long ones than are resident at once should fill their last turn: 1600 lists of 128 tiles
+    // take 152 and 169 us, 512 on 444 places 74 and 64 us (512 of 21 to 63 tiles 32.0 and 36.7 us).
+    const u64 places = (p.segments + resident - 1) / resident * resident;
+    p.whole = p.tiles <= whole_tiles(p.nt) && 2 * p.tiles <= p.segments + 64 &&
+              (p.tiles <= 64 || p.segments <= resident || p.segments * 5 >= places * 4) &&
+              (!weights || p.lists * p.row_tiles == 1);
     if (p.whole) {
         p.workers = static_cast<u32>(p.segments);
         return p;  // no workspace
@@ -949,8 +960,10 @@ template <int D, int NT, bool kWhole>
 bool launch_attention(const AttentionArgs& a, cudaStream_t s)
 {
     static std::atomic<u64> seen{0};
-    if (!kv_allow_smem(attention_kernel<D, NT, kWhole>, Layout<D, NT>::bytes, seen)) return false;
-    attention_kernel<D, NT, kWhole><<<a.workers, kWarps * 32, Layout<D, NT>::bytes, s>>>(a);
+    using L = Layout<D, NT>;
+    if (!kv_allow_smem(attention_kernel<D, NT, kWhole>, kWhole ? L::most : L::bytes, seen)) return false;
+    const u32 sums = kWhole && a.weights ? a.tiles * 8 * NT * 8 : 0;
+    attention_kernel<D, NT, kWhole><<<a.workers, kWarps * 32, std::max(L::bytes, L::whole_sums + sums), s>>>(a);
     return cudaGetLastError() == cudaSuccess;
 }
 

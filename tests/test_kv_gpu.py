@@ -464,7 +464,7 @@ def test_many_sequences():
     q = torch.from_numpy(rng.standard_normal((64, 1, 2 * heads, dim))).to(torch.bfloat16).cuda()
     q = q.repeat(seqs // 64, 1, 1, 1)
     gpu = to_gpu(small)
-    wide = np.concatenate([table, np.full((seqs, 40), -1, np.int32)], 1)  # not finished in one kernel
+    wide = np.concatenate([table, np.full((seqs, 40), -1, np.int32)], 1)
     probe = rng.integers(0, seqs, 50)
     want = ko.attention(small, q[probe].double().cpu().numpy(), table[probe], lengths[probe], dim ** -0.5)
     for t in (table, wide):
@@ -477,6 +477,49 @@ def test_many_sequences():
     rest = kv_evict(torch.zeros((seqs, 2), dtype=torch.int64, device="cuda"),
                     torch.rand((seqs, heads, 2), device="cuda"), int32(table), int32(lengths), keep=2)
     assert not rest.freed_counts.any()
+
+
+@pytest.mark.parametrize("dim, block, heads, group, kind", [
+    (128, 16, 4, 4, "bf16"), (64, 32, 5, 8, "f16"), (256, 16, 4, 1, "bf16")])
+def test_attention_many_short_rows(dim, block, heads, group, kind):
+    """Enough (sequence, head) pairs for each to be finished by one thread block up to 70 tiles of
+    16 tokens; the same rows shared out and joined, in a wider table; lists of them."""
+    torch = torch_()
+    rng = np.random.default_rng(dim + block)
+    lengths = [0, 1, 70 * 16, 69 * 16 + 1, 15, 513] + [int(x) for x in rng.integers(0, 70 * 16, 14)]
+    small = random_cache(rng, 30, heads, block, dim)
+    width = 70 * 16 // block
+    table = rng.integers(0, 30, (len(lengths), width)).astype(np.int32)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), 1, heads * group, dim))).to(type_of(kind)).cuda()
+    whole = attend_and_check(small, q, table, lengths)
+    again = attend_and_check(small, q, table, lengths)
+    for a, b in zip(whole, again):
+        assert torch.equal(a, b)
+    wide = np.concatenate([table, np.full((len(lengths), 200), -1, np.int32)], 1)
+    attend_and_check(small, q, wide, lengths)
+    have = [-(-n // block) for n in lengths]
+    lists = [[[[int(j) for j in rng.permutation(have[b])[:width - 1]] for _ in range(heads)]] for b in range(len(lengths))]
+    attend_and_check(small, q, wide, lengths, lists)
+
+
+def test_many_sequences_wide_tables():
+    """The split over more (sequence, head) pairs than a grid's second axis holds."""
+    torch = torch_()
+    from hbfsim_b200 import kv_attention
+    rng = np.random.default_rng(19)
+    seqs, heads, dim, block = 40000, 2, 64, 16
+    small = random_cache(rng, 8, heads, block, dim)
+    table = np.full((seqs, 140), -1, np.int32)
+    table[:, :2] = rng.integers(0, 8, (seqs, 2))
+    lengths = rng.integers(0, 33, seqs)
+    q = torch.from_numpy(rng.standard_normal((64, 1, 2 * heads, dim))).to(torch.bfloat16).cuda()
+    q = q.repeat(seqs // 64, 1, 1, 1)
+    probe = rng.integers(0, seqs, 50)
+    want = ko.attention(small, q[probe].double().cpu().numpy(), table[probe], lengths[probe], dim ** -0.5)
+    got = kv_attention(to_gpu(small), q, int32(table), int32(lengths), weights=True)
+    assert np.abs(got.out[probe].double().cpu().numpy() - want[0]).max() <= \
+        (2.0 ** -8 * np.abs(want[0]) + 2.0 ** -10 * want[3] + 2.0 ** -20).max()
+    assert np.abs(got.weights[probe].double().cpu().numpy() - want[2]).max() <= 2.0 ** -17
 
 
 # ---------------------------------------------------------------------------
