@@ -27,7 +27,16 @@
 // asynchronous copies of its own (no block barrier inside the loop), join
 // through shared memory and leave one partial result per segment met;
 // finish_kernel joins the partials of a segment and turns the tiles' sums
-// into block weights.
+// into block weights.  Short segments have a CTA each and need neither.
+//
+// One decode step of 64 sequences of 1024 to 32768 tokens, 8 heads of 128
+// channels with 4 rows each, takes 399 us with weights: 2.21 GB at 5.5 TB/s,
+// 86 % of a copy's rate, DRAM's bound; 12 warps an SM take 41 % of the issue
+// slots, 271 instructions for the 4 KB of a tile.  128 listed blocks per head
+// take 63 us (272 MB at 4.3 TB/s): shares of 150 tiles begin and join more
+// often.  One sequence of 262,147 tokens takes 104 us (539 MB at 5.2 TB/s).
+// 40 rows on 8 sequences of 700 to 9001 tokens take 64 us, three passes that
+// are bound by the latency of their instructions (46 % of the slots).
 #include "kv.h"
 
 #include <algorithm>
@@ -768,6 +777,8 @@ __device__ __forceinline__ void put_pair(const AttentionArgs& a, u64 at, float x
         *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + at) = __floats2half2_rn(x, y);
 }
 
+// 11 to 16 us by itself (parts and tile sums come out of the L2), of which a
+// call shows 2 to 12 us, since its start overlaps the end of the kernel before.
 // CTAs (sequence * heads + head, y).  The segments of a (sequence, head) are
 // joined by the CTAs y = 0, 1, .. in turn, or, with more CTAs than segments,
 // each by `slices` of them; with weights every CTA also sums those of its

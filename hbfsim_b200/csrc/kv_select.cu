@@ -19,6 +19,11 @@
 // in registers, up to kShortRow blocks; else by list_kernel, a team (a CTA, or
 // a cluster for few long rows) per row with the keys in shared memory up to
 // kHeldKeys a CTA.  Each kernel is set up while the one before it runs.
+//
+// One decode step of 64 sequences of 1024 to 32768 tokens, 8 heads of 128
+// channels, blocks of 16: 41 us.  score_kernel takes 31 us of them, 143 MB of
+// bounds in pieces of 256 bytes at 4.6 TB/s (71 % of a copy's rate, 41 % of
+// the issue slots), short_list_kernel 8 us, a barrier for each of some 20 bits.
 #include "kv.h"
 
 #include <algorithm>
