@@ -52,9 +52,10 @@ constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
 constexpr float kAbove = 8.0f;
 constexpr float kNoScore = -3.0e38f;  // reference of a row without a score
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Tiles of a segment that one CTA may take whole, at most.  With two row tiles or more the work per
-// tile is larger: 400 segments of 125 tiles and 16 rows took 78 us whole and 58 us split.
-constexpr u32 whole_tiles(u32 nt) { return nt == 1 ? 128 : 32; }
+// Tiles of a segment that one CTA of so many warps may take whole, at most.  With two row tiles or
+// more the sums of their weights cost CTAs on an SM: 400 segments of 125 tiles and 16 rows took 78
+// us whole and 58 us split.
+constexpr u32 whole_tiles(u32 nt, u32 warps) { return nt == 1 || warps > kWarps ? 128 : 32; }
 constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
 struct AttentionArgs {
@@ -256,28 +257,27 @@ constexpr u32 per_sm(u32 dim, u32 nt)
 }
 template <int D>
 constexpr u32 kStages = D == 256 ? 3 : 4;
-template <int D>
-constexpr u32 kRing = kWarps * kStages<D> * 32 * D;  // bytes
 // One row tile's queries stay in registers; more are read from shared memory for each tile.
 template <int D, int NT>
 constexpr bool kSharedQueries = NT > 1 || D == 256;
 // Shared memory: rings (later the joined values), notes, sums, queries, row factors and ends, a word.
-template <int D, int NT>
+template <int D, int NT, u32 W>  // W warps
 struct Layout {
-    static constexpr u32 join = kWarps * 8 * NT * (D + 8) * 4;
-    static constexpr u32 notes = kRing<D> > join ? kRing<D> : join;
-    static constexpr u32 join_ml = notes + kWarps * kStages<D> * 16;
-    static constexpr u32 queries = join_ml + kWarps * 8 * NT * 8;
+    static constexpr u32 ring = W * kStages<D> * 32 * D;
+    static constexpr u32 join = W * 8 * NT * (D + 8) * 4;
+    static constexpr u32 notes = ring > join ? ring : join;
+    static constexpr u32 join_ml = notes + W * kStages<D> * 16;
+    static constexpr u32 queries = join_ml + W * 8 * NT * 8;
     static constexpr u32 factors = queries + (kSharedQueries<D, NT> ? NT * D * 16 : 0);
     static constexpr u32 ends = factors + 8 * NT * 4;
     static constexpr u32 line = ends + 8 * NT * 4;  // of the split; for whole segments:
     static constexpr u32 whole_sums = line;         // [tiles][8 NT], if there are weights
-    static constexpr u32 bytes = line + 8 * kWarps + sizeof(u64) * 4;
-    static constexpr u32 most = whole_sums + whole_tiles(NT) * 8 * NT * 8;
+    static constexpr u32 bytes = line + 8 * W + sizeof(u64) * 4;
+    static constexpr u32 most = whole_sums + whole_tiles(NT, W) * 8 * NT * 8;
 };
 
 // One segment's tiles [first, end) by one CTA; the partial result goes to `part`.
-template <int D, int NT, bool kWhole>
+template <int D, int NT, bool kWhole, u32 W>
 __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segment& seg, u32 first,
                                             u32 end, u64 part, u8* smem)
 {
@@ -288,12 +288,12 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     constexpr u32 kSide = 16 * D;   // bytes of a tile's keys, and of its values
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u;
     u8* ring = smem + warp * NS * 2 * kSide;
-    // after the loop [kWarps][R][D + 8], channels in the joined order
+    // after the loop [W][R][D + 8], channels in the joined order
     float* join_o = reinterpret_cast<float*>(smem);
-    using L = Layout<D, NT>;
+    using L = Layout<D, NT, W>;
     constexpr bool kShared = kSharedQueries<D, NT>;
     int4* note = reinterpret_cast<int4*>(smem + L::notes) + warp * NS;  // position, -, scales
-    float2* join_ml = reinterpret_cast<float2*>(smem + L::join_ml);     // [kWarps][R]
+    float2* join_ml = reinterpret_cast<float2*>(smem + L::join_ml);     // [W][R]
     uint4* queries = reinterpret_cast<uint4*>(smem + L::queries);       // [NT][D / 32][32 lanes]
     float* factors = reinterpret_cast<float*>(smem + L::factors);       // [R]
     int* ends = reinterpret_cast<int*>(smem + L::ends);                 // [R]: last position a row sees
@@ -309,7 +309,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                                                  a.c.heads + seg.h) * a.top
                                : nullptr;
     const u32 have = (static_cast<u32>(seg.length) + block - 1) / block;
-    const u32 turns = first + warp < end ? (end - first - warp + kWarps - 1) / kWarps : 0;
+    const u32 turns = first + warp < end ? (end - first - warp + W - 1) / W : 0;
 
     const u32 page_bytes = a.c.heads * 2 * block * D, page_scales = a.c.heads * 2;
     const u8* head_data = a.c.data + seg.h * 2 * block * D + lane * 16;
@@ -323,14 +323,14 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             if (i % 32 == 0) {
                 my_page = -1;
                 if (i + lane < turns) {
-                    my_block = (first + warp + (i + lane) * kWarps) >> sub_bits;
+                    my_block = (first + warp + (i + lane) * W) >> sub_bits;
                     if (list) my_block = static_cast<u32>(list[my_block]);
                     if (my_block < have) my_page = kv_page(table, my_block, a.c.pages);
                 }
             }
             const int page = __shfl_sync(0xffffffffu, my_page, i % 32);
             const u32 j = __shfl_sync(0xffffffffu, my_block, i % 32);
-            const u32 sub = (first + warp + i * kWarps) & ((1u << sub_bits) - 1u);
+            const u32 sub = (first + warp + i * W) & ((1u << sub_bits) - 1u);
             const int p0 = static_cast<int>(j * block + sub * 16);
             const bool there = page >= 0 && p0 <= sees_most;
             if (lane == 0) note[stage].x = there ? p0 : -1;
@@ -362,7 +362,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     // [2^14, 2^15); its factor is scale2 over that power.
     u32 qf[kShared ? 1 : D / 16][2];
     float factor0 = 0.0f, factor1 = 0.0f;  // of the columns 2c, 2c + 1
-    for (u32 nt = kShared ? warp : 0; nt < NT; nt += kShared ? kWarps : 1) {
+    for (u32 nt = kShared ? warp : 0; nt < NT; nt += kShared ? W : 1) {
         const u32 n = nt * 8 + g;
         float x[KC][16];
         float most = 0.0f;
@@ -667,7 +667,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             consume(std::false_type{}, tile, noted.x, __int_as_float(noted.z), __int_as_float(noted.w),
                     tile_out);
         }
-        if (tile_out) tile_out += kWarps * R;
+        if (tile_out) tile_out += W * R;
     }
     kv_copy_wait<0>();
     __syncthreads();  // every ring is at rest: its memory takes the joined values
@@ -693,11 +693,11 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         const u32 row = x / D, at = x % D;  // `at`: in the joined order
         float top = -INFINITY;
 #pragma unroll
-        for (u32 w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * R + row].x);
+        for (u32 w = 0; w < W; ++w) top = fmaxf(top, join_ml[w * R + row].x);
         const float base = top == -INFINITY ? 0.0f : top;
         float sum = 0.0f, value = 0.0f;
 #pragma unroll
-        for (u32 w = 0; w < kWarps; ++w) {
+        for (u32 w = 0; w < W; ++w) {
             const float f = exp2_fast(join_ml[w * R + row].x - base);
             sum += join_ml[w * R + row].y * f;
             value += join_o[(w * R + row) * (D + 8) + at] * f;
@@ -733,14 +733,14 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     }
 }
 
-template <int D, int NT, bool kWhole>
-__global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(const AttentionArgs a)
+template <int D, int NT, bool kWhole, u32 W>
+__global__ void __launch_bounds__(W * 32, W == kWarps ? per_sm(D, NT) : 1) attention_kernel(const AttentionArgs a)
 {
     extern __shared__ __align__(128) u8 smem[];
-    using L = Layout<D, NT>;
+    using L = Layout<D, NT, W>;
     if constexpr (kWhole) {  // one CTA per segment, which it finishes
         const Segment seg = segment_of(a, blockIdx.x);
-        run_segment<D, NT, true>(a, seg, 0, seg.tiles, 0, smem);
+        run_segment<D, NT, true, W>(a, seg, 0, seg.tiles, 0, smem);
         return;
     }
     kv_let_next();
@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(kWarps * 32, per_sm(D, NT)) attention_kernel(c
             if (first == 0) a.span[seg.index].x = blockIdx.x;
             if (end == tiles) a.span[seg.index].y = blockIdx.x;
         }
-        run_segment<D, NT, false>(a, seg, first, end, static_cast<u64>(blockIdx.x) + seg.index, smem);
+        run_segment<D, NT, false, W>(a, seg, first, end, static_cast<u64>(blockIdx.x) + seg.index, smem);
         at = here + end;
     }
 }
@@ -906,7 +906,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
 }
 
 struct Plan {
-    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole;
+    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole, warps;
     u64 segments, part_o, part_ml, span, tile_sums, bytes;
 };
 
@@ -927,14 +927,18 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     const u64 resident = static_cast<u64>(per_sm(v.dim, p.nt)) * kv_sm_count();
     p.workers = static_cast<u32>(std::max<u64>(1, std::min<u64>(most, resident)));
     // Short segments (by the table's width or the lists' length) are finished where they are
-    // summed: one launch, where the even split takes two and joins.  The longer they are, the more
-    // of them there have to be.  With 128 channels 64 segments of 20 tiles take 9.7 us whole and
-    // 15.5 us split, 64 of 63 tiles 15.1 and 16.7 us (16 of them 14.9 and 15.1 us), 64 of 94 tiles
-    // 19.6 and 18.4 us, 128 of 94 tiles 19.8 and 21.0 us, 400 of 128 tiles 36.6 and 41.2 us.  More
-    // long ones than are resident at once should fill their last turn: 1600 lists of 128 tiles
-    // take 152 and 169 us, 512 on 444 places 74 and 64 us (512 of 21 to 63 tiles 32.0 and 36.7 us).
+    // summed: one launch, where the even split takes two and joins.  With an SM for each, they get
+    // CTAs of 8 warps: 64 of 38 tiles (128 channels) take 9.9 us, 12.4 us with 4 warps and 15.8 us
+    // split.  The longer they are, the more of them there have to be: 64 of 128 tiles take 17.7 us
+    // whole and 21.5 us split, 8 take 13.2 us split; 8 of 63 tiles 12.0 and 15.5 us.
+    const u32 sms = static_cast<u32>(kv_sm_count());
+    p.warps = p.segments <= sms ? 2 * kWarps : kWarps;
+    // With 4 warps: 400 of 128 tiles take 36.6 us whole and 41.2 us split.  More long ones than are
+    // resident at once should fill their last turn: 1600 lists of 128 tiles take 152 and 169 us,
+    // 512 on 444 places 74 and 64 us (512 of 21 to 63 tiles 32.0 and 36.7 us).
     const u64 places = (p.segments + resident - 1) / resident * resident;
-    p.whole = p.tiles <= whole_tiles(p.nt) && 2 * p.tiles <= p.segments + 64 &&
+    p.whole = p.tiles <= whole_tiles(p.nt, p.warps) &&
+              (p.segments <= sms ? p.tiles <= p.segments + 64 : 2 * p.tiles <= p.segments + 64) &&
               (p.tiles <= 64 || p.segments <= resident || p.segments * 5 >= places * 4) &&
               (!weights || p.lists * p.row_tiles == 1);
     if (p.whole) {
@@ -967,22 +971,27 @@ int check_args(const hbfsim_kv_attention_args_v1* g)
     return HBFSIM_OK;
 }
 
-template <int D, int NT, bool kWhole>
+template <int D, int NT, bool kWhole, u32 W>
 bool launch_attention(const AttentionArgs& a, cudaStream_t s)
 {
     static std::atomic<u64> seen{0};
-    using L = Layout<D, NT>;
-    if (!kv_allow_smem(attention_kernel<D, NT, kWhole>, kWhole ? L::most : L::bytes, seen)) return false;
+    using L = Layout<D, NT, W>;
+    auto* kernel = attention_kernel<D, NT, kWhole, W>;
+    if (!kv_allow_smem(kernel, kWhole ? L::most : L::bytes, seen)) return false;
     const u32 sums = kWhole && a.weights ? a.tiles * 8 * NT * 8 : 0;
-    attention_kernel<D, NT, kWhole><<<a.workers, kWarps * 32, std::max(L::bytes, L::whole_sums + sums), s>>>(a);
+    kernel<<<a.workers, W * 32, std::max(L::bytes, L::whole_sums + sums), s>>>(a);
     return cudaGetLastError() == cudaSuccess;
 }
 
 template <int D, int NT>
-int launch(const AttentionArgs& a, bool whole, cudaStream_t s)
+int launch(const AttentionArgs& a, const Plan& p, cudaStream_t s)
 {
-    if (whole) return launch_attention<D, NT, true>(a, s) ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
-    if (!launch_attention<D, NT, false>(a, s)) return HBFSIM_CUDA_ERROR;
+    if (p.whole) {
+        const bool ok = p.warps == kWarps ? launch_attention<D, NT, true, kWarps>(a, s)
+                                          : launch_attention<D, NT, true, 2 * kWarps>(a, s);
+        return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    }
+    if (!launch_attention<D, NT, false, kWarps>(a, s)) return HBFSIM_CUDA_ERROR;
     // one CTA per segment or more, up to what is resident at once; for the weights no more than
     // have blocks to sum
     const u32 pairs = a.q.seqs * a.c.heads, segments = a.lists * a.row_tiles;
@@ -1049,13 +1058,13 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     a.tile_sums = a.weights && !p.whole ? reinterpret_cast<float2*>(w + p.tile_sums) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (a.c.dim * 8 + p.nt) {
-    case 64 * 8 + 1: return launch<64, 1>(a, p.whole, s);
-    case 64 * 8 + 2: return launch<64, 2>(a, p.whole, s);
-    case 64 * 8 + 3: return launch<64, 3>(a, p.whole, s);
-    case 128 * 8 + 1: return launch<128, 1>(a, p.whole, s);
-    case 128 * 8 + 2: return launch<128, 2>(a, p.whole, s);
-    case 128 * 8 + 3: return launch<128, 3>(a, p.whole, s);
-    case 256 * 8 + 1: return launch<256, 1>(a, p.whole, s);
-    default: return launch<256, 2>(a, p.whole, s);
+    case 64 * 8 + 1: return launch<64, 1>(a, p, s);
+    case 64 * 8 + 2: return launch<64, 2>(a, p, s);
+    case 64 * 8 + 3: return launch<64, 3>(a, p, s);
+    case 128 * 8 + 1: return launch<128, 1>(a, p, s);
+    case 128 * 8 + 2: return launch<128, 2>(a, p, s);
+    case 128 * 8 + 3: return launch<128, 3>(a, p, s);
+    case 256 * 8 + 1: return launch<256, 1>(a, p, s);
+    default: return launch<256, 2>(a, p, s);
     }
 }

@@ -480,7 +480,8 @@ def test_many_sequences():
 
 
 @pytest.mark.parametrize("dim, block, heads, group, kind", [
-    (128, 16, 4, 4, "bf16"), (64, 32, 5, 8, "f16"), (256, 16, 4, 1, "bf16")])
+    (128, 16, 4, 4, "bf16"), (64, 32, 5, 8, "f16"), (256, 16, 4, 1, "bf16"), (128, 16, 8, 2, "f16"),
+    (64, 64, 9, 5, "bf16"), (128, 32, 5, 16, "bf16"), (256, 32, 4, 13, "f16"), (64, 16, 4, 24, "f16")])
 def test_attention_many_short_rows(dim, block, heads, group, kind):
     """Enough (sequence, head) pairs for each to be finished by one thread block up to 70 tiles of
     16 tokens; the same rows shared out and joined, in a wider table; lists of them."""
