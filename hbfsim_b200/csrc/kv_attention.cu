@@ -27,7 +27,8 @@
 // asynchronous copies of its own (no block barrier inside the loop), join
 // through shared memory and leave one partial result per segment met;
 // finish_kernel joins the partials of a segment and turns the tiles' sums
-// into block weights.  Short segments have a CTA each and need neither.
+// into block weights.  Short segments have a CTA each, of 8 warps if it has an
+// SM to itself, and need neither (one of 301 tokens takes 6.7 us).
 //
 // One decode step of 64 sequences of 1024 to 32768 tokens, 8 heads of 128
 // channels with 4 rows each, takes 399 us with weights: 2.21 GB at 5.5 TB/s,

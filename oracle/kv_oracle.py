@@ -1,5 +1,5 @@
 """The operators of include/hbfsim/kv_v1.h in 64 bits, one value at a time
-where that is clearest (numpy; the checker, not the product path).  Caches
+where that is clearest (numpy; not the product path).  Caches
 are dicts of numpy arrays: data (uint8 e4m3 codes [P, H, 2, T, D]), scale
 (float64 [P, H, 2]), bounds (int8 [P, H, 2, D])."""
 from __future__ import annotations
