@@ -113,7 +113,7 @@ def test_select_refusals(lib, top, sink, recent, size, blocks):
     dict(blocks=4096, counts=4096, top=0), dict(out=None), dict(out=4097), dict(lse=4098),
     dict(weights=4098), dict(workspace=None), dict(workspace=4104), dict(workspace_bytes=16)])
 def test_attention_refusals(lib, over):
-    wide = query(width=40, table_stride=40)  # a call that needs a workspace
+    wide = query(width=200, table_stride=200)  # a call that needs a workspace
     assert lib.hbfsim_kv_attention_v1(ref(cache()), ref(wide), ref(attention(**over)),
                                       None) == INVALID
 
