@@ -28,7 +28,8 @@
 // through shared memory and leave one partial result per segment met;
 // finish_kernel joins the partials of a segment and turns the tiles' sums
 // into block weights.  Short segments have a CTA each, of 8 warps if it has an
-// SM to itself, and need neither (one of 301 tokens takes 6.7 us).
+// SM to itself, and need neither (one of 301 tokens takes 6.7 us); few that
+// are longer have a team of CTAs each.
 //
 // One decode step of 64 sequences of 1024 to 32768 tokens, 8 heads of 128
 // channels with 4 rows each, takes 399 us with weights: 2.21 GB at 5.5 TB/s,
@@ -57,6 +58,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // more the sums of their weights cost CTAs on an SM: 400 segments of 125 tiles and 16 rows took 78
 // us whole and 58 us split.
 constexpr u32 whole_tiles(u32 nt, u32 warps) { return nt == 1 || warps > kWarps ? 128 : 32; }
+// Few longer segments are finished by teams of up to 8 CTAs (a cluster) that join through
+// distributed shared memory: from 64 tiles on, 16 to a CTA at least (38 tiles took 11.0 us by two
+// CTAs and 9.7 us by one), as long as all teams are resident at once.
+constexpr u32 kTeamFrom = 64, kTeamTiles = 16, kTeamPlaces = 128;
 constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
 struct AttentionArgs {
@@ -74,6 +79,7 @@ struct AttentionArgs {
     u32 lists, row_tiles, rows;   // rows of one (sequence, list, head)
     u32 units, per_unit;
     u32 workers;                  // CTAs of attention_kernel
+    u32 team;                     // CTAs (a cluster) that finish a segment together
     u32 tiles;                    // 16-token tiles per segment at most
     float* part_o;                // [workers + segments][8 NT][D], at worker + segment, channels
                                   // in the joined order
@@ -277,7 +283,14 @@ struct Layout {
     static constexpr u32 most = whole_sums + whole_tiles(NT, W) * 8 * NT * 8;
 };
 
-// One segment's tiles [first, end) by one CTA; the partial result goes to `part`.
+// Tiles of each CTA of a team, whole blocks.
+HD constexpr u32 part_of(u32 tiles, u32 team, u32 block_tiles)
+{
+    return (tiles + team * block_tiles - 1) / (team * block_tiles) * block_tiles;
+}
+
+// One segment's tiles [first, end) by one CTA; the partial result goes to `part` (a whole segment:
+// joined with those of its team, in which this CTA is number `part`).
 template <int D, int NT, bool kWhole, u32 W>
 __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segment& seg, u32 first,
                                             u32 end, u64 part, u8* smem)
@@ -690,6 +703,15 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         }
     __syncthreads();
     float* inverses = reinterpret_cast<float*>(ends);
+    // what a team's CTA joins lies behind its warps' values, in what was the ring
+    const u32 team = kWhole && W > kWarps ? a.team : 1u, rank = kWhole ? static_cast<u32>(part) : 0u;
+    float* cta_o = reinterpret_cast<float*>(smem + L::join);     // [R][D]
+    float2* cta_ml = reinterpret_cast<float2*>(smem + L::notes); // [R]
+    static_assert(W == kWarps || (L::join + R * D * 4 <= L::ring && NS * W * 16 >= R * 8));
+    auto peek2 = [](const float2* mine, u32 r) {
+        const u64 x = kv_peek(reinterpret_cast<const u64*>(mine), r);
+        return make_float2(__uint_as_float(static_cast<u32>(x)), __uint_as_float(static_cast<u32>(x >> 32)));
+    };
     for (u32 x = threadIdx.x; x < R * D; x += blockDim.x) {
         const u32 row = x / D, at = x % D;  // `at`: in the joined order
         float top = -INFINITY;
@@ -706,6 +728,9 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         if constexpr (!kWhole) {
             a.part_o[part * R * D + x] = value;
             if (at == 0) a.part_ml[part * R + row] = make_float2(top, sum);
+        } else if (team > 1) {
+            cta_o[x] = value;
+            if (at == 0) cta_ml[row] = make_float2(top, sum);
         } else if (row < rows) {
             put_out(a, seg, seg.rt * R + row, channel_of(D, at), sum == 0.0f ? 0.0f : value / sum);
             if (at == 0) {
@@ -715,23 +740,58 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             }
         }
     }
-    __syncthreads();  // before the next segment's copies
-    if (kWhole && a.weights) {  // one row tile and one list: the weights are this CTA's
-        float* weights = a.weights + (static_cast<u64>(seg.seq) * a.c.heads + seg.h) * a.q.width;
-        const u32 listed = (end + (1u << sub_bits) - 1) >> sub_bits;
-        if (list || listed < a.q.width) {
-            for (u32 j = threadIdx.x; j < a.q.width; j += blockDim.x) weights[j] = 0.0f;
-            __syncthreads();
+    float* weights = nullptr;
+    if (kWhole && a.weights) {  // one row tile and one list: the weights are this segment's
+        weights = a.weights + (static_cast<u64>(seg.seq) * a.c.heads + seg.h) * a.q.width;
+        const u32 from = list ? 0 : (seg.tiles + (1u << sub_bits) - 1) >> sub_bits;
+        for (u32 j = from + rank * blockDim.x + threadIdx.x; j < a.q.width; j += team * blockDim.x) weights[j] = 0.0f;
+    }
+    if (team > 1) {
+        // join the CTAs, each a run of the values: their sums at the team's maximum
+        kv_team_sync(KvTeam{rank, team});
+        auto total = [&](u32 row, float& base, float& sum) {
+            float top = -INFINITY;
+            for (u32 r = 0; r < team; ++r) top = fmaxf(top, peek2(cta_ml + row, r).x);
+            base = top == -INFINITY ? 0.0f : top;
+            sum = 0.0f;
+            for (u32 r = 0; r < team; ++r) {
+                const float2 its = peek2(cta_ml + row, r);
+                sum += its.y * exp2_fast(its.x - base);
+            }
+        };
+        const u32 run = R * D / team;
+        for (u32 x = rank * run + threadIdx.x; x < (rank + 1) * run; x += blockDim.x) {
+            const u32 row = x / D, at = x % D;
+            if (row >= rows) continue;
+            float base, sum, value = 0.0f;
+            total(row, base, sum);
+            for (u32 r = 0; r < team; ++r)
+                value += __uint_as_float(kv_peek(reinterpret_cast<const u32*>(cta_o + x), r)) *
+                         exp2_fast(peek2(cta_ml + row, r).x - base);
+            put_out(a, seg, seg.rt * R + row, channel_of(D, at), sum == 0.0f ? 0.0f : value / sum);
+            if (at == 0 && a.lse)
+                a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
         }
-        for (u32 k = threadIdx.x; k < listed; k += blockDim.x) {
+        if (weights && threadIdx.x < rows) {
+            float base, sum;
+            total(threadIdx.x, base, sum);
+            factors[threadIdx.x] = base;
+            inverses[threadIdx.x] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        }
+    }
+    __syncthreads();  // before the next segment's copies
+    if (weights) {
+        const u32 to = (end + (1u << sub_bits) - 1) >> sub_bits;
+        for (u32 k = (first >> sub_bits) + threadIdx.x; k < to; k += blockDim.x) {
             float w = 0.0f;
-            for (u32 t = k << sub_bits; t < min((k + 1) << sub_bits, end); ++t)
+            for (u32 t = (k << sub_bits) - first; t < min((k + 1) << sub_bits, end) - first; ++t)
                 for (u32 r = 0; r < rows; ++r)
                     w += whole_sums[t * R + r].x * (exp2_fast(whole_sums[t * R + r].y - factors[r]) * inverses[r]);
             const u32 j = list ? static_cast<u32>(list[k]) : k;
             if (j < a.q.width) weights[j] = w;
         }
     }
+    if (team > 1) kv_team_sync(KvTeam{rank, team});  // nobody leaves while another may read its sums
 }
 
 template <int D, int NT, bool kWhole, u32 W>
@@ -739,9 +799,11 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? per_sm(D, NT) : 1) atten
 {
     extern __shared__ __align__(128) u8 smem[];
     using L = Layout<D, NT, W>;
-    if constexpr (kWhole) {  // one CTA per segment, which it finishes
-        const Segment seg = segment_of(a, blockIdx.x);
-        run_segment<D, NT, true, W>(a, seg, 0, seg.tiles, 0, smem);
+    if constexpr (kWhole) {  // a CTA or a team per segment, which it finishes
+        const u32 team = W > kWarps ? a.team : 1u, rank = blockIdx.x % team;
+        const Segment seg = segment_of(a, blockIdx.x / team);
+        const u32 each = part_of(seg.tiles, team, a.c.block / 16), first = min(rank * each, seg.tiles);
+        run_segment<D, NT, true, W>(a, seg, first, min(first + each, seg.tiles), rank, smem);
         return;
     }
     kv_let_next();
@@ -907,7 +969,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
 }
 
 struct Plan {
-    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole, warps;
+    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole, warps, team;
     u64 segments, part_o, part_ml, span, tile_sums, bytes;
 };
 
@@ -930,20 +992,26 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     // Short segments (by the table's width or the lists' length) are finished where they are
     // summed: one launch, where the even split takes two and joins.  With an SM for each, they get
     // CTAs of 8 warps: 64 of 38 tiles (128 channels) take 9.9 us, 12.4 us with 4 warps and 15.8 us
-    // split.  The longer they are, the more of them there have to be: 64 of 128 tiles take 17.7 us
-    // whole and 21.5 us split, 8 take 13.2 us split; 8 of 63 tiles 12.0 and 15.5 us.
+    // split.  Longer ones get teams of CTAs: 8 of 128 tiles take 10.1 us and 13.2 us split, 32 of
+    // 256 tiles 14.0 and 22.0 us, 8 of 1024 tiles 19.9 and 21.4 us.  The more tiles a CTA has, the
+    // more CTAs there have to be: 64 of 128 tiles take 17.7 us by one CTA each and 21.5 us split.
     const u32 sms = static_cast<u32>(kv_sm_count());
     p.warps = p.segments <= sms ? 2 * kWarps : kWarps;
+    p.team = 1;
+    while (p.team < 8 && p.tiles >= kTeamFrom && p.segments * p.team * 2 <= kTeamPlaces &&
+           p.tiles >= p.team * 2 * kTeamTiles)
+        p.team *= 2;
+    const u32 each = part_of(p.tiles, p.team, v.block / 16);
     // With 4 warps: 400 of 128 tiles take 36.6 us whole and 41.2 us split.  More long ones than are
     // resident at once should fill their last turn: 1600 lists of 128 tiles take 152 and 169 us,
     // 512 on 444 places 74 and 64 us (512 of 21 to 63 tiles 32.0 and 36.7 us).
     const u64 places = (p.segments + resident - 1) / resident * resident;
-    p.whole = p.tiles <= whole_tiles(p.nt, p.warps) &&
-              (p.segments <= sms ? p.tiles <= p.segments + 64 : 2 * p.tiles <= p.segments + 64) &&
+    p.whole = each <= whole_tiles(p.nt, p.warps) &&
+              (p.segments <= sms ? each <= p.segments * p.team + 64 : 2 * p.tiles <= p.segments + 64) &&
               (p.tiles <= 64 || p.segments <= resident || p.segments * 5 >= places * 4) &&
               (!weights || p.lists * p.row_tiles == 1);
     if (p.whole) {
-        p.workers = static_cast<u32>(p.segments);
+        p.workers = static_cast<u32>(p.segments) * p.team;
         return p;  // no workspace
     }
     u64 at = 0;
@@ -979,8 +1047,10 @@ bool launch_attention(const AttentionArgs& a, cudaStream_t s)
     using L = Layout<D, NT, W>;
     auto* kernel = attention_kernel<D, NT, kWhole, W>;
     if (!kv_allow_smem(kernel, kWhole ? L::most : L::bytes, seen)) return false;
-    const u32 sums = kWhole && a.weights ? a.tiles * 8 * NT * 8 : 0;
-    kernel<<<a.workers, W * 32, std::max(L::bytes, L::whole_sums + sums), s>>>(a);
+    const u32 sums = kWhole && a.weights ? part_of(a.tiles, a.team, a.c.block / 16) * 8 * NT * 8 : 0;
+    const u32 smem = std::max(L::bytes, L::whole_sums + sums);
+    if (kWhole && a.team > 1) return kv_launch(kernel, dim3(a.workers), W * 32, s, smem, a.team, false, a);
+    kernel<<<a.workers, W * 32, smem, s>>>(a);
     return cudaGetLastError() == cudaSuccess;
 }
 
@@ -1051,6 +1121,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     a.units = p.units;
     a.per_unit = p.per_unit;
     a.workers = p.workers;
+    a.team = p.team;
     a.tiles = p.tiles;
     u8* w = static_cast<u8*>(args->workspace);
     a.part_o = reinterpret_cast<float*>(w + p.part_o);

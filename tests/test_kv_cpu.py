@@ -113,7 +113,7 @@ def test_select_refusals(lib, top, sink, recent, size, blocks):
     dict(blocks=4096, counts=4096, top=0), dict(out=None), dict(out=4097), dict(lse=4098),
     dict(weights=4098), dict(workspace=None), dict(workspace=4104), dict(workspace_bytes=16)])
 def test_attention_refusals(lib, over):
-    wide = query(width=200, table_stride=200)  # a call that needs a workspace
+    wide = query(width=5000, table_stride=5000)  # a call that needs a workspace
     assert lib.hbfsim_kv_attention_v1(ref(cache()), ref(wide), ref(attention(**over)),
                                       None) == INVALID
 
@@ -122,7 +122,7 @@ def test_attention_workspace_sizes(lib):
     """Short rows need none; wide ones grow with the sequences and with the weights."""
     size = lambda q, **over: lib.hbfsim_kv_attention_workspace_v1(ref(cache()), ref(q), ref(attention(**over)))
     assert size(query()) == 0
-    wide = [size(query(width=200, seqs=s), weights=w) for s in (2, 4) for w in (None, 4096)]
+    wide = [size(query(width=5000, seqs=s), weights=w) for s in (2, 4) for w in (None, 4096)]
     assert 0 < wide[0] < wide[1] and wide[0] < wide[2] < wide[3]
     assert all(w % 256 == 0 for w in wide)
 

@@ -503,6 +503,32 @@ def test_attention_many_short_rows(dim, block, heads, group, kind):
     attend_and_check(small, q, wide, lengths, lists)
 
 
+@pytest.mark.parametrize("dim, block, heads, group, tokens, kind, tiles", [
+    (128, 16, 1, 4, 1, "bf16", 64), (64, 32, 2, 8, 1, "f16", 130), (128, 64, 3, 5, 1, "bf16", 300),
+    (256, 16, 2, 2, 1, "f16", 200), (128, 16, 1, 16, 1, "bf16", 1000), (64, 16, 4, 3, 2, "f16", 128),
+    (256, 64, 1, 12, 1, "bf16", 96), (128, 32, 4, 24, 1, "f16", 66), (64, 64, 8, 1, 1, "bf16", 65)])
+def test_attention_teams(dim, block, heads, group, tokens, kind, tiles):
+    """Few longer rows, each finished by several thread blocks; some of them have nothing to do for
+    a short sequence."""
+    torch = torch_()
+    rng = np.random.default_rng(tiles + dim)
+    width = -(-tiles * 16 // block)
+    lengths = [width * block, 0, width * block // 2 + 3, 5]
+    small = random_cache(rng, 30, heads, block, dim)
+    table = rng.integers(0, 30, (len(lengths), width)).astype(np.int32)
+    table[rng.random(table.shape) < 0.03] = -1
+    x = rng.standard_normal((len(lengths), tokens, heads * group, dim))
+    q = torch.from_numpy(x).to(type_of(kind)).cuda()
+    got = attend_and_check(small, q, table, lengths)
+    again = attend_and_check(small, q, table, lengths)
+    for a, b in zip(got, again):
+        assert torch.equal(a, b)
+    have = [-(-n // block) for n in lengths]
+    lists = [[[[int(j) for j in rng.permutation(have[b])] for _ in range(heads)]
+              for _ in range(tokens)] for b in range(len(lengths))]
+    attend_and_check(small, q, table, lengths, lists)
+
+
 def test_many_sequences_wide_tables():
     """The split over more (sequence, head) pairs than a grid's second axis holds."""
     torch = torch_()
