@@ -781,7 +781,8 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     }
     __syncthreads();  // before the next segment's copies
     if (weights) {
-        const u32 to = (end + (1u << sub_bits) - 1) >> sub_bits;
+        // (a CTA of a team without tiles begins where the segment ends, inside a block perhaps)
+        const u32 to = first < end ? (end + (1u << sub_bits) - 1) >> sub_bits : 0;
         for (u32 k = (first >> sub_bits) + threadIdx.x; k < to; k += blockDim.x) {
             float w = 0.0f;
             for (u32 t = (k << sub_bits) - first; t < min((k + 1) << sub_bits, end) - first; ++t)

@@ -529,6 +529,37 @@ def test_attention_teams(dim, block, heads, group, tokens, kind, tiles):
     attend_and_check(small, q, table, lengths, lists)
 
 
+@pytest.mark.parametrize("dim, block, heads, group, tokens, kind, tiles, seqs", [
+    (64, 16, 2, 8, 5, "bf16", 20, 3), (128, 32, 2, 16, 4, "f16", 150, 2), (256, 16, 1, 5, 8, "bf16", 70, 4),
+    (64, 64, 4, 24, 2, "f16", 40, 30), (128, 16, 1, 7, 16, "bf16", 500, 1)])
+def test_attention_many_rows_without_weights(dim, block, heads, group, tokens, kind, tiles, seqs):
+    """Several row tiles per key/value head, each finished by its own thread blocks."""
+    torch = torch_()
+    rng = np.random.default_rng(tiles + dim + seqs)
+    width = -(-tiles * 16 // block)
+    lengths = [width * block] + [int(x) for x in rng.integers(0, width * block, seqs - 1)]
+    small = random_cache(rng, 30, heads, block, dim)
+    table = rng.integers(0, 30, (seqs, width)).astype(np.int32)
+    q = torch.from_numpy(rng.standard_normal((seqs, tokens, heads * group, dim))).to(type_of(kind)).cuda()
+    attend_and_check(small, q, table, lengths, weights=False)
+
+
+@pytest.mark.parametrize("block", [32, 64])
+def test_attention_team_ends_inside_a_block(block):
+    """Sequences of fewer tokens than a team has thread blocks for, and of a part of a block behind
+    whole parts: the weights of the last block come from one of them."""
+    torch = torch_()
+    rng = np.random.default_rng(block)
+    heads, dim, group = 2, 64, 4
+    width = 128 * 16 // block
+    lengths = [1, 17, 33, block + 1, block + 17, 3 * block + 1, width * block - 17]
+    small = random_cache(rng, 30, heads, block, dim)
+    table = rng.integers(0, 30, (len(lengths), width)).astype(np.int32)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), 1, heads * group, dim))).to(torch.bfloat16).cuda()
+    for _ in range(20):
+        attend_and_check(small, q, table, lengths)
+
+
 def test_many_sequences_wide_tables():
     """The split over more (sequence, head) pairs than a grid's second axis holds."""
     torch = torch_()
