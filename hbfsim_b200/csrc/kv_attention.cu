@@ -11,14 +11,17 @@
 // K and V are read in their natural order straight into the fragments of
 // mma.m16n8k16: the order of the channels inside a dot product and of the
 // tokens inside a sum is free, so each lane takes 16 contiguous bytes.  e4m3
-// widens to f16 without loss; a block's scales are powers of two and are
-// applied in fp32 to the scores and to the probabilities (relative to the
-// largest value scale met so far), so no product is rounded by them.  Queries
-// are scaled per row by a power of two into f16's range, exact as well.
+// widens to f16 without loss.  A block's scales are powers of two: the keys'
+// is applied in fp32 to the scores, the values' to the probabilities, relative
+// to a reference of the row.  Queries are scaled per row by a power of two
+// into f16's range, which keeps all that is within 2^29 of the row's largest.
 // Scores, the running maximum, sums and the output accumulate in fp32.  The
-// probabilities are rounded to f16 (2^-11 relative, no more than the output
-// type's own rounding) for the second product only; the sums and the block
-// weights use them unrounded.
+// probabilities, times the value scale, are rounded to f16 for the second
+// product only: 2^-11 relative, no more than the output type's own rounding,
+// down to 2^-23 of the row's largest (2^-13 where the scales differ by
+// kNear); what is smaller loses 2^-34 (2^-24) of the largest.  Where scales
+// differ by more, the product takes bf16 pairs (2^-17 relative).  The sums and
+// the block weights use the probabilities unrounded.
 //
 // Work: the 16-token tiles of all segments (sequence, head, row tile; for
 // lists also the token) form one line that is cut into equal shares, one per
@@ -49,9 +52,20 @@ namespace {
 
 constexpr u32 kWarps = 4;
 constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
-// How far (in log2) a score may exceed the reference before the reference moves: a tile then
-// costs a vote instead of a maximum over the lanes.  2^kAbove keeps f16 probabilities finite.
-constexpr float kAbove = 8.0f;
+// The probabilities of a row stand against a reference of its scores (log2, a whole number), which
+// moves up only when a score is 2^kAbove above it: a tile then costs a vote instead of a maximum over
+// the lanes.  After a move the largest is at 2^kPlace or half of it, so that f16 holds them all and
+// keeps its 11 bits down to 2^-23 of the largest.  For the product with the values they are multiplied by their
+// block's value scale over the greatest that the warp has met.
+constexpr float kAbove = 15.0f, kPlace = 10.0f;
+// That holds for scales within kNear of each other.  Past it a block of large scale and no weight
+// would push the others out of f16's range, so from there on the warp keeps a second reference for
+// each row, of scores plus the logarithm of their value scale, which what really counts sets, and
+// takes pairs of bf16 (16 bits, fp32's range) in twice the products.  They lie 2^kLift higher: up to
+// 2^kFarAbove, which times 448 times 2^31 tokens is still a number, and down to 2^-126, so that not
+// even values that are all 0 in a block of large scale and weight hide the others.
+constexpr float kNear = 1024.0f;
+constexpr float kFarAbove = 85.0f, kFarPlace = 81.0f, kLift = 70.0f;
 constexpr float kNoScore = -3.0e38f;  // reference of a row without a score
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Tiles of a segment that one CTA of so many warps may take whole, at most.  With two row tiles or
@@ -83,7 +97,8 @@ struct AttentionArgs {
     u32 tiles;                    // 16-token tiles per segment at most
     float* part_o;                // [workers + segments][8 NT][D], at worker + segment, channels
                                   // in the joined order
-    float2* part_ml;              // [workers + segments][8 NT]: maximum, sum
+    float2* part_ml;              // [workers + segments][8 NT]: reference of the scores, sum
+    float* part_ref;              // [workers + segments][8 NT]: reference of the values
     uint2* span;                  // [segments]: first and last worker (segments with tiles)
     float2* tile_sums;            // [segments][tiles][8 NT] or NULL: sum of exponentials, reference
 };
@@ -124,6 +139,34 @@ __device__ __forceinline__ u32 times(u32 pair, __half2 by)
     return *reinterpret_cast<const u32*>(&y);
 }
 
+__device__ __forceinline__ void mma16816_bf16(float (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0,
+                                              u32 b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ u32 pack_bf16(float lo, float hi)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const u32*>(&h);
+}
+
+// Stored values from f16 to bf16: exact (4 significant bits, 2^-9 to 448).
+__device__ __forceinline__ u32 bf16_of(u32 pair)
+{
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    return pack_bf16(y.x, y.y);
+}
+
+// What two bf16 roundings leave of a pair.
+__device__ __forceinline__ u32 rest_of(u32 pair, float lo, float hi)
+{
+    return pack_bf16(lo - __uint_as_float(pair << 16), hi - __uint_as_float(pair & 0xffff0000u));
+}
+
 __device__ __forceinline__ float exp2_fast(float x)  // 2^-22 relative, 0 for -inf
 {
     float r;
@@ -135,6 +178,17 @@ __device__ __forceinline__ float exp2_fast(float x)  // 2^-22 relative, 0 for -i
 __device__ __forceinline__ float inverse_power(float x)
 {
     return __int_as_float((254 << 23) - __float_as_int(x));
+}
+
+// Exponent of a power of two.
+__device__ __forceinline__ float exponent_of(float x) { return static_cast<float>((__float_as_int(x) >> 23 & 0xff) - 127); }
+
+// x * 2^by in two steps (by: a whole number): the power may be past fp32's range where the result
+// is not.
+__device__ __forceinline__ float at_power(float x, float by)
+{
+    const float half = rintf(0.5f * by);
+    return x * exp2_fast(half) * exp2_fast(by - half);
 }
 
 // Place of byte o of a tile side in shared memory: the 16-byte pieces of a
@@ -274,7 +328,10 @@ struct Layout {
     static constexpr u32 join = W * 8 * NT * (D + 8) * 4;
     static constexpr u32 notes = ring > join ? ring : join;
     static constexpr u32 join_ml = notes + W * kStages<D> * 16;
-    static constexpr u32 queries = join_ml + W * 8 * NT * 8;
+    static constexpr u32 join_ref = join_ml + W * 8 * NT * 8;
+    static constexpr u32 join_factor = join_ref + W * 8 * NT * 4;
+    static constexpr u32 row_power = join_factor + W * 8 * NT * 8;
+    static constexpr u32 queries = row_power + 8 * NT * 8;
     static constexpr u32 factors = queries + (kSharedQueries<D, NT> ? NT * D * 16 : 0);
     static constexpr u32 ends = factors + 8 * NT * 4;
     static constexpr u32 line = ends + 8 * NT * 4;  // of the split; for whole segments:
@@ -308,6 +365,9 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     constexpr bool kShared = kSharedQueries<D, NT>;
     int4* note = reinterpret_cast<int4*>(smem + L::notes) + warp * NS;  // position, -, scales
     float2* join_ml = reinterpret_cast<float2*>(smem + L::join_ml);     // [W][R]
+    float* join_ref = reinterpret_cast<float*>(smem + L::join_ref);     // [W][R]
+    float2* join_factor = reinterpret_cast<float2*>(smem + L::join_factor);  // [W][R]
+    float2* row_power = reinterpret_cast<float2*>(smem + L::row_power);      // [R]
     uint4* queries = reinterpret_cast<uint4*>(smem + L::queries);       // [NT][D / 32][32 lanes]
     float* factors = reinterpret_cast<float*>(smem + L::factors);       // [R]
     int* ends = reinterpret_cast<int*>(smem + L::ends);                 // [R]: last position a row sees
@@ -436,15 +496,16 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     __syncthreads();
 
     float o[NT][D / 16][4];
-    float m[NT][2], l[NT][2];
-    float value_scale = 0.0f, value_inverse = 0.0f;
+    float m[NT][2], l[NT][2], ref[NT][2];  // reference and sum of the scores; of the values, if far
+    // the greatest value scale met, its inverse, 1 / kNear of it; the least
+    float value_scale = 0.0f, value_inverse = 0.0f, floor_scale = 0.0f, least_scale = INFINITY;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.0f;
-        m[nt][0] = m[nt][1] = kNoScore;
+        m[nt][0] = m[nt][1] = ref[nt][0] = ref[nt][1] = kNoScore;
         l[nt][0] = l[nt][1] = 0.0f;
     }
     // where the lane's pieces lie in a tile side, and the same 8 tokens further: at D = 64 that
@@ -471,10 +532,19 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         t = min(t, __shfl_xor_sync(0xffffffffu, t, 1));
         return min(t, __shfl_xor_sync(0xffffffffu, t, 2));
     };
-    // One tile.  `edge`: some row does not see all of its tokens.
-    auto consume = [&](auto is_edge, const u8* tile, int p0, float key_scale, float new_scale,
-                       float2* tile_out) {
-        constexpr bool kEdge = decltype(is_edge)::value;
+    auto multiply = [&](float by) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[nt][k][x] *= by;
+    };
+    // One tile.  `edge`: some row does not see all of its tokens; `far`: see kNear.  False, with
+    // nothing summed, where this tile's value scale is the first that is far from those before it.
+    auto consume = [&](auto is_edge, auto is_far, const u8* tile, int p0, float key_scale, float new_scale,
+                       float2* tile_out) -> bool {
+        constexpr bool kEdge = decltype(is_edge)::value, kFar = decltype(is_far)::value;
         // with one row tile two sums, so that products need not wait for each other
         constexpr int kSums = NT == 1 ? 2 : 1;
         float s[NT][kSums][4];
@@ -533,43 +603,46 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 }
             }
         }
-        // largest value scale so far; a change rescales what is summed
-        if (new_scale > value_scale) {
-            value_inverse = inverse_power(new_scale);
-            const float carry = value_scale * value_inverse;
-            value_scale = new_scale;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[nt][k][i] *= carry;
+        if constexpr (!kFar) {
+            least_scale = fminf(least_scale, new_scale);
+            if (new_scale > value_scale || new_scale < floor_scale) {
+                if (value_scale > 0.0f && fmaxf(new_scale, value_scale) > least_scale * kNear) return false;
+                value_inverse = inverse_power(new_scale);
+                multiply(value_scale * value_inverse);  // a change rescales what is summed
+                value_scale = new_scale;
+                floor_scale = new_scale * (1.0f / kNear);
+            }
         }
+        const float value_log2 = exponent_of(new_scale);
         const __half2 relative = __float2half2_rn(new_scale * value_inverse);
-        u32 b[NT][2];
+        u32 b[NT][2], b_rest[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float p[4], sum[2];
+            float p[4], w[4], sum[2];  // scores against the references, then probabilities and factors
             float2 factor = make_float2(factor0, factor1);
             if constexpr (kShared) factor = *reinterpret_cast<const float2*>(factors + nt * 8 + 2 * c);
             const float scaled[2] = {factor.x * key_scale, factor.y * key_scale};
-            // scores against the reference of their row
             auto against = [&]() {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     p[i] = fmaf(s[nt][0][i], scaled[i], -m[nt][i]);
                     p[2 + i] = fmaf(s[nt][0][2 + i], scaled[i], -m[nt][i]);
+                    if constexpr (kFar) {
+                        const float at = value_log2 - ref[nt][i];  // exact: whole numbers
+                        w[i] = fmaf(s[nt][0][i], scaled[i], at);
+                        w[2 + i] = fmaf(s[nt][0][2 + i], scaled[i], at);
+                    }
                     if constexpr (kEdge) {
                         const int end = ends[nt * 8 + 2 * c + i];
-                        if (p0 + static_cast<int>(g) > end) p[i] = -INFINITY;
-                        if (p0 + static_cast<int>(g) + 8 > end) p[2 + i] = -INFINITY;
+                        if (p0 + static_cast<int>(g) > end) p[i] = w[i] = -INFINITY;
+                        if (p0 + static_cast<int>(g) + 8 > end) p[2 + i] = w[2 + i] = -INFINITY;
                     }
                 }
             };
             against();
-            // the reference of the exponentials follows the maximum only when a score is far
-            // above it; until then probabilities reach 2^kAbove
-            if (__any_sync(0xffffffffu, fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])) > kAbove)) {
+            bool moves = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])) > kAbove;
+            if constexpr (kFar) moves |= fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > kFarAbove;
+            if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float most = -INFINITY;
@@ -578,14 +651,26 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1)
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-                    const float now = fmaxf(m[nt][i], most);
+                    const float now = fmaxf(m[nt][i], ceilf(most) - kPlace);
                     const float shrink = exp2_fast(m[nt][i] - now);
-                    m[nt][i] = now;
                     l[nt][i] *= shrink;
+                    m[nt][i] = now;
+                    float once = shrink, again = 1.0f;
+                    if constexpr (kFar) {
+                        const float now_ref = fmaxf(ref[nt][i], ceilf(most + value_log2) - kFarPlace);
+                        const float by = ref[nt][i] - now_ref, half = rintf(0.5f * by);  // as at_power
+                        once = exp2_fast(half);
+                        again = exp2_fast(by - half);
+                        ref[nt][i] = now_ref;
+                    }
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
-                        o[nt][k][i] *= shrink;
-                        o[nt][k][2 + i] *= shrink;
+                        o[nt][k][i] *= once;
+                        o[nt][k][2 + i] *= once;
+                        if constexpr (kFar) {
+                            o[nt][k][i] *= again;
+                            o[nt][k][2 + i] *= again;
+                        }
                     }
                 }
                 against();
@@ -597,8 +682,17 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 sum[i] = p[i] + p[2 + i];
                 l[nt][i] += sum[i];
             }
-            b[nt][0] = transpose8x8(times(pack_f16(p[0], p[1]), relative));
-            b[nt][1] = transpose8x8(times(pack_f16(p[2], p[3]), relative));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (kFar) {
+                    const float x = exp2_fast(w[2 * i]), y = exp2_fast(w[2 * i + 1]);
+                    const u32 most = pack_bf16(x, y);
+                    b[nt][i] = transpose8x8(most);
+                    b_rest[nt][i] = transpose8x8(rest_of(most, x, y));
+                } else {
+                    b[nt][i] = transpose8x8(times(pack_f16(p[2 * i], p[2 * i + 1]), relative));
+                }
+            }
             if (tile_out) {
                 // the two columns' sums over the lanes of all g, the even g keeping the first
                 const float mine = g & 1 ? sum[1] : sum[0], other = g & 1 ? sum[0] : sum[1];
@@ -653,11 +747,21 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                         }
                     }
                 }
+                if constexpr (kFar) {
+                    a0 = bf16_of(a0), a1 = bf16_of(a1), a2 = bf16_of(a2), a3 = bf16_of(a3);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    mma16816(o[nt][k], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816_bf16(o[nt][k], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                        mma16816_bf16(o[nt][k], a0, a1, a2, a3, b_rest[nt][0], b_rest[nt][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma16816(o[nt][k], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                }
             }
         }
+        return true;
     };
 
     u32 stage = 0;
@@ -665,27 +769,50 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     float2* tile_out = nullptr;
     if (a.weights)
         tile_out = (kWhole ? whole_sums : a.tile_sums + (static_cast<u64>(seg.index) * a.tiles + first) * R) + warp * R;
-    for (u32 i = 0; i < turns; ++i) {
+    auto nothing = [&]() {
+        if (tile_out && lane < rows) tile_out[lane] = make_float2(0.0f, kNoScore);
+    };
+    u32 i = 0;
+    auto next = [&]() {
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        if (tile_out) tile_out += W * R;
+        ++i;
+    };
+    auto wait = [&]() {
         kv_copy_wait<NS - 2>();
         __syncwarp();  // the stage is there, and every lane is done with the one before it
         issue(i + NS - 1, stage == 0 ? NS - 1 : stage - 1);
+    };
+    for (; i < turns; next()) {
+        wait();
         const int4 noted = note[stage];
         const u8* tile = ring + stage * 2 * kSide;
-        stage = stage + 1 == NS ? 0 : stage + 1;
-        if (noted.x < 0) {
-            if (tile_out && lane < rows) tile_out[lane] = make_float2(0.0f, kNoScore);
-        } else if (noted.x + 15 > sees_least) {
-            consume(std::true_type{}, tile, noted.x, __int_as_float(noted.z), __int_as_float(noted.w),
-                    tile_out);
-        } else {
-            consume(std::false_type{}, tile, noted.x, __int_as_float(noted.z), __int_as_float(noted.w),
-                    tile_out);
-        }
-        if (tile_out) tile_out += W * R;
+        const float key_scale = __int_as_float(noted.z), new_scale = __int_as_float(noted.w);
+        bool done = true;
+        if (noted.x < 0) nothing();
+        else if (noted.x + 15 > sees_least)
+            done = consume(std::true_type{}, std::false_type{}, tile, noted.x, key_scale, new_scale, tile_out);
+        else
+            done = consume(std::false_type{}, std::false_type{}, tile, noted.x, key_scale, new_scale, tile_out);
+        if (!done) break;
+    }
+    // the references of the rows' values, lifted
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) ref[nt][x] = m[nt][x] + (exponent_of(value_scale) - kLift);
+    multiply(kv_power(static_cast<int>(kLift)));
+    for (bool waited = true; i < turns; next(), waited = false) {
+        if (!waited) wait();
+        const int4 noted = note[stage];
+        if (noted.x < 0) nothing();
+        else
+            consume(std::true_type{}, std::true_type{}, ring + stage * 2 * kSide, noted.x, __int_as_float(noted.z),
+                    __int_as_float(noted.w), tile_out);
     }
     kv_copy_wait<0>();
     __syncthreads();  // every ring is at rest: its memory takes the joined values
-    // join the warps: every warp's sums at its own maximum, values times its scale
+    // join the warps: every warp's sums and values at its own references
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -694,12 +821,14 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             const u32 row = nt * 8 + 2 * c + i;
-            if (g == 0)
+            if (g == 0) {
                 join_ml[warp * R + row] = make_float2(m[nt][i] == kNoScore ? -INFINITY : m[nt][i], sum);
+                join_ref[warp * R + row] = ref[nt][i];
+            }
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
                 *reinterpret_cast<float2*>(join_o + (warp * R + row) * (D + 8) + k * 16 + g * 2) =
-                    make_float2(o[nt][k][i] * value_scale, o[nt][k][2 + i] * value_scale);
+                    make_float2(o[nt][k][i], o[nt][k][2 + i]);
         }
     __syncthreads();
     float* inverses = reinterpret_cast<float*>(ends);
@@ -707,37 +836,64 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
     const u32 team = kWhole && W > kWarps ? a.team : 1u, rank = kWhole ? static_cast<u32>(part) : 0u;
     float* cta_o = reinterpret_cast<float*>(smem + L::join);     // [R][D]
     float2* cta_ml = reinterpret_cast<float2*>(smem + L::notes); // [R]
-    static_assert(W == kWarps || (L::join + R * D * 4 <= L::ring && NS * W * 16 >= R * 8));
+    float* cta_ref = reinterpret_cast<float*>(cta_ml + R);       // [R]
+    static_assert(W == kWarps || (L::join + R * D * 4 <= L::ring && NS * W * 16 >= R * 12));
+    auto peek = [](const float* mine, u32 r) { return __uint_as_float(kv_peek(reinterpret_cast<const u32*>(mine), r)); };
     auto peek2 = [](const float2* mine, u32 r) {
         const u64 x = kv_peek(reinterpret_cast<const u64*>(mine), r);
         return make_float2(__uint_as_float(static_cast<u32>(x)), __uint_as_float(static_cast<u32>(x >> 32)));
     };
+    // a thread for each row and warp: the powers of two that the warp's values are multiplied by, in
+    // two steps as at_power takes them; the first warp's also finish the row's sum
+    auto steps = [](float by) {
+        const float half = rintf(0.5f * by);
+        return make_float2(exp2_fast(half), exp2_fast(by - half));
+    };
+    if (threadIdx.x < W * R) {
+        const u32 row = threadIdx.x % R;
+        float value_top = kNoScore;
+#pragma unroll
+        for (u32 w = 0; w < W; ++w) value_top = fmaxf(value_top, join_ref[w * R + row]);
+        join_factor[threadIdx.x] = steps(join_ref[threadIdx.x] - value_top);
+        if (threadIdx.x < R) {
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (u32 w = 0; w < W; ++w) top = fmaxf(top, join_ml[w * R + row].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (u32 w = 0; w < W; ++w) sum += join_ml[w * R + row].y * exp2_fast(join_ml[w * R + row].x - base);
+            if constexpr (!kWhole) {
+                a.part_ml[part * R + row] = make_float2(top, sum);
+                a.part_ref[part * R + row] = value_top;
+            } else if (team > 1) {
+                cta_ml[row] = make_float2(top, sum);
+                cta_ref[row] = value_top;
+            } else {
+                factors[row] = base;  // the queries' factors and ends are not needed any more
+                inverses[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                row_power[row] = steps(value_top - base);
+                if (row < rows && a.lse)
+                    a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
+            }
+        }
+    }
+    __syncthreads();
     for (u32 x = threadIdx.x; x < R * D; x += blockDim.x) {
         const u32 row = x / D, at = x % D;  // `at`: in the joined order
-        float top = -INFINITY;
-#pragma unroll
-        for (u32 w = 0; w < W; ++w) top = fmaxf(top, join_ml[w * R + row].x);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, value = 0.0f;
+        float value = 0.0f;
 #pragma unroll
         for (u32 w = 0; w < W; ++w) {
-            const float f = exp2_fast(join_ml[w * R + row].x - base);
-            sum += join_ml[w * R + row].y * f;
-            value += join_o[(w * R + row) * (D + 8) + at] * f;
+            const float2 f = join_factor[w * R + row];
+            value += join_o[(w * R + row) * (D + 8) + at] * f.x * f.y;
         }
         if constexpr (!kWhole) {
             a.part_o[part * R * D + x] = value;
-            if (at == 0) a.part_ml[part * R + row] = make_float2(top, sum);
         } else if (team > 1) {
             cta_o[x] = value;
-            if (at == 0) cta_ml[row] = make_float2(top, sum);
         } else if (row < rows) {
-            put_out(a, seg, seg.rt * R + row, channel_of(D, at), sum == 0.0f ? 0.0f : value / sum);
-            if (at == 0) {
-                factors[row] = base;  // the queries' factors and ends are not needed any more
-                inverses[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (a.lse) a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
-            }
+            const float inverse = inverses[row];  // 0: the row sees nothing
+            const float2 f = row_power[row];
+            put_out(a, seg, seg.rt * R + row, channel_of(D, at), inverse == 0.0f ? 0.0f : value * inverse * f.x * f.y);
         }
     }
     float* weights = nullptr;
@@ -763,12 +919,13 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         for (u32 x = rank * run + threadIdx.x; x < (rank + 1) * run; x += blockDim.x) {
             const u32 row = x / D, at = x % D;
             if (row >= rows) continue;
-            float base, sum, value = 0.0f;
+            float base, sum, value = 0.0f, value_top = kNoScore;
             total(row, base, sum);
+            for (u32 r = 0; r < team; ++r) value_top = fmaxf(value_top, peek(cta_ref + row, r));
             for (u32 r = 0; r < team; ++r)
-                value += __uint_as_float(kv_peek(reinterpret_cast<const u32*>(cta_o + x), r)) *
-                         exp2_fast(peek2(cta_ml + row, r).x - base);
-            put_out(a, seg, seg.rt * R + row, channel_of(D, at), sum == 0.0f ? 0.0f : value / sum);
+                value += at_power(peek(cta_o + x, r), peek(cta_ref + row, r) - value_top);
+            put_out(a, seg, seg.rt * R + row, channel_of(D, at),
+                    sum == 0.0f ? 0.0f : at_power(value / sum, value_top - base));
             if (at == 0 && a.lse)
                 a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
         }
@@ -849,7 +1006,8 @@ __device__ __forceinline__ void put_pair(const AttentionArgs& a, u64 at, float x
 // share of the blocks.  All sums run in a fixed order.
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionArgs a, u32 R, u32 slices)
 {
-    __shared__ float row_top[24], row_sum[24], row_inverse[24];  // of the segment at hand
+    // of the segment at hand
+    __shared__ float row_top[24], row_sum[24], row_inverse[24], row_ref[24];
     __shared__ float4 join[kFinishThreads];
     const u32 i = threadIdx.x, lane = i & 31u, warp = i >> 5;
     kv_wait_before();
@@ -872,12 +1030,19 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
         const u32 parts = span.y + 1 - span.x;
         const u64 first = static_cast<u64>(span.x) + index;
         const float2* ml = a.part_ml + first * R;
+        const float* ref = a.part_ref + first * R;
         __syncthreads();
         for (u32 r = warp; r < rows; r += kFinishThreads / 32) {
-            float top = -INFINITY, all = 0.0f;
-            for (u32 s = lane; s < parts; s += 32) top = fmaxf(top, ml[s * R + r].x);
+            float top = -INFINITY, value_top = kNoScore, all = 0.0f;
+            for (u32 s = lane; s < parts; s += 32) {
+                top = fmaxf(top, ml[s * R + r].x);
+                value_top = fmaxf(value_top, ref[s * R + r]);
+            }
 #pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = 16; o; o >>= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                value_top = fmaxf(value_top, __shfl_xor_sync(0xffffffffu, value_top, o));
+            }
             const float base = top == -INFINITY ? 0.0f : top;
             for (u32 s = lane; s < parts; s += 32) all += ml[s * R + r].y * exp2_fast(ml[s * R + r].x - base);
 #pragma unroll
@@ -886,6 +1051,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                 row_top[r] = base;
                 row_sum[r] = all;
                 row_inverse[r] = all == 0.0f ? 0.0f : 1.0f / all;
+                row_ref[r] = value_top;
             }
         }
         __syncthreads();
@@ -899,17 +1065,17 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
             const u32 group = i / pieces;
             for (u32 at = pieces < kFinishThreads ? i % pieces : i; at < pieces; at += kFinishThreads) {
                 const u32 x = piece0 + at, r = x * 4 / D;
-                const float base = row_top[r];
+                const float base = row_ref[r];
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (group < groups || groups == 1) {
 #pragma unroll 8
                     for (u32 s = groups == 1 ? 0 : group; s < parts; s += groups) {
                         const float4 y = part[static_cast<u64>(s) * (R * D / 4) + x];
-                        const float f = exp2_fast(ml[s * R + r].x - base);
-                        v.x += y.x * f;
-                        v.y += y.y * f;
-                        v.z += y.z * f;
-                        v.w += y.w * f;
+                        const float by = ref[s * R + r] - base;
+                        v.x += at_power(y.x, by);
+                        v.y += at_power(y.y, by);
+                        v.z += at_power(y.z, by);
+                        v.w += at_power(y.w, by);
                     }
                 }
                 if (groups > 1) {
@@ -924,16 +1090,17 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
                         v.w += y.w;
                     }
                 }
-                const float inverse = row_inverse[r];
+                const float by = base - row_top[r];
+                auto mean = [&](float x) { return at_power(x * row_inverse[r], by); };
                 // two pairs of neighbouring channels, D / 8 apart
                 const u32 row = rt * R + r, at_row = x * 4 % D, d = channel_of(D, at_row);
                 const u32 tt = a.blocks ? t : row / a.q.group;
                 const u32 qh = h * a.q.group + row % a.q.group;
                 const u64 to = (static_cast<u64>(seq) * a.q.tokens + tt) * a.q.q_heads + qh;
-                put_pair(a, to * D + d, v.x * inverse, v.y * inverse);
-                put_pair(a, to * D + d + D / 8, v.z * inverse, v.w * inverse);
+                put_pair(a, to * D + d, mean(v.x), mean(v.y));
+                put_pair(a, to * D + d + D / 8, mean(v.z), mean(v.w));
                 if (at_row == 0 && a.lse)
-                    a.lse[to] = row_sum[r] == 0.0f ? -INFINITY : (log2f(row_sum[r]) + base) * kLn2;
+                    a.lse[to] = row_sum[r] == 0.0f ? -INFINITY : (log2f(row_sum[r]) + row_top[r]) * kLn2;
             }
         }
         if (!weights) continue;
@@ -971,7 +1138,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
 
 struct Plan {
     u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole, warps, team;
-    u64 segments, part_o, part_ml, span, tile_sums, bytes;
+    u64 segments, part_o, part_ml, part_ref, span, tile_sums, bytes;
 };
 
 Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weights)
@@ -1023,6 +1190,7 @@ Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weight
     };
     p.part_o = take((p.segments + p.workers) * R * v.dim * 4);
     p.part_ml = take((p.segments + p.workers) * R * 8);
+    p.part_ref = take((p.segments + p.workers) * R * 4);
     p.span = take(p.segments * 8);
     p.tile_sums = take(weights ? p.segments * p.tiles * R * 8 : 0);
     p.bytes = at;
@@ -1127,6 +1295,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     u8* w = static_cast<u8*>(args->workspace);
     a.part_o = reinterpret_cast<float*>(w + p.part_o);
     a.part_ml = reinterpret_cast<float2*>(w + p.part_ml);
+    a.part_ref = reinterpret_cast<float*>(w + p.part_ref);
     a.span = reinterpret_cast<uint2*>(w + p.span);
     a.tile_sums = a.weights && !p.whole ? reinterpret_cast<float2*>(w + p.tile_sums) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
