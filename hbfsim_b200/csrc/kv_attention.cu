@@ -43,6 +43,7 @@
 // 40 rows on 8 sequences of 700 to 9001 tokens take 64 us, three passes that
 // are bound by the latency of their instructions (46 % of the slots).
 #include "kv.h"
+#include "kv_plan.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -50,13 +51,11 @@
 namespace hbfb {
 namespace {
 
-constexpr u32 kWarps = 4;
-constexpr u32 kShare = 8;           // tiles of a share at least: two per warp
 // The probabilities of a row stand against a reference of its scores (log2, a whole number), which
 // moves up only when a score is 2^kAbove above it: a tile then costs a vote instead of a maximum over
 // the lanes.  After a move the largest is at 2^kPlace or half of it, so that f16 holds them all and
-// keeps its 11 bits down to 2^-23 of the largest.  For the product with the values they are multiplied by their
-// block's value scale over the greatest that the warp has met.
+// keeps its 11 bits down to 2^-23 of the largest.  For the product with the values they are
+// multiplied by their block's value scale over the greatest that the warp has met.
 constexpr float kAbove = 15.0f, kPlace = 10.0f;
 // That holds for scales within kNear of each other.  Past it a block of large scale and no weight
 // would push the others out of f16's range, so from there on the warp keeps a second reference for
@@ -68,14 +67,6 @@ constexpr float kNear = 1024.0f;
 constexpr float kFarAbove = 85.0f, kFarPlace = 81.0f, kLift = 70.0f;
 constexpr float kNoScore = -3.0e38f;  // reference of a row without a score
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Tiles of a segment that one CTA of so many warps may take whole, at most.  With two row tiles or
-// more the sums of their weights cost CTAs on an SM: 400 segments of 125 tiles and 16 rows took 78
-// us whole and 58 us split.
-constexpr u32 whole_tiles(u32 nt, u32 warps) { return nt == 1 || warps > kWarps ? 128 : 32; }
-// Few longer segments are finished by teams of up to 8 CTAs (a cluster) that join through
-// distributed shared memory: from 64 tiles on, 16 to a CTA at least (38 tiles took 11.0 us by two
-// CTAs and 9.7 us by one), as long as all teams are resident at once.
-constexpr u32 kTeamFrom = 64, kTeamTiles = 16, kTeamPlaces = 128;
 constexpr u32 kFinishThreads = 256; // blocks per CTA of finish_kernel
 
 struct AttentionArgs {
@@ -286,12 +277,6 @@ __device__ __forceinline__ int row_position(const AttentionArgs& a, const Segmen
     return max(s.length - static_cast<int>(a.q.tokens) + static_cast<int>(t), -1);
 }
 
-// Row tiles of 8 rows that a pass takes.  Wide passes widen the cache's values
-// less often but leave fewer warps on an SM: 24 rows of 128 channels in one
-// pass took 45 us where two passes of 16 took 49, 40 rows in three passes of
-// 16 took 63 where two of 24 took 69 (8 sequences of 700 to 9001 tokens, 8
-// heads).  At 256 channels the accumulators leave room for 16 rows.
-constexpr u32 pass_width(u32 eights, u32 dim) { return eights <= 2 || (eights == 3 && dim < 256) ? eights : 2; }
 // Joined values lie as the lanes hold them: channel g D/8 + 2k + e of a row at
 // 16 k + 2 g + e, so that lanes that write or read together meet different
 // banks.  The channel at a place:
@@ -311,11 +296,7 @@ __device__ __forceinline__ void put_out(const AttentionArgs& a, const Segment& s
     else static_cast<__half*>(a.out)[at] = __float2half_rn(y);
 }
 
-// CTAs per SM and the depth of a warp's ring, by registers and about 192 KB of rings.
-constexpr u32 per_sm(u32 dim, u32 nt)
-{
-    return dim == 256 ? 2 : dim == 128 ? (nt == 3 ? 2 : 3) : (nt <= 2 ? 4 : 3);
-}
+// Depth of a warp's ring.
 template <int D>
 constexpr u32 kStages = D == 256 ? 3 : 4;
 // One row tile's queries stay in registers; more are read from shared memory for each tile.
@@ -339,12 +320,6 @@ struct Layout {
     static constexpr u32 bytes = line + 8 * W + sizeof(u64) * 4;
     static constexpr u32 most = whole_sums + whole_tiles(NT, W) * 8 * NT * 8;
 };
-
-// Tiles of each CTA of a team, whole blocks.
-HD constexpr u32 part_of(u32 tiles, u32 team, u32 block_tiles)
-{
-    return (tiles + team * block_tiles - 1) / (team * block_tiles) * block_tiles;
-}
 
 // One segment's tiles [first, end) by one CTA; the partial result goes to `part` (a whole segment:
 // joined with those of its team, in which this CTA is number `part`).
@@ -1136,65 +1111,10 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const AttentionA
     }
 }
 
-struct Plan {
-    u32 nt, lists, rows, row_tiles, units, per_unit, workers, tiles, whole, warps, team;
-    u64 segments, part_o, part_ml, part_ref, span, tile_sums, bytes;
-};
-
-Plan plan_of(const KvView& v, const KvQuery& q, bool lists, u32 top, bool weights)
+Plan plan_of(const KvView& v, const KvQuery& q, const hbfsim_kv_attention_args_v1& g)
 {
-    Plan p{};
-    p.lists = lists ? q.tokens : 1;
-    p.rows = lists ? q.group : q.group * q.tokens;
-    p.nt = pass_width((p.rows + 7) / 8, v.dim);
-    const u32 R = 8 * p.nt;
-    p.row_tiles = (p.rows + R - 1) / R;
-    p.tiles = (lists ? top : q.width) * (v.block / 16);
-    p.units = lists ? q.seqs * q.tokens * v.heads : q.seqs;
-    p.per_unit = lists ? p.row_tiles : v.heads * p.row_tiles;
-    p.segments = static_cast<u64>(p.units) * p.per_unit;
-    // as many CTAs as are resident at once, fewer for little work
-    const u64 most = (p.segments * p.tiles + kShare - 1) / kShare;
-    const u64 resident = static_cast<u64>(per_sm(v.dim, p.nt)) * kv_sm_count();
-    p.workers = static_cast<u32>(std::max<u64>(1, std::min<u64>(most, resident)));
-    // Short segments (by the table's width or the lists' length) are finished where they are
-    // summed: one launch, where the even split takes two and joins.  With an SM for each, they get
-    // CTAs of 8 warps: 64 of 38 tiles (128 channels) take 9.9 us, 12.4 us with 4 warps and 15.8 us
-    // split.  Longer ones get teams of CTAs: 8 of 128 tiles take 10.1 us and 13.2 us split, 32 of
-    // 256 tiles 14.0 and 22.0 us, 8 of 1024 tiles 19.9 and 21.4 us.  The more tiles a CTA has, the
-    // more CTAs there have to be: 64 of 128 tiles take 17.7 us by one CTA each and 21.5 us split.
-    const u32 sms = static_cast<u32>(kv_sm_count());
-    p.warps = p.segments <= sms ? 2 * kWarps : kWarps;
-    p.team = 1;
-    while (p.team < 8 && p.tiles >= kTeamFrom && p.segments * p.team * 2 <= kTeamPlaces &&
-           p.tiles >= p.team * 2 * kTeamTiles)
-        p.team *= 2;
-    const u32 each = part_of(p.tiles, p.team, v.block / 16);
-    // With 4 warps: 400 of 128 tiles take 36.6 us whole and 41.2 us split.  More long ones than are
-    // resident at once should fill their last turn: 1600 lists of 128 tiles take 152 and 169 us,
-    // 512 on 444 places 74 and 64 us (512 of 21 to 63 tiles 32.0 and 36.7 us).
-    const u64 places = (p.segments + resident - 1) / resident * resident;
-    p.whole = each <= whole_tiles(p.nt, p.warps) &&
-              (p.segments <= sms ? each <= p.segments * p.team + 64 : 2 * p.tiles <= p.segments + 64) &&
-              (p.tiles <= 64 || p.segments <= resident || p.segments * 5 >= places * 4) &&
-              (!weights || p.lists * p.row_tiles == 1);
-    if (p.whole) {
-        p.workers = static_cast<u32>(p.segments) * p.team;
-        return p;  // no workspace
-    }
-    u64 at = 0;
-    auto take = [&](u64 bytes) {
-        const u64 here = at;
-        at += kv_round_up(bytes, 256);
-        return here;
-    };
-    p.part_o = take((p.segments + p.workers) * R * v.dim * 4);
-    p.part_ml = take((p.segments + p.workers) * R * 8);
-    p.part_ref = take((p.segments + p.workers) * R * 4);
-    p.span = take(p.segments * 8);
-    p.tile_sums = take(weights ? p.segments * p.tiles * R * 8 : 0);
-    p.bytes = at;
-    return p;
+    return plan_of(PlanCall{q.seqs, q.tokens, v.heads, q.group, v.dim, v.block, q.width, g.top, g.blocks != nullptr,
+                            g.weights != nullptr}, static_cast<u32>(kv_sm_count()));
 }
 
 int check_args(const hbfsim_kv_attention_args_v1* g)
@@ -1258,7 +1178,7 @@ extern "C" uint64_t hbfsim_kv_attention_workspace_v1(const hbfsim_kv_cache_v1* c
     KvQuery q{};
     if (kv_check_cache(cache, v) || kv_check_query(query, v, q) || check_args(args)) return 0;
     if (q.seqs == 0 || q.tokens == 0) return 0;
-    return plan_of(v, q, args->blocks != nullptr, args->top, args->weights != nullptr).bytes;
+    return plan_of(v, q, *args).bytes;
 }
 
 extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
@@ -1270,7 +1190,7 @@ extern "C" int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
     if (const int rc = kv_check_query(query, a.c, a.q)) return rc;
     if (const int rc = check_args(args)) return rc;
     if (a.q.seqs == 0 || a.q.tokens == 0) return HBFSIM_OK;
-    const Plan p = plan_of(a.c, a.q, args->blocks != nullptr, args->top, args->weights != nullptr);
+    const Plan p = plan_of(a.c, a.q, *args);
     if (p.segments > 0x7fffffffull) return HBFSIM_UNSUPPORTED;
     if (!args->out || (p.bytes && !args->workspace) || args->workspace_bytes < p.bytes ||
         !kv_aligned(args->workspace, 16) || !kv_aligned(args->out, 4) ||
