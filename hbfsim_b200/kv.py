@@ -337,13 +337,22 @@ def kv_block_reads(cache: KvCache, table, blocks, counts, base: int):
     listed block and head of its keys and values (2 * block_tokens * head_dim
     bytes, 4 KiB at 16 tokens of 128), in list order.  Page p, head h lies at
     base + (p * kv_heads + h) * block_bytes: the cache's own layout placed at
-    `base` in the simulated address space."""
+    `base` in the simulated address space.  An index that the table does not
+    have, or whose page is not in the pool, is passed over, as the attention
+    does."""
     import torch
-    seqs, tokens, heads, top = blocks.shape
+    _need(blocks.dim() == 4 and table.dim() == 2 and table.shape[0] == blocks.shape[0]
+          and counts.shape == blocks.shape[:3],
+          "blocks: [seqs, tokens, kv_heads, top] with counts and table of the same seqs")
+    heads, top = blocks.shape[2:]
+    width = table.shape[1]
     rank = torch.arange(top, device=blocks.device)
-    listed = rank < counts[..., None]
-    index = torch.where(listed, blocks, 0).long()
-    page = torch.gather(table.long(), 1, index.view(seqs, -1)).view_as(index)
+    listed = (rank < counts[..., None]) & (blocks >= 0) & (blocks < width)
+    if width == 0:  # listed by no one
+        page = torch.zeros_like(blocks, dtype=torch.int64)
+    else:
+        index = torch.where(listed, blocks, 0).long()
+        page = torch.gather(table.long(), 1, index.flatten(1)).view_as(index)
     listed &= (page >= 0) & (page < cache.pages)
     head = torch.arange(heads, device=blocks.device)[:, None]
     address = base + (page * heads + head) * cache.block_bytes
