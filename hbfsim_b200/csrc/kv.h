@@ -527,7 +527,8 @@ __device__ void kv_rank_limit(const KvTeam& team, u32 n, u32 rank, Key lo, Key h
         } else {
             lo += static_cast<Key>(bin) << width;
         }
-        hi = min(hi, static_cast<Key>(lo + ((Key{1} << width) - 1)));
+        const Key last = (Key{1} << width) - 1;  // lo + last may be past the type's range
+        if (hi - lo > last) hi = lo + last;
         if (rank == count) {  // the whole bin
             limit = hi;
             equals = kKvAll;
