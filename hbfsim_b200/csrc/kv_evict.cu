@@ -13,6 +13,8 @@
 // blocks 13 us with a team of 8: a chain of a dozen barriers, not memory.
 #include "kv.h"
 
+#include <algorithm>
+
 namespace hbfb {
 namespace {
 
@@ -129,6 +131,36 @@ __global__ void __launch_bounds__(1024) evict_kernel(const EvictArgs a, u32 team
         for (u32 j = blocks - leave + threadIdx.x; j < blocks; j += blockDim.x) score_out[j] = 0;
 }
 
+struct Memory {
+    std::uintptr_t from, end;
+    Memory(const void* p, u64 bytes) : from(reinterpret_cast<std::uintptr_t>(p)), end(from + bytes) {}
+    bool meets(const Memory& other) const { return from < other.end && other.from < end; }
+};
+
+// Whether an output lies in an input's memory or in another output's: every thread block writes its
+// outputs while others still read.
+bool would_race(const hbfsim_kv_evict_batch_v1& b)
+{
+    const u64 seqs = b.seqs, row = u64{b.width} * 4;
+    const Memory out[] = {{b.score_out, seqs * row * 2}, {b.table_out, seqs * row}, {b.lengths_out, seqs * 4},
+                          {b.freed, seqs * row}, {b.freed_counts, seqs * 4}};
+    const Memory in[] = {{b.score, seqs * row * 2}, {b.weights, seqs * b.kv_heads * row}, {b.lengths, seqs * 4}};
+    // the table's rows, from the first to the last; one by one only where something lies among them
+    const int* last = b.table + static_cast<i64>(seqs - 1) * b.table_stride;
+    const Memory table(std::min(b.table, last), reinterpret_cast<std::uintptr_t>(std::max(b.table, last)) -
+                                                    reinterpret_cast<std::uintptr_t>(std::min(b.table, last)) + row);
+    for (const Memory& o : out) {
+        for (const Memory& i : in)
+            if (o.meets(i)) return true;
+        for (const Memory* p = out; p != &o; ++p)
+            if (o.meets(*p)) return true;
+        if (o.meets(table))
+            for (u64 s = 0; s < seqs; ++s)
+                if (o.meets(Memory(b.table + static_cast<i64>(s) * b.table_stride, row))) return true;
+    }
+    return false;
+}
+
 }  // namespace
 }  // namespace hbfb
 
@@ -150,11 +182,11 @@ extern "C" int hbfsim_kv_evict_v1(const hbfsim_kv_evict_batch_v1* b, void* strea
         (b->width && (!b->score || !b->weights || !b->table || !b->score_out || !b->table_out ||
                       !b->freed)))
         return HBFSIM_INVALID_ARGUMENT;
-    if (b->width && (b->score == b->score_out || b->table == b->table_out))
-        return HBFSIM_INVALID_ARGUMENT;
     if (!kv_aligned(b->score, 8) || !kv_aligned(b->score_out, 8) || !kv_aligned(b->weights, 4) ||
-        !kv_aligned(b->table, 4) || !kv_aligned(b->table_out, 4) || !kv_aligned(b->freed, 4))
+        !kv_aligned(b->table, 4) || !kv_aligned(b->table_out, 4) || !kv_aligned(b->freed, 4) ||
+        !kv_aligned(b->lengths, 4) || !kv_aligned(b->lengths_out, 4) || !kv_aligned(b->freed_counts, 4))
         return HBFSIM_INVALID_ARGUMENT;
+    if (would_race(*b)) return HBFSIM_INVALID_ARGUMENT;
     EvictArgs a{b->score,      b->weights, b->table,        b->table_stride, b->lengths,
                 b->score_out,  b->table_out, b->lengths_out, b->freed,       b->freed_counts,
                 b->kv_heads,   b->width,   b->block_tokens, b->keep,         b->sink,

@@ -176,9 +176,10 @@ int hbfsim_kv_attention_v1(const hbfsim_kv_cache_v1* cache,
  * (sink + recent <= keep, recent >= 1, so that the block being filled
  * stays).  The others close up in order.  Table entries are carried along as
  * they are.
- * Out (not the inputs' memory): score, table (rows of `width`, 0 and -1
- * behind the last block), lengths (less the evicted blocks' tokens), freed
- * (the evicted blocks' table entries in block order, -1 behind), freed_counts. */
+ * Out (in memory apart from the inputs' and from each other's): score, table
+ * (rows of `width`, 0 and -1 behind the last block), lengths (less the evicted
+ * blocks' tokens), freed (the evicted blocks' table entries in block order, -1
+ * behind), freed_counts. */
 typedef struct hbfsim_kv_evict_batch_v1 {
     uint32_t struct_size;
     uint32_t version;

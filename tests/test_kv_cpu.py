@@ -190,3 +190,22 @@ def test_oracle_rounding_matches_the_type():
     assert np.array_equal(ko.E4M3[ko.encode(x)], ko.E4M3[want])
     assert ko.encode(np.array([1e9, -np.inf])).tolist() == [126, 254]
     assert ko.encode(np.array([np.nan])).tolist() == [127]
+
+
+# kv_evict with every array where it has room of its own: 2 sequences of 3 blocks, 2 heads
+APART = dict(score=0x10000, weights=0x20000, table=0x30000, lengths=0x40000, score_out=0x50000,
+             table_out=0x60000, lengths_out=0x70000, freed=0x80000, freed_counts=0x90000)
+
+
+@pytest.mark.parametrize("over", [
+    dict(lengths=0x40002), dict(lengths_out=0x70002), dict(freed_counts=0x90002),  # not of 4 bytes
+    # an output in an input's memory
+    dict(lengths_out=0x40000), dict(lengths_out=0x40004), dict(freed_counts=0x40000),
+    dict(freed=0x30000), dict(table_out=0x30014), dict(score_out=0x10028), dict(score_out=0x0ffd8),
+    dict(table_out=0x20000), dict(freed=0x2002c), dict(score_out=0x30008), dict(table_out=0x10000),
+    dict(lengths_out=0x10000), dict(freed_counts=0x30000),
+    dict(table_stride=100, freed=0x30000 + 400), dict(table_stride=-3, freed=0x30000 - 12),
+    # outputs in each other's
+    dict(lengths_out=0x90004), dict(freed=0x60000), dict(table_out=0x80014), dict(freed=0x50000 + 44)])
+def test_evict_refuses_memory_that_would_race(lib, over):
+    assert lib.hbfsim_kv_evict_v1(ref(evict(**{**APART, **over})), None) == INVALID

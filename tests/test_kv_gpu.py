@@ -829,3 +829,42 @@ def test_example(capsys):
     assert got["evicted_blocks"] == sum(12 + n for n in begun)
     assert got["every_reads"] > 3 * got["listed_reads"]
     assert got["every_us_per_step"] > got["listed_us_per_step"] > 0
+
+
+def test_evict_into_memory_between_the_inputs():
+    """Outputs beside the inputs in one allocation, between the rows of a strided table too."""
+    import ctypes
+    torch = torch_()
+    from hbfsim_b200 import _lib
+    rng = np.random.default_rng(41)
+    seqs, heads, width, keep = 3, 2, 40, 9
+    pool = torch.zeros(1 << 14, dtype=torch.int32, device="cuda")
+    at = dict(table=0, table_out=40, freed=160, lengths=300, lengths_out=303, freed_counts=306, weights=400,
+              score=1000, score_out=1000 + 2 * seqs * width)
+    stride = 4096  # rows of the table, the outputs between the first two
+
+    def put(name, x):
+        x = torch.from_numpy(np.ascontiguousarray(x)).cuda().view(torch.int32).flatten()
+        pool[at[name]:at[name] + x.numel()] = x
+
+    table = rng.permutation(seqs * width).reshape(seqs, width).astype(np.int32)
+    for b in range(seqs):
+        pool[b * stride:b * stride + width] = torch.from_numpy(table[b]).cuda()
+    score = rng.integers(0, 1 << 40, (seqs, width))
+    weights = rng.random((seqs, heads, width)).astype(np.float32)
+    lengths = np.array([40 * 16, 100, 39 * 16 + 1], np.int32)
+    put("score", score)
+    put("weights", weights)
+    put("lengths", lengths)
+    where = {k: pool.data_ptr() + 4 * v for k, v in at.items()}
+    batch = _lib.KvEvictBatchV1(struct_size=ctypes.sizeof(_lib.KvEvictBatchV1), version=1, seqs=seqs, kv_heads=heads,
+                                width=width, block_tokens=16, keep=keep, sink=1, recent=1, decay=4,
+                                table_stride=stride, **where)
+    torch.cuda.synchronize()
+    assert _lib.load().hbfsim_kv_evict_v1(ctypes.byref(batch), None) == 0
+    torch.cuda.synchronize()
+    want = ko.evict(score, weights, table, lengths, keep, 16, 1, 1, 4)
+    got = pool.cpu().numpy()
+    for name, x in zip(("score_out", "table_out", "lengths_out", "freed", "freed_counts"), want):
+        flat = np.ascontiguousarray(x).view(np.int32).ravel()
+        assert np.array_equal(got[at[name]:at[name] + flat.size], flat), name
