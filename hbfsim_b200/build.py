@@ -59,11 +59,17 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         made = Path(tmp) / LIB.name
         _run([*flags, "-shared", "-cudart", "static", "-o", str(made), *map(str, objects),
               "-Xlinker", f"--version-script={script}"], verbose)
-        # in place at once: a process that has the old file loaded keeps it
-        staged = LIB.with_suffix(".so.new")
-        shutil.copyfile(made, staged)
-        staged.chmod(0o755)
-        os.replace(staged, LIB)
+        # in place at once: a process that has the old file loaded keeps it; under a name of its
+        # own first: two builds at once do not write one file
+        handle, staged = tempfile.mkstemp(prefix="." + LIB.stem + ".", suffix=".so", dir=LIB.parent)
+        os.close(handle)
+        try:
+            shutil.copyfile(made, staged)
+            os.chmod(staged, 0o755)
+            os.replace(staged, LIB)
+        except BaseException:
+            os.unlink(staged)
+            raise
     return LIB
 
 
