@@ -59,6 +59,10 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _counts(names: str, *values: int) -> None:
+    _need(min(values) >= 0 and max(values) < 1 << 32, names + " are counts of 32 bits")
+
+
 class KvCache:
     """The cache's three tensors (a view of them; nothing is copied):
     data (float8_e4m3fn [pages, kv_heads, 2, block_tokens, head_dim]), scale
@@ -230,7 +234,8 @@ def kv_select(cache: KvCache, q, table, lengths, top: int, sink: int = 1, recent
     if not _here(cache.index, stream):
         with _On(cache.index, stream):
             return kv_select(cache, q, table, lengths, top, sink, recent)
-    _need(top >= 0 and sink >= 0 and recent >= 0, "top, sink and recent are counts")
+    _counts("top, sink and recent", top, sink, recent)
+    _need(top <= 1 << 24, "a list has room for 2^24 blocks at most")  # as many as a table
     query, seqs, tokens, _, _ = _query(cache, q, table, lengths)
     lib = _lib.load()
     blocks = table.new_empty((seqs, tokens, cache.kv_heads, top))
@@ -284,6 +289,8 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
         mass_at = mass.data_ptr()
     if scale is None:
         scale = cache.head_dim ** -0.5
+    else:
+        _need(not abs(scale) > 3.0e38, "the scale has to fit 32 bits")
     head = (_ATTENTION.size, 1, scale, top, blocks_at, counts_at, out.data_ptr(), lse.data_ptr(),
             mass_at)
     size = lib.hbfsim_kv_attention_workspace_v1(cache._packed, query, _ATTENTION.pack(*head, 0, 0))
@@ -316,8 +323,7 @@ def kv_evict(score, weights, table, lengths, keep: int, block_tokens: int = 16, 
           and weights.shape[2] == width and weights.is_contiguous()
           and weights.get_device() == index,
           "weights: float32 [seqs, kv_heads, width], contiguous")
-    _need(min(keep, block_tokens, sink, recent, decay) >= 0,
-          "keep, block_tokens, sink, recent and decay are counts")
+    _counts("keep, block_tokens, sink, recent and decay", keep, block_tokens, sink, recent, decay)
     plain, like = torch.contiguous_format, torch.empty_like
     new_score = like(score)
     new_table, freed = like(table, memory_format=plain), like(table, memory_format=plain)

@@ -868,3 +868,31 @@ def test_evict_into_memory_between_the_inputs():
     for name, x in zip(("score_out", "table_out", "lengths_out", "freed", "freed_counts"), want):
         flat = np.ascontiguousarray(x).view(np.int32).ravel()
         assert np.array_equal(got[at[name]:at[name] + flat.size], flat), name
+
+
+@pytest.mark.parametrize("name", ["top", "sink", "recent", "keep", "block_tokens", "esink", "erecent", "decay"])
+@pytest.mark.parametrize("value", [-1, 1 << 32, (1 << 32) + 1, 1 << 70])
+def test_counts_that_do_not_fit_are_refused(name, value):
+    """A count past 32 bits is not taken for what remains of it."""
+    torch = torch_()
+    from hbfsim_b200 import KvCache, kv_evict, kv_select
+    table = torch.zeros((1, 3), dtype=torch.int32, device="cuda")
+    if name in ("top", "sink", "recent"):
+        q = torch.ones((1, 1, 2, 64), dtype=torch.float16, device="cuda")
+        with pytest.raises(ValueError):
+            kv_select(KvCache.empty(2, 2, 64), q, table, int32([40]), **{"top": 3, name: value})
+    else:
+        score = torch.zeros((1, 3), dtype=torch.int64, device="cuda")
+        with pytest.raises(ValueError):
+            kv_evict(score, torch.zeros((1, 1, 3), device="cuda"), table, int32([40]),
+                     **{"keep": 2, name.lstrip("e"): value})
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, float("inf"), 10 ** 400])
+def test_scales_that_do_not_fit_are_refused(scale):
+    torch = torch_()
+    from hbfsim_b200 import HbfsimError, KvCache, kv_attention
+    q = torch.ones((1, 1, 2, 64), dtype=torch.float16, device="cuda")
+    with pytest.raises((ValueError, HbfsimError)):
+        kv_attention(KvCache.empty(2, 2, 64), q, torch.zeros((1, 3), dtype=torch.int32, device="cuda"), int32([40]),
+                     scale=scale)
