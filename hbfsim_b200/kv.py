@@ -10,7 +10,9 @@ One decode step of a layer is
     reads = kv_block_reads(cache, table, pick.blocks, pick.counts, base)  # for Context.submit
 
 kv_attention without lists reads every block.  Arguments that do not fit
-raise ValueError here, or HbfsimError from the C ABI.  Calls are asynchronous
+raise ValueError here, or HbfsimError from the C ABI; so do keys, values and
+queries that ask for a gradient, since there is no backward pass (inside
+torch.no_grad() they are taken as they are).  Calls are asynchronous
 on `stream` (default: torch's current stream); outputs and workspace belong
 to that stream.
 """
@@ -61,6 +63,12 @@ def _need(ok: bool, what: str) -> None:
 
 def _counts(names: str, *values: int) -> None:
     _need(min(values) >= 0 and max(values) < 1 << 32, names + " are counts of 32 bits")
+
+
+def _no_gradient(*tensors) -> None:
+    import torch
+    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)),
+          "no gradient passes through the cache: detach the tensors or call under torch.no_grad()")
 
 
 class KvCache:
@@ -183,6 +191,7 @@ def kv_append(cache: KvCache, k, v, table, start, offsets=None, stream=None) -> 
           and shape[-2] == cache.kv_heads and shape[-1] == cache.head_dim,
           "k and v: one shape and type, [seqs, n, kv_heads, head_dim] or with offsets "
           "[tokens, kv_heads, head_dim], on the cache's device")
+    _no_gradient(k, v)
     if offsets is None:
         _need(shape[0] == seqs, "k: as many sequences as the table")
         k, v = k.flatten(0, 1), v.flatten(0, 1)  # a copy where one stride cannot serve both axes
@@ -263,6 +272,7 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
         with _On(cache.index, stream):
             return kv_attention(cache, q, table, lengths, scale, blocks, counts, weights)
     import torch
+    _no_gradient(q)
     query, seqs, tokens, q_heads, width = _query(cache, q, table, lengths)
     top = blocks_at = counts_at = 0
     if blocks is not None:

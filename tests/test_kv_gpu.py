@@ -896,3 +896,30 @@ def test_scales_that_do_not_fit_are_refused(scale):
     with pytest.raises((ValueError, HbfsimError)):
         kv_attention(KvCache.empty(2, 2, 64), q, torch.zeros((1, 3), dtype=torch.int32, device="cuda"), int32([40]),
                      scale=scale)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+def test_gradients_are_refused_not_dropped(which):
+    """No operator here has a backward pass: a tensor that asks for one raises, unless gradients
+    are off."""
+    torch = torch_()
+    from hbfsim_b200 import KvCache, kv_append, kv_attention, kv_select
+    gpu = KvCache.empty(4, 2, 64)
+    table = torch.zeros((1, 3), dtype=torch.int32, device="cuda")
+    make = lambda heads, name: torch.ones((1, 1, heads, 64), dtype=torch.float16, device="cuda",  # noqa: E731
+                                          requires_grad=which == name)
+    q, k, v = make(4, "q"), make(2, "k"), make(2, "v")
+
+    def call():
+        kv_append(gpu, k, v, table, int32([0]))
+        return kv_attention(gpu, q * 1, table, int32([1]))
+
+    with pytest.raises(ValueError, match="gradient"):
+        call()
+    kv_select(gpu, q, table, int32([1]), top=2)  # block lists have no gradient
+    with torch.no_grad():
+        want = call()
+    with torch.inference_mode():
+        assert torch.equal(call().out, want.out)
+    q, k, v = q.detach(), k.detach(), v.detach()
+    assert torch.equal(call().out, want.out)
