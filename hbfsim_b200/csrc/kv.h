@@ -92,15 +92,22 @@ inline int kv_check_query(const hbfsim_kv_query_v1* q, const KvView& v, KvQuery&
     return HBFSIM_OK;
 }
 
+// Whether a runtime call succeeded.  Calls report their own status and leave no error behind for
+// the next one.
+inline bool kv_ok(cudaError_t status)
+{
+    if (status != cudaSuccess) cudaGetLastError();
+    return status == cudaSuccess;
+}
+
 inline int kv_sm_count()
 {
     static std::atomic<int> counts[64];  // by device; the value does not change
     int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || device > 63) return 148;
+    if (!kv_ok(cudaGetDevice(&device)) || device > 63) return 148;
     int n = counts[device].load(std::memory_order_relaxed);
     if (n == 0) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0)
-            n = 148;
+        if (!kv_ok(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device)) || n <= 0) return 148;
         counts[device].store(n, std::memory_order_relaxed);
     }
     return n;
@@ -113,11 +120,11 @@ template <typename Kernel>
 inline bool kv_allow_smem(Kernel* kernel, u32 bytes, std::atomic<u64>& seen)
 {
     int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess) return false;
+    if (!kv_ok(cudaGetDevice(&device))) return false;
     const u64 bit = device < 64 ? u64{1} << device : 0;
     if (seen.load(std::memory_order_acquire) & bit) return true;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(bytes)) != cudaSuccess)
+    if (!kv_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(bytes))))
         return false;
     seen.fetch_or(bit, std::memory_order_release);
     return true;
@@ -166,7 +173,7 @@ inline bool kv_launch(void (*kernel)(Params...), dim3 grid, u32 threads, cudaStr
         attributes[config.numAttrs].val.clusterDim.y = 1;
         attributes[config.numAttrs++].val.clusterDim.z = 1;
     }
-    return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess;
+    return kv_ok(cudaLaunchKernelEx(&config, kernel, args...));
 }
 
 __device__ __forceinline__ void kv_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

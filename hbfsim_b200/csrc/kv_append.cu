@@ -410,13 +410,13 @@ int launch(const AppendArgs& a, cudaStream_t s)
     const dim3 grid((a.tokens + a.chunk - 1) / a.chunk, (a.c.heads * 2 + kAppendWarps - 1) / kAppendWarps);
     auto run = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
-        if (a.wide) append_kernel<T, D, true><<<grid, kAppendWarps * 32, 0, s>>>(a);
-        else append_kernel<T, D, false><<<grid, kAppendWarps * 32, 0, s>>>(a);
+        return kv_launch(a.wide ? append_kernel<T, D, true> : append_kernel<T, D, false>, grid, kAppendWarps * 32, s,
+                         0, 1, false, a);
     };
-    if (a.c.dim == 64) run(std::integral_constant<int, 64>{});
-    else if (a.c.dim == 128) run(std::integral_constant<int, 128>{});
-    else run(std::integral_constant<int, 256>{});
-    return cudaGetLastError() == cudaSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    const bool ok = a.c.dim == 64    ? run(std::integral_constant<int, 64>{})
+                    : a.c.dim == 128 ? run(std::integral_constant<int, 128>{})
+                                     : run(std::integral_constant<int, 256>{});
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
 }  // namespace

@@ -1138,9 +1138,7 @@ bool launch_attention(const AttentionArgs& a, cudaStream_t s)
     if (!kv_allow_smem(kernel, kWhole ? L::most : L::bytes, seen)) return false;
     const u32 sums = kWhole && a.weights ? part_of(a.tiles, a.team, a.c.block / 16) * 8 * NT * 8 : 0;
     const u32 smem = std::max(L::bytes, L::whole_sums + sums);
-    if (kWhole && a.team > 1) return kv_launch(kernel, dim3(a.workers), W * 32, s, smem, a.team, false, a);
-    kernel<<<a.workers, W * 32, smem, s>>>(a);
-    return cudaGetLastError() == cudaSuccess;
+    return kv_launch(kernel, dim3(a.workers), W * 32, s, smem, kWhole ? a.team : 1, false, a);
 }
 
 template <int D, int NT>

@@ -507,10 +507,10 @@ int launch(const SelectArgs& a, cudaStream_t s)
     const u32 rows = a.q.seqs * a.q.tokens * a.c.heads;
     bool ok = true;
     if (a.q.width) {
-        query_kernel<D><<<(rows + kQueryWarps - 1) / kQueryWarps, kQueryWarps * 32, 0, s>>>(a);
+        ok = kv_launch(query_kernel<D>, dim3((rows + kQueryWarps - 1) / kQueryWarps), kQueryWarps * 32, s, 0, 1, false, a);
         const u64 most = (static_cast<u64>(a.q.seqs) * a.q.width + kScoreShare - 1) / kScoreShare;
         const u32 grid = static_cast<u32>(std::min<u64>(most, static_cast<u64>(score_per_sm(D)) * kv_sm_count()));
-        ok = kv_launch(score_kernel<D>, dim3(grid), kScoreWarps * 32, s, kScoreSmem<D>, 1, true, a);
+        ok = ok && kv_launch(score_kernel<D>, dim3(grid), kScoreWarps * 32, s, kScoreSmem<D>, 1, true, a);
     }
     if (a.q.width <= kShortRow) {
         // Keys per lane against warps per barrier: 16 x 4 took 41.0 us for 512 rows of up to 2048
@@ -521,8 +521,8 @@ int launch(const SelectArgs& a, cudaStream_t s)
         if (a.q.width > 2048) kernel = short_list_kernel<16, 8>, warps = 16;
         if (a.q.width > 4096) kernel = short_list_kernel<32, 8>, warps = 32;
         if (a.q.width > 8192) kernel = short_list_kernel<32, 16>, warps = 32;
-        ok = kv_launch(kernel, dim3(rows), warps * 32, s, 0, 1, true, a) && ok;
-        return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+        ok = ok && kv_launch(kernel, dim3(rows), warps * 32, s, 0, 1, true, a);
+        return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
     }
     static std::atomic<u64> seen_list{0};
     if (!kv_allow_smem(list_kernel, kHeldKeys * 4, seen_list)) return HBFSIM_CUDA_ERROR;
@@ -534,9 +534,9 @@ int launch(const SelectArgs& a, cudaStream_t s)
     // many rows: small CTAs, several to an SM
     u32 threads = kv_team_threads(slice);
     if (rows > 2 * static_cast<u32>(kv_sm_count())) threads = std::min(threads, 256u);
-    ok = kv_launch(list_kernel, dim3(rows * team), threads, s, slice <= kHeldKeys ? slice * 4 : 0, team, true, a,
-                   team, slice) && ok;
-    return cudaGetLastError() == cudaSuccess && ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+    ok = ok && kv_launch(list_kernel, dim3(rows * team), threads, s, slice <= kHeldKeys ? slice * 4 : 0, team, true, a,
+                         team, slice);
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
 }  // namespace

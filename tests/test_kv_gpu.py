@@ -923,3 +923,46 @@ def test_gradients_are_refused_not_dropped(which):
         assert torch.equal(call().out, want.out)
     q, k, v = q.detach(), k.detach(), v.detach()
     assert torch.equal(call().out, want.out)
+
+
+STALE_ERROR = """
+import ctypes
+import torch
+from hbfsim_b200 import HbfsimError, KvCache, kv_append, kv_evict
+
+gpu = KvCache.empty(4, 2, 64)
+table = torch.zeros((1, 3), dtype=torch.int32, device="cuda")
+lengths = torch.tensor([20], dtype=torch.int32, device="cuda")
+k = torch.ones((1, 1, 2, 64), dtype=torch.float16, device="cuda")
+score, weights = torch.zeros((1, 3), dtype=torch.int64, device="cuda"), torch.zeros((1, 2, 3), device="cuda")
+kv_append(gpu, k, k, table, lengths)
+kv_evict(score, weights, table, lengths, keep=2)
+torch.cuda.synchronize()
+runtime = ctypes.CDLL("libcudart.so.12")  # the one that torch has loaded
+handle = ctypes.c_void_p()
+assert runtime.cudaStreamCreate(ctypes.byref(handle)) == 0  # ordered with the legacy stream
+assert runtime.cudaStreamBeginCapture(handle, 0) == 0
+# a launch into the legacy stream is an error as long as the capture lasts, and ends it
+refused = False
+try:
+    kv_evict(score, weights, table, lengths, keep=2)
+except HbfsimError:
+    refused = True
+graph = ctypes.c_void_p()
+assert runtime.cudaStreamEndCapture(handle, ctypes.byref(graph)) != 0 and refused
+runtime.cudaGetLastError()
+kv_append(gpu, k, k, table, lengths)  # its launch succeeds: no error of the call before
+torch.cuda.synchronize()
+print("fine")
+"""
+
+
+def test_an_error_is_reported_once():
+    """A launch that failed does not make the next call fail."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+    run = subprocess.run([sys.executable, "-c", STALE_ERROR], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parent.parent, env=dict(os.environ))
+    assert run.returncode == 0 and "fine" in run.stdout, run.stderr[-2000:]
