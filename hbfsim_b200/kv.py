@@ -37,6 +37,9 @@ _ATTENTION = struct.Struct("<2IfI7Q")
 _EVICT = struct.Struct("<10I3Qq6Q")
 
 
+_NO_GRADIENT = "no gradient passes through the cache: detach the tensors or call under torch.no_grad()"
+
+
 class KvAttention(NamedTuple):
     out: object
     lse: object
@@ -59,16 +62,6 @@ class KvEviction(NamedTuple):
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
-
-
-def _counts(names: str, *values: int) -> None:
-    _need(min(values) >= 0 and max(values) < 1 << 32, names + " are counts of 32 bits")
-
-
-def _no_gradient(*tensors) -> None:
-    import torch
-    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)),
-          "no gradient passes through the cache: detach the tensors or call under torch.no_grad()")
 
 
 class KvCache:
@@ -191,7 +184,7 @@ def kv_append(cache: KvCache, k, v, table, start, offsets=None, stream=None) -> 
           and shape[-2] == cache.kv_heads and shape[-1] == cache.head_dim,
           "k and v: one shape and type, [seqs, n, kv_heads, head_dim] or with offsets "
           "[tokens, kv_heads, head_dim], on the cache's device")
-    _no_gradient(k, v)
+    _need(not (k.requires_grad or v.requires_grad) or not torch.is_grad_enabled(), _NO_GRADIENT)
     if offsets is None:
         _need(shape[0] == seqs, "k: as many sequences as the table")
         k, v = k.flatten(0, 1), v.flatten(0, 1)  # a copy where one stride cannot serve both axes
@@ -243,7 +236,7 @@ def kv_select(cache: KvCache, q, table, lengths, top: int, sink: int = 1, recent
     if not _here(cache.index, stream):
         with _On(cache.index, stream):
             return kv_select(cache, q, table, lengths, top, sink, recent)
-    _counts("top, sink and recent", top, sink, recent)
+    _need(not (top | sink | recent) >> 32, "top, sink and recent are counts of 32 bits")
     _need(top <= 1 << 24, "a list has room for 2^24 blocks at most")  # as many as a table
     query, seqs, tokens, _, _ = _query(cache, q, table, lengths)
     lib = _lib.load()
@@ -272,7 +265,7 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
         with _On(cache.index, stream):
             return kv_attention(cache, q, table, lengths, scale, blocks, counts, weights)
     import torch
-    _no_gradient(q)
+    _need(not q.requires_grad or not torch.is_grad_enabled(), _NO_GRADIENT)
     query, seqs, tokens, q_heads, width = _query(cache, q, table, lengths)
     top = blocks_at = counts_at = 0
     if blocks is not None:
@@ -333,7 +326,8 @@ def kv_evict(score, weights, table, lengths, keep: int, block_tokens: int = 16, 
           and weights.shape[2] == width and weights.is_contiguous()
           and weights.get_device() == index,
           "weights: float32 [seqs, kv_heads, width], contiguous")
-    _counts("keep, block_tokens, sink, recent and decay", keep, block_tokens, sink, recent, decay)
+    _need(not (keep | block_tokens | sink | recent | decay) >> 32,
+          "keep, block_tokens, sink, recent and decay are counts of 32 bits")
     plain, like = torch.contiguous_format, torch.empty_like
     new_score = like(score)
     new_table, freed = like(table, memory_format=plain), like(table, memory_format=plain)
