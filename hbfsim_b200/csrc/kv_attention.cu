@@ -18,8 +18,8 @@
 // Scores, the running maximum, sums and the output accumulate in fp32.  The
 // probabilities, times the value scale, are rounded to f16 for the second
 // product only: 2^-11 relative, no more than the output type's own rounding,
-// down to 2^-23 of the row's largest (2^-13 where the scales differ by
-// kNear); what is smaller loses 2^-34 (2^-24) of the largest.  Where scales
+// down to 2^-24 of the row's largest (2^-14 where the scales differ by
+// kNear); what is smaller loses 2^-35 (2^-25) of the largest.  Where scales
 // differ by more, the product takes bf16 pairs (2^-17 relative).  The sums and
 // the block weights use the probabilities unrounded.
 //
@@ -51,15 +51,16 @@
 namespace hbfb {
 namespace {
 
-// The probabilities of a row stand against a reference of its scores (log2, a whole number), which
-// moves up only when a score is 2^kAbove above it: a tile then costs a vote instead of a maximum over
-// the lanes.  After a move the largest is at 2^kPlace or half of it, so that f16 holds them all and
-// keeps its 11 bits down to 2^-23 of the largest.  For the product with the values they are
-// multiplied by their block's value scale over the greatest that the warp has met.
+// The probabilities of a row stand against a reference of its scores (log2), which moves up only when
+// a score is 2^kAbove above it: a tile then costs a vote instead of a maximum over the lanes.  After a
+// move the largest is 2^kPlace, which f16 holds exactly (it may be nearly all of the row), and f16
+// keeps its 11 bits down to 2^-24 of it.  For the product with the values they are multiplied by
+// their block's value scale over the greatest that the warp has met.
 constexpr float kAbove = 15.0f, kPlace = 10.0f;
 // That holds for scales within kNear of each other.  Past it a block of large scale and no weight
 // would push the others out of f16's range, so from there on the warp keeps a second reference for
-// each row, of scores plus the logarithm of their value scale, which what really counts sets, and
+// each row, of scores plus the logarithm of their value scale, a whole number that only what really
+// counts moves up, and
 // takes pairs of bf16 (16 bits, fp32's range) in twice the products.  They lie 2^kLift higher: up to
 // 2^kFarAbove, which times 448 times 2^31 tokens is still a number, and down to 2^-126, so that not
 // even values that are all 0 in a block of large scale and weight hide the others.
@@ -174,8 +175,7 @@ __device__ __forceinline__ float inverse_power(float x)
 // Exponent of a power of two.
 __device__ __forceinline__ float exponent_of(float x) { return static_cast<float>((__float_as_int(x) >> 23 & 0xff) - 127); }
 
-// x * 2^by in two steps (by: a whole number): the power may be past fp32's range where the result
-// is not.
+// x * 2^by in two steps: the power may be past fp32's range where the result is not.
 __device__ __forceinline__ float at_power(float x, float by)
 {
     const float half = rintf(0.5f * by);
@@ -626,7 +626,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1)
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-                    const float now = fmaxf(m[nt][i], ceilf(most) - kPlace);
+                    const float now = fmaxf(m[nt][i], most - kPlace);
                     const float shrink = exp2_fast(m[nt][i] - now);
                     l[nt][i] *= shrink;
                     m[nt][i] = now;
@@ -771,12 +771,19 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             done = consume(std::false_type{}, std::false_type{}, tile, noted.x, key_scale, new_scale, tile_out);
         if (!done) break;
     }
-    // the references of the rows' values, lifted
+    // the references of the rows' values, whole numbers from here on, lifted
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) ref[nt][x] = m[nt][x] + (exponent_of(value_scale) - kLift);
-    multiply(kv_power(static_cast<int>(kLift)));
+        for (int x = 0; x < 2; ++x) {
+            const float up = ceilf(m[nt][x]), by = exp2_fast(m[nt][x] - up + kLift);
+            ref[nt][x] = up + (exponent_of(value_scale) - kLift);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                o[nt][k][x] *= by;
+                o[nt][k][2 + x] *= by;
+            }
+        }
     for (bool waited = true; i < turns; next(), waited = false) {
         if (!waited) wait();
         const int4 noted = note[stage];

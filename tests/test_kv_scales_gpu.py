@@ -6,9 +6,9 @@ largest value in view: the probabilities keep a relative precision of 2^-11,
 so an output is off by that share of its mass (softmax mean of |values|), by
 2 d + 2^-20 from the scores and the exponentials (d = 2^-19 * reach) and by
 the output type's half unit.  Probabilities may be held in f16 among blocks
-whose scales are within 2^10 of each other, the largest at 2^9 or more, so
-that each is off by 2^-34 of the largest probability times scale among those
-of one size of scale; half of that is asked, tokens * 2^-35 * 448 * largest.
+whose scales are within 2^10 of each other, the largest at 2^10 or more, so
+that each is off by 2^-35 of the largest probability times scale among those
+of one size of scale: tokens * 2^-35 * 448 * largest in all.
 """
 import numpy as np
 import pytest
@@ -144,3 +144,26 @@ def test_values_near_the_largest():
         table = make_table(rng, [blocks * block], block, blocks, extra=extra)
         q = torch.from_numpy(0.1 * rng.standard_normal((1, 1, 4, dim))).to(torch.bfloat16).cuda()
         attend_and_check(cache, q, table, blocks * block, np.array([], int), split=split)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,extra,seqs,split", [(64, 0, 40, False), (128, 90, 4, False), (256, 10, 4, False),
+                                                  (64, 20000, 40, True), (128, 20000, 40, True)])
+def test_a_row_of_one_token_is_its_value(dim, extra, seqs, split, kind):
+    """The one probability is 1 whatever the score: the output is the stored value, bit for bit."""
+    torch = torch_()
+    from hbfsim_b200 import kv_attention
+    rng = np.random.default_rng(dim + extra)
+    block, heads, group = 16, 2, 4
+    cache = random_cache(rng, seqs, heads, block, dim)
+    cache["scale"][:, :, 1] = 2.0 ** rng.integers(-9, 3, (seqs, heads))
+    table = make_table(rng, [1] * seqs, block, seqs, extra=extra)
+    q = torch.from_numpy(3 * rng.standard_normal((seqs, 1, heads * group, dim))).to(type_of(kind)).cuda()
+    gpu, tab, lens = to_gpu(cache), int32(table), int32([1] * seqs)
+    assert splits(gpu, q, tab, lens, None, True) == split, "not the form that is meant"
+    got = kv_attention(gpu, q, tab, lens, weights=True)
+    value = ko.E4M3[cache["data"][table[:, 0], :, 1, 0]] * cache["scale"][table[:, 0], :, 1][..., None]
+    want = np.repeat(value, group, 1)[:, None]
+    assert np.array_equal(got.out.double().cpu().numpy(), want)
+    assert np.abs(got.weights[:, :, 0].double().cpu().numpy() - group).max() <= 2.0 ** -18
+    assert not got.weights[:, :, 1:].any()
