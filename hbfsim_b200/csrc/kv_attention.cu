@@ -831,6 +831,21 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         const float half = rintf(0.5f * by);
         return make_float2(exp2_fast(half), exp2_fast(by - half));
     };
+    // what the output of a whole segment's row and the weights of its blocks need
+    auto finish_row = [&](u32 row, float base, float sum, float value_top, bool puts) {
+        factors[row] = base;  // the queries' factors and ends are not needed any more
+        inverses[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        row_power[row] = steps(value_top - base);
+        if (puts && row < rows && a.lse)
+            a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
+    };
+    auto put_value = [&](u32 x, float value) {
+        const u32 row = x / D;
+        if (row >= rows) return;
+        const float inverse = inverses[row];  // 0: the row sees nothing
+        const float2 f = row_power[row];
+        put_out(a, seg, seg.rt * R + row, channel_of(D, x % D), inverse == 0.0f ? 0.0f : value * inverse * f.x * f.y);
+    };
     if (threadIdx.x < W * R) {
         const u32 row = threadIdx.x % R;
         float value_top = kNoScore;
@@ -851,11 +866,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
                 cta_ml[row] = make_float2(top, sum);
                 cta_ref[row] = value_top;
             } else {
-                factors[row] = base;  // the queries' factors and ends are not needed any more
-                inverses[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                row_power[row] = steps(value_top - base);
-                if (row < rows && a.lse)
-                    a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
+                finish_row(row, base, sum, value_top, true);
             }
         }
     }
@@ -872,10 +883,8 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
             a.part_o[part * R * D + x] = value;
         } else if (team > 1) {
             cta_o[x] = value;
-        } else if (row < rows) {
-            const float inverse = inverses[row];  // 0: the row sees nothing
-            const float2 f = row_power[row];
-            put_out(a, seg, seg.rt * R + row, channel_of(D, at), inverse == 0.0f ? 0.0f : value * inverse * f.x * f.y);
+        } else {
+            put_value(x, value);
         }
     }
     float* weights = nullptr;
@@ -885,37 +894,34 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         for (u32 j = from + rank * blockDim.x + threadIdx.x; j < a.q.width; j += team * blockDim.x) weights[j] = 0.0f;
     }
     if (team > 1) {
-        // join the CTAs, each a run of the values: their sums at the team's maximum
+        // join the CTAs, each a run of the values, as the warps were joined
         kv_team_sync(KvTeam{rank, team});
-        auto total = [&](u32 row, float& base, float& sum) {
-            float top = -INFINITY;
-            for (u32 r = 0; r < team; ++r) top = fmaxf(top, peek2(cta_ml + row, r).x);
-            base = top == -INFINITY ? 0.0f : top;
-            sum = 0.0f;
-            for (u32 r = 0; r < team; ++r) {
-                const float2 its = peek2(cta_ml + row, r);
-                sum += its.y * exp2_fast(its.x - base);
+        if (threadIdx.x < team * R) {
+            const u32 row = threadIdx.x % R;
+            float value_top = kNoScore;
+            for (u32 r = 0; r < team; ++r) value_top = fmaxf(value_top, peek(cta_ref + row, r));
+            join_factor[threadIdx.x] = steps(peek(cta_ref + row, threadIdx.x / R) - value_top);
+            if (threadIdx.x < R) {
+                float top = -INFINITY, sum = 0.0f;
+                for (u32 r = 0; r < team; ++r) top = fmaxf(top, peek2(cta_ml + row, r).x);
+                const float base = top == -INFINITY ? 0.0f : top;
+                for (u32 r = 0; r < team; ++r) {
+                    const float2 its = peek2(cta_ml + row, r);
+                    sum += its.y * exp2_fast(its.x - base);
+                }
+                finish_row(row, base, sum, value_top, rank == 0);
             }
-        };
+        }
+        __syncthreads();
         const u32 run = R * D / team;
         for (u32 x = rank * run + threadIdx.x; x < (rank + 1) * run; x += blockDim.x) {
-            const u32 row = x / D, at = x % D;
-            if (row >= rows) continue;
-            float base, sum, value = 0.0f, value_top = kNoScore;
-            total(row, base, sum);
-            for (u32 r = 0; r < team; ++r) value_top = fmaxf(value_top, peek(cta_ref + row, r));
-            for (u32 r = 0; r < team; ++r)
-                value += at_power(peek(cta_o + x, r), peek(cta_ref + row, r) - value_top);
-            put_out(a, seg, seg.rt * R + row, channel_of(D, at),
-                    sum == 0.0f ? 0.0f : at_power(value / sum, value_top - base));
-            if (at == 0 && a.lse)
-                a.lse[out_row(a, seg, seg.rt * R + row)] = sum == 0.0f ? -INFINITY : (log2f(sum) + base) * kLn2;
-        }
-        if (weights && threadIdx.x < rows) {
-            float base, sum;
-            total(threadIdx.x, base, sum);
-            factors[threadIdx.x] = base;
-            inverses[threadIdx.x] = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const u32 row = x / D;
+            float value = 0.0f;
+            for (u32 r = 0; r < team; ++r) {
+                const float2 f = join_factor[r * R + row];
+                value += peek(cta_o + x, r) * f.x * f.y;
+            }
+            put_value(x, value);
         }
     }
     __syncthreads();  // before the next segment's copies
