@@ -10,9 +10,10 @@
 // power of two away from the input, so the only rounding is the one to e4m3.
 //
 // Prompts of 31,668 tokens in all (8 heads of 128 channels) take 42 us: 199 MB
-// of input and blocks at 4.7 TB/s, 73 % of a copy's rate, with half of the
-// issue slots taken (9 instructions a value) at 24 warps an SM.  A step's 64
-// tokens take 4.2 us and one token 3.2 us, a launch and one chain of reads
+// of input and blocks at 4.7 TB/s, 73 % of a copy's rate.  Nothing is full (53 %
+// of the issue slots, 24 warps an SM): a warp loads 16 rows, converts and
+// stores them with no other load under way, so latency bounds it.  A step's 64
+// tokens take 4.2 us and one token 3.3 us, a launch and one chain of reads
 // (start, table, the block's scale, its values).
 #include "kv.h"
 

@@ -31,15 +31,15 @@
 // through shared memory and leave one partial result per segment met;
 // finish_kernel joins the partials of a segment and turns the tiles' sums
 // into block weights.  Short segments have a CTA each, of 8 warps if it has an
-// SM to itself, and need neither (one of 301 tokens takes 6.7 us); few that
+// SM to itself, and need neither (one of 301 tokens takes 7.0 us); few that
 // are longer have a team of CTAs each.
 //
 // One decode step of 64 sequences of 1024 to 32768 tokens, 8 heads of 128
-// channels with 4 rows each, takes 399 us with weights: 2.21 GB at 5.5 TB/s,
-// 86 % of a copy's rate, DRAM's bound; 12 warps an SM take 41 % of the issue
-// slots, 271 instructions for the 4 KB of a tile.  128 listed blocks per head
-// take 63 us (272 MB at 4.3 TB/s): shares of 150 tiles begin and join more
-// often.  One sequence of 262,147 tokens takes 104 us (539 MB at 5.2 TB/s).
+// channels with 4 rows each, takes 402 us with weights: 2.21 GB at 5.5 TB/s,
+// 85 % of a copy's rate, DRAM's bound; 12 warps an SM take 43 % of the issue
+// slots, 282 instructions for the 4 KB of a tile.  128 listed blocks per head
+// take 64 us (272 MB at 4.2 TB/s): shares of 150 tiles begin and join more
+// often.  One sequence of 262,147 tokens takes 105 us (539 MB at 5.1 TB/s).
 // 40 rows on 8 sequences of 700 to 9001 tokens take 64 us, three passes that
 // are bound by the latency of their instructions (46 % of the slots).
 #include "kv.h"
@@ -63,7 +63,9 @@ constexpr float kAbove = 15.0f, kPlace = 10.0f;
 // counts moves up, and
 // takes pairs of bf16 (16 bits, fp32's range) in twice the products.  They lie 2^kLift higher: up to
 // 2^kFarAbove, which times 448 times 2^31 tokens is still a number, and down to 2^-126, so that not
-// even values that are all 0 in a block of large scale and weight hide the others.
+// even values that are all 0 in a block of large scale and weight hide the others.  With every other
+// block 2^40 below its neighbours the decode step takes 457 us instead of 402, 40 rows 92 instead of
+// 64; all in pairs from the start would cost every call that.
 constexpr float kNear = 1024.0f;
 constexpr float kFarAbove = 85.0f, kFarPlace = 81.0f, kLift = 70.0f;
 constexpr float kNoScore = -3.0e38f;  // reference of a row without a score

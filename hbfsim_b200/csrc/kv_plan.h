@@ -71,8 +71,8 @@ inline Plan plan_of(const PlanCall& c, u32 sms)
     // Short segments (by the table's width or the lists' length) are finished where they are
     // summed: one launch, where the even split takes two and joins.  With an SM for each, they get
     // CTAs of 8 warps: 64 of 38 tiles (128 channels) take 9.9 us, 12.4 us with 4 warps and 15.8 us
-    // split.  Longer ones get teams of CTAs: 8 of 128 tiles take 10.1 us and 13.2 us split, 32 of
-    // 256 tiles 14.0 and 22.0 us, 8 of 1024 tiles 19.9 and 21.4 us.  The more tiles a CTA has, the
+    // split.  Longer ones get teams of CTAs: 8 of 128 tiles take 10.0 us and 13.2 us split, 32 of
+    // 256 tiles 14.4 and 22.0 us, 8 of 1024 tiles 20.0 and 21.4 us.  The more tiles a CTA has, the
     // more CTAs there have to be: 64 of 128 tiles take 17.7 us by one CTA each and 21.5 us split.
     p.warps = p.segments <= sms ? 2 * kWarps : kWarps;
     p.team = 1;  // CTAs of 4 warps take a segment each

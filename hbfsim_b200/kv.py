@@ -255,7 +255,9 @@ def kv_attention(cache: KvCache, q, table, lengths, scale: float | None = None, 
     """Attention of the newest tokens: q [seqs, tokens, q_heads, head_dim],
     token t at position lengths - tokens + t.  scale: of the products
     (default head_dim ** -0.5).  blocks, counts: lists as kv_select returns
-    them (default: every block).
+    them (default: every block).  The table's width decides how the call is
+    spread over the device: narrow it (table[:, :n]) where all sequences are
+    known to be short.
 
     Returns out (q's type and shape), lse (float32 [seqs, tokens, q_heads],
     natural logarithm of the sum of exponentials) and, if asked for, weights

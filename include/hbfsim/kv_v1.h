@@ -28,6 +28,18 @@
  * return an hbfsim_error; they can be captured in a CUDA graph.  A call with
  * no work returns HBFSIM_OK and launches nothing.  Results do not depend on
  * the order in which thread blocks run.
+ *
+ * Limits, beyond which a call returns HBFSIM_INVALID_ARGUMENT: 2^31 - 1 pages,
+ * 1024 key/value heads, 65536 sequences, 2^24 blocks and 2^31 - 1 tokens to a
+ * table's row, 2^31 - 1 query rows (sequences * tokens * heads), 2^22 tokens to
+ * an append.
+ *
+ * How a call is spread over the device follows from what the host knows: the
+ * table's width and the room of the lists, not the lengths, which the device
+ * reads.  A table much wider than its longest sequence takes the form for long
+ * rows (one of 301 tokens then takes two kernels, 10 us, instead of one, 7 us):
+ * where the lengths are known to be short, pass a smaller width with the same
+ * table_stride.
  */
 #ifndef HBFSIM_KV_V1_H
 #define HBFSIM_KV_V1_H
@@ -122,11 +134,12 @@ typedef struct hbfsim_kv_query_v1 {
 /* Block lists by a cheap score.  The queries of a group (the query heads of
  * one key/value head) become whole numbers, qi = rint(q * 2^(7-x)) within
  * +-127, x the binary exponent of their largest magnitude; block j scores
- * (float)(sum_d sum_g max(qi, 0) * hi + min(qi, 0) * lo) * key scale, which
- * bounds the group's summed products from above.  The sums are whole
- * numbers, so lists are equal however they are computed.  The first `sink`
- * blocks and the last `recent` of what the token sees are always listed,
- * then the greatest scores, the lowest index among equals.
+ * (float)(sum_d sum_g max(qi, 0) * hi + min(qi, 0) * lo) * key scale, which,
+ * up to the rounding of the queries, bounds the group's summed products from
+ * above.  The sums are whole numbers, so lists are equal however they are
+ * computed.  The first `sink` blocks and the last `recent` of what the token
+ * sees are always listed, then the greatest scores, the lowest index among
+ * equals.
  * blocks: int32 [seqs][tokens][kv_heads][top], ascending, -1 behind the
  * count; counts: int32 [seqs][tokens][kv_heads].  sink + recent <= top,
  * recent >= 1.  Elements of q that are not finite count as 0. */
