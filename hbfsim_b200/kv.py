@@ -353,9 +353,8 @@ def kv_block_reads(cache: KvCache, table, blocks, counts, base: int):
     have, or whose page is not in the pool, is passed over, as the attention
     does."""
     import torch
-    _need(blocks.dim() == 4 and table.dim() == 2 and table.shape[0] == blocks.shape[0]
-          and counts.shape == blocks.shape[:3],
-          "blocks: [seqs, tokens, kv_heads, top] with counts and table of the same seqs")
+    _need(blocks.dim() == 4 and table.dim() == 2 and table.shape[0] >= blocks.shape[0],
+          "blocks: [seqs, tokens, kv_heads, top] with a row of the table for each of seqs")
     heads, top = blocks.shape[2:]
     width = table.shape[1]
     rank = torch.arange(top, device=blocks.device)

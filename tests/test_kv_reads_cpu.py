@@ -49,3 +49,12 @@ def test_views():
     table = int32([[9, 4, 5, 9], [9, 6, 7, 9]])[:, 1:3]
     every = torch.arange(2, dtype=torch.int32).expand(2, 1, 2, 2)
     assert reads(table, every, int32([2, 1])[:, None, None].expand(2, 1, 2)) == [8, 10, 9, 11, 12, 13]
+
+
+def test_counts_for_all_heads_and_a_longer_table():
+    """Counts that broadcast, and rows of the table behind the sequences at hand."""
+    table = int32([[4, 5], [6, 7], [1, 1]])
+    blocks = int32([[[[0, 1], [1, 0]]], [[[1, 0], [0, 1]]]])
+    assert reads(table, blocks, int32([[[1]], [[2]]])) == [8, 11, 14, 12, 13, 15]
+    with pytest.raises(ValueError):
+        reads(table[:1], blocks, int32([[[1]], [[2]]]))
