@@ -474,8 +474,7 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
 
     float o[NT][D / 16][4];
     float m[NT][2], l[NT][2], ref[NT][2];  // reference and sum of the scores; of the values, if far
-    // the greatest value scale met, its inverse, 1 / kNear of it; the least
-    float value_scale = 0.0f, value_inverse = 0.0f, floor_scale = 0.0f, least_scale = INFINITY;
+    float value_scale = 0.0f, least_scale = INFINITY;  // the greatest and the least value scale met
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -582,16 +581,14 @@ __device__ __forceinline__ void run_segment(const AttentionArgs& a, const Segmen
         }
         if constexpr (!kFar) {
             least_scale = fminf(least_scale, new_scale);
-            if (new_scale > value_scale || new_scale < floor_scale) {
+            if (new_scale > value_scale || new_scale * kNear < value_scale) {
                 if (value_scale > 0.0f && fmaxf(new_scale, value_scale) > least_scale * kNear) return false;
-                value_inverse = inverse_power(new_scale);
-                multiply(value_scale * value_inverse);  // a change rescales what is summed
+                multiply(value_scale * inverse_power(new_scale));  // a change rescales what is summed
                 value_scale = new_scale;
-                floor_scale = new_scale * (1.0f / kNear);
             }
         }
         const float value_log2 = exponent_of(new_scale);
-        const __half2 relative = __float2half2_rn(new_scale * value_inverse);
+        const __half2 relative = __float2half2_rn(new_scale * inverse_power(value_scale));
         u32 b[NT][2], b_rest[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
