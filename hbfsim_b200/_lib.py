@@ -148,6 +148,7 @@ class LinkResultV1(ctypes.Structure):
 
 # include/hbfsim/kv_v1.h
 KV_BF16, KV_F16 = 0, 1
+KV_P_BF16, KV_P_F16, KV_P_F32 = 0, 1, 2
 
 
 class KvCacheV1(ctypes.Structure):
@@ -183,6 +184,47 @@ class KvEvictBatchV1(ctypes.Structure):
                 ("recent", u32), ("decay", u32), ("score", vp), ("weights", vp), ("table", vp),
                 ("table_stride", i64), ("lengths", vp), ("score_out", vp), ("table_out", vp),
                 ("lengths_out", vp), ("freed", vp), ("freed_counts", vp)]
+
+
+class KvRotaryV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("q_heads", u32), ("axes", u32),
+                ("pairs", u32), ("neighbours", u32), ("q", vp), ("q_stride_token", i64),
+                ("q_stride_head", i64), ("q_out", vp), ("positions", vp),
+                ("positions_stride", i64), ("freq", vp), ("axis", vp)]
+
+
+class KvVerifyBatchV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("type", u32), ("seqs", u32),
+                ("drafts", u32), ("vocab", u32), ("target", vp), ("target_stride_seq", i64),
+                ("target_stride_token", i64), ("draft", vp), ("draft_stride_seq", i64),
+                ("draft_stride_token", i64), ("tokens", vp), ("accept", vp), ("sample", vp),
+                ("counts", vp), ("lengths", vp), ("accepted", vp), ("tokens_out", vp),
+                ("lengths_out", vp)]
+
+
+class KvResizeBatchV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("seqs", u32), ("width", u32),
+                ("block_tokens", u32), ("freed_rows", u32), ("freed_width", u32),
+                ("reserved", u32), ("pages", u64), ("refs", vp), ("table", vp),
+                ("table_stride", i64), ("lengths", vp), ("want", vp), ("freed", vp),
+                ("freed_counts", vp), ("refs_out", vp), ("table_out", vp),
+                ("table_out_stride", i64), ("limits", vp), ("src", vp), ("dst", vp),
+                ("workspace", vp), ("workspace_bytes", u64)]
+
+
+class KvForkBatchV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("seqs", u32), ("rows", u32),
+                ("width", u32), ("block_tokens", u32), ("pages", u64), ("refs", vp), ("table", vp),
+                ("table_stride", i64), ("lengths", vp), ("parents", vp), ("refs_out", vp),
+                ("table_out", vp), ("lengths_out", vp)]
+
+
+class KvCompactBatchV1(ctypes.Structure):
+    _fields_ = [("struct_size", u32), ("version", u32), ("seqs", u32), ("width", u32),
+                ("pages", u64), ("refs", vp), ("table", vp), ("table_stride", i64),
+                ("refs_out", vp), ("table_out", vp), ("table_out_stride", i64), ("src", vp),
+                ("dst", vp), ("live", vp), ("where", vp), ("workspace", vp),
+                ("workspace_bytes", u64)]
 
 
 # Every exported function with its signature (restype, argtypes).
@@ -242,6 +284,14 @@ SIGNATURES = {
     "hbfsim_kv_attention_workspace_v1": (u64, [vp, vp, vp]),
     "hbfsim_kv_attention_v1": (i32, [vp, vp, vp, vp]),
     "hbfsim_kv_evict_v1": (i32, [vp, vp]),
+    "hbfsim_kv_append_rotary_v1": (i32, [vp, vp, vp, vp]),
+    "hbfsim_kv_verify_v1": (i32, [vp, vp]),
+    "hbfsim_kv_resize_workspace_v1": (u64, [vp]),
+    "hbfsim_kv_resize_v1": (i32, [vp, vp]),
+    "hbfsim_kv_fork_v1": (i32, [vp, vp]),
+    "hbfsim_kv_compact_workspace_v1": (u64, [vp]),
+    "hbfsim_kv_compact_v1": (i32, [vp, vp]),
+    "hbfsim_kv_copy_v1": (i32, [vp, vp, vp, vp, u64, vp]),
 }
 
 

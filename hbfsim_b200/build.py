@@ -21,7 +21,8 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["timing.cu", "empirical.cu", "context.cu", "thermal.cu", "capacity.cu",
            "retention.cu", "prefetch.cu", "link.cu", "kv_append.cu", "kv_select.cu",
-           "kv_attention.cu", "kv_evict.cu", "profile.cpp"]
+           "kv_attention.cu", "kv_evict.cu", "kv_rotary.cu", "kv_verify.cu", "kv_pages.cu",
+           "profile.cpp"]
 
 
 def sources() -> list[Path]:

@@ -1,0 +1,819 @@
+// kv_pages.cu -- who has which page of the cache (kv_v1.h): pages for new
+// tokens and back, children of sequences, the pages in use moved to the front,
+// and the copies that both lead to.
+//
+// The work is a few passes over the counts and the table, each of which needs
+// all of the one before: what goes back has to be counted before free pages are
+// ranked, and ranked before they are given.  The passes are device functions of
+// a team of thread blocks.  A small pool is done by one cluster of 8 in one
+// launch, with cluster barriers between the passes; a large one by as many
+// blocks as the device has SMs, a launch to a pass.  A pass shares its elements
+// out evenly, in order, so that ranks are sums over the blocks before.
+#include "kv.h"
+
+namespace hbfb {
+namespace {
+
+constexpr u32 kPageThreads = 1024;
+constexpr u32 kPageTeam = 8;      // blocks of the cluster
+constexpr u32 kMaxParts = 1024;   // blocks of a pass at most
+constexpr u32 kUnit = 512;        // entries of a table's row that a warp takes at a time
+// Counts and entries that one cluster takes; beyond, a launch to a pass.
+constexpr u64 kClusterElements = 1u << 19;
+
+// The elements [from, end) of a block, in pieces of `grain`.
+struct Share {
+    u32 from, end;
+};
+__device__ __forceinline__ Share share_of(u32 n, u32 grain, const KvTeam& team)
+{
+    const u64 pieces = (static_cast<u64>(n) + grain - 1) / grain;
+    const u64 from = pieces * team.rank / team.size * grain, end = pieces * (team.rank + 1) / team.size * grain;
+    return {static_cast<u32>(min(from, static_cast<u64>(n))), static_cast<u32>(min(end, static_cast<u64>(n)))};
+}
+
+// Sum of parts[0..team.rank) and of all parts, by every thread of the block.
+struct Before {
+    u32 mine, all;
+};
+__device__ __forceinline__ Before before_of(const u32* parts, const KvTeam& team, u32* room)
+{
+    __syncthreads();  // earlier readers of `room` are done
+    if (threadIdx.x < 32) {
+        u32 mine = 0, all = 0;
+        for (u32 i = threadIdx.x; i < team.size; i += 32) {
+            all += parts[i];
+            if (i < team.rank) mine += parts[i];
+        }
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        all = __reduce_add_sync(0xffffffffu, all);
+        if (threadIdx.x == 0) {
+            room[0] = mine;
+            room[1] = all;
+        }
+    }
+    __syncthreads();
+    return {room[0], room[1]};
+}
+
+// Sum over the block, by every thread.
+__device__ __forceinline__ u32 block_sum(u32 x, u32* warp_sums)
+{
+    x = __reduce_add_sync(0xffffffffu, x);
+    __syncthreads();
+    if ((threadIdx.x & 31u) == 0) warp_sums[threadIdx.x >> 5] = x;
+    __syncthreads();
+    const u32 lane = threadIdx.x & 31u;
+    return __reduce_add_sync(0xffffffffu, lane < blockDim.x >> 5 ? warp_sums[lane] : 0);
+}
+
+struct PageShared {
+    u32 warp_sums[33];
+    u32 room[2];
+};
+
+// Calls entry(row, j) for every entry of a table, a run of a row to a warp.
+template <typename Entry>
+__device__ __forceinline__ void for_entries(u32 rows, u32 width, const KvTeam& team, const Entry& entry)
+{
+    const u32 lane = threadIdx.x & 31u, warps = team.size * (blockDim.x >> 5);
+    const u32 per_row = (width + kUnit - 1) / kUnit;
+    const u64 units = static_cast<u64>(rows) * per_row;
+    for (u64 u = team.rank * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
+        const u32 row = static_cast<u32>(u / per_row), from = static_cast<u32>(u - static_cast<u64>(row) * per_row) * kUnit;
+        entry(row, from + lane, min(from + kUnit, width));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Pages for new tokens and back
+
+struct ResizeArgs {
+    const int* refs;
+    const int* table;
+    i64 table_stride;
+    const int* lengths;
+    const int* want;
+    const int* freed;
+    const int* freed_counts;
+    int* refs_out;
+    int* table_out;
+    i64 table_out_stride;
+    int* limits;
+    int* src;
+    int* dst;
+    u32 seqs, width, block, freed_rows, freed_width, pages;
+    // workspace
+    u32* asked;    // [seqs + 1] blocks that earlier sequences ask for
+    u32* free_part;   // [kMaxParts] free pages of a block's share
+    u32* claim_part;  // [kMaxParts] claims of a block's share
+    int* claims;   // [pages] of a shared page: how often it is asked for
+    int* last;     // [pages] and by which sequence last
+    int* pool;     // free pages in ascending order, as many as may be asked for
+    u8* state;     // [asked] what becomes of an asked block
+};
+enum State : u8 { kKeep = 0, kNew = 1, kPart = 2, kStays = 3 };
+
+struct Row {
+    u32 held, goal, first, need;  // tokens; asked blocks [first, need) if goal > held
+};
+__device__ __forceinline__ Row row_of(const ResizeArgs& a, u32 s)
+{
+    Row r;
+    r.held = static_cast<u32>(kv_length(a.lengths, s, a.width, a.block));
+    r.goal = static_cast<u32>(kv_length(a.want, s, a.width, a.block));
+    r.first = r.held / a.block;
+    r.need = (r.goal + a.block - 1) / a.block;
+    return r;
+}
+
+// Counts into their new place, rows' asked blocks added up.
+__device__ void resize_begin(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+{
+    const u32 at = team.rank * blockDim.x + threadIdx.x, threads = team.size * blockDim.x;
+    if (a.refs_out != a.refs)
+        for (u32 p = at; p < a.pages; p += threads) a.refs_out[p] = a.refs[p];
+    for (u32 s = at; s < a.seqs; s += threads) {
+        a.limits[s] = static_cast<int>(row_of(a, s).goal);
+        a.src[s] = a.dst[s] = -1;
+    }
+    if (team.rank) return;
+    u32 sum = 0;
+    for (u32 s0 = 0; s0 < a.seqs; s0 += blockDim.x) {
+        const u32 s = s0 + threadIdx.x;
+        u32 mine = 0;
+        if (s < a.seqs) {
+            const Row r = row_of(a, s);
+            mine = r.goal > r.held ? r.need - r.first : 0;
+        }
+        const u32 upto = kv_block_scan(mine, sm.warp_sums);
+        if (s < a.seqs) a.asked[s] = sum + upto - mine;
+        sum += sm.warp_sums[32];
+    }
+    if (threadIdx.x == 0) a.asked[a.seqs] = sum;
+}
+
+// What lies behind the rows' new ends goes back, and what an eviction freed.
+__device__ void resize_back(const ResizeArgs& a, const KvTeam& team)
+{
+    for_entries(a.seqs, a.width, team, [&](u32 s, u32 j, u32 end) {
+        const Row r = row_of(a, s);
+        const int* from = a.table + static_cast<i64>(s) * a.table_stride;
+        int* to = a.table_out + static_cast<i64>(s) * a.table_out_stride;
+        for (; j < end; j += 32) {
+            const int e = from[j];
+            const bool there = static_cast<u32>(e) < a.pages;
+            if (j >= r.need) {
+                if (there) atomicSub(a.refs_out + e, 1);
+                if (to != from || e != -1) to[j] = -1;
+            } else {
+                if (there && j >= r.first && r.goal > r.held) {  // asked for; counted in the next pass
+                    a.claims[e] = 0;
+                    a.last[e] = -1;
+                }
+                if (to != from) to[j] = e;
+            }
+        }
+    });
+    for_entries(a.freed_rows, a.freed_width, team, [&](u32 s, u32 j, u32 end) {
+        end = min(end, static_cast<u32>(max(a.freed_counts[s], 0)));
+        for (; j < end; j += 32) {
+            const int e = a.freed[static_cast<u64>(s) * a.freed_width + j];
+            if (static_cast<u32>(e) < a.pages) atomicSub(a.refs_out + e, 1);
+        }
+    });
+}
+
+// The sequence of an asked block: the last whose blocks begin at or before it.
+__device__ __forceinline__ u32 asked_by(const ResizeArgs& a, u32 i)
+{
+    u32 lo = 0, hi = a.seqs;
+    while (hi - lo > 1) {
+        const u32 mid = (lo + hi) >> 1;
+        if (a.asked[mid] <= i) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Asked block i: its sequence, its place in the table.
+struct Asked {
+    u32 seq, block, first;
+    int* entry;
+};
+__device__ __forceinline__ Asked asked_at(const ResizeArgs& a, u32 i)
+{
+    const u32 s = asked_by(a, i);
+    const u32 first = static_cast<u32>(kv_length(a.lengths, s, a.width, a.block)) / a.block;
+    const u32 j = first + (i - a.asked[s]);
+    return {s, j, first, a.table_out + static_cast<i64>(s) * a.table_out_stride + j};
+}
+
+// Free pages of the block's share are counted, and how often shared pages are asked for.
+__device__ void resize_count(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+{
+    const Share own = share_of(a.pages, kPageThreads, team);
+    u32 free = 0;
+    for (u32 p = own.from + threadIdx.x; p < own.end; p += blockDim.x) free += a.refs_out[p] < 1;
+    free = block_sum(free, sm.warp_sums);
+    if (threadIdx.x == 0) a.free_part[team.rank] = free;
+    const Share asked = share_of(a.asked[a.seqs], kPageThreads, team);
+    for (u32 i = asked.from + threadIdx.x; i < asked.end; i += blockDim.x) {
+        const Asked x = asked_at(a, i);
+        const int e = *x.entry;
+        if (static_cast<u32>(e) < a.pages && a.refs_out[e] > 1) {
+            atomicAdd(a.claims + e, 1);
+            atomicMax(a.last + e, static_cast<int>(x.seq));
+        }
+    }
+}
+
+// Free pages in ascending order, as many as may be asked for; what becomes of the asked blocks.
+__device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+{
+    const u32 all = a.asked[a.seqs];
+    const Share asked = share_of(all, kPageThreads, team);
+    u32 claims = 0;
+    for (u32 i = asked.from + threadIdx.x; i < asked.end; i += blockDim.x) {
+        const Asked x = asked_at(a, i);
+        const int e = *x.entry;
+        u8 state = kNew;
+        if (static_cast<u32>(e) < a.pages) {
+            state = kKeep;
+            if (const int count = a.refs_out[e]; count > 1)
+                state = a.claims[e] >= count && a.last[e] == static_cast<int>(x.seq) ? kStays : kPart;
+        }
+        a.state[i] = state;
+        claims += state == kNew || state == kPart;
+    }
+    claims = block_sum(claims, sm.warp_sums);
+    if (threadIdx.x == 0) a.claim_part[team.rank] = claims;
+    const Share own = share_of(a.pages, kPageThreads, team);
+    u32 rank = before_of(a.free_part, team, sm.room).mine;
+    for (u32 p0 = own.from; p0 < own.end && rank < all; p0 += blockDim.x) {
+        const u32 p = p0 + threadIdx.x;
+        const bool free = p < own.end && a.refs_out[p] < 1;
+        const u32 upto = kv_block_scan(free, sm.warp_sums);
+        if (free && rank + upto - 1 < all) a.pool[rank + upto - 1] = static_cast<int>(p);
+        rank += sm.warp_sums[32];
+    }
+}
+
+// Claims get their pages.
+__device__ void resize_give(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+{
+    const u32 free = before_of(a.free_part, team, sm.room).all;
+    const Share asked = share_of(a.asked[a.seqs], kPageThreads, team);
+    u32 rank = before_of(a.claim_part, team, sm.room).mine;
+    for (u32 i0 = asked.from; i0 < asked.end; i0 += blockDim.x) {
+        const u32 i = i0 + threadIdx.x;
+        const u8 state = i < asked.end ? a.state[i] : kKeep;
+        const bool claim = state == kNew || state == kPart;
+        const u32 upto = kv_block_scan(claim, sm.warp_sums);
+        const u32 before = rank + upto - claim;
+        rank += sm.warp_sums[32];
+        if (state == kKeep) continue;
+        const Asked x = asked_at(a, i);
+        const u32 held = static_cast<u32>(kv_length(a.lengths, x.seq, a.width, a.block));
+        if (claim ? before >= free : before > free) {  // not served
+            atomicMin(a.limits + x.seq, static_cast<int>(max(held, x.block * a.block)));
+        } else if (claim) {
+            const int page = a.pool[before];
+            if (state == kPart) {
+                const int old = *x.entry;
+                atomicSub(a.refs_out + old, 1);
+                if (x.block == x.first && held % a.block) {
+                    a.src[x.seq] = old;
+                    a.dst[x.seq] = page;
+                }
+            }
+            a.refs_out[page] = 1;
+            *x.entry = page;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kPageThreads) resize_cluster_kernel(const ResizeArgs a)
+{
+    __shared__ PageShared sm;
+    const KvTeam team{blockIdx.x, kPageTeam};
+    resize_begin(a, team, sm);
+    kv_team_sync(team);
+    resize_back(a, team);
+    kv_team_sync(team);
+    resize_count(a, team, sm);
+    kv_team_sync(team);
+    resize_rank(a, team, sm);
+    kv_team_sync(team);
+    resize_give(a, team, sm);
+}
+
+template <int kPass>
+__global__ void __launch_bounds__(kPageThreads) resize_pass_kernel(const ResizeArgs a)
+{
+    __shared__ PageShared sm;
+    kv_let_next();
+    kv_wait_before();
+    const KvTeam team{blockIdx.x, gridDim.x};
+    if constexpr (kPass == 0) resize_begin(a, team, sm);
+    else if constexpr (kPass == 1) resize_back(a, team);
+    else if constexpr (kPass == 2) resize_count(a, team, sm);
+    else if constexpr (kPass == 3) resize_rank(a, team, sm);
+    else resize_give(a, team, sm);
+}
+
+// ---------------------------------------------------------------------------
+// Children
+
+struct ForkArgs {
+    const int* refs;
+    const int* table;
+    i64 table_stride;
+    const int* lengths;
+    const int* parents;
+    int* refs_out;
+    int* table_out;
+    int* lengths_out;
+    u32 seqs, rows, width, block, pages;
+};
+
+__device__ void fork_begin(const ForkArgs& a, const KvTeam& team)
+{
+    const u32 threads = team.size * blockDim.x;
+    for (u32 p = team.rank * blockDim.x + threadIdx.x; p < a.pages; p += threads) a.refs_out[p] = a.refs[p];
+}
+
+__device__ __forceinline__ u32 blocks_held(const ForkArgs& a, u32 s)
+{
+    return (static_cast<u32>(kv_length(a.lengths, s, a.width, a.block)) + a.block - 1) / a.block;
+}
+
+// The new rows take their pages, the old ones give theirs back; a row that goes on as itself does
+// neither for the blocks that it holds.
+__device__ void fork_rows(const ForkArgs& a, const KvTeam& team)
+{
+    const u32 threads = team.size * blockDim.x;
+    for (u32 r = team.rank * blockDim.x + threadIdx.x; r < a.rows; r += threads) {
+        const u32 parent = static_cast<u32>(a.parents[r]);
+        a.lengths_out[r] = parent < a.seqs ? kv_length(a.lengths, parent, a.width, a.block) : 0;
+    }
+    for_entries(a.rows, a.width, team, [&](u32 r, u32 j, u32 end) {
+        const u32 parent = static_cast<u32>(a.parents[r]);
+        const bool real = parent < a.seqs;
+        const u32 blocks = real ? blocks_held(a, parent) : 0;
+        const int* from = a.table + static_cast<i64>(real ? parent : 0) * a.table_stride;
+        int* to = a.table_out + static_cast<u64>(r) * a.width;
+        for (; j < end; j += 32) {
+            const int e = j < blocks ? from[j] : -1;
+            to[j] = e;
+            if (parent != r && static_cast<u32>(e) < a.pages) atomicAdd(a.refs_out + e, 1);
+        }
+    });
+    for_entries(a.seqs, a.width, team, [&](u32 s, u32 j, u32 end) {
+        const u32 stay = s < a.rows && a.parents[s] == static_cast<int>(s) ? blocks_held(a, s) : 0;
+        const int* from = a.table + static_cast<i64>(s) * a.table_stride;
+        for (; j < end; j += 32) {
+            const int e = j < stay ? -1 : from[j];
+            if (static_cast<u32>(e) < a.pages) atomicSub(a.refs_out + e, 1);
+        }
+    });
+}
+
+__global__ void __launch_bounds__(kPageThreads) fork_cluster_kernel(const ForkArgs a)
+{
+    const KvTeam team{blockIdx.x, kPageTeam};
+    fork_begin(a, team);
+    kv_team_sync(team);
+    fork_rows(a, team);
+}
+
+template <int kPass>
+__global__ void __launch_bounds__(kPageThreads) fork_pass_kernel(const ForkArgs a)
+{
+    kv_let_next();
+    kv_wait_before();
+    const KvTeam team{blockIdx.x, gridDim.x};
+    if constexpr (kPass == 0) fork_begin(a, team);
+    else fork_rows(a, team);
+}
+
+// ---------------------------------------------------------------------------
+// Pages in use to the front
+
+struct CompactArgs {
+    const int* refs;
+    const int* table;
+    i64 table_stride;
+    int* refs_out;
+    int* table_out;
+    i64 table_out_stride;
+    int* src;
+    int* dst;
+    int* live;
+    int* where;
+    u32 seqs, width, pages;
+    u32* live_part;  // workspace: [kMaxParts] pages in use of a block's share
+};
+
+__device__ void compact_count(const CompactArgs& a, const KvTeam& team, PageShared& sm)
+{
+    const Share own = share_of(a.pages, kPageThreads, team);
+    u32 live = 0;
+    for (u32 p = own.from + threadIdx.x; p < own.end; p += blockDim.x) live += a.refs[p] > 0;
+    live = block_sum(live, sm.warp_sums);
+    if (threadIdx.x == 0) a.live_part[team.rank] = live;
+    const u32 threads = team.size * blockDim.x, room = a.pages / 2;
+    for (u32 i = team.rank * blockDim.x + threadIdx.x; i < room; i += threads) a.src[i] = a.dst[i] = -1;
+}
+
+// The moves: page p in use past the n that are has n - (pages in use up to p) such pages above it,
+// free page p below has p - (pages in use before p) free ones below it.  Until the next pass, `where`
+// holds -2 - move of a page that moves.
+__device__ void compact_rank(const CompactArgs& a, const KvTeam& team, PageShared& sm)
+{
+    const Before before = before_of(a.live_part, team, sm.room);
+    const u32 n = before.all;
+    if (team.rank == 0 && threadIdx.x == 0) *a.live = static_cast<int>(n);
+    const Share own = share_of(a.pages, kPageThreads, team);
+    u32 rank = before.mine;
+    for (u32 p0 = own.from; p0 < own.end; p0 += blockDim.x) {
+        const u32 p = p0 + threadIdx.x;
+        const int count = p < own.end ? a.refs[p] : 0;
+        const bool live = count > 0;
+        const u32 upto = rank + kv_block_scan(live, sm.warp_sums);
+        rank += sm.warp_sums[32];
+        if (p >= own.end) continue;
+        int place = -1;
+        if (p < n) {
+            if (live) {
+                place = static_cast<int>(p);
+                if (a.refs_out != a.refs) a.refs_out[p] = count;
+            } else {
+                a.dst[p - upto] = static_cast<int>(p);  // its count comes with the page
+            }
+        } else if (live) {
+            const u32 move = n - upto;
+            a.src[move] = static_cast<int>(p);
+            place = -2 - static_cast<int>(move);  // its count leaves with the page
+        } else {
+            a.refs_out[p] = 0;
+        }
+        a.where[p] = place;
+    }
+}
+
+__device__ void compact_move(const CompactArgs& a, const KvTeam& team)
+{
+    const u32 threads = team.size * blockDim.x, room = a.pages / 2;
+    // entries: a page that moves is found by its number or, if the loop below was faster, by its place
+    for_entries(a.seqs, a.width, team, [&](u32 s, u32 j, u32 end) {
+        const int* from = a.table + static_cast<i64>(s) * a.table_stride;
+        int* to = a.table_out + static_cast<i64>(s) * a.table_out_stride;
+        for (; j < end; j += 32) {
+            int e = from[j];
+            if (static_cast<u32>(e) < a.pages) {
+                e = *static_cast<volatile int*>(a.where + e);
+                if (e < -1) e = a.dst[-2 - e];
+            }
+            to[j] = e;
+        }
+    });
+    for (u32 i = team.rank * blockDim.x + threadIdx.x; i < room; i += threads) {
+        const int from = a.src[i];
+        if (from < 0) break;  // moves are listed without gaps
+        const int to = a.dst[i], count = a.refs[from];
+        a.refs_out[to] = count;
+        a.refs_out[from] = 0;
+        *static_cast<volatile int*>(a.where + from) = to;
+    }
+}
+
+__global__ void __launch_bounds__(kPageThreads) compact_cluster_kernel(const CompactArgs a)
+{
+    __shared__ PageShared sm;
+    const KvTeam team{blockIdx.x, kPageTeam};
+    compact_count(a, team, sm);
+    kv_team_sync(team);
+    compact_rank(a, team, sm);
+    kv_team_sync(team);
+    compact_move(a, team);
+}
+
+template <int kPass>
+__global__ void __launch_bounds__(kPageThreads) compact_pass_kernel(const CompactArgs a)
+{
+    __shared__ PageShared sm;
+    kv_let_next();
+    kv_wait_before();
+    const KvTeam team{blockIdx.x, gridDim.x};
+    if constexpr (kPass == 0) compact_count(a, team, sm);
+    else if constexpr (kPass == 1) compact_rank(a, team, sm);
+    else compact_move(a, team);
+}
+
+// ---------------------------------------------------------------------------
+// Copies
+
+constexpr u32 kCopyThreads = 256, kCopyDeep = 4;
+constexpr u32 kCopyPiece = kCopyThreads * kCopyDeep * 16;  // bytes of a thread block at a time
+
+struct CopyArgs {
+    KvView from, to;
+    const int* src;
+    const int* dst;
+    u64 pieces;          // of all moves
+    u32 per_page;        // pieces of a page's data, and one more for its scales and bounds
+    u64 page_bytes;
+};
+
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyArgs a)
+{
+    for (u64 piece = blockIdx.x; piece < a.pieces; piece += gridDim.x) {
+        const u64 move = piece / a.per_page;
+        const u32 part = static_cast<u32>(piece - move * a.per_page);
+        const u32 src = static_cast<u32>(a.src[move]), dst = static_cast<u32>(a.dst[move]);
+        if (src >= a.from.pages || dst >= a.to.pages) continue;
+        if (part + 1 < a.per_page) {
+            const u64 at = static_cast<u64>(part) * kCopyPiece + threadIdx.x * 16;
+            const u8* from = a.from.data + src * a.page_bytes;
+            u8* to = a.to.data + dst * a.page_bytes;
+            uint4 x[kCopyDeep];
+#pragma unroll
+            for (u32 i = 0; i < kCopyDeep; ++i)
+                if (at + i * kCopyThreads * 16 < a.page_bytes)
+                    x[i] = *reinterpret_cast<const uint4*>(from + at + i * kCopyThreads * 16);
+#pragma unroll
+            for (u32 i = 0; i < kCopyDeep; ++i)
+                if (at + i * kCopyThreads * 16 < a.page_bytes)
+                    *reinterpret_cast<uint4*>(to + at + i * kCopyThreads * 16) = x[i];
+            continue;
+        }
+        const u32 bounds = a.from.heads * 2 * a.from.dim, scales = a.from.heads;  // bytes; pairs
+        const uint4* from = reinterpret_cast<const uint4*>(a.from.bounds + static_cast<u64>(src) * bounds);
+        uint4* to = reinterpret_cast<uint4*>(a.to.bounds + static_cast<u64>(dst) * bounds);
+        for (u32 i = threadIdx.x; i < bounds / 16; i += kCopyThreads) to[i] = from[i];
+        const float2* scale = reinterpret_cast<const float2*>(a.from.scale) + static_cast<u64>(src) * scales;
+        float2* scale_to = reinterpret_cast<float2*>(a.to.scale) + static_cast<u64>(dst) * scales;
+        for (u32 i = threadIdx.x; i < scales; i += kCopyThreads) scale_to[i] = scale[i];
+    }
+}
+
+// ---------------------------------------------------------------------------
+
+// Memory [p, p + bytes), to see whether two ranges meet.
+struct Extent {
+    std::uintptr_t from, end;
+    Extent(const void* p, u64 bytes) : from(reinterpret_cast<std::uintptr_t>(p)), end(from + bytes) {}
+    // rows of a table, from the lowest to the highest
+    Extent(const int* p, u64 rows, u64 width, i64 stride) : from(0), end(0)
+    {
+        if (rows == 0 || width == 0) return;
+        const int* last = p + static_cast<i64>(rows - 1) * stride;
+        from = reinterpret_cast<std::uintptr_t>(std::min(p, last));
+        end = reinterpret_cast<std::uintptr_t>(std::max(p, last)) + width * 4;
+    }
+    bool meets(const Extent& o) const { return from < end && o.from < o.end && from < o.end && o.from < end; }
+};
+
+// Whether an output meets an input or another output.  same[i]: the input that output i may be.
+template <int kOut, int kIn>
+bool would_race(const Extent (&out)[kOut], const Extent (&in)[kIn], const int (&same)[kOut])
+{
+    for (int i = 0; i < kOut; ++i) {
+        for (int k = 0; k < kIn; ++k) {
+            if (!out[i].meets(in[k])) continue;
+            if (same[i] != k || out[i].from != in[k].from || out[i].end != in[k].end) return true;
+        }
+        for (int k = 0; k < i; ++k)
+            if (out[i].meets(out[k])) return true;
+    }
+    return false;
+}
+
+bool table_fits(u64 rows, u64 width) { return rows * width <= 0x7fffffffull; }
+
+// Takes parts of a workspace one after the other, 256 bytes aligned.
+struct Room {
+    u64 at = 0;
+    u64 take(u64 bytes)
+    {
+        const u64 here = at;
+        at += kv_round_up(bytes, 256);
+        return here;
+    }
+};
+
+struct ResizeRoom {
+    u64 asked, free_part, claim_part, claims, last, pool, state, bytes;
+};
+ResizeRoom resize_room(const hbfsim_kv_resize_batch_v1& b)
+{
+    Room room;
+    ResizeRoom r{};
+    r.asked = room.take((u64{b.seqs} + 1) * 4);
+    r.free_part = room.take(kMaxParts * 4);
+    r.claim_part = room.take(kMaxParts * 4);
+    r.claims = room.take(b.pages * 4);
+    r.last = room.take(b.pages * 4);
+    r.pool = room.take(std::min(b.pages, u64{b.seqs} * b.width) * 4);
+    r.state = room.take(u64{b.seqs} * b.width);
+    r.bytes = room.at;
+    return r;
+}
+
+int resize_check(const hbfsim_kv_resize_batch_v1* b)
+{
+    if (!b || b->struct_size != sizeof(*b) || b->version != HBFSIM_KV_V1_VERSION || b->reserved)
+        return HBFSIM_INVALID_ARGUMENT;
+    if (b->block_tokens != 16 && b->block_tokens != 32 && b->block_tokens != 64) return HBFSIM_UNSUPPORTED;
+    if (b->seqs > kKvMaxSeqs || b->width > kKvMaxWidth || b->pages > 0x7fffffffull ||
+        u64{b->width} * b->block_tokens > 0x7fffffffull || !table_fits(b->seqs, b->width) ||
+        !table_fits(b->freed_rows, b->freed_width))
+        return HBFSIM_INVALID_ARGUMENT;
+    return HBFSIM_OK;
+}
+
+// Launches a pass over so many blocks, set up behind the one before.
+template <typename Args>
+bool pass(void (*kernel)(Args), u32 blocks, bool behind, const Args& a, cudaStream_t s)
+{
+    return kv_launch(kernel, dim3(blocks), kPageThreads, s, 0, 1, behind, a);
+}
+
+template <typename Args>
+bool cluster(void (*kernel)(Args), const Args& a, cudaStream_t s)
+{
+    return kv_launch(kernel, dim3(kPageTeam), kPageThreads, s, 0, kPageTeam, false, a);
+}
+
+u32 pass_blocks() { return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count()) * 2); }
+
+}  // namespace
+}  // namespace hbfb
+
+using namespace hbfb;
+
+extern "C" uint64_t hbfsim_kv_resize_workspace_v1(const hbfsim_kv_resize_batch_v1* b)
+{
+    return resize_check(b) == HBFSIM_OK ? resize_room(*b).bytes : 0;
+}
+
+extern "C" int hbfsim_kv_resize_v1(const hbfsim_kv_resize_batch_v1* b, void* stream)
+{
+    if (const int rc = resize_check(b)) return rc;
+    if (b->seqs == 0 && b->freed_rows == 0 && b->refs_out == b->refs) return HBFSIM_OK;
+    const u64 entries = u64{b->seqs} * b->width, listed = u64{b->freed_rows} * b->freed_width;
+    if ((b->pages && (!b->refs || !b->refs_out)) || (entries && (!b->table || !b->table_out)) ||
+        (b->seqs && (!b->lengths || !b->want || !b->limits || !b->src || !b->dst)) ||
+        (listed && (!b->freed || !b->freed_counts)) || !b->workspace)
+        return HBFSIM_INVALID_ARGUMENT;
+    for (const void* p : {static_cast<const void*>(b->refs), static_cast<const void*>(b->table),
+                          static_cast<const void*>(b->lengths), static_cast<const void*>(b->want),
+                          static_cast<const void*>(b->freed), static_cast<const void*>(b->freed_counts),
+                          static_cast<const void*>(b->refs_out), static_cast<const void*>(b->table_out),
+                          static_cast<const void*>(b->limits), static_cast<const void*>(b->src),
+                          static_cast<const void*>(b->dst)})
+        if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
+    const ResizeRoom room = resize_room(*b);
+    if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < room.bytes) return HBFSIM_INVALID_ARGUMENT;
+    if (b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
+    // rows of an output may not lie in one another
+    if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
+    const Extent out[] = {{b->refs_out, b->pages * 4},
+                          {b->table_out, b->seqs, b->width, b->table_out_stride},
+                          {b->limits, u64{b->seqs} * 4},
+                          {b->src, u64{b->seqs} * 4},
+                          {b->dst, u64{b->seqs} * 4},
+                          {b->workspace, room.bytes}};
+    const Extent in[] = {{b->refs, b->pages * 4},          {b->table, b->seqs, b->width, b->table_stride},
+                         {b->lengths, u64{b->seqs} * 4},   {b->want, u64{b->seqs} * 4},
+                         {b->freed, listed * 4},           {b->freed_counts, u64{b->freed_rows} * 4}};
+    if (would_race(out, in, {0, 1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
+    u8* w = static_cast<u8*>(b->workspace);
+    const ResizeArgs a{b->refs, b->table, b->table_stride, b->lengths, b->want, b->freed, b->freed_counts,
+                       b->refs_out, b->table_out, b->table_out_stride, b->limits, b->src, b->dst, b->seqs, b->width,
+                       b->block_tokens, listed ? b->freed_rows : 0, b->freed_width, static_cast<u32>(b->pages),
+                       reinterpret_cast<u32*>(w + room.asked), reinterpret_cast<u32*>(w + room.free_part),
+                       reinterpret_cast<u32*>(w + room.claim_part), reinterpret_cast<int*>(w + room.claims),
+                       reinterpret_cast<int*>(w + room.last), reinterpret_cast<int*>(w + room.pool), w + room.state};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    bool ok;
+    if (b->pages + entries + listed <= kClusterElements) {
+        ok = cluster(resize_cluster_kernel, a, s);
+    } else {
+        const u32 blocks = pass_blocks();
+        ok = pass(resize_pass_kernel<0>, blocks, false, a, s) && pass(resize_pass_kernel<1>, blocks, true, a, s) &&
+             pass(resize_pass_kernel<2>, blocks, true, a, s) && pass(resize_pass_kernel<3>, blocks, true, a, s) &&
+             pass(resize_pass_kernel<4>, blocks, true, a, s);
+    }
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+}
+
+extern "C" int hbfsim_kv_fork_v1(const hbfsim_kv_fork_batch_v1* b, void* stream)
+{
+    if (!b || b->struct_size != sizeof(*b) || b->version != HBFSIM_KV_V1_VERSION) return HBFSIM_INVALID_ARGUMENT;
+    if (b->block_tokens != 16 && b->block_tokens != 32 && b->block_tokens != 64) return HBFSIM_UNSUPPORTED;
+    if (b->seqs > kKvMaxSeqs || b->rows > kKvMaxSeqs || b->width > kKvMaxWidth || b->pages > 0x7fffffffull ||
+        u64{b->width} * b->block_tokens > 0x7fffffffull || !table_fits(b->seqs, b->width) ||
+        !table_fits(b->rows, b->width))
+        return HBFSIM_INVALID_ARGUMENT;
+    if (b->seqs == 0 && b->rows == 0 && b->refs_out == b->refs) return HBFSIM_OK;
+    const u64 entries = u64{b->seqs} * b->width, made = u64{b->rows} * b->width;
+    if ((b->pages && (!b->refs || !b->refs_out)) || (entries && !b->table) || (b->seqs && !b->lengths) ||
+        (b->rows && (!b->parents || !b->lengths_out)) || (made && !b->table_out))
+        return HBFSIM_INVALID_ARGUMENT;
+    for (const void* p : {static_cast<const void*>(b->refs), static_cast<const void*>(b->table),
+                          static_cast<const void*>(b->lengths), static_cast<const void*>(b->parents),
+                          static_cast<const void*>(b->refs_out), static_cast<const void*>(b->table_out),
+                          static_cast<const void*>(b->lengths_out)})
+        if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
+    const Extent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, made * 4}, {b->lengths_out, u64{b->rows} * 4}};
+    const Extent in[] = {{b->refs, b->pages * 4},
+                         {b->table, b->seqs, b->width, b->table_stride},
+                         {b->lengths, u64{b->seqs} * 4},
+                         {b->parents, u64{b->rows} * 4}};
+    if (would_race(out, in, {0, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
+    const ForkArgs a{b->refs, b->table, b->table_stride, b->lengths, b->parents, b->refs_out, b->table_out,
+                     b->lengths_out, b->seqs, b->rows, b->width, b->block_tokens, static_cast<u32>(b->pages)};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool apart = b->refs_out != b->refs;
+    bool ok;
+    if (apart && b->pages + entries + made <= kClusterElements) {
+        ok = cluster(fork_cluster_kernel, a, s);
+    } else {
+        const u32 blocks = pass_blocks();
+        ok = (!apart || pass(fork_pass_kernel<0>, blocks, false, a, s)) &&
+             pass(fork_pass_kernel<1>, blocks, apart, a, s);
+    }
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+}
+
+static int compact_check(const hbfsim_kv_compact_batch_v1* b)
+{
+    if (!b || b->struct_size != sizeof(*b) || b->version != HBFSIM_KV_V1_VERSION) return HBFSIM_INVALID_ARGUMENT;
+    if (b->seqs > kKvMaxSeqs || b->width > kKvMaxWidth || b->pages > 0x7fffffffull ||
+        !table_fits(b->seqs, b->width))
+        return HBFSIM_INVALID_ARGUMENT;
+    return HBFSIM_OK;
+}
+
+extern "C" uint64_t hbfsim_kv_compact_workspace_v1(const hbfsim_kv_compact_batch_v1* b)
+{
+    return compact_check(b) == HBFSIM_OK ? kMaxParts * 4 : 0;
+}
+
+extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* stream)
+{
+    if (const int rc = compact_check(b)) return rc;
+    const u64 entries = u64{b->seqs} * b->width, room = b->pages / 2;
+    if (!b->live || (b->pages && (!b->refs || !b->refs_out || !b->where)) || (room && (!b->src || !b->dst)) ||
+        (entries && (!b->table || !b->table_out)) || !b->workspace)
+        return HBFSIM_INVALID_ARGUMENT;
+    for (const void* p : {static_cast<const void*>(b->refs), static_cast<const void*>(b->table),
+                          static_cast<const void*>(b->refs_out), static_cast<const void*>(b->table_out),
+                          static_cast<const void*>(b->src), static_cast<const void*>(b->dst),
+                          static_cast<const void*>(b->live), static_cast<const void*>(b->where)})
+        if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
+    if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < kMaxParts * 4) return HBFSIM_INVALID_ARGUMENT;
+    if (b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
+    if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
+    const Extent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, b->seqs, b->width, b->table_out_stride},
+                          {b->src, room * 4},          {b->dst, room * 4},
+                          {b->live, 4},                {b->where, b->pages * 4},
+                          {b->workspace, kMaxParts * 4}};
+    const Extent in[] = {{b->refs, b->pages * 4}, {b->table, b->seqs, b->width, b->table_stride}};
+    if (would_race(out, in, {0, 1, -1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
+    const CompactArgs a{b->refs, b->table, b->table_stride, b->refs_out, b->table_out, b->table_out_stride, b->src,
+                        b->dst, b->live, b->where, b->seqs, b->width, static_cast<u32>(b->pages),
+                        static_cast<u32*>(b->workspace)};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    bool ok;
+    if (b->pages + entries <= kClusterElements) {
+        ok = cluster(compact_cluster_kernel, a, s);
+    } else {
+        const u32 blocks = pass_blocks();
+        ok = pass(compact_pass_kernel<0>, blocks, false, a, s) && pass(compact_pass_kernel<1>, blocks, true, a, s) &&
+             pass(compact_pass_kernel<2>, blocks, true, a, s);
+    }
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+}
+
+extern "C" int hbfsim_kv_copy_v1(const hbfsim_kv_cache_v1* from, const hbfsim_kv_cache_v1* to, const int32_t* src,
+                                 const int32_t* dst, uint64_t count, void* stream)
+{
+    CopyArgs a{};
+    if (const int rc = kv_check_cache(from, a.from)) return rc;
+    if (const int rc = kv_check_cache(to, a.to)) return rc;
+    if (a.from.heads != a.to.heads || a.from.dim != a.to.dim || a.from.block != a.to.block || count > 0x7fffffffull)
+        return HBFSIM_INVALID_ARGUMENT;
+    if (count == 0) return HBFSIM_OK;
+    if (!src || !dst || !kv_aligned(src, 4) || !kv_aligned(dst, 4)) return HBFSIM_INVALID_ARGUMENT;
+    a.src = src;
+    a.dst = dst;
+    a.page_bytes = 2ull * a.from.heads * a.from.block * a.from.dim;
+    a.per_page = static_cast<u32>((a.page_bytes + kCopyPiece - 1) / kCopyPiece) + 1;
+    a.pieces = count * a.per_page;
+    const u32 blocks = static_cast<u32>(std::min<u64>(a.pieces, static_cast<u64>(kv_sm_count()) * 8));
+    const bool ok = kv_launch(copy_kernel, dim3(blocks), kCopyThreads, static_cast<cudaStream_t>(stream), 0, 1, false, a);
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+}

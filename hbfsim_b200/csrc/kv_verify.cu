@@ -1,0 +1,311 @@
+// kv_verify.cu -- drafted tokens against the target's probabilities (kv_v1.h).
+//
+// One row of the target (and one of the draft) decides a sequence's next token,
+// and which row follows from a few gathered probabilities, so a cluster of up to
+// 8 CTAs takes a sequence: every CTA looks up the drafted tokens, reads its slice
+// of the row once, and its warps add up whole weights, each over a contiguous
+// segment.  The CTAs' sums meet through distributed shared memory; the one whose
+// slice holds the border reads the segment that holds it again and finds the
+// token.
+#include "kv.h"
+
+#include <type_traits>
+
+namespace hbfb {
+namespace {
+
+constexpr u32 kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
+constexpr u32 kMaxDrafts = 32;
+constexpr u32 kMaxVocab = 1u << 22;  // sums stay below 2^62
+constexpr u32 kMaxTeam = 8;
+
+struct VerifyArgs {
+    const void* target;
+    i64 target_seq, target_token;
+    const void* draft;
+    i64 draft_seq, draft_token;
+    const int* tokens;
+    const float* accept;
+    const float* sample;
+    const int* counts;
+    const int* lengths;
+    int* accepted;
+    int* tokens_out;
+    int* lengths_out;
+    u32 drafts, vocab, segment;  // segment: elements of a warp, a multiple of 256
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+// A probability in whole multiples of 2^-40.
+__device__ __forceinline__ i64 whole(float p)
+{
+    return __float2ll_rn(fminf(fmaxf(p, 0.0f), 1.0f) * 1099511627776.0f);  // fmaxf drops NaN; the product is exact
+}
+
+// N neighbouring probabilities in 32 bits.
+template <typename T, int N>
+__device__ __forceinline__ void load_values(const T* from, float (&x)[N])
+{
+    static_assert(sizeof(T) * N == 16, "one load");
+    const uint4 y = *reinterpret_cast<const uint4*>(from);
+    const T* z = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_float(z[i]);
+}
+
+struct Sums {
+    u64 left, target;  // of the weights, of the target alone
+};
+
+__device__ __forceinline__ void add_to(Sums& s, float p, float q)
+{
+    const i64 a = whole(p), d = a - whole(q);
+    s.target += static_cast<u64>(a);
+    s.left += static_cast<u64>(d > 0 ? d : 0);
+}
+
+// Sums of [from, end) by a warp.
+template <typename T, bool kWide, bool kDraft>
+__device__ __forceinline__ Sums sum_segment(const T* p, const T* q, u32 from, u32 end)
+{
+    constexpr int N = 16 / sizeof(T);
+    const u32 lane = threadIdx.x & 31u;
+    Sums s{0, 0};
+    u32 i = from + lane * N;
+    if constexpr (kWide) {
+        constexpr int U = 4;
+        for (; i + (U - 1) * 32 * N + N <= end; i += U * 32 * N) {
+            float x[U][N], y[U][N];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                load_values<T, N>(p + i + u * 32 * N, x[u]);
+                if constexpr (kDraft) load_values<T, N>(q + i + u * 32 * N, y[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < N; ++k) add_to(s, x[u][k], kDraft ? y[u][k] : 0.0f);
+        }
+        for (; i + N <= end; i += 32 * N) {
+            float x[N], y[N];
+            load_values<T, N>(p + i, x);
+            if constexpr (kDraft) load_values<T, N>(q + i, y);
+#pragma unroll
+            for (int k = 0; k < N; ++k) add_to(s, x[k], kDraft ? y[k] : 0.0f);
+        }
+        for (; i < end; ++i) add_to(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);  // one lane's rest
+    } else {
+        for (i = from + lane; i < end; i += 32) add_to(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);
+    }
+    return s;
+}
+
+__device__ __forceinline__ u64 warp_sum(u64 x)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+// Inclusive prefix sums over a warp.
+__device__ __forceinline__ u64 warp_scan(u64 x)
+{
+    const u32 lane = threadIdx.x & 31u;
+#pragma unroll
+    for (u32 o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+struct VerifyShared {
+    u32 accepted, count;
+    int refused;                     // the token that was not accepted, -1 without one
+    u64 warp_left[kVerifyWarps], warp_target[kVerifyWarps];
+    u64 left, target;                // of the CTA: other CTAs read them
+    u64 border;                      // from the segment's beginning on
+    u32 segment;                     // the warp's whose segment holds it; kVerifyWarps: none here
+    u32 alone;                       // whether the target alone counts
+    u64 prefix[kVerifyWarps];
+};
+
+template <typename T, bool kWide>
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a, const u32 size)
+{
+    __shared__ VerifyShared sm;
+    const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const u32 seq = blockIdx.x / size;
+    const KvTeam team{blockIdx.x - seq * size, size};
+    const T* target = static_cast<const T*>(a.target) + static_cast<i64>(seq) * a.target_seq;
+    const T* draft = static_cast<const T*>(a.draft) + static_cast<i64>(seq) * a.draft_seq;
+    if (warp == 0) {
+        const u32 count = a.counts ? static_cast<u32>(min(max(a.counts[seq], 0), static_cast<int>(a.drafts))) : a.drafts;
+        bool good = false;
+        int token = -1;
+        if (lane < count) {
+            const u64 at = static_cast<u64>(seq) * a.drafts + lane;
+            token = a.tokens[at];
+            if (static_cast<u32>(token) < a.vocab) {
+                const double p = to_float(target[static_cast<i64>(lane) * a.target_token + token]);
+                const double q = a.draft ? to_float(draft[static_cast<i64>(lane) * a.draft_token + token]) : 1.0f;
+                good = static_cast<double>(a.accept[at]) * q < p;  // 24 bits by 24: exact
+            } else {
+                token = -1;
+            }
+        }
+        const u32 accepted = __ffs(~__ballot_sync(0xffffffffu, good)) - 1u;  // ~0 where all 32 are
+        const u32 n = min(accepted, count);
+        const int refused = n < count ? __shfl_sync(0xffffffffu, token, static_cast<int>(n)) : -1;
+        if (lane == 0) {
+            sm.accepted = n;
+            sm.count = count;
+            sm.refused = refused;
+        }
+        if (team.rank == 0) {
+            int* out = a.tokens_out + static_cast<u64>(seq) * (a.drafts + 1);
+            if (lane < n) out[lane] = token;
+            for (u32 i = n + 1 + lane; i <= a.drafts; i += 32) out[i] = -1;
+            if (lane == 0) {
+                a.accepted[seq] = static_cast<int>(n);
+                if (a.lengths_out) a.lengths_out[seq] = a.lengths[seq] - static_cast<int>(count - n);
+            }
+        }
+    }
+    __syncthreads();
+    const u32 accepted = sm.accepted;
+    const bool rejected = accepted < sm.count;
+    const T* p = target + static_cast<i64>(accepted) * a.target_token;
+    const T* q = rejected && a.draft ? draft + static_cast<i64>(accepted) * a.draft_token : nullptr;
+    const u32 refused = rejected && !a.draft ? static_cast<u32>(sm.refused) : ~0u;
+    auto bounds = [&](u32 segment, u32& from, u32& end) {
+        const u64 at = static_cast<u64>(team.rank * kVerifyWarps + segment) * a.segment;
+        from = static_cast<u32>(min(at, static_cast<u64>(a.vocab)));
+        end = static_cast<u32>(min(at + a.segment, static_cast<u64>(a.vocab)));
+    };
+    u32 from, end;
+    bounds(warp, from, end);
+    Sums s = q ? sum_segment<T, kWide, true>(p, q, from, end) : sum_segment<T, kWide, false>(p, q, from, end);
+    s.left = warp_sum(s.left);
+    s.target = warp_sum(s.target);
+    if (lane == 0) {
+        if (refused >= from && refused < end) s.left -= static_cast<u64>(whole(to_float(p[refused])));
+        sm.warp_left[warp] = s.left;
+        sm.warp_target[warp] = s.target;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const u64 l = warp_sum(lane < kVerifyWarps ? sm.warp_left[lane] : 0);
+        const u64 t = warp_sum(lane < kVerifyWarps ? sm.warp_target[lane] : 0);
+        if (lane == 0) {
+            sm.left = l;
+            sm.target = t;
+        }
+    }
+    kv_team_sync(team);
+    if (warp == 0) {
+        u64 l = lane == 0 ? sm.left : 0, t = lane == 0 ? sm.target : 0;
+        if (size > 1) {
+            l = lane < size ? kv_peek(&sm.left, lane) : 0;
+            t = lane < size ? kv_peek(&sm.target, lane) : 0;
+        }
+        const bool alone = warp_sum(l) == 0;
+        const u64 mine = alone ? t : l, sum = warp_sum(mine), upto = warp_scan(mine);
+        const u64 before = __shfl_sync(0xffffffffu, upto - mine, static_cast<int>(size > 1 ? team.rank : 0));
+        // floor(u * sum / 2^24), sum < 2^62
+        const float at = a.sample[seq];
+        const u32 u = static_cast<u32>(fminf(fmaxf(at, 0.0f) * 16777216.0f, 16777215.0f));
+        const u64 border = (u * (sum >> 32) << 8) + (u * (sum & 0xffffffffu) >> 24);
+        // the segment of this CTA that holds it
+        const u64 weight = lane < kVerifyWarps ? (alone ? sm.warp_target[lane] : sm.warp_left[lane]) : 0;
+        const u64 inclusive = before + warp_scan(weight);
+        const bool here = sum > 0 && border < inclusive && border >= inclusive - weight;
+        const u32 who = __ballot_sync(0xffffffffu, here);
+        if (here) sm.border = border - (inclusive - weight);
+        if (lane == 0) {
+            sm.segment = who ? static_cast<u32>(__ffs(who) - 1) : kVerifyWarps;
+            sm.alone = alone;
+            if (sum == 0 && team.rank == 0) a.tokens_out[static_cast<u64>(seq) * (a.drafts + 1) + accepted] = -1;
+        }
+    }
+    kv_team_sync(team);  // nobody leaves while another may read its sums
+    if (sm.segment == kVerifyWarps) return;
+    // the segment again, a run of neighbours to a thread
+    bounds(sm.segment, from, end);
+    const u32 each = (end - from + kVerifyThreads - 1) / kVerifyThreads;
+    const u32 first = min(from + threadIdx.x * each, end), last = min(first + each, end);
+    const bool alone = sm.alone != 0;
+    auto weight_at = [&](u32 i) {
+        const i64 x = whole(to_float(p[i]));
+        if (alone) return static_cast<u64>(x);
+        if (i == refused) return u64{0};
+        const i64 d = q ? x - whole(to_float(q[i])) : x;
+        return static_cast<u64>(d > 0 ? d : 0);
+    };
+    u64 mine = 0;
+    for (u32 i = first; i < last; ++i) mine += weight_at(i);
+    const u64 upto = warp_scan(mine);
+    if (lane == 31) sm.prefix[warp] = upto;
+    __syncthreads();
+    u64 before = upto - mine;
+    for (u32 w = 0; w < warp; ++w) before += sm.prefix[w];
+    const u64 border = sm.border;
+    if (border < before || border >= before + mine) return;
+    for (u32 i = first; i < last; ++i) {
+        before += weight_at(i);
+        if (border < before) {
+            a.tokens_out[static_cast<u64>(seq) * (a.drafts + 1) + accepted] = static_cast<int>(i);
+            return;
+        }
+    }
+}
+
+template <typename T>
+bool launch(VerifyArgs& a, u32 seqs, cudaStream_t s)
+{
+    constexpr u32 N = 16 / sizeof(T);
+    auto wide = [&](const void* p, i64 seq, i64 token) {
+        return kv_aligned(p, 16) && seq % N == 0 && token % N == 0;
+    };
+    const bool all = wide(a.target, a.target_seq, a.target_token) &&
+                     (!a.draft || wide(a.draft, a.draft_seq, a.draft_token));
+    u32 team = 1;
+    while (team < kMaxTeam && static_cast<u64>(seqs) * team * 2 <= 4ull * kv_sm_count() && a.vocab / (team * 2) >= 4096)
+        team *= 2;
+    a.segment = (a.vocab + team * kVerifyWarps * 256 - 1) / (team * kVerifyWarps * 256) * 256;
+    return kv_launch(all ? verify_kernel<T, true> : verify_kernel<T, false>, dim3(seqs * team), kVerifyThreads, s, 0,
+                     team, false, a, team);
+}
+
+}  // namespace
+}  // namespace hbfb
+
+using namespace hbfb;
+
+extern "C" int hbfsim_kv_verify_v1(const hbfsim_kv_verify_batch_v1* b, void* stream)
+{
+    if (!b || b->struct_size != sizeof(*b) || b->version != HBFSIM_KV_V1_VERSION) return HBFSIM_INVALID_ARGUMENT;
+    if (b->type > HBFSIM_KV_P_F32 || b->drafts > kMaxDrafts) return HBFSIM_UNSUPPORTED;
+    if (b->seqs > kKvMaxSeqs || b->vocab == 0 || b->vocab > kMaxVocab) return HBFSIM_INVALID_ARGUMENT;
+    if (b->seqs == 0) return HBFSIM_OK;
+    if (!b->target || !b->sample || !b->accepted || !b->tokens_out || (b->drafts && (!b->tokens || !b->accept)) ||
+        (b->lengths_out && !b->lengths))
+        return HBFSIM_INVALID_ARGUMENT;
+    const u32 size = b->type == HBFSIM_KV_P_F32 ? 4 : 2;
+    if (!kv_aligned(b->target, size) || !kv_aligned(b->draft, size) || !kv_aligned(b->tokens, 4) ||
+        !kv_aligned(b->accept, 4) || !kv_aligned(b->sample, 4) || !kv_aligned(b->counts, 4) ||
+        !kv_aligned(b->lengths, 4) || !kv_aligned(b->accepted, 4) || !kv_aligned(b->tokens_out, 4) ||
+        !kv_aligned(b->lengths_out, 4))
+        return HBFSIM_INVALID_ARGUMENT;
+    VerifyArgs a{b->target, b->target_stride_seq, b->target_stride_token, b->draft, b->draft_stride_seq,
+                 b->draft_stride_token, b->tokens, b->accept, b->sample, b->counts, b->lengths, b->accepted,
+                 b->tokens_out, b->lengths_out, b->drafts, b->vocab, 0};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool ok = b->type == HBFSIM_KV_P_F32    ? launch<float>(a, b->seqs, s)
+                    : b->type == HBFSIM_KV_P_BF16 ? launch<__nv_bfloat16>(a, b->seqs, s)
+                                                  : launch<__half>(a, b->seqs, s);
+    return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
+}

@@ -9,8 +9,15 @@ One decode step of a layer is
     rest = kv_evict(score, got.weights, table, lengths, keep=...)
     reads = kv_block_reads(cache, table, pick.blocks, pick.counts, base)  # for Context.submit
 
-kv_attention without lists reads every block.  Arguments that do not fit
-raise ValueError here, or HbfsimError from the C ABI; so do keys, values and
+kv_attention without lists reads every block.  Around it:
+
+    room = kv_resize(refs, table, lengths, want)         # pages for the step's tokens, or back
+    kv_copy(cache, room.src, room.dst)                   # blocks that were shared, every layer
+    q = kv_append_rotary(cache, q, k, v, table, start, positions, rotary)  # positions turned in
+    kept = kv_verify(target, draft, tokens, accept, sample, lengths=lengths)  # drafted tokens
+    kv_fork, kv_compact                                  # children of sequences; a smaller pool
+
+Arguments that do not fit raise ValueError here, or HbfsimError from the C ABI; so do keys, values and
 queries that ask for a gradient, since there is no backward pass (inside
 torch.no_grad() they are taken as they are).  Calls are asynchronous
 on `stream` (default: torch's current stream); outputs and workspace belong
@@ -25,8 +32,10 @@ from . import _lib
 from ._lib import check
 from .api import CUDA_STREAM_LEGACY
 
-__all__ = ["KvCache", "KvAttention", "KvSelection", "KvEviction", "kv_append", "kv_attention",
-           "kv_select", "kv_evict", "kv_block_reads"]
+__all__ = ["KvCache", "KvAttention", "KvSelection", "KvEviction", "KvRotary", "KvVerified",
+           "KvResized", "KvForked", "KvCompacted", "kv_append", "kv_append_rotary", "kv_attention",
+           "kv_select", "kv_evict", "kv_block_reads", "kv_verify", "kv_resize", "kv_fork",
+           "kv_copy", "kv_compact"]
 
 # The C structures of kv_v1.h as packed bytes (no padding: 8-byte fields lie at multiples of 8);
 # _lib has the same structures field by field.
@@ -35,6 +44,11 @@ _APPEND = struct.Struct("<6I3Q4qQq2Q")
 _QUERY = struct.Struct("<8IQ3qQqQ")
 _ATTENTION = struct.Struct("<2IfI7Q")
 _EVICT = struct.Struct("<10I3Qq6Q")
+_ROTARY = struct.Struct("<6IQ2q2Qq2Q")
+_VERIFY = struct.Struct("<6IQ2qQ2q8Q")
+_RESIZE = struct.Struct("<8I3Qq6Qq5Q")
+_FORK = struct.Struct("<6I3Qq5Q")
+_COMPACT = struct.Struct("<4I3Qq2Qq6Q")
 
 
 _NO_GRADIENT = "no gradient passes through the cache: detach the tensors or call under torch.no_grad()"
@@ -57,6 +71,35 @@ class KvEviction(NamedTuple):
     lengths: object
     freed: object
     freed_counts: object
+
+
+class KvVerified(NamedTuple):
+    accepted: object
+    tokens: object
+    lengths: object
+
+
+class KvResized(NamedTuple):
+    refs: object
+    table: object
+    limits: object
+    src: object
+    dst: object
+
+
+class KvForked(NamedTuple):
+    refs: object
+    table: object
+    lengths: object
+
+
+class KvCompacted(NamedTuple):
+    refs: object
+    table: object
+    src: object
+    dst: object
+    live: object
+    where: object
 
 
 def _need(ok: bool, what: str) -> None:
@@ -176,6 +219,14 @@ def kv_append(cache: KvCache, k, v, table, start, offsets=None, stream=None) -> 
     if not _here(cache.index, stream):
         with _On(cache.index, stream):
             return kv_append(cache, k, v, table, start, offsets)
+    batch, tokens, _held = _append(cache, k, v, table, start, offsets)
+    if tokens:
+        check(_lib.load().hbfsim_kv_append_v1(cache._packed, batch, _handle(cache.index)),
+              "hbfsim_kv_append_v1")
+
+
+def _append(cache: KvCache, k, v, table, start, offsets) -> tuple:
+    """The packed append, its tokens, and what has to live until the launch (copies of k and v)."""
     import torch
     seqs, width = _check_table(cache.index, table, start, "start")
     shape = k.shape
@@ -196,15 +247,104 @@ def kv_append(cache: KvCache, k, v, table, start, offsets=None, stream=None) -> 
         at = offsets.data_ptr()
     tokens = k.shape[0]
     if tokens == 0:
-        return
+        return b"", 0, None
     k_token, k_head, k_dim = k.stride()
     v_token, v_head, v_dim = v.stride()
     _need(k_dim == 1 and v_dim == 1, "the last axis of k and v has to be contiguous")
-    batch = _APPEND.pack(_APPEND.size, 1, _type(k), seqs, width, 0, tokens, k.data_ptr(),
-                         v.data_ptr(), k_token, k_head, v_token, v_head, table.data_ptr(),
-                         table.stride(0), start.data_ptr(), at)
-    check(_lib.load().hbfsim_kv_append_v1(cache._packed, batch, _handle(cache.index)),
-          "hbfsim_kv_append_v1")
+    return _APPEND.pack(_APPEND.size, 1, _type(k), seqs, width, 0, tokens, k.data_ptr(),
+                        v.data_ptr(), k_token, k_head, v_token, v_head, table.data_ptr(),
+                        table.stride(0), start.data_ptr(), at), tokens, (k, v)
+
+
+class KvRotary:
+    """How pairs of channels turn with their positions (a view of two tensors):
+    freq (float64 [pairs], radians a position) and axis (uint8 [pairs], which
+    axis of the positions a pair follows).  A head's first 2 * pairs channels are
+    turned: channel i with i + pairs, or with `neighbours` 2i with 2i + 1."""
+
+    __slots__ = ("freq", "axis", "pairs", "neighbours", "index")
+
+    def __init__(self, freq, axis, neighbours: bool = False):
+        import torch
+        _need(freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous(),
+              "freq: float64 [pairs], contiguous")
+        _need(axis.dtype == torch.uint8 and axis.shape == freq.shape and axis.is_contiguous(),
+              "axis: uint8 [pairs], contiguous")
+        self.index = index = freq.get_device()
+        _need(index >= 0 and axis.get_device() == index,
+              "freq and axis have to be on one CUDA device")
+        self.freq, self.axis, self.neighbours = freq, axis, bool(neighbours)
+        self.pairs = freq.shape[0]
+
+    @classmethod
+    def of(cls, head_dim: int, base: float = 10000.0, rotated: int | None = None, sections=None,
+           neighbours: bool = False, device="cuda") -> "KvRotary":
+        """Frequencies base ** (-2 i / rotated) for the first `rotated` channels (default: all);
+        `sections`: how many pairs in turn follow each axis (default: all the only one)."""
+        import torch
+        rotated = head_dim if rotated is None else rotated
+        _need(0 < rotated <= head_dim and rotated % 2 == 0, "rotated: an even number of channels")
+        pairs = rotated // 2
+        sections = (pairs,) if sections is None else tuple(sections)
+        _need(1 <= len(sections) <= 4 and min(sections) >= 0 and sum(sections) == pairs,
+              "sections: one to four numbers of pairs that add up to rotated / 2")
+        freq = float(base) ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+        axis = torch.repeat_interleave(torch.arange(len(sections), dtype=torch.uint8),
+                                       torch.tensor(sections))
+        return cls(freq.to(device), axis.to(device), neighbours)
+
+
+def kv_append_rotary(cache: KvCache, q, k, v, table, start, positions, rotary: KvRotary,
+                     offsets=None, stream=None):
+    """kv_append with the keys turned by their positions on the way into the cache, and the queries
+    of the same tokens with them.
+
+    k, v, table, start, offsets: as for kv_append.  q: [seqs, n, q_heads, head_dim], or with
+    `offsets` [tokens, q_heads, head_dim], of k's type; None: keys alone.  positions: int32 [axes,
+    seqs, n], or with `offsets` [axes, tokens], 1 to 4 axes (a single one may be left out).
+    rotary: a KvRotary on the cache's device; its pairs are a multiple of head_dim / 32.
+
+    Returns the turned queries (q's type and shape; every row, rows that belong to no sequence
+    too), None without q."""
+    if not _here(cache.index, stream):
+        with _On(cache.index, stream):
+            return kv_append_rotary(cache, q, k, v, table, start, positions, rotary, offsets)
+    import torch
+    batch, tokens, _held = _append(cache, k, v, table, start, offsets)
+    lead = k.shape[:-2]
+    _need(rotary.index == cache.index, "rotary: on the cache's device")
+    axes = positions.shape[0] if positions.dim() == len(lead) + 1 else 1
+    _need(positions.dtype == torch.int32 and positions.get_device() == cache.index
+          and positions.shape[-len(lead):] == lead and positions.dim() <= len(lead) + 1
+          and 1 <= axes <= 4, "positions: int32 [axes, seqs, n] or with offsets [axes, tokens], 1 to 4 "
+          "axes, on the cache's device")
+    out, q_heads, q_at, q_token, q_head = None, 0, 0, 0, 0
+    if q is not None:
+        _need(q.dtype == k.dtype and q.get_device() == cache.index and q.dim() == len(lead) + 2
+              and q.shape[:-2] == lead and q.shape[-1] == cache.head_dim,
+              "q: [seqs, n, q_heads, head_dim] or with offsets [tokens, q_heads, head_dim], of k's "
+              "type, on the cache's device")
+        _need(not q.requires_grad or not torch.is_grad_enabled(), _NO_GRADIENT)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_heads = q.shape[-2]
+        if q_heads and tokens:
+            if offsets is None:
+                q = q.flatten(0, 1)
+            q_token, q_head, q_dim = q.stride()
+            _need(q_dim == 1, "the last axis of q has to be contiguous")
+            q_at = q.data_ptr()
+    if tokens == 0:
+        return out
+    places = positions.reshape(axes, tokens)
+    if places.stride(1) != 1 and tokens > 1:
+        places = places.contiguous()
+    packed = _ROTARY.pack(_ROTARY.size, 1, q_heads, axes, rotary.pairs, rotary.neighbours, q_at,
+                          q_token, q_head, out.data_ptr() if q_heads else 0, places.data_ptr(),
+                          places.stride(0), rotary.freq.data_ptr(), rotary.axis.data_ptr())
+    check(_lib.load().hbfsim_kv_append_rotary_v1(cache._packed, batch, packed,
+                                                 _handle(cache.index)),
+          "hbfsim_kv_append_rotary_v1")
+    return out
 
 
 def _query(cache: KvCache, q, table, lengths) -> tuple:
@@ -341,6 +481,215 @@ def kv_evict(score, weights, table, lengths, keep: int, block_tokens: int = 16, 
                         freed_counts.data_ptr())
     check(_lib.load().hbfsim_kv_evict_v1(batch, _handle(index)), "hbfsim_kv_evict_v1")
     return KvEviction(new_score, new_table, new_lengths, freed, freed_counts)
+
+
+def kv_verify(target, draft, tokens, accept, sample, counts=None, lengths=None,
+              stream=None) -> KvVerified:
+    """Drafted tokens against the target's probabilities, from given random numbers.
+
+    target: [seqs, n + 1, vocab], float32, bfloat16 or float16; draft: what they were drawn from,
+    [seqs, n, vocab] of the same type, or None for tokens that were looked up.  tokens: int32
+    [seqs, n] (n at most 32).  accept: float32 [seqs, n], sample: float32 [seqs], uniform in [0, 1).
+    counts: int32 [seqs], how many of its n drafts a sequence has (default: all).
+
+    Token i is accepted while accept * draft < target at it.  The next token is drawn with `sample`
+    from what target has over draft in the row of the first token that was not accepted (with no
+    draft: from target without that token), or from the last row where all were.  Returns accepted
+    (int32 [seqs]), tokens (int32 [seqs, n + 1]: those accepted, the next one, -1 behind) and,
+    where `lengths` (int32 [seqs], with the drafted tokens) is given, the lengths without those that
+    were not accepted; else None.  kv_resize gives back the pages behind them."""
+    index = target.get_device()
+    _need(index >= 0, "the tensors have to be on a CUDA device")
+    if not _here(index, stream):
+        with _On(index, stream):
+            return kv_verify(target, draft, tokens, accept, sample, counts, lengths)
+    import torch
+    kind = {torch.float32: _lib.KV_P_F32, torch.bfloat16: _lib.KV_P_BF16,
+            torch.float16: _lib.KV_P_F16}.get(target.dtype)
+    _need(kind is not None and target.dim() == 3 and target.shape[1] > 0 and target.shape[2] > 0,
+          "target: float32, bfloat16 or float16 [seqs, n + 1, vocab]")
+    seqs, rows, vocab = target.shape
+    n = rows - 1
+    by_seq, by_token, by_value = target.stride()
+    _need(by_value == 1 or vocab == 1, "the last axis of target has to be contiguous")
+    draft_at = draft_seq = draft_token = 0
+    if draft is not None:
+        _need(draft.dtype == target.dtype and draft.shape == (seqs, n, vocab)
+              and draft.get_device() == index and (draft.stride(2) == 1 or vocab == 1 or n == 0),
+              "draft: [seqs, n, vocab] of target's type on its device, the last axis contiguous")
+        draft_seq, draft_token, _ = draft.stride()
+        draft_at = draft.data_ptr() or 256  # 0: no draft
+    for x, of, shape, name in ((tokens, torch.int32, (seqs, n), "tokens: int32 [seqs, n]"),
+                               (accept, torch.float32, (seqs, n), "accept: float32 [seqs, n]"),
+                               (sample, torch.float32, (seqs,), "sample: float32 [seqs]"),
+                               (counts, torch.int32, (seqs,), "counts: int32 [seqs]"),
+                               (lengths, torch.int32, (seqs,), "lengths: int32 [seqs]")):
+        if x is None and (of, shape) == (torch.int32, (seqs,)):
+            continue  # counts and lengths may be left out
+        _need(x is not None and x.dtype == of and x.shape == shape and x.is_contiguous()
+              and x.get_device() == index, name + ", contiguous, on target's device")
+    _need(not (target.requires_grad or draft is not None and draft.requires_grad)
+          or not torch.is_grad_enabled(), "no gradient passes through a draw: detach the tensors or "
+          "call under torch.no_grad()")
+    out = tokens.new_empty((seqs, rows))
+    if lengths is None:
+        accepted, kept = tokens.new_empty(seqs), None
+    else:
+        accepted, kept = tokens.new_empty((2, seqs)).unbind()
+    batch = _VERIFY.pack(_VERIFY.size, 1, kind, seqs, n, vocab, target.data_ptr(), by_seq, by_token,
+                         draft_at, draft_seq, draft_token, tokens.data_ptr(), accept.data_ptr(),
+                         sample.data_ptr(), counts.data_ptr() if counts is not None else 0,
+                         lengths.data_ptr() if kept is not None else 0, accepted.data_ptr(),
+                         out.data_ptr(), kept.data_ptr() if kept is not None else 0)
+    check(_lib.load().hbfsim_kv_verify_v1(batch, _handle(index)), "hbfsim_kv_verify_v1")
+    return KvVerified(accepted, out, kept)
+
+
+def _check_pool(refs, table, index) -> None:
+    import torch
+    _need(refs.dtype == torch.int32 and refs.dim() == 1 and refs.is_contiguous()
+          and refs.get_device() == index, "refs: int32 [pages] on the table's device, contiguous")
+
+
+def kv_resize(refs, table, lengths, want, block_tokens: int = 16, freed=None, freed_counts=None,
+              inplace: bool = False, stream=None) -> KvResized:
+    """Every sequence gets or gives back pages, so that it can hold `want` tokens of which it holds
+    `lengths` (int32 [seqs] both; want 0: the sequence is finished).
+
+    refs: int32 [pages], how many table entries name a page; it is free below 1.  Entries behind
+    `want` become -1 and their pages go back, and so do listed pages (freed, freed_counts: as
+    kv_evict returns them).  Blocks that tokens from `lengths` on fall into get the lowest free
+    pages, in order of sequence and block, where they have none or share theirs with others.
+
+    Returns refs, table (new, or with `inplace` the arguments themselves, changed), limits (int32
+    [seqs]: the tokens that a sequence may be filled up to; below `want` only if pages ran out) and
+    src, dst (int32 [seqs]): the pages to copy with kv_copy before the append, for blocks that
+    were shared and go on being filled; -1 for none."""
+    index = table.get_device()
+    _need(index >= 0, "the tensors have to be on a CUDA device")
+    if not _here(index, stream):
+        with _On(index, stream):
+            return kv_resize(refs, table, lengths, want, block_tokens, freed, freed_counts, inplace)
+    import torch
+    seqs, width = _check_table(index, table, lengths, "lengths")
+    _check_table(index, table, want, "want")
+    _check_pool(refs, table, index)
+    _need(not block_tokens >> 32, "block_tokens is a count of 32 bits")
+    freed_rows = freed_width = freed_at = freed_counts_at = 0
+    if freed is not None:
+        _need(freed_counts is not None and freed.dtype == torch.int32 and freed.dim() == 2
+              and freed_counts.dtype == torch.int32 and freed_counts.shape == freed.shape[:1]
+              and freed.is_contiguous() and freed_counts.is_contiguous()
+              and freed.get_device() == index and freed_counts.get_device() == index,
+              "freed: int32 [rows, width], freed_counts: int32 [rows], contiguous, on the table's device")
+        freed_rows, freed_width = freed.shape
+        freed_at, freed_counts_at = freed.data_ptr(), freed_counts.data_ptr()
+    else:
+        _need(freed_counts is None, "freed_counts without freed")
+    if inplace:
+        new_refs, new_table = refs, table
+    else:
+        new_refs, new_table = torch.empty_like(refs), refs.new_empty((seqs, width))
+    limits, src, dst = refs.new_empty((3, seqs)).unbind()
+    head = (_RESIZE.size, 1, seqs, width, block_tokens, freed_rows, freed_width, 0, refs.shape[0],
+            refs.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(), want.data_ptr(),
+            freed_at, freed_counts_at, new_refs.data_ptr(), new_table.data_ptr(),
+            new_table.stride(0), limits.data_ptr(), src.data_ptr(), dst.data_ptr())
+    lib = _lib.load()
+    size = lib.hbfsim_kv_resize_workspace_v1(_RESIZE.pack(*head, 0, 0))
+    space = torch.empty(size, dtype=torch.uint8, device=table.device)
+    check(lib.hbfsim_kv_resize_v1(_RESIZE.pack(*head, space.data_ptr(), size), _handle(index)),
+          "hbfsim_kv_resize_v1")
+    return KvResized(new_refs, new_table, limits, src, dst)
+
+
+def kv_fork(refs, table, lengths, parents, block_tokens: int = 16, inplace: bool = False,
+            stream=None) -> KvForked:
+    """Sequences go on as children of others: row r of the new table is the row of parents[r]
+    (int32 [rows]; outside [0, seqs): an empty row), as far as its length reaches.  Rows that no
+    child goes on from give their pages back.  A block that is still filled is shared until
+    kv_resize parts it.
+
+    Returns refs (int32 [pages]; with `inplace` the argument itself, changed), the new table (int32
+    [rows, width]) and lengths (int32 [rows])."""
+    index = table.get_device()
+    _need(index >= 0, "the tensors have to be on a CUDA device")
+    if not _here(index, stream):
+        with _On(index, stream):
+            return kv_fork(refs, table, lengths, parents, block_tokens, inplace)
+    import torch
+    seqs, width = _check_table(index, table, lengths, "lengths")
+    _check_pool(refs, table, index)
+    _need(not block_tokens >> 32, "block_tokens is a count of 32 bits")
+    _need(parents.dtype == torch.int32 and parents.dim() == 1 and parents.is_contiguous()
+          and parents.get_device() == index, "parents: int32 [rows] on the table's device, contiguous")
+    rows = parents.shape[0]
+    new_refs = refs if inplace else torch.empty_like(refs)
+    new_table, new_lengths = refs.new_empty((rows, width)), refs.new_empty(rows)
+    batch = _FORK.pack(_FORK.size, 1, seqs, rows, width, block_tokens, refs.shape[0],
+                       refs.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(),
+                       parents.data_ptr(), new_refs.data_ptr(), new_table.data_ptr(),
+                       new_lengths.data_ptr())
+    check(_lib.load().hbfsim_kv_fork_v1(batch, _handle(index)), "hbfsim_kv_fork_v1")
+    return KvForked(new_refs, new_table, new_lengths)
+
+
+def kv_copy(cache: KvCache, src, dst, source: KvCache | None = None, stream=None) -> None:
+    """Page dst[i] of the cache becomes page src[i] of `source` (default: of the cache itself); src,
+    dst: int32 [n], as kv_resize and kv_compact return them.  An entry outside its pool is passed
+    over.  No page of dst may occur twice, nor among the pages that are read."""
+    if not _here(cache.index, stream):
+        with _On(cache.index, stream):
+            return kv_copy(cache, src, dst, source)
+    import torch
+    source = cache if source is None else source
+    _need(source.index == cache.index and source.kv_heads == cache.kv_heads
+          and source.head_dim == cache.head_dim and source.block_tokens == cache.block_tokens,
+          "source: pages of the same shape on the cache's device")
+    for x in (src, dst):
+        _need(x.dtype == torch.int32 and x.dim() == 1 and x.shape == src.shape
+              and x.is_contiguous() and x.get_device() == cache.index,
+              "src and dst: int32 [n], contiguous, on the cache's device")
+    check(_lib.load().hbfsim_kv_copy_v1(source._packed, cache._packed, src.data_ptr(),
+                                        dst.data_ptr(), src.shape[0], _handle(cache.index)),
+          "hbfsim_kv_copy_v1")
+
+
+def kv_compact(refs, table, inplace: bool = False, stream=None) -> KvCompacted:
+    """The pages in use move to the front of the pool: the highest goes to the lowest free page, as
+    long as there is a free one below.
+
+    Returns refs and table after the moves (new, or with `inplace` the arguments themselves,
+    changed), src and dst (int32 [pages // 2], -1 behind the moves: for kv_copy, on every layer's
+    cache), live (int32 [1]: pages in use) and where (int32 [pages]: the new place of every page in
+    use, -1 for the others; for other tables on the same pool)."""
+    index = table.get_device()
+    _need(index >= 0, "the tensors have to be on a CUDA device")
+    if not _here(index, stream):
+        with _On(index, stream):
+            return kv_compact(refs, table, inplace)
+    import torch
+    shape = table.shape
+    _need(len(shape) == 2 and table.dtype == torch.int32 and (table.stride(1) == 1 or shape[1] <= 1),
+          "table: int32 [seqs, width], rows contiguous")
+    _check_pool(refs, table, index)
+    seqs, width = shape
+    pages = refs.shape[0]
+    if inplace:
+        new_refs, new_table = refs, table
+    else:
+        new_refs, new_table = torch.empty_like(refs), refs.new_empty((seqs, width))
+    src, dst = refs.new_empty((2, pages // 2)).unbind()
+    live, where = refs.new_empty(1), torch.empty_like(refs)
+    head = (_COMPACT.size, 1, seqs, width, pages, refs.data_ptr(), table.data_ptr(),
+            table.stride(0), new_refs.data_ptr(), new_table.data_ptr(), new_table.stride(0),
+            src.data_ptr(), dst.data_ptr(), live.data_ptr(), where.data_ptr())
+    lib = _lib.load()
+    size = lib.hbfsim_kv_compact_workspace_v1(_COMPACT.pack(*head, 0, 0))
+    space = torch.empty(size, dtype=torch.uint8, device=table.device)
+    check(lib.hbfsim_kv_compact_v1(_COMPACT.pack(*head, space.data_ptr(), size), _handle(index)),
+          "hbfsim_kv_compact_v1")
+    return KvCompacted(new_refs, new_table, src, dst, live, where)
 
 
 def kv_block_reads(cache: KvCache, table, blocks, counts, base: int):

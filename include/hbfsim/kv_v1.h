@@ -110,6 +110,43 @@ typedef struct hbfsim_kv_append_batch_v1 {
 int hbfsim_kv_append_v1(const hbfsim_kv_cache_v1* cache,
                         const hbfsim_kv_append_batch_v1* batch, void* stream);
 
+/* An append whose keys are turned by their positions on the way into the
+ * cache, and the queries of the same tokens with them.
+ *
+ * A head's first 2 * pairs channels form pairs: channel i with i + pairs, or
+ * with `neighbours` 2i with 2i + 1.  Pair i of token t turns by the angle
+ *   a = positions[axis[i]][t] * freq[i]      (rounded to 64 bits)
+ * with cos a and sin a rounded to 32 bits:
+ *   (x, y) -> (x cos a - y sin a, x sin a + y cos a)
+ * every product and sum rounded to 32 bits; other channels stay.  Queries are
+ * rounded once, to the batch's type; keys go on in 32 bits as the new values of
+ * the append above.  Values are not turned.  Every row of q is turned, rows
+ * that belong to no sequence too.
+ * axes: 1 to 4 (a text's one, or time, height and width); an axis of a pair
+ * past them is read as the last.  pairs: a multiple of head_dim / 32, at most
+ * head_dim / 2.  q_heads 0: keys alone.  q_out: the batch's type, [tokens]
+ * [q_heads][head_dim], 16-byte aligned, in memory apart from the inputs. */
+typedef struct hbfsim_kv_rotary_v1 {
+    uint32_t struct_size;
+    uint32_t version;
+    uint32_t q_heads;            /* at most 65536 */
+    uint32_t axes;
+    uint32_t pairs;
+    uint32_t neighbours;         /* 0 or 1 */
+    const void* q;               /* last axis contiguous, strides in elements */
+    int64_t q_stride_token;
+    int64_t q_stride_head;
+    void* q_out;
+    const int32_t* positions;    /* [axes][tokens], rows positions_stride apart */
+    int64_t positions_stride;
+    const double* freq;          /* [pairs] */
+    const uint8_t* axis;         /* [pairs] */
+} hbfsim_kv_rotary_v1;
+
+int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache,
+                               const hbfsim_kv_append_batch_v1* batch,
+                               const hbfsim_kv_rotary_v1* rotary, void* stream);
+
 /* Queries: the newest `tokens` tokens of every sequence (at most 16);
  * lengths counts them.  Token t of sequence s is at position
  * lengths[s] - tokens + t and sees positions up to its own. */
@@ -217,6 +254,179 @@ typedef struct hbfsim_kv_evict_batch_v1 {
 } hbfsim_kv_evict_batch_v1;
 
 int hbfsim_kv_evict_v1(const hbfsim_kv_evict_batch_v1* batch, void* stream);
+
+/* Drafted tokens against the target's probabilities.  Sequence s has
+ * d = counts[s] drafted tokens (clamped to [0, drafts]; NULL: drafts).  Token
+ * i < d is accepted, as long as all before it are, if
+ *   accept[i] * draft[i][token] < target[i][token]   (in 64 bits, exactly)
+ * where `draft` NULL stands for 1 (tokens that were looked up, not drawn); a
+ * token outside [0, vocab) is not.  With a accepted, the next token is drawn
+ * from row a of the target: probabilities are read as whole multiples of
+ * 2^-40, p40 = rint(p * 2^40) (halves to even; p clamped to [0, 1], NaN as 0),
+ * with weights
+ *   max(target40 - draft40, 0)   if a < d (draft NULL: target40, and 0 for the
+ *                                token that was not accepted)
+ *   target40                     if a = d, or if the former are all 0.
+ * The next token is the least one whose inclusive sum of weights exceeds
+ * floor(u * sum / 2^24), u = floor(sample * 2^24) within [0, 2^24) (NaN as 0);
+ * -1 where every weight is 0.  Sums are whole numbers: results do not depend on
+ * their order.
+ * tokens_out: int32 [seqs][drafts + 1]: the accepted tokens, the next one, -1
+ * behind.  accepted: int32 [seqs].  lengths_out (NULL to skip): lengths - (d -
+ * a), the tokens that stay in the cache of a sequence whose `lengths` counts its
+ * drafted ones.
+ * Limits: 32 drafts, 65536 sequences, a vocabulary of 2^22. */
+enum hbfsim_kv_probability_type {
+    HBFSIM_KV_P_BF16 = 0,
+    HBFSIM_KV_P_F16 = 1,
+    HBFSIM_KV_P_F32 = 2
+};
+
+typedef struct hbfsim_kv_verify_batch_v1 {
+    uint32_t struct_size;
+    uint32_t version;
+    uint32_t type;               /* hbfsim_kv_probability_type of target and draft */
+    uint32_t seqs;
+    uint32_t drafts;
+    uint32_t vocab;
+    const void* target;          /* [seqs][drafts + 1][vocab], last axis contiguous */
+    int64_t target_stride_seq;   /* in elements */
+    int64_t target_stride_token;
+    const void* draft;           /* [seqs][drafts][vocab] or NULL */
+    int64_t draft_stride_seq;
+    int64_t draft_stride_token;
+    const int32_t* tokens;       /* [seqs][drafts] */
+    const float* accept;         /* [seqs][drafts], in [0, 1) */
+    const float* sample;         /* [seqs], in [0, 1) */
+    const int32_t* counts;       /* [seqs] or NULL */
+    const int32_t* lengths;      /* [seqs] or NULL */
+    int32_t* accepted;
+    int32_t* tokens_out;
+    int32_t* lengths_out;
+} hbfsim_kv_verify_batch_v1;
+
+int hbfsim_kv_verify_v1(const hbfsim_kv_verify_batch_v1* batch, void* stream);
+
+/* Pages.  refs (int32 [pages]) counts the table entries that name a page; a
+ * page is free while its count is below 1.  Tables are as above, of blocks of
+ * 16, 32 or 64 tokens; pages, seqs * width and the lists' entries are below
+ * 2^31.  Outputs that have an input's type and shape (refs, table) may be that
+ * input's own memory (for tables: with the same stride); everything else lies in
+ * memory apart.  Counts change by whole numbers: results do not depend on any
+ * order. */
+
+/* Every sequence gets or gives back pages, so that it can hold want[s] tokens
+ * of which it holds lengths[s] (both clamped to [0, width * block_tokens]).
+ * In this order:
+ *  - entries from block ceil(want / block_tokens) on become -1, and their pages'
+ *    counts go down by one; so do the counts of listed pages (freed: int32
+ *    [freed_rows][freed_width], the first freed_counts[...] of a row, as an
+ *    eviction gives them; NULL: none).
+ *  - if want > lengths, blocks from floor(lengths / block_tokens) on are asked
+ *    for.  One without a page claims a free page; so does one whose page has a
+ *    count above 1, unless the call asks for that page as often as it is
+ *    counted and no later sequence does: then it stays.
+ *  - claims are served in order of sequence and block by the free pages in
+ *    ascending order.  The new page is counted once, a page that was left goes
+ *    down by one.  Where the first asked block holds earlier tokens and left its
+ *    page, src[s] and dst[s] say what to copy (hbfsim_kv_copy_v1, for every
+ *    layer, before the append); else they are -1.
+ * limits[s]: the tokens that sequence s may now be filled up to: want, or, where
+ * free pages ran out, the beginning of its first block that was not served (a
+ * page that stays is not served where one claim before it was not), but no less
+ * than lengths.  Blocks that were not served stay as they were. */
+typedef struct hbfsim_kv_resize_batch_v1 {
+    uint32_t struct_size;
+    uint32_t version;
+    uint32_t seqs;
+    uint32_t width;
+    uint32_t block_tokens;
+    uint32_t freed_rows;
+    uint32_t freed_width;
+    uint32_t reserved;
+    uint64_t pages;
+    const int32_t* refs;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* want;
+    const int32_t* freed;
+    const int32_t* freed_counts;
+    int32_t* refs_out;
+    int32_t* table_out;
+    int64_t table_out_stride;
+    int32_t* limits;
+    int32_t* src;
+    int32_t* dst;
+    void* workspace;
+    uint64_t workspace_bytes;
+} hbfsim_kv_resize_batch_v1;
+
+uint64_t hbfsim_kv_resize_workspace_v1(const hbfsim_kv_resize_batch_v1* batch);
+int hbfsim_kv_resize_v1(const hbfsim_kv_resize_batch_v1* batch, void* stream);
+
+/* Sequences go on as children of others: row r of the new table (int32
+ * [rows][width]) is the row of parents[r], as far as its length reaches and -1
+ * behind, or empty where parents[r] is outside [0, seqs).  Every entry of the old
+ * table gives its page's count back, every entry of the new one takes one; a
+ * block that is still filled is shared until hbfsim_kv_resize_v1 parts it.
+ * lengths_out: int32 [rows].  table_out lies in memory apart from table. */
+typedef struct hbfsim_kv_fork_batch_v1 {
+    uint32_t struct_size;
+    uint32_t version;
+    uint32_t seqs;
+    uint32_t rows;
+    uint32_t width;
+    uint32_t block_tokens;
+    uint64_t pages;
+    const int32_t* refs;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* parents;      /* [rows] */
+    int32_t* refs_out;
+    int32_t* table_out;          /* [rows][width] */
+    int32_t* lengths_out;
+} hbfsim_kv_fork_batch_v1;
+
+int hbfsim_kv_fork_v1(const hbfsim_kv_fork_batch_v1* batch, void* stream);
+
+/* Pages in use move to the front: with n of them, the highest at or past n goes
+ * to the lowest free page, the next highest to the next.  src, dst (int32 [pages
+ * / 2]): the moves in that order, -1 behind; live (int32 [1]): n; where (int32
+ * [pages]): the place of every page in use, -1 for the others.  refs_out: the
+ * counts at the new places, 0 from n on.  Entries of the table that name a page
+ * become its new place (-1 for a free one); others stay. */
+typedef struct hbfsim_kv_compact_batch_v1 {
+    uint32_t struct_size;
+    uint32_t version;
+    uint32_t seqs;
+    uint32_t width;
+    uint64_t pages;
+    const int32_t* refs;
+    const int32_t* table;
+    int64_t table_stride;
+    int32_t* refs_out;
+    int32_t* table_out;
+    int64_t table_out_stride;
+    int32_t* src;
+    int32_t* dst;
+    int32_t* live;
+    int32_t* where;
+    void* workspace;
+    uint64_t workspace_bytes;
+} hbfsim_kv_compact_batch_v1;
+
+uint64_t hbfsim_kv_compact_workspace_v1(const hbfsim_kv_compact_batch_v1* batch);
+int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* batch, void* stream);
+
+/* Contents of pages: page dst[i] of `to` becomes page src[i] of `from` (data,
+ * scale and bounds; the caches may be one) for i < count.  An entry outside its
+ * pool, on either side, is passed over.  No page of dst may occur twice, nor
+ * among the pages of src if the caches are one. */
+int hbfsim_kv_copy_v1(const hbfsim_kv_cache_v1* from,
+                      const hbfsim_kv_cache_v1* to, const int32_t* src,
+                      const int32_t* dst, uint64_t count, void* stream);
 
 #ifdef __cplusplus
 }

@@ -180,3 +180,159 @@ def evict(score, weights, table, lengths, keep, block, sink, recent, decay):
         freed[b, :leave] = table[b, sorted(gone)]
         counts[b], out_l[b] = leave, length - leave * block
     return out_s, out_t, out_l, freed, counts
+
+
+def rotate(x, positions, freq, axis, neighbours):
+    """x: float32 [tokens, heads, D], positions: [axes, tokens].  Angles, sines and cosines in 64
+    bits; sines, cosines, products and sums rounded to 32."""
+    x = np.asarray(x, np.float32)
+    out = x.copy()
+    pairs = len(freq)
+    for i in range(pairs):
+        a = positions[min(int(axis[i]), len(positions) - 1)].astype(np.float64) * freq[i]
+        c, s = (f(a).astype(np.float32)[:, None] for f in (np.cos, np.sin))
+        m, n = (2 * i, 2 * i + 1) if neighbours else (i, i + pairs)
+        out[:, :, m] = x[:, :, m] * c - x[:, :, n] * s
+        out[:, :, n] = x[:, :, m] * s + x[:, :, n] * c
+    return out
+
+
+def _p40(p):
+    """A probability in whole multiples of 2^-40, halves to even."""
+    p = float(p)
+    return 0 if p != p else round(min(max(p, 0.0), 1.0) * 2.0 ** 40)
+
+
+def verify(target, draft, tokens, accept, sample, counts, lengths):
+    """Python's whole numbers and fractions throughout.  Returns accepted, tokens, lengths."""
+    from fractions import Fraction
+    seqs, rows, vocab = target.shape
+    n = rows - 1
+    accepted, out, kept = [], np.full((seqs, rows), -1, np.int32), []
+    for b in range(seqs):
+        d = min(max(int(counts[b]), 0), n)
+        a = 0
+        while a < d:
+            t = int(tokens[b, a])
+            if not 0 <= t < vocab:
+                break
+            p, u = float(target[b, a, t]), float(accept[b, a])
+            q = 1.0 if draft is None else float(draft[b, a, t])
+            if all(np.isfinite([p, u, q])):
+                good = Fraction(u) * Fraction(q) < Fraction(p)
+            else:  # as 64-bit numbers compare: a NaN accepts nothing
+                good = u * q < p
+            if not good:
+                break
+            a += 1
+        whole = [_p40(p) for p in target[b, a]]
+        left = list(whole)
+        if a < d:
+            if draft is not None:
+                left = [max(p - _p40(q), 0) for p, q in zip(whole, draft[b, a])]
+            elif 0 <= int(tokens[b, a]) < vocab:
+                left[int(tokens[b, a])] = 0
+        if sum(left) == 0:
+            left = whole
+        out[b, :a] = tokens[b, :a]
+        if sum(left):
+            s = float(sample[b])
+            u = 0 if s != s else min(max(int(min(max(s, -1.0), 2.0) * 2 ** 24), 0), 2 ** 24 - 1)
+            border = u * sum(left) >> 24
+            total = 0
+            for i, w in enumerate(left):
+                total += w
+                if total > border:
+                    out[b, a] = i
+                    break
+        accepted.append(a)
+        kept.append(int(lengths[b]) - (d - a))
+    return np.array(accepted, np.int32), out, np.array(kept, np.int32)
+
+
+def resize(refs, table, lengths, want, block, freed=None, freed_counts=None):
+    """One claim after the other.  Returns refs, table, limits, src, dst."""
+    refs, table = refs.astype(np.int64).copy(), table.copy()
+    pages, (seqs, width) = len(refs), table.shape
+    real = lambda p: 0 <= p < pages  # noqa: E731
+    held = [min(max(int(x), 0), width * block) for x in lengths]
+    goal = [min(max(int(x), 0), width * block) for x in want]
+    need = [-(-g // block) for g in goal]
+    for b in range(seqs):
+        for j in range(need[b], width):
+            if real(table[b, j]):
+                refs[table[b, j]] -= 1
+            table[b, j] = -1
+    if freed is not None:
+        for row, count in zip(freed, freed_counts):
+            for p in row[:max(0, int(count))]:
+                if real(p):
+                    refs[p] -= 1
+    start = refs.copy()
+    asked = [(b, j) for b in range(seqs) if goal[b] > held[b] for j in range(held[b] // block, need[b])]
+    by_page = {}
+    for b, j in asked:
+        p = int(table[b, j])
+        if real(p) and start[p] > 1:
+            by_page.setdefault(p, []).append(b)
+    free = [p for p in range(pages) if start[p] < 1]
+    limits, src, dst = list(goal), np.full(seqs, -1, np.int32), np.full(seqs, -1, np.int32)
+    claims = 0
+    for b, j in asked:
+        p = int(table[b, j])
+        shared = real(p) and start[p] > 1
+        if real(p) and not shared:
+            continue
+        if shared and len(by_page[p]) >= start[p] and max(by_page[p]) == b:
+            served = claims <= len(free)
+        else:
+            served = claims < len(free)
+            if served:
+                new = free[claims]
+                refs[new] = 1
+                table[b, j] = new
+                if shared:
+                    refs[p] -= 1
+                    if j == held[b] // block and held[b] % block:
+                        src[b], dst[b] = p, new
+            claims += 1
+        if not served:
+            limits[b] = min(limits[b], max(held[b], j * block))
+    return refs.astype(np.int32), table, np.array(limits, np.int32), src, dst
+
+
+def fork(refs, table, lengths, parents, block):
+    """Returns refs, table, lengths."""
+    refs = refs.astype(np.int64).copy()
+    pages, (seqs, width) = len(refs), table.shape
+    new = np.full((len(parents), width), -1, np.int32)
+    kept = np.zeros(len(parents), np.int32)
+    for r, s in enumerate(parents):
+        if 0 <= s < seqs:
+            kept[r] = min(max(int(lengths[s]), 0), width * block)
+            many = -(-int(kept[r]) // block)
+            new[r, :many] = table[s, :many]
+    for t, by in ((new, 1), (table, -1)):
+        for p in t.ravel():
+            if 0 <= p < pages:
+                refs[p] += by
+    return refs.astype(np.int32), new, kept
+
+
+def compact(refs, table):
+    """Returns refs, table, src, dst, live, where."""
+    pages = len(refs)
+    used = [p for p in range(pages) if refs[p] > 0]
+    n = len(used)
+    holes = [p for p in range(n) if refs[p] <= 0]
+    movers = [p for p in reversed(used) if p >= n]
+    src, dst = (np.full(pages // 2, -1, np.int32) for _ in range(2))
+    src[:len(movers)], dst[:len(holes)] = movers, holes
+    where = np.full(pages, -1, np.int32)
+    where[used] = used
+    where[movers] = holes
+    new_refs = np.zeros(pages, np.int32)
+    for p in used:
+        new_refs[where[p]] = refs[p]
+    new_table = np.array([[where[p] if 0 <= p < pages else p for p in row] for row in table], np.int32)
+    return new_refs, new_table.reshape(table.shape), src, dst, np.array([n], np.int32), where
