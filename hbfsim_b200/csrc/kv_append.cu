@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, D == 256 ? 3 : 6) append_ke
 {
     const u32 pair = blockIdx.y * kAppendWarps + (threadIdx.x >> 5), head = pair >> 1, side = pair & 1u;
     if (head >= a.c.heads) return;
-    const Lead mine = lead_of(a);
+    const Lead mine = lead_of(a, blockIdx.x);
     for (u32 left = __ballot_sync(0xffffffffu, mine.leads); left; left &= left - 1) {
         const int who = __ffs(left) - 1;
         const u32 its_token = blockIdx.x * a.chunk + static_cast<u32>(who);

@@ -404,15 +404,15 @@ struct Lead {
     u32 slot, count;  // tokens that the block held before, new ones
 };
 
-__device__ __forceinline__ Lead lead_of(const AppendArgs& a)
+__device__ __forceinline__ Lead lead_of(const AppendArgs& a, u32 chunk)
 {
     const u32 lane = threadIdx.x & 31u;
-    const i64 token = static_cast<i64>(blockIdx.x) * a.chunk + lane;
+    const i64 token = static_cast<i64>(chunk) * a.chunk + lane;
     bool leads = lane < a.chunk && token < a.tokens;
     int page = -1;
     u32 slot = 0, count = 0, seq_first = 0, seq_last = 0;
     if (a.offsets) {  // sequences of the chunk's first and last token
-        const i64 base = static_cast<i64>(blockIdx.x) * a.chunk;
+        const i64 base = static_cast<i64>(chunk) * a.chunk;
         seq_first = sequence_of(a, base);
         seq_last = a.chunk > 1 ? sequence_of(a, min(base + a.chunk, static_cast<i64>(a.tokens)) - 1) : seq_first;
     }

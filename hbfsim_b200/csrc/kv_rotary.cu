@@ -1,21 +1,23 @@
 // kv_rotary.cu -- new tokens into the 8-bit paged cache with keys and queries
 // turned by their positions (kv_v1.h).
 //
-// A CTA takes a chunk of tokens.  It makes the cosines and sines of all pairs
-// once, in shared memory, and its warps turn rows with them: eight heads of a
-// token's queries at a time, and the blocks that begin in the chunk, a warp per
-// head and side as in kv_append.cu.  The keys never exist in 16 bits: a block of
-// new tokens alone is read and turned twice, for the largest magnitude and for the
-// stored values (the second time from the L1 cache).  Products and
-// sums are rounded one by one, so that what is stored does not depend on how a
-// compiler joins them.
+// One launch, three kinds of CTA.  Keys: a chunk of tokens as in kv_append.cu, whose
+// blocks' cosines and sines are made once, in shared memory; a warp turns a head's
+// rows of a block twice, for the largest magnitude and for the stored values (the
+// second time from the caches), so the keys never exist in 16 bits.  Values: as in
+// kv_append.cu.  Queries: every warp by itself.  It takes a token's heads, asks for
+// the first rows, makes the token's cosines and sines meanwhile, and reads the next
+// rows while it turns the ones at hand.  Keys and values come first: their CTAs take
+// longest (mixed with the queries' the call took as long).  Products and sums are
+// rounded one by one, so that what is stored does not depend on how a compiler joins
+// them.
 #include "kv_append.cuh"
 
 namespace hbfb {
 namespace {
 
 constexpr u32 kRotaryWarps = 4;
-constexpr u32 kRotaryHeads = 8;  // query heads of a token that a warp has in registers
+constexpr u32 kRotaryHeads = 8;  // query heads that a warp reads at a time
 constexpr u32 kMaxAxes = 4;
 
 struct RotaryArgs {
@@ -28,7 +30,9 @@ struct RotaryArgs {
     const double* freq;
     const u8* axis;
     u32 q_heads, axes, pairs;
-    bool append;  // whether any block is there
+    // thread blocks for keys, then for values, so many to a chunk; the others are for queries
+    u32 key_blocks, key_spread, value_blocks, value_spread;
+    u32 parts, part;  // warps to a token's queries, groups of heads of each
 };
 
 // sin and cos in 64 bits, rounded to 32.  Cody and Waite's reduction by multiples of pi/2 in two
@@ -38,9 +42,12 @@ __device__ __forceinline__ void sine(double angle, float& sin32, float& cos32)
 {
     double s, c;
     if (fabs(angle) < 1073741824.0) {
-        const double k = rint(angle * 0.63661977236758134);  // 2 / pi
-        double r = fma(-k, 1.5707963267948966, angle);       // pi / 2 ...
-        r = fma(-k, 6.123233995736766e-17, r);               // ... and the rest of it
+        // the nearest whole number of quarter turns: added to 1.5 * 2^52, it is the sum's last bits
+        const double shifted = fma(angle, 0.63661977236758134, 6755399441055744.0);  // 2 / pi
+        const double k = shifted - 6755399441055744.0;
+        const int quarter = __double2loint(shifted);
+        double r = fma(-k, 1.5707963267948966, angle);  // pi / 2 ...
+        r = fma(-k, 6.123233995736766e-17, r);          // ... and the rest of it
         const double z = r * r;
         s = fma(z, fma(z, fma(z, fma(z, fma(z, fma(z, -1.0 / 1307674368000.0, 1.0 / 6227020800.0), -1.0 / 39916800.0),
                                      1.0 / 362880.0), -1.0 / 5040.0), 1.0 / 120.0), -1.0 / 6.0);
@@ -48,7 +55,6 @@ __device__ __forceinline__ void sine(double angle, float& sin32, float& cos32)
         c = fma(z, fma(z, fma(z, fma(z, fma(z, fma(z, -1.0 / 87178291200.0, 1.0 / 479001600.0), -1.0 / 3628800.0),
                                      1.0 / 40320.0), -1.0 / 720.0), 1.0 / 24.0), -0.5);
         c = fma(z, c, 1.0);
-        const int quarter = static_cast<int>(k);
         const double t = s;
         if (quarter & 1) {
             s = c;
@@ -63,84 +69,26 @@ __device__ __forceinline__ void sine(double angle, float& sin32, float& cos32)
     cos32 = static_cast<float>(c);
 }
 
-// What a lane needs to turn its channels of a row: its cosines and (signed) sines for a token.
-template <int D, bool kNeighbours>
-struct Turn {
-    static constexpr int W = D / 64;
-    bool turns;   // whether the lane's channels are among the pairs
-    u32 first;    // its first pair
-    int partner;  // the lane that has the other channels
-    bool minus;
-    float c[2 * W], s[2 * W];
+__device__ __forceinline__ void circle_at(const RotaryArgs& r, u32 token, u32 pair, float& sin32, float& cos32)
+{
+    const u32 axis = min(static_cast<u32>(r.axis[pair]), r.axes - 1);
+    const int position = r.positions[static_cast<i64>(axis) * r.positions_stride + token];
+    sine(__dmul_rn(static_cast<double>(position), r.freq[pair]), sin32, cos32);
+}
 
-    __device__ __forceinline__ explicit Turn(u32 pairs)
-    {
-        const u32 lane = threadIdx.x & 31u;
-        if constexpr (kNeighbours) {
-            turns = lane < pairs / W;
-            first = turns ? lane * W : 0;
-            partner = static_cast<int>(lane);
-            minus = false;
-        } else {
-            const u32 lanes = pairs / (2 * W);
-            turns = lane < 2 * lanes;
-            minus = lane < lanes;
-            partner = static_cast<int>(!turns ? lane : minus ? lane + lanes : lane - lanes);
-            first = turns ? (minus ? lane : lane - lanes) * 2 * W : 0;
-        }
-    }
+// Two products in 32 bits at once; sums one by one: a sum of two at once after them is joined with
+// a product into one rounding, whatever the instructions say.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    u64 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(r)
+        : "l"(*reinterpret_cast<u64*>(&a)), "l"(*reinterpret_cast<u64*>(&b)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
 
-    __device__ __forceinline__ void load(const float* cosines, const float* sines)
-    {
-        constexpr int N = kNeighbours ? W : 2 * W;
-        float x[N], y[N];
-        read<N>(cosines + first, x);
-        read<N>(sines + first, y);
-#pragma unroll
-        for (int i = 0; i < 2 * W; ++i) {
-            c[i] = x[kNeighbours ? i / 2 : i];
-            s[i] = y[kNeighbours ? i / 2 : i];
-            if (kNeighbours ? i % 2 == 0 : minus) s[i] = -s[i];
-        }
-    }
-
-    // A row's channels of the lane, turned, in 32 bits.
-    template <typename T>
-    __device__ __forceinline__ void apply(const u32 (&raw)[W], float2 (&y)[W]) const
-    {
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 x = Pair<T>::floats(raw[w]);
-            float2 p = make_float2(x.y, x.x);
-            if constexpr (!kNeighbours) p = Pair<T>::floats(__shfl_sync(0xffffffffu, raw[w], partner));
-            y[w].x = __fadd_rn(__fmul_rn(x.x, c[2 * w]), __fmul_rn(p.x, s[2 * w]));
-            y[w].y = __fadd_rn(__fmul_rn(x.y, c[2 * w + 1]), __fmul_rn(p.y, s[2 * w + 1]));
-            if (!turns) y[w] = x;
-        }
-    }
-
-private:
-    template <int N>
-    static __device__ __forceinline__ void read(const float* from, float (&x)[N])
-    {
-        if constexpr (N == 1) {
-            x[0] = *from;
-        } else if constexpr (N == 2) {
-            const float2 y = *reinterpret_cast<const float2*>(from);
-            x[0] = y.x;
-            x[1] = y.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                const float4 y = *reinterpret_cast<const float4*>(from + i);
-                x[i] = y.x;
-                x[i + 1] = y.y;
-                x[i + 2] = y.z;
-                x[i + 3] = y.w;
-            }
-        }
-    }
-};
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return make_float2(__fsub_rn(a.x, b.x), __fsub_rn(a.y, b.y)); }
 
 __device__ __forceinline__ u32 packed(float2 x, __nv_bfloat16)
 {
@@ -153,227 +101,462 @@ __device__ __forceinline__ u32 packed(float2 x, __half)
     return *reinterpret_cast<const u32*>(&y);
 }
 
-template <int W>
-__device__ __forceinline__ void store_row(u16* to, const u32 (&x)[W])
+// N words of two elements or of two numbers.
+template <int N, bool kWide>
+__device__ __forceinline__ void load_words(const u16* from, u32 (&x)[N])
 {
-    if constexpr (W == 1) *reinterpret_cast<u32*>(to) = x[0];
-    else if constexpr (W == 2) *reinterpret_cast<uint2*>(to) = make_uint2(x[0], x[1]);
+    load_row<N, kWide>(from, x);
+}
+template <int N>
+__device__ __forceinline__ void store_words(u16* to, const u32 (&x)[N])
+{
+    if constexpr (N == 1) *reinterpret_cast<u32*>(to) = x[0];
+    else if constexpr (N == 2) *reinterpret_cast<uint2*>(to) = make_uint2(x[0], x[1]);
     else *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
 }
+template <int N>
+__device__ __forceinline__ void load_floats(const float* from, float2 (&x)[N])
+{
+    if constexpr (N == 1) {
+        x[0] = *reinterpret_cast<const float2*>(from);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float4 y = *reinterpret_cast<const float4*>(from + 2 * i);
+            x[i] = make_float2(y.x, y.y);
+            x[i + 1] = make_float2(y.z, y.w);
+        }
+    }
+}
+
+// Half a warp takes a row: a lane has V neighbouring pairs, that is, V channels at `lo` and V at
+// `hi`.  Channels i and i + pairs are in one lane that way, and a warp turns two rows at once.
+// Lanes past the pairs carry the channels that stay.
+enum Layout { kSplit, kNeighbours, kWhole };  // i with i + pairs; 2i with 2i + 1; i with i + D / 2
+template <int D, int kLayout>
+struct Lane {
+    static constexpr int V = D / 32, N = V / 2;
+    u32 lo, hi, pair;
+    bool turns;
+
+    __device__ __forceinline__ explicit Lane(u32 pairs)
+    {
+        pair = (threadIdx.x & 15u) * V;
+        turns = kLayout == kWhole || pair < pairs;
+        lo = kLayout == kNeighbours || !turns ? 2 * pair : pair;
+        hi = lo + (kLayout == kWhole ? D / 2 : kLayout == kNeighbours || !turns ? V : pairs);
+        if (!turns) pair = 0;
+    }
+
+    struct Circle {
+        float2 c[N], s[N];
+    };
+    __device__ __forceinline__ void load(const float* cosines, const float* sines, Circle& a) const
+    {
+        load_floats<N>(cosines + pair, a.c);
+        load_floats<N>(sines + pair, a.s);
+    }
+    // The same made here: the two lanes that turn by the same pairs make half of them each.
+    __device__ __forceinline__ void make(const RotaryArgs& r, u32 token, Circle& a) const
+    {
+        const u32 half = (threadIdx.x & 31u) >> 4;
+        float c[N], s[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            c[i] = s[i] = 0.0f;
+            if (turns) circle_at(r, token, pair + half * N + i, s[i], c[i]);
+        }
+        float* all_c = reinterpret_cast<float*>(a.c);
+        float* all_s = reinterpret_cast<float*>(a.s);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float oc = __shfl_xor_sync(0xffffffffu, c[i], 16), os = __shfl_xor_sync(0xffffffffu, s[i], 16);
+            all_c[i] = half ? oc : c[i];
+            all_c[N + i] = half ? c[i] : oc;
+            all_s[i] = half ? os : s[i];
+            all_s[N + i] = half ? s[i] : os;
+        }
+    }
+
+    // The lane's channels at lo (x) and hi (y) in 32 bits, turned.
+    template <typename T>
+    __device__ __forceinline__ void apply(const u32 (&low)[N], const u32 (&high)[N], const Circle& a, float2 (&x)[N],
+                                          float2 (&y)[N]) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = Pair<T>::floats(low[i]);
+            y[i] = Pair<T>::floats(high[i]);
+        }
+        if (!turns) return;
+        if constexpr (kLayout == kNeighbours) {
+            float2 p[2 * N];  // pairs of channels
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                p[i] = x[i];
+                p[N + i] = y[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * N; ++i) {
+                const float c = i & 1 ? a.c[i / 2].y : a.c[i / 2].x, s = i & 1 ? a.s[i / 2].y : a.s[i / 2].x;
+                p[i] = add2(mul2(p[i], make_float2(c, c)), mul2(make_float2(p[i].y, p[i].x), make_float2(-s, s)));
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[i] = p[i];
+                y[i] = p[N + i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float2 m = sub2(mul2(x[i], a.c[i]), mul2(y[i], a.s[i]));
+                y[i] = add2(mul2(x[i], a.s[i]), mul2(y[i], a.c[i]));
+                x[i] = m;
+            }
+        }
+    }
+};
 
 // The cosines and sines in shared memory: [tokens of the CTA][pairs] each.
-struct Circle {
+struct Table {
     const float* cosines;
     const float* sines;
     u32 pairs;
 };
 
-// A head's new keys, turned: the `row` of append_block; `circle` begins with the block's first new
-// token.
-template <typename T, int D, bool kWide, bool kNeighbours>
+// A head's new keys, turned: the `row` of append_block, a lane's channels side by side; `table`
+// begins with the block's first new token.
+template <typename T, int D, bool kWide, int kLayout>
 struct TurnedRow {
     static constexpr int W = D / 64;
-    const u16* x;
+    const u16* x;  // the lane's channels of the first token
     i64 stride;
-    Circle circle;
+    Table table;
     __device__ __forceinline__ void operator()(u32 t, float2 (&y)[W]) const
     {
-        u32 raw[W];
+        const u32 channel = (threadIdx.x & 31u) * 2 * W, pairs = table.pairs;
+        const bool turns = channel < 2 * pairs, second = channel >= pairs;
+        const u32 pair = !turns ? 0 : kLayout == kNeighbours ? channel / 2 : second ? channel - pairs : channel;
+        const float* c = table.cosines + t * pairs + pair;
+        const float* s = table.sines + t * pairs + pair;
+        u32 raw[W], other[W];
         load_row<W, kWide>(x + t * stride, raw);
-        Turn<D, kNeighbours> turn(circle.pairs);
-        turn.load(circle.cosines + t * circle.pairs, circle.sines + t * circle.pairs);
-        turn.template apply<T>(raw, y);
+        const int away = kLayout == kNeighbours || !turns ? 0 : second ? -static_cast<int>(pairs) : static_cast<int>(pairs);
+        load_row<W, kWide>(x + t * stride + away, other);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            y[w] = Pair<T>::floats(raw[w]);
+            if (!turns) continue;
+            float2 p = Pair<T>::floats(other[w]), cc, ss;
+            if constexpr (kLayout == kNeighbours) {
+                p = make_float2(p.y, p.x);
+                cc = make_float2(c[w], c[w]);
+                ss = make_float2(-s[w], s[w]);
+            } else {
+                cc = make_float2(c[2 * w], c[2 * w + 1]);
+                ss = make_float2(s[2 * w], s[2 * w + 1]);
+                if (!second) ss = make_float2(-ss.x, -ss.y);
+            }
+            y[w] = add2(mul2(y[w], cc), mul2(p, ss));
+        }
     }
 };
+
+// The lesser and the greater of two, NaN if either is.
+__device__ __forceinline__ float least_of(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float greatest_of(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// N words of two stored values.
+template <int N>
+__device__ __forceinline__ void store_values(u8* to, const u32 (&b)[N])
+{
+    if constexpr (N == 1) *reinterpret_cast<u16*>(to) = static_cast<u16>(b[0]);
+    else if constexpr (N == 2) *reinterpret_cast<u32*>(to) = b[0] | b[1] << 16;
+    else *reinterpret_cast<uint2*>(to) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+}
 
 // A head's keys of a block whose tokens are all new, by one warp; false, with nothing written, where
 // a turned element is not finite.  Rounding keeps the order, so the least and greatest of a channel
 // give its bounds.
-template <typename T, int D, bool kWide, bool kNeighbours>
+template <typename T, int D, bool kWide, int kLayout>
 __device__ __forceinline__ bool append_full_turned(const AppendArgs& a, u32 head, u32 token, int page,
-                                                   const Circle& circle)
+                                                   const Table& table)
 {
-    constexpr int W = D / 64;
-    const u32 lane = threadIdx.x & 31u, block = a.c.block;
+    using Of = Lane<D, kLayout>;
+    constexpr int N = Of::N;
+    constexpr u32 R = 4;  // steps of two rows at a time
+    const Of mine(table.pairs);
+    const u32 half = (threadIdx.x & 31u) >> 4, block = a.c.block;
     const i64 stride = a.stride_token[0];
-    const u16* x = static_cast<const u16*>(a.x[0]) + static_cast<i64>(token) * stride +
-                   static_cast<i64>(head) * a.stride_head[0] + lane * 2 * W;
+    const u16* x = static_cast<const u16*>(a.x[0]) + (static_cast<i64>(token) + half) * stride +
+                   static_cast<i64>(head) * a.stride_head[0];
     const u64 at = (static_cast<u64>(page) * a.c.heads + head) * 2;
-    constexpr u32 R = 8;  // rows at a time
-    u32 raw[R][W];
-    float2 lo[W], hi[W];
-    auto load_rows = [&](u32 row0) {
-#pragma unroll
-        for (u32 r = 0; r < R; ++r) load_row<W, kWide>(x + (row0 + r) * stride, raw[r]);
-    };
-    Turn<D, kNeighbours> turn(circle.pairs);
-    auto turned = [&](u32 row0, u32 r, float2 (&y)[W]) {
-        turn.load(circle.cosines + (row0 + r) * circle.pairs, circle.sines + (row0 + r) * circle.pairs);
-        turn.template apply<T>(raw[r], y);
-    };
-    load_rows(0);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        lo[w] = make_float2(3.402823466e38f, 3.402823466e38f);
-        hi[w] = make_float2(-3.402823466e38f, -3.402823466e38f);
-    }
-    bool finite = true;
-    for (u32 row0 = 0;;) {
+    // turned: the channels at mine.lo and at mine.hi (16 rows held from the first time on, and 16
+    // warps on an SM instead of 24, took 149 us for prompts that take 136)
+    float2 y[R][2][N];
+    auto turn_rows = [&](u32 row0) {
+        u32 low[R][N], high[R][N];
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
-            float2 y[W];
-            turned(row0, r, y);
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                finite &= fabsf(y[w].x) <= 3.402823466e38f && fabsf(y[w].y) <= 3.402823466e38f;
-                lo[w] = make_float2(fminf(lo[w].x, y[w].x), fminf(lo[w].y, y[w].y));
-                hi[w] = make_float2(fmaxf(hi[w].x, y[w].x), fmaxf(hi[w].y, y[w].y));
-            }
+            load_words<N, kWide>(x + (row0 + 2 * r) * stride + mine.lo, low[r]);
+            load_words<N, kWide>(x + (row0 + 2 * r) * stride + mine.hi, high[r]);
         }
-        row0 += R;
-        if (row0 == block) break;
-        load_rows(row0);
+#pragma unroll
+        for (u32 r = 0; r < R; ++r) {
+            typename Of::Circle circle;
+            const u32 row = (row0 + 2 * r + half) * table.pairs;
+            mine.load(table.cosines + row, table.sines + row, circle);
+            mine.template apply<T>(low[r], high[r], circle, y[r][0], y[r][1]);
+        }
+    };
+    float2 lo[2][N], hi[2][N];  // least and greatest of the channels
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            lo[k][i] = make_float2(3.402823466e38f, 3.402823466e38f);
+            hi[k][i] = make_float2(-3.402823466e38f, -3.402823466e38f);
+        }
+    for (u32 row0 = 0; row0 < block; row0 += 2 * R) {
+        turn_rows(row0);
+#pragma unroll
+        for (u32 r = 0; r < R; ++r)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float2 z = y[r][k][i];
+                    lo[k][i] = make_float2(least_of(lo[k][i].x, z.x), least_of(lo[k][i].y, z.y));
+                    hi[k][i] = make_float2(greatest_of(hi[k][i].x, z.x), greatest_of(hi[k][i].y, z.y));
+                }
     }
-    if (!__all_sync(0xffffffffu, finite)) return false;
     float most = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-        most = fmaxf(most, fmaxf(fmaxf(fabsf(lo[w].x), fabsf(lo[w].y)), fmaxf(fabsf(hi[w].x), fabsf(hi[w].y))));
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        for (int i = 0; i < N; ++i)
+            most = greatest_of(most, greatest_of(greatest_of(fabsf(lo[k][i].x), fabsf(lo[k][i].y)),
+                                                 greatest_of(fabsf(hi[k][i].x), fabsf(hi[k][i].y))));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = greatest_of(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (!(most <= 3.402823466e38f)) return false;
     const float now = kv_power(scale_exponent(most)), inverse = 1.0f / now;
-    if (lane == 0) a.c.scale[at] = now;
-    auto stored = [&](float2 y) { return store_e4m3(make_float2(y.x * inverse, y.y * inverse)); };
-    u8* out = a.c.data + at * block * D + lane * 2 * W;
-    for (u32 row0 = 0;;) {
-        load_rows(row0);
+    if ((threadIdx.x & 31u) == 0) a.c.scale[at] = now;
+    auto stored = [&](float2 y) { return store_e4m3(mul2(y, make_float2(inverse, inverse))); };
+    u8* out = a.c.data + at * block * D + half * D;
+    for (u32 row0 = 0; row0 < block; row0 += 2 * R) {
+        turn_rows(row0);
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
-            float2 y[W];
-            u32 b[W];
-            turned(row0, r, y);
+            u32 b[2][N];
 #pragma unroll
-            for (int w = 0; w < W; ++w) b[w] = stored(y[w]);
-            put_row<W>(out + (row0 + r) * D, b);
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) b[k][i] = stored(y[r][k][i]);
+            store_values<N>(out + (row0 + 2 * r) * D + mine.lo, b[0]);
+            store_values<N>(out + (row0 + 2 * r) * D + mine.hi, b[1]);
         }
-        row0 += R;
-        if (row0 == block) break;
     }
-    u32 least[W], greatest[W];
+    // bounds: the lower lanes' and the upper lanes' rows together; half a warp each for the two ends
+    std::int8_t* bound = a.c.bounds + (static_cast<u64>(page) * a.c.heads + head) * 2 * D + half * D;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        least[w] = stored(lo[w]);
-        greatest[w] = stored(hi[w]);
-    }
-    put_bounds<D>(a, page, head, least, greatest);
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float2 give = half ? lo[k][i] : hi[k][i], keep = half ? hi[k][i] : lo[k][i];
+            float2 other;
+            other.x = __shfl_xor_sync(0xffffffffu, give.x, 16);
+            other.y = __shfl_xor_sync(0xffffffffu, give.y, 16);
+            const float2 end = half ? make_float2(fmaxf(keep.x, other.x), fmaxf(keep.y, other.y))
+                                    : make_float2(fminf(keep.x, other.x), fminf(keep.y, other.y));
+            const float2 z = __half22float2(stored_f16(stored(end)));
+            const float2 q = make_float2(z.x * 0.25f, z.y * 0.25f);
+            const u32 channel = (k ? mine.hi : mine.lo) + 2 * i;
+            *reinterpret_cast<char2*>(bound + channel) =
+                half ? make_char2(static_cast<signed char>(ceilf(q.x)), static_cast<signed char>(ceilf(q.y)))
+                     : make_char2(static_cast<signed char>(floorf(q.x)), static_cast<signed char>(floorf(q.y)));
+        }
     return true;
 }
 
-// Heads [head0, head0 + kRotaryHeads) of a token's queries by one warp.
-template <typename T, int D, bool kWide, bool kNeighbours>
-__device__ __forceinline__ void turn_queries(const RotaryArgs& r, u32 token, u32 head0, const Circle& circle)
+// `part` groups of heads of a token's queries by one warp.
+template <typename T, int D, bool kWide, int kLayout>
+__device__ __forceinline__ void turn_queries(const RotaryArgs& r, u32 token, u32 group)
 {
-    constexpr int W = D / 64;
-    const u32 lane = threadIdx.x & 31u;
-    const u16* x = static_cast<const u16*>(r.q) + static_cast<i64>(token) * r.q_token + lane * 2 * W;
-    u16* out = static_cast<u16*>(r.q_out) + (static_cast<u64>(token) * r.q_heads + head0) * D + lane * 2 * W;
-    u32 raw[kRotaryHeads][W];
+    using Of = Lane<D, kLayout>;
+    constexpr int N = Of::N;
+    constexpr u32 R = kRotaryHeads / 2;
+    const Of mine(r.pairs);
+    const u32 half = (threadIdx.x & 31u) >> 4, end = min(r.q_heads, (group + r.part) * kRotaryHeads);
+    u32 head = group * kRotaryHeads + half;  // the first of the lane's rows at hand
+    const u16* x = static_cast<const u16*>(r.q) + static_cast<i64>(token) * r.q_token +
+                   static_cast<i64>(head) * r.q_head + mine.lo;
+    u16* out = static_cast<u16*>(r.q_out) + (static_cast<u64>(token) * r.q_heads + head) * D + mine.lo;
+    const u32 away = mine.hi - mine.lo;
+    const i64 two = 2 * r.q_head;
+    u32 low[2][R][N], high[2][R][N];  // rows at hand, rows on their way
+    auto load_rows = [&](u32 first, u32 (&l)[R][N], u32 (&h)[R][N]) {
 #pragma unroll
-    for (u32 h = 0; h < kRotaryHeads; ++h) {
-        if (head0 + h < r.q_heads) {
-            load_row<W, kWide>(x + static_cast<i64>(head0 + h) * r.q_head, raw[h]);
-        } else {
-#pragma unroll
-            for (int w = 0; w < W; ++w) raw[h][w] = 0;
+        for (u32 i = 0; i < R; ++i) {
+            if (first + 2 * i < end) {
+                load_words<N, kWide>(x, l[i]);
+                load_words<N, kWide>(x + away, h[i]);
+            }
+            x += two;
         }
-    }
-    Turn<D, kNeighbours> turn(circle.pairs);
-    turn.load(circle.cosines, circle.sines);
+    };
+    load_rows(head, low[0], high[0]);
+    typename Of::Circle circle;
+    mine.make(r, token, circle);
+    for (;;) {
 #pragma unroll
-    for (u32 h = 0; h < kRotaryHeads; ++h) {
-        float2 y[W];
-        u32 b[W];
-        turn.template apply<T>(raw[h], y);
+        for (int k = 0; k < 2; ++k) {
+            load_rows(head + kRotaryHeads, low[1 - k], high[1 - k]);
 #pragma unroll
-        for (int w = 0; w < W; ++w) b[w] = packed(y[w], T{});
-        if (head0 + h < r.q_heads) store_row<W>(out + h * D, b);
+            for (u32 i = 0; i < R; ++i) {
+                float2 p[N], q[N];
+                u32 b[2][N];
+                mine.template apply<T>(low[k][i], high[k][i], circle, p, q);
+#pragma unroll
+                for (int w = 0; w < N; ++w) {
+                    b[0][w] = packed(p[w], T{});
+                    b[1][w] = packed(q[w], T{});
+                }
+                if (head + 2 * i < end) {
+                    store_words<N>(out + 2 * i * D, b[0]);
+                    store_words<N>(out + 2 * i * D + away, b[1]);
+                }
+            }
+            head += kRotaryHeads;
+            out += kRotaryHeads * D;
+            if (head - half >= end) return;
+        }
     }
 }
 
-template <typename T, int D, bool kWide, bool kNeighbours>
+// The block of a chunk's lead that a warp's `u`-th piece of work is in, `each` pieces to a block.
+struct Piece {
+    u32 who, head;
+    int page;
+    u32 slot, count;
+};
+__device__ __forceinline__ Piece piece_at(const Lead& lead, u32 leads, u32 u, u32 each)
+{
+    const u32 which = u / each;
+    for (u32 i = 0; i < which; ++i) leads &= leads - 1;
+    const int who = __ffs(leads) - 1;
+    return {static_cast<u32>(who), u - which * each, __shfl_sync(0xffffffffu, lead.page, who),
+            __shfl_sync(0xffffffffu, lead.slot, who), __shfl_sync(0xffffffffu, lead.count, who)};
+}
+
+// A chunk's keys.
+template <typename T, int D, bool kWide, int kLayout>
+__device__ __forceinline__ void append_keys(const RotaryArgs& r, u32 block, float* shared)
+{
+    const AppendArgs& a = r.a;
+    const u32 lane = threadIdx.x & 31u, pairs = r.pairs, chunk = block / r.key_spread;
+    const u32 base = chunk * a.chunk;
+    const Lead lead = lead_of(a, chunk);
+    const u32 leads = __ballot_sync(0xffffffffu, lead.leads);
+    if (leads == 0) return;
+    // cosines and sines of the blocks' tokens
+    const u32 first = static_cast<u32>(__ffs(leads) - 1);
+    const u32 tokens = __reduce_max_sync(0xffffffffu, lead.leads ? lane + lead.count : 0) - first;
+    float* cosines = shared;
+    float* sines = cosines + tokens * pairs;
+    for (u32 i = threadIdx.x; i < tokens * pairs; i += blockDim.x) {
+        const u32 token = i / pairs;
+        circle_at(r, base + first + token, i - token * pairs, sines[i], cosines[i]);
+    }
+    __syncthreads();
+    const u32 total = __popc(leads) * a.c.heads;
+    for (u32 u = (block - chunk * r.key_spread) * kRotaryWarps + (threadIdx.x >> 5); u < total;
+         u += r.key_spread * kRotaryWarps) {
+        const Piece p = piece_at(lead, leads, u, a.c.heads);
+        const u32 token = base + p.who, row = (p.who - first) * pairs;
+        const Table table{cosines + row, sines + row, pairs};
+        if (p.count < a.c.block || !append_full_turned<T, D, kWide, kLayout>(a, p.head, token, p.page, table)) {
+            const PlainRow<T, D, kWide> from(a, p.head, 0, token);
+            append_block<D>(a, p.head, 0, p.page, p.slot, p.count,
+                            TurnedRow<T, D, kWide, kLayout>{from.x, from.stride, table});
+        }
+    }
+}
+
+// A chunk's values.
+template <typename T, int D, bool kWide>
+__device__ __forceinline__ void append_values(const RotaryArgs& r, u32 block)
+{
+    const AppendArgs& a = r.a;
+    const u32 chunk = block / r.value_spread;
+    const Lead lead = lead_of(a, chunk);
+    const u32 leads = __ballot_sync(0xffffffffu, lead.leads), total = __popc(leads) * a.c.heads;
+    for (u32 u = (block - chunk * r.value_spread) * kRotaryWarps + (threadIdx.x >> 5); u < total;
+         u += r.value_spread * kRotaryWarps) {
+        const Piece p = piece_at(lead, leads, u, a.c.heads);
+        append_plain<T, D, kWide>(a, p.head, 1, chunk * a.chunk + p.who, p.page, p.slot, p.count);
+    }
+}
+
+template <typename T, int D, bool kWide, int kLayout>
 __global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : 6) rotary_kernel(const RotaryArgs r)
 {
     extern __shared__ float4 shared[];
-    const AppendArgs& a = r.a;
-    const u32 base = blockIdx.x * a.chunk, mine = min(a.chunk, a.tokens - base), pairs = r.pairs;
-    const Lead lead = r.append ? lead_of(a) : Lead{false, -1, 0, 0};
-    const u32 leads = __ballot_sync(0xffffffffu, lead.leads);
-    // tokens of the chunk, and those behind it of blocks that begin in it
-    const u32 all = max(mine, __reduce_max_sync(0xffffffffu, lead.leads ? (threadIdx.x & 31u) + lead.count : 0));
-    float* cosines = reinterpret_cast<float*>(shared);
-    float* sines = cosines + all * pairs;
-    for (u32 i = threadIdx.x; i < all * pairs; i += blockDim.x) {
-        const u32 token = i / pairs, pair = i - token * pairs;
-        const u32 axis = min(static_cast<u32>(r.axis[pair]), r.axes - 1);
-        const int position = r.positions[static_cast<i64>(axis) * r.positions_stride + base + token];
-        sine(__dmul_rn(static_cast<double>(position), r.freq[pair]), sines[i], cosines[i]);
+    u32 block = blockIdx.x;
+    if (block < r.key_blocks) {
+        append_keys<T, D, kWide, kLayout>(r, block, reinterpret_cast<float*>(shared));
+        return;
     }
-    __syncthreads();
-    // warps share the blocks' heads and sides, then the tokens' heads
-    const u32 sides = a.c.heads * 2, blocks = __popc(leads) * sides;
-    const u32 groups = (r.q_heads + kRotaryHeads - 1) / kRotaryHeads, total = blocks + mine * groups;
-    for (u32 u = blockIdx.y * kRotaryWarps + (threadIdx.x >> 5); u < total; u += gridDim.y * kRotaryWarps) {
-        if (u >= blocks) {
-            const u32 token = (u - blocks) / groups, head0 = ((u - blocks) - token * groups) * kRotaryHeads;
-            turn_queries<T, D, kWide, kNeighbours>(r, base + token, head0,
-                                                   Circle{cosines + token * pairs, sines + token * pairs, pairs});
-            continue;
-        }
-        const u32 which = u / sides, head = (u - which * sides) >> 1, side = u & 1u;  // `sides` is even
-        u32 left = leads;
-        for (u32 i = 0; i < which; ++i) left &= left - 1;
-        const int who = __ffs(left) - 1;
-        const int page = __shfl_sync(0xffffffffu, lead.page, who);
-        const u32 slot = __shfl_sync(0xffffffffu, lead.slot, who), count = __shfl_sync(0xffffffffu, lead.count, who);
-        const u32 token = base + static_cast<u32>(who);
-        if (side) {
-            append_plain<T, D, kWide>(a, head, side, token, page, slot, count);
-            continue;
-        }
-        const Circle circle{cosines + static_cast<u32>(who) * pairs, sines + static_cast<u32>(who) * pairs, pairs};
-        if (count < a.c.block || !append_full_turned<T, D, kWide, kNeighbours>(a, head, token, page, circle)) {
-            const PlainRow<T, D, kWide> from(a, head, 0, token);
-            append_block<D>(a, head, 0, page, slot, count,
-                            TurnedRow<T, D, kWide, kNeighbours>{from.x, from.stride, circle});
-        }
+    block -= r.key_blocks;
+    if (block < r.value_blocks) {
+        append_values<T, D, kWide>(r, block);
+        return;
     }
+    block -= r.value_blocks;
+    const u64 item = static_cast<u64>(block) * kRotaryWarps + (threadIdx.x >> 5);
+    const u32 token = static_cast<u32>(item / r.parts);
+    if (token < r.a.tokens)
+        turn_queries<T, D, kWide, kLayout>(r, token, static_cast<u32>(item - static_cast<u64>(token) * r.parts) * r.part);
 }
 
-template <typename T, int D, bool kWide, bool kNeighbours>
-bool launch(const RotaryArgs& r, u32 spread, cudaStream_t s)
+template <typename T, int D, bool kWide, int kLayout>
+bool launch(const RotaryArgs& r, cudaStream_t s)
 {
-    const u32 smem = (r.a.chunk - 1 + r.a.c.block) * r.pairs * 8;
+    const u32 smem = r.key_blocks ? (r.a.chunk - 1 + r.a.c.block) * r.pairs * 8 : 0;
     constexpr u32 kMost = (15 + 64) * (D / 2) * 8;
     static std::atomic<u64> seen{0};
-    if (smem > 48 * 1024 && !kv_allow_smem(rotary_kernel<T, D, kWide, kNeighbours>, kMost, seen)) return false;
-    const dim3 grid((r.a.tokens + r.a.chunk - 1) / r.a.chunk, spread);
-    return kv_launch(rotary_kernel<T, D, kWide, kNeighbours>, grid, kRotaryWarps * 32, s, smem, 1, false, r);
+    if (smem > 48 * 1024 && !kv_allow_smem(rotary_kernel<T, D, kWide, kLayout>, kMost, seen)) return false;
+    const u64 items = static_cast<u64>(r.a.tokens) * r.parts;
+    const u64 blocks = r.key_blocks + r.value_blocks + (items + kRotaryWarps - 1) / kRotaryWarps;
+    return kv_launch(rotary_kernel<T, D, kWide, kLayout>, dim3(static_cast<u32>(blocks)), kRotaryWarps * 32, s, smem, 1,
+                     false, r);
 }
 
 template <typename T, int D>
-bool launch_wide(const RotaryArgs& r, u32 spread, bool neighbours, cudaStream_t s)
+bool launch_wide(const RotaryArgs& r, bool neighbours, cudaStream_t s)
 {
-    if (r.a.wide) return neighbours ? launch<T, D, true, true>(r, spread, s) : launch<T, D, true, false>(r, spread, s);
-    return neighbours ? launch<T, D, false, true>(r, spread, s) : launch<T, D, false, false>(r, spread, s);
+    if (!r.a.wide) return neighbours ? launch<T, D, false, kNeighbours>(r, s) : launch<T, D, false, kSplit>(r, s);
+    if (neighbours) return launch<T, D, true, kNeighbours>(r, s);
+    return r.pairs == D / 2 ? launch<T, D, true, kWhole>(r, s) : launch<T, D, true, kSplit>(r, s);
 }
 
 template <typename T>
-bool launch_dim(const RotaryArgs& r, u32 spread, bool neighbours, cudaStream_t s)
+bool launch_dim(const RotaryArgs& r, bool neighbours, cudaStream_t s)
 {
     switch (r.a.c.dim) {
-    case 64: return launch_wide<T, 64>(r, spread, neighbours, s);
-    case 128: return launch_wide<T, 128>(r, spread, neighbours, s);
-    default: return launch_wide<T, 256>(r, spread, neighbours, s);
+    case 64: return launch_wide<T, 64>(r, neighbours, s);
+    case 128: return launch_wide<T, 128>(r, neighbours, s);
+    default: return launch_wide<T, 256>(r, neighbours, s);
     }
 }
 
@@ -399,8 +582,8 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
         return HBFSIM_INVALID_ARGUMENT;
     if (!kv_aligned(x->q, 2) || !kv_aligned(x->q_out, 16) || !kv_aligned(x->positions, 4) || !kv_aligned(x->freq, 8))
         return HBFSIM_INVALID_ARGUMENT;
-    r.append = b->width != 0 && a.c.pages != 0;
-    if (!r.append && x->q_heads == 0) return HBFSIM_OK;
+    const bool append = b->width != 0 && a.c.pages != 0;
+    if (!append && x->q_heads == 0) return HBFSIM_OK;
     r.q = x->q;
     r.q_token = x->q_stride_token;
     r.q_head = x->q_stride_head;
@@ -413,15 +596,23 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
     r.axes = x->axes;
     r.pairs = x->pairs;
     a.wide = a.wide && (x->q_heads == 0 || kv_rows_wide(x->q, x->q_stride_token, x->q_stride_head));
-    // warps' work of a token: groups of query heads, and its share of the blocks' heads and sides
-    const u32 groups = (r.q_heads + kRotaryHeads - 1) / kRotaryHeads, sides = a.c.heads * 2;
+    // Chunks as in kv_append.cu; few tokens get a warp to each head and side.
+    const u32 heads = a.c.heads, groups = (r.q_heads + kRotaryHeads - 1) / kRotaryHeads;
+    const u64 warps = static_cast<u64>(kv_sm_count()) * 16;  // resident at once
     a.chunk = 1;
-    while (a.chunk < 16 &&
-           static_cast<u64>(a.tokens) * (groups + sides) > static_cast<u64>(a.chunk) * 16 * kv_sm_count())
-        a.chunk *= 2;
-    const u32 spread = std::max(1u, (groups + sides + kRotaryWarps * a.chunk - 1) / (kRotaryWarps * a.chunk));
+    while (a.chunk < 16 && static_cast<u64>(a.tokens) * heads * 2 > a.chunk * warps) a.chunk *= 2;
+    if (append) {
+        const u32 chunks = (a.tokens + a.chunk - 1) / a.chunk, by = kRotaryWarps * (a.chunk == 1 ? 1 : 2);
+        r.key_spread = (heads + by - 1) / by;
+        r.value_spread = (heads + kRotaryWarps - 1) / kRotaryWarps;
+        r.key_blocks = chunks * r.key_spread;
+        r.value_blocks = chunks * r.value_spread;
+    }
+    // A token's queries: all heads to a warp that are not needed to fill the device.
+    r.part = static_cast<u32>(std::max<u64>(1, std::min<u64>(groups, static_cast<u64>(a.tokens) * groups / warps)));
+    r.parts = (groups + r.part - 1) / r.part;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool ok = b->type == HBFSIM_KV_BF16 ? launch_dim<__nv_bfloat16>(r, spread, x->neighbours != 0, s)
-                                              : launch_dim<__half>(r, spread, x->neighbours != 0, s);
+    const bool ok = b->type == HBFSIM_KV_BF16 ? launch_dim<__nv_bfloat16>(r, x->neighbours != 0, s)
+                                              : launch_dim<__half>(r, x->neighbours != 0, s);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
