@@ -45,61 +45,73 @@ __device__ __forceinline__ i64 whole(float p)
     return __float2ll_rn(fminf(fmaxf(p, 0.0f), 1.0f) * 1099511627776.0f);  // fmaxf drops NaN; the product is exact
 }
 
-// N neighbouring probabilities in 32 bits.
-template <typename T, int N>
-__device__ __forceinline__ void load_values(const T* from, float (&x)[N])
+// 16 bytes of probabilities, asked for in the order that is written here: the loads of a step are
+// all under way before the first is used.
+__device__ __forceinline__ uint4 load16(const void* from)
 {
-    static_assert(sizeof(T) * N == 16, "one load");
-    const uint4 y = *reinterpret_cast<const uint4*>(from);
-    const T* z = reinterpret_cast<const T*>(&y);
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_float(z[i]);
+    uint4 x;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "l"(from));
+    return x;
 }
 
 struct Sums {
     u64 left, target;  // of the weights, of the target alone
 };
 
+template <bool kDraft>
 __device__ __forceinline__ void add_to(Sums& s, float p, float q)
 {
-    const i64 a = whole(p), d = a - whole(q);
+    const i64 a = whole(p);
     s.target += static_cast<u64>(a);
-    s.left += static_cast<u64>(d > 0 ? d : 0);
+    if constexpr (kDraft) {
+        const i64 d = a - whole(q);
+        s.left += static_cast<u64>(d > 0 ? d : 0);
+    }
+}
+
+// The probabilities of 16 bytes.
+template <typename T, bool kDraft>
+__device__ __forceinline__ void add_16(Sums& s, const uint4& x, const uint4& y)
+{
+    const T* p = reinterpret_cast<const T*>(&x);
+    const T* q = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (u32 k = 0; k < 16 / sizeof(T); ++k) add_to<kDraft>(s, to_float(p[k]), kDraft ? to_float(q[k]) : 0.0f);
 }
 
 // Sums of [from, end) by a warp.
 template <typename T, bool kWide, bool kDraft>
 __device__ __forceinline__ Sums sum_segment(const T* p, const T* q, u32 from, u32 end)
 {
-    constexpr int N = 16 / sizeof(T);
+    constexpr u32 N = 16 / sizeof(T), U = kDraft ? 4 : 8;
     const u32 lane = threadIdx.x & 31u;
     Sums s{0, 0};
-    u32 i = from + lane * N;
     if constexpr (kWide) {
-        constexpr int U = 4;
+        u32 i = from + lane * N;
         for (; i + (U - 1) * 32 * N + N <= end; i += U * 32 * N) {
-            float x[U][N], y[U][N];
+            uint4 x[U], y[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                load_values<T, N>(p + i + u * 32 * N, x[u]);
-                if constexpr (kDraft) load_values<T, N>(q + i + u * 32 * N, y[u]);
+            for (u32 u = 0; u < U; ++u) {
+                x[u] = load16(p + i + u * 32 * N);
+                if constexpr (kDraft) y[u] = load16(q + i + u * 32 * N);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int k = 0; k < N; ++k) add_to(s, x[u][k], kDraft ? y[u][k] : 0.0f);
+            for (u32 u = 0; u < U; ++u) add_16<T, kDraft>(s, x[u], y[u]);
         }
         for (; i + N <= end; i += 32 * N) {
-            float x[N], y[N];
-            load_values<T, N>(p + i, x);
-            if constexpr (kDraft) load_values<T, N>(q + i, y);
-#pragma unroll
-            for (int k = 0; k < N; ++k) add_to(s, x[k], kDraft ? y[k] : 0.0f);
+            const uint4 x = load16(p + i), y = kDraft ? load16(q + i) : x;
+            add_16<T, kDraft>(s, x, y);
         }
-        for (; i < end; ++i) add_to(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);  // one lane's rest
+        for (; i < end; ++i)  // one lane's rest
+            add_to<kDraft>(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);
     } else {
-        for (i = from + lane; i < end; i += 32) add_to(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);
+#pragma unroll 4
+        for (u32 i = from + lane; i < end; i += 32)
+            add_to<kDraft>(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);
     }
+    if constexpr (!kDraft) s.left = s.target;
     return s;
 }
 
@@ -124,6 +136,7 @@ __device__ __forceinline__ u64 warp_scan(u64 x)
 
 struct VerifyShared {
     u32 accepted, count;
+    int tokens[kMaxDrafts];          // those that were accepted
     int refused;                     // the token that was not accepted, -1 without one
     u64 warp_left[kVerifyWarps], warp_target[kVerifyWarps];
     u64 left, target;                // of the CTA: other CTAs read them
@@ -134,7 +147,7 @@ struct VerifyShared {
 };
 
 template <typename T, bool kWide>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a, const u32 size)
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyArgs a, const u32 size)
 {
     __shared__ VerifyShared sm;
     const u32 lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
@@ -142,22 +155,26 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     const KvTeam team{blockIdx.x - seq * size, size};
     const T* target = static_cast<const T*>(a.target) + static_cast<i64>(seq) * a.target_seq;
     const T* draft = static_cast<const T*>(a.draft) + static_cast<i64>(seq) * a.draft_seq;
+    float sample = 0.0f;
+    int length = 0;
     if (warp == 0) {
-        const u32 count = a.counts ? static_cast<u32>(min(max(a.counts[seq], 0), static_cast<int>(a.drafts))) : a.drafts;
+        // what does not hang together is asked for at once
+        const u64 at = static_cast<u64>(seq) * a.drafts + lane;
+        const int given = a.counts ? a.counts[seq] : static_cast<int>(a.drafts);
+        int token = lane < a.drafts ? a.tokens[at] : -1;
+        const double u = lane < a.drafts ? a.accept[at] : 0.0f;
+        sample = a.sample[seq];
+        if (a.lengths_out) length = a.lengths[seq];
+        const u32 count = static_cast<u32>(min(max(given, 0), static_cast<int>(a.drafts)));
         bool good = false;
-        int token = -1;
-        if (lane < count) {
-            const u64 at = static_cast<u64>(seq) * a.drafts + lane;
-            token = a.tokens[at];
-            if (static_cast<u32>(token) < a.vocab) {
-                const double p = to_float(target[static_cast<i64>(lane) * a.target_token + token]);
-                const double q = a.draft ? to_float(draft[static_cast<i64>(lane) * a.draft_token + token]) : 1.0f;
-                good = static_cast<double>(a.accept[at]) * q < p;  // 24 bits by 24: exact
-            } else {
-                token = -1;
-            }
+        if (static_cast<u32>(token) < a.vocab) {
+            const double p = to_float(target[static_cast<i64>(lane) * a.target_token + token]);
+            const double q = a.draft ? to_float(draft[static_cast<i64>(lane) * a.draft_token + token]) : 1.0f;
+            good = u * q < p;  // 24 bits by 24: exact
+        } else {
+            token = -1;
         }
-        const u32 accepted = __ffs(~__ballot_sync(0xffffffffu, good)) - 1u;  // ~0 where all 32 are
+        const u32 accepted = __ffs(~__ballot_sync(0xffffffffu, good && lane < count)) - 1u;  // ~0 where all 32 are
         const u32 n = min(accepted, count);
         const int refused = n < count ? __shfl_sync(0xffffffffu, token, static_cast<int>(n)) : -1;
         if (lane == 0) {
@@ -165,19 +182,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
             sm.count = count;
             sm.refused = refused;
         }
-        if (team.rank == 0) {
-            int* out = a.tokens_out + static_cast<u64>(seq) * (a.drafts + 1);
-            if (lane < n) out[lane] = token;
-            for (u32 i = n + 1 + lane; i <= a.drafts; i += 32) out[i] = -1;
-            if (lane == 0) {
-                a.accepted[seq] = static_cast<int>(n);
-                if (a.lengths_out) a.lengths_out[seq] = a.lengths[seq] - static_cast<int>(count - n);
-            }
-        }
+        if (lane < n) sm.tokens[lane] = token;
     }
     __syncthreads();
     const u32 accepted = sm.accepted;
     const bool rejected = accepted < sm.count;
+    int* out = a.tokens_out + static_cast<u64>(seq) * (a.drafts + 1);
     const T* p = target + static_cast<i64>(accepted) * a.target_token;
     const T* q = rejected && a.draft ? draft + static_cast<i64>(accepted) * a.draft_token : nullptr;
     const u32 refused = rejected && !a.draft ? static_cast<u32>(sm.refused) : ~0u;
@@ -205,6 +215,37 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
             sm.target = t;
         }
     }
+    auto find = [&]() {
+        if (sm.segment == kVerifyWarps) return;
+        // the segment again, a run of neighbours to a thread
+        bounds(sm.segment, from, end);
+        const u32 each = (end - from + kVerifyThreads - 1) / kVerifyThreads;
+        const u32 first = min(from + threadIdx.x * each, end), last = min(first + each, end);
+        const bool alone = sm.alone != 0;
+        auto weight_at = [&](u32 i) {
+            const i64 x = whole(to_float(p[i]));
+            if (alone) return static_cast<u64>(x);
+            if (i == refused) return u64{0};
+            const i64 d = q ? x - whole(to_float(q[i])) : x;
+            return static_cast<u64>(d > 0 ? d : 0);
+        };
+        u64 mine = 0;
+        for (u32 i = first; i < last; ++i) mine += weight_at(i);
+        const u64 upto = warp_scan(mine);
+        if (lane == 31) sm.prefix[warp] = upto;
+        __syncthreads();
+        u64 before = upto - mine;
+        for (u32 w = 0; w < warp; ++w) before += sm.prefix[w];
+        const u64 border = sm.border;
+        if (border < before || border >= before + mine) return;
+        for (u32 i = first; i < last; ++i) {
+            before += weight_at(i);
+            if (border < before) {
+                out[accepted] = static_cast<int>(i);
+                return;
+            }
+        }
+    };
     kv_team_sync(team);
     if (warp == 0) {
         u64 l = lane == 0 ? sm.left : 0, t = lane == 0 ? sm.target : 0;
@@ -212,12 +253,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
             l = lane < size ? kv_peek(&sm.left, lane) : 0;
             t = lane < size ? kv_peek(&sm.target, lane) : 0;
         }
+        if (size > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
         const bool alone = warp_sum(l) == 0;
         const u64 mine = alone ? t : l, sum = warp_sum(mine), upto = warp_scan(mine);
         const u64 before = __shfl_sync(0xffffffffu, upto - mine, static_cast<int>(size > 1 ? team.rank : 0));
         // floor(u * sum / 2^24), sum < 2^62
-        const float at = a.sample[seq];
-        const u32 u = static_cast<u32>(fminf(fmaxf(at, 0.0f) * 16777216.0f, 16777215.0f));
+        const u32 u = static_cast<u32>(fminf(fmaxf(sample, 0.0f) * 16777216.0f, 16777215.0f));
         const u64 border = (u * (sum >> 32) << 8) + (u * (sum & 0xffffffffu) >> 24);
         // the segment of this CTA that holds it
         const u64 weight = lane < kVerifyWarps ? (alone ? sm.warp_target[lane] : sm.warp_left[lane]) : 0;
@@ -228,39 +269,22 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         if (lane == 0) {
             sm.segment = who ? static_cast<u32>(__ffs(who) - 1) : kVerifyWarps;
             sm.alone = alone;
-            if (sum == 0 && team.rank == 0) a.tokens_out[static_cast<u64>(seq) * (a.drafts + 1) + accepted] = -1;
         }
+        if (team.rank == 0) {
+            for (u32 i = lane; i <= a.drafts; i += 32)
+                if (i != accepted || sum == 0) out[i] = i < accepted ? sm.tokens[i] : -1;
+            if (lane == 0) {
+                a.accepted[seq] = static_cast<int>(accepted);
+                if (a.lengths_out) a.lengths_out[seq] = length - static_cast<int>(sm.count - accepted);
+            }
+        }
+    } else if (size > 1) {
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     }
-    kv_team_sync(team);  // nobody leaves while another may read its sums
-    if (sm.segment == kVerifyWarps) return;
-    // the segment again, a run of neighbours to a thread
-    bounds(sm.segment, from, end);
-    const u32 each = (end - from + kVerifyThreads - 1) / kVerifyThreads;
-    const u32 first = min(from + threadIdx.x * each, end), last = min(first + each, end);
-    const bool alone = sm.alone != 0;
-    auto weight_at = [&](u32 i) {
-        const i64 x = whole(to_float(p[i]));
-        if (alone) return static_cast<u64>(x);
-        if (i == refused) return u64{0};
-        const i64 d = q ? x - whole(to_float(q[i])) : x;
-        return static_cast<u64>(d > 0 ? d : 0);
-    };
-    u64 mine = 0;
-    for (u32 i = first; i < last; ++i) mine += weight_at(i);
-    const u64 upto = warp_scan(mine);
-    if (lane == 31) sm.prefix[warp] = upto;
     __syncthreads();
-    u64 before = upto - mine;
-    for (u32 w = 0; w < warp; ++w) before += sm.prefix[w];
-    const u64 border = sm.border;
-    if (border < before || border >= before + mine) return;
-    for (u32 i = first; i < last; ++i) {
-        before += weight_at(i);
-        if (border < before) {
-            a.tokens_out[static_cast<u64>(seq) * (a.drafts + 1) + accepted] = static_cast<int>(i);
-            return;
-        }
-    }
+    find();
+    // nobody leaves while another may read its sums
+    if (size > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 template <typename T>
@@ -272,8 +296,11 @@ bool launch(VerifyArgs& a, u32 seqs, cudaStream_t s)
     };
     const bool all = wide(a.target, a.target_seq, a.target_token) &&
                      (!a.draft || wide(a.draft, a.draft_seq, a.draft_token));
+    // CTAs to a sequence: a power of two, as long as all are resident at once (two to an SM, less what
+    // clusters leave unused) and each has 4096 values or more.
     u32 team = 1;
-    while (team < kMaxTeam && static_cast<u64>(seqs) * team * 2 <= 4ull * kv_sm_count() && a.vocab / (team * 2) >= 4096)
+    while (team < kMaxTeam && static_cast<u64>(seqs) * team * 2 <= static_cast<u64>(kv_sm_count()) * 7 / 4 &&
+           a.vocab / (team * 2) >= 4096)
         team *= 2;
     a.segment = (a.vocab + team * kVerifyWarps * 256 - 1) / (team * kVerifyWarps * 256) * 256;
     return kv_launch(all ? verify_kernel<T, true> : verify_kernel<T, false>, dim3(seqs * team), kVerifyThreads, s, 0,
