@@ -14,10 +14,11 @@
 namespace hbfb {
 namespace {
 
-constexpr u32 kPageThreads = 1024;
+constexpr u32 kPageThreads = 1024, kPageWarps = kPageThreads / 32;
 constexpr u32 kPageTeam = 8;      // blocks of the cluster
 constexpr u32 kMaxParts = 1024;   // blocks of a pass at most
-constexpr u32 kUnit = 512;        // entries of a table's row that a warp takes at a time
+constexpr u32 kDeep = 16;         // entries of a table's row that a lane has under way
+constexpr u32 kSeqsShared = 2048; // sequences whose sums of asked blocks fit shared memory
 // Counts and entries that one cluster takes; beyond, a launch to a pass.
 constexpr u64 kClusterElements = 1u << 19;
 
@@ -32,28 +33,70 @@ __device__ __forceinline__ Share share_of(u32 n, u32 grain, const KvTeam& team)
     return {static_cast<u32>(min(from, static_cast<u64>(n))), static_cast<u32>(min(end, static_cast<u64>(n)))};
 }
 
-// Sum of parts[0..team.rank) and of all parts, by every thread of the block.
-struct Before {
-    u32 mine, all;
-};
-__device__ __forceinline__ Before before_of(const u32* parts, const KvTeam& team, u32* room)
+// The counts of a warp: a run of whole 128s (four to a lane and step).
+__device__ __forceinline__ Share warp_share(u32 n, const KvTeam& team)
 {
-    __syncthreads();  // earlier readers of `room` are done
-    if (threadIdx.x < 32) {
-        u32 mine = 0, all = 0;
-        for (u32 i = threadIdx.x; i < team.size; i += 32) {
-            all += parts[i];
-            if (i < team.rank) mine += parts[i];
-        }
-        mine = __reduce_add_sync(0xffffffffu, mine);
-        all = __reduce_add_sync(0xffffffffu, all);
-        if (threadIdx.x == 0) {
-            room[0] = mine;
-            room[1] = all;
-        }
+    const u32 warps = team.size * kPageWarps, warp = team.rank * kPageWarps + (threadIdx.x >> 5);
+    const u64 each = (static_cast<u64>(n) + warps * 128 - 1) / (warps * 128) * 128, from = each * warp;
+    return {static_cast<u32>(min(from, static_cast<u64>(n))), static_cast<u32>(min(from + each, static_cast<u64>(n)))};
+}
+
+// A lane's four counts of a step from p (a multiple of 4) on, `other` past the end.
+struct Four {
+    int x[4];
+};
+__device__ __forceinline__ Four load_four(const int* counts, u32 p, u32 end, int other)
+{
+    Four f;
+    if (p + 4 <= end && (reinterpret_cast<std::uintptr_t>(counts) & 15) == 0) {
+        const int4 y = *reinterpret_cast<const int4*>(counts + p);
+        f.x[0] = y.x;
+        f.x[1] = y.y;
+        f.x[2] = y.z;
+        f.x[3] = y.w;
+    } else {
+#pragma unroll
+        for (u32 i = 0; i < 4; ++i) f.x[i] = p + i < end ? counts[p + i] : other;
     }
-    __syncthreads();
-    return {room[0], room[1]};
+    return f;
+}
+
+// Of four marks per lane, in order of lane and mark: how many there are before each, and in all.
+struct Ranks {
+    u32 before[4], all;
+};
+__device__ __forceinline__ Ranks rank_four(const bool (&mark)[4])
+{
+    const u32 lane = threadIdx.x & 31u, below = (1u << lane) - 1;
+    Ranks r{{0, 0, 0, 0}, 0};
+    u32 lower = 0;
+#pragma unroll
+    for (u32 i = 0; i < 4; ++i) {
+        const u32 who = __ballot_sync(0xffffffffu, mark[i]);
+        lower += __popc(who & below);
+        r.all += __popc(who);
+    }
+#pragma unroll
+    for (u32 i = 0; i < 4; ++i) {
+        r.before[i] = lower;
+        lower += mark[i];
+    }
+    return r;
+}
+
+// How many of a warp's counts are marked.
+template <typename Mark>
+__device__ __forceinline__ u32 count_marked(const int* counts, u32 n, const KvTeam& team, int other, const Mark& mark)
+{
+    const Share own = warp_share(n, team);
+    u32 sum = 0;
+#pragma unroll 4
+    for (u32 p = own.from + (threadIdx.x & 31u) * 4; p < own.end; p += 128) {
+        const Four f = load_four(counts, p, own.end, other);
+#pragma unroll
+        for (u32 i = 0; i < 4; ++i) sum += mark(f.x[i]);
+    }
+    return __reduce_add_sync(0xffffffffu, sum);
 }
 
 // Sum over the block, by every thread.
@@ -64,25 +107,51 @@ __device__ __forceinline__ u32 block_sum(u32 x, u32* warp_sums)
     if ((threadIdx.x & 31u) == 0) warp_sums[threadIdx.x >> 5] = x;
     __syncthreads();
     const u32 lane = threadIdx.x & 31u;
-    return __reduce_add_sync(0xffffffffu, lane < blockDim.x >> 5 ? warp_sums[lane] : 0);
+    return __reduce_add_sync(0xffffffffu, lane < kPageWarps ? warp_sums[lane] : 0);
+}
+
+// Sums of the parts of earlier warps (of every block) and of all.
+struct Before {
+    u32 mine, all;
+};
+__device__ __forceinline__ Before before_of(const u32* parts, const KvTeam& team, u32* warp_sums)
+{
+    const u32 lane = threadIdx.x & 31u, own = team.rank * kPageWarps, n = team.size * kPageWarps;
+    u32 earlier = 0, all = 0;
+    for (u32 i = threadIdx.x; i < n; i += kPageThreads) {
+        all += parts[i];
+        if (i < own) earlier += parts[i];
+    }
+    earlier = block_sum(earlier, warp_sums);
+    all = block_sum(all, warp_sums);
+    const u32 inside = lane < threadIdx.x >> 5 ? parts[own + lane] : 0;
+    return {earlier + __reduce_add_sync(0xffffffffu, inside), all};
 }
 
 struct PageShared {
     u32 warp_sums[33];
-    u32 room[2];
+    u32 asked[kSeqsShared + 1];
 };
 
-// Calls entry(row, j) for every entry of a table, a run of a row to a warp.
-template <typename Entry>
-__device__ __forceinline__ void for_entries(u32 rows, u32 width, const KvTeam& team, const Entry& entry)
+// Calls run(row, from, end) for runs of a table's rows, up to 32 * kDeep entries to a warp.
+template <typename Run>
+__device__ __forceinline__ void for_runs(u32 rows, u32 width, const KvTeam& team, const Run& run)
 {
-    const u32 lane = threadIdx.x & 31u, warps = team.size * (blockDim.x >> 5);
-    const u32 per_row = (width + kUnit - 1) / kUnit;
+    const u32 warps = team.size * kPageWarps, per_row = (width + 32 * kDeep - 1) / (32 * kDeep);
     const u64 units = static_cast<u64>(rows) * per_row;
-    for (u64 u = team.rank * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const u32 row = static_cast<u32>(u / per_row), from = static_cast<u32>(u - static_cast<u64>(row) * per_row) * kUnit;
-        entry(row, from + lane, min(from + kUnit, width));
+    for (u64 u = team.rank * kPageWarps + (threadIdx.x >> 5); u < units; u += warps) {
+        const u32 row = static_cast<u32>(u / per_row);
+        const u32 from = static_cast<u32>(u - static_cast<u64>(row) * per_row) * 32 * kDeep;
+        run(row, from, min(from + 32 * kDeep, width));
     }
+}
+
+// A lane's entries of a run, all under way at once: from[first + lane + 32 i], -1 past the end.
+__device__ __forceinline__ void load_run(const int* from, u32 first, u32 end, int (&e)[kDeep])
+{
+    const u32 lane = threadIdx.x & 31u;
+#pragma unroll
+    for (u32 i = 0; i < kDeep; ++i) e[i] = first + lane + 32 * i < end ? from[first + lane + 32 * i] : -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -105,7 +174,7 @@ struct ResizeArgs {
     u32 seqs, width, block, freed_rows, freed_width, pages;
     // workspace
     u32* asked;    // [seqs + 1] blocks that earlier sequences ask for
-    u32* free_part;   // [kMaxParts] free pages of a block's share
+    u32* free_part;   // [kMaxParts * kPageWarps] free pages of a warp's share
     u32* claim_part;  // [kMaxParts] claims of a block's share
     int* claims;   // [pages] of a shared page: how often it is asked for
     int* last;     // [pages] and by which sequence last
@@ -127,12 +196,30 @@ __device__ __forceinline__ Row row_of(const ResizeArgs& a, u32 s)
     return r;
 }
 
+// The counts of a pool into their new place.
+__device__ __forceinline__ void copy_counts(const int* from, int* to, u32 n, const KvTeam& team)
+{
+    if (from == to) return;
+    const bool wide = (reinterpret_cast<std::uintptr_t>(to) & 15) == 0;
+    const Share own = warp_share(n, team);
+#pragma unroll 4
+    for (u32 p = own.from + (threadIdx.x & 31u) * 4; p < own.end; p += 128) {
+        const Four f = load_four(from, p, own.end, 0);
+        if (wide && p + 4 <= own.end) {
+            *reinterpret_cast<int4*>(to + p) = make_int4(f.x[0], f.x[1], f.x[2], f.x[3]);
+        } else {
+#pragma unroll
+            for (u32 i = 0; i < 4; ++i)
+                if (p + i < own.end) to[p + i] = f.x[i];
+        }
+    }
+}
+
 // Counts into their new place, rows' asked blocks added up.
 __device__ void resize_begin(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
 {
     const u32 at = team.rank * blockDim.x + threadIdx.x, threads = team.size * blockDim.x;
-    if (a.refs_out != a.refs)
-        for (u32 p = at; p < a.pages; p += threads) a.refs_out[p] = a.refs[p];
+    copy_counts(a.refs, a.refs_out, a.pages, team);
     for (u32 s = at; s < a.seqs; s += threads) {
         a.limits[s] = static_cast<int>(row_of(a, s).goal);
         a.src[s] = a.dst[s] = -1;
@@ -156,86 +243,94 @@ __device__ void resize_begin(const ResizeArgs& a, const KvTeam& team, PageShared
 // What lies behind the rows' new ends goes back, and what an eviction freed.
 __device__ void resize_back(const ResizeArgs& a, const KvTeam& team)
 {
-    for_entries(a.seqs, a.width, team, [&](u32 s, u32 j, u32 end) {
-        const Row r = row_of(a, s);
+    const u32 lane = threadIdx.x & 31u;
+    for_runs(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
         const int* from = a.table + static_cast<i64>(s) * a.table_stride;
         int* to = a.table_out + static_cast<i64>(s) * a.table_out_stride;
-        for (; j < end; j += 32) {
-            const int e = from[j];
-            const bool there = static_cast<u32>(e) < a.pages;
-            if (j >= r.need) {
-                if (there) atomicSub(a.refs_out + e, 1);
-                if (to != from || e != -1) to[j] = -1;
-            } else {
-                if (there && j >= r.first && r.goal > r.held) {  // asked for; counted in the next pass
-                    a.claims[e] = 0;
-                    a.last[e] = -1;
-                }
-                if (to != from) to[j] = e;
+        int e[kDeep];
+        load_run(from, first, end, e);
+        const Row r = row_of(a, s);
+#pragma unroll
+        for (u32 i = 0; i < kDeep; ++i) {
+            const u32 j = first + lane + 32 * i;
+            if (j >= end) break;
+            const bool there = static_cast<u32>(e[i]) < a.pages, behind = j >= r.need;
+            if (there && behind) {
+                atomicSub(a.refs_out + e[i], 1);
+            } else if (there && j >= r.first && r.goal > r.held) {  // asked for; counted in the next pass
+                a.claims[e[i]] = 0;
+                a.last[e[i]] = -1;
             }
+            if (to != from || (behind && e[i] != -1)) to[j] = behind ? -1 : e[i];
         }
     });
-    for_entries(a.freed_rows, a.freed_width, team, [&](u32 s, u32 j, u32 end) {
+    for_runs(a.freed_rows, a.freed_width, team, [&](u32 s, u32 first, u32 end) {
         end = min(end, static_cast<u32>(max(a.freed_counts[s], 0)));
-        for (; j < end; j += 32) {
-            const int e = a.freed[static_cast<u64>(s) * a.freed_width + j];
-            if (static_cast<u32>(e) < a.pages) atomicSub(a.refs_out + e, 1);
-        }
+        if (first >= end) return;
+        int e[kDeep];
+        load_run(a.freed + static_cast<u64>(s) * a.freed_width, first, end, e);
+#pragma unroll
+        for (u32 i = 0; i < kDeep; ++i)
+            if (static_cast<u32>(e[i]) < a.pages) atomicSub(a.refs_out + e[i], 1);
     });
 }
 
-// The sequence of an asked block: the last whose blocks begin at or before it.
-__device__ __forceinline__ u32 asked_by(const ResizeArgs& a, u32 i)
+// The asked blocks of a thread block, and the sums that find their sequences.
+struct AskedShare {
+    u32 from, end, all;
+    const u32* sums;
+};
+__device__ __forceinline__ AskedShare asked_share(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+{
+    const u32 all = a.asked[a.seqs];
+    const Share own = share_of(all, kPageThreads, team);
+    const bool close = a.seqs <= kSeqsShared;
+    if (close && own.from < own.end) {
+        for (u32 s = threadIdx.x; s <= a.seqs; s += blockDim.x) sm.asked[s] = a.asked[s];
+        __syncthreads();
+    }
+    return {own.from, own.end, all, close ? sm.asked : a.asked};
+}
+
+// Asked block i: its sequence (the last whose blocks begin at or before it), its place in the table.
+struct Asked {
+    u32 seq, block, first, held;
+    int* entry;
+};
+__device__ __forceinline__ Asked asked_at(const ResizeArgs& a, const u32* sums, u32 i)
 {
     u32 lo = 0, hi = a.seqs;
     while (hi - lo > 1) {
         const u32 mid = (lo + hi) >> 1;
-        if (a.asked[mid] <= i) lo = mid;
+        if (sums[mid] <= i) lo = mid;
         else hi = mid;
     }
-    return lo;
+    const u32 held = static_cast<u32>(kv_length(a.lengths, lo, a.width, a.block)), first = held / a.block;
+    const u32 j = first + (i - sums[lo]);
+    return {lo, j, first, held, a.table_out + static_cast<i64>(lo) * a.table_out_stride + j};
 }
 
-// Asked block i: its sequence, its place in the table.
-struct Asked {
-    u32 seq, block, first;
-    int* entry;
-};
-__device__ __forceinline__ Asked asked_at(const ResizeArgs& a, u32 i)
+// Free pages are counted, and how often shared pages are asked for.
+__device__ void resize_count(const ResizeArgs& a, const KvTeam& team, const AskedShare& asked)
 {
-    const u32 s = asked_by(a, i);
-    const u32 first = static_cast<u32>(kv_length(a.lengths, s, a.width, a.block)) / a.block;
-    const u32 j = first + (i - a.asked[s]);
-    return {s, j, first, a.table_out + static_cast<i64>(s) * a.table_out_stride + j};
-}
-
-// Free pages of the block's share are counted, and how often shared pages are asked for.
-__device__ void resize_count(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
-{
-    const Share own = share_of(a.pages, kPageThreads, team);
-    u32 free = 0;
-    for (u32 p = own.from + threadIdx.x; p < own.end; p += blockDim.x) free += a.refs_out[p] < 1;
-    free = block_sum(free, sm.warp_sums);
-    if (threadIdx.x == 0) a.free_part[team.rank] = free;
-    const Share asked = share_of(a.asked[a.seqs], kPageThreads, team);
     for (u32 i = asked.from + threadIdx.x; i < asked.end; i += blockDim.x) {
-        const Asked x = asked_at(a, i);
+        const Asked x = asked_at(a, asked.sums, i);
         const int e = *x.entry;
         if (static_cast<u32>(e) < a.pages && a.refs_out[e] > 1) {
             atomicAdd(a.claims + e, 1);
             atomicMax(a.last + e, static_cast<int>(x.seq));
         }
     }
+    const u32 free = count_marked(a.refs_out, a.pages, team, 1, [](int x) { return x < 1; });
+    if ((threadIdx.x & 31u) == 0) a.free_part[team.rank * kPageWarps + (threadIdx.x >> 5)] = free;
 }
 
 // Free pages in ascending order, as many as may be asked for; what becomes of the asked blocks.
-__device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+__device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, const AskedShare& asked, PageShared& sm)
 {
-    const u32 all = a.asked[a.seqs];
-    const Share asked = share_of(all, kPageThreads, team);
     u32 claims = 0;
     for (u32 i = asked.from + threadIdx.x; i < asked.end; i += blockDim.x) {
-        const Asked x = asked_at(a, i);
+        const Asked x = asked_at(a, asked.sums, i);
         const int e = *x.entry;
         u8 state = kNew;
         if (static_cast<u32>(e) < a.pages) {
@@ -248,23 +343,30 @@ __device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, PageShared&
     }
     claims = block_sum(claims, sm.warp_sums);
     if (threadIdx.x == 0) a.claim_part[team.rank] = claims;
-    const Share own = share_of(a.pages, kPageThreads, team);
-    u32 rank = before_of(a.free_part, team, sm.room).mine;
-    for (u32 p0 = own.from; p0 < own.end && rank < all; p0 += blockDim.x) {
-        const u32 p = p0 + threadIdx.x;
-        const bool free = p < own.end && a.refs_out[p] < 1;
-        const u32 upto = kv_block_scan(free, sm.warp_sums);
-        if (free && rank + upto - 1 < all) a.pool[rank + upto - 1] = static_cast<int>(p);
-        rank += sm.warp_sums[32];
+    u32 rank = before_of(a.free_part, team, sm.warp_sums).mine;
+    const Share own = warp_share(a.pages, team);
+    for (u32 p0 = own.from; p0 < own.end && rank < asked.all; p0 += 128) {
+        const u32 p = p0 + (threadIdx.x & 31u) * 4;
+        const Four f = load_four(a.refs_out, p, own.end, 1);
+        const bool free[4] = {f.x[0] < 1, f.x[1] < 1, f.x[2] < 1, f.x[3] < 1};
+        const Ranks r = rank_four(free);
+#pragma unroll
+        for (u32 i = 0; i < 4; ++i)
+            if (free[i] && rank + r.before[i] < asked.all) a.pool[rank + r.before[i]] = static_cast<int>(p + i);
+        rank += r.all;
     }
 }
 
 // Claims get their pages.
-__device__ void resize_give(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+__device__ void resize_give(const ResizeArgs& a, const KvTeam& team, const AskedShare& asked, PageShared& sm)
 {
-    const u32 free = before_of(a.free_part, team, sm.room).all;
-    const Share asked = share_of(a.asked[a.seqs], kPageThreads, team);
-    u32 rank = before_of(a.claim_part, team, sm.room).mine;
+    if (asked.from >= asked.end) return;
+    const u32 lane = threadIdx.x & 31u;
+    u32 free = 0, rank = 0;  // free pages; claims of earlier blocks: by every warp for itself
+    for (u32 i = lane; i < team.size * kPageWarps; i += 32) free += a.free_part[i];
+    for (u32 i = lane; i < team.rank; i += 32) rank += a.claim_part[i];
+    free = __reduce_add_sync(0xffffffffu, free);
+    rank = __reduce_add_sync(0xffffffffu, rank);
     for (u32 i0 = asked.from; i0 < asked.end; i0 += blockDim.x) {
         const u32 i = i0 + threadIdx.x;
         const u8 state = i < asked.end ? a.state[i] : kKeep;
@@ -273,16 +375,15 @@ __device__ void resize_give(const ResizeArgs& a, const KvTeam& team, PageShared&
         const u32 before = rank + upto - claim;
         rank += sm.warp_sums[32];
         if (state == kKeep) continue;
-        const Asked x = asked_at(a, i);
-        const u32 held = static_cast<u32>(kv_length(a.lengths, x.seq, a.width, a.block));
+        const Asked x = asked_at(a, asked.sums, i);
         if (claim ? before >= free : before > free) {  // not served
-            atomicMin(a.limits + x.seq, static_cast<int>(max(held, x.block * a.block)));
+            atomicMin(a.limits + x.seq, static_cast<int>(max(x.held, x.block * a.block)));
         } else if (claim) {
             const int page = a.pool[before];
             if (state == kPart) {
                 const int old = *x.entry;
                 atomicSub(a.refs_out + old, 1);
-                if (x.block == x.first && held % a.block) {
+                if (x.block == x.first && x.held % a.block) {
                     a.src[x.seq] = old;
                     a.dst[x.seq] = page;
                 }
@@ -301,11 +402,12 @@ __global__ void __launch_bounds__(kPageThreads) resize_cluster_kernel(const Resi
     kv_team_sync(team);
     resize_back(a, team);
     kv_team_sync(team);
-    resize_count(a, team, sm);
+    const AskedShare asked = asked_share(a, team, sm);
+    resize_count(a, team, asked);
     kv_team_sync(team);
-    resize_rank(a, team, sm);
+    resize_rank(a, team, asked, sm);
     kv_team_sync(team);
-    resize_give(a, team, sm);
+    resize_give(a, team, asked, sm);
 }
 
 template <int kPass>
@@ -317,9 +419,9 @@ __global__ void __launch_bounds__(kPageThreads) resize_pass_kernel(const ResizeA
     const KvTeam team{blockIdx.x, gridDim.x};
     if constexpr (kPass == 0) resize_begin(a, team, sm);
     else if constexpr (kPass == 1) resize_back(a, team);
-    else if constexpr (kPass == 2) resize_count(a, team, sm);
-    else if constexpr (kPass == 3) resize_rank(a, team, sm);
-    else resize_give(a, team, sm);
+    else if constexpr (kPass == 2) resize_count(a, team, asked_share(a, team, sm));
+    else if constexpr (kPass == 3) resize_rank(a, team, asked_share(a, team, sm), sm);
+    else resize_give(a, team, asked_share(a, team, sm), sm);
 }
 
 // ---------------------------------------------------------------------------
@@ -337,44 +439,49 @@ struct ForkArgs {
     u32 seqs, rows, width, block, pages;
 };
 
-__device__ void fork_begin(const ForkArgs& a, const KvTeam& team)
-{
-    const u32 threads = team.size * blockDim.x;
-    for (u32 p = team.rank * blockDim.x + threadIdx.x; p < a.pages; p += threads) a.refs_out[p] = a.refs[p];
-}
-
 __device__ __forceinline__ u32 blocks_held(const ForkArgs& a, u32 s)
 {
     return (static_cast<u32>(kv_length(a.lengths, s, a.width, a.block)) + a.block - 1) / a.block;
 }
 
-// The new rows take their pages, the old ones give theirs back; a row that goes on as itself does
-// neither for the blocks that it holds.
+// The new rows.
 __device__ void fork_rows(const ForkArgs& a, const KvTeam& team)
 {
-    const u32 threads = team.size * blockDim.x;
+    const u32 lane = threadIdx.x & 31u, threads = team.size * blockDim.x;
+    copy_counts(a.refs, a.refs_out, a.pages, team);
     for (u32 r = team.rank * blockDim.x + threadIdx.x; r < a.rows; r += threads) {
         const u32 parent = static_cast<u32>(a.parents[r]);
         a.lengths_out[r] = parent < a.seqs ? kv_length(a.lengths, parent, a.width, a.block) : 0;
     }
-    for_entries(a.rows, a.width, team, [&](u32 r, u32 j, u32 end) {
+    for_runs(a.rows, a.width, team, [&](u32 r, u32 first, u32 end) {
         const u32 parent = static_cast<u32>(a.parents[r]);
-        const bool real = parent < a.seqs;
-        const u32 blocks = real ? blocks_held(a, parent) : 0;
-        const int* from = a.table + static_cast<i64>(real ? parent : 0) * a.table_stride;
+        const u32 blocks = parent < a.seqs ? blocks_held(a, parent) : 0;
+        const int* from = a.table + static_cast<i64>(parent < a.seqs ? parent : 0) * a.table_stride;
         int* to = a.table_out + static_cast<u64>(r) * a.width;
-        for (; j < end; j += 32) {
-            const int e = j < blocks ? from[j] : -1;
-            to[j] = e;
-            if (parent != r && static_cast<u32>(e) < a.pages) atomicAdd(a.refs_out + e, 1);
-        }
+        int e[kDeep];
+        load_run(from, first, min(end, blocks), e);
+#pragma unroll
+        for (u32 i = 0; i < kDeep; ++i)
+            if (first + lane + 32 * i < end) to[first + lane + 32 * i] = e[i];
     });
-    for_entries(a.seqs, a.width, team, [&](u32 s, u32 j, u32 end) {
-        const u32 stay = s < a.rows && a.parents[s] == static_cast<int>(s) ? blocks_held(a, s) : 0;
-        const int* from = a.table + static_cast<i64>(s) * a.table_stride;
-        for (; j < end; j += 32) {
-            const int e = j < stay ? -1 : from[j];
-            if (static_cast<u32>(e) < a.pages) atomicSub(a.refs_out + e, 1);
+}
+
+// Pages are counted for every child that goes on from an old row, less the row itself.
+__device__ void fork_count(const ForkArgs& a, const KvTeam& team)
+{
+    const u32 lane = threadIdx.x & 31u;
+    for_runs(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
+        int e[kDeep];
+        load_run(a.table + static_cast<i64>(s) * a.table_stride, first, end, e);
+        const u32 blocks = blocks_held(a, s);
+        u32 children = 0;
+#pragma unroll 8
+        for (u32 r = lane; r < a.rows; r += 32) children += a.parents[r] == static_cast<int>(s);
+        children = __reduce_add_sync(0xffffffffu, children);
+#pragma unroll
+        for (u32 i = 0; i < kDeep; ++i) {
+            const int by = first + lane + 32 * i < blocks ? static_cast<int>(children) - 1 : -1;
+            if (by != 0 && static_cast<u32>(e[i]) < a.pages) atomicAdd(a.refs_out + e[i], by);
         }
     });
 }
@@ -382,9 +489,9 @@ __device__ void fork_rows(const ForkArgs& a, const KvTeam& team)
 __global__ void __launch_bounds__(kPageThreads) fork_cluster_kernel(const ForkArgs a)
 {
     const KvTeam team{blockIdx.x, kPageTeam};
-    fork_begin(a, team);
-    kv_team_sync(team);
     fork_rows(a, team);
+    kv_team_sync(team);
+    fork_count(a, team);
 }
 
 template <int kPass>
@@ -393,8 +500,8 @@ __global__ void __launch_bounds__(kPageThreads) fork_pass_kernel(const ForkArgs 
     kv_let_next();
     kv_wait_before();
     const KvTeam team{blockIdx.x, gridDim.x};
-    if constexpr (kPass == 0) fork_begin(a, team);
-    else fork_rows(a, team);
+    if constexpr (kPass != 1) fork_rows(a, team);
+    if constexpr (kPass != 0) fork_count(a, team);
 }
 
 // ---------------------------------------------------------------------------
@@ -412,16 +519,13 @@ struct CompactArgs {
     int* live;
     int* where;
     u32 seqs, width, pages;
-    u32* live_part;  // workspace: [kMaxParts] pages in use of a block's share
+    u32* live_part;  // workspace: [kMaxParts * kPageWarps] pages in use of a warp's share
 };
 
-__device__ void compact_count(const CompactArgs& a, const KvTeam& team, PageShared& sm)
+__device__ void compact_count(const CompactArgs& a, const KvTeam& team)
 {
-    const Share own = share_of(a.pages, kPageThreads, team);
-    u32 live = 0;
-    for (u32 p = own.from + threadIdx.x; p < own.end; p += blockDim.x) live += a.refs[p] > 0;
-    live = block_sum(live, sm.warp_sums);
-    if (threadIdx.x == 0) a.live_part[team.rank] = live;
+    const u32 live = count_marked(a.refs, a.pages, team, 0, [](int x) { return x > 0; });
+    if ((threadIdx.x & 31u) == 0) a.live_part[team.rank * kPageWarps + (threadIdx.x >> 5)] = live;
     const u32 threads = team.size * blockDim.x, room = a.pages / 2;
     for (u32 i = team.rank * blockDim.x + threadIdx.x; i < room; i += threads) a.src[i] = a.dst[i] = -1;
 }
@@ -431,51 +535,59 @@ __device__ void compact_count(const CompactArgs& a, const KvTeam& team, PageShar
 // holds -2 - move of a page that moves.
 __device__ void compact_rank(const CompactArgs& a, const KvTeam& team, PageShared& sm)
 {
-    const Before before = before_of(a.live_part, team, sm.room);
+    const Before before = before_of(a.live_part, team, sm.warp_sums);
     const u32 n = before.all;
     if (team.rank == 0 && threadIdx.x == 0) *a.live = static_cast<int>(n);
-    const Share own = share_of(a.pages, kPageThreads, team);
+    const Share own = warp_share(a.pages, team);
     u32 rank = before.mine;
-    for (u32 p0 = own.from; p0 < own.end; p0 += blockDim.x) {
-        const u32 p = p0 + threadIdx.x;
-        const int count = p < own.end ? a.refs[p] : 0;
-        const bool live = count > 0;
-        const u32 upto = rank + kv_block_scan(live, sm.warp_sums);
-        rank += sm.warp_sums[32];
-        if (p >= own.end) continue;
-        int place = -1;
-        if (p < n) {
-            if (live) {
-                place = static_cast<int>(p);
-                if (a.refs_out != a.refs) a.refs_out[p] = count;
+    for (u32 p0 = own.from; p0 < own.end; p0 += 128) {
+        const u32 first = p0 + (threadIdx.x & 31u) * 4;
+        const Four f = load_four(a.refs, first, own.end, 0);
+        const bool live[4] = {f.x[0] > 0, f.x[1] > 0, f.x[2] > 0, f.x[3] > 0};
+        const Ranks r = rank_four(live);
+#pragma unroll
+        for (u32 i = 0; i < 4; ++i) {
+            const u32 p = first + i, earlier = rank + r.before[i];  // pages in use before p
+            if (p >= own.end) break;
+            int place = -1;
+            if (p < n) {
+                if (live[i]) {
+                    place = static_cast<int>(p);
+                    if (a.refs_out != a.refs) a.refs_out[p] = f.x[i];
+                } else {
+                    a.dst[p - earlier] = static_cast<int>(p);  // its count comes with the page
+                }
+            } else if (live[i]) {
+                const u32 move = n - 1 - earlier;
+                a.src[move] = static_cast<int>(p);
+                place = -2 - static_cast<int>(move);  // its count leaves with the page
             } else {
-                a.dst[p - upto] = static_cast<int>(p);  // its count comes with the page
+                a.refs_out[p] = 0;
             }
-        } else if (live) {
-            const u32 move = n - upto;
-            a.src[move] = static_cast<int>(p);
-            place = -2 - static_cast<int>(move);  // its count leaves with the page
-        } else {
-            a.refs_out[p] = 0;
+            a.where[p] = place;
         }
-        a.where[p] = place;
+        rank += r.all;
     }
 }
 
 __device__ void compact_move(const CompactArgs& a, const KvTeam& team)
 {
-    const u32 threads = team.size * blockDim.x, room = a.pages / 2;
+    const u32 lane = threadIdx.x & 31u, threads = team.size * blockDim.x, room = a.pages / 2;
     // entries: a page that moves is found by its number or, if the loop below was faster, by its place
-    for_entries(a.seqs, a.width, team, [&](u32 s, u32 j, u32 end) {
-        const int* from = a.table + static_cast<i64>(s) * a.table_stride;
+    for_runs(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
         int* to = a.table_out + static_cast<i64>(s) * a.table_out_stride;
-        for (; j < end; j += 32) {
-            int e = from[j];
-            if (static_cast<u32>(e) < a.pages) {
-                e = *static_cast<volatile int*>(a.where + e);
-                if (e < -1) e = a.dst[-2 - e];
-            }
-            to[j] = e;
+        int e[kDeep];
+        bool there[kDeep];
+        load_run(a.table + static_cast<i64>(s) * a.table_stride, first, end, e);
+#pragma unroll
+        for (u32 i = 0; i < kDeep; ++i) {
+            there[i] = static_cast<u32>(e[i]) < a.pages;
+            if (there[i]) e[i] = *static_cast<volatile int*>(a.where + e[i]);
+        }
+#pragma unroll
+        for (u32 i = 0; i < kDeep; ++i) {
+            if (there[i] && e[i] < -1) e[i] = a.dst[-2 - e[i]];
+            if (first + lane + 32 * i < end) to[first + lane + 32 * i] = e[i];
         }
     });
     for (u32 i = team.rank * blockDim.x + threadIdx.x; i < room; i += threads) {
@@ -492,7 +604,7 @@ __global__ void __launch_bounds__(kPageThreads) compact_cluster_kernel(const Com
 {
     __shared__ PageShared sm;
     const KvTeam team{blockIdx.x, kPageTeam};
-    compact_count(a, team, sm);
+    compact_count(a, team);
     kv_team_sync(team);
     compact_rank(a, team, sm);
     kv_team_sync(team);
@@ -506,7 +618,7 @@ __global__ void __launch_bounds__(kPageThreads) compact_pass_kernel(const Compac
     kv_let_next();
     kv_wait_before();
     const KvTeam team{blockIdx.x, gridDim.x};
-    if constexpr (kPass == 0) compact_count(a, team, sm);
+    if constexpr (kPass == 0) compact_count(a, team);
     else if constexpr (kPass == 1) compact_rank(a, team, sm);
     else compact_move(a, team);
 }
@@ -611,7 +723,7 @@ ResizeRoom resize_room(const hbfsim_kv_resize_batch_v1& b)
     Room room;
     ResizeRoom r{};
     r.asked = room.take((u64{b.seqs} + 1) * 4);
-    r.free_part = room.take(kMaxParts * 4);
+    r.free_part = room.take(kMaxParts * kPageWarps * 4);
     r.claim_part = room.take(kMaxParts * 4);
     r.claims = room.take(b.pages * 4);
     r.last = room.take(b.pages * 4);
@@ -646,7 +758,7 @@ bool cluster(void (*kernel)(Args), const Args& a, cudaStream_t s)
     return kv_launch(kernel, dim3(kPageTeam), kPageThreads, s, 0, kPageTeam, false, a);
 }
 
-u32 pass_blocks() { return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count()) * 2); }
+u32 pass_blocks() { return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count())); }
 
 }  // namespace
 }  // namespace hbfb
@@ -738,12 +850,13 @@ extern "C" int hbfsim_kv_fork_v1(const hbfsim_kv_fork_batch_v1* b, void* stream)
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool apart = b->refs_out != b->refs;
     bool ok;
-    if (apart && b->pages + entries + made <= kClusterElements) {
+    const u32 blocks = pass_blocks();
+    if (!apart) {  // the counts are where they belong: no pass waits for another
+        ok = pass(fork_pass_kernel<2>, blocks, false, a, s);
+    } else if (b->pages + entries + made <= kClusterElements) {
         ok = cluster(fork_cluster_kernel, a, s);
     } else {
-        const u32 blocks = pass_blocks();
-        ok = (!apart || pass(fork_pass_kernel<0>, blocks, false, a, s)) &&
-             pass(fork_pass_kernel<1>, blocks, apart, a, s);
+        ok = pass(fork_pass_kernel<0>, blocks, false, a, s) && pass(fork_pass_kernel<1>, blocks, true, a, s);
     }
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
@@ -759,7 +872,7 @@ static int compact_check(const hbfsim_kv_compact_batch_v1* b)
 
 extern "C" uint64_t hbfsim_kv_compact_workspace_v1(const hbfsim_kv_compact_batch_v1* b)
 {
-    return compact_check(b) == HBFSIM_OK ? kMaxParts * 4 : 0;
+    return compact_check(b) == HBFSIM_OK ? kMaxParts * kPageWarps * 4 : 0;
 }
 
 extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* stream)
@@ -774,13 +887,13 @@ extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* s
                           static_cast<const void*>(b->src), static_cast<const void*>(b->dst),
                           static_cast<const void*>(b->live), static_cast<const void*>(b->where)})
         if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
-    if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < kMaxParts * 4) return HBFSIM_INVALID_ARGUMENT;
+    if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < kMaxParts * kPageWarps * 4) return HBFSIM_INVALID_ARGUMENT;
     if (b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
     if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
     const Extent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, b->seqs, b->width, b->table_out_stride},
                           {b->src, room * 4},          {b->dst, room * 4},
                           {b->live, 4},                {b->where, b->pages * 4},
-                          {b->workspace, kMaxParts * 4}};
+                          {b->workspace, kMaxParts * kPageWarps * 4}};
     const Extent in[] = {{b->refs, b->pages * 4}, {b->table, b->seqs, b->width, b->table_stride}};
     if (would_race(out, in, {0, 1, -1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
     const CompactArgs a{b->refs, b->table, b->table_stride, b->refs_out, b->table_out, b->table_out_stride, b->src,
