@@ -5,10 +5,10 @@
 // The work is a few passes over the counts and the table, each of which needs
 // all of the one before: what goes back has to be counted before free pages are
 // ranked, and ranked before they are given.  The passes are device functions of
-// a team of thread blocks.  A small pool is done by one cluster of 8 in one
+// a team of thread blocks.  A small pool is done by one cluster of up to 8 in one
 // launch, with cluster barriers between the passes; a large one by as many
-// blocks as the device has SMs, a launch to a pass.  A pass shares its elements
-// out evenly, in order, so that ranks are sums over the blocks before.
+// blocks as the device has SMs, a launch to a pass.  Where ranks count, a warp has
+// a contiguous share, so that they are sums over the warps before it.
 #include "kv.h"
 
 namespace hbfb {
@@ -18,20 +18,13 @@ constexpr u32 kPageThreads = 1024, kPageWarps = kPageThreads / 32;
 constexpr u32 kPageTeam = 8;      // blocks of the cluster
 constexpr u32 kMaxParts = 1024;   // blocks of a pass at most
 constexpr u32 kDeep = 16;         // entries of a table's row that a lane has under way
-constexpr u32 kSeqsShared = 2048; // sequences whose sums of asked blocks fit shared memory
-// Counts and entries that one cluster takes; beyond, a launch to a pass.
-constexpr u64 kClusterElements = 1u << 19;
+// Counts and entries that are worth a block of a cluster, and that one takes at most.
+constexpr u64 kCountsEach = 16384, kEntriesEach = 16384, kCountsMost = 32768, kEntriesMost = 16384;
 
-// The elements [from, end) of a block, in pieces of `grain`.
+// The elements [from, end) of a warp.
 struct Share {
     u32 from, end;
 };
-__device__ __forceinline__ Share share_of(u32 n, u32 grain, const KvTeam& team)
-{
-    const u64 pieces = (static_cast<u64>(n) + grain - 1) / grain;
-    const u64 from = pieces * team.rank / team.size * grain, end = pieces * (team.rank + 1) / team.size * grain;
-    return {static_cast<u32>(min(from, static_cast<u64>(n))), static_cast<u32>(min(end, static_cast<u64>(n)))};
-}
 
 // The counts of a warp: a run of whole 128s (four to a lane and step).
 __device__ __forceinline__ Share warp_share(u32 n, const KvTeam& team)
@@ -59,6 +52,17 @@ __device__ __forceinline__ Four load_four(const int* counts, u32 p, u32 end, int
         for (u32 i = 0; i < 4; ++i) f.x[i] = p + i < end ? counts[p + i] : other;
     }
     return f;
+}
+
+__device__ __forceinline__ void store_four(int* counts, u32 p, u32 end, const Four& f)
+{
+    if (p + 4 <= end && (reinterpret_cast<std::uintptr_t>(counts) & 15) == 0) {
+        *reinterpret_cast<int4*>(counts + p) = make_int4(f.x[0], f.x[1], f.x[2], f.x[3]);
+    } else {
+#pragma unroll
+        for (u32 i = 0; i < 4; ++i)
+            if (p + i < end) counts[p + i] = f.x[i];
+    }
 }
 
 // Of four marks per lane, in order of lane and mark: how many there are before each, and in all.
@@ -99,59 +103,79 @@ __device__ __forceinline__ u32 count_marked(const int* counts, u32 n, const KvTe
     return __reduce_add_sync(0xffffffffu, sum);
 }
 
-// Sum over the block, by every thread.
-__device__ __forceinline__ u32 block_sum(u32 x, u32* warp_sums)
+// Sums over the block, by every thread.
+template <u32 N>
+__device__ __forceinline__ void block_sums(u32 (&x)[N], u32 (*warp_sums)[kPageWarps])
 {
-    x = __reduce_add_sync(0xffffffffu, x);
-    __syncthreads();
-    if ((threadIdx.x & 31u) == 0) warp_sums[threadIdx.x >> 5] = x;
-    __syncthreads();
     const u32 lane = threadIdx.x & 31u;
-    return __reduce_add_sync(0xffffffffu, lane < kPageWarps ? warp_sums[lane] : 0);
+#pragma unroll
+    for (u32 k = 0; k < N; ++k) x[k] = __reduce_add_sync(0xffffffffu, x[k]);
+    __syncthreads();  // earlier readers of warp_sums are done
+    if (lane == 0) {
+#pragma unroll
+        for (u32 k = 0; k < N; ++k) warp_sums[k][threadIdx.x >> 5] = x[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (u32 k = 0; k < N; ++k) x[k] = __reduce_add_sync(0xffffffffu, warp_sums[k][lane]);
 }
 
-// Sums of the parts of earlier warps (of every block) and of all.
+// Sums of the parts of earlier warps (of every block) and of all; of other parts, if given, of all.
 struct Before {
-    u32 mine, all;
+    u32 mine, all, others;
 };
-__device__ __forceinline__ Before before_of(const u32* parts, const KvTeam& team, u32* warp_sums)
+__device__ __forceinline__ Before before_of(const u32* parts, const KvTeam& team, u32 (*warp_sums)[kPageWarps],
+                                            const u32* others = nullptr)
 {
     const u32 lane = threadIdx.x & 31u, own = team.rank * kPageWarps, n = team.size * kPageWarps;
-    u32 earlier = 0, all = 0;
-    for (u32 i = threadIdx.x; i < n; i += kPageThreads) {
-        all += parts[i];
-        if (i < own) earlier += parts[i];
-    }
-    earlier = block_sum(earlier, warp_sums);
-    all = block_sum(all, warp_sums);
     const u32 inside = lane < threadIdx.x >> 5 ? parts[own + lane] : 0;
-    return {earlier + __reduce_add_sync(0xffffffffu, inside), all};
+    u32 x[3] = {0, 0, 0};
+    for (u32 i = threadIdx.x; i < n; i += kPageThreads) {
+        const u32 part = parts[i];
+        x[1] += part;
+        if (i < own) x[0] += part;
+        if (others) x[2] += others[i];
+    }
+    block_sums(x, warp_sums);
+    return {x[0] + __reduce_add_sync(0xffffffffu, inside), x[1], x[2]};
 }
 
-struct PageShared {
-    u32 warp_sums[33];
-    u32 asked[kSeqsShared + 1];
-};
-
-// Calls run(row, from, end) for runs of a table's rows, up to 32 * kDeep entries to a warp.
-template <typename Run>
+// Calls run(row, from, end) for runs of a table's rows, up to 32 * Deep entries to a warp; the
+// blocks of a team take them in turn, so that few runs are spread over all of them.
+template <u32 Deep, typename Run>
 __device__ __forceinline__ void for_runs(u32 rows, u32 width, const KvTeam& team, const Run& run)
 {
-    const u32 warps = team.size * kPageWarps, per_row = (width + 32 * kDeep - 1) / (32 * kDeep);
+    const u32 per_row = (width + 32 * Deep - 1) / (32 * Deep);
     const u64 units = static_cast<u64>(rows) * per_row;
-    for (u64 u = team.rank * kPageWarps + (threadIdx.x >> 5); u < units; u += warps) {
+    for (u64 u = (threadIdx.x >> 5) * team.size + team.rank; u < units; u += team.size * kPageWarps) {
         const u32 row = static_cast<u32>(u / per_row);
-        const u32 from = static_cast<u32>(u - static_cast<u64>(row) * per_row) * 32 * kDeep;
-        run(row, from, min(from + 32 * kDeep, width));
+        const u32 from = static_cast<u32>(u - static_cast<u64>(row) * per_row) * 32 * Deep;
+        run(row, from, min(from + 32 * Deep, width));
     }
 }
 
 // A lane's entries of a run, all under way at once: from[first + lane + 32 i], -1 past the end.
-__device__ __forceinline__ void load_run(const int* from, u32 first, u32 end, int (&e)[kDeep])
+template <u32 Deep>
+__device__ __forceinline__ void load_run(const int* from, u32 first, u32 end, int (&e)[Deep])
 {
     const u32 lane = threadIdx.x & 31u;
 #pragma unroll
-    for (u32 i = 0; i < kDeep; ++i) e[i] = first + lane + 32 * i < end ? from[first + lane + 32 * i] : -1;
+    for (u32 i = 0; i < Deep; ++i) e[i] = first + lane + 32 * i < end ? from[first + lane + 32 * i] : -1;
+}
+
+// The counts of a pool into their new place.
+__device__ __forceinline__ void copy_counts(const int* from, int* to, u32 n, const KvTeam& team)
+{
+    if (from == to) return;
+    const Share own = warp_share(n, team);
+#pragma unroll 1
+    for (u32 p = own.from + (threadIdx.x & 31u) * 4; p < own.end; p += 512) {
+        Four f[4];
+#pragma unroll
+        for (u32 i = 0; i < 4; ++i) f[i] = load_four(from, p + 128 * i, own.end, 0);
+#pragma unroll
+        for (u32 i = 0; i < 4; ++i) store_four(to, p + 128 * i, own.end, f[i]);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -173,15 +197,16 @@ struct ResizeArgs {
     int* dst;
     u32 seqs, width, block, freed_rows, freed_width, pages;
     // workspace
-    u32* asked;    // [seqs + 1] blocks that earlier sequences ask for
     u32* free_part;   // [kMaxParts * kPageWarps] free pages of a warp's share
-    u32* claim_part;  // [kMaxParts] claims of a block's share
-    int* claims;   // [pages] of a shared page: how often it is asked for
-    int* last;     // [pages] and by which sequence last
-    int* pool;     // free pages in ascending order, as many as may be asked for
-    u8* state;     // [asked] what becomes of an asked block
+    u32* asked_part;  // [kMaxParts * kPageWarps] asked blocks of a warp's runs
+    u32* claim_part;  // [kMaxParts * kPageWarps] claims of a warp's runs
+    u32* free_all;    // free pages
+    int* claims;      // [pages] of a shared page: how often it is asked for
+    int* last;        // [pages] and by which sequence last
+    int* pool;        // the first free pages in ascending order
+    u8* state;        // [seqs][width] what becomes of an asked block
 };
-enum State : u8 { kKeep = 0, kNew = 1, kPart = 2, kStays = 3 };
+enum State : u32 { kKeep = 0, kNew = 1, kPart = 2, kStays = 3 };
 
 struct Row {
     u32 held, goal, first, need;  // tokens; asked blocks [first, need) if goal > held
@@ -196,232 +221,264 @@ __device__ __forceinline__ Row row_of(const ResizeArgs& a, u32 s)
     return r;
 }
 
-// The counts of a pool into their new place.
-__device__ __forceinline__ void copy_counts(const int* from, int* to, u32 n, const KvTeam& team)
+// Runs of the table's rows that are a warp's, in order: [from, end).
+struct Runs {
+    u64 from, end;
+    u32 per_row;
+};
+__device__ __forceinline__ Runs runs_of(const ResizeArgs& a, const KvTeam& team)
 {
-    if (from == to) return;
-    const bool wide = (reinterpret_cast<std::uintptr_t>(to) & 15) == 0;
-    const Share own = warp_share(n, team);
-#pragma unroll 4
-    for (u32 p = own.from + (threadIdx.x & 31u) * 4; p < own.end; p += 128) {
-        const Four f = load_four(from, p, own.end, 0);
-        if (wide && p + 4 <= own.end) {
-            *reinterpret_cast<int4*>(to + p) = make_int4(f.x[0], f.x[1], f.x[2], f.x[3]);
-        } else {
-#pragma unroll
-            for (u32 i = 0; i < 4; ++i)
-                if (p + i < own.end) to[p + i] = f.x[i];
-        }
+    const u32 per_row = (a.width + 32 * kDeep - 1) / (32 * kDeep);
+    const u64 units = static_cast<u64>(a.seqs) * per_row, warps = team.size * kPageWarps;
+    const u64 warp = team.rank * kPageWarps + (threadIdx.x >> 5);
+    const u64 each = (units + warps - 1) / warps;
+    return {min(each * warp, units), min(each * (warp + 1), units), per_row};
+}
+
+// A run: entries [first, end) of a row, of which blocks [from, to) are asked for.
+struct Run {
+    u32 seq, first, end, from, to;
+    Row row;
+    const int* in;
+    int* out;
+    u8* state;
+
+    __device__ __forceinline__ Run(const ResizeArgs& a, const Runs& runs, u64 u)
+    {
+        seq = static_cast<u32>(u / runs.per_row);
+        first = static_cast<u32>(u - static_cast<u64>(seq) * runs.per_row) * 32 * kDeep;
+        end = min(first + 32 * kDeep, a.width);
+        row = row_of(a, seq);
+        from = max(first, row.first);
+        to = row.goal > row.held ? min(row.need, end) : 0;
+        in = a.table + static_cast<i64>(seq) * a.table_stride;
+        out = a.table_out + static_cast<i64>(seq) * a.table_out_stride;
+        state = a.state + static_cast<u64>(seq) * a.width;
+    }
+};
+// The asked blocks of a warp's runs, in order, 128 at a time: asked(run, j), where the lane's blocks
+// are j + 32 i, i < kStep, as far as they lie before run.to.  Most runs of a decode step ask for none,
+// those of a prompt for all: loops of a few loads each keep the instructions few, which bound a
+// cluster's 8 SMs.
+constexpr u32 kStep = 4;
+template <typename Asked>
+__device__ __forceinline__ void for_asked(const ResizeArgs& a, const KvTeam& team, const Asked& asked)
+{
+    const Runs runs = runs_of(a, team);
+#pragma unroll 1
+    for (u64 u = runs.from; u < runs.end; ++u) {
+        const Run run(a, runs, u);
+#pragma unroll 1
+        for (u32 j = run.from; j < run.to; j += 32 * kStep) asked(run, j + (threadIdx.x & 31u));
     }
 }
 
-// Counts into their new place, rows' asked blocks added up.
-__device__ void resize_begin(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
+// Counts into their new place.
+__device__ void resize_begin(const ResizeArgs& a, const KvTeam& team)
 {
-    const u32 at = team.rank * blockDim.x + threadIdx.x, threads = team.size * blockDim.x;
     copy_counts(a.refs, a.refs_out, a.pages, team);
-    for (u32 s = at; s < a.seqs; s += threads) {
+    const u32 threads = team.size * blockDim.x;
+    for (u32 s = team.rank * blockDim.x + threadIdx.x; s < a.seqs; s += threads) {
         a.limits[s] = static_cast<int>(row_of(a, s).goal);
         a.src[s] = a.dst[s] = -1;
     }
-    if (team.rank) return;
-    u32 sum = 0;
-    for (u32 s0 = 0; s0 < a.seqs; s0 += blockDim.x) {
-        const u32 s = s0 + threadIdx.x;
-        u32 mine = 0;
-        if (s < a.seqs) {
-            const Row r = row_of(a, s);
-            mine = r.goal > r.held ? r.need - r.first : 0;
-        }
-        const u32 upto = kv_block_scan(mine, sm.warp_sums);
-        if (s < a.seqs) a.asked[s] = sum + upto - mine;
-        sum += sm.warp_sums[32];
-    }
-    if (threadIdx.x == 0) a.asked[a.seqs] = sum;
 }
 
-// What lies behind the rows' new ends goes back, and what an eviction freed.
-__device__ void resize_back(const ResizeArgs& a, const KvTeam& team)
+// What lies behind the rows' new ends goes back.
+__device__ __forceinline__ void resize_rows(const ResizeArgs& a, const KvTeam& team)
 {
     const u32 lane = threadIdx.x & 31u;
-    for_runs(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
-        const int* from = a.table + static_cast<i64>(s) * a.table_stride;
-        int* to = a.table_out + static_cast<i64>(s) * a.table_out_stride;
+    const bool apart = a.table_out != a.table;
+    const Runs runs = runs_of(a, team);
+    for (u64 u = runs.from; u < runs.end; ++u) {
+        const Run run(a, runs, u);
+        const bool still = run.end <= run.row.need && run.from >= run.to;  // nothing happens to these
+        if (still && !apart) continue;
         int e[kDeep];
-        load_run(from, first, end, e);
-        const Row r = row_of(a, s);
+        load_run(run.in, run.first, run.end, e);
+        if (still) {
+#pragma unroll
+            for (u32 i = 0; i < kDeep; ++i)
+                if (run.first + lane + 32 * i < run.end) run.out[run.first + lane + 32 * i] = e[i];
+            continue;
+        }
 #pragma unroll
         for (u32 i = 0; i < kDeep; ++i) {
-            const u32 j = first + lane + 32 * i;
-            if (j >= end) break;
-            const bool there = static_cast<u32>(e[i]) < a.pages, behind = j >= r.need;
-            if (there && behind) {
-                atomicSub(a.refs_out + e[i], 1);
-            } else if (there && j >= r.first && r.goal > r.held) {  // asked for; counted in the next pass
+            const u32 j = run.first + lane + 32 * i;
+            const bool there = static_cast<u32>(e[i]) < a.pages, behind = j >= run.row.need;
+            if (there && behind) atomicSub(a.refs_out + e[i], 1);
+            if (there && j >= run.from && j < run.to) {  // asked for: counted in the next pass
                 a.claims[e[i]] = 0;
                 a.last[e[i]] = -1;
             }
-            if (to != from || (behind && e[i] != -1)) to[j] = behind ? -1 : e[i];
+            if (j < run.end && (apart || (behind && e[i] != -1))) run.out[j] = behind ? -1 : e[i];
         }
-    });
-    for_runs(a.freed_rows, a.freed_width, team, [&](u32 s, u32 first, u32 end) {
-        end = min(end, static_cast<u32>(max(a.freed_counts[s], 0)));
-        if (first >= end) return;
-        int e[kDeep];
-        load_run(a.freed + static_cast<u64>(s) * a.freed_width, first, end, e);
+    }
+}
+
+// And what an eviction freed.
+__device__ void give_back_listed(const ResizeArgs& a, const KvTeam& team)
+{
+    for (u32 r = (threadIdx.x >> 5) * team.size + team.rank; r < a.freed_rows; r += team.size * kPageWarps) {
+        const int* list = a.freed + static_cast<u64>(r) * a.freed_width;
+        const u32 end = min(static_cast<u32>(max(a.freed_counts[r], 0)), a.freed_width);
+#pragma unroll 1
+        for (u32 j = 0; j < end; j += 128) {
+            int e[4];
+            load_run(list, j, end, e);
 #pragma unroll
-        for (u32 i = 0; i < kDeep; ++i)
-            if (static_cast<u32>(e[i]) < a.pages) atomicSub(a.refs_out + e[i], 1);
-    });
-}
-
-// The asked blocks of a thread block, and the sums that find their sequences.
-struct AskedShare {
-    u32 from, end, all;
-    const u32* sums;
-};
-__device__ __forceinline__ AskedShare asked_share(const ResizeArgs& a, const KvTeam& team, PageShared& sm)
-{
-    const u32 all = a.asked[a.seqs];
-    const Share own = share_of(all, kPageThreads, team);
-    const bool close = a.seqs <= kSeqsShared;
-    if (close && own.from < own.end) {
-        for (u32 s = threadIdx.x; s <= a.seqs; s += blockDim.x) sm.asked[s] = a.asked[s];
-        __syncthreads();
-    }
-    return {own.from, own.end, all, close ? sm.asked : a.asked};
-}
-
-// Asked block i: its sequence (the last whose blocks begin at or before it), its place in the table.
-struct Asked {
-    u32 seq, block, first, held;
-    int* entry;
-};
-__device__ __forceinline__ Asked asked_at(const ResizeArgs& a, const u32* sums, u32 i)
-{
-    u32 lo = 0, hi = a.seqs;
-    while (hi - lo > 1) {
-        const u32 mid = (lo + hi) >> 1;
-        if (sums[mid] <= i) lo = mid;
-        else hi = mid;
-    }
-    const u32 held = static_cast<u32>(kv_length(a.lengths, lo, a.width, a.block)), first = held / a.block;
-    const u32 j = first + (i - sums[lo]);
-    return {lo, j, first, held, a.table_out + static_cast<i64>(lo) * a.table_out_stride + j};
-}
-
-// Free pages are counted, and how often shared pages are asked for.
-__device__ void resize_count(const ResizeArgs& a, const KvTeam& team, const AskedShare& asked)
-{
-    for (u32 i = asked.from + threadIdx.x; i < asked.end; i += blockDim.x) {
-        const Asked x = asked_at(a, asked.sums, i);
-        const int e = *x.entry;
-        if (static_cast<u32>(e) < a.pages && a.refs_out[e] > 1) {
-            atomicAdd(a.claims + e, 1);
-            atomicMax(a.last + e, static_cast<int>(x.seq));
+            for (u32 i = 0; i < 4; ++i)
+                if (static_cast<u32>(e[i]) < a.pages) atomicSub(a.refs_out + e[i], 1);
         }
     }
-    const u32 free = count_marked(a.refs_out, a.pages, team, 1, [](int x) { return x < 1; });
-    if ((threadIdx.x & 31u) == 0) a.free_part[team.rank * kPageWarps + (threadIdx.x >> 5)] = free;
 }
 
-// Free pages in ascending order, as many as may be asked for; what becomes of the asked blocks.
-__device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, const AskedShare& asked, PageShared& sm)
+__device__ void resize_back(const ResizeArgs& a, const KvTeam& team)
+{
+    resize_rows(a, team);
+    give_back_listed(a, team);
+}
+
+// How often shared pages are asked for, and how many are free.
+__device__ void resize_count(const ResizeArgs& a, const KvTeam& team)
+{
+    u32 asked = 0;
+    for_asked(a, team, [&](const Run& run, u32 j) {
+        int e[kStep], count[kStep];
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i) {
+            asked += j + 32 * i < run.to;
+            e[i] = j + 32 * i < run.to ? run.out[j + 32 * i] : -1;
+        }
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i) count[i] = static_cast<u32>(e[i]) < a.pages ? a.refs_out[e[i]] : 0;
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i)
+            if (count[i] > 1) {
+                atomicAdd(a.claims + e[i], 1);
+                atomicMax(a.last + e[i], static_cast<int>(run.seq));
+            }
+    });
+    const u32 free = count_marked(a.refs_out, a.pages, team, 1, [](int x) { return x < 1; });
+    asked = __reduce_add_sync(0xffffffffu, asked);
+    if ((threadIdx.x & 31u) == 0) {
+        a.free_part[team.rank * kPageWarps + (threadIdx.x >> 5)] = free;
+        a.asked_part[team.rank * kPageWarps + (threadIdx.x >> 5)] = asked;
+    }
+}
+
+// What becomes of the asked blocks; the free pages in ascending order, as many as may be asked for.
+__device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, u32 (*warp_sums)[kPageWarps])
 {
     u32 claims = 0;
-    for (u32 i = asked.from + threadIdx.x; i < asked.end; i += blockDim.x) {
-        const Asked x = asked_at(a, asked.sums, i);
-        const int e = *x.entry;
-        u8 state = kNew;
-        if (static_cast<u32>(e) < a.pages) {
-            state = kKeep;
-            if (const int count = a.refs_out[e]; count > 1)
-                state = a.claims[e] >= count && a.last[e] == static_cast<int>(x.seq) ? kStays : kPart;
-        }
-        a.state[i] = state;
-        claims += state == kNew || state == kPart;
-    }
-    claims = block_sum(claims, sm.warp_sums);
-    if (threadIdx.x == 0) a.claim_part[team.rank] = claims;
-    u32 rank = before_of(a.free_part, team, sm.warp_sums).mine;
-    const Share own = warp_share(a.pages, team);
-    for (u32 p0 = own.from; p0 < own.end && rank < asked.all; p0 += 128) {
-        const u32 p = p0 + (threadIdx.x & 31u) * 4;
-        const Four f = load_four(a.refs_out, p, own.end, 1);
-        const bool free[4] = {f.x[0] < 1, f.x[1] < 1, f.x[2] < 1, f.x[3] < 1};
-        const Ranks r = rank_four(free);
+    for_asked(a, team, [&](const Run& run, u32 j) {
+        int e[kStep], count[kStep];
 #pragma unroll
-        for (u32 i = 0; i < 4; ++i)
-            if (free[i] && rank + r.before[i] < asked.all) a.pool[rank + r.before[i]] = static_cast<int>(p + i);
-        rank += r.all;
+        for (u32 i = 0; i < kStep; ++i) e[i] = j + 32 * i < run.to ? run.out[j + 32 * i] : -1;
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i) count[i] = static_cast<u32>(e[i]) < a.pages ? a.refs_out[e[i]] : 0;
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i) {
+            if (j + 32 * i >= run.to) break;
+            State state = static_cast<u32>(e[i]) < a.pages ? kKeep : kNew;
+            if (count[i] > 1)
+                state = a.claims[e[i]] >= count[i] && a.last[e[i]] == static_cast<int>(run.seq) ? kStays : kPart;
+            run.state[j + 32 * i] = static_cast<u8>(state);
+            claims += state == kNew || state == kPart;
+        }
+    });
+    claims = __reduce_add_sync(0xffffffffu, claims);
+    if ((threadIdx.x & 31u) == 0) a.claim_part[team.rank * kPageWarps + (threadIdx.x >> 5)] = claims;
+    const Before before = before_of(a.free_part, team, warp_sums, a.asked_part);
+    if (team.rank == 0 && threadIdx.x == 0) *a.free_all = before.all;
+    u32 rank = before.mine;
+    const Share own = warp_share(a.pages, team);
+#pragma unroll 1
+    for (u32 p0 = own.from; p0 < own.end && rank < before.others; p0 += 512) {
+        const u32 p = p0 + (threadIdx.x & 31u) * 4;
+        Four f[4];
+#pragma unroll
+        for (u32 k = 0; k < 4; ++k) f[k] = load_four(a.refs_out, p + 128 * k, own.end, 1);
+#pragma unroll
+        for (u32 k = 0; k < 4; ++k) {
+            const bool free[4] = {f[k].x[0] < 1, f[k].x[1] < 1, f[k].x[2] < 1, f[k].x[3] < 1};
+            const Ranks r = rank_four(free);
+#pragma unroll
+            for (u32 i = 0; i < 4; ++i)
+                if (free[i] && rank + r.before[i] < before.others)
+                    a.pool[rank + r.before[i]] = static_cast<int>(p + 128 * k + i);
+            rank += r.all;
+        }
     }
 }
 
 // Claims get their pages.
-__device__ void resize_give(const ResizeArgs& a, const KvTeam& team, const AskedShare& asked, PageShared& sm)
+__device__ void resize_give(const ResizeArgs& a, const KvTeam& team, u32 (*warp_sums)[kPageWarps])
 {
-    if (asked.from >= asked.end) return;
-    const u32 lane = threadIdx.x & 31u;
-    u32 free = 0, rank = 0;  // free pages; claims of earlier blocks: by every warp for itself
-    for (u32 i = lane; i < team.size * kPageWarps; i += 32) free += a.free_part[i];
-    for (u32 i = lane; i < team.rank; i += 32) rank += a.claim_part[i];
-    free = __reduce_add_sync(0xffffffffu, free);
-    rank = __reduce_add_sync(0xffffffffu, rank);
-    for (u32 i0 = asked.from; i0 < asked.end; i0 += blockDim.x) {
-        const u32 i = i0 + threadIdx.x;
-        const u8 state = i < asked.end ? a.state[i] : kKeep;
-        const bool claim = state == kNew || state == kPart;
-        const u32 upto = kv_block_scan(claim, sm.warp_sums);
-        const u32 before = rank + upto - claim;
-        rank += sm.warp_sums[32];
-        if (state == kKeep) continue;
-        const Asked x = asked_at(a, asked.sums, i);
-        if (claim ? before >= free : before > free) {  // not served
-            atomicMin(a.limits + x.seq, static_cast<int>(max(x.held, x.block * a.block)));
-        } else if (claim) {
-            const int page = a.pool[before];
-            if (state == kPart) {
-                const int old = *x.entry;
-                atomicSub(a.refs_out + old, 1);
-                if (x.block == x.first && x.held % a.block) {
-                    a.src[x.seq] = old;
-                    a.dst[x.seq] = page;
-                }
-            }
-            a.refs_out[page] = 1;
-            *x.entry = page;
+    const u32 lane = threadIdx.x & 31u, free = *a.free_all;
+    u32 rank = before_of(a.claim_part, team, warp_sums).mine;
+    for_asked(a, team, [&](const Run& run, u32 j) {
+        u32 state[kStep], before[kStep];
+        int page[kStep];
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i) state[i] = j + 32 * i < run.to ? run.state[j + 32 * i] : kKeep;
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i) {
+            const bool claim = state[i] == kNew || state[i] == kPart;
+            const u32 who = __ballot_sync(0xffffffffu, claim);
+            before[i] = rank + __popc(who & ((1u << lane) - 1));
+            rank += __popc(who);
+            page[i] = claim && before[i] < free ? a.pool[before[i]] : -1;
         }
-    }
+#pragma unroll
+        for (u32 i = 0; i < kStep; ++i) {
+            if (state[i] == kKeep) continue;
+            const u32 block = j + 32 * i;
+            if (state[i] == kStays ? before[i] > free : page[i] < 0) {  // not served
+                atomicMin(a.limits + run.seq, static_cast<int>(max(run.row.held, block * a.block)));
+            } else if (state[i] != kStays) {
+                if (state[i] == kPart) {
+                    const int old = run.out[block];
+                    atomicSub(a.refs_out + old, 1);
+                    if (block == run.row.first && run.row.held % a.block) {
+                        a.src[run.seq] = old;
+                        a.dst[run.seq] = page[i];
+                    }
+                }
+                a.refs_out[page[i]] = 1;
+                run.out[block] = page[i];
+            }
+        }
+    });
 }
 
 __global__ void __launch_bounds__(kPageThreads) resize_cluster_kernel(const ResizeArgs a)
 {
-    __shared__ PageShared sm;
-    const KvTeam team{blockIdx.x, kPageTeam};
-    resize_begin(a, team, sm);
-    kv_team_sync(team);
+    __shared__ u32 warp_sums[3][kPageWarps];
+    const KvTeam team{blockIdx.x, gridDim.x};
+    resize_begin(a, team);
+    if (a.refs_out != a.refs) kv_team_sync(team);
     resize_back(a, team);
     kv_team_sync(team);
-    const AskedShare asked = asked_share(a, team, sm);
-    resize_count(a, team, asked);
+    resize_count(a, team);
     kv_team_sync(team);
-    resize_rank(a, team, asked, sm);
+    resize_rank(a, team, warp_sums);
     kv_team_sync(team);
-    resize_give(a, team, asked, sm);
+    resize_give(a, team, warp_sums);
 }
 
 template <int kPass>
 __global__ void __launch_bounds__(kPageThreads) resize_pass_kernel(const ResizeArgs a)
 {
-    __shared__ PageShared sm;
+    __shared__ u32 warp_sums[3][kPageWarps];
     kv_let_next();
     kv_wait_before();
     const KvTeam team{blockIdx.x, gridDim.x};
-    if constexpr (kPass == 0) resize_begin(a, team, sm);
+    if constexpr (kPass == 0) resize_begin(a, team);
     else if constexpr (kPass == 1) resize_back(a, team);
-    else if constexpr (kPass == 2) resize_count(a, team, asked_share(a, team, sm));
-    else if constexpr (kPass == 3) resize_rank(a, team, asked_share(a, team, sm), sm);
-    else resize_give(a, team, asked_share(a, team, sm), sm);
+    else if constexpr (kPass == 2) resize_count(a, team);
+    else if constexpr (kPass == 3) resize_rank(a, team, warp_sums);
+    else resize_give(a, team, warp_sums);
 }
 
 // ---------------------------------------------------------------------------
@@ -453,15 +510,15 @@ __device__ void fork_rows(const ForkArgs& a, const KvTeam& team)
         const u32 parent = static_cast<u32>(a.parents[r]);
         a.lengths_out[r] = parent < a.seqs ? kv_length(a.lengths, parent, a.width, a.block) : 0;
     }
-    for_runs(a.rows, a.width, team, [&](u32 r, u32 first, u32 end) {
+    for_runs<8>(a.rows, a.width, team, [&](u32 r, u32 first, u32 end) {
         const u32 parent = static_cast<u32>(a.parents[r]);
         const u32 blocks = parent < a.seqs ? blocks_held(a, parent) : 0;
         const int* from = a.table + static_cast<i64>(parent < a.seqs ? parent : 0) * a.table_stride;
         int* to = a.table_out + static_cast<u64>(r) * a.width;
-        int e[kDeep];
+        int e[8];
         load_run(from, first, min(end, blocks), e);
 #pragma unroll
-        for (u32 i = 0; i < kDeep; ++i)
+        for (u32 i = 0; i < 8; ++i)
             if (first + lane + 32 * i < end) to[first + lane + 32 * i] = e[i];
     });
 }
@@ -470,8 +527,8 @@ __device__ void fork_rows(const ForkArgs& a, const KvTeam& team)
 __device__ void fork_count(const ForkArgs& a, const KvTeam& team)
 {
     const u32 lane = threadIdx.x & 31u;
-    for_runs(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
-        int e[kDeep];
+    for_runs<4>(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
+        int e[4];
         load_run(a.table + static_cast<i64>(s) * a.table_stride, first, end, e);
         const u32 blocks = blocks_held(a, s);
         u32 children = 0;
@@ -479,23 +536,15 @@ __device__ void fork_count(const ForkArgs& a, const KvTeam& team)
         for (u32 r = lane; r < a.rows; r += 32) children += a.parents[r] == static_cast<int>(s);
         children = __reduce_add_sync(0xffffffffu, children);
 #pragma unroll
-        for (u32 i = 0; i < kDeep; ++i) {
+        for (u32 i = 0; i < 4; ++i) {
             const int by = first + lane + 32 * i < blocks ? static_cast<int>(children) - 1 : -1;
             if (by != 0 && static_cast<u32>(e[i]) < a.pages) atomicAdd(a.refs_out + e[i], by);
         }
     });
 }
 
-__global__ void __launch_bounds__(kPageThreads) fork_cluster_kernel(const ForkArgs a)
-{
-    const KvTeam team{blockIdx.x, kPageTeam};
-    fork_rows(a, team);
-    kv_team_sync(team);
-    fork_count(a, team);
-}
-
 template <int kPass>
-__global__ void __launch_bounds__(kPageThreads) fork_pass_kernel(const ForkArgs a)
+__global__ void __launch_bounds__(kPageThreads, 2) fork_pass_kernel(const ForkArgs a)
 {
     kv_let_next();
     kv_wait_before();
@@ -533,9 +582,9 @@ __device__ void compact_count(const CompactArgs& a, const KvTeam& team)
 // The moves: page p in use past the n that are has n - (pages in use up to p) such pages above it,
 // free page p below has p - (pages in use before p) free ones below it.  Until the next pass, `where`
 // holds -2 - move of a page that moves.
-__device__ void compact_rank(const CompactArgs& a, const KvTeam& team, PageShared& sm)
+__device__ void compact_rank(const CompactArgs& a, const KvTeam& team, u32 (*warp_sums)[kPageWarps])
 {
-    const Before before = before_of(a.live_part, team, sm.warp_sums);
+    const Before before = before_of(a.live_part, team, warp_sums);
     const u32 n = before.all;
     if (team.rank == 0 && threadIdx.x == 0) *a.live = static_cast<int>(n);
     const Share own = warp_share(a.pages, team);
@@ -545,14 +594,15 @@ __device__ void compact_rank(const CompactArgs& a, const KvTeam& team, PageShare
         const Four f = load_four(a.refs, first, own.end, 0);
         const bool live[4] = {f.x[0] > 0, f.x[1] > 0, f.x[2] > 0, f.x[3] > 0};
         const Ranks r = rank_four(live);
+        Four place;
 #pragma unroll
         for (u32 i = 0; i < 4; ++i) {
             const u32 p = first + i, earlier = rank + r.before[i];  // pages in use before p
-            if (p >= own.end) break;
-            int place = -1;
+            place.x[i] = -1;
+            if (p >= own.end) continue;
             if (p < n) {
                 if (live[i]) {
-                    place = static_cast<int>(p);
+                    place.x[i] = static_cast<int>(p);
                     if (a.refs_out != a.refs) a.refs_out[p] = f.x[i];
                 } else {
                     a.dst[p - earlier] = static_cast<int>(p);  // its count comes with the page
@@ -560,12 +610,12 @@ __device__ void compact_rank(const CompactArgs& a, const KvTeam& team, PageShare
             } else if (live[i]) {
                 const u32 move = n - 1 - earlier;
                 a.src[move] = static_cast<int>(p);
-                place = -2 - static_cast<int>(move);  // its count leaves with the page
+                place.x[i] = -2 - static_cast<int>(move);  // its count leaves with the page
             } else {
                 a.refs_out[p] = 0;
             }
-            a.where[p] = place;
         }
+        if (first < own.end) store_four(a.where, first, own.end, place);
         rank += r.all;
     }
 }
@@ -574,18 +624,18 @@ __device__ void compact_move(const CompactArgs& a, const KvTeam& team)
 {
     const u32 lane = threadIdx.x & 31u, threads = team.size * blockDim.x, room = a.pages / 2;
     // entries: a page that moves is found by its number or, if the loop below was faster, by its place
-    for_runs(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
+    for_runs<8>(a.seqs, a.width, team, [&](u32 s, u32 first, u32 end) {
         int* to = a.table_out + static_cast<i64>(s) * a.table_out_stride;
-        int e[kDeep];
-        bool there[kDeep];
+        int e[8];
+        bool there[8];
         load_run(a.table + static_cast<i64>(s) * a.table_stride, first, end, e);
 #pragma unroll
-        for (u32 i = 0; i < kDeep; ++i) {
+        for (u32 i = 0; i < 8; ++i) {
             there[i] = static_cast<u32>(e[i]) < a.pages;
             if (there[i]) e[i] = *static_cast<volatile int*>(a.where + e[i]);
         }
 #pragma unroll
-        for (u32 i = 0; i < kDeep; ++i) {
+        for (u32 i = 0; i < 8; ++i) {
             if (there[i] && e[i] < -1) e[i] = a.dst[-2 - e[i]];
             if (first + lane + 32 * i < end) to[first + lane + 32 * i] = e[i];
         }
@@ -602,8 +652,8 @@ __device__ void compact_move(const CompactArgs& a, const KvTeam& team)
 
 __global__ void __launch_bounds__(kPageThreads) compact_cluster_kernel(const CompactArgs a)
 {
-    __shared__ PageShared sm;
-    const KvTeam team{blockIdx.x, kPageTeam};
+    __shared__ u32 sm[3][kPageWarps];
+    const KvTeam team{blockIdx.x, gridDim.x};
     compact_count(a, team);
     kv_team_sync(team);
     compact_rank(a, team, sm);
@@ -612,9 +662,9 @@ __global__ void __launch_bounds__(kPageThreads) compact_cluster_kernel(const Com
 }
 
 template <int kPass>
-__global__ void __launch_bounds__(kPageThreads) compact_pass_kernel(const CompactArgs a)
+__global__ void __launch_bounds__(kPageThreads, 2) compact_pass_kernel(const CompactArgs a)
 {
-    __shared__ PageShared sm;
+    __shared__ u32 sm[3][kPageWarps];
     kv_let_next();
     kv_wait_before();
     const KvTeam team{blockIdx.x, gridDim.x};
@@ -716,15 +766,16 @@ struct Room {
 };
 
 struct ResizeRoom {
-    u64 asked, free_part, claim_part, claims, last, pool, state, bytes;
+    u64 free_part, asked_part, claim_part, free_all, claims, last, pool, state, bytes;
 };
 ResizeRoom resize_room(const hbfsim_kv_resize_batch_v1& b)
 {
     Room room;
     ResizeRoom r{};
-    r.asked = room.take((u64{b.seqs} + 1) * 4);
     r.free_part = room.take(kMaxParts * kPageWarps * 4);
-    r.claim_part = room.take(kMaxParts * 4);
+    r.asked_part = room.take(kMaxParts * kPageWarps * 4);
+    r.claim_part = room.take(kMaxParts * kPageWarps * 4);
+    r.free_all = room.take(4);
     r.claims = room.take(b.pages * 4);
     r.last = room.take(b.pages * 4);
     r.pool = room.take(std::min(b.pages, u64{b.seqs} * b.width) * 4);
@@ -753,9 +804,18 @@ bool pass(void (*kernel)(Args), u32 blocks, bool behind, const Args& a, cudaStre
 }
 
 template <typename Args>
-bool cluster(void (*kernel)(Args), const Args& a, cudaStream_t s)
+bool cluster(void (*kernel)(Args), u32 team, const Args& a, cudaStream_t s)
 {
-    return kv_launch(kernel, dim3(kPageTeam), kPageThreads, s, 0, kPageTeam, false, a);
+    return kv_launch(kernel, dim3(team), kPageThreads, s, 0, team, false, a);
+}
+
+// Blocks of a cluster that does `counts` counts and `entries` entries in one launch; 0: too much for
+// it.  (The entries of an eviction's lists are not counted: few of their places are taken.)
+u32 cluster_size(u64 counts, u64 entries)
+{
+    u32 team = 1;
+    while (team < kPageTeam && (counts > team * kCountsEach || entries > team * kEntriesEach)) team *= 2;
+    return counts > kPageTeam * kCountsMost || entries > team * kEntriesMost ? 0 : team;
 }
 
 u32 pass_blocks() { return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count())); }
@@ -805,13 +865,14 @@ extern "C" int hbfsim_kv_resize_v1(const hbfsim_kv_resize_batch_v1* b, void* str
     const ResizeArgs a{b->refs, b->table, b->table_stride, b->lengths, b->want, b->freed, b->freed_counts,
                        b->refs_out, b->table_out, b->table_out_stride, b->limits, b->src, b->dst, b->seqs, b->width,
                        b->block_tokens, listed ? b->freed_rows : 0, b->freed_width, static_cast<u32>(b->pages),
-                       reinterpret_cast<u32*>(w + room.asked), reinterpret_cast<u32*>(w + room.free_part),
-                       reinterpret_cast<u32*>(w + room.claim_part), reinterpret_cast<int*>(w + room.claims),
+                       reinterpret_cast<u32*>(w + room.free_part), reinterpret_cast<u32*>(w + room.asked_part),
+                       reinterpret_cast<u32*>(w + room.claim_part),
+                       reinterpret_cast<u32*>(w + room.free_all), reinterpret_cast<int*>(w + room.claims),
                        reinterpret_cast<int*>(w + room.last), reinterpret_cast<int*>(w + room.pool), w + room.state};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     bool ok;
-    if (b->pages + entries + listed <= kClusterElements) {
-        ok = cluster(resize_cluster_kernel, a, s);
+    if (const u32 team = cluster_size(b->pages, entries)) {
+        ok = cluster(resize_cluster_kernel, team, a, s);
     } else {
         const u32 blocks = pass_blocks();
         ok = pass(resize_pass_kernel<0>, blocks, false, a, s) && pass(resize_pass_kernel<1>, blocks, true, a, s) &&
@@ -849,15 +910,10 @@ extern "C" int hbfsim_kv_fork_v1(const hbfsim_kv_fork_batch_v1* b, void* stream)
                      b->lengths_out, b->seqs, b->rows, b->width, b->block_tokens, static_cast<u32>(b->pages)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool apart = b->refs_out != b->refs;
-    bool ok;
+    // counts that are where they belong need no pass of their own
     const u32 blocks = pass_blocks();
-    if (!apart) {  // the counts are where they belong: no pass waits for another
-        ok = pass(fork_pass_kernel<2>, blocks, false, a, s);
-    } else if (b->pages + entries + made <= kClusterElements) {
-        ok = cluster(fork_cluster_kernel, a, s);
-    } else {
-        ok = pass(fork_pass_kernel<0>, blocks, false, a, s) && pass(fork_pass_kernel<1>, blocks, true, a, s);
-    }
+    const bool ok = apart ? pass(fork_pass_kernel<0>, blocks, false, a, s) && pass(fork_pass_kernel<1>, blocks, true, a, s)
+                          : pass(fork_pass_kernel<2>, blocks, false, a, s);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
 
@@ -901,8 +957,8 @@ extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* s
                         static_cast<u32*>(b->workspace)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     bool ok;
-    if (b->pages + entries <= kClusterElements) {
-        ok = cluster(compact_cluster_kernel, a, s);
+    if (const u32 team = cluster_size(b->pages, entries)) {
+        ok = cluster(compact_cluster_kernel, team, a, s);
     } else {
         const u32 blocks = pass_blocks();
         ok = pass(compact_pass_kernel<0>, blocks, false, a, s) && pass(compact_pass_kernel<1>, blocks, true, a, s) &&

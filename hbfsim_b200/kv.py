@@ -46,9 +46,11 @@ _ATTENTION = struct.Struct("<2IfI7Q")
 _EVICT = struct.Struct("<10I3Qq6Q")
 _ROTARY = struct.Struct("<6IQ2q2Qq2Q")
 _VERIFY = struct.Struct("<6IQ2qQ2q8Q")
-_RESIZE = struct.Struct("<8I3Qq6Qq5Q")
+_RESIZE = struct.Struct("<8I3Qq6Qq3Q")  # both without their workspace
 _FORK = struct.Struct("<6I3Qq5Q")
-_COMPACT = struct.Struct("<4I3Qq2Qq6Q")
+_COMPACT = struct.Struct("<4I3Qq2Qq4Q")
+_WORKSPACE = struct.Struct("<2Q")
+_NO_WORKSPACE = _WORKSPACE.pack(0, 0)
 
 
 _NO_GRADIENT = "no gradient passes through the cache: detach the tensors or call under torch.no_grad()"
@@ -531,11 +533,11 @@ def kv_verify(target, draft, tokens, accept, sample, counts=None, lengths=None,
     _need(not (target.requires_grad or draft is not None and draft.requires_grad)
           or not torch.is_grad_enabled(), "no gradient passes through a draw: detach the tensors or "
           "call under torch.no_grad()")
-    out = tokens.new_empty((seqs, rows))
     if lengths is None:
-        accepted, kept = tokens.new_empty(seqs), None
+        accepted, kept, out = tokens.new_empty(seqs), None, tokens.new_empty((seqs, rows))
     else:
-        accepted, kept = tokens.new_empty((2, seqs)).unbind()
+        accepted, kept, out = _parts(tokens, seqs, seqs, seqs * rows)
+        out = out.view(seqs, rows)
     batch = _VERIFY.pack(_VERIFY.size, 1, kind, seqs, n, vocab, target.data_ptr(), by_seq, by_token,
                          draft_at, draft_seq, draft_token, tokens.data_ptr(), accept.data_ptr(),
                          sample.data_ptr(), counts.data_ptr() if counts is not None else 0,
@@ -543,6 +545,11 @@ def kv_verify(target, draft, tokens, accept, sample, counts=None, lengths=None,
                          out.data_ptr(), kept.data_ptr() if kept is not None else 0)
     check(_lib.load().hbfsim_kv_verify_v1(batch, _handle(index)), "hbfsim_kv_verify_v1")
     return KvVerified(accepted, out, kept)
+
+
+def _parts(like, *sizes):
+    """New tensors of `like`'s type and device, one after the other in one allocation."""
+    return like.new_empty(sum(sizes)).unsafe_split_with_sizes(sizes)
 
 
 def _check_pool(refs, table, index) -> None:
@@ -572,7 +579,8 @@ def kv_resize(refs, table, lengths, want, block_tokens: int = 16, freed=None, fr
             return kv_resize(refs, table, lengths, want, block_tokens, freed, freed_counts, inplace)
     import torch
     seqs, width = _check_table(index, table, lengths, "lengths")
-    _check_table(index, table, want, "want")
+    _need(want.dtype == torch.int32 and want.shape == lengths.shape and want.is_contiguous()
+          and want.get_device() == index, "want: int32 [seqs] on the table's device, contiguous")
     _check_pool(refs, table, index)
     _need(not block_tokens >> 32, "block_tokens is a count of 32 bits")
     freed_rows = freed_width = freed_at = freed_counts_at = 0
@@ -589,16 +597,18 @@ def kv_resize(refs, table, lengths, want, block_tokens: int = 16, freed=None, fr
     if inplace:
         new_refs, new_table = refs, table
     else:
-        new_refs, new_table = torch.empty_like(refs), refs.new_empty((seqs, width))
-    limits, src, dst = refs.new_empty((3, seqs)).unbind()
-    head = (_RESIZE.size, 1, seqs, width, block_tokens, freed_rows, freed_width, 0, refs.shape[0],
+        new_refs = torch.empty_like(refs)
+        new_table = torch.empty_like(table, memory_format=torch.contiguous_format)
+    limits, src, dst = _parts(refs, seqs, seqs, seqs)
+    batch = _RESIZE.pack(
+            _RESIZE.size + _WORKSPACE.size, 1, seqs, width, block_tokens, freed_rows, freed_width, 0, refs.shape[0],
             refs.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(), want.data_ptr(),
             freed_at, freed_counts_at, new_refs.data_ptr(), new_table.data_ptr(),
             new_table.stride(0), limits.data_ptr(), src.data_ptr(), dst.data_ptr())
     lib = _lib.load()
-    size = lib.hbfsim_kv_resize_workspace_v1(_RESIZE.pack(*head, 0, 0))
-    space = torch.empty(size, dtype=torch.uint8, device=table.device)
-    check(lib.hbfsim_kv_resize_v1(_RESIZE.pack(*head, space.data_ptr(), size), _handle(index)),
+    size = lib.hbfsim_kv_resize_workspace_v1(batch + _NO_WORKSPACE)
+    space = refs.new_empty(size // 4)
+    check(lib.hbfsim_kv_resize_v1(batch + _WORKSPACE.pack(space.data_ptr(), size), _handle(index)),
           "hbfsim_kv_resize_v1")
     return KvResized(new_refs, new_table, limits, src, dst)
 
@@ -625,7 +635,7 @@ def kv_fork(refs, table, lengths, parents, block_tokens: int = 16, inplace: bool
           and parents.get_device() == index, "parents: int32 [rows] on the table's device, contiguous")
     rows = parents.shape[0]
     new_refs = refs if inplace else torch.empty_like(refs)
-    new_table, new_lengths = refs.new_empty((rows, width)), refs.new_empty(rows)
+    new_table, new_lengths = refs.new_empty((rows, width)), torch.empty_like(parents)
     batch = _FORK.pack(_FORK.size, 1, seqs, rows, width, block_tokens, refs.shape[0],
                        refs.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(),
                        parents.data_ptr(), new_refs.data_ptr(), new_table.data_ptr(),
@@ -678,17 +688,19 @@ def kv_compact(refs, table, inplace: bool = False, stream=None) -> KvCompacted:
     if inplace:
         new_refs, new_table = refs, table
     else:
-        new_refs, new_table = torch.empty_like(refs), refs.new_empty((seqs, width))
-    src, dst = refs.new_empty((2, pages // 2)).unbind()
-    live, where = refs.new_empty(1), torch.empty_like(refs)
-    head = (_COMPACT.size, 1, seqs, width, pages, refs.data_ptr(), table.data_ptr(),
+        new_refs = torch.empty_like(refs)
+        new_table = torch.empty_like(table, memory_format=torch.contiguous_format)
+    src, dst, live = _parts(refs, pages // 2, pages // 2, 1)
+    where = torch.empty_like(refs)
+    batch = _COMPACT.pack(
+            _COMPACT.size + _WORKSPACE.size, 1, seqs, width, pages, refs.data_ptr(), table.data_ptr(),
             table.stride(0), new_refs.data_ptr(), new_table.data_ptr(), new_table.stride(0),
             src.data_ptr(), dst.data_ptr(), live.data_ptr(), where.data_ptr())
     lib = _lib.load()
-    size = lib.hbfsim_kv_compact_workspace_v1(_COMPACT.pack(*head, 0, 0))
-    space = torch.empty(size, dtype=torch.uint8, device=table.device)
-    check(lib.hbfsim_kv_compact_v1(_COMPACT.pack(*head, space.data_ptr(), size), _handle(index)),
-          "hbfsim_kv_compact_v1")
+    size = lib.hbfsim_kv_compact_workspace_v1(batch + _NO_WORKSPACE)
+    space = refs.new_empty(size // 4)
+    check(lib.hbfsim_kv_compact_v1(batch + _WORKSPACE.pack(space.data_ptr(), size),
+                                   _handle(index)), "hbfsim_kv_compact_v1")
     return KvCompacted(new_refs, new_table, src, dst, live, where)
 
 

@@ -180,12 +180,15 @@ def test_null_structures(lib):
 def test_packed_structures():
     """The structures that Python packs are those of the header, byte for byte."""
     from hbfsim_b200 import kv
-    for packed, struct in ((kv._ROTARY, _lib.KvRotaryV1), (kv._VERIFY, _lib.KvVerifyBatchV1),
-                           (kv._RESIZE, _lib.KvResizeBatchV1), (kv._FORK, _lib.KvForkBatchV1),
-                           (kv._COMPACT, _lib.KvCompactBatchV1)):
-        assert packed.size == ctypes.sizeof(struct)
+    for packed, struct in (((kv._ROTARY,), _lib.KvRotaryV1), ((kv._VERIFY,), _lib.KvVerifyBatchV1),
+                           ((kv._RESIZE, kv._WORKSPACE), _lib.KvResizeBatchV1),
+                           ((kv._FORK,), _lib.KvForkBatchV1),
+                           ((kv._COMPACT, kv._WORKSPACE), _lib.KvCompactBatchV1)):
+        assert sum(p.size for p in packed) == ctypes.sizeof(struct)
         values = [7 * i + 1 for i in range(len(struct._fields_))]
-        assert packed.pack(*values) == bytes(struct(*values))
+        rest = 2 if len(packed) == 2 else 0
+        parts = (values[:len(values) - rest], values[len(values) - rest:])
+        assert b"".join(p.pack(*v) for p, v in zip(packed, parts)) == bytes(struct(*values))
 
 
 def test_python_refusals():
