@@ -274,7 +274,7 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, u32 head, u32 
     if (side == 0) load_held(0);  // the keys' bounds need them in any case
     const float was = slot ? a.c.scale[at] : 0.0f;
     float most = 0.0f;
-#pragma unroll 2
+#pragma unroll 4
     for (u32 t = 0; t < count; ++t) {
         float2 y[W];
         row(t, y);

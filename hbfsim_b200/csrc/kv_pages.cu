@@ -18,7 +18,11 @@ constexpr u32 kPageThreads = 1024, kPageWarps = kPageThreads / 32;
 constexpr u32 kPageTeam = 8;      // blocks of the cluster
 constexpr u32 kMaxParts = 1024;   // blocks of a pass at most
 constexpr u32 kDeep = 16;         // entries of a table's row that a lane has under way
-// Counts and entries that are worth a block of a cluster, and that one takes at most.
+// Counts and entries that are worth a block of a cluster, and that one takes at most.  A cluster costs
+// about 2 us: a pool of 2,600 counts and 4,000 entries is compacted in 6.2 us by one block, in 8.0 us by
+// two to eight and in 8.4 us by a launch to a pass; before a step of 64 rows of 2048 entries, 70,000
+// counts, a resize takes 17.6 us by 8 blocks and 16.6 us by a launch to a pass, which cost the host 10 us
+// more; 200 rows of 190 entries 17.1 us by 8 blocks and 23.6 us by 4, with two rows to a warp.
 constexpr u64 kCountsEach = 16384, kEntriesEach = 16384, kCountsMost = 32768, kEntriesMost = 16384;
 
 // The elements [from, end) of a warp.
@@ -589,34 +593,40 @@ __device__ void compact_rank(const CompactArgs& a, const KvTeam& team, u32 (*war
     if (team.rank == 0 && threadIdx.x == 0) *a.live = static_cast<int>(n);
     const Share own = warp_share(a.pages, team);
     u32 rank = before.mine;
-    for (u32 p0 = own.from; p0 < own.end; p0 += 128) {
-        const u32 first = p0 + (threadIdx.x & 31u) * 4;
-        const Four f = load_four(a.refs, first, own.end, 0);
-        const bool live[4] = {f.x[0] > 0, f.x[1] > 0, f.x[2] > 0, f.x[3] > 0};
-        const Ranks r = rank_four(live);
-        Four place;
+#pragma unroll 1
+    for (u32 p0 = own.from; p0 < own.end; p0 += 256) {
+        Four f[2];
 #pragma unroll
-        for (u32 i = 0; i < 4; ++i) {
-            const u32 p = first + i, earlier = rank + r.before[i];  // pages in use before p
-            place.x[i] = -1;
-            if (p >= own.end) continue;
-            if (p < n) {
-                if (live[i]) {
-                    place.x[i] = static_cast<int>(p);
-                    if (a.refs_out != a.refs) a.refs_out[p] = f.x[i];
+        for (u32 k = 0; k < 2; ++k) f[k] = load_four(a.refs, p0 + 128 * k + (threadIdx.x & 31u) * 4, own.end, 0);
+#pragma unroll
+        for (u32 k = 0; k < 2; ++k) {
+            const u32 first = p0 + 128 * k + (threadIdx.x & 31u) * 4;
+            const bool live[4] = {f[k].x[0] > 0, f[k].x[1] > 0, f[k].x[2] > 0, f[k].x[3] > 0};
+            const Ranks r = rank_four(live);
+            Four place;
+#pragma unroll
+            for (u32 i = 0; i < 4; ++i) {
+                const u32 p = first + i, earlier = rank + r.before[i];  // pages in use before p
+                place.x[i] = -1;
+                if (p >= own.end) continue;
+                if (p < n) {
+                    if (live[i]) {
+                        place.x[i] = static_cast<int>(p);
+                        if (a.refs_out != a.refs) a.refs_out[p] = f[k].x[i];
+                    } else {
+                        a.dst[p - earlier] = static_cast<int>(p);  // its count comes with the page
+                    }
+                } else if (live[i]) {
+                    const u32 move = n - 1 - earlier;
+                    a.src[move] = static_cast<int>(p);
+                    place.x[i] = -2 - static_cast<int>(move);  // its count leaves with the page
                 } else {
-                    a.dst[p - earlier] = static_cast<int>(p);  // its count comes with the page
+                    a.refs_out[p] = 0;
                 }
-            } else if (live[i]) {
-                const u32 move = n - 1 - earlier;
-                a.src[move] = static_cast<int>(p);
-                place.x[i] = -2 - static_cast<int>(move);  // its count leaves with the page
-            } else {
-                a.refs_out[p] = 0;
             }
+            if (first < own.end) store_four(a.where, first, own.end, place);
+            rank += r.all;
         }
-        if (first < own.end) store_four(a.where, first, own.end, place);
-        rank += r.all;
     }
 }
 
@@ -811,14 +821,19 @@ bool cluster(void (*kernel)(Args), u32 team, const Args& a, cudaStream_t s)
 
 // Blocks of a cluster that does `counts` counts and `entries` entries in one launch; 0: too much for
 // it.  (The entries of an eviction's lists are not counted: few of their places are taken.)
-u32 cluster_size(u64 counts, u64 entries)
+// `runs`: of rows, a warp each.
+u32 cluster_size(u64 counts, u64 entries, u64 runs)
 {
     u32 team = 1;
-    while (team < kPageTeam && (counts > team * kCountsEach || entries > team * kEntriesEach)) team *= 2;
+    while (team < kPageTeam && (counts > team * kCountsEach || entries > team * kEntriesEach || runs > team * kPageWarps))
+        team *= 2;
     return counts > kPageTeam * kCountsMost || entries > team * kEntriesMost ? 0 : team;
 }
 
-u32 pass_blocks() { return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count())); }
+u32 pass_blocks()
+{
+    return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count()));
+}
 
 }  // namespace
 }  // namespace hbfb
@@ -871,7 +886,7 @@ extern "C" int hbfsim_kv_resize_v1(const hbfsim_kv_resize_batch_v1* b, void* str
                        reinterpret_cast<int*>(w + room.last), reinterpret_cast<int*>(w + room.pool), w + room.state};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     bool ok;
-    if (const u32 team = cluster_size(b->pages, entries)) {
+    if (const u32 team = cluster_size(b->pages, entries, u64{b->seqs} * ((b->width + 32 * kDeep - 1) / (32 * kDeep)))) {
         ok = cluster(resize_cluster_kernel, team, a, s);
     } else {
         const u32 blocks = pass_blocks();
@@ -957,7 +972,7 @@ extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* s
                         static_cast<u32*>(b->workspace)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     bool ok;
-    if (const u32 team = cluster_size(b->pages, entries)) {
+    if (const u32 team = cluster_size(b->pages, entries, 0)) {
         ok = cluster(compact_cluster_kernel, team, a, s);
     } else {
         const u32 blocks = pass_blocks();

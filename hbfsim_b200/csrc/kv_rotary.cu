@@ -2,15 +2,17 @@
 // turned by their positions (kv_v1.h).
 //
 // One launch, three kinds of CTA.  Keys: a chunk of tokens as in kv_append.cu, whose
-// blocks' cosines and sines are made once, in shared memory; a warp turns a head's
-// rows of a block twice, for the largest magnitude and for the stored values (the
-// second time from the caches), so the keys never exist in 16 bits.  Values: as in
-// kv_append.cu.  Queries: every warp by itself.  It takes a token's heads, asks for
-// the first rows, makes the token's cosines and sines meanwhile, and reads the next
-// rows while it turns the ones at hand.  Keys and values come first: their CTAs take
-// longest (mixed with the queries' the call took as long).  Products and sums are
-// rounded one by one, so that what is stored does not depend on how a compiler joins
-// them.
+// blocks' cosines and sines are made once, in shared memory; a warp turns up to 16 of
+// a head's rows of a block twice, for the largest magnitude and for the stored values
+// (the second time from the caches), so the keys never exist in 16 bits; blocks of 32
+// or 64 tokens are shared by two or four warps (2,000 tokens in blocks of 64 took 99
+// us by one, 31 us by four).  Values: as in kv_append.cu.  Queries: every warp by
+// itself.  It takes a token's heads, asks for the first rows, makes the token's
+// cosines and sines meanwhile, and reads the next rows while it turns the ones at
+// hand.  Keys and values come first: their CTAs take longest (mixed with the queries'
+// the call took as long).  Products and sums are rounded one by one, so that what is
+// stored does not depend on how a compiler joins them.
+//
 #include "kv_append.cuh"
 
 namespace hbfb {
@@ -284,23 +286,64 @@ __device__ __forceinline__ void store_values(u8* to, const u32 (&b)[N])
     else if constexpr (N == 2) *reinterpret_cast<u32*>(to) = b[0] | b[1] << 16;
     else *reinterpret_cast<uint2*>(to) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
 }
+template <int N>
+__device__ __forceinline__ void load_values(const u8* from, u32 (&b)[N])
+{
+    if constexpr (N == 1) {
+        b[0] = *reinterpret_cast<const u16*>(from);
+    } else if constexpr (N == 2) {
+        const u32 x = *reinterpret_cast<const u32*>(from);
+        b[0] = x & 0xffffu;
+        b[1] = x >> 16;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(from);
+        b[0] = x.x & 0xffffu;
+        b[1] = x.x >> 16;
+        b[2] = x.y & 0xffffu;
+        b[3] = x.y >> 16;
+    }
+}
 
-// A head's keys of a block whose tokens are all new, by one warp; false, with nothing written, where
-// a turned element is not finite.  Rounding keeps the order, so the least and greatest of a channel
-// give its bounds.
+// A head's keys of a block by one warp, a row at a time.
 template <typename T, int D, bool kWide, int kLayout>
-__device__ __forceinline__ bool append_full_turned(const AppendArgs& a, u32 head, u32 token, int page,
-                                                   const Table& table)
+__device__ __forceinline__ void append_rows(const AppendArgs& a, u32 head, u32 token, int page, u32 slot, u32 count,
+                                         const Table& table)
+{
+    const PlainRow<T, D, kWide> from(a, head, 0, token);
+    append_block<D>(a, head, 0, page, slot, count, TurnedRow<T, D, kWide, kLayout>{from.x, from.stride, table});
+}
+
+// Where the warps that share a block meet: each 16 of its rows.
+template <int D>
+struct Join {
+    float most[kRotaryWarps];
+    float ends[kRotaryWarps][2][D];  // least and greatest of the channels
+};
+
+// A head's keys of a block by `parts` warps (block / 16 of them), of which this is the part-th; all
+// warps of the CTA come here, the same number of times.  Rounding keeps the order, so the least and
+// greatest of a channel give its bounds.  `table` begins with the block's first new token.  kFull: all
+// 16 rows are new, and the block is one warp's.  False, with nothing written, where a turned element
+// is not finite.
+template <typename T, int D, bool kWide, int kLayout, bool kFull>
+__device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, u32 head, u32 token, int page, u32 slot,
+                                              u32 count, u32 part, u32 parts, const Table& table, Join<D>& join)
 {
     using Of = Lane<D, kLayout>;
     constexpr int N = Of::N;
     constexpr u32 R = 4;  // steps of two rows at a time
     const Of mine(table.pairs);
-    const u32 half = (threadIdx.x & 31u) >> 4, block = a.c.block;
-    const i64 stride = a.stride_token[0];
-    const u16* x = static_cast<const u16*>(a.x[0]) + (static_cast<i64>(token) + half) * stride +
-                   static_cast<i64>(head) * a.stride_head[0];
+    const u32 lane = threadIdx.x & 31u, half = lane >> 4, warp = threadIdx.x >> 5, block = a.c.block;
     const u64 at = (static_cast<u64>(page) * a.c.heads + head) * 2;
+    u8* out = a.c.data + at * block * D;
+    // the warp's rows: [first, held) are there already, [from, to) are new
+    const u32 first = kFull ? 0 : part * 16, held = kFull ? 0 : min(slot, first + 16), from = kFull ? 0 : max(slot, first);
+    const u32 to = kFull ? 16 : active ? min(slot + count, first + 16) : 0;
+    const i64 stride = a.stride_token[0];
+    const u16* x = static_cast<const u16*>(a.x[0]) + (static_cast<i64>(token) - (kFull ? 0 : slot)) * stride +
+                   static_cast<i64>(head) * a.stride_head[0];
+    // past the end: the last row again
+    auto row_at = [&](u32 row) { return kFull ? row : min(row, to - 1); };
     // turned: the channels at mine.lo and at mine.hi (16 rows held from the first time on, and 16
     // warps on an SM instead of 24, took 149 us for prompts that take 136)
     float2 y[R][2][N];
@@ -308,67 +351,127 @@ __device__ __forceinline__ bool append_full_turned(const AppendArgs& a, u32 head
         u32 low[R][N], high[R][N];
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
-            load_words<N, kWide>(x + (row0 + 2 * r) * stride + mine.lo, low[r]);
-            load_words<N, kWide>(x + (row0 + 2 * r) * stride + mine.hi, high[r]);
+            const u32 row = row_at(row0 + 2 * r + half);
+            load_words<N, kWide>(x + row * stride + mine.lo, low[r]);
+            load_words<N, kWide>(x + row * stride + mine.hi, high[r]);
         }
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
             typename Of::Circle circle;
-            const u32 row = (row0 + 2 * r + half) * table.pairs;
+            const u32 row = (row_at(row0 + 2 * r + half) - (kFull ? 0 : slot)) * table.pairs;
             mine.load(table.cosines + row, table.sines + row, circle);
             mine.template apply<T>(low[r], high[r], circle, y[r][0], y[r][1]);
         }
     };
+    const float was = !kFull && active && slot ? a.c.scale[at] : 0.0f;  // written only after all have met
+    constexpr float kMost = 3.402823466e38f;
     float2 lo[2][N], hi[2][N];  // least and greatest of the channels
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            lo[k][i] = make_float2(3.402823466e38f, 3.402823466e38f);
-            hi[k][i] = make_float2(-3.402823466e38f, -3.402823466e38f);
+            lo[k][i] = make_float2(kMost, kMost);
+            hi[k][i] = make_float2(-kMost, -kMost);
         }
-    for (u32 row0 = 0; row0 < block; row0 += 2 * R) {
+    auto span = [&](int k, int i, float2 z) {
+        lo[k][i] = make_float2(least_of(lo[k][i].x, z.x), least_of(lo[k][i].y, z.y));
+        hi[k][i] = make_float2(greatest_of(hi[k][i].x, z.x), greatest_of(hi[k][i].y, z.y));
+    };
+    for (u32 row0 = from; row0 < to; row0 += 2 * R) {
         turn_rows(row0);
 #pragma unroll
         for (u32 r = 0; r < R; ++r)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float2 z = y[r][k][i];
-                    lo[k][i] = make_float2(least_of(lo[k][i].x, z.x), least_of(lo[k][i].y, z.y));
-                    hi[k][i] = make_float2(greatest_of(hi[k][i].x, z.x), greatest_of(hi[k][i].y, z.y));
-                }
+                for (int i = 0; i < N; ++i) span(k, i, y[r][k][i]);
     }
-    float most = 0.0f;
+    float most = 0.0f;  // NaN if any is
+    if (from < to) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                most = greatest_of(most, greatest_of(greatest_of(fabsf(lo[k][i].x), fabsf(lo[k][i].y)),
+                                                     greatest_of(fabsf(hi[k][i].x), fabsf(hi[k][i].y))));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = greatest_of(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (!kFull && parts > 1) {
+        if (lane == 0) join.most[warp] = most;
+        __syncthreads();
+        for (u32 i = 0; i < parts; ++i) most = greatest_of(most, join.most[warp - part + i]);
+    }
+    const bool plain = most <= kMost;
+    const float now = fmaxf(kv_power(scale_exponent(plain ? most : 0.0f)), was), inverse = 1.0f / now;
+    if (active && plain) {
+        if (lane == 0 && part == 0) a.c.scale[at] = now;
+        for (u32 row0 = from; row0 < to; row0 += 2 * R) {
+            turn_rows(row0);
+#pragma unroll
+            for (u32 r = 0; r < R; ++r) {
+                u32 b[2][N];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) b[k][i] = store_e4m3(mul2(y[r][k][i], make_float2(inverse, inverse)));
+                const u32 row = row0 + 2 * r + half;
+                if (kFull || row < to) {
+                    store_values<N>(out + row * D + mine.lo, b[0]);
+                    store_values<N>(out + row * D + mine.hi, b[1]);
+                }
+            }
+        }
+        const u32 none[N] = {};
+        if (!kFull)
+            for (u32 row = max(slot + count, first) + half; row < first + 16; row += 2) {
+                store_values<N>(out + row * D + mine.lo, none);
+                store_values<N>(out + row * D + mine.hi, none);
+            }
+    }
+    // from here on in units of the scale
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            most = greatest_of(most, greatest_of(greatest_of(fabsf(lo[k][i].x), fabsf(lo[k][i].y)),
-                                                 greatest_of(fabsf(hi[k][i].x), fabsf(hi[k][i].y))));
+        for (int i = 0; i < N; ++i) {
+            lo[k][i] = mul2(lo[k][i], make_float2(inverse, inverse));
+            hi[k][i] = mul2(hi[k][i], make_float2(inverse, inverse));
+        }
+    if (!kFull && active && plain) {  // what the block held before: rounded again if the scale grew
+        const float shrink = slot ? was / now : 1.0f;
+        for (u32 row0 = first; row0 < held; row0 += 2 * R) {
+            u32 b[R][2][N];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) most = greatest_of(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (!(most <= 3.402823466e38f)) return false;
-    const float now = kv_power(scale_exponent(most)), inverse = 1.0f / now;
-    if ((threadIdx.x & 31u) == 0) a.c.scale[at] = now;
-    auto stored = [&](float2 y) { return store_e4m3(mul2(y, make_float2(inverse, inverse))); };
-    u8* out = a.c.data + at * block * D + half * D;
-    for (u32 row0 = 0; row0 < block; row0 += 2 * R) {
-        turn_rows(row0);
+            for (u32 r = 0; r < R; ++r) {
+                const u32 row = min(row0 + 2 * r + half, held - 1);
+                load_values<N>(out + row * D + mine.lo, b[r][0]);
+                load_values<N>(out + row * D + mine.hi, b[r][1]);
+            }
+            __syncwarp();  // the last row may be read by both halves
 #pragma unroll
-        for (u32 r = 0; r < R; ++r) {
-            u32 b[2][N];
+            for (u32 r = 0; r < R; ++r) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < N; ++i) b[k][i] = stored(y[r][k][i]);
-            store_values<N>(out + (row0 + 2 * r) * D + mine.lo, b[0]);
-            store_values<N>(out + (row0 + 2 * r) * D + mine.hi, b[1]);
+                    for (int i = 0; i < N; ++i) {
+                        float2 z = __half22float2(stored_f16(b[r][k][i]));
+                        if (shrink != 1.0f) {
+                            b[r][k][i] = store_e4m3(mul2(z, make_float2(shrink, shrink)));
+                            z = __half22float2(stored_f16(b[r][k][i]));
+                        }
+                        span(k, i, make_float2(z.x == z.x ? z.x : 0.0f, z.y == z.y ? z.y : 0.0f));  // NaN counts as 0
+                    }
+                const u32 row = row0 + 2 * r + half;
+                if (shrink != 1.0f && row < held) {
+                    store_values<N>(out + row * D + mine.lo, b[r][0]);
+                    store_values<N>(out + row * D + mine.hi, b[r][1]);
+                }
+            }
+            __syncwarp();
         }
     }
-    // bounds: the lower lanes' and the upper lanes' rows together; half a warp each for the two ends
-    std::int8_t* bound = a.c.bounds + (static_cast<u64>(page) * a.c.heads + head) * 2 * D + half * D;
+    // the rows of both halves together: the lower half has the least, the upper one the greatest
+    float2 ends[2][N];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -377,12 +480,36 @@ __device__ __forceinline__ bool append_full_turned(const AppendArgs& a, u32 head
             float2 other;
             other.x = __shfl_xor_sync(0xffffffffu, give.x, 16);
             other.y = __shfl_xor_sync(0xffffffffu, give.y, 16);
-            const float2 end = half ? make_float2(fmaxf(keep.x, other.x), fmaxf(keep.y, other.y))
-                                    : make_float2(fminf(keep.x, other.x), fminf(keep.y, other.y));
-            const float2 z = __half22float2(stored_f16(stored(end)));
+            ends[k][i] = half ? make_float2(fmaxf(keep.x, other.x), fmaxf(keep.y, other.y))
+                              : make_float2(fminf(keep.x, other.x), fminf(keep.y, other.y));
+        }
+    if (!kFull && parts > 1) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                *reinterpret_cast<float2*>(&join.ends[warp][half][(k ? mine.hi : mine.lo) + 2 * i]) = ends[k][i];
+        __syncthreads();
+        for (u32 w = warp + 1; part == 0 && w < warp + parts; ++w)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float2 z = *reinterpret_cast<const float2*>(&join.ends[w][half][(k ? mine.hi : mine.lo) + 2 * i]);
+                    const float2 e = ends[k][i];
+                    ends[k][i] = half ? make_float2(fmaxf(e.x, z.x), fmaxf(e.y, z.y))
+                                      : make_float2(fminf(e.x, z.x), fminf(e.y, z.y));
+                }
+    }
+    if (!active || part || !plain) return plain;
+    std::int8_t* bound = a.c.bounds + (static_cast<u64>(page) * a.c.heads + head) * 2 * D + half * D;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float2 z = __half22float2(stored_f16(store_e4m3(ends[k][i])));
             const float2 q = make_float2(z.x * 0.25f, z.y * 0.25f);
-            const u32 channel = (k ? mine.hi : mine.lo) + 2 * i;
-            *reinterpret_cast<char2*>(bound + channel) =
+            *reinterpret_cast<char2*>(bound + (k ? mine.hi : mine.lo) + 2 * i) =
                 half ? make_char2(static_cast<signed char>(ceilf(q.x)), static_cast<signed char>(ceilf(q.y)))
                      : make_char2(static_cast<signed char>(floorf(q.x)), static_cast<signed char>(floorf(q.y)));
         }
@@ -479,17 +606,24 @@ __device__ __forceinline__ void append_keys(const RotaryArgs& r, u32 block, floa
         circle_at(r, base + first + token, i - token * pairs, sines[i], cosines[i]);
     }
     __syncthreads();
-    const u32 total = __popc(leads) * a.c.heads;
-    for (u32 u = (block - chunk * r.key_spread) * kRotaryWarps + (threadIdx.x >> 5); u < total;
-         u += r.key_spread * kRotaryWarps) {
-        const Piece p = piece_at(lead, leads, u, a.c.heads);
-        const u32 token = base + p.who, row = (p.who - first) * pairs;
+    // `parts` warps to a block and head, all warps of the CTA the same number of times
+    Join<D>& join = *reinterpret_cast<Join<D>*>(sines + tokens * pairs);
+    const u32 total = __popc(leads) * a.c.heads, parts = a.c.block / 16, teams = kRotaryWarps / parts;
+    const u32 team = (threadIdx.x >> 5) / parts, part = (threadIdx.x >> 5) - team * parts;
+    for (u32 u0 = (block - chunk * r.key_spread) * teams; u0 < total; u0 += r.key_spread * teams) {
+        const bool active = u0 + team < total;
+        const Piece p = piece_at(lead, leads, active ? u0 + team : u0, a.c.heads);
+        const u32 row = (p.who - first) * pairs, token = base + p.who;
         const Table table{cosines + row, sines + row, pairs};
-        if (p.count < a.c.block || !append_full_turned<T, D, kWide, kLayout>(a, p.head, token, p.page, table)) {
-            const PlainRow<T, D, kWide> from(a, p.head, 0, token);
-            append_block<D>(a, p.head, 0, p.page, p.slot, p.count,
-                            TurnedRow<T, D, kWide, kLayout>{from.x, from.stride, table});
-        }
+        bool done = false;
+        if (parts > 1 || (active && p.count > 4 && p.count < 16))
+            done = append_turned<T, D, kWide, kLayout, false>(a, active, p.head, token, p.page, p.slot, p.count, part,
+                                                              parts, table, join);
+        else if (active && p.count == 16)
+            done = append_turned<T, D, kWide, kLayout, true>(a, true, p.head, token, p.page, 0, 16, 0, 1, table, join);
+        // few tokens, for which the code for many takes longer, and elements that are not finite
+        if (active && part == 0 && !done)
+            append_rows<T, D, kWide, kLayout>(a, p.head, token, p.page, p.slot, p.count, table);
     }
 }
 
@@ -509,7 +643,7 @@ __device__ __forceinline__ void append_values(const RotaryArgs& r, u32 block)
 }
 
 template <typename T, int D, bool kWide, int kLayout>
-__global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : 6) rotary_kernel(const RotaryArgs r)
+__global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : D == 128 ? 5 : 6) rotary_kernel(const RotaryArgs r)
 {
     extern __shared__ float4 shared[];
     u32 block = blockIdx.x;
@@ -532,8 +666,8 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : 6) rotary_ke
 template <typename T, int D, bool kWide, int kLayout>
 bool launch(const RotaryArgs& r, cudaStream_t s)
 {
-    const u32 smem = r.key_blocks ? (r.a.chunk - 1 + r.a.c.block) * r.pairs * 8 : 0;
-    constexpr u32 kMost = (15 + 64) * (D / 2) * 8;
+    const u32 smem = r.key_blocks ? (r.a.chunk - 1 + r.a.c.block) * r.pairs * 8 + (r.a.c.block > 16 ? sizeof(Join<D>) : 0) : 0;
+    constexpr u32 kMost = (15 + 64) * (D / 2) * 8 + sizeof(Join<D>);
     static std::atomic<u64> seen{0};
     if (smem > 48 * 1024 && !kv_allow_smem(rotary_kernel<T, D, kWide, kLayout>, kMost, seen)) return false;
     const u64 items = static_cast<u64>(r.a.tokens) * r.parts;
@@ -602,7 +736,11 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
     a.chunk = 1;
     while (a.chunk < 16 && static_cast<u64>(a.tokens) * heads * 2 > a.chunk * warps) a.chunk *= 2;
     if (append) {
-        const u32 chunks = (a.tokens + a.chunk - 1) / a.chunk, by = kRotaryWarps * (a.chunk == 1 ? 1 : 2);
+        // A CTA takes as many heads' keys of a block at once as it has warps for, 16 rows to a warp; where
+        // that makes many more CTAs than are resident, twice as many share a block's cosines.
+        const u32 chunks = (a.tokens + a.chunk - 1) / a.chunk, teams = kRotaryWarps / (a.c.block / 16);
+        const u64 pieces = (static_cast<u64>(a.tokens) / a.c.block + a.seqs) * heads;
+        const u32 by = teams * (pieces > 2ull * teams * kv_sm_count() * 6 ? 2 : 1);
         r.key_spread = (heads + by - 1) / by;
         r.value_spread = (heads + kRotaryWarps - 1) / kRotaryWarps;
         r.key_blocks = chunks * r.key_spread;

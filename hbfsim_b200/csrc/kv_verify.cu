@@ -56,6 +56,20 @@ __device__ __forceinline__ uint4 load16(const void* from)
     return x;
 }
 
+template <typename T>
+__device__ __forceinline__ T load_one(const T* from)
+{
+    if constexpr (sizeof(T) == 4) {
+        u32 x;
+        asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(x) : "l"(from));
+        return *reinterpret_cast<const T*>(&x);
+    } else {
+        u16 x;
+        asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(x) : "l"(from));
+        return *reinterpret_cast<const T*>(&x);
+    }
+}
+
 struct Sums {
     u64 left, target;  // of the weights, of the target alone
 };
@@ -107,9 +121,20 @@ __device__ __forceinline__ Sums sum_segment(const T* p, const T* q, u32 from, u3
         for (; i < end; ++i)  // one lane's rest
             add_to<kDraft>(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);
     } else {
-#pragma unroll 4
-        for (u32 i = from + lane; i < end; i += 32)
-            add_to<kDraft>(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);
+        // rows that begin anywhere: one value to a lane and load
+        constexpr u32 M = 2 * U;
+        u32 i = from + lane;
+        for (; i + (M - 1) * 32 < end; i += M * 32) {
+            T x[M], y[M];
+#pragma unroll
+            for (u32 u = 0; u < M; ++u) {
+                x[u] = load_one(p + i + u * 32);
+                if constexpr (kDraft) y[u] = load_one(q + i + u * 32);
+            }
+#pragma unroll
+            for (u32 u = 0; u < M; ++u) add_to<kDraft>(s, to_float(x[u]), kDraft ? to_float(y[u]) : 0.0f);
+        }
+        for (; i < end; i += 32) add_to<kDraft>(s, to_float(p[i]), kDraft ? to_float(q[i]) : 0.0f);
     }
     if constexpr (!kDraft) s.left = s.target;
     return s;

@@ -337,7 +337,7 @@ def kv_append_rotary(cache: KvCache, q, k, v, table, start, positions, rotary: K
             q_at = q.data_ptr()
     if tokens == 0:
         return out
-    places = positions.reshape(axes, tokens)
+    places = positions if offsets is not None and positions.dim() == 2 else positions.reshape(axes, tokens)
     if places.stride(1) != 1 and tokens > 1:
         places = places.contiguous()
     packed = _ROTARY.pack(_ROTARY.size, 1, q_heads, axes, rotary.pairs, rotary.neighbours, q_at,
