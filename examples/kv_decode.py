@@ -2,11 +2,13 @@
 
 One layer of a paged 8-bit KV cache lies in a simulated HBF range: page p,
 head h at base + (p * kv_heads + h) * block_bytes, 4 KiB each at 16 tokens of
-128 channels.  Every step appends a token per sequence, lists the blocks worth
-reading per head (kv_select), attends over them (kv_attention), lets the
-blocks of least accumulated attention weight go (kv_evict), and times two
-traces on the per-die model: the reads of the lists, and the reads that
-attention over every block would have made.
+128 channels.  Every step gives the sequences pages for a token (kv_resize, which
+takes back what the step before evicted), appends it with its position turned
+in (kv_append_rotary), lists the blocks worth reading per head (kv_select),
+attends over them (kv_attention), lets the blocks of least accumulated
+attention weight go (kv_evict), and times two traces on the per-die model: the
+reads of the lists, and the reads that attention over every block would have
+made.
 
     python examples/kv_decode.py --seqs 16 --context 4096 --steps 32 --top 64 --keep 200
 """
@@ -21,8 +23,8 @@ from pathlib import Path
 import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
-from hbfsim_b200 import (Context, KvCache, RANGE_TIMING, kv_append, kv_attention,  # noqa: E402
-                         kv_block_reads, kv_evict, kv_select)
+from hbfsim_b200 import (Context, KvCache, KvRotary, RANGE_TIMING, kv_append_rotary,  # noqa: E402
+                         kv_attention, kv_block_reads, kv_evict, kv_resize, kv_select)
 from hbfsim_b200 import workloads as wl  # noqa: E402
 
 
@@ -45,7 +47,8 @@ def run(seqs: int, context: int, steps: int, top: int, keep: int, q_heads: int =
     keep = min(keep, width)
     cache = KvCache.empty(seqs * width, kv_heads, head_dim, block)
     table = torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
-    free = torch.randperm(seqs * width, generator=gen, device="cuda").to(torch.int32).tolist()
+    refs = torch.zeros(seqs * width, dtype=torch.int32, device="cuda")  # every page is free
+    rotary = KvRotary.of(head_dim)
 
     with tempfile.TemporaryDirectory() as tmp:
         work = wl.c1_workload()  # the profile of the decode workloads: 4 stacks of 16 channels
@@ -57,27 +60,31 @@ def run(seqs: int, context: int, steps: int, top: int, keep: int, q_heads: int =
             ctx.register_device(wl.RANGE_BASE, size, mode=RANGE_TIMING, permissions=3)
 
         # the prompts
-        blocks = -(-context // block)
-        for b in range(seqs):
-            table[b, :blocks] = torch.tensor([free.pop() for _ in range(blocks)])
         zero = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+        room = kv_resize(refs, table, zero, zero + context, block_tokens=block, inplace=True)
+        assert (room.limits == context).all()
         channel = torch.exp(0.5 * torch.randn((kv_heads, head_dim), generator=gen, device="cuda"))
         for at in range(0, context, 4096):  # in chunks: start grows
             n = min(4096, context - at)
             k = (normal(seqs, n, kv_heads, head_dim) * channel).to(torch.bfloat16)
-            kv_append(cache, k, normal(seqs, n, kv_heads, head_dim), table, zero + at)
+            place = torch.arange(at, at + n, dtype=torch.int32, device="cuda").expand(seqs, n)
+            kv_append_rotary(cache, None, k, normal(seqs, n, kv_heads, head_dim), table, zero + at,
+                             place, rotary)
 
         lengths = zero + context
         score = torch.zeros((seqs, width), dtype=torch.int64, device="cuda")
         total = {"steps": steps, "listed_ns": 0, "every_ns": 0, "listed_reads": 0, "every_reads": 0,
                  "evicted_blocks": 0}
-        for _ in range(steps):
-            full = (lengths % block == 0).nonzero().flatten().tolist()
-            for b in full:  # a new block begins
-                table[b, int(lengths[b]) // block] = free.pop()
+        freed = freed_counts = None
+        for step in range(steps):
+            room = kv_resize(refs, table, lengths, lengths + 1, block_tokens=block, freed=freed,
+                             freed_counts=freed_counts)
+            refs, table = room.refs, room.table
             q = normal(seqs, 1, q_heads, head_dim)
             k = (normal(seqs, 1, kv_heads, head_dim) * channel).to(torch.bfloat16)
-            kv_append(cache, k, normal(seqs, 1, kv_heads, head_dim), table, lengths)
+            # positions count what was evicted too
+            q = kv_append_rotary(cache, q, k, normal(seqs, 1, kv_heads, head_dim), table, lengths,
+                                 zero.view(seqs, 1) + context + step, rotary)
             lengths = lengths + 1
 
             pick = kv_select(cache, q, table, lengths, top=top)
@@ -97,12 +104,11 @@ def run(seqs: int, context: int, steps: int, top: int, keep: int, q_heads: int =
             rest = kv_evict(score, got.weights, table, lengths, keep=keep, block_tokens=block,
                             decay=8)
             score, table, lengths = rest.score, rest.table, rest.lengths
-            for b, n in enumerate(rest.freed_counts.tolist()):
-                free += rest.freed[b, :n].tolist()
-                total["evicted_blocks"] += n
+            freed, freed_counts = rest.freed, rest.freed_counts
+            total["evicted_blocks"] += int(freed_counts.sum())
         for ctx in (listed, every):
             ctx.close()
-    assert torch.isfinite(got.out).all()
+    assert torch.isfinite(got.out).all() and (room.limits >= lengths - 1).all()
     total["listed_us_per_step"] = round(total.pop("listed_ns") / steps / 1e3, 3)
     total["every_us_per_step"] = round(total.pop("every_ns") / steps / 1e3, 3)
     return total
