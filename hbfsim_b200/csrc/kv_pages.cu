@@ -686,47 +686,72 @@ __global__ void __launch_bounds__(kPageThreads, 2) compact_pass_kernel(const Com
 // ---------------------------------------------------------------------------
 // Copies
 
-constexpr u32 kCopyThreads = 256, kCopyDeep = 4;
+// A page's data in pieces of 16 KB, eight loads of a thread under way, and no more thread blocks than
+// there are pieces: the hardware hands them out (a gigabyte of 32 KB pages takes 310 us, 96 % of a copy's
+// rate; a grid that stays and strides over the pieces took 330 to 360 us, pieces of 32 KB by 512 threads
+// 351 us).  Lists kept at capacity are mostly empty: long ones go by up to 32 moves to a thread block, which
+// costs a few per cent where they are full (groups of 6: 319 us).
+constexpr u32 kCopyThreads = 128, kCopyDeep = 8, kCopyGroup = 32;
 constexpr u32 kCopyPiece = kCopyThreads * kCopyDeep * 16;  // bytes of a thread block at a time
 
 struct CopyArgs {
     KvView from, to;
     const int* src;
     const int* dst;
-    u64 pieces;          // of all moves
-    u32 per_page;        // pieces of a page's data, and one more for its scales and bounds
+    u64 count, groups;
+    u32 group;     // moves of a thread block
+    u32 per_page;  // pieces of a page's data; its scales and bounds go with the first
     u64 page_bytes;
 };
 
+__device__ __forceinline__ uint4 load_once(const uint4* from)
+{
+    uint4 x;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "l"(from)
+                 : "memory");
+    return x;
+}
+
+// A piece of page `src` to page `dst`.
+__device__ __forceinline__ void copy_piece(const CopyArgs& a, u32 src, u32 dst, u32 part)
+{
+    const u64 first = static_cast<u64>(part) * kCopyPiece;
+    const uint4* from = reinterpret_cast<const uint4*>(a.from.data + src * a.page_bytes + first) + threadIdx.x;
+    uint4* to = reinterpret_cast<uint4*>(a.to.data + dst * a.page_bytes + first) + threadIdx.x;
+    const u32 left = static_cast<u32>(min(a.page_bytes - first, static_cast<u64>(kCopyPiece))) / 16;
+    uint4 x[kCopyDeep];
+#pragma unroll
+    for (u32 i = 0; i < kCopyDeep; ++i)
+        if (threadIdx.x + i * kCopyThreads < left) x[i] = load_once(from + i * kCopyThreads);
+    if (part == 0) {
+        const u32 bounds = a.from.heads * 2 * a.from.dim / 16, scales = a.from.heads;  // of 16 and of 8 bytes
+        const uint4* b = reinterpret_cast<const uint4*>(a.from.bounds) + static_cast<u64>(src) * bounds;
+        uint4* b_to = reinterpret_cast<uint4*>(a.to.bounds) + static_cast<u64>(dst) * bounds;
+        for (u32 i = threadIdx.x; i < bounds; i += kCopyThreads) b_to[i] = b[i];
+        const float2* s = reinterpret_cast<const float2*>(a.from.scale) + static_cast<u64>(src) * scales;
+        float2* s_to = reinterpret_cast<float2*>(a.to.scale) + static_cast<u64>(dst) * scales;
+        for (u32 i = threadIdx.x; i < scales; i += kCopyThreads) s_to[i] = s[i];
+    }
+#pragma unroll
+    for (u32 i = 0; i < kCopyDeep; ++i)
+        if (threadIdx.x + i * kCopyThreads < left) to[i * kCopyThreads] = x[i];
+}
+
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyArgs a)
 {
-    for (u64 piece = blockIdx.x; piece < a.pieces; piece += gridDim.x) {
-        const u64 move = piece / a.per_page;
-        const u32 part = static_cast<u32>(piece - move * a.per_page);
-        const u32 src = static_cast<u32>(a.src[move]), dst = static_cast<u32>(a.dst[move]);
-        if (src >= a.from.pages || dst >= a.to.pages) continue;
-        if (part + 1 < a.per_page) {
-            const u64 at = static_cast<u64>(part) * kCopyPiece + threadIdx.x * 16;
-            const u8* from = a.from.data + src * a.page_bytes;
-            u8* to = a.to.data + dst * a.page_bytes;
-            uint4 x[kCopyDeep];
-#pragma unroll
-            for (u32 i = 0; i < kCopyDeep; ++i)
-                if (at + i * kCopyThreads * 16 < a.page_bytes)
-                    x[i] = *reinterpret_cast<const uint4*>(from + at + i * kCopyThreads * 16);
-#pragma unroll
-            for (u32 i = 0; i < kCopyDeep; ++i)
-                if (at + i * kCopyThreads * 16 < a.page_bytes)
-                    *reinterpret_cast<uint4*>(to + at + i * kCopyThreads * 16) = x[i];
-            continue;
+    const u32 lane = threadIdx.x & 31u;
+    for (u64 unit = blockIdx.x; unit < a.groups * a.per_page; unit += gridDim.x) {
+        const u64 group = unit / a.per_page, move = group * a.group + lane;
+        const u32 part = static_cast<u32>(unit - group * a.per_page);
+        const bool listed = lane < a.group && move < a.count;
+        const u32 page = listed ? static_cast<u32>(a.src[move]) : ~0u, page_to = listed ? static_cast<u32>(a.dst[move]) : ~0u;
+        u32 left_moves = __ballot_sync(0xffffffffu, page < a.from.pages && page_to < a.to.pages);
+        for (; left_moves; left_moves &= left_moves - 1) {
+            const int which = __ffs(left_moves) - 1;
+            copy_piece(a, __shfl_sync(0xffffffffu, page, which), __shfl_sync(0xffffffffu, page_to, which), part);
         }
-        const u32 bounds = a.from.heads * 2 * a.from.dim, scales = a.from.heads;  // bytes; pairs
-        const uint4* from = reinterpret_cast<const uint4*>(a.from.bounds + static_cast<u64>(src) * bounds);
-        uint4* to = reinterpret_cast<uint4*>(a.to.bounds + static_cast<u64>(dst) * bounds);
-        for (u32 i = threadIdx.x; i < bounds / 16; i += kCopyThreads) to[i] = from[i];
-        const float2* scale = reinterpret_cast<const float2*>(a.from.scale) + static_cast<u64>(src) * scales;
-        float2* scale_to = reinterpret_cast<float2*>(a.to.scale) + static_cast<u64>(dst) * scales;
-        for (u32 i = threadIdx.x; i < scales; i += kCopyThreads) scale_to[i] = scale[i];
     }
 }
 
@@ -995,9 +1020,12 @@ extern "C" int hbfsim_kv_copy_v1(const hbfsim_kv_cache_v1* from, const hbfsim_kv
     a.src = src;
     a.dst = dst;
     a.page_bytes = 2ull * a.from.heads * a.from.block * a.from.dim;
-    a.per_page = static_cast<u32>((a.page_bytes + kCopyPiece - 1) / kCopyPiece) + 1;
-    a.pieces = count * a.per_page;
-    const u32 blocks = static_cast<u32>(std::min<u64>(a.pieces, static_cast<u64>(kv_sm_count()) * 8));
+    a.per_page = static_cast<u32>((a.page_bytes + kCopyPiece - 1) / kCopyPiece);
+    // thread blocks of several moves where there would be more than 512 to an SM
+    a.count = count;
+    a.group = static_cast<u32>(std::min<u64>(kCopyGroup, count * a.per_page / (512ull * kv_sm_count()) + 1));
+    a.groups = (count + a.group - 1) / a.group;
+    const u32 blocks = static_cast<u32>(std::min<u64>(a.groups * a.per_page, 0x7fffffffull));
     const bool ok = kv_launch(copy_kernel, dim3(blocks), kCopyThreads, static_cast<cudaStream_t>(stream), 0, 1, false, a);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
