@@ -888,7 +888,7 @@ extern "C" int hbfsim_kv_resize_v1(const hbfsim_kv_resize_batch_v1* b, void* str
         if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
     const ResizeRoom room = resize_room(*b);
     if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < room.bytes) return HBFSIM_INVALID_ARGUMENT;
-    if (b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
+    if (entries && b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
     // rows of an output may not lie in one another
     if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
     const Extent out[] = {{b->refs_out, b->pages * 4},
@@ -984,7 +984,7 @@ extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* s
                           static_cast<const void*>(b->live), static_cast<const void*>(b->where)})
         if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
     if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < kMaxParts * kPageWarps * 4) return HBFSIM_INVALID_ARGUMENT;
-    if (b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
+    if (entries && b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
     if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
     const Extent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, b->seqs, b->width, b->table_out_stride},
                           {b->src, room * 4},          {b->dst, room * 4},

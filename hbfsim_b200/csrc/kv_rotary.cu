@@ -337,7 +337,8 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
     const u64 at = (static_cast<u64>(page) * a.c.heads + head) * 2;
     u8* out = a.c.data + at * block * D;
     // the warp's rows: [first, held) are there already, [from, to) are new
-    const u32 first = kFull ? 0 : part * 16, held = kFull ? 0 : min(slot, first + 16), from = kFull ? 0 : max(slot, first);
+    const u32 first = kFull ? 0 : part * 16, from = kFull ? 0 : max(slot, first);
+    u32 held = kFull ? 0 : min(slot, first + 16);
     const u32 to = kFull ? 16 : active ? min(slot + count, first + 16) : 0;
     const i64 stride = a.stride_token[0];
     const u16* x = static_cast<const u16*>(a.x[0]) + (static_cast<i64>(token) - (kFull ? 0 : slot)) * stride +
@@ -437,7 +438,8 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
             lo[k][i] = mul2(lo[k][i], make_float2(inverse, inverse));
             hi[k][i] = mul2(hi[k][i], make_float2(inverse, inverse));
         }
-    if (!kFull && active && plain) {  // what the block held before: rounded again if the scale grew
+    if constexpr (!kFull) {  // what the block held before: rounded again if the scale grew
+        if (!active || !plain) held = 0;
         const float shrink = slot ? was / now : 1.0f;
         for (u32 row0 = first; row0 < held; row0 += 2 * R) {
             u32 b[R][2][N];

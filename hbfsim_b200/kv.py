@@ -172,7 +172,7 @@ def _check_table(index, table, per_seq, name):
     import torch
     shape = table.shape
     _need(len(shape) == 2 and table.dtype == torch.int32 and table.get_device() == index
-          and (table.stride(1) == 1 or shape[1] <= 1),
+          and (table.stride(1) == 1 or shape[1] <= 1 or shape[0] == 0),
           "table: int32 [seqs, width] on the cache's device, rows contiguous")
     _need(per_seq.dtype == torch.int32 and per_seq.shape == shape[:1]
           and per_seq.get_device() == index and (per_seq.stride(0) == 1 or shape[0] <= 1),
@@ -680,7 +680,8 @@ def kv_compact(refs, table, inplace: bool = False, stream=None) -> KvCompacted:
             return kv_compact(refs, table, inplace)
     import torch
     shape = table.shape
-    _need(len(shape) == 2 and table.dtype == torch.int32 and (table.stride(1) == 1 or shape[1] <= 1),
+    _need(len(shape) == 2 and table.dtype == torch.int32
+          and (table.stride(1) == 1 or shape[1] <= 1 or shape[0] == 0),
           "table: int32 [seqs, width], rows contiguous")
     _check_pool(refs, table, index)
     seqs, width = shape

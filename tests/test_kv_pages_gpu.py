@@ -217,3 +217,30 @@ def test_refusals(bad):
             kv_resize(refs.cpu(), table, one, one)
         else:  # rows of the table in one another cannot be changed in place
             kv_resize(refs, table.flatten().as_strided((2, 4), (2, 1)), one, one, inplace=True)
+
+
+@pytest.mark.parametrize("seqs,width,pages", [(0, 3, 5), (0, 0, 0), (3, 0, 5), (3, 4, 0), (1, 1, 0)])
+def test_nothing_there(seqs, width, pages):
+    """No sequences, no room in the table, no pages."""
+    from hbfsim_b200 import KvCache, kv_compact, kv_copy, kv_fork
+    refs, table = np.zeros(pages, np.int32), np.full((seqs, width), -1, np.int32)
+    lengths = np.zeros(seqs, np.int32)
+    freed = np.full((2, 3), 1, np.int32)
+    out = resize_and_check(refs, table, lengths, lengths + 20, 16, freed, np.array([2, 3]))
+    assert (out[2] == 0).all() or width == 0 or pages
+    parents = np.array([0, -1, 5], np.int32)
+    same(kv_fork(int32(refs), int32(table), int32(lengths), int32(parents)), ko.fork(refs, table, lengths, parents, 16))
+    same(kv_compact(int32(refs), int32(table)), ko.compact(refs, table))
+    if pages == 0:
+        kv_copy(KvCache.empty(0, 1, 64), int32([0, -1, 3]), int32([0, 1, 2]))
+
+
+def test_rows_that_are_one_row():
+    """A table whose rows are one row in memory (as expand gives it): every row counts."""
+    from hbfsim_b200 import kv_fork, kv_resize
+    row = int32([[2, 0, -1]])
+    refs = np.array([4, 0, 4, 0], np.int32)
+    table, lengths = row.expand(4, 3), np.array([20, 20, 20, 20], np.int32)
+    plain = row.cpu().numpy().repeat(4, 0)
+    same(kv_resize(int32(refs), table, int32(lengths), int32(lengths - 10)), ko.resize(refs, plain, lengths, lengths - 10, 16))
+    same(kv_fork(int32(refs), table, int32(lengths), int32([1, 1])), ko.fork(refs, plain, lengths, [1, 1], 16))

@@ -261,3 +261,34 @@ def test_refusals(bad):
     if "gradient" in bad:
         with torch.no_grad():
             kv_append_rotary(gpu, **call)
+
+
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_blocks_begun_and_ended_inside(dim, block):
+    """Every number of tokens held before and of new ones that a block can have, in one call; scales
+    that grow over what is held and scales that do not; values near the largest of 32 bits."""
+    torch = torch_()
+    from hbfsim_b200 import KvRotary, kv_append_rotary
+    rng = np.random.default_rng(dim + block)
+    pairs = [(s, n) for s in range(0, block, 5) for n in (1, 2, 4, 5, 7, 15, 16, 17, 31, 63, 64) if s + n <= block]
+    start = np.array([s for s, _ in pairs], np.int32)
+    count = np.array([n for _, n in pairs])
+    offsets = np.concatenate([[0], np.cumsum(count)]).astype(np.int32)
+    heads, pages, total = 3, len(pairs), int(offsets[-1])
+    cache = random_cache(rng, pages, heads, block, dim)
+    cache["scale"] *= 2.0 ** rng.integers(-12, 13, cache["scale"].shape)
+    cache["scale"][::7] = 2.0 ** 120
+    cache["data"][::7] = ko.encode(np.clip(ko.E4M3[cache["data"][::7]], -255, 255))
+    cache["data"][3::11, 1, 0, 0, 5] = 0x7f  # held values that are no numbers
+    table = rng.permutation(pages).astype(np.int32)[:, None]
+    size = 10.0 ** rng.uniform(-4, 4, (total, 1, 1)) * np.where(rng.random((total, 1, 1)) < 0.02, 1e34, 1)
+    x = torch.from_numpy(rng.standard_normal((total, 2 * heads, dim)) * size).to(torch.bfloat16).cuda()
+    rotary = KvRotary.of(dim, sections=(dim // 4, dim // 4))
+    positions = rng.integers(0, 5000, (2, total)).astype(np.int32)
+    gpu = to_gpu(cache)
+    assert kv_append_rotary(gpu, None, x[:, :heads], x[:, heads:], int32(table), int32(start), int32(positions), rotary,
+                            offsets=int32(offsets)) is None
+    turned = ko.rotate(plain(x[:, :heads]), positions, rotary.freq.cpu().numpy(), rotary.axis.cpu().numpy(), False)
+    ko.append(cache, turned.astype(np.float64), x[:, heads:].double().cpu().numpy(), table, start, offsets)
+    same_cache(gpu, cache)
