@@ -201,9 +201,9 @@ struct ResizeArgs {
     int* dst;
     u32 seqs, width, block, freed_rows, freed_width, pages;
     // workspace
-    u32* free_part;   // [kMaxParts * kPageWarps] free pages of a warp's share
-    u32* asked_part;  // [kMaxParts * kPageWarps] asked blocks of a warp's runs
-    u32* claim_part;  // [kMaxParts * kPageWarps] claims of a warp's runs
+    u32* free_part;   // [blocks][kPageWarps] free pages of a warp's share
+    u32* asked_part;  // [blocks][kPageWarps] asked blocks of a warp's runs
+    u32* claim_part;  // [blocks][kPageWarps] claims of a warp's runs
     u32* free_all;    // free pages
     int* claims;      // [pages] of a shared page: how often it is asked for
     int* last;        // [pages] and by which sequence last
@@ -572,7 +572,7 @@ struct CompactArgs {
     int* live;
     int* where;
     u32 seqs, width, pages;
-    u32* live_part;  // workspace: [kMaxParts * kPageWarps] pages in use of a warp's share
+    u32* live_part;  // workspace: [blocks][kPageWarps] pages in use of a warp's share
 };
 
 __device__ void compact_count(const CompactArgs& a, const KvTeam& team)
@@ -800,6 +800,15 @@ struct Room {
     }
 };
 
+// Thread blocks of a pass.
+u32 pass_blocks()
+{
+    return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count()));
+}
+
+// A count for every warp of a pass or a cluster.
+u64 part_bytes() { return kv_round_up(u64{std::max(pass_blocks(), kPageTeam)} * kPageWarps * 4, 256); }
+
 struct ResizeRoom {
     u64 free_part, asked_part, claim_part, free_all, claims, last, pool, state, bytes;
 };
@@ -807,9 +816,9 @@ ResizeRoom resize_room(const hbfsim_kv_resize_batch_v1& b)
 {
     Room room;
     ResizeRoom r{};
-    r.free_part = room.take(kMaxParts * kPageWarps * 4);
-    r.asked_part = room.take(kMaxParts * kPageWarps * 4);
-    r.claim_part = room.take(kMaxParts * kPageWarps * 4);
+    r.free_part = room.take(part_bytes());
+    r.asked_part = room.take(part_bytes());
+    r.claim_part = room.take(part_bytes());
     r.free_all = room.take(4);
     r.claims = room.take(b.pages * 4);
     r.last = room.take(b.pages * 4);
@@ -855,10 +864,6 @@ u32 cluster_size(u64 counts, u64 entries, u64 runs)
     return counts > kPageTeam * kCountsMost || entries > team * kEntriesMost ? 0 : team;
 }
 
-u32 pass_blocks()
-{
-    return std::min<u32>(kMaxParts, static_cast<u32>(kv_sm_count()));
-}
 
 }  // namespace
 }  // namespace hbfb
@@ -968,7 +973,7 @@ static int compact_check(const hbfsim_kv_compact_batch_v1* b)
 
 extern "C" uint64_t hbfsim_kv_compact_workspace_v1(const hbfsim_kv_compact_batch_v1* b)
 {
-    return compact_check(b) == HBFSIM_OK ? kMaxParts * kPageWarps * 4 : 0;
+    return compact_check(b) == HBFSIM_OK ? part_bytes() : 0;
 }
 
 extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* stream)
@@ -983,13 +988,13 @@ extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* s
                           static_cast<const void*>(b->src), static_cast<const void*>(b->dst),
                           static_cast<const void*>(b->live), static_cast<const void*>(b->where)})
         if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
-    if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < kMaxParts * kPageWarps * 4) return HBFSIM_INVALID_ARGUMENT;
+    if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < part_bytes()) return HBFSIM_INVALID_ARGUMENT;
     if (entries && b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
     if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
     const Extent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, b->seqs, b->width, b->table_out_stride},
                           {b->src, room * 4},          {b->dst, room * 4},
                           {b->live, 4},                {b->where, b->pages * 4},
-                          {b->workspace, kMaxParts * kPageWarps * 4}};
+                          {b->workspace, part_bytes()}};
     const Extent in[] = {{b->refs, b->pages * 4}, {b->table, b->seqs, b->width, b->table_stride}};
     if (would_race(out, in, {0, 1, -1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
     const CompactArgs a{b->refs, b->table, b->table_stride, b->refs_out, b->table_out, b->table_out_stride, b->src,

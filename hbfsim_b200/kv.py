@@ -506,8 +506,9 @@ def kv_verify(target, draft, tokens, accept, sample, counts=None, lengths=None,
         with _On(index, stream):
             return kv_verify(target, draft, tokens, accept, sample, counts, lengths)
     import torch
-    kind = {torch.float32: _lib.KV_P_F32, torch.bfloat16: _lib.KV_P_BF16,
-            torch.float16: _lib.KV_P_F16}.get(target.dtype)
+    of = target.dtype
+    kind = _lib.KV_P_F32 if of == torch.float32 else _lib.KV_P_BF16 if of == torch.bfloat16 else \
+        _lib.KV_P_F16 if of == torch.float16 else None
     _need(kind is not None and target.dim() == 3 and target.shape[1] > 0 and target.shape[2] > 0,
           "target: float32, bfloat16 or float16 [seqs, n + 1, vocab]")
     seqs, rows, vocab = target.shape
@@ -521,15 +522,20 @@ def kv_verify(target, draft, tokens, accept, sample, counts=None, lengths=None,
               "draft: [seqs, n, vocab] of target's type on its device, the last axis contiguous")
         draft_seq, draft_token, _ = draft.stride()
         draft_at = draft.data_ptr() or 256  # 0: no draft
-    for x, of, shape, name in ((tokens, torch.int32, (seqs, n), "tokens: int32 [seqs, n]"),
-                               (accept, torch.float32, (seqs, n), "accept: float32 [seqs, n]"),
-                               (sample, torch.float32, (seqs,), "sample: float32 [seqs]"),
-                               (counts, torch.int32, (seqs,), "counts: int32 [seqs]"),
-                               (lengths, torch.int32, (seqs,), "lengths: int32 [seqs]")):
-        if x is None and (of, shape) == (torch.int32, (seqs,)):
-            continue  # counts and lengths may be left out
-        _need(x is not None and x.dtype == of and x.shape == shape and x.is_contiguous()
-              and x.get_device() == index, name + ", contiguous, on target's device")
+    per_draft, per_seq = (seqs, n), (seqs,)
+    _need(tokens is not None and tokens.dtype == torch.int32 and tokens.shape == per_draft
+          and tokens.get_device() == index and tokens.is_contiguous(),
+          "tokens: int32 [seqs, n], contiguous, on target's device")
+    _need(accept.dtype == torch.float32 and accept.shape == per_draft and accept.get_device() == index
+          and accept.is_contiguous(), "accept: float32 [seqs, n], contiguous, on target's device")
+    _need(sample.dtype == torch.float32 and sample.shape == per_seq and sample.get_device() == index
+          and sample.is_contiguous(), "sample: float32 [seqs], contiguous, on target's device")
+    _need(counts is None or counts.dtype == torch.int32 and counts.shape == per_seq
+          and counts.get_device() == index and counts.is_contiguous(),
+          "counts: int32 [seqs], contiguous, on target's device")
+    _need(lengths is None or lengths.dtype == torch.int32 and lengths.shape == per_seq
+          and lengths.get_device() == index and lengths.is_contiguous(),
+          "lengths: int32 [seqs], contiguous, on target's device")
     _need(not (target.requires_grad or draft is not None and draft.requires_grad)
           or not torch.is_grad_enabled(), "no gradient passes through a draw: detach the tensors or "
           "call under torch.no_grad()")
@@ -601,10 +607,10 @@ def kv_resize(refs, table, lengths, want, block_tokens: int = 16, freed=None, fr
         new_table = torch.empty_like(table, memory_format=torch.contiguous_format)
     limits, src, dst = _parts(refs, seqs, seqs, seqs)
     batch = _RESIZE.pack(
-            _RESIZE.size + _WORKSPACE.size, 1, seqs, width, block_tokens, freed_rows, freed_width, 0, refs.shape[0],
-            refs.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(), want.data_ptr(),
-            freed_at, freed_counts_at, new_refs.data_ptr(), new_table.data_ptr(),
-            new_table.stride(0), limits.data_ptr(), src.data_ptr(), dst.data_ptr())
+        _RESIZE.size + _WORKSPACE.size, 1, seqs, width, block_tokens, freed_rows, freed_width, 0,
+        refs.shape[0], refs.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(),
+        want.data_ptr(), freed_at, freed_counts_at, new_refs.data_ptr(), new_table.data_ptr(),
+        new_table.stride(0), limits.data_ptr(), src.data_ptr(), dst.data_ptr())
     lib = _lib.load()
     size = lib.hbfsim_kv_resize_workspace_v1(batch + _NO_WORKSPACE)
     space = refs.new_empty(size // 4)
@@ -691,15 +697,16 @@ def kv_compact(refs, table, inplace: bool = False, stream=None) -> KvCompacted:
     else:
         new_refs = torch.empty_like(refs)
         new_table = torch.empty_like(table, memory_format=torch.contiguous_format)
-    src, dst, live = _parts(refs, pages // 2, pages // 2, 1)
+    lib = _lib.load()
+    size = lib.hbfsim_kv_compact_workspace_v1(_COMPACT.pack(
+        _COMPACT.size + _WORKSPACE.size, 1, seqs, width, pages, *[0] * 10) + _NO_WORKSPACE)
+    # the workspace is small: some bytes for every warp
+    space, src, dst, live = _parts(refs, size // 4, pages // 2, pages // 2, 1)
     where = torch.empty_like(refs)
     batch = _COMPACT.pack(
-            _COMPACT.size + _WORKSPACE.size, 1, seqs, width, pages, refs.data_ptr(), table.data_ptr(),
-            table.stride(0), new_refs.data_ptr(), new_table.data_ptr(), new_table.stride(0),
-            src.data_ptr(), dst.data_ptr(), live.data_ptr(), where.data_ptr())
-    lib = _lib.load()
-    size = lib.hbfsim_kv_compact_workspace_v1(batch + _NO_WORKSPACE)
-    space = refs.new_empty(size // 4)
+        _COMPACT.size + _WORKSPACE.size, 1, seqs, width, pages, refs.data_ptr(), table.data_ptr(),
+        table.stride(0), new_refs.data_ptr(), new_table.data_ptr(), new_table.stride(0),
+        src.data_ptr(), dst.data_ptr(), live.data_ptr(), where.data_ptr())
     check(lib.hbfsim_kv_compact_v1(batch + _WORKSPACE.pack(space.data_ptr(), size),
                                    _handle(index)), "hbfsim_kv_compact_v1")
     return KvCompacted(new_refs, new_table, src, dst, live, where)
