@@ -192,21 +192,12 @@ struct Lane {
         }
         if (!turns) return;
         if constexpr (kLayout == kNeighbours) {
-            float2 p[2 * N];  // pairs of channels
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                p[i] = x[i];
-                p[N + i] = y[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 2 * N; ++i) {
+            for (int i = 0; i < 2 * N; ++i) {  // pairs of channels, N at lo and N at hi
                 const float c = i & 1 ? a.c[i / 2].y : a.c[i / 2].x, s = i & 1 ? a.s[i / 2].y : a.s[i / 2].x;
-                p[i] = add2(mul2(p[i], make_float2(c, c)), mul2(make_float2(p[i].y, p[i].x), make_float2(-s, s)));
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                x[i] = p[i];
-                y[i] = p[N + i];
+                float2& p = i < N ? x[i % N] : y[i % N];
+                p = make_float2(__fsub_rn(__fmul_rn(p.x, c), __fmul_rn(p.y, s)),
+                                __fadd_rn(__fmul_rn(p.x, s), __fmul_rn(p.y, c)));
             }
         } else {
 #pragma unroll
@@ -322,49 +313,48 @@ struct Join {
 
 // A head's keys of a block by `parts` warps (block / 16 of them), of which this is the part-th; all
 // warps of the CTA come here, the same number of times.  Rounding keeps the order, so the least and
-// greatest of a channel give its bounds.  `table` begins with the block's first new token.  kFull: all
-// 16 rows are new, and the block is one warp's.  False, with nothing written, where a turned element
-// is not finite.
-template <typename T, int D, bool kWide, int kLayout, bool kFull>
+// greatest of a channel give its bounds.  `table` begins with the block's first new token.  False, with
+// nothing written, where a turned element is not finite.
+template <typename T, int D, bool kWide, int kLayout>
 __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, u32 head, u32 token, int page, u32 slot,
                                               u32 count, u32 part, u32 parts, const Table& table, Join<D>& join)
 {
     using Of = Lane<D, kLayout>;
     constexpr int N = Of::N;
-    constexpr u32 R = 4;  // steps of two rows at a time
+    constexpr u32 R = 2;  // steps of two rows at a time
     const Of mine(table.pairs);
     const u32 lane = threadIdx.x & 31u, half = lane >> 4, warp = threadIdx.x >> 5, block = a.c.block;
     const u64 at = (static_cast<u64>(page) * a.c.heads + head) * 2;
     u8* out = a.c.data + at * block * D;
     // the warp's rows: [first, held) are there already, [from, to) are new
-    const u32 first = kFull ? 0 : part * 16, from = kFull ? 0 : max(slot, first);
-    u32 held = kFull ? 0 : min(slot, first + 16);
-    const u32 to = kFull ? 16 : active ? min(slot + count, first + 16) : 0;
+    const u32 first = part * 16, from = max(slot, first), to = active ? min(slot + count, first + 16) : 0;
+    const u32 held = min(slot, first + 16);
+    const bool full = from + 16 == to;  // of new ones: the rows' places are plain then
     const i64 stride = a.stride_token[0];
-    const u16* x = static_cast<const u16*>(a.x[0]) + (static_cast<i64>(token) - (kFull ? 0 : slot)) * stride +
+    const u16* x = static_cast<const u16*>(a.x[0]) + (static_cast<i64>(token) - slot) * stride +
                    static_cast<i64>(head) * a.stride_head[0];
-    // past the end: the last row again
-    auto row_at = [&](u32 row) { return kFull ? row : min(row, to - 1); };
-    // turned: the channels at mine.lo and at mine.hi (16 rows held from the first time on, and 16
-    // warps on an SM instead of 24, took 149 us for prompts that take 136)
+    // Turned: the channels at mine.lo and at mine.hi.  16 rows kept from the first time on, with 16
+    // warps on an SM, took 149 us for prompts that take 143 with 8 rows at a time (20 warps) and 139
+    // with 4 (24 warps).
     float2 y[R][2][N];
-    auto turn_rows = [&](u32 row0) {
+    auto turn_rows = [&](u32 row0, auto plain_rows) {
+        constexpr bool kPlain = decltype(plain_rows)::value;
+        auto row_at = [&](u32 r) { return kPlain ? row0 + 2 * r + half : min(row0 + 2 * r + half, to - 1); };  // or the last again
         u32 low[R][N], high[R][N];
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
-            const u32 row = row_at(row0 + 2 * r + half);
-            load_words<N, kWide>(x + row * stride + mine.lo, low[r]);
-            load_words<N, kWide>(x + row * stride + mine.hi, high[r]);
+            load_words<N, kWide>(x + row_at(r) * stride + mine.lo, low[r]);
+            load_words<N, kWide>(x + row_at(r) * stride + mine.hi, high[r]);
         }
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
             typename Of::Circle circle;
-            const u32 row = (row_at(row0 + 2 * r + half) - (kFull ? 0 : slot)) * table.pairs;
+            const u32 row = (row_at(r) - slot) * table.pairs;
             mine.load(table.cosines + row, table.sines + row, circle);
             mine.template apply<T>(low[r], high[r], circle, y[r][0], y[r][1]);
         }
     };
-    const float was = !kFull && active && slot ? a.c.scale[at] : 0.0f;  // written only after all have met
+    const float was = active && slot ? a.c.scale[at] : 0.0f;  // written only after all have met
     constexpr float kMost = 3.402823466e38f;
     float2 lo[2][N], hi[2][N];  // least and greatest of the channels
 #pragma unroll
@@ -378,15 +368,20 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
         lo[k][i] = make_float2(least_of(lo[k][i].x, z.x), least_of(lo[k][i].y, z.y));
         hi[k][i] = make_float2(greatest_of(hi[k][i].x, z.x), greatest_of(hi[k][i].y, z.y));
     };
-    for (u32 row0 = from; row0 < to; row0 += 2 * R) {
-        turn_rows(row0);
+    auto find_ends = [&](auto plain_rows) {
+#pragma unroll 1
+        for (u32 row0 = from; row0 < to; row0 += 2 * R) {
+            turn_rows(row0, plain_rows);
 #pragma unroll
-        for (u32 r = 0; r < R; ++r)
+            for (u32 r = 0; r < R; ++r)
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < N; ++i) span(k, i, y[r][k][i]);
-    }
+                    for (int i = 0; i < N; ++i) span(k, i, y[r][k][i]);
+        }
+    };
+    if (full) find_ends(std::true_type{});
+    else find_ends(std::false_type{});
     float most = 0.0f;  // NaN if any is
     if (from < to) {
 #pragma unroll
@@ -398,17 +393,18 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) most = greatest_of(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (!kFull && parts > 1) {
+    if (parts > 1) {
         if (lane == 0) join.most[warp] = most;
         __syncthreads();
         for (u32 i = 0; i < parts; ++i) most = greatest_of(most, join.most[warp - part + i]);
     }
     const bool plain = most <= kMost;
     const float now = fmaxf(kv_power(scale_exponent(plain ? most : 0.0f)), was), inverse = 1.0f / now;
-    if (active && plain) {
-        if (lane == 0 && part == 0) a.c.scale[at] = now;
+    auto store_rows = [&](auto plain_rows) {
+        constexpr bool kPlain = decltype(plain_rows)::value;
+#pragma unroll 1
         for (u32 row0 = from; row0 < to; row0 += 2 * R) {
-            turn_rows(row0);
+            turn_rows(row0, plain_rows);
 #pragma unroll
             for (u32 r = 0; r < R; ++r) {
                 u32 b[2][N];
@@ -417,18 +413,22 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
 #pragma unroll
                     for (int i = 0; i < N; ++i) b[k][i] = store_e4m3(mul2(y[r][k][i], make_float2(inverse, inverse)));
                 const u32 row = row0 + 2 * r + half;
-                if (kFull || row < to) {
+                if (kPlain || row < to) {
                     store_values<N>(out + row * D + mine.lo, b[0]);
                     store_values<N>(out + row * D + mine.hi, b[1]);
                 }
             }
         }
+    };
+    if (active && plain) {
+        if (lane == 0 && part == 0) a.c.scale[at] = now;
+        if (full) store_rows(std::true_type{});
+        else store_rows(std::false_type{});
         const u32 none[N] = {};
-        if (!kFull)
-            for (u32 row = max(slot + count, first) + half; row < first + 16; row += 2) {
-                store_values<N>(out + row * D + mine.lo, none);
-                store_values<N>(out + row * D + mine.hi, none);
-            }
+        for (u32 row = max(slot + count, first) + half; row < first + 16; row += 2) {
+            store_values<N>(out + row * D + mine.lo, none);
+            store_values<N>(out + row * D + mine.hi, none);
+        }
     }
     // from here on in units of the scale
 #pragma unroll
@@ -438,8 +438,7 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
             lo[k][i] = mul2(lo[k][i], make_float2(inverse, inverse));
             hi[k][i] = mul2(hi[k][i], make_float2(inverse, inverse));
         }
-    if constexpr (!kFull) {  // what the block held before: rounded again if the scale grew
-        if (!active || !plain) held = 0;
+    if (active && plain) {  // what the block held before: rounded again if the scale grew
         const float shrink = slot ? was / now : 1.0f;
         for (u32 row0 = first; row0 < held; row0 += 2 * R) {
             u32 b[R][2][N];
@@ -485,7 +484,7 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
             ends[k][i] = half ? make_float2(fmaxf(keep.x, other.x), fmaxf(keep.y, other.y))
                               : make_float2(fminf(keep.x, other.x), fminf(keep.y, other.y));
         }
-    if (!kFull && parts > 1) {
+    if (parts > 1) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -618,11 +617,9 @@ __device__ __forceinline__ void append_keys(const RotaryArgs& r, u32 block, floa
         const u32 row = (p.who - first) * pairs, token = base + p.who;
         const Table table{cosines + row, sines + row, pairs};
         bool done = false;
-        if (parts > 1 || (active && p.count > 4 && p.count < 16))
-            done = append_turned<T, D, kWide, kLayout, false>(a, active, p.head, token, p.page, p.slot, p.count, part,
-                                                              parts, table, join);
-        else if (active && p.count == 16)
-            done = append_turned<T, D, kWide, kLayout, true>(a, true, p.head, token, p.page, 0, 16, 0, 1, table, join);
+        if (parts > 1 || (active && p.count > 4))
+            done = append_turned<T, D, kWide, kLayout>(a, active, p.head, token, p.page, p.slot, p.count, part, parts,
+                                                       table, join);
         // few tokens, for which the code for many takes longer, and elements that are not finite
         if (active && part == 0 && !done)
             append_rows<T, D, kWide, kLayout>(a, p.head, token, p.page, p.slot, p.count, table);
@@ -645,7 +642,7 @@ __device__ __forceinline__ void append_values(const RotaryArgs& r, u32 block)
 }
 
 template <typename T, int D, bool kWide, int kLayout>
-__global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : D == 128 ? 5 : 6) rotary_kernel(const RotaryArgs r)
+__global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : D == 128 ? 6 : 8) rotary_kernel(const RotaryArgs r)
 {
     extern __shared__ float4 shared[];
     u32 block = blockIdx.x;
@@ -739,10 +736,10 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
     while (a.chunk < 16 && static_cast<u64>(a.tokens) * heads * 2 > a.chunk * warps) a.chunk *= 2;
     if (append) {
         // A CTA takes as many heads' keys of a block at once as it has warps for, 16 rows to a warp; where
-        // that makes many more CTAs than are resident, twice as many share a block's cosines.
+        // that makes many more CTAs than are resident, eight share a block's cosines, one after the other.
         const u32 chunks = (a.tokens + a.chunk - 1) / a.chunk, teams = kRotaryWarps / (a.c.block / 16);
         const u64 pieces = (static_cast<u64>(a.tokens) / a.c.block + a.seqs) * heads;
-        const u32 by = teams * (pieces > 2ull * teams * kv_sm_count() * 6 ? 2 : 1);
+        const u32 by = pieces > 12ull * teams * kv_sm_count() ? 8 : teams;
         r.key_spread = (heads + by - 1) / by;
         r.value_spread = (heads + kRotaryWarps - 1) / kRotaryWarps;
         r.key_blocks = chunks * r.key_spread;
