@@ -754,7 +754,8 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyArgs a)
         const u64 group = unit / a.per_page, move = group * a.group + lane;
         const u32 part = static_cast<u32>(unit - group * a.per_page);
         const bool listed = lane < a.group && move < a.count;
-        const u32 page = listed ? static_cast<u32>(a.src[move]) : ~0u, page_to = listed ? static_cast<u32>(a.dst[move]) : ~0u;
+        const u32 page = listed ? static_cast<u32>(a.src[move]) : ~0u;
+        const u32 page_to = listed ? static_cast<u32>(a.dst[move]) : ~0u;
         u32 left_moves = __ballot_sync(0xffffffffu, page < a.from.pages && page_to < a.to.pages);
         for (; left_moves; left_moves &= left_moves - 1) {
             const int which = __ffs(left_moves) - 1;
@@ -867,7 +868,8 @@ bool cluster(void (*kernel)(Args), u32 team, const Args& a, cudaStream_t s)
 u32 cluster_size(u64 counts, u64 entries, u64 runs)
 {
     u32 team = 1;
-    while (team < kPageTeam && (counts > team * kCountsEach || entries > team * kEntriesEach || runs > team * kPageWarps))
+    while (team < kPageTeam &&
+           (counts > team * kCountsEach || entries > team * kEntriesEach || runs > team * kPageWarps))
         team *= 2;
     return counts > kPageTeam * kCountsMost || entries > team * kEntriesMost ? 0 : team;
 }
@@ -965,7 +967,8 @@ extern "C" int hbfsim_kv_fork_v1(const hbfsim_kv_fork_batch_v1* b, void* stream)
     const bool apart = b->refs_out != b->refs;
     // counts that are where they belong need no pass of their own
     const u32 blocks = pass_blocks();
-    const bool ok = apart ? pass(fork_pass_kernel<0>, blocks, false, a, s) && pass(fork_pass_kernel<1>, blocks, true, a, s)
+    const bool ok = apart ? pass(fork_pass_kernel<0>, blocks, false, a, s) &&
+                                pass(fork_pass_kernel<1>, blocks, true, a, s)
                           : pass(fork_pass_kernel<2>, blocks, false, a, s);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }
@@ -1039,6 +1042,7 @@ extern "C" int hbfsim_kv_copy_v1(const hbfsim_kv_cache_v1* from, const hbfsim_kv
     a.group = static_cast<u32>(std::min<u64>(kCopyGroup, count * a.per_page / (512ull * kv_sm_count()) + 1));
     a.groups = (count + a.group - 1) / a.group;
     const u32 blocks = static_cast<u32>(std::min<u64>(a.groups * a.per_page, 0x7fffffffull));
-    const bool ok = kv_launch(copy_kernel, dim3(blocks), kCopyThreads, static_cast<cudaStream_t>(stream), 0, 1, false, a);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool ok = kv_launch(copy_kernel, dim3(blocks), kCopyThreads, s, 0, 1, false, a);
     return ok ? HBFSIM_OK : HBFSIM_CUDA_ERROR;
 }

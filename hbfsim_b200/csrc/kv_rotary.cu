@@ -94,9 +94,14 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b)
         : "l"(*reinterpret_cast<u64*>(&a)), "l"(*reinterpret_cast<u64*>(&b)));
     return *reinterpret_cast<float2*>(&r);
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
-
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return make_float2(__fsub_rn(a.x, b.x), __fsub_rn(a.y, b.y)); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
+}
+__device__ __forceinline__ float2 sub2(float2 a, float2 b)
+{
+    return make_float2(__fsub_rn(a.x, b.x), __fsub_rn(a.y, b.y));
+}
 
 __device__ __forceinline__ u32 packed(float2 x, __nv_bfloat16)
 {
@@ -109,12 +114,7 @@ __device__ __forceinline__ u32 packed(float2 x, __half)
     return *reinterpret_cast<const u32*>(&y);
 }
 
-// N words of two elements or of two numbers.
-template <int N, bool kWide>
-__device__ __forceinline__ void load_words(const u16* from, u32 (&x)[N])
-{
-    load_row<N, kWide>(from, x);
-}
+// N words of two elements, or N pairs of numbers.
 template <int N>
 __device__ __forceinline__ void store_words(u16* to, const u32 (&x)[N])
 {
@@ -240,7 +240,8 @@ struct TurnedRow {
         const float* s = table.sines + t * pairs + pair;
         u32 raw[W], other[W];
         load_row<W, kWide>(x + t * stride, raw);
-        const int away = kLayout == kNeighbours || !turns ? 0 : second ? -static_cast<int>(pairs) : static_cast<int>(pairs);
+        const int apart = static_cast<int>(pairs);
+        const int away = kLayout == kNeighbours || !turns ? 0 : second ? -apart : apart;
         load_row<W, kWide>(x + t * stride + away, other);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -304,7 +305,7 @@ __device__ __forceinline__ void load_values(const u8* from, u32 (&b)[N])
 // A head's keys of a block by one warp, a row at a time.
 template <typename T, int D, bool kWide, int kLayout>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, u32 head, u32 token, int page, u32 slot, u32 count,
-                                         const Table& table)
+                                            const Table& table)
 {
     const PlainRow<T, D, kWide> from(a, head, 0, token);
     append_block<D>(a, head, 0, page, slot, count, TurnedRow<T, D, kWide, kLayout>{from.x, from.stride, table});
@@ -345,12 +346,14 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
     float2 y[R][2][N];
     auto turn_rows = [&](u32 row0, auto plain_rows) {
         constexpr bool kPlain = decltype(plain_rows)::value;
-        auto row_at = [&](u32 r) { return kPlain ? row0 + 2 * r + half : min(row0 + 2 * r + half, to - 1); };  // or the last again
+        auto row_at = [&](u32 r) {  // past the end: the last again
+            return kPlain ? row0 + 2 * r + half : min(row0 + 2 * r + half, to - 1);
+        };
         u32 low[R][N], high[R][N];
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
-            load_words<N, kWide>(x + row_at(r) * stride + mine.lo, low[r]);
-            load_words<N, kWide>(x + row_at(r) * stride + mine.hi, high[r]);
+            load_row<N, kWide>(x + row_at(r) * stride + mine.lo, low[r]);
+            load_row<N, kWide>(x + row_at(r) * stride + mine.hi, high[r]);
         }
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
@@ -502,8 +505,8 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float2 z = *reinterpret_cast<const float2*>(&join.ends[w][half][(k ? mine.hi : mine.lo) + 2 * i]);
-                    const float2 e = ends[k][i];
+                    const float* other = &join.ends[w][half][(k ? mine.hi : mine.lo) + 2 * i];
+                    const float2 z = *reinterpret_cast<const float2*>(other), e = ends[k][i];
                     ends[k][i] = half ? make_float2(fmaxf(e.x, z.x), fmaxf(e.y, z.y))
                                       : make_float2(fminf(e.x, z.x), fminf(e.y, z.y));
                 }
@@ -543,8 +546,8 @@ __device__ __forceinline__ void turn_queries(const RotaryArgs& r, u32 token, u32
 #pragma unroll
         for (u32 i = 0; i < R; ++i) {
             if (first + 2 * i < end) {
-                load_words<N, kWide>(x, l[i]);
-                load_words<N, kWide>(x + away, h[i]);
+                load_row<N, kWide>(x, l[i]);
+                load_row<N, kWide>(x + away, h[i]);
             }
             x += two;
         }
@@ -664,14 +667,15 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : D == 128 ? 6
     block -= r.value_blocks;
     const u64 item = static_cast<u64>(block) * kRotaryWarps + (threadIdx.x >> 5);
     const u32 token = static_cast<u32>(item / r.parts);
-    if (token < r.a.tokens)
-        turn_queries<T, D, kWide, kLayout>(r, token, static_cast<u32>(item - static_cast<u64>(token) * r.parts) * r.part);
+    const u32 part = static_cast<u32>(item - static_cast<u64>(token) * r.parts);
+    if (token < r.a.tokens) turn_queries<T, D, kWide, kLayout>(r, token, part * r.part);
 }
 
 template <typename T, int D, bool kWide, int kLayout>
 bool launch(const RotaryArgs& r, cudaStream_t s)
 {
-    const u32 smem = r.key_blocks ? (r.a.chunk - 1 + r.a.c.block) * r.pairs * 8 + (r.a.c.block > 16 ? sizeof(Join<D>) : 0) : 0;
+    const u32 join = r.a.c.block > 16 ? sizeof(Join<D>) : 0;
+    const u32 smem = r.key_blocks ? (r.a.chunk - 1 + r.a.c.block) * r.pairs * 8 + join : 0;
     constexpr u32 kMost = (15 + 64) * (D / 2) * 8 + sizeof(Join<D>);
     static std::atomic<u64> seen{0};
     if (smem > 48 * 1024 && !kv_allow_smem(rotary_kernel<T, D, kWide, kLayout>, kMost, seen)) return false;
