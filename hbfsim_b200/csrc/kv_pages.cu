@@ -5,9 +5,9 @@
 // The work is a few passes over the counts and the table, each of which needs
 // all of the one before: what goes back has to be counted before free pages are
 // ranked, and ranked before they are given.  The passes are device functions of
-// a team of thread blocks.  A small pool is done by one cluster of up to 8 in one
-// launch, with cluster barriers between the passes; a large one by as many
-// blocks as the device has SMs, a launch to a pass.  Where ranks count, a warp has
+// a team of thread blocks.  A small pool is done in one launch by one of them, or for
+// a resize by a cluster of up to 8 with cluster barriers between the passes; a large
+// one by as many blocks as the device has SMs, a launch to a pass.  Where ranks count, a warp has
 // a contiguous share, so that they are sums over the warps before it.
 //
 // Latency bounds all of it but the copies: every pass is two or three dependent reads
@@ -26,12 +26,14 @@ constexpr u32 kPageThreads = 1024, kPageWarps = kPageThreads / 32;
 constexpr u32 kPageTeam = 8;      // blocks of the cluster
 constexpr u32 kMaxParts = 1024;   // blocks of a pass at most
 constexpr u32 kDeep = 16;         // entries of a table's row that a lane has under way
-// Counts and entries that are worth a block of a cluster, and that one takes at most.  A cluster costs
-// about 2 us: a pool of 2,600 counts and 4,000 entries is compacted in 6.2 us by one block, in 8.0 us by
-// two to eight and in 8.4 us by a launch to a pass; before a step of 64 rows of 2048 entries, 70,000
-// counts, a resize takes 17.6 us by 8 blocks and 16.6 us by a launch to a pass, which cost the host 10 us
-// more; 200 rows of 190 entries 17.1 us by 8 blocks and 23.6 us by 4, with two rows to a warp.
+// Of a resize: counts and entries that are worth a block of a cluster, and that one takes at most.  A
+// cluster costs about 2 us.  Before a step of 64 rows of 2048 entries, 70,000 counts, a resize takes 17.6
+// us by 8 blocks and 16.6 us by a launch to a pass, which cost the host 10 us more; 200 rows of 190
+// entries 17.1 us by 8 blocks and 23.6 us by 4, with two rows to a warp.
 constexpr u64 kCountsEach = 16384, kEntriesEach = 16384, kCountsMost = 32768, kEntriesMost = 16384;
+// Of a compaction: counts and entries that one block does alone: 4,000 of both in 8.0 us and 9.8 us by a
+// launch to a pass, 8,000 in 11.0 and 10.4 us (and 5 us more of the host), 16,000 in 19.9 and 10.6 us.
+constexpr u64 kCompactMost = 8192;
 
 // The elements [from, end) of a warp.
 struct Share {
@@ -668,7 +670,7 @@ __device__ void compact_move(const CompactArgs& a, const KvTeam& team)
     }
 }
 
-__global__ void __launch_bounds__(kPageThreads) compact_cluster_kernel(const CompactArgs a)
+__global__ void __launch_bounds__(kPageThreads) compact_small_kernel(const CompactArgs a)
 {
     __shared__ u32 sm[3][kPageWarps];
     const KvTeam team{blockIdx.x, gridDim.x};
@@ -863,7 +865,7 @@ bool cluster(void (*kernel)(Args), u32 team, const Args& a, cudaStream_t s)
 }
 
 // Blocks of a cluster that does `counts` counts and `entries` entries in one launch; 0: too much for
-// it.  (The entries of an eviction's lists are not counted: few of their places are taken.)
+// it.  The entries of an eviction's lists are not counted: few of their places are taken.
 // `runs`: of rows, a warp each.
 u32 cluster_size(u64 counts, u64 entries, u64 runs)
 {
@@ -1008,13 +1010,17 @@ extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* s
                           {b->workspace, part_bytes()}};
     const Extent in[] = {{b->refs, b->pages * 4}, {b->table, b->seqs, b->width, b->table_stride}};
     if (would_race(out, in, {0, 1, -1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
-    const CompactArgs a{b->refs, b->table, b->table_stride, b->refs_out, b->table_out, b->table_out_stride, b->src,
-                        b->dst, b->live, b->where, b->seqs, b->width, static_cast<u32>(b->pages),
-                        static_cast<u32*>(b->workspace)};
+    CompactArgs a{b->refs, b->table, b->table_stride, b->refs_out, b->table_out, b->table_out_stride, b->src,
+                  b->dst, b->live, b->where, b->seqs, b->width, static_cast<u32>(b->pages),
+                  static_cast<u32*>(b->workspace)};
+    if (b->table_stride == static_cast<i64>(b->width) && b->table_out_stride == static_cast<i64>(b->width)) {
+        a.seqs = 1;  // rows side by side are one: narrow ones would each take a warp
+        a.width = static_cast<u32>(entries);
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     bool ok;
-    if (const u32 team = cluster_size(b->pages, entries, 0)) {
-        ok = cluster(compact_cluster_kernel, team, a, s);
+    if (b->pages <= kCompactMost && entries <= kCompactMost) {
+        ok = cluster(compact_small_kernel, 1, a, s);
     } else {
         const u32 blocks = pass_blocks();
         ok = pass(compact_pass_kernel<0>, blocks, false, a, s) && pass(compact_pass_kernel<1>, blocks, true, a, s) &&
