@@ -488,11 +488,11 @@ __global__ void __launch_bounds__(kPageThreads) resize_pass_kernel(const ResizeA
     kv_let_next();
     kv_wait_before();
     const KvTeam team{blockIdx.x, gridDim.x};
-    if constexpr (kPass == 0) resize_begin(a, team);
-    else if constexpr (kPass == 1) resize_back(a, team);
-    else if constexpr (kPass == 2) resize_count(a, team);
-    else if constexpr (kPass == 3) resize_rank(a, team, warp_sums);
-    else resize_give(a, team, warp_sums);
+    if constexpr (kPass == 0 || kPass == 5) resize_begin(a, team);
+    if constexpr (kPass == 1 || kPass == 5) resize_back(a, team);
+    if constexpr (kPass == 2) resize_count(a, team);
+    if constexpr (kPass == 3) resize_rank(a, team, warp_sums);
+    if constexpr (kPass == 4) resize_give(a, team, warp_sums);
 }
 
 // ---------------------------------------------------------------------------
@@ -932,7 +932,10 @@ extern "C" int hbfsim_kv_resize_v1(const hbfsim_kv_resize_batch_v1* b, void* str
         ok = cluster(resize_cluster_kernel, team, a, s);
     } else {
         const u32 blocks = pass_blocks();
-        ok = pass(resize_pass_kernel<0>, blocks, false, a, s) && pass(resize_pass_kernel<1>, blocks, true, a, s) &&
+        // counts that are where they belong need not be there before others change
+        ok = (b->refs_out == b->refs ? pass(resize_pass_kernel<5>, blocks, false, a, s)
+                                     : pass(resize_pass_kernel<0>, blocks, false, a, s) &&
+                                           pass(resize_pass_kernel<1>, blocks, true, a, s)) &&
              pass(resize_pass_kernel<2>, blocks, true, a, s) && pass(resize_pass_kernel<3>, blocks, true, a, s) &&
              pass(resize_pass_kernel<4>, blocks, true, a, s);
     }

@@ -14,8 +14,8 @@
 // stored does not depend on how a compiler joins them.
 //
 // Prompts of 31,668 tokens in all (32 query and 8 key/value heads of 128 channels)
-// take 140 us, 718 MB of input, queries and blocks at 5.1 TB/s, 78 % of a copy's rate:
-// the queries alone 90 us (5.8 TB/s, DRAM), the keys and values alone 79 us, where
+// take 134 us, 718 MB of input, queries and blocks at 5.4 TB/s, 82 % of a copy's rate:
+// the queries alone 90 us (5.8 TB/s, DRAM), the keys and values alone 75 us, where
 // warps wait for their rows at 60 % of the issue slots.  A step's 64 tokens take 5.8
 // us: a launch, the chain of reads of an append, the positions and one turn of 64-bit
 // arithmetic.
@@ -342,7 +342,7 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
                    static_cast<i64>(head) * a.stride_head[0];
     // Turned: the channels at mine.lo and at mine.hi.  16 rows kept from the first time on, with 16
     // warps on an SM, took 149 us for prompts that take 143 with 8 rows at a time (20 warps) and 139
-    // with 4 (24 warps).
+    // with 4 (24 warps), in chunks of 16 tokens.
     float2 y[R][2][N];
     auto turn_rows = [&](u32 row0, auto plain_rows) {
         constexpr bool kPlain = decltype(plain_rows)::value;
@@ -676,7 +676,7 @@ bool launch(const RotaryArgs& r, cudaStream_t s)
 {
     const u32 join = r.a.c.block > 16 ? sizeof(Join<D>) : 0;
     const u32 smem = r.key_blocks ? (r.a.chunk - 1 + r.a.c.block) * r.pairs * 8 + join : 0;
-    constexpr u32 kMost = (15 + 64) * (D / 2) * 8 + sizeof(Join<D>);
+    constexpr u32 kMost = (31 + 64) * (D / 2) * 8 + sizeof(Join<D>);
     static std::atomic<u64> seen{0};
     if (smem > 48 * 1024 && !kv_allow_smem(rotary_kernel<T, D, kWide, kLayout>, kMost, seen)) return false;
     const u64 items = static_cast<u64>(r.a.tokens) * r.parts;
@@ -739,11 +739,15 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
     r.axes = x->axes;
     r.pairs = x->pairs;
     a.wide = a.wide && (x->q_heads == 0 || kv_rows_wide(x->q, x->q_stride_token, x->q_stride_head));
-    // Chunks as in kv_append.cu; few tokens get a warp to each head and side.
+    // Chunks as in kv_append.cu; few tokens get a warp to each head and side.  Large batches in blocks of
+    // 16 get chunks of 32 tokens: what comes before the first row of a chunk (the search for its blocks,
+    // the cosines) is shared by two blocks (prompts of 31,668 tokens: 139 us with 16, 134 us with 32; in
+    // blocks of 32, 142 and 160 us).
     const u32 heads = a.c.heads, groups = (r.q_heads + kRotaryHeads - 1) / kRotaryHeads;
     const u64 warps = static_cast<u64>(kv_sm_count()) * 16;  // resident at once
     a.chunk = 1;
-    while (a.chunk < 16 && static_cast<u64>(a.tokens) * heads * 2 > a.chunk * warps) a.chunk *= 2;
+    const u32 most = a.c.block == 16 ? 32 : 16;
+    while (a.chunk < most && static_cast<u64>(a.tokens) * heads * 2 > a.chunk * warps) a.chunk *= 2;
     if (append) {
         // A CTA takes as many heads' keys of a block at once as it has warps for, 16 rows to a warp; where
         // that makes many more CTAs than are resident, eight share a block's cosines, one after the other.
