@@ -135,24 +135,31 @@ __device__ __forceinline__ void block_sums(u32 (&x)[N], u32 (*warp_sums)[kPageWa
 }
 
 // Sums of the parts of earlier warps (of every block) and of all; of other parts, if given, of all.
+// begin() asks for them, end() adds them up.
 struct Before {
     u32 mine, all, others;
-};
-__device__ __forceinline__ Before before_of(const u32* parts, const KvTeam& team, u32 (*warp_sums)[kPageWarps],
-                                            const u32* others = nullptr)
-{
-    const u32 lane = threadIdx.x & 31u, own = team.rank * kPageWarps, n = team.size * kPageWarps;
-    const u32 inside = lane < threadIdx.x >> 5 ? parts[own + lane] : 0;
-    u32 x[3] = {0, 0, 0};
-    for (u32 i = threadIdx.x; i < n; i += kPageThreads) {
-        const u32 part = parts[i];
-        x[1] += part;
-        if (i < own) x[0] += part;
-        if (others) x[2] += others[i];
+    u32 inside, x[3];
+
+    __device__ __forceinline__ void begin(const u32* parts, const KvTeam& team, const u32* more = nullptr)
+    {
+        const u32 lane = threadIdx.x & 31u, own = team.rank * kPageWarps, n = team.size * kPageWarps;
+        inside = lane < threadIdx.x >> 5 ? parts[own + lane] : 0;
+        x[0] = x[1] = x[2] = 0;
+        for (u32 i = threadIdx.x; i < n; i += kPageThreads) {
+            const u32 part = parts[i];
+            x[1] += part;
+            if (i < own) x[0] += part;
+            if (more) x[2] += more[i];
+        }
     }
-    block_sums(x, warp_sums);
-    return {x[0] + __reduce_add_sync(0xffffffffu, inside), x[1], x[2]};
-}
+    __device__ __forceinline__ void end(u32 (*warp_sums)[kPageWarps])
+    {
+        block_sums(x, warp_sums);
+        mine = x[0] + __reduce_add_sync(0xffffffffu, inside);
+        all = x[1];
+        others = x[2];
+    }
+};
 
 // Calls run(row, from, end) for runs of a table's rows, up to 32 * Deep entries to a warp; the
 // blocks of a team take them in turn, so that few runs are spread over all of them.
@@ -385,6 +392,16 @@ __device__ void resize_count(const ResizeArgs& a, const KvTeam& team)
 __device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, u32 (*warp_sums)[kPageWarps])
 {
     u32 claims = 0;
+    Before before;
+    before.begin(a.free_part, team, a.asked_part);
+    // the first of the warp's counts, on their way while the asked blocks are looked at
+    const Share own = warp_share(a.pages, team);
+    Four f[4];
+    auto load_counts = [&](u32 p0) {
+#pragma unroll
+        for (u32 k = 0; k < 4; ++k) f[k] = load_four(a.refs_out, p0 + 128 * k + (threadIdx.x & 31u) * 4, own.end, 1);
+    };
+    load_counts(own.from);
     for_asked(a, team, [&](const Run& run, u32 j) {
         int e[kStep], count[kStep];
 #pragma unroll
@@ -403,16 +420,13 @@ __device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, u32 (*warp_
     });
     claims = __reduce_add_sync(0xffffffffu, claims);
     if ((threadIdx.x & 31u) == 0) a.claim_part[team.rank * kPageWarps + (threadIdx.x >> 5)] = claims;
-    const Before before = before_of(a.free_part, team, warp_sums, a.asked_part);
+    before.end(warp_sums);
     if (team.rank == 0 && threadIdx.x == 0) *a.free_all = before.all;
     u32 rank = before.mine;
-    const Share own = warp_share(a.pages, team);
 #pragma unroll 1
     for (u32 p0 = own.from; p0 < own.end && rank < before.others; p0 += 512) {
         const u32 p = p0 + (threadIdx.x & 31u) * 4;
-        Four f[4];
-#pragma unroll
-        for (u32 k = 0; k < 4; ++k) f[k] = load_four(a.refs_out, p + 128 * k, own.end, 1);
+        if (p0 != own.from) load_counts(p0);
 #pragma unroll
         for (u32 k = 0; k < 4; ++k) {
             const bool free[4] = {f[k].x[0] < 1, f[k].x[1] < 1, f[k].x[2] < 1, f[k].x[3] < 1};
@@ -430,7 +444,10 @@ __device__ void resize_rank(const ResizeArgs& a, const KvTeam& team, u32 (*warp_
 __device__ void resize_give(const ResizeArgs& a, const KvTeam& team, u32 (*warp_sums)[kPageWarps])
 {
     const u32 lane = threadIdx.x & 31u, free = *a.free_all;
-    u32 rank = before_of(a.claim_part, team, warp_sums).mine;
+    Before claims_before;
+    claims_before.begin(a.claim_part, team);
+    claims_before.end(warp_sums);
+    u32 rank = claims_before.mine;
     for_asked(a, team, [&](const Run& run, u32 j) {
         u32 state[kStep], before[kStep];
         int page[kStep];
@@ -598,7 +615,9 @@ __device__ void compact_count(const CompactArgs& a, const KvTeam& team)
 // holds -2 - move of a page that moves.
 __device__ void compact_rank(const CompactArgs& a, const KvTeam& team, u32 (*warp_sums)[kPageWarps])
 {
-    const Before before = before_of(a.live_part, team, warp_sums);
+    Before before;
+    before.begin(a.live_part, team);
+    before.end(warp_sums);
     const u32 n = before.all;
     if (team.rank == 0 && threadIdx.x == 0) *a.live = static_cast<int>(n);
     const Share own = warp_share(a.pages, team);
