@@ -7,16 +7,17 @@
 // ranked, and ranked before they are given.  The passes are device functions of
 // a team of thread blocks.  A small pool is done in one launch by one of them, or for
 // a resize by a cluster of up to 8 with cluster barriers between the passes; a large
-// one by as many blocks as the device has SMs, a launch to a pass.  Where ranks count, a warp has
-// a contiguous share, so that they are sums over the warps before it.
+// one by as many blocks as the device has SMs, a launch to a pass.  Where ranks
+// count, a warp has a contiguous share, so that they are sums over the warps before
+// it.
 //
 // Latency bounds all of it but the copies: every pass is two or three dependent reads
 // and a launch or a cluster barrier of 1 to 2 us.  A resize before a decode step (64
-// rows of 2,048 entries, 70,000 counts) takes 17.6 us, of a pool of 1.2 million pages
+// rows of 2,048 entries, 70,000 counts) takes 17.3 us, of a pool of 1.2 million pages
 // with 510 rows of 4,096 entries 32 us for 26 MB; a compaction of such a pool 21 us
 // for 31 MB (its random reads of the pages' new places are half of that), of one of
-// 2,600 pages 6.4 us; a fork of 64 beams 5.2 us, of 4 documents into 256 rows of
-// 16,385 entries 8.5 us for 17 MB.
+// 2,600 pages 6.6 us; a fork of 64 beams 5.3 us, of 4 documents into 256 rows of
+// 16,385 entries 8.4 us for 17 MB.
 #include "kv.h"
 
 namespace hbfb {

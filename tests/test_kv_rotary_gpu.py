@@ -289,6 +289,7 @@ def test_blocks_begun_and_ended_inside(dim, block):
     gpu = to_gpu(cache)
     assert kv_append_rotary(gpu, None, x[:, :heads], x[:, heads:], int32(table), int32(start), int32(positions), rotary,
                             offsets=int32(offsets)) is None
-    turned = ko.rotate(plain(x[:, :heads]), positions, rotary.freq.cpu().numpy(), rotary.axis.cpu().numpy(), False)
+    with np.errstate(over="ignore"):  # some turn into infinities
+        turned = ko.rotate(plain(x[:, :heads]), positions, rotary.freq.cpu().numpy(), rotary.axis.cpu().numpy(), False)
     ko.append(cache, turned.astype(np.float64), x[:, heads:].double().cpu().numpy(), table, start, offsets)
     same_cache(gpu, cache)
