@@ -312,8 +312,8 @@ int hbfsim_kv_verify_v1(const hbfsim_kv_verify_batch_v1* batch, void* stream);
  * 16, 32 or 64 tokens; pages, seqs * width and the lists' entries are below
  * 2^31.  Outputs that have an input's type and shape (refs, table) may be that
  * input's own memory (for tables: with the same stride); everything else lies in
- * memory apart.  Counts change by whole numbers: results do not depend on any
- * order. */
+ * memory apart, where a table's memory is all from its lowest row to its highest.
+ * Counts change by whole numbers: results do not depend on any order. */
 
 /* Every sequence gets or gives back pages, so that it can hold want[s] tokens
  * of which it holds lengths[s] (both clamped to [0, width * block_tokens]).

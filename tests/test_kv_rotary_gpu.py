@@ -293,3 +293,35 @@ def test_blocks_begun_and_ended_inside(dim, block):
         turned = ko.rotate(plain(x[:, :heads]), positions, rotary.freq.cpu().numpy(), rotary.axis.cpu().numpy(), False)
     ko.append(cache, turned.astype(np.float64), x[:, heads:].double().cpu().numpy(), table, start, offsets)
     same_cache(gpu, cache)
+
+
+def test_pool_and_queries_past_32_bit_offsets():
+    """Pages behind 2^32 bytes of a pool, tokens behind 2^31 elements of the projection."""
+    torch = torch_()
+    from hbfsim_b200 import KvCache, KvRotary, kv_append_rotary
+    rng = np.random.default_rng(12)
+    heads, dim, block = 8, 128, 16
+    pages = (1 << 32) // (heads * 2 * block * dim) + 5
+    gpu = KvCache.empty(pages, heads, dim, block)
+    rotary = KvRotary.of(dim)
+    qkv = torch.from_numpy(rng.standard_normal((40, 3 * heads, dim))).to(torch.bfloat16).cuda()
+    # 40 tokens whose rows lie 2^26 elements apart: the last 2.6 * 2^30 elements from the first
+    far = torch.empty(39 * (1 << 26) + 3 * heads * dim, dtype=torch.bfloat16, device="cuda")
+    rows = far.as_strided((40, 3 * heads, dim), (1 << 26, dim, 1))
+    rows.copy_(qkv)
+    table, start = np.array([[pages - 1, 3, pages - 4]], np.int32), np.array([5], np.int32)
+    places = np.arange(40, dtype=np.int32)[None] * 1000
+    q, k, v = rows[:, :heads], rows[:, heads:2 * heads], rows[:, 2 * heads:]
+    got = kv_append_rotary(gpu, q, k, v, int32(table), int32(start), int32(places), rotary, offsets=int32([0, 40]))
+    freq, axis = rotary.freq.cpu().numpy(), rotary.axis.cpu().numpy()
+    same_queries(got, qkv[:, :heads], places, freq, axis, False)
+    small = KvCache.empty(4, heads, dim, block)
+    cache = from_gpu(small)
+    turned = ko.rotate(plain(qkv[:, heads:2 * heads]), places, freq, axis, False).astype(np.float64)
+    ko.append(cache, turned, qkv[:, 2 * heads:].double().cpu().numpy(), np.array([[0, 1, 2]]), start, [0, 40])
+    for there, here in zip(table[0], range(3)):
+        assert np.array_equal(ko.E4M3[gpu.data.view(torch.uint8)[int(there)].cpu().numpy()], ko.E4M3[cache["data"][here]])
+        assert np.array_equal(gpu.scale[int(there)].double().cpu().numpy(), cache["scale"][here])
+        assert np.array_equal(gpu.bounds[int(there)].cpu().numpy(), cache["bounds"][here])
+    others = gpu.data.view(torch.uint8).view(pages, -1)
+    assert not others[[0, 1, 2, 4, pages - 2, pages - 3, pages - 5]].any()

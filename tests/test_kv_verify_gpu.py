@@ -170,3 +170,22 @@ def test_refusals(bad):
         call["tokens"] = None
     with pytest.raises((ValueError, HbfsimError)):
         kv_verify(**call)
+
+
+def test_rows_past_32_bit_offsets():
+    """The largest vocabulary, rows that begin behind 2^31 elements."""
+    torch = torch_()
+    from hbfsim_b200 import kv_verify
+    vocab, seqs = 1 << 22, 180
+    target = torch.zeros((seqs, 3, vocab), device="cuda")
+    target[:, :, 7] = 0.25
+    target[-1, 0, vocab - 1] = 0.5
+    target[-1, 1, 100] = 0.75
+    tokens = np.full((seqs, 2), 7, np.int32)
+    tokens[-1] = [vocab - 1, 3]
+    one = torch.full((seqs, 2), 0.3, device="cuda")
+    got = kv_verify(target, None, int32(tokens), one, torch.full((seqs,), 0.9, device="cuda"))
+    assert got.accepted.tolist() == [0] * (seqs - 1) + [1]
+    # all weight lies on the token that was not accepted: the target alone counts
+    assert got.tokens[:-1].tolist() == [[7, -1, -1]] * (seqs - 1)
+    assert got.tokens[-1].tolist() == [vocab - 1, 100, -1]
