@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 
 namespace hbfb {
 
@@ -43,6 +44,40 @@ struct KvQuery {
 inline bool kv_aligned(const void* p, std::uintptr_t a)
 {
     return reinterpret_cast<std::uintptr_t>(p) % a == 0;
+}
+
+// Memory [from, end), to see whether two ranges meet.
+struct KvExtent {
+    std::uintptr_t from, end;
+    KvExtent(const void* p, u64 bytes) : from(reinterpret_cast<std::uintptr_t>(p)), end(from + bytes) {}
+    // rows of a table, from the lowest to the highest
+    KvExtent(const int* p, u64 rows, u64 width, i64 stride) : KvExtent(p, rows, stride, 1, 0, width, 4) {}
+    // rows of `width` elements of `size` bytes on two axes, likewise; strides in elements
+    KvExtent(const void* p, u64 n, i64 stride, u64 m, i64 step, u64 width, u32 size) : from(0), end(0)
+    {
+        if (n == 0 || m == 0 || width == 0) return;
+        from = end = reinterpret_cast<std::uintptr_t>(p);
+        for (const u64 last : {(n - 1) * static_cast<u64>(stride) * size, (m - 1) * static_cast<u64>(step) * size})
+            (static_cast<i64>(last) < 0 ? from : end) += last;
+        end += width * size;
+    }
+    bool meets(const KvExtent& o) const { return from < end && o.from < o.end && from < o.end && o.from < end; }
+};
+
+// Whether an output meets an input or another output: thread blocks write the ones while others still
+// read.  same[i]: the input whose own memory output i may be, -1 for none.
+template <int kOut, int kIn>
+inline bool kv_would_race(const KvExtent (&out)[kOut], const KvExtent (&in)[kIn], const int (&same)[kOut])
+{
+    for (int i = 0; i < kOut; ++i) {
+        for (int k = 0; k < kIn; ++k) {
+            if (!out[i].meets(in[k])) continue;
+            if (same[i] != k || out[i].from != in[k].from || out[i].end != in[k].end) return true;
+        }
+        for (int k = 0; k < i; ++k)
+            if (out[i].meets(out[k])) return true;
+    }
+    return false;
 }
 
 // Checks a cache description; fills `v`.

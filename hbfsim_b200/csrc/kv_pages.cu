@@ -788,36 +788,6 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyArgs a)
 
 // ---------------------------------------------------------------------------
 
-// Memory [p, p + bytes), to see whether two ranges meet.
-struct Extent {
-    std::uintptr_t from, end;
-    Extent(const void* p, u64 bytes) : from(reinterpret_cast<std::uintptr_t>(p)), end(from + bytes) {}
-    // rows of a table, from the lowest to the highest
-    Extent(const int* p, u64 rows, u64 width, i64 stride) : from(0), end(0)
-    {
-        if (rows == 0 || width == 0) return;
-        const int* last = p + static_cast<i64>(rows - 1) * stride;
-        from = reinterpret_cast<std::uintptr_t>(std::min(p, last));
-        end = reinterpret_cast<std::uintptr_t>(std::max(p, last)) + width * 4;
-    }
-    bool meets(const Extent& o) const { return from < end && o.from < o.end && from < o.end && o.from < end; }
-};
-
-// Whether an output meets an input or another output.  same[i]: the input that output i may be.
-template <int kOut, int kIn>
-bool would_race(const Extent (&out)[kOut], const Extent (&in)[kIn], const int (&same)[kOut])
-{
-    for (int i = 0; i < kOut; ++i) {
-        for (int k = 0; k < kIn; ++k) {
-            if (!out[i].meets(in[k])) continue;
-            if (same[i] != k || out[i].from != in[k].from || out[i].end != in[k].end) return true;
-        }
-        for (int k = 0; k < i; ++k)
-            if (out[i].meets(out[k])) return true;
-    }
-    return false;
-}
-
 bool table_fits(u64 rows, u64 width) { return rows * width <= 0x7fffffffull; }
 
 // Takes parts of a workspace one after the other, 256 bytes aligned.
@@ -928,16 +898,16 @@ extern "C" int hbfsim_kv_resize_v1(const hbfsim_kv_resize_batch_v1* b, void* str
     if (entries && b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
     // rows of an output may not lie in one another
     if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
-    const Extent out[] = {{b->refs_out, b->pages * 4},
+    const KvExtent out[] = {{b->refs_out, b->pages * 4},
                           {b->table_out, b->seqs, b->width, b->table_out_stride},
                           {b->limits, u64{b->seqs} * 4},
                           {b->src, u64{b->seqs} * 4},
                           {b->dst, u64{b->seqs} * 4},
                           {b->workspace, room.bytes}};
-    const Extent in[] = {{b->refs, b->pages * 4},          {b->table, b->seqs, b->width, b->table_stride},
+    const KvExtent in[] = {{b->refs, b->pages * 4},          {b->table, b->seqs, b->width, b->table_stride},
                          {b->lengths, u64{b->seqs} * 4},   {b->want, u64{b->seqs} * 4},
                          {b->freed, listed * 4},           {b->freed_counts, u64{b->freed_rows} * 4}};
-    if (would_race(out, in, {0, 1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
+    if (kv_would_race(out, in, {0, 1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
     u8* w = static_cast<u8*>(b->workspace);
     const ResizeArgs a{b->refs, b->table, b->table_stride, b->lengths, b->want, b->freed, b->freed_counts,
                        b->refs_out, b->table_out, b->table_out_stride, b->limits, b->src, b->dst, b->seqs, b->width,
@@ -980,12 +950,12 @@ extern "C" int hbfsim_kv_fork_v1(const hbfsim_kv_fork_batch_v1* b, void* stream)
                           static_cast<const void*>(b->refs_out), static_cast<const void*>(b->table_out),
                           static_cast<const void*>(b->lengths_out)})
         if (!kv_aligned(p, 4)) return HBFSIM_INVALID_ARGUMENT;
-    const Extent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, made * 4}, {b->lengths_out, u64{b->rows} * 4}};
-    const Extent in[] = {{b->refs, b->pages * 4},
+    const KvExtent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, made * 4}, {b->lengths_out, u64{b->rows} * 4}};
+    const KvExtent in[] = {{b->refs, b->pages * 4},
                          {b->table, b->seqs, b->width, b->table_stride},
                          {b->lengths, u64{b->seqs} * 4},
                          {b->parents, u64{b->rows} * 4}};
-    if (would_race(out, in, {0, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
+    if (kv_would_race(out, in, {0, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
     const ForkArgs a{b->refs, b->table, b->table_stride, b->lengths, b->parents, b->refs_out, b->table_out,
                      b->lengths_out, b->seqs, b->rows, b->width, b->block_tokens, static_cast<u32>(b->pages)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1027,12 +997,12 @@ extern "C" int hbfsim_kv_compact_v1(const hbfsim_kv_compact_batch_v1* b, void* s
     if (!kv_aligned(b->workspace, 16) || b->workspace_bytes < part_bytes()) return HBFSIM_INVALID_ARGUMENT;
     if (entries && b->table_out == b->table && b->table_out_stride != b->table_stride) return HBFSIM_INVALID_ARGUMENT;
     if (b->seqs > 1 && std::abs(b->table_out_stride) < static_cast<i64>(b->width)) return HBFSIM_INVALID_ARGUMENT;
-    const Extent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, b->seqs, b->width, b->table_out_stride},
+    const KvExtent out[] = {{b->refs_out, b->pages * 4}, {b->table_out, b->seqs, b->width, b->table_out_stride},
                           {b->src, room * 4},          {b->dst, room * 4},
                           {b->live, 4},                {b->where, b->pages * 4},
                           {b->workspace, part_bytes()}};
-    const Extent in[] = {{b->refs, b->pages * 4}, {b->table, b->seqs, b->width, b->table_stride}};
-    if (would_race(out, in, {0, 1, -1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
+    const KvExtent in[] = {{b->refs, b->pages * 4}, {b->table, b->seqs, b->width, b->table_stride}};
+    if (kv_would_race(out, in, {0, 1, -1, -1, -1, -1, -1})) return HBFSIM_INVALID_ARGUMENT;
     CompactArgs a{b->refs, b->table, b->table_stride, b->refs_out, b->table_out, b->table_out_stride, b->src,
                   b->dst, b->live, b->where, b->seqs, b->width, static_cast<u32>(b->pages),
                   static_cast<u32*>(b->workspace)};

@@ -358,6 +358,19 @@ extern "C" int hbfsim_kv_verify_v1(const hbfsim_kv_verify_batch_v1* b, void* str
         !kv_aligned(b->lengths, 4) || !kv_aligned(b->accepted, 4) || !kv_aligned(b->tokens_out, 4) ||
         !kv_aligned(b->lengths_out, 4))
         return HBFSIM_INVALID_ARGUMENT;
+    // a sequence's own count and length are read before its outputs are written
+    const u64 seqs = b->seqs, per_seq = seqs * 4, per_draft = per_seq * b->drafts;
+    const KvExtent out[] = {{b->accepted, per_seq}, {b->tokens_out, per_draft + per_seq},
+                            {b->lengths_out, b->lengths_out ? per_seq : 0}};
+    const KvExtent in[] = {{b->counts, b->counts ? per_seq : 0},
+                           {b->lengths, b->lengths_out ? per_seq : 0},
+                           {b->tokens, per_draft},
+                           {b->accept, per_draft},
+                           {b->sample, per_seq},
+                           {b->target, seqs, b->target_stride_seq, b->drafts + 1ull, b->target_stride_token, b->vocab, size},
+                           {b->draft, b->draft ? seqs : 0, b->draft_stride_seq, b->drafts, b->draft_stride_token, b->vocab,
+                            size}};
+    if (kv_would_race(out, in, {0, -1, 1})) return HBFSIM_INVALID_ARGUMENT;
     VerifyArgs a{b->target, b->target_stride_seq, b->target_stride_token, b->draft, b->draft_stride_seq,
                  b->draft_stride_token, b->tokens, b->accept, b->sample, b->counts, b->lengths, b->accepted,
                  b->tokens_out, b->lengths_out, b->drafts, b->vocab, 0};

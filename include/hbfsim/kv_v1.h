@@ -275,6 +275,8 @@ int hbfsim_kv_evict_v1(const hbfsim_kv_evict_batch_v1* batch, void* stream);
  * behind.  accepted: int32 [seqs].  lengths_out (NULL to skip): lengths - (d -
  * a), the tokens that stay in the cache of a sequence whose `lengths` counts its
  * drafted ones.
+ * Outputs lie in memory apart from the inputs' and from each other's, but
+ * accepted may be counts' own memory and lengths_out that of lengths.
  * Limits: 32 drafts, 65536 sequences, a vocabulary of 2^22. */
 enum hbfsim_kv_probability_type {
     HBFSIM_KV_P_BF16 = 0,
