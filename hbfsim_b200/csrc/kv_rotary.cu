@@ -727,6 +727,23 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
         return HBFSIM_INVALID_ARGUMENT;
     const bool append = b->width != 0 && a.c.pages != 0;
     if (!append && x->q_heads == 0) return HBFSIM_OK;
+    if (x->q_heads) {
+        const u64 heads = a.c.heads, dim = a.c.dim, values = static_cast<u64>(a.c.pages) * heads * 2 * dim;
+        const KvExtent out[] = {{x->q_out, u64{a.tokens} * x->q_heads * dim * 2}};
+        const KvExtent in[] = {{x->q, a.tokens, x->q_stride_token, x->q_heads, x->q_stride_head, dim, 2},
+                               {b->k, a.tokens, b->k_stride_token, heads, b->k_stride_head, dim, 2},
+                               {b->v, a.tokens, b->v_stride_token, heads, b->v_stride_head, dim, 2},
+                               {x->positions, x->axes, a.tokens, x->positions_stride},
+                               {x->freq, u64{x->pairs} * 8},
+                               {x->axis, x->pairs},
+                               {b->table, a.seqs, a.width, b->table_stride},
+                               {b->start, u64{a.seqs} * 4},
+                               {b->offsets, b->offsets ? u64{a.seqs} * 4 + 4 : 0},
+                               {a.c.data, values * a.c.block},
+                               {a.c.bounds, values},
+                               {a.c.scale, values / dim * 4}};
+        if (kv_would_race(out, in, {-1})) return HBFSIM_INVALID_ARGUMENT;
+    }
     r.q = x->q;
     r.q_token = x->q_stride_token;
     r.q_head = x->q_stride_head;

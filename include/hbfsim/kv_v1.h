@@ -125,7 +125,8 @@ int hbfsim_kv_append_v1(const hbfsim_kv_cache_v1* cache,
  * axes: 1 to 4 (a text's one, or time, height and width); an axis of a pair
  * past them is read as the last.  pairs: a multiple of head_dim / 32, at most
  * head_dim / 2.  q_heads 0: keys alone.  q_out: the batch's type, [tokens]
- * [q_heads][head_dim], 16-byte aligned, in memory apart from the inputs. */
+ * [q_heads][head_dim], 16-byte aligned, in memory apart from the inputs' and
+ * the cache's (from an input's lowest row to its highest). */
 typedef struct hbfsim_kv_rotary_v1 {
     uint32_t struct_size;
     uint32_t version;
