@@ -228,6 +228,7 @@ struct Table {
 template <typename T, int D, bool kWide, int kLayout>
 struct TurnedRow {
     static constexpr int W = D / 64;
+    static constexpr int kAhead = 4;
     const u16* x;  // the lane's channels of the first token
     i64 stride;
     Table table;
