@@ -277,14 +277,7 @@ __device__ __forceinline__ float greatest_of(float a, float b)
     return r;
 }
 
-// N words of two stored values.
-template <int N>
-__device__ __forceinline__ void store_values(u8* to, const u32 (&b)[N])
-{
-    if constexpr (N == 1) *reinterpret_cast<u16*>(to) = static_cast<u16>(b[0]);
-    else if constexpr (N == 2) *reinterpret_cast<u32*>(to) = b[0] | b[1] << 16;
-    else *reinterpret_cast<uint2*>(to) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-}
+// N words of two stored values, as put_row writes them.
 template <int N>
 __device__ __forceinline__ void load_values(const u8* from, u32 (&b)[N])
 {
@@ -424,8 +417,8 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
                     for (int i = 0; i < N; ++i) b[k][i] = store_e4m3(mul2(y[r][k][i], make_float2(inverse, inverse)));
                 const u32 row = row0 + 2 * r + half;
                 if (kPlain || row < to) {
-                    store_values<N>(out + row * D + mine.lo, b[0]);
-                    store_values<N>(out + row * D + mine.hi, b[1]);
+                    put_row<N>(out + row * D + mine.lo, b[0]);
+                    put_row<N>(out + row * D + mine.hi, b[1]);
                 }
             }
         }
@@ -436,8 +429,8 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
         else store_rows(std::false_type{});
         const u32 none[N] = {};
         for (u32 row = max(slot + count, first) + half; row < first + 16; row += 2) {
-            store_values<N>(out + row * D + mine.lo, none);
-            store_values<N>(out + row * D + mine.hi, none);
+            put_row<N>(out + row * D + mine.lo, none);
+            put_row<N>(out + row * D + mine.hi, none);
         }
     }
     // from here on in units of the scale
@@ -474,8 +467,8 @@ __device__ __forceinline__ bool append_turned(const AppendArgs& a, bool active, 
                     }
                 const u32 row = row0 + 2 * r + half;
                 if (shrink != 1.0f && row < held) {
-                    store_values<N>(out + row * D + mine.lo, b[r][0]);
-                    store_values<N>(out + row * D + mine.hi, b[r][1]);
+                    put_row<N>(out + row * D + mine.lo, b[r][0]);
+                    put_row<N>(out + row * D + mine.hi, b[r][1]);
                 }
             }
             __syncwarp();
