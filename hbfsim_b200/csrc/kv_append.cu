@@ -10,10 +10,10 @@
 // power of two away from the input, so the only rounding is the one to e4m3.
 //
 // Prompts of 31,668 tokens in all (8 heads of 128 channels) take 42 us: 199 MB
-// of input and blocks at 4.7 TB/s, 73 % of a copy's rate.  Nothing is full (53 %
+// of input and blocks at 4.8 TB/s, 73 % of a copy's rate.  Nothing is full (56 %
 // of the issue slots, 24 warps an SM): a warp loads 16 rows, converts and
 // stores them with no other load under way, so latency bounds it.  A step's 64
-// tokens take 4.2 us and one token 3.3 us, a launch and one chain of reads
+// tokens take 4.4 us and one token 3.1 us, a launch and one chain of reads
 // (start, table, the block's scale, its values).
 #include "kv_append.cuh"
 
@@ -65,7 +65,7 @@ extern "C" int hbfsim_kv_append_v1(const hbfsim_kv_cache_v1* cache,
     if (const int rc = append_check(cache, b, a)) return rc;
     if (b->tokens == 0 || b->width == 0 || a.c.pages == 0) return HBFSIM_OK;  // no block is there
     // One token to a chunk while all chunks' warps are resident at once (16 to an SM), up to 16
-    // beyond (8 heads of 128 channels: 64 tokens took 4.2 us with 1 and 26 us with 16, 31,668
+    // beyond (8 heads of 128 channels: 64 tokens take 4.4 us with 1, took 26 us with 16, 31,668
     // tokens 145 us with 1 and 42 us with 16).
     a.chunk = 1;
     while (a.chunk < 16 && static_cast<u64>(a.tokens) * a.c.heads * 2 > static_cast<u64>(a.chunk) * 16 * kv_sm_count())

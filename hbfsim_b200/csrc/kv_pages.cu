@@ -17,7 +17,8 @@
 // with 510 rows of 4,096 entries 32 us for 26 MB; a compaction of such a pool 21 us
 // for 31 MB (its random reads of the pages' new places are half of that), of one of
 // 2,600 pages 6.6 us; a fork of 64 beams 5.3 us, of 4 documents into 256 rows of
-// 16,385 entries 8.4 us for 17 MB.
+// 16,385 entries 8.4 us for 17 MB, of 4,096 rows of 2,048 entries into as many 72 us
+// for 67 MB (every old row's children are counted by going over all parents).
 #include "kv.h"
 
 namespace hbfb {
@@ -28,12 +29,15 @@ constexpr u32 kPageTeam = 8;      // blocks of the cluster
 constexpr u32 kMaxParts = 1024;   // blocks of a pass at most
 constexpr u32 kDeep = 16;         // entries of a table's row that a lane has under way
 // Of a resize: counts and entries that are worth a block of a cluster, and that one takes at most.  A
-// cluster costs about 2 us.  Before a step of 64 rows of 2048 entries, 70,000 counts, a resize takes 17.6
-// us by 8 blocks and 16.6 us by a launch to a pass, which cost the host 10 us more; 200 rows of 190
-// entries 17.1 us by 8 blocks and 23.6 us by 4, with two rows to a warp.
+// cluster costs about 2 us.  Before a step of 64 rows of 2048 entries, 70,000 counts, a resize takes 17.3
+// us by 8 blocks, 22.0 us by 4 and 16.9 us by a launch to a pass, which cost the host 10 us more; 200 rows
+// of 190 entries (100,000 counts) 18.6 us by 8 blocks, 25.6 us by 4 and 18.9 us by a launch to a pass.
+// More rows take longer by 8 blocks, a run of a row to a warp after the other: 1,024 of 128 entries 34 us
+// (19 by a launch to a pass), 4,096 of 32 97 us (20), 65,536 of 2 1.3 ms (87 us); the rule does not look
+// at that.
 constexpr u64 kCountsEach = 16384, kEntriesEach = 16384, kCountsMost = 32768, kEntriesMost = 16384;
-// Of a compaction: counts and entries that one block does alone: 4,000 of both in 8.0 us and 9.8 us by a
-// launch to a pass, 8,000 in 11.0 and 10.4 us (and 5 us more of the host), 16,000 in 19.9 and 10.6 us.
+// Of a compaction: counts and entries that one block does alone: 4,000 of both in 8.4 us and 9.3 us by a
+// launch to a pass, 8,000 in 12.8 and 10.4 us (and 5 us more of the host), 16,000 in 23.6 and 10.5 us.
 constexpr u64 kCompactMost = 8192;
 
 // The elements [from, end) of a warp.
@@ -717,10 +721,12 @@ __global__ void __launch_bounds__(kPageThreads, 2) compact_pass_kernel(const Com
 // Copies
 
 // A page's data in pieces of 16 KB, eight loads of a thread under way, and no more thread blocks than
-// there are pieces: the hardware hands them out (a gigabyte of 32 KB pages takes 310 us, 96 % of a copy's
+// there are pieces: the hardware hands them out (a gigabyte of 32 KB pages takes 307 us, 97 % of a copy's
 // rate; a grid that stays and strides over the pieces took 330 to 360 us, pieces of 32 KB by 512 threads
 // 351 us).  Lists kept at capacity are mostly empty: long ones go by up to 32 moves to a thread block, which
-// costs a few per cent where they are full (groups of 6: 319 us).
+// costs a few per cent where they are full (groups of 6: 319 us).  600,000 entries of such pages take 40
+// us with no move among them, 63 us with 1,000 (floor 11), 152 us with 9,000 (floor 96); 10,000 entries
+// with none 12 us.
 constexpr u32 kCopyThreads = 128, kCopyDeep = 8, kCopyGroup = 32;
 constexpr u32 kCopyPiece = kCopyThreads * kCopyDeep * 16;  // bytes of a thread block at a time
 

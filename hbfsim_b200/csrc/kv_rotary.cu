@@ -15,10 +15,10 @@
 //
 // Prompts of 31,668 tokens in all (32 query and 8 key/value heads of 128 channels)
 // take 134 us, 718 MB of input, queries and blocks at 5.4 TB/s, 82 % of a copy's rate:
-// the queries alone 90 us (5.8 TB/s, DRAM), the keys and values alone 75 us, where
-// warps wait for their rows at 60 % of the issue slots.  A step's 64 tokens take 5.8
-// us: a launch, the chain of reads of an append, the positions and one turn of 64-bit
-// arithmetic.
+// the queries alone 80 us (6.5 TB/s, a copy's rate), the keys and values alone 74 us,
+// where warps wait for their rows at 53 % of the issue slots.  Rows off 16 bytes, of q,
+// k or v, take 181 us by loads of 2 bytes.  A step's 64 tokens take 5.8 us: a launch,
+// the chain of reads of an append, the positions and one turn of 64-bit arithmetic.
 #include "kv_append.cuh"
 
 namespace hbfb {
@@ -644,6 +644,8 @@ __device__ __forceinline__ void append_values(const RotaryArgs& r, u32 block)
     }
 }
 
+// 80 registers at 128 channels, of which bf16 spills 56 bytes (whole heads; f16 76); the stack frame of 40
+// bytes in every form belongs to sincos.
 template <typename T, int D, bool kWide, int kLayout>
 __global__ void __launch_bounds__(kRotaryWarps * 32, D == 256 ? 3 : D == 128 ? 6 : 8) rotary_kernel(const RotaryArgs r)
 {
@@ -753,7 +755,7 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
     // Chunks as in kv_append.cu; few tokens get a warp to each head and side.  Large batches in blocks of
     // 16 get chunks of 32 tokens: what comes before the first row of a chunk (the search for its blocks,
     // the cosines) is shared by two blocks (prompts of 31,668 tokens: 139 us with 16, 134 us with 32; in
-    // blocks of 32, 142 and 160 us).
+    // blocks of 32, 141 and 160 us, of 64, 173 and 207 us).
     const u32 heads = a.c.heads, groups = (r.q_heads + kRotaryHeads - 1) / kRotaryHeads;
     const u64 warps = static_cast<u64>(kv_sm_count()) * 16;  // resident at once
     a.chunk = 1;
@@ -761,7 +763,9 @@ extern "C" int hbfsim_kv_append_rotary_v1(const hbfsim_kv_cache_v1* cache, const
     while (a.chunk < most && static_cast<u64>(a.tokens) * heads * 2 > a.chunk * warps) a.chunk *= 2;
     if (append) {
         // A CTA takes as many heads' keys of a block at once as it has warps for, 16 rows to a warp; where
-        // that makes many more CTAs than are resident, eight share a block's cosines, one after the other.
+        // that makes many more CTAs than are resident, eight share a block's cosines, one after the other
+        // (those prompts in blocks of 16: 145 us by four, 134 us by eight; of 32: 176 by two, 141 by eight;
+        // of 64: 259 by one, 206 by two, 178 by four, 173 by eight).
         const u32 chunks = (a.tokens + a.chunk - 1) / a.chunk, teams = kRotaryWarps / (a.c.block / 16);
         const u64 pieces = (static_cast<u64>(a.tokens) / a.c.block + a.seqs) * heads;
         const u32 by = pieces > 12ull * teams * kv_sm_count() ? 8 : teams;
